@@ -7,7 +7,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import (POINTER, byref, c_bool, c_char_p, c_float, c_int32, c_uint16, c_uint32, c_uint64,
+from ctypes import (POINTER, byref, c_bool, c_char_p, c_double, c_float, c_int32, c_uint16, c_uint32, c_uint64,
                     c_void_p)
 
 from .gturbo import MoEExpertOffsets
@@ -57,6 +57,26 @@ class FFGTurboLayoutInfo(ctypes.Structure):
 
 class FFTraceEntry(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char * 40), ("launches", c_uint64), ("milliseconds", ctypes.c_double)]
+
+
+class FFAttentionConfig(ctypes.Structure):
+    _fields_ = [(n, c_uint32) for n in
+                ("heads", "kvHeads", "headDim", "pageTokens", "maxRequests", "maxTokens")]
+
+
+class FFAttentionInfo(ctypes.Structure):
+    _fields_ = [("kernelLaunches", c_uint64), ("scratchBytes", c_uint64), ("deviceOrdinal", c_uint32),
+                ("smCount", c_uint32), ("deviceErrorFlag", c_uint32), ("reserved", c_uint32)]
+
+
+class FFRopeConfig(ctypes.Structure):
+    _fields_ = [("base", c_double), ("rotaryDim", c_uint32), ("scaling", c_uint32), ("factor", c_double),
+                ("lowTurns", c_double), ("highTurns", c_double), ("originalContext", c_double),
+                ("amplitude", c_double)]
+
+
+class FFRope(ctypes.Structure):
+    _fields_ = [("table", c_void_p), ("positions", c_uint32), ("rotaryDim", c_uint32), ("layout", c_uint32)]
 
 
 _ERR = POINTER(c_char_p)
@@ -120,6 +140,20 @@ SIGNATURES = {
     "ff_ep_set_tracing": (None, [c_void_p, c_bool]),
     "ff_ep_get_phase_times": (c_uint32, [c_void_p, POINTER(ctypes.c_double), c_uint32]),
     "ff_ep_set_placement": (c_bool, [c_void_p, c_uint32, _P, _P, _ERR]),
+    "ff_attention_create": (c_void_p, [c_int32, POINTER(FFAttentionConfig), _ERR]),
+    "ff_attention_destroy": (None, [c_void_p]),
+    "ff_attention_get_info": (FFAttentionInfo, [c_void_p]),
+    "ff_attention_reset_device_error": (c_bool, [c_void_p, _ERR]),
+    "ff_cache_page_bytes": (c_uint64, [POINTER(FFAttentionConfig)]),
+    "ff_cache_plan": (c_bool, [c_void_p, _P, _P, c_uint32, _P, c_uint32, _P, c_uint32, _P, _P, _P, _P, _P, c_uint32,
+                               _P, _ERR]),
+    "ff_rope_table": (c_bool, [c_void_p, POINTER(FFRopeConfig), _P, c_uint32, _P, _ERR]),
+    "ff_rope": (c_bool, [c_void_p, _P, c_uint32, POINTER(FFRope), _P, c_uint32, c_uint32, _P, c_uint32, _P, _ERR]),
+    "ff_cache_append": (c_bool, [c_void_p, _P, c_uint32, _P, c_uint32, _P, c_uint32, POINTER(FFRope), _P, _P, c_uint32,
+                                 _P, c_uint32, _P, c_uint32, _P, _ERR]),
+    "ff_cache_read": (c_bool, [c_void_p, _P, c_uint32, _P, c_uint32, _P, _P, _P, _ERR]),
+    "ff_attention": (c_bool, [c_void_p, _P, c_uint32, c_uint32, _P, c_uint32, _P, c_uint32, _P, _P, c_uint32, c_uint32,
+                              c_float, c_uint32, c_uint32, _P, c_uint32, _P, _ERR]),
 }
 
 _lib = None

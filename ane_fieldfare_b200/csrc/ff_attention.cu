@@ -1,0 +1,332 @@
+// Attention over the paged INT4 key/value cache: the handle, the entry points' checks, the kernels.
+#include <algorithm>
+#include <string>
+
+#include "ff_attention.cuh"
+
+namespace ff {
+
+// ---- a warp a key ------------------------------------------------------------------------------
+
+// One CTA per (row, query head); its warps take the keys in turn, a key at a time, with a running maximum and sum, and
+// are joined at the end.
+template <int DIM>
+__global__ void __launch_bounds__(128) k_attend_simple(const AttendArgs a) {
+    constexpr int kValues = DIM / 32;  // of a lane: codes [kValues * lane, +kValues) of a head
+    __shared__ float shared[4][DIM + 2];
+    const uint32_t row = blockIdx.x / a.heads, head = blockIdx.x % a.heads, warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    const uint32_t kvHead = head / (a.heads / a.kvHeads);
+    // the row's request
+    uint32_t r = 0;
+    while (r < a.requests && a.rowStart[r + 1] <= row) ++r;
+    float o[kValues], top = -INFINITY, sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kValues; ++i) o[i] = 0.0f;
+    if (r < a.requests) {
+        const int64_t rows = (int64_t)a.rowStart[r + 1] - a.rowStart[r], length = a.lengths[r];
+        const int64_t p = length - rows + (row - a.rowStart[r]);
+        float q[kValues];
+        for (int i = 0; i < kValues; ++i) q[i] = __uint_as_float((uint32_t)a.q[(size_t)row * a.qStride + head * DIM + lane * kValues + i] << 16);
+        const int64_t low = a.window ? p - a.window + 1 : 0;
+        for (int64_t j = warp; j <= p; j += 4) {
+            if (j < low && j >= a.sinks) j += (low - j) / 4 * 4;
+            if (j < low && j >= a.sinks) continue;
+            const uint32_t index = (uint32_t)(j / a.page.pageTokens), inPage = (uint32_t)(j % a.page.pageTokens);
+            const uint32_t page = index < a.tableStride ? a.blockTable[(size_t)r * a.tableStride + index] : FF_NO_PAGE;
+            if (page >= a.pageCount) {
+                if (lane == 0) *a.errorFlag = index < a.tableStride ? kFlagPage : kFlagTableRow;
+                continue;
+            }
+            const uint8_t *block = a.pages + (uint64_t)page * a.page.pageBytes + (uint64_t)kvHead * a.page.blockBytes;
+            float kv[2][kValues];
+#pragma unroll
+            for (int side = 0; side < 2; ++side) {
+                const uint8_t *part = block + side * a.page.values;
+                const uint32_t sb = *reinterpret_cast<const uint32_t *>(part + a.page.keyWords + inPage * a.page.wordBytes + lane * kValues / kGroup * 4);
+                const uint8_t *codes = part + inPage * a.page.codeBytes + lane * kValues / 2;
+#pragma unroll
+                for (int i = 0; i < kValues; ++i) {
+                    const float code = (float)(codes[i / 2] >> (4 * (i & 1)) & 15);
+                    kv[side][i] = fmaf(code, __uint_as_float(sb << 16), __uint_as_float(sb & 0xFFFF0000u));
+                }
+            }
+            float s = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kValues; ++i) s = fmaf(q[i], kv[0][i], s);
+#pragma unroll
+            for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, d);
+            s *= a.scale;
+            const float next = fmaxf(top, s), keep = top == -INFINITY ? 0.0f : expf(top - next), w = expf(s - next);
+            sum = sum * keep + w;
+#pragma unroll
+            for (int i = 0; i < kValues; ++i) o[i] = fmaf(w, kv[1][i], o[i] * keep);
+            top = next;
+        }
+    }
+    for (int i = 0; i < kValues; ++i) shared[warp][lane * kValues + i] = o[i];
+    if (lane == 0) shared[warp][DIM] = top, shared[warp][DIM + 1] = sum;
+    __syncthreads();
+    float all = -INFINITY, total = 0.0f;
+    for (int w = 0; w < 4; ++w) all = fmaxf(all, shared[w][DIM]);
+    for (int w = 0; w < 4; ++w)
+        if (shared[w][DIM] != -INFINITY) total += shared[w][DIM + 1] * expf(shared[w][DIM] - all);
+    for (uint32_t i = threadIdx.x; i < DIM; i += 128) {
+        float v = 0.0f;
+        for (int w = 0; w < 4; ++w)
+            if (shared[w][DIM] != -INFINITY) v += shared[w][i] * expf(shared[w][DIM] - all);
+        v = total != 0.0f ? v / total : 0.0f;
+        uint32_t packed;
+        asm("cvt.rn.bf16x2.f32 %0, %1, %1;" : "=r"(packed) : "f"(v));
+        a.out[(size_t)row * a.outStride + head * DIM + i] = (uint16_t)packed;
+    }
+}
+
+bool launch_attend(FFAttention *att, const AttendArgs &a, cudaStream_t stream, const char **error) {
+    if (a.tokens == 0) return true;
+    const dim3 grid(a.tokens * a.heads);
+    if (att->cfg.headDim == 64) k_attend_simple<64><<<grid, 128, 0, stream>>>(a);
+    else if (att->cfg.headDim == 128) k_attend_simple<128><<<grid, 128, 0, stream>>>(a);
+    else k_attend_simple<256><<<grid, 128, 0, stream>>>(a);
+    return launched(att, cudaSuccess, "k_attend", error);
+}
+
+}  // namespace ff
+
+using namespace ff;
+
+namespace {
+
+bool supported(const FFAttentionConfig &c, const char **error) {
+    if (c.kvHeads == 0 || c.heads == 0 || c.heads % c.kvHeads || c.heads / c.kvHeads > 64 || c.heads > 1024)
+        return fail(error, "heads must be a multiple of kvHeads, up to 64 query heads a key/value head and 1024 in all");
+    if (c.headDim != 64 && c.headDim != 128 && c.headDim != 256) return fail(error, "headDim must be 64, 128 or 256");
+    if (c.pageTokens < 16 || c.pageTokens > 256 || (c.pageTokens & (c.pageTokens - 1)))
+        return fail(error, "pageTokens must be 16, 32, 64, 128 or 256");
+    if (c.maxRequests == 0 || c.maxTokens == 0 || c.maxRequests > (1u << 20) || c.maxTokens > (1u << 24))
+        return fail(error, "need 1..2^20 requests and 1..2^24 rows");
+    return true;
+}
+
+bool begin(FFAttention *att, const char **error) {
+    if (error) *error = nullptr;
+    if (!att) return fail(error, "null attention handle");
+    FF_CUDA_OK(cudaSetDevice(att->device), error);
+    return true;
+}
+
+bool aligned(const void *p, uint32_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1u)) == 0; }
+
+// rows of `heads` heads: 16-byte pieces, and indexes that stay below 2^64
+bool check_heads(const FFAttention *att, const void *x, uint32_t stride, uint32_t heads, const char *what, const char **error) {
+    if (!x) return fail(error, std::string(what) + " pointer is null");
+    if (stride < heads * att->cfg.headDim) return fail(error, std::string(what) + " row stride is too small");
+    if (!aligned(x, 16) || stride % 8) return fail(error, std::string(what) + " rows must be 16-byte aligned (stride a multiple of 8 elements)");
+    return true;
+}
+
+bool check_tokens(const FFAttention *att, uint32_t tokens, const char **error) {
+    if (tokens > att->cfg.maxTokens)
+        return fail(error, std::to_string(tokens) + " rows exceed the handle's maxTokens " + std::to_string(att->cfg.maxTokens));
+    return true;
+}
+
+bool check_cache(const FFAttention *att, const void *pages, uint32_t pageCount, const char **error) {
+    if (!pages) return fail(error, "pages pointer is null");
+    if (!aligned(pages, 16)) return fail(error, "pages must be 16-byte aligned");
+    if ((uint64_t)pageCount * att->cfg.pageTokens >= FF_NO_SLOT) return fail(error, "the cache has more slots than 32 bits name");
+    return true;
+}
+
+bool check_rope(const FFAttention *att, const FFRope *rope, const uint32_t *positions, const char **error) {
+    if (!rope) return fail(error, "rope is null");
+    if (rope->rotaryDim % 16 || rope->rotaryDim > att->cfg.headDim) return fail(error, "rotaryDim must be a multiple of 16 up to headDim");
+    if (rope->layout != FF_ROPE_HALVES && rope->layout != FF_ROPE_INTERLEAVED) return fail(error, "unknown rotary layout");
+    if (rope->rotaryDim && (!rope->table || !aligned(rope->table, 16) || rope->positions == 0))
+        return fail(error, "the rotary table must be non-null, 16-byte aligned and hold a position");
+    if (rope->rotaryDim && (!positions || !aligned(positions, 4))) return fail(error, "positions must be non-null and 4-byte aligned");
+    return true;
+}
+
+}  // namespace
+
+extern "C" {
+
+uint64_t ff_cache_page_bytes(const FFAttentionConfig *config) {
+    return config && supported(*config, nullptr) ? page_layout(*config).pageBytes : 0;
+}
+
+void ff_attention_destroy(FFAttention *att) {
+    if (!att) return;
+    cudaSetDevice(att->device);
+    cudaDeviceSynchronize();
+    cudaFree(att->errorFlag);
+    cudaFree(att->planCount);
+    delete att;
+}
+
+FFAttention *ff_attention_create(int32_t deviceOrdinal, const FFAttentionConfig *config, const char **error) {
+    if (error) *error = nullptr;
+    if (!config) {
+        fail(error, "config is null");
+        return nullptr;
+    }
+    if (!supported(*config, error)) return nullptr;
+    int count = 0;
+    cudaError_t st = cudaGetDeviceCount(&count);
+    if (st != cudaSuccess || count == 0) {
+        fail(error, std::string("no CUDA device: ") + (st != cudaSuccess ? cudaGetErrorString(st) : "device count is 0"));
+        return nullptr;
+    }
+    if (deviceOrdinal < 0 || deviceOrdinal >= count) {
+        fail(error, "device ordinal " + std::to_string(deviceOrdinal) + " out of range");
+        return nullptr;
+    }
+    cudaDeviceProp prop{};
+    if ((st = cudaSetDevice(deviceOrdinal)) != cudaSuccess || (st = cudaGetDeviceProperties(&prop, deviceOrdinal)) != cudaSuccess) {
+        fail(error, std::string("device: ") + cudaGetErrorString(st));
+        return nullptr;
+    }
+    if (prop.major != 10) {
+        fail(error, "this library is built for sm_100a only; device is sm_" + std::to_string(prop.major) + std::to_string(prop.minor));
+        return nullptr;
+    }
+    FFAttention *att = new FFAttention();
+    att->device = deviceOrdinal;
+    att->smCount = prop.multiProcessorCount;
+    att->cfg = *config;
+    auto alloc = [&](auto **p, size_t n) {
+        if (st != cudaSuccess) return;
+        const size_t bytes = std::max<size_t>(n, 1) * sizeof(**p);
+        st = cudaMalloc(reinterpret_cast<void **>(p), bytes);
+        if (st == cudaSuccess) st = cudaMemset(*p, 0, bytes);
+        att->scratchBytes += bytes;
+    };
+    alloc(&att->errorFlag, 1);
+    alloc(&att->planCount, 1);
+    if (st == cudaSuccess) st = cudaDeviceSynchronize();
+    if (st != cudaSuccess) {
+        fail(error, std::string("attention scratch: ") + cudaGetErrorString(st));
+        ff_attention_destroy(att);
+        return nullptr;
+    }
+    return att;
+}
+
+FFAttentionInfo ff_attention_get_info(const FFAttention *att) {
+    FFAttentionInfo info{};
+    if (!att) return info;
+    info.kernelLaunches = att->kernelLaunches;
+    info.scratchBytes = att->scratchBytes;
+    info.deviceOrdinal = (uint32_t)att->device;
+    info.smCount = (uint32_t)att->smCount;
+    cudaSetDevice(att->device);
+    cudaMemcpy(&info.deviceErrorFlag, att->errorFlag, sizeof(uint32_t), cudaMemcpyDeviceToHost);
+    return info;
+}
+
+bool ff_attention_reset_device_error(FFAttention *att, const char **error) {
+    if (!begin(att, error)) return false;
+    FF_CUDA_OK(cudaDeviceSynchronize(), error);
+    FF_CUDA_OK(cudaMemset(att->errorFlag, 0, sizeof(uint32_t)), error);
+    return true;
+}
+
+bool ff_cache_plan(FFAttention *att, const uint32_t *oldLengths, const uint32_t *newLengths, uint32_t requests, uint32_t *blockTable,
+                   uint32_t tableStride, uint32_t *freePages, uint32_t pageCount, const uint32_t *freeCountIn, uint32_t *freeCountOut,
+                   uint32_t *rowStart, uint32_t *positions, uint32_t *slots, uint32_t rows, void *stream, const char **error) {
+    if (!begin(att, error)) return false;
+    if (requests > att->cfg.maxRequests)
+        return fail(error, std::to_string(requests) + " requests exceed the handle's maxRequests " + std::to_string(att->cfg.maxRequests));
+    if (!check_tokens(att, rows, error)) return false;
+    if (!oldLengths || !newLengths || !blockTable || !freePages || !freeCountIn || !freeCountOut || !rowStart || (rows && (!positions || !slots)))
+        return fail(error, "null argument");
+    const uintptr_t all = reinterpret_cast<uintptr_t>(oldLengths) | reinterpret_cast<uintptr_t>(newLengths) | reinterpret_cast<uintptr_t>(blockTable) |
+                          reinterpret_cast<uintptr_t>(freePages) | reinterpret_cast<uintptr_t>(freeCountIn) | reinterpret_cast<uintptr_t>(freeCountOut) |
+                          reinterpret_cast<uintptr_t>(rowStart) | reinterpret_cast<uintptr_t>(positions) | reinterpret_cast<uintptr_t>(slots);
+    if (all & 3u) return fail(error, "arrays must be 4-byte aligned");
+    if (tableStride == 0) return fail(error, "tableStride must be positive");
+    if ((uint64_t)pageCount * att->cfg.pageTokens >= FF_NO_SLOT) return fail(error, "the cache has more slots than 32 bits name");
+    return launch_cache_plan(att, oldLengths, newLengths, requests, blockTable, tableStride, freePages, pageCount, freeCountIn, freeCountOut,
+                             rowStart, positions, slots, rows, static_cast<cudaStream_t>(stream), error);
+}
+
+bool ff_rope_table(FFAttention *att, const FFRopeConfig *config, float *table, uint32_t positions, void *stream, const char **error) {
+    if (!begin(att, error)) return false;
+    if (!config || !table) return fail(error, "null argument");
+    if (!aligned(table, 16)) return fail(error, "the rotary table must be 16-byte aligned");
+    if (config->rotaryDim % 16 || config->rotaryDim > att->cfg.headDim) return fail(error, "rotaryDim must be a multiple of 16 up to headDim");
+    if (!(config->base > 0.0)) return fail(error, "base must be positive");
+    if (config->scaling > FF_ROPE_BY_PARTS) return fail(error, "unknown rotary scaling");
+    if (config->scaling != FF_ROPE_PLAIN && !(config->factor > 0.0)) return fail(error, "factor must be positive");
+    if (config->scaling == FF_ROPE_BY_PARTS && !(config->highTurns > config->lowTurns && config->originalContext > 0.0))
+        return fail(error, "scaling by parts needs highTurns above lowTurns and an original context");
+    return launch_rope_table(att, *config, table, positions, static_cast<cudaStream_t>(stream), error);
+}
+
+bool ff_rope(FFAttention *att, const uint16_t *x, uint32_t xStride, const FFRope *rope, const uint32_t *positions, uint32_t heads, uint32_t tokens,
+             uint16_t *y, uint32_t yStride, void *stream, const char **error) {
+    if (!begin(att, error)) return false;
+    if (heads == 0 || heads > 1024) return fail(error, "need 1..1024 heads");
+    if (tokens == 0) return true;
+    if (!check_tokens(att, tokens, error) || !check_heads(att, x, xStride, heads, "input", error) ||
+        !check_heads(att, y, yStride, heads, "output", error) || !check_rope(att, rope, positions, error))
+        return false;
+    RopeRows rows{};
+    rows.q = x;
+    rows.qStride = xStride;
+    rows.qHeads = heads;
+    rows.qOut = y;
+    rows.qOutStride = yStride;
+    return launch_rope_rows(att, rows, *rope, positions, nullptr, tokens, nullptr, 0, static_cast<cudaStream_t>(stream), error);
+}
+
+bool ff_cache_append(FFAttention *att, const uint16_t *q, uint32_t qStride, const uint16_t *k, uint32_t kStride, const uint16_t *v,
+                     uint32_t vStride, const FFRope *rope, const uint32_t *positions, const uint32_t *slots, uint32_t tokens, uint16_t *qOut,
+                     uint32_t qOutStride, void *pages, uint32_t pageCount, void *stream, const char **error) {
+    if (!begin(att, error)) return false;
+    const FFAttentionConfig &c = att->cfg;
+    if (tokens == 0) return true;
+    if (!check_tokens(att, tokens, error) || !check_heads(att, k, kStride, c.kvHeads, "key", error) ||
+        !check_heads(att, v, vStride, c.kvHeads, "value", error) || !check_rope(att, rope, positions, error) ||
+        !check_cache(att, pages, pageCount, error))
+        return false;
+    if (q && (!check_heads(att, q, qStride, c.heads, "query", error) || !check_heads(att, qOut, qOutStride, c.heads, "query output", error)))
+        return false;
+    if (!slots || !aligned(slots, 4)) return fail(error, "slots must be non-null and 4-byte aligned");
+    RopeRows rows{q, k, v, qStride, kStride, vStride, c.heads, qOut, qOutStride};
+    return launch_rope_rows(att, rows, *rope, positions, slots, tokens, static_cast<uint8_t *>(pages), pageCount, static_cast<cudaStream_t>(stream), error);
+}
+
+bool ff_cache_read(FFAttention *att, const void *pages, uint32_t pageCount, const uint32_t *slots, uint32_t tokens, uint16_t *k, uint16_t *v,
+                   void *stream, const char **error) {
+    if (!begin(att, error)) return false;
+    if (tokens == 0) return true;
+    if (!check_tokens(att, tokens, error) || !check_cache(att, pages, pageCount, error)) return false;
+    if (!slots || !aligned(slots, 4)) return fail(error, "slots must be non-null and 4-byte aligned");
+    if (!aligned(k, 16) || !aligned(v, 16)) return fail(error, "output rows must be 16-byte aligned");
+    return launch_cache_read(att, static_cast<const uint8_t *>(pages), pageCount, slots, tokens, k, v, static_cast<cudaStream_t>(stream), error);
+}
+
+bool ff_attention(FFAttention *att, const uint16_t *q, uint32_t qStride, uint32_t tokens, const void *pages, uint32_t pageCount,
+                  const uint32_t *blockTable, uint32_t tableStride, const uint32_t *rowStart, const uint32_t *lengths, uint32_t requests,
+                  uint32_t maxRows, float scale, uint32_t window, uint32_t sinks, uint16_t *out, uint32_t outStride, void *stream,
+                  const char **error) {
+    if (!begin(att, error)) return false;
+    const FFAttentionConfig &c = att->cfg;
+    if (tokens == 0) return true;
+    if (!check_tokens(att, tokens, error) || !check_heads(att, q, qStride, c.heads, "query", error) ||
+        !check_heads(att, out, outStride, c.heads, "output", error) || !check_cache(att, pages, pageCount, error))
+        return false;
+    if (requests > c.maxRequests)
+        return fail(error, std::to_string(requests) + " requests exceed the handle's maxRequests " + std::to_string(c.maxRequests));
+    if (!blockTable || !rowStart || !lengths) return fail(error, "null argument");
+    if (!aligned(blockTable, 4) || !aligned(rowStart, 4) || !aligned(lengths, 4)) return fail(error, "arrays must be 4-byte aligned");
+    if (tableStride == 0 || maxRows == 0) return fail(error, "tableStride and maxRows must be positive");
+    if (!(scale > 0.0f && scale < INFINITY)) return fail(error, "scale must be positive and finite");
+    if (sinks && !window) return fail(error, "sinks need a window");
+    AttendArgs a{q, out, qStride, outStride, tokens, static_cast<const uint8_t *>(pages), pageCount, tableStride, blockTable, rowStart, lengths,
+                 requests, std::min(maxRows, std::max(1u, tokens)), scale, window, sinks, c.heads, c.kvHeads, page_layout(c), att->errorFlag};
+    return launch_attend(att, a, static_cast<cudaStream_t>(stream), error);
+}
+
+}  // extern "C"

@@ -434,6 +434,136 @@ uint32_t ff_ep_get_phase_times(const FFEPGroup *group, double *milliseconds, uin
 /* Rows the last block sent to another GPU (each also came back as a partial row). */
 uint64_t ff_ep_last_rows_sent(const FFEPGroup *group);
 
+/* ---- attention over a paged INT4 key/value cache --------------------------------------------- */
+
+/* The half of a layer in front of ff_post_attn_setup: rotary positions, the key/value cache, attention.
+ * The cache holds keys and values in the encoding of the weights: affine INT4, groups of 64 values
+ * of a head, a bf16 scale and bias each.  It lives in pages of `pageTokens` tokens, in device memory of
+ * the caller's, one array per layer:
+ *   page    [kvHeads][block], ff_cache_page_bytes() bytes; a layer's pages follow one another
+ *   block   [pageTokens][headDim/2] key codes | [pageTokens][headDim/64] key scale words |
+ *           [pageTokens][headDim/2] value codes | [pageTokens][headDim/64] value scale words
+ * two codes a byte, the first in the low nibble; a scale word is scale (low half) | bias.  A value is
+ * code * scale + bias.  All 16-byte aligned.
+ * A block table row names a request's pages in order; slot = page * pageTokens + position % pageTokens.
+ * Rows of a call are the new tokens of its requests, one request behind the other; rowStart[r] is the first row
+ * of request r.  All arrays are device memory; nothing is read by the host, so that a step's calls can
+ * stand in one CUDA graph, with spare rows for what varies.  (The reference keeps bf16 rings,
+ * Runtime/KVCache; it has no pages and no 4-bit cache.) */
+typedef struct FFAttention FFAttention;
+
+typedef struct {
+    uint32_t heads;        /* query heads, a multiple of kvHeads                        */
+    uint32_t kvHeads;      /* key/value heads                                           */
+    uint32_t headDim;      /* 64, 128 or 256                                            */
+    uint32_t pageTokens;   /* 16, 32, 64, 128 or 256                                    */
+    uint32_t maxRequests;  /* largest number of requests any call will pass             */
+    uint32_t maxTokens;    /* largest number of rows any call will pass                 */
+} FFAttentionConfig;
+
+typedef struct {
+    uint64_t kernelLaunches;  /* kernels this handle has enqueued                       */
+    uint64_t scratchBytes;    /* device scratch owned by the handle                     */
+    uint32_t deviceOrdinal, smCount;
+    uint32_t deviceErrorFlag; /* see ff_attention_reset_device_error (after a sync)     */
+    uint32_t reserved;
+} FFAttentionInfo;
+
+#define FF_NO_PAGE 0xFFFFFFFFu
+#define FF_NO_SLOT 0xFFFFFFFFu
+
+/* Owns the kernels' scratch for one shape of attention; any number of layers and caches use it.  Calls on one
+ * handle share that scratch: the caller orders them (one stream, or events). */
+FFAttention *ff_attention_create(int32_t deviceOrdinal, const FFAttentionConfig *config, const char **error);
+void ff_attention_destroy(FFAttention *attention);
+FFAttentionInfo ff_attention_get_info(const FFAttention *attention);
+/* Waits for the device and clears the flag that FFAttentionInfo reports.  It is sticky; a kernel sets it to
+ * 13: no free page was left, 14: a request is longer than its block table row, 15: more rows than the
+ * arrays hold, 16: a page or slot outside the cache, 17: a wait was given up, 18: a position outside the
+ * rotary table.  What such an entry names is left out; nothing outside the arrays is touched. */
+bool ff_attention_reset_device_error(FFAttention *attention, const char **error);
+/* Bytes of one page of one layer; 0 for a configuration that ff_attention_create refuses. */
+uint64_t ff_cache_page_bytes(const FFAttentionConfig *config);
+
+/* One step of the cache's book-keeping, from request lengths alone.  Request r goes from oldLengths[r]
+ * to newLengths[r] tokens.  Where it shrinks (rejected rows taken back, an end: 0) the pages it no longer needs go
+ * back on the free stack; where it grows it takes pages from the stack's top and its new tokens become rows.
+ * Pages go back before any is taken, both in (request, page) order; so the result is defined to the page.
+ *   blockTable [requests][tableStride]  entries of new pages are written, all others stay
+ *   freePages  [pageCount] stack, the next page on top; freeCountIn / freeCountOut its height before and after (they
+ *              may be the same word)
+ *   rowStart   [requests + 1], positions and slots [rows]: rows behind the last request's get position 0 and
+ *              FF_NO_SLOT
+ * A request that finds no page, or no room in its table row, gets FF_NO_PAGE entries and FF_NO_SLOT rows (flags 13
+ * and 14). */
+bool ff_cache_plan(FFAttention *attention, const uint32_t *oldLengths, const uint32_t *newLengths, uint32_t requests,
+                   uint32_t *blockTable, uint32_t tableStride, uint32_t *freePages, uint32_t pageCount,
+                   const uint32_t *freeCountIn, uint32_t *freeCountOut, uint32_t *rowStart, uint32_t *positions,
+                   uint32_t *slots, uint32_t rows, void *stream, const char **error);
+
+/* How a model's rotary frequencies base^(-2i/rotaryDim) are scaled for contexts longer than it was trained on. */
+typedef enum {
+    FF_ROPE_PLAIN = 0,
+    FF_ROPE_LINEAR = 1,   /* every frequency / factor                                         */
+    FF_ROPE_BY_PARTS = 2  /* / factor where the originalContext holds fewer than lowTurns turns, as it is where it
+                           * holds more than highTurns, between them blended linearly by the number of turns */
+} FFRopeScaling;
+typedef struct {
+    double base;
+    uint32_t rotaryDim;       /* values of a head that rotate: a multiple of 16                  */
+    uint32_t scaling;         /* FFRopeScaling                                                   */
+    double factor, lowTurns, highTurns, originalContext;
+    double amplitude;         /* multiplies every cosine and sine; 0 stands for 1                */
+} FFRopeConfig;
+/* Cosines and sines of positions 0 .. positions-1, fp32 [positions][rotaryDim/2][2], formed in 64 bits: laid out
+ * once per model. */
+bool ff_rope_table(FFAttention *attention, const FFRopeConfig *config, float *table, uint32_t positions, void *stream,
+                   const char **error);
+
+typedef enum {
+    FF_ROPE_HALVES = 0,       /* value i turns with value i + rotaryDim/2                     */
+    FF_ROPE_INTERLEAVED = 1   /* value 2i turns with value 2i + 1                            */
+} FFRopeLayout;
+/* The rotary table as a call uses it: (a, b) -> (a c - b s, a s + b c) for the first rotaryDim values of a head, in
+ * fp32, each product and sum rounded by itself, then to bf16; the other values stay. */
+typedef struct {
+    const float *table;
+    uint32_t positions, rotaryDim, layout;
+} FFRope;
+
+/* Rotates `heads` heads per row: x, y bf16 [tokens][heads][headDim], rows xStride / yStride elements apart
+ * (y may be x). */
+bool ff_rope(FFAttention *attention, const uint16_t *x, uint32_t xStride, const FFRope *rope, const uint32_t *positions,
+             uint32_t heads, uint32_t tokens, uint16_t *y, uint32_t yStride, void *stream, const char **error);
+
+/* The rows' queries rotated into qOut (q may be NULL), their keys rotated and their values as they are quantized into
+ * the cache at slots[row] (FF_NO_SLOT: the row has no place and is left out).  Per group of 64 bf16 values: scale =
+ * bf16((max - min) / 15), bias = min, code = the nearest of 0..15 to (x - min) * (1 / scale) in fp32, ties to even.  A
+ * group with a value that is not finite, or a range beyond bf16, stands for NaN throughout.  Slots of a call differ. */
+bool ff_cache_append(FFAttention *attention, const uint16_t *q, uint32_t qStride, const uint16_t *k, uint32_t kStride,
+                     const uint16_t *v, uint32_t vStride, const FFRope *rope, const uint32_t *positions,
+                     const uint32_t *slots, uint32_t tokens, uint16_t *qOut, uint32_t qOutStride, void *pages,
+                     uint32_t pageCount, void *stream, const char **error);
+
+/* The keys and values that slots hold, as bf16 [tokens][kvHeads][headDim] (contiguous; either may be NULL); zeros for
+ * FF_NO_SLOT. */
+bool ff_cache_read(FFAttention *attention, const void *pages, uint32_t pageCount, const uint32_t *slots, uint32_t tokens,
+                   uint16_t *k, uint16_t *v, void *stream, const char **error);
+
+/* Attention of the rows of a call over their requests' cached keys, their own among them (append first).
+ *   q    bf16 [tokens][heads][headDim], rows qStride elements apart; query heads [g*heads/kvHeads, +heads/kvHeads)
+ *        read key/value head g
+ *   lengths[r] keys of request r, its rows' included; its row i stands at position lengths[r] - rows + i
+ * A row at position p sees key j <= p if window is 0, j > p - window, or j < sinks.  out [tokens][heads][headDim]
+ * (rows outStride apart) = softmax(scale q.k) v; a row that sees no key, and rows behind the last request's, are zero.
+ * maxRows: no request has more rows (it chooses the kernel; rows past it are zero, flag 15).  Up to 16 rows a request
+ * decode and verify blocks are split over the keys, so that one request fills the GPU; longer ones run on the
+ * 5th-generation tensor cores.  Keys on a page outside the cache are not seen (flag 16). */
+bool ff_attention(FFAttention *attention, const uint16_t *q, uint32_t qStride, uint32_t tokens, const void *pages,
+                  uint32_t pageCount, const uint32_t *blockTable, uint32_t tableStride, const uint32_t *rowStart,
+                  const uint32_t *lengths, uint32_t requests, uint32_t maxRows, float scale, uint32_t window,
+                  uint32_t sinks, uint16_t *out, uint32_t outStride, void *stream, const char **error);
+
 /* Device-side result of the last ff_moe_prefill permute, copied to the host after a sync:
  * the expert-sorted pairs and per-expert row offsets [experts+1].  For parity tests. */
 bool ff_last_prefill_routes(FFContext *ctx, FFTokenExpertPair *sortedPairs, uint32_t *offsets,
