@@ -1,0 +1,813 @@
+// Attention of few rows a request (decode steps, verify blocks) over the paged INT4 cache: bound by the cache's bytes.
+//
+// The columns of a request's key/value head are its rows times the query heads that share the head; they stand in
+// tiles of 8 NT.  A unit of work is one (request, key/value head, column tile); its keys are tiles of 64, and all
+// units' tiles end to end are cut into equal runs, one per CTA, so that one long request fills the GPU and a ragged
+// batch leaves no SM with more than another.  A unit that several CTAs share is joined by whichever of them ends last,
+// in the CTAs' order: the same bits every time, and nothing waits.
+//
+// In a CTA one warp copies (TMA boxes of codes, bulk copies of scale words, a ring of tiles); four warps take 16 keys of
+// a tile each, with a maximum, sum and output of their own, joined at the end of a unit.  Per 16 keys:
+//   S = K q   codes as they lie are the A operand: a nibble masked in place IS an f16, the subnormal code * 2^-24 or
+//             * 2^-20, exact, so a word of eight codes costs five instructions.  q is B, in f16 at a power of two of its
+//             own (bf16 fits f16's 11 bits; what lies 2^-28 below the largest is lost).  Per group of 64 the 32-bit sum
+//             takes the group's scale, and the bias times the group's sum of q is added, in fp32.
+//   O += V p  codes of two keys are merged by a byte permute; the value scale goes into p (f16, one rounding more), at a
+//             power of two E that keeps the largest scale and bias of the unit so far within f16 (raised like the
+//             running maximum); one more MMA adds up p * bias per group and p itself.
+// Logits are then exact but for 32-bit sums; weights carry two roundings to 11 bits.
+#include <algorithm>
+#include <cuda_fp16.h>
+#include <string>
+
+#include "ff_attention.cuh"
+#include "ff_mma_device.cuh"
+
+namespace ff {
+
+namespace {
+
+constexpr int kConsumers = 4;                      // warps that compute, 16 keys of a tile each
+constexpr int kRowsThreads = 32 * (kConsumers + 1);
+constexpr uint32_t kTileKeys = 16 * kConsumers;
+constexpr float kLazy = 8.0f;                      // log2 by which a logit may pass the maximum before all is rescaled
+
+struct RowsArgs {
+    AttendArgs a;
+    float *partials;      // [2 CTAs][columns][DIM]
+    float2 *stats;        // [2 CTAs][columns] maximum (log2), sum
+    uint32_t *arrived;    // [CTAs], zero between launches
+    uint32_t pageShift;
+};
+
+__host__ __device__ constexpr uint32_t rows_stage_bytes(int dim) { return (kTileKeys * (dim + dim / 8) + 1023u) & ~1023u; }
+__host__ __device__ constexpr uint32_t rows_stages(int dim) { return dim == 256 ? 4u : 6u; }
+__host__ __device__ constexpr uint32_t rows_smem(int dim, int nt) {
+    return 1024u + rows_stages(dim) * rows_stage_bytes(dim) + 2u * 8u * nt * (dim + 4) * 4u;
+}
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, int w, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
+                 "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t a) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
+    return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t a) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+    return v;
+}
+// the NG scale words of a key
+template <int NG>
+__device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&w)[NG]) {
+    if (NG == 4) asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1 % NG]), "=r"(w[2 % NG]), "=r"(w[3 % NG]) : "r"(a));
+    else if (NG == 2) asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1 % NG]) : "r"(a));
+    else w[0] = lds32(a);
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+// a * b - c
+__device__ __forceinline__ uint32_t residual_f16x2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    asm("{\n.reg .b32 n;\nneg.f16x2 n, %3;\nfma.rn.f16x2 %0, %1, %2, n;\n}" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
+__device__ __forceinline__ uint32_t max_f16x2(uint32_t a, uint32_t b) {  // NaN if either is
+    uint32_t r;
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ float low16(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float high16(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
+__device__ __forceinline__ float power_of_two(int e) { return e < -126 ? 0.0f : __uint_as_float((uint32_t)(min(e, 127) + 127) << 23); }
+// nibbles u and u + 4 of a word as an f16 pair: codes * 2^-24 (u even) or * 2^-20
+template <int U>
+__device__ __forceinline__ uint32_t nibbles(uint32_t w, uint32_t upper) {
+    return (U < 2 ? w : upper) & (U % 2 ? 0x00F000F0u : 0x000F000Fu);
+}
+
+// One request as the kernel sees it.
+struct RowsRequest {
+    uint32_t firstRow, rows, tilesSink, lowTile, tiles, columnTiles;
+    int length, p0;  // p0: position of its first row
+};
+
+// MMA row r (0..7) of eight keys: the key it stands for.  A permutation with which the eight lanes a quarter reads codes
+// of fall into different banks under the copies' swizzle.
+template <int DIM>
+__device__ __forceinline__ uint32_t key_of_row(uint32_t r) {
+    if (DIM == 256) return r;
+    const uint32_t t = r >> 1, odd = r & 1u;
+    return DIM == 128 ? (t & 1u) | (odd << 1) | ((t & 2u) << 1) : t | (odd << 2);
+}
+// 16-byte chunks of a key's codes are exchanged by the key's place (the tensor map's swizzle)
+template <int DIM>
+__device__ __forceinline__ uint32_t chunk_flip(uint32_t key) {
+    return DIM == 256 ? (key & 7u) << 4 : DIM == 128 ? ((key >> 1) & 3u) << 4 : ((key >> 2) & 1u) << 4;
+}
+
+template <int DIM, int NT, bool SPLIT>
+__global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_attend_rows(const __grid_constant__ CUtensorMap map, const RowsArgs args) {
+    constexpr int NG = DIM / 64, CB = DIM / 2, WB = NG * 4;
+    constexpr uint32_t kStage = rows_stage_bytes(DIM), kStages = rows_stages(DIM), kColumns = SPLIT ? 4 : 8 * NT;
+    static_assert(!SPLIT || NT == 1, "four columns, each twice");
+    constexpr uint32_t kKeyWords = kTileKeys * CB * 2, kValueWords = kKeyWords + kTileKeys * WB;
+    extern __shared__ uint8_t rowsSmem[];
+    __shared__ __align__(8) uint64_t barriers[2 * 6];
+    __shared__ uint32_t first[kRowsThreads + 1], warpSums[kConsumers + 1], holes[6];
+    __shared__ float2 joinStats[kConsumers][kColumns];
+    __shared__ float joinBias[kConsumers][NG][kColumns];
+    __shared__ uint32_t lastPart;
+    const AttendArgs &a = args.a;
+    const uint32_t tid = threadIdx.x, warp = (uint32_t)warp_index(), lane = tid & 31u;
+    const uint32_t ring = (sm_addr(rowsSmem) + 1023u) & ~1023u;
+    float *joined = reinterpret_cast<float *>(rowsSmem + (ring - sm_addr(rowsSmem)) + kStages * kStage);
+    const uint32_t group = a.heads / a.kvHeads;
+    const uint32_t barFull = sm_addr(barriers), barEmpty = barFull + 8 * kStages;
+    if (tid == 0) {
+        for (uint32_t s = 0; s < kStages; ++s) {
+            bar_init(barFull + 8 * s, 1);
+            bar_init(barEmpty + 8 * s, kConsumers);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    pdl_enter();
+
+    // ---- the plan: how many tiles each request is, and this CTA's run of them ----
+    auto request_of = [&](uint32_t r) {
+        RowsRequest q{};
+        const uint32_t begin = min(__ldg(a.rowStart + r), a.tokens), end = min(__ldg(a.rowStart + r + 1), a.tokens);
+        const uint32_t rows = end > begin ? end - begin : 0u;
+        q.firstRow = begin;
+        q.length = (int)min(__ldg(a.lengths + r), 0x7FFFFFFFu);
+        q.p0 = q.length - (int)rows;
+        q.rows = min(rows, a.maxRows);
+        if (q.rows == 0) return q;
+        q.columnTiles = (q.rows * group + kColumns - 1) / kColumns;
+        const uint32_t ends = ((uint32_t)max(0, q.p0 + (int)q.rows) + kTileKeys - 1) / kTileKeys;
+        if (a.window) {
+            const uint32_t low = (uint32_t)max((long long)0, (long long)q.p0 - (long long)a.window + 1);
+            q.lowTile = min(low / kTileKeys, ends);
+            q.tilesSink = min((uint32_t)(((unsigned long long)a.sinks + kTileKeys - 1) / kTileKeys), q.lowTile);
+        }
+        q.tiles = max(1u, q.tilesSink + ends - q.lowTile);  // (a request without keys: one tile that nobody sees)
+        return q;
+    };
+    const uint32_t run = (a.requests + kRowsThreads - 1) / kRowsThreads;
+    const uint32_t r0 = min(tid * run, a.requests), r1 = min(r0 + run, a.requests);
+    uint32_t sum = 0;
+    for (uint32_t r = r0; r < r1; ++r) {
+        const RowsRequest q = request_of(r);
+        sum += q.tiles * q.columnTiles * a.kvHeads;
+    }
+    uint32_t scan = sum;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, scan, d);
+        if (lane >= (uint32_t)d) scan += v;
+    }
+    if (lane == 31u) warpSums[warp] = scan;
+    __syncthreads();
+    uint32_t before = 0, total = 0;
+#pragma unroll
+    for (uint32_t w = 0; w <= (uint32_t)kConsumers; ++w) {
+        if (w < warp) before += warpSums[w];
+        total += warpSums[w];
+    }
+    first[tid] = before + scan - sum;
+    if (tid == 0) first[kRowsThreads] = total;
+    __syncthreads();
+
+    // rows that no unit writes: behind the last request's, and past maxRows
+    {
+        const uint32_t covered = a.requests ? min(__ldg(a.rowStart + a.requests), a.tokens) : 0u;
+        const uint32_t perRow = a.heads * DIM / 8;
+        for (uint32_t row = covered + blockIdx.x; row < a.tokens; row += gridDim.x)
+            for (uint32_t i = tid; i < perRow; i += kRowsThreads) *reinterpret_cast<uint4 *>(a.out + (size_t)row * a.outStride + i * 8) = make_uint4(0u, 0u, 0u, 0u);
+        if (blockIdx.x == 0) {
+            if (tid == 0 && a.requests && __ldg(a.rowStart + a.requests) > a.tokens) *a.errorFlag = kFlagRows;
+            for (uint32_t r = r0; r < r1; ++r) {
+                const uint32_t begin = min(__ldg(a.rowStart + r), a.tokens), end = min(__ldg(a.rowStart + r + 1), a.tokens);
+                for (uint32_t row = begin + a.maxRows; row < end; ++row) {
+                    *a.errorFlag = kFlagRows;
+                    for (uint32_t i = 0; i < perRow; ++i) *reinterpret_cast<uint4 *>(a.out + (size_t)row * a.outStride + i * 8) = make_uint4(0u, 0u, 0u, 0u);
+                }
+            }
+        }
+    }
+    if (total == 0) return;
+    const uint32_t ctas = min(gridDim.x, total), cta = blockIdx.x;
+    if (cta >= ctas) return;
+    auto start_of = [&](uint32_t c) { return (uint32_t)((unsigned long long)c * total / ctas); };
+    auto cta_of = [&](uint32_t x) { return (uint32_t)((((unsigned long long)x + 1) * ctas - 1) / total); };
+    const uint32_t begin = start_of(cta), end = start_of(cta + 1);
+
+    // Where the run stands: request, head, column tile, tile.
+    struct Walk {
+        uint32_t r, inRequest, x;  // request, units' tiles before x within it
+        RowsRequest q;
+    };
+    auto locate = [&](uint32_t x) {
+        uint32_t low = 0, high = kRowsThreads;
+        while (high - low > 1) {
+            const uint32_t mid = (low + high) >> 1;
+            if (first[mid] <= x) low = mid;
+            else high = mid;
+        }
+        Walk w;
+        w.x = x;
+        uint32_t n = x - first[low];
+        for (w.r = low * run;; ++w.r) {
+            w.q = request_of(w.r);
+            const uint32_t mine = w.q.tiles * w.q.columnTiles * a.kvHeads;
+            if (n < mine) break;
+            n -= mine;
+        }
+        w.inRequest = n;
+        return w;
+    };
+    auto next_request = [&](Walk &w) {
+        w.inRequest = 0;
+        do {
+            w.q = request_of(++w.r);
+        } while (w.q.rows == 0);
+    };
+
+    if (warp == (uint32_t)kConsumers) {
+        // ---------------- copies ----------------
+        // A lane holds the page of one piece (the keys of a tile on one page): 32 pieces at a time, the next 32 in flight.
+        const uint32_t pieceKeys = min(kTileKeys, a.page.pageTokens), pieces = kTileKeys / pieceKeys;
+        const uint32_t tilesPer = 32u / pieces;  // tiles whose pieces a warp holds
+        uint32_t stage = 0, phase = 0;
+        Walk w = locate(begin);
+        uint32_t x = begin;
+        while (x < end) {
+            const uint32_t unitTiles = w.q.tiles, t0 = w.inRequest % unitTiles, head = w.inRequest / unitTiles / w.q.columnTiles;
+            const uint32_t count = min(end - x, unitTiles - t0);
+            const int keysEnd = w.q.p0 + (int)w.q.rows;
+            auto key_at = [&](uint32_t t) { return (t < w.q.tilesSink ? t : w.q.lowTile + t - w.q.tilesSink) * kTileKeys; };
+            auto page_of = [&](uint32_t base) {
+                const uint32_t t = base + lane / pieces;
+                uint32_t page = FF_NO_PAGE;
+                if (t < t0 + count) {
+                    const uint32_t key = key_at(t) + lane % pieces * pieceKeys;
+                    if ((int)key < keysEnd) {
+                        const uint32_t index = key >> args.pageShift;
+                        if (index < a.tableStride) page = __ldg(a.blockTable + (size_t)w.r * a.tableStride + index);
+                        else *a.errorFlag = kFlagTableRow;
+                        if (page >= a.pageCount && index < a.tableStride) *a.errorFlag = kFlagPage;
+                    }
+                }
+                return page;
+            };
+            uint32_t pagesNext = page_of(t0);
+            for (uint32_t t = t0; t < t0 + count; t += tilesPer) {
+                const uint32_t pagesNow = pagesNext;
+                pagesNext = page_of(t + tilesPer);
+                const uint32_t many = min(tilesPer, t0 + count - t);
+                for (uint32_t i = 0; i < many; ++i) {
+                    // lane = 4 piece + kind: key codes, value codes, key words, value words
+                    const uint32_t piece = lane >> 2, kind = lane & 3u;
+                    const uint32_t page = __shfl_sync(0xFFFFFFFFu, pagesNow, (i * pieces + piece) & 31u);
+                    const bool live = piece < pieces && page < a.pageCount;
+                    const uint32_t lives = __ballot_sync(0xFFFFFFFFu, live);
+                    if (!mbar_try_wait(barEmpty + 8 * stage, phase ^ 1u) && !slot_wait_slow(barEmpty + 8 * stage, phase ^ 1u) && lane == 0) *a.errorFlag = kFlagWait;
+                    __syncwarp();
+                    const uint32_t bar = barFull + 8 * stage, base = ring + stage * kStage;
+                    if (lane == 0) {
+                        uint32_t gone = 0;
+                        for (uint32_t p = 0; p < pieces; ++p) gone |= (lives >> (4 * p) & 1u ? 0u : 1u) << p;
+                        holes[stage] = gone;
+                        bar_expect(bar, (uint32_t)__popc(lives) / 4u * pieceKeys * 2u * (CB + WB));
+                    }
+                    __syncwarp();
+                    if (live) {
+                        const uint32_t inPage = (key_at(t + i) + piece * pieceKeys) & (a.page.pageTokens - 1u);
+                        const uint32_t block = page * a.kvHeads + head;
+                        if (kind < 2) {
+                            tma_load_4d(base + kind * (kTileKeys * CB) + piece * pieceKeys * CB, &map, 0, (int)inPage, (int)kind, (int)block, bar);
+                        } else {
+                            const uint8_t *src = a.pages + (uint64_t)block * a.page.blockBytes + (kind == 2 ? a.page.keyWords : a.page.valueWords) + inPage * WB;
+                            bulk_copy(base + (kind == 2 ? kKeyWords : kValueWords) + piece * pieceKeys * WB, src, pieceKeys * WB, bar);
+                        }
+                    }
+                    if (++stage == kStages) stage = 0, phase ^= 1u;
+                }
+            }
+            x += count;
+            w.inRequest += count;
+            if (x < end && w.inRequest == unitTiles * w.q.columnTiles * a.kvHeads) next_request(w);
+        }
+        return;
+    }
+
+    // ---------------- 16 keys of every tile ----------------
+    const uint32_t g = lane >> 2, t = lane & 3u;
+    const uint32_t keyA = 16 * warp + key_of_row<DIM>(g);  // the S fragments' rows: keys keyA and keyA + 8 of a tile
+    const uint32_t kOff = keyA * CB + ((t * 8) ^ chunk_flip<DIM>(keyA));
+    uint32_t vKey[2], vOff[2];  // the P fragments' keys 2t and 2t + 1, and those + 8
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        vKey[i] = 16 * warp + key_of_row<DIM>(2 * t + i);
+        vOff[i] = vKey[i] * CB + ((g * 4) ^ chunk_flip<DIM>(vKey[i]));
+    }
+    uint32_t stage = 0, phase = 0;
+    Walk w = locate(begin);
+    uint32_t x = begin;
+    while (x < end) {
+        const uint32_t unitTiles = w.q.tiles, t0 = w.inRequest % unitTiles, unit = w.inRequest / unitTiles;
+        const uint32_t head = unit / w.q.columnTiles, column0 = unit % w.q.columnTiles * kColumns;
+        const uint32_t columns = w.q.rows * group, count = min(end - x, unitTiles - t0);
+        const uint32_t pieceKeys = min(kTileKeys, a.page.pageTokens);
+
+        // queries: f16 at a power of two of the column's largest value
+        uint32_t qf[NG][4][NT][2];
+        float qSum[NG][NT][2], toLog2[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const uint32_t column = column0 + 8 * n + (SPLIT ? g & 3u : g), row = column / group;
+            const bool there = column < columns;
+            const uint16_t *src = a.q + (size_t)(w.q.firstRow + row) * a.qStride + (head * group + column % group) * DIM + 16 * t;
+            uint4 v[NG][2];
+            uint32_t largest = 0;
+#pragma unroll
+            for (int G = 0; G < NG; ++G)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    v[G][i] = there ? __ldg(reinterpret_cast<const uint4 *>(src + 64 * G + 8 * i)) : make_uint4(0u, 0u, 0u, 0u);
+                    largest = __vmaxu2(largest, __vmaxu2(__vmaxu2(v[G][i].x & 0x7FFF7FFFu, v[G][i].y & 0x7FFF7FFFu), __vmaxu2(v[G][i].z & 0x7FFF7FFFu, v[G][i].w & 0x7FFF7FFFu)));
+                }
+            uint32_t exponent = max(largest & 0xFFFFu, largest >> 16) >> 7;
+            exponent = max(exponent, __shfl_xor_sync(0xFFFFFFFFu, exponent, 1));
+            exponent = max(exponent, __shfl_xor_sync(0xFFFFFFFFu, exponent, 2));
+            exponent = max(exponent, 13u);
+            const float down = __uint_as_float((267u - exponent) << 23);  // 2^(13 - (exponent - 127)): the largest is 2^13 .. 2^14
+            float mine[NG];
+#pragma unroll
+            for (int G = 0; G < NG; ++G) {
+                float f[16];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t u[4] = {v[G][i].x, v[G][i].y, v[G][i].z, v[G][i].w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) f[8 * i + 2 * j] = low16(u[j]) * down, f[8 * i + 2 * j + 1] = high16(u[j]) * down;
+                }
+                mine[G] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) mine[G] += f[i];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const float odd = u % 2 ? 0.0625f : 1.0f;
+                    qf[G][u][n][0] = pack_f16(f[u] * odd, f[u + 4] * odd);
+                    qf[G][u][n][1] = pack_f16(f[8 + u] * odd, f[12 + u] * odd);
+                }
+                mine[G] += __shfl_xor_sync(0xFFFFFFFFu, mine[G], 1);
+                mine[G] += __shfl_xor_sync(0xFFFFFFFFu, mine[G], 2);
+            }
+            // the S fragments' columns are 2t and 2t + 1
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const uint32_t from = (2 * t + c) * 4;
+#pragma unroll
+                for (int G = 0; G < NG; ++G) qSum[G][n][c] = __shfl_sync(0xFFFFFFFFu, mine[G], from) * 0x1p-24f;
+                const int e = (int)__shfl_sync(0xFFFFFFFFu, exponent, from) - 140;  // q = f16 * 2^e; the codes are 2^-24 of theirs
+                toLog2[n][c] = a.scale * 1.4426950408889634f * power_of_two(e + 4);
+            }
+        }
+
+        float o[NG][4][NT][4], extra[NT][4], top[NT][2];
+        int E = -120;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int G = 0; G < NG; ++G)
+#pragma unroll
+                for (int v = 0; v < 4; ++v)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[G][v][n][i] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) extra[n][i] = 0.0f;
+            top[n][0] = top[n][1] = -INFINITY;
+        }
+        const int pFirst = w.q.p0 + (int)(column0 / group), pLast = w.q.p0 + (int)((min(columns, column0 + kColumns) - 1) / group);
+
+        for (uint32_t i = t0; i < t0 + count; ++i) {
+            const uint32_t tileKey = (i < w.q.tilesSink ? i : w.q.lowTile + i - w.q.tilesSink) * kTileKeys;
+            const int j0 = (int)(tileKey + 16 * warp);
+            const uint32_t base = ring + stage * kStage;
+            if (!mbar_try_wait(barFull + 8 * stage, phase) && !slot_wait_slow(barFull + 8 * stage, phase) && lane == 0) *a.errorFlag = kFlagWait;
+            __syncwarp();
+            const bool hole = holes[stage] >> (16 * warp / pieceKeys) & 1u;
+            // keys that not every row of the tile sees
+            const bool careful = hole || j0 + 15 > pFirst || (a.window && (long long)j0 <= (long long)pLast - a.window && (uint32_t)j0 + 16u > a.sinks);
+            auto sees = [&](int key, int p) {
+                return !hole && key <= p && (!a.window || (long long)key > (long long)p - a.window || (uint32_t)key < a.sinks);
+            };
+
+            // ---- value scales as f16 pairs of keys, at 2^-E ----
+            uint32_t vWords[4][NG];  // keys 2t, 2t + 1, 2t + 8, 2t + 9
+#pragma unroll
+            for (int k = 0; k < 4; ++k) lds_words<NG>(base + kValueWords + (vKey[k & 1] + 8 * (k >> 1)) * WB, vWords[k]);
+            if (careful) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int key = (int)tileKey + (int)vKey[k & 1] + 8 * (k >> 1);
+                    const int p = max(key, pFirst);  // of the rows that may see it, the one whose window goes back furthest
+                    if (p > pLast || !sees(key, p))
+#pragma unroll
+                        for (int G = 0; G < NG; ++G) vWords[k][G] = 0u;
+                }
+            }
+            uint32_t vScale[NG][2], vBias[2];
+            auto convert = [&] {
+                const float f = power_of_two(-E);
+                uint32_t most = 0;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                    for (int G = 0; G < NG; ++G) {
+                        vScale[G][h] = pack_f16(low16(vWords[2 * h][G]) * f, low16(vWords[2 * h + 1][G]) * f);
+                        most = max_f16x2(most, vScale[G][h]);
+                    }
+                    uint32_t b0 = 0, b1 = 0;
+#pragma unroll
+                    for (int G = 0; G < NG; ++G)
+                        if (g == (uint32_t)G) b0 = vWords[2 * h][G], b1 = vWords[2 * h + 1][G];
+                    vBias[h] = pack_f16(high16(b0) * f, high16(b1) * f);
+                    most = max_f16x2(most, vBias[h] & 0x7FFF7FFFu);
+                }
+                // beyond 2^6, or NaN
+                const __half2 m = *reinterpret_cast<const __half2 *>(&most);
+                return !(__low2float(m) <= 64.0f && __high2float(m) <= 64.0f);
+            };
+            bool brokenKeys = false;
+            if (__any_sync(0xFFFFFFFFu, convert())) {
+                uint32_t most = 0;
+                bool broken = false;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    bool bad = false;
+#pragma unroll
+                    for (int G = 0; G < NG; ++G) bad |= (vWords[k][G] & 0x7F80u) == 0x7F80u || (vWords[k][G] & 0x7F800000u) == 0x7F800000u;
+                    broken |= bad;
+#pragma unroll
+                    for (int G = 0; G < NG; ++G) {
+                        if (bad) vWords[k][G] = 0u;
+                        most = max(most, max(((vWords[k][G] & 0x7FFFu) >> 7) + 4u, (vWords[k][G] & 0x7FFF0000u) >> 23));
+                    }
+                }
+                brokenKeys = __any_sync(0xFFFFFFFFu, broken);
+                most = __reduce_max_sync(0xFFFFFFFFu, most);
+                const int raised = min(max((int)most - 127 - 5, E), 120);
+                if (raised > E) {
+                    const float f = power_of_two(E - raised);
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                        for (int G = 0; G < NG; ++G)
+#pragma unroll
+                            for (int v = 0; v < 4; ++v)
+#pragma unroll
+                                for (int k = 0; k < 4; ++k) o[G][v][n][k] *= f;
+                        extra[n][0] *= f;
+                        extra[n][1] *= f;
+                    }
+                    E = raised;
+                }
+                convert();
+            }
+
+            // ---- logits ----
+            float s[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+            uint32_t kWords[2][NG];
+            lds_words<NG>(base + kKeyWords + keyA * WB, kWords[0]);
+            lds_words<NG>(base + kKeyWords + (keyA + 8) * WB, kWords[1]);
+#pragma unroll
+            for (int G = 0; G < NG; ++G) {
+                const uint2 wa = lds64((base + kOff) ^ (uint32_t)(G * 32)), wb = lds64((base + kOff + 8 * CB) ^ (uint32_t)(G * 32));
+                const uint32_t ax = wa.x >> 8, ay = wa.y >> 8, bx = wb.x >> 8, by = wb.y >> 8;
+                float acc[NT][4];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) mma_f16(acc[n], nibbles<0>(wa.x, ax), nibbles<0>(wb.x, bx), nibbles<0>(wa.y, ay), nibbles<0>(wb.y, by), qf[G][0][n][0], qf[G][0][n][1]);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) mma_f16(acc[n], nibbles<1>(wa.x, ax), nibbles<1>(wb.x, bx), nibbles<1>(wa.y, ay), nibbles<1>(wb.y, by), qf[G][1][n][0], qf[G][1][n][1]);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) mma_f16(acc[n], nibbles<2>(wa.x, ax), nibbles<2>(wb.x, bx), nibbles<2>(wa.y, ay), nibbles<2>(wb.y, by), qf[G][2][n][0], qf[G][2][n][1]);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) mma_f16(acc[n], nibbles<3>(wa.x, ax), nibbles<3>(wb.x, bx), nibbles<3>(wa.y, ay), nibbles<3>(wb.y, by), qf[G][3][n][0], qf[G][3][n][1]);
+                const float sa = low16(kWords[0][G]), ba = high16(kWords[0][G]), sb = low16(kWords[1][G]), bb = high16(kWords[1][G]);
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    s[n][0] = fmaf(sa, acc[n][0], fmaf(ba, qSum[G][n][0], s[n][0]));
+                    s[n][1] = fmaf(sa, acc[n][1], fmaf(ba, qSum[G][n][1], s[n][1]));
+                    s[n][2] = fmaf(sb, acc[n][2], fmaf(bb, qSum[G][n][0], s[n][2]));
+                    s[n][3] = fmaf(sb, acc[n][3], fmaf(bb, qSum[G][n][1], s[n][3]));
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) s[n][k] = (s[n][k] * 0x1p20f) * toLog2[n][k & 1];
+            if (careful || brokenKeys) {
+                bool bad[2] = {false, false};
+                if (brokenKeys) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t words[NG];
+                        lds_words<NG>(base + kValueWords + (keyA + 8 * h) * WB, words);
+#pragma unroll
+                        for (int G = 0; G < NG; ++G) bad[h] |= (words[G] & 0x7F80u) == 0x7F80u || (words[G] & 0x7F800000u) == 0x7F800000u;
+                    }
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t column = column0 + 8 * n + (2 * t + (k & 1)) % kColumns;
+                        const int p = w.q.p0 + (int)(column / group);
+                        if (!sees((int)tileKey + (int)keyA + 8 * (k >> 1), p)) s[n][k] = -INFINITY;
+                        else if (bad[k >> 1]) s[n][k] = NAN;
+                    }
+            }
+
+            // ---- weights ----
+            bool above = false;
+            float most[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    float m = fmaxf(s[n][c], s[n][c + 2]);
+                    m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 4));
+                    m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 8));
+                    m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 16));
+                    most[n][c] = m;
+                    above |= m > top[n][c] + kLazy;
+                }
+            if (__any_sync(0xFFFFFFFFu, above)) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float f[2];
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const float next = fmaxf(top[n][c], most[n][c]);
+                        f[c] = top[n][c] == -INFINITY ? 0.0f : exp2_fast(top[n][c] - next);
+                        top[n][c] = next;
+                    }
+#pragma unroll
+                    for (int G = 0; G < NG; ++G)
+#pragma unroll
+                        for (int v = 0; v < 4; ++v)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) o[G][v][n][k] *= f[k & 1];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) extra[n][k] *= f[k & 1];
+                }
+            }
+            uint32_t p[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const float m0 = top[n][0] == -INFINITY ? 0.0f : top[n][0], m1 = top[n][1] == -INFINITY ? 0.0f : top[n][1];
+                p[n][0] = transposed(pack_f16(exp2_fast(s[n][0] - m0), exp2_fast(s[n][1] - m1)));
+                p[n][1] = transposed(pack_f16(exp2_fast(s[n][2] - m0), exp2_fast(s[n][3] - m1)));
+            }
+
+            // ---- values; row 8 of the last product adds up the weights, rows 0 .. NG - 1 the biases ----
+            const uint32_t ones = g == 0 ? 0x3C003C00u : 0u;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma_f16(extra[n], vBias[0], ones, vBias[1], ones, p[n][0], p[n][1]);
+#pragma unroll
+            for (int G = 0; G < NG; ++G) {
+                uint32_t lo[2], hi[2];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t wa = lds32((base + kTileKeys * CB + vOff[0] + 8 * h * CB) ^ (uint32_t)(G * 32));
+                    const uint32_t wb = lds32((base + kTileKeys * CB + vOff[1] + 8 * h * CB) ^ (uint32_t)(G * 32));
+                    lo[h] = __byte_perm(wa, wb, 0x5410);
+                    hi[h] = __byte_perm(wa, wb, 0x7632);
+                }
+                const uint32_t lo0 = lo[0] >> 8, lo1 = lo[1] >> 8, hi0 = hi[0] >> 8, hi1 = hi[1] >> 8;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    uint32_t b0 = mul_f16x2(p[n][0], vScale[G][0]), b1 = mul_f16x2(p[n][1], vScale[G][1]);
+                    const uint32_t rest0 = residual_f16x2(p[n][0], vScale[G][0], b0), rest1 = residual_f16x2(p[n][1], vScale[G][1], b1);
+                    if (SPLIT && g >= 4) b0 = rest0, b1 = rest1;
+                    mma_f16(o[G][0][n], nibbles<0>(lo[0], lo0), nibbles<0>(hi[0], hi0), nibbles<0>(lo[1], lo1), nibbles<0>(hi[1], hi1), b0, b1);
+                    mma_f16(o[G][1][n], nibbles<1>(lo[0], lo0), nibbles<1>(hi[0], hi0), nibbles<1>(lo[1], lo1), nibbles<1>(hi[1], hi1), b0, b1);
+                    mma_f16(o[G][2][n], nibbles<2>(lo[0], lo0), nibbles<2>(hi[0], hi0), nibbles<2>(lo[1], lo1), nibbles<2>(hi[1], hi1), b0, b1);
+                    mma_f16(o[G][3][n], nibbles<3>(lo[0], lo0), nibbles<3>(hi[0], hi0), nibbles<3>(lo[1], lo1), nibbles<3>(hi[1], hi1), b0, b1);
+                    if (!SPLIT) {
+                        mma_f16(o[G][0][n], nibbles<0>(lo[0], lo0), nibbles<0>(hi[0], hi0), nibbles<0>(lo[1], lo1), nibbles<0>(hi[1], hi1), rest0, rest1);
+                        mma_f16(o[G][1][n], nibbles<1>(lo[0], lo0), nibbles<1>(hi[0], hi0), nibbles<1>(lo[1], lo1), nibbles<1>(hi[1], hi1), rest0, rest1);
+                        mma_f16(o[G][2][n], nibbles<2>(lo[0], lo0), nibbles<2>(hi[0], hi0), nibbles<2>(lo[1], lo1), nibbles<2>(hi[1], hi1), rest0, rest1);
+                        mma_f16(o[G][3][n], nibbles<3>(lo[0], lo0), nibbles<3>(hi[0], hi0), nibbles<3>(lo[1], lo1), nibbles<3>(hi[1], hi1), rest0, rest1);
+                    }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(barEmpty + 8 * stage);
+            if (++stage == kStages) stage = 0, phase ^= 1u;
+        }
+
+        // ---- the warps' outputs joined ----
+        const float unscale = power_of_two(E);
+        const bool mineToo = !SPLIT || t < 2;  // columns 4 .. 7 are the rests of columns 0 .. 3
+        if (SPLIT)
+#pragma unroll
+            for (int G = 0; G < NG; ++G)
+#pragma unroll
+                for (int v = 0; v < 4; ++v)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) o[G][v][0][k] += __shfl_xor_sync(0xFFFFFFFFu, o[G][v][0][k], 2);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                if (!mineToo) continue;
+                if (g == 0) joinStats[warp][8 * n + 2 * t + c] = make_float2(top[n][c], extra[n][2 + c]);
+                if (g < (uint32_t)NG) joinBias[warp][g][8 * n + 2 * t + c] = extra[n][c] * unscale;
+            }
+        named_barrier(1, 32 * kConsumers);
+        float *mine = joined + (warp & 1u) * kColumns * (DIM + 4);
+#pragma unroll
+        for (int turn = 0; turn < 2; ++turn) {
+            if ((int)(warp >> 1) == turn && mineToo) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        const uint32_t column = 8 * n + 2 * t + c;
+                        float all = joinStats[0][column].x;
+#pragma unroll
+                        for (int k = 1; k < kConsumers; ++k) all = fmaxf(all, joinStats[k][column].x);
+                        const float f = top[n][c] == -INFINITY ? 0.0f : exp2_fast(top[n][c] - all);
+#pragma unroll
+                        for (int G = 0; G < NG; ++G) {
+                            const float bias = joinBias[warp][G][column];
+#pragma unroll
+                            for (int v = 0; v < 4; ++v)
+#pragma unroll
+                                for (int h = 0; h < 2; ++h) {
+                                    float *to = mine + column * (DIM + 4) + 64 * G + 8 * g + v + 4 * h;
+                                    // (a weight of zero times an output that is none is none: a warp that saw a NaN has a NaN sum)
+                                    const float value = f * fmaf(o[G][v][n][2 * h + c] * (v % 2 ? 0x1p20f : 0x1p24f), unscale, bias);
+                                    *to = turn ? *to + value : value;
+                                }
+                        }
+                    }
+            }
+            named_barrier(1, 32 * kConsumers);
+        }
+
+        // ---- the unit's rows, or this CTA's part of them ----
+        const uint32_t used = min(kColumns, columns - column0);
+        const uint32_t unitBegin = x - t0, unitEnd = unitBegin + unitTiles;
+        const bool whole = count == unitTiles;
+        const uint32_t slot = 2 * cta + (t0 == 0 ? 1u : 0u);
+        for (uint32_t e = tid; e < used * (DIM / 4); e += 32 * kConsumers) {
+            const uint32_t column = e / (DIM / 4), at = e % (DIM / 4) * 4;
+            const float4 u = *reinterpret_cast<const float4 *>(joined + column * (DIM + 4) + at);
+            const float4 v = *reinterpret_cast<const float4 *>(joined + (kColumns + column) * (DIM + 4) + at);
+            float all = joinStats[0][column].x, weights = 0.0f;
+#pragma unroll
+            for (int k = 1; k < kConsumers; ++k) all = fmaxf(all, joinStats[k][column].x);
+#pragma unroll
+            for (int k = 0; k < kConsumers; ++k) weights += joinStats[k][column].x == -INFINITY ? (joinStats[k][column].y != joinStats[k][column].y ? NAN : 0.0f) : joinStats[k][column].y * exp2_fast(joinStats[k][column].x - all);
+            const float4 sum4 = make_float4(u.x + v.x, u.y + v.y, u.z + v.z, u.w + v.w);
+            if (whole) {
+                const float f = weights == 0.0f ? 0.0f : 1.0f / weights;
+                const uint32_t global = column0 + column;
+                uint16_t *to = a.out + (size_t)(w.q.firstRow + global / group) * a.outStride + (head * group + global % group) * DIM + at;
+                *reinterpret_cast<uint2 *>(to) = make_uint2(pack_bf16x2(sum4.x * f, sum4.y * f), pack_bf16x2(sum4.z * f, sum4.w * f));
+            } else {
+                *reinterpret_cast<float4 *>(args.partials + ((size_t)slot * kColumns + column) * DIM + at) = sum4;
+                if (at == 0) args.stats[slot * kColumns + column] = make_float2(all, weights);
+            }
+        }
+        if (!whole) {
+            const uint32_t c0 = cta_of(unitBegin), c1 = cta_of(unitEnd - 1);
+            __threadfence();
+            named_barrier(1, 32 * kConsumers);
+            if (tid == 0) {
+                const uint32_t n = atomicAdd(args.arrived + c0, 1u);
+                lastPart = n == c1 - c0;
+                if (n == c1 - c0) args.arrived[c0] = 0u;
+            }
+            named_barrier(1, 32 * kConsumers);
+            if (lastPart) {
+                __threadfence();
+                for (uint32_t e = tid; e < used * (DIM / 4); e += 32 * kConsumers) {
+                    const uint32_t column = e / (DIM / 4), at = e % (DIM / 4) * 4;
+                    auto slot_of = [&](uint32_t c) { return 2 * c + (c == c0 ? 1u : 0u); };
+                    float all = -INFINITY;
+                    for (uint32_t c = c0; c <= c1; ++c) all = fmaxf(all, __ldcg(args.stats + slot_of(c) * kColumns + column).x);
+                    float weights = 0.0f;
+                    float4 sum4 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+                    for (uint32_t c = c0; c <= c1; ++c) {
+                        const float2 st = __ldcg(args.stats + slot_of(c) * kColumns + column);
+                        const float4 v = __ldcg(reinterpret_cast<const float4 *>(args.partials + ((size_t)slot_of(c) * kColumns + column) * DIM + at));
+                        const float f = st.x == -INFINITY ? (st.y != st.y ? NAN : 0.0f) : exp2_fast(st.x - all);
+                        weights = fmaf(st.y, f, weights);
+                        sum4.x = fmaf(v.x, f, sum4.x), sum4.y = fmaf(v.y, f, sum4.y), sum4.z = fmaf(v.z, f, sum4.z), sum4.w = fmaf(v.w, f, sum4.w);
+                    }
+                    const float f = weights == 0.0f ? 0.0f : 1.0f / weights;
+                    const uint32_t global = column0 + column;
+                    uint16_t *to = a.out + (size_t)(w.q.firstRow + global / group) * a.outStride + (head * group + global % group) * DIM + at;
+                    *reinterpret_cast<uint2 *>(to) = make_uint2(pack_bf16x2(sum4.x * f, sum4.y * f), pack_bf16x2(sum4.z * f, sum4.w * f));
+                }
+            }
+        }
+        x += count;
+        w.inRequest += count;
+        if (x < end) {
+            named_barrier(1, 32 * kConsumers);  // the joining buffers are free
+            if (w.inRequest == unitTiles * w.q.columnTiles * a.kvHeads) next_request(w);
+        }
+    }
+}
+
+KernelSmemMemo rowsMemo[3][4];
+
+template <int DIM, int NT, bool SPLIT = false>
+bool launch_rows(FFAttention *att, KernelSmemMemo &memo, const CUtensorMap &map, const RowsArgs &args, cudaStream_t stream, const char **error) {
+    const size_t smem = rows_smem(DIM, NT);
+    int perSm = 0;
+    if (!memo.prepare(k_attend_rows<DIM, NT, SPLIT>, att->device, smem, kRowsThreads, &perSm, error)) return false;
+    const uint32_t grid = std::min((uint32_t)(att->smCount * std::max(1, perSm)), att->rowsCtas);
+    return launched(att, launch_pdl(k_attend_rows<DIM, NT, SPLIT>, dim3(grid), dim3(kRowsThreads), smem, stream, map, args), "k_attend_rows", error);
+}
+
+}  // namespace
+
+uint32_t attend_rows_ctas(int smCount) { return 2u * (uint32_t)smCount; }
+
+bool launch_attend_rows(FFAttention *att, const AttendArgs &a, cudaStream_t stream, const char **error) {
+    const uint32_t dim = att->cfg.headDim;
+    RowsArgs args{a, att->partials, att->stats, att->arrived, (uint32_t)__builtin_ctz(att->cfg.pageTokens)};
+    // codes of one tile and page: [bytes][tokens][keys, values][blocks]
+    CUtensorMap map;
+    const cuuint64_t dims[4] = {dim / 2, a.page.pageTokens, 2, (cuuint64_t)a.pageCount * a.kvHeads};
+    const cuuint64_t strides[3] = {dim / 2, a.page.values, a.page.blockBytes};
+    const cuuint32_t box[4] = {dim / 2, std::min(kTileKeys, a.page.pageTokens), 1, 1}, elem[4] = {1, 1, 1, 1};
+    const EncodeTiledFn encode = encode_tiled(error);
+    if (!encode) return false;
+    const CUresult rc = encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<uint8_t *>(a.pages), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                               dim == 256 ? CU_TENSOR_MAP_SWIZZLE_128B : dim == 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B,
+                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (rc != CUDA_SUCCESS) return fail(error, "cuTensorMapEncodeTiled(cache pages) failed: " + std::to_string((int)rc));
+    const uint32_t columns = a.maxRows * (a.heads / a.kvHeads);
+    if (dim == 256) {
+        if (columns <= 4) return launch_rows<256, 1, true>(att, rowsMemo[0][0], map, args, stream, error);
+        if (columns <= 8) return launch_rows<256, 1>(att, rowsMemo[0][1], map, args, stream, error);
+        return launch_rows<256, 2>(att, rowsMemo[0][2], map, args, stream, error);
+    }
+    if (dim == 128) {
+        if (columns <= 4) return launch_rows<128, 1, true>(att, rowsMemo[1][0], map, args, stream, error);
+        if (columns <= 8) return launch_rows<128, 1>(att, rowsMemo[1][1], map, args, stream, error);
+        if (columns <= 16) return launch_rows<128, 2>(att, rowsMemo[1][2], map, args, stream, error);
+        return launch_rows<128, 4>(att, rowsMemo[1][3], map, args, stream, error);
+    }
+    if (columns <= 4) return launch_rows<64, 1, true>(att, rowsMemo[2][0], map, args, stream, error);
+    if (columns <= 8) return launch_rows<64, 1>(att, rowsMemo[2][1], map, args, stream, error);
+    if (columns <= 16) return launch_rows<64, 2>(att, rowsMemo[2][2], map, args, stream, error);
+    return launch_rows<64, 4>(att, rowsMemo[2][3], map, args, stream, error);
+}
+
+}  // namespace ff

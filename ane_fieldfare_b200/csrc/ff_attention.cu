@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(128) k_attend_simple(const AttendArgs a) {
 }
 
 bool launch_attend(FFAttention *att, const AttendArgs &a, cudaStream_t stream, const char **error) {
-    if (a.tokens == 0) return true;
+    if (a.maxRows <= 16) return launch_attend_rows(att, a, stream, error);
     const dim3 grid(a.tokens * a.heads);
     if (att->cfg.headDim == 64) k_attend_simple<64><<<grid, 128, 0, stream>>>(a);
     else if (att->cfg.headDim == 128) k_attend_simple<128><<<grid, 128, 0, stream>>>(a);
@@ -161,6 +161,9 @@ void ff_attention_destroy(FFAttention *att) {
     cudaDeviceSynchronize();
     cudaFree(att->errorFlag);
     cudaFree(att->planCount);
+    cudaFree(att->partials);
+    cudaFree(att->stats);
+    cudaFree(att->arrived);
     delete att;
 }
 
@@ -203,6 +206,10 @@ FFAttention *ff_attention_create(int32_t deviceOrdinal, const FFAttentionConfig 
     };
     alloc(&att->errorFlag, 1);
     alloc(&att->planCount, 1);
+    att->rowsCtas = attend_rows_ctas(att->smCount);
+    alloc(&att->partials, (size_t)2 * att->rowsCtas * kPartialValues);
+    alloc(&att->stats, (size_t)2 * att->rowsCtas * kPartialColumns);
+    alloc(&att->arrived, att->rowsCtas);
     if (st == cudaSuccess) st = cudaDeviceSynchronize();
     if (st != cudaSuccess) {
         fail(error, std::string("attention scratch: ") + cudaGetErrorString(st));

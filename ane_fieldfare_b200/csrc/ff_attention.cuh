@@ -9,6 +9,10 @@ struct FFAttention {
     FFAttentionConfig cfg{};
     uint32_t *errorFlag = nullptr;  // device: one of the AttentionFlag values
     uint32_t *planCount = nullptr;  // device: CTAs of ff_cache_plan that are done (zero between launches)
+    uint32_t rowsCtas = 0;          // CTAs that the scratch below serves
+    float *partials = nullptr;      // device: outputs of units that several CTAs share, two parts a CTA
+    float2 *stats = nullptr;        // device: their maxima and sums
+    uint32_t *arrived = nullptr;    // device: parts of a shared unit that are there (zero between launches)
     uint64_t kernelLaunches = 0;
     uint64_t scratchBytes = 0;
 };
@@ -43,6 +47,9 @@ inline PageLayout page_layout(const FFAttentionConfig &c) {
     l.pageBytes = (uint64_t)l.blockBytes * c.kvHeads;
     return l;
 }
+
+// Columns (rows times query heads of a key/value head) that a unit of few rows has at most, and their output values.
+constexpr uint32_t kPartialColumns = 32, kPartialValues = 4096;
 
 // Counts a launch and reports what it says.
 inline bool launched(FFAttention *att, cudaError_t status, const char *what, const char **error) {
@@ -83,6 +90,10 @@ bool launch_rope_rows(FFAttention *att, const RopeRows &rows, const FFRope &rope
                       uint32_t tokens, uint8_t *pages, uint32_t pageCount, cudaStream_t stream, const char **error);
 bool launch_cache_read(FFAttention *att, const uint8_t *pages, uint32_t pageCount, const uint32_t *slots, uint32_t tokens, uint16_t *k,
                        uint16_t *v, cudaStream_t stream, const char **error);
+
+// ff_attend_rows.cu
+uint32_t attend_rows_ctas(int smCount);
+bool launch_attend_rows(FFAttention *att, const AttendArgs &args, cudaStream_t stream, const char **error);
 
 // ff_attention.cu
 bool launch_attend(FFAttention *att, const AttendArgs &args, cudaStream_t stream, const char **error);
