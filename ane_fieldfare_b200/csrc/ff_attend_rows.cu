@@ -17,11 +17,9 @@
 //             running maximum); one more MMA adds up p * bias per group and p itself.
 // Logits are then exact but for 32-bit sums; weights carry two roundings to 11 bits.
 #include <algorithm>
-#include <cuda_fp16.h>
 #include <string>
 
-#include "ff_attention.cuh"
-#include "ff_mma_device.cuh"
+#include "ff_attention_device.cuh"
 
 namespace ff {
 
@@ -29,8 +27,7 @@ namespace {
 
 constexpr int kConsumers = 4;                      // warps that compute, 16 keys of a tile each
 constexpr int kRowsThreads = 32 * (kConsumers + 1);
-constexpr uint32_t kTileKeys = 16 * kConsumers;
-constexpr float kLazy = 8.0f;                      // log2 by which a logit may pass the maximum before all is rescaled
+static_assert(kTileKeys == 16 * kConsumers, "a warp takes 16 keys");
 
 struct RowsArgs {
     AttendArgs a;
@@ -46,21 +43,6 @@ __host__ __device__ constexpr uint32_t rows_smem(int dim, int nt) {
     return 1024u + rows_stages(dim) * rows_stage_bytes(dim) + 2u * 8u * nt * (dim + 4) * 4u;
 }
 
-__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, int w, uint32_t bar) {
-    asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
-                 "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
-                 : "memory");
-}
-__device__ __forceinline__ uint32_t lds32(uint32_t a) {
-    uint32_t v;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(a));
-    return v;
-}
-__device__ __forceinline__ uint2 lds64(uint32_t a) {
-    uint2 v;
-    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
-    return v;
-}
 // the NG scale words of a key
 template <int NG>
 __device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&w)[NG]) {
@@ -78,21 +60,6 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-__device__ __forceinline__ uint32_t pack_bf16x2(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
 __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
     uint32_t r;
     asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
@@ -109,9 +76,6 @@ __device__ __forceinline__ uint32_t max_f16x2(uint32_t a, uint32_t b) {  // NaN 
     asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
-__device__ __forceinline__ float low16(uint32_t w) { return __uint_as_float(w << 16); }
-__device__ __forceinline__ float high16(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
-__device__ __forceinline__ float power_of_two(int e) { return e < -126 ? 0.0f : __uint_as_float((uint32_t)(min(e, 127) + 127) << 23); }
 // nibbles u and u + 4 of a word as an f16 pair: codes * 2^-24 (u even) or * 2^-20
 template <int U>
 __device__ __forceinline__ uint32_t nibbles(uint32_t w, uint32_t upper) {
@@ -132,12 +96,6 @@ __device__ __forceinline__ uint32_t key_of_row(uint32_t r) {
     const uint32_t t = r >> 1, odd = r & 1u;
     return DIM == 128 ? (t & 1u) | (odd << 1) | ((t & 2u) << 1) : t | (odd << 2);
 }
-// 16-byte chunks of a key's codes are exchanged by the key's place (the tensor map's swizzle)
-template <int DIM>
-__device__ __forceinline__ uint32_t chunk_flip(uint32_t key) {
-    return DIM == 256 ? (key & 7u) << 4 : DIM == 128 ? ((key >> 1) & 3u) << 4 : ((key >> 2) & 1u) << 4;
-}
-
 template <int DIM, int NT, bool SPLIT>
 __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_attend_rows(const __grid_constant__ CUtensorMap map, const RowsArgs args) {
     constexpr int NG = DIM / 64, CB = DIM / 2, WB = NG * 4;
@@ -480,12 +438,12 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
                 for (int k = 0; k < 4; ++k) {
                     bool bad = false;
 #pragma unroll
-                    for (int G = 0; G < NG; ++G) bad |= (vWords[k][G] & 0x7F80u) == 0x7F80u || (vWords[k][G] & 0x7F800000u) == 0x7F800000u;
+                    for (int G = 0; G < NG; ++G) bad |= is_broken(vWords[k][G]);
                     broken |= bad;
 #pragma unroll
                     for (int G = 0; G < NG; ++G) {
                         if (bad) vWords[k][G] = 0u;
-                        most = max(most, max(((vWords[k][G] & 0x7FFFu) >> 7) + 4u, (vWords[k][G] & 0x7FFF0000u) >> 23));
+                        most = max(most, word_exponent(vWords[k][G]));
                     }
                 }
                 brokenKeys = __any_sync(0xFFFFFFFFu, broken);
@@ -552,7 +510,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
                         uint32_t words[NG];
                         lds_words<NG>(base + kValueWords + (keyA + 8 * h) * WB, words);
 #pragma unroll
-                        for (int G = 0; G < NG; ++G) bad[h] |= (words[G] & 0x7F80u) == 0x7F80u || (words[G] & 0x7F800000u) == 0x7F800000u;
+                        for (int G = 0; G < NG; ++G) bad[h] |= is_broken(words[G]);
                     }
                 }
 #pragma unroll
@@ -776,22 +734,26 @@ bool launch_rows(FFAttention *att, KernelSmemMemo &memo, const CUtensorMap &map,
 
 }  // namespace
 
-uint32_t attend_rows_ctas(int smCount) { return 2u * (uint32_t)smCount; }
-
-bool launch_attend_rows(FFAttention *att, const AttendArgs &a, cudaStream_t stream, const char **error) {
-    const uint32_t dim = att->cfg.headDim;
-    RowsArgs args{a, att->partials, att->stats, att->arrived, (uint32_t)__builtin_ctz(att->cfg.pageTokens)};
-    // codes of one tile and page: [bytes][tokens][keys, values][blocks]
-    CUtensorMap map;
+bool make_pages_map(CUtensorMap *map, const AttendArgs &a, uint32_t dim, const char **error) {
     const cuuint64_t dims[4] = {dim / 2, a.page.pageTokens, 2, (cuuint64_t)a.pageCount * a.kvHeads};
     const cuuint64_t strides[3] = {dim / 2, a.page.values, a.page.blockBytes};
     const cuuint32_t box[4] = {dim / 2, std::min(kTileKeys, a.page.pageTokens), 1, 1}, elem[4] = {1, 1, 1, 1};
     const EncodeTiledFn encode = encode_tiled(error);
     if (!encode) return false;
-    const CUresult rc = encode(&map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<uint8_t *>(a.pages), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+    const CUresult rc = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<uint8_t *>(a.pages), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
                                dim == 256 ? CU_TENSOR_MAP_SWIZZLE_128B : dim == 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B,
                                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (rc != CUDA_SUCCESS) return fail(error, "cuTensorMapEncodeTiled(cache pages) failed: " + std::to_string((int)rc));
+    return true;
+}
+
+uint32_t attend_rows_ctas(int smCount) { return 2u * (uint32_t)smCount; }
+
+bool launch_attend_rows(FFAttention *att, const AttendArgs &a, cudaStream_t stream, const char **error) {
+    const uint32_t dim = att->cfg.headDim;
+    RowsArgs args{a, att->partials, att->stats, att->arrived, (uint32_t)__builtin_ctz(att->cfg.pageTokens)};
+    CUtensorMap map;
+    if (!make_pages_map(&map, a, dim, error)) return false;
     const uint32_t columns = a.maxRows * (a.heads / a.kvHeads);
     if (dim == 256) {
         if (columns <= 4) return launch_rows<256, 1, true>(att, rowsMemo[0][0], map, args, stream, error);

@@ -1,0 +1,748 @@
+// Attention of many rows a request (prefill chunks) over the paged INT4 cache, on tcgen05: bound by the tensor core.
+//
+// A row tile is up to 128 rows of one request and key/value head (tokens times the query heads that share the head).
+// A unit of work is one row tile; its keys are tiles of 64, and all units' tiles end to end are cut into equal runs, one
+// per CTA, one CTA per SM.  A unit that several CTAs share is joined by whichever of them ends last, in the CTAs' order.
+//
+// Per key tile, warp by role: one copies packed codes and scale words; eight turn them into f16 tiles in shared memory
+// (128-byte swizzle, keys and values alike [64 values][key][128 bytes]); one issues the MMAs; four own a row a thread:
+//   S = Q K^T   A: the rows' queries, in tensor memory for the whole unit (read from shared memory they would cost the
+//               128 bytes a cycle that dequantizing needs); B: the keys, K-major
+//   P = 2^(S f + E - M)   in registers, back into S's columns as f16
+//   O += P V    A: P; B: the values, N-major; O stays in tensor memory
+// Tensor memory: Q dim/2, O dim, S two tiles of 64 columns: all 512 at dim 256.
+//
+// f16 holds 11 bits of keys, values and weights where bf16 would hold 8; its range is kept by powers of two: a row's
+// own for the queries, a tile's own for keys (taken back with the logits) and for values (E, part of the exponent of P and
+// of the maximum M that P stays below 2^8 of).  A code masked in place is the f16 code * 2^-24 or * 2^-20, and one FMA
+// with scale times 2^24 or 2^20 and the bias rounds once: nine instructions a word of eight codes.
+#include <algorithm>
+#include <string>
+
+#include "ff_attention_device.cuh"
+
+namespace ff {
+
+namespace {
+
+constexpr int kDequantWarps = 8, kSoftmaxWarps = 4;
+constexpr int kFirstDequant = 2, kFirstSoftmax = kFirstDequant + kDequantWarps;
+constexpr int kTilesThreads = 32 * (kFirstSoftmax + kSoftmaxWarps);
+constexpr uint32_t kRows = kTileRows;
+// Tiles whose scale words and exponents are kept.  Those of tile n + 8 are written once the keys of n + 6 are expanded, so once
+// the logits of n + 4 are formed, which are issued behind the products of the values of n + 2: tile n is done with.
+constexpr uint32_t kInfo = 8;
+constexpr uint32_t kSlots = 4, kPacked = 4;
+
+struct TilesArgs {
+    AttendArgs a;
+    float *partials;      // [2 CTAs][rows][DIM]
+    float2 *stats;        // [2 CTAs][rows]
+    uint32_t *arrived;    // [CTAs], zero between launches
+    uint32_t pageShift, tileTokens;  // tokens of a row tile
+};
+
+__host__ __device__ constexpr uint32_t slot_bytes(int dim) { return kTileKeys * dim * 2; }
+__host__ __device__ constexpr uint32_t packed_bytes(int dim) { return (kTileKeys * (dim / 2 + 2 * (dim / 16)) + 1023u) & ~1023u; }  // codes, key words, value words
+__host__ __device__ constexpr uint32_t tiles_smem(int dim) { return 1024u + kSlots * slot_bytes(dim) + kPacked * packed_bytes(dim) + kInfo * kTileKeys * (dim / 64) * 4u; }
+
+// K-major or N-major tile of f16 with the 128-byte swizzle: rows of 128 bytes, groups of eight 1024 bytes apart; N-major:
+// the next 64 values `lead` bytes further.
+__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr, uint32_t lead) {
+    uint64_t d = (uint64_t)((addr & 0x3FFFFu) >> 4);
+    d |= (uint64_t)(lead >> 4) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+// f16 x f16 -> fp32, 128 rows, n columns
+__device__ __forceinline__ uint32_t idesc_f16(uint32_t n, bool bNMajor) { return (1u << 4) | ((bNMajor ? 1u : 0u) << 16) | ((n >> 3) << 17) | ((128u >> 4) << 24); }
+__device__ __forceinline__ void mma_a_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+        "}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c) {
+    uint32_t r;
+    asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+    return r;
+}
+
+// A row tile of a request as the kernel sees it.
+struct RowTileOf {
+    uint32_t r, firstRow, tokens;          // its request, first row of q, tokens
+    int p0;                                // position of its first token
+    uint32_t tilesSink, lowTile, tiles;    // key tiles: the first tilesSink, then from lowTile on
+};
+
+template <int DIM>
+__global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_constant__ CUtensorMap map, const TilesArgs args) {
+    constexpr int NG = DIM / 64, CB = DIM / 2, WB = NG * 4;
+    constexpr uint32_t kSlot = slot_bytes(DIM), kPack = packed_bytes(DIM);
+    constexpr uint32_t kKeyWords = kTileKeys * CB, kValueWords = kKeyWords + kTileKeys * WB;
+    constexpr uint32_t kSlotWarps = 2 * NG, kGroupsOfWarps = kDequantWarps / kSlotWarps;
+    constexpr uint32_t kColQ = 0, kColO = DIM / 2, kColS = kColO + DIM;
+    extern __shared__ uint8_t tilesSmem[];
+    __shared__ __align__(8) uint64_t barriers[2 * kSlots + 2 * kPacked + 8 + kInfo + kGroupsOfWarps];
+    __shared__ uint32_t tmemSlot, lastPart;
+    __shared__ volatile uint32_t abortFlag;
+    __shared__ uint32_t firstTile[kTilesThreads + 1], firstWork[kTilesThreads + 1], warpSums[32];
+    __shared__ uint32_t slotMax[kGroupsOfWarps][2][2][kSlotWarps];
+    __shared__ uint32_t holes[kPacked], broken[kInfo][2], hidden[kInfo][2];
+    __shared__ int exponents[kInfo][2];
+    const AttendArgs &a = args.a;
+    const uint32_t tid = threadIdx.x, warp = (uint32_t)warp_index(), lane = tid & 31u;
+    const uint32_t slots = (sm_addr(tilesSmem) + 1023u) & ~1023u, packed = slots + kSlots * kSlot, words = packed + kPacked * kPack;
+    const uint32_t group = a.heads / a.kvHeads;
+    const uint32_t bar0 = sm_addr(barriers);
+    const uint32_t barTile = bar0, barTileFree = bar0 + 8 * kSlots, barPack = barTileFree + 8 * kSlots, barPackFree = barPack + 8 * kPacked;
+    const uint32_t barS = barPackFree + 8 * kPacked, barP = barS + 16, barO = barP + 16, barQ = barO + 16;
+    const uint32_t barJoin = barQ + 8, barInfo = barJoin + 8, barMax = barInfo + 8 * kInfo;
+    if (tid == 0) {
+        abortFlag = 0;
+        for (uint32_t s = 0; s < kSlots; ++s) {
+            mbar_init(barTile + 8 * s, kSlotWarps);
+            mbar_init(barTileFree + 8 * s, 1);
+        }
+        for (uint32_t s = 0; s < kPacked; ++s) {
+            mbar_init(barPack + 8 * s, 1);
+            mbar_init(barPackFree + 8 * s, kSlotWarps);
+        }
+        for (uint32_t s = 0; s < 2; ++s) {
+            mbar_init(barS + 8 * s, 1);
+            mbar_init(barP + 8 * s, kSoftmaxWarps);
+        }
+        mbar_init(barO, 1);
+        mbar_init(barO + 8, 1);
+        mbar_init(barQ, kSoftmaxWarps);
+        mbar_init(barJoin, kSoftmaxWarps);
+        for (uint32_t s = 0; s < kInfo; ++s) mbar_init(barInfo + 8 * s, kSlotWarps);
+        for (uint32_t s = 0; s < kGroupsOfWarps; ++s) mbar_init(barMax + 8 * s, kSlotWarps);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sm_addr(&tmemSlot)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, tmemSlot, 0);
+    pdl_enter();
+
+    // ---- the plan: row tiles of the requests, key tiles of those, this CTA's run ----
+    auto rows_of = [&](uint32_t r) {
+        const uint32_t begin = min(__ldg(a.rowStart + r), a.tokens), end = min(__ldg(a.rowStart + r + 1), a.tokens);
+        return end > begin ? min(end - begin, a.maxRows) : 0u;
+    };
+    auto row_tile = [&](uint32_t r, uint32_t i) {
+        RowTileOf q;
+        const uint32_t begin = min(__ldg(a.rowStart + r), a.tokens), end = min(__ldg(a.rowStart + r + 1), a.tokens);
+        const uint32_t rows = end > begin ? end - begin : 0u, used = min(rows, a.maxRows);
+        q.r = r;
+        q.firstRow = begin + i * args.tileTokens;
+        q.tokens = min(args.tileTokens, used - i * args.tileTokens);
+        q.p0 = (int)min(__ldg(a.lengths + r), 0x7FFFFFFFu) - (int)rows + (int)(i * args.tileTokens);
+        const uint32_t ends = ((uint32_t)max(0, q.p0 + (int)q.tokens) + kTileKeys - 1) / kTileKeys;
+        q.lowTile = q.tilesSink = 0;
+        if (a.window) {
+            const uint32_t low = (uint32_t)max((long long)0, (long long)q.p0 - (long long)a.window + 1);
+            q.lowTile = min(low / kTileKeys, ends);
+            q.tilesSink = min((uint32_t)(((unsigned long long)a.sinks + kTileKeys - 1) / kTileKeys), q.lowTile);
+        }
+        q.tiles = max(1u, q.tilesSink + ends - q.lowTile);  // (rows without keys: one tile that nobody sees)
+        return q;
+    };
+    auto block_scan = [&](uint32_t sum, uint32_t *first) {  // first[t]: sum over the threads before t
+        uint32_t scan = sum;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, scan, d);
+            if (lane >= (uint32_t)d) scan += v;
+        }
+        if (lane == 31u) warpSums[warp] = scan;
+        __syncthreads();
+        uint32_t before = 0, total = 0;
+        for (uint32_t w = 0; w < kTilesThreads / 32; ++w) {
+            if (w < warp) before += warpSums[w];
+            total += warpSums[w];
+        }
+        first[tid] = before + scan - sum;
+        if (tid == 0) first[kTilesThreads] = total;
+        __syncthreads();
+        return total;
+    };
+    auto search = [&](const uint32_t *first, uint32_t n) {
+        uint32_t low = 0, high = kTilesThreads;
+        while (high - low > 1) {
+            const uint32_t mid = (low + high) >> 1;
+            if (first[mid] <= n) low = mid;
+            else high = mid;
+        }
+        return low;
+    };
+    const uint32_t run = (a.requests + kTilesThreads - 1) / kTilesThreads;
+    const uint32_t r0 = min(tid * run, a.requests), r1 = min(r0 + run, a.requests);
+    uint32_t mineTiles = 0;
+    for (uint32_t r = r0; r < r1; ++r) mineTiles += (rows_of(r) + args.tileTokens - 1) / args.tileTokens;
+    const uint32_t rowTiles = block_scan(mineTiles, firstTile);
+    // the n-th row tile
+    struct Place {
+        uint32_t r, i, count;  // request, row tile of it, row tiles that it has
+    };
+    auto place_of = [&](uint32_t n) {
+        const uint32_t low = search(firstTile, n);
+        n -= firstTile[low];
+        Place p{low * run, 0u, 0u};
+        for (;; ++p.r) {
+            p.count = (rows_of(p.r) + args.tileTokens - 1) / args.tileTokens;
+            if (n < p.count) break;
+            n -= p.count;
+        }
+        p.i = n;
+        return p;
+    };
+    auto advance = [&](Place &p) {
+        if (++p.i < p.count) return;
+        p.i = 0;
+        do {
+            ++p.r;
+            p.count = (rows_of(p.r) + args.tileTokens - 1) / args.tileTokens;
+        } while (p.count == 0);
+    };
+    const uint32_t perThread = (rowTiles + kTilesThreads - 1) / kTilesThreads;
+    const uint32_t n0 = min(tid * perThread, rowTiles), n1 = min(n0 + perThread, rowTiles);
+    uint32_t work = 0;
+    if (n0 < n1) {
+        Place p = place_of(n0);
+        for (uint32_t n = n0; n < n1; ++n) {
+            work += row_tile(p.r, p.i).tiles * a.kvHeads;
+            if (n + 1 < n1) advance(p);
+        }
+    }
+    const uint32_t total = block_scan(work, firstWork);
+
+    // rows that no unit writes: behind the last request's, and past maxRows
+    {
+        const uint32_t covered = a.requests ? min(__ldg(a.rowStart + a.requests), a.tokens) : 0u;
+        const uint32_t perRow = a.heads * DIM / 8;
+        for (uint32_t row = covered + blockIdx.x; row < a.tokens; row += gridDim.x)
+            for (uint32_t i = tid; i < perRow; i += kTilesThreads) *reinterpret_cast<uint4 *>(a.out + (size_t)row * a.outStride + i * 8) = make_uint4(0u, 0u, 0u, 0u);
+        if (blockIdx.x == 0) {
+            if (tid == 0 && a.requests && __ldg(a.rowStart + a.requests) > a.tokens) *a.errorFlag = kFlagRows;
+            for (uint32_t r = r0; r < r1; ++r) {
+                const uint32_t begin = min(__ldg(a.rowStart + r), a.tokens), end = min(__ldg(a.rowStart + r + 1), a.tokens);
+                for (uint32_t row = begin + a.maxRows; row < end; ++row) {
+                    *a.errorFlag = kFlagRows;
+                    for (uint32_t i = 0; i < perRow; ++i) *reinterpret_cast<uint4 *>(a.out + (size_t)row * a.outStride + i * 8) = make_uint4(0u, 0u, 0u, 0u);
+                }
+            }
+        }
+    }
+    const uint32_t ctas = min(gridDim.x, total), cta = blockIdx.x;
+    auto start_of = [&](uint32_t c) { return (uint32_t)((unsigned long long)c * total / ctas); };
+    auto cta_of = [&](uint32_t x) { return (uint32_t)((((unsigned long long)x + 1) * ctas - 1) / total); };
+    const uint32_t begin = cta < ctas ? start_of(cta) : 0u, end = cta < ctas ? start_of(cta + 1) : 0u;
+
+    // The run's segments: consecutive key tiles of one unit.
+    struct Walk {
+        Place place;
+        RowTileOf q;
+        uint32_t inTile, head, t0, count;  // inTile: work of the row tile before this; segment [t0, t0 + count)
+    };
+    auto set_segment = [&](Walk &w, uint32_t x) {
+        w.head = w.inTile / w.q.tiles;
+        w.t0 = w.inTile % w.q.tiles;
+        w.count = min(end - x, w.q.tiles - w.t0);
+    };
+    auto locate = [&](uint32_t x) {
+        Walk w;
+        const uint32_t low = search(firstWork, x);
+        w.place = place_of(low * perThread);
+        uint32_t n = x - firstWork[low];
+        for (;; advance(w.place)) {
+            w.q = row_tile(w.place.r, w.place.i);
+            if (n < w.q.tiles * a.kvHeads) break;
+            n -= w.q.tiles * a.kvHeads;
+        }
+        w.inTile = n;
+        set_segment(w, x);
+        return w;
+    };
+    auto next_segment = [&](Walk &w, uint32_t x) {  // x: where the last one ended, below `end`
+        w.inTile += w.count;
+        if (w.inTile == w.q.tiles * a.kvHeads) {
+            advance(w.place);
+            w.q = row_tile(w.place.r, w.place.i);
+            w.inTile = 0;
+        }
+        set_segment(w, x);
+    };
+    auto key_at = [&](const RowTileOf &q, uint32_t t) { return (t < q.tilesSink ? t : q.lowTile + t - q.tilesSink) * kTileKeys; };
+    const uint32_t pieceKeys = min(kTileKeys, a.page.pageTokens), pieces = kTileKeys / pieceKeys;
+
+    if (begin < end) {
+        if (warp == 0) {
+            // ---------------- copies: K0, K1, V0, K2, V1, ... of every segment ----------------
+            uint32_t stage = 0, phase = 0;
+            bool ok = true;
+            Walk w = locate(begin);
+            for (uint32_t x = begin; x < end && ok;) {
+                const int keysEnd = w.q.p0 + (int)w.q.tokens;
+                const uint32_t tilesPer = 32u / pieces;
+                // a lane holds the page of one piece: of `tilesPer` tiles from `base` on, for keys and for values apart
+                auto page_of = [&](uint32_t base) {
+                    const uint32_t t = base + lane / pieces;
+                    uint32_t page = FF_NO_PAGE;
+                    if (t < w.t0 + w.count) {
+                        const uint32_t key = key_at(w.q, t) + lane % pieces * pieceKeys;
+                        if ((int)key < keysEnd) {
+                            const uint32_t index = key >> args.pageShift;
+                            if (index < a.tableStride) {
+                                page = __ldg(a.blockTable + (size_t)w.q.r * a.tableStride + index);
+                                if (page >= a.pageCount) *a.errorFlag = kFlagPage;
+                            } else {
+                                *a.errorFlag = kFlagTableRow;
+                            }
+                        }
+                    }
+                    return page;
+                };
+                uint32_t pagesK = page_of(w.t0), pagesV = pagesK, nextK = page_of(w.t0 + tilesPer);
+                auto copy = [&](uint32_t t, bool key, uint32_t pagesNow) {
+                    // lane = 4 piece + kind: codes, key words, value words (values: codes alone)
+                    const uint32_t piece = lane >> 2, kind = lane & 3u;
+                    const uint32_t page = __shfl_sync(0xFFFFFFFFu, pagesNow, ((t - w.t0) % tilesPer * pieces + piece) & 31u);
+                    const bool live = piece < pieces && page < a.pageCount;
+                    const uint32_t lives = __ballot_sync(0xFFFFFFFFu, live);
+                    if (!mbar_wait_warp<true, Order::kLocal>(barPackFree + 8 * stage, phase ^ 1u, &abortFlag)) {
+                        ok = false;
+                        return;
+                    }
+                    const uint32_t bar = barPack + 8 * stage, base = packed + stage * kPack;
+                    if (lane == 0) {
+                        uint32_t gone = 0;
+                        for (uint32_t p = 0; p < pieces; ++p) gone |= (lives >> (4 * p) & 1u ? 0u : 1u) << p;
+                        holes[stage] = gone;
+                        mbar_expect_tx(bar, (uint32_t)__popc(lives) / 4u * pieceKeys * (key ? CB + 2 * WB : CB));
+                    }
+                    __syncwarp();
+                    if (live && kind < (key ? 3u : 1u)) {
+                        const uint32_t inPage = (key_at(w.q, t) + piece * pieceKeys) & (a.page.pageTokens - 1u);
+                        const uint32_t block = page * a.kvHeads + w.head;
+                        if (kind == 0) {
+                            tma_load_4d(base + piece * pieceKeys * CB, &map, 0, (int)inPage, key ? 0 : 1, (int)block, bar);
+                        } else {
+                            const uint8_t *src = a.pages + (uint64_t)block * a.page.blockBytes + (kind == 1 ? a.page.keyWords : a.page.valueWords) + inPage * WB;
+                            bulk_copy(base + (kind == 1 ? kKeyWords : kValueWords) + piece * pieceKeys * WB, src, pieceKeys * WB, bar);
+                        }
+                    }
+                    if (++stage == kPacked) stage = 0, phase ^= 1u;
+                };
+                const uint32_t last = w.t0 + w.count - 1;
+                copy(w.t0, true, pagesK);
+                for (uint32_t t = w.t0; t <= last && ok; ++t) {
+                    if (t < last) {
+                        if ((t + 1 - w.t0) % tilesPer == 0) {
+                            pagesK = nextK;
+                            nextK = page_of(t + 1 + tilesPer);
+                        }
+                        copy(t + 1, true, pagesK);
+                    }
+                    if (!ok) break;
+                    if ((t - w.t0) % tilesPer == 0 && t != w.t0) pagesV = pagesK;  // (keys are one tile ahead: the same pages)
+                    copy(t, false, pagesV);
+                }
+                x += w.count;
+                if (x < end) next_segment(w, x);
+            }
+        } else if (warp == 1) {
+            // ---------------- MMAs ----------------
+            uint32_t slot = 0, phase = 0, tile = 0, unitNo = 0;  // tile: key tiles so far (its S buffer, the barriers' parities)
+            bool ok = true;
+            Walk w = locate(begin);
+            const uint32_t idescS = idesc_f16(kTileKeys, false), idescO = idesc_f16(DIM, true);
+            auto scores = [&](uint32_t n) {  // S of the n-th tile, from the slot that is next
+                if (!mbar_wait_warp<false, Order::kLocal>(barTile + 8 * slot, phase, &abortFlag)) return false;
+                tc_fence_after();
+                const uint64_t desc = desc_sw128(slots + slot * kSlot, 16);
+                const uint32_t d = tmem + kColS + (n & 1u) * kTileKeys;
+                if (elect_one()) {
+#pragma unroll
+                    for (uint32_t k = 0; k < DIM / 16; ++k)
+                        mma_a_tmem(d, tmem + kColQ + 8 * k, desc + (k / 4) * (kTileKeys * 128 >> 4) + 2 * (k % 4), idescS, k != 0);
+                    commit(barTileFree + 8 * slot);
+                    commit(barS + 8 * (n & 1u));
+                }
+                __syncwarp();
+                if (++slot == kSlots) slot = 0, phase ^= 1u;
+                return true;
+            };
+            for (uint32_t x = begin; x < end && ok;) {
+                ok = mbar_wait_warp<false, Order::kLocal>(barQ, unitNo & 1u, &abortFlag);
+                tc_fence_after();
+                ok = ok && scores(tile);
+                for (uint32_t i = 0; i < w.count && ok; ++i, ++tile) {
+                    if (i + 1 < w.count && !(ok = scores(tile + 1))) break;
+                    if (!(ok = mbar_wait_warp<false, Order::kLocal>(barTile + 8 * slot, phase, &abortFlag))) break;
+                    if (!(ok = mbar_wait_warp<false, Order::kLocal>(barP + 8 * (tile & 1u), tile >> 1 & 1u, &abortFlag))) break;
+                    tc_fence_after();
+                    const uint64_t desc = desc_sw128(slots + slot * kSlot, kTileKeys * 128);
+                    const uint32_t p = tmem + kColS + (tile & 1u) * kTileKeys;
+                    if (elect_one()) {
+#pragma unroll
+                        for (uint32_t k = 0; k < kTileKeys / 16; ++k) mma_a_tmem(tmem + kColO, p + 8 * k, desc + k * (2048 >> 4), idescO, (i | k) != 0);
+                        commit(barTileFree + 8 * slot);
+                        commit(barO + 8 * (tile & 1u));
+                    }
+                    __syncwarp();
+                    if (++slot == kSlots) slot = 0, phase ^= 1u;
+                }
+                ++unitNo;
+                x += w.count;
+                if (x < end) next_segment(w, x);
+            }
+        } else if (warp < (uint32_t)kFirstSoftmax) {
+            // ---------------- dequantizing ----------------
+            // 2 NG warps a slot, a thread one group of 64 values of one key; with fewer values a head, groups of warps take
+            // slots in turn.
+            const uint32_t dw = warp - kFirstDequant, grp = dw / kSlotWarps, inGroup = dw % kSlotWarps;
+            const uint32_t unit = inGroup * 32 + lane, key = unit % kTileKeys, G = unit / kTileKeys;  // (a warp's keys follow one another)
+            const uint32_t codesAt = key * CB, flip = chunk_flip<DIM>(key);
+            uint32_t item = 0, tile = 0, keySlots = 0;  // slots filled by all groups; key tiles so far; key slots of this group
+            bool ok = true;
+            Walk w = locate(begin);
+            auto expand = [&](uint32_t src, uint32_t dst, uint32_t word, int E) {
+                const float f = power_of_two(-E);
+                const float s = low16(word) * f, b = high16(word) * f;
+                const uint32_t s0 = pack_f16(s * 0x1p24f, s * 0x1p24f), s1 = pack_f16(s * 0x1p20f, s * 0x1p20f), bb = pack_f16(b, b);
+                const uint32_t to = dst + G * (kTileKeys * 128) + key * 128;
+#pragma unroll
+                for (uint32_t h = 0; h < 2; ++h) {
+                    const uint4 v = lds128(src + codesAt + ((G * 32 + 16 * h) ^ flip));
+                    const uint32_t c[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; ++i) {
+                        const uint32_t upper = c[i] >> 8;
+                        sts128(to + (((4 * h + i) ^ (key & 7u)) << 4), fma_f16x2(c[i] & 0x000F000Fu, s0, bb), fma_f16x2(c[i] & 0x00F000F0u, s1, bb),
+                               fma_f16x2(upper & 0x000F000Fu, s0, bb), fma_f16x2(upper & 0x00F000F0u, s1, bb));
+                    }
+                }
+            };
+            auto fill = [&](uint32_t t, uint32_t n, bool isKey) {  // tile t of the segment, the n-th of the CTA
+                if (item % kGroupsOfWarps != grp) {
+                    ++item;
+                    return;
+                }
+                const uint32_t slot = item % kSlots, slotPhase = item / kSlots & 1u, pack = item % kPacked, packPhase = item / kPacked & 1u;
+                ++item;
+                if (!mbar_wait<Order::kLocal>(barPack + 8 * pack, packPhase, &abortFlag)) {
+                    ok = false;
+                    return;
+                }
+                const uint32_t src = packed + pack * kPack, info = n % kInfo;
+                uint32_t word;
+                int E;
+                if (isKey) {
+                    // the tile's scale words, keys' and values': what no row sees is nothing, what is no number is marked
+                    word = lds32(src + kKeyWords + key * WB + G * 4);
+                    uint32_t value = lds32(src + kValueWords + key * WB + G * 4);
+                    const int j = (int)(key_at(w.q, t) + key), pLast = w.q.p0 + (int)w.q.tokens - 1, p = max(j, w.q.p0);
+                    const bool hole = holes[pack] >> (key / pieceKeys) & 1u;
+                    const bool seen = p <= pLast && (!a.window || (long long)j > (long long)p - a.window || (uint32_t)j < a.sinks);
+                    const bool bad = seen && !hole && (is_broken(word) || is_broken(value));
+                    if (!seen || hole || bad) word = value = 0u;
+                    const uint32_t most = __reduce_max_sync(0xFFFFFFFFu, word_exponent(word)), mostValue = __reduce_max_sync(0xFFFFFFFFu, word_exponent(value));
+                    const uint32_t marked = __ballot_sync(0xFFFFFFFFu, bad), gone = __ballot_sync(0xFFFFFFFFu, seen && hole);
+                    // (what is kept of the tile kInfo back is used: its values are multiplied.  The maxima of the key slot two
+                    // back are read: every warp has been at the barrier of the one between.)
+                    const uint32_t turn = keySlots & 1u;
+                    if (inGroup < 2 && lane == 0) {
+                        broken[info][inGroup] = 0u;
+                        hidden[info][inGroup] = gone;
+                    }
+                    if (lane == 0) {
+                        slotMax[grp][turn][0][inGroup] = most;
+                        slotMax[grp][turn][1][inGroup] = mostValue;
+                    }
+                    asm volatile("st.shared.u32 [%0], %1;" ::"r"(words + ((info * NG + G) * kTileKeys + key) * 4), "r"(value) : "memory");
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(barMax + 8 * grp);
+                    if (!mbar_wait<Order::kLocal>(barMax + 8 * grp, keySlots & 1u, &abortFlag)) {
+                        ok = false;
+                        return;
+                    }
+                    ++keySlots;
+                    uint32_t top = 0, topValue = 0;
+#pragma unroll
+                    for (uint32_t i = 0; i < kSlotWarps; ++i) {
+                        top = max(top, slotMax[grp][turn][0][i]);
+                        topValue = max(topValue, slotMax[grp][turn][1][i]);
+                    }
+                    E = min(max((int)top - 127 + 6, -120), 120);  // the largest is 2^-6 .. 2^-5
+                    if (marked && lane == 0) atomicOr(&broken[info][inGroup & 1u], marked);
+                    if (inGroup == 0 && lane == 0) {
+                        exponents[info][0] = E;
+                        exponents[info][1] = min(max((int)topValue - 127 + 6, -120), 120);
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(barInfo + 8 * info);
+                } else {
+                    if (!mbar_wait<Order::kLocal>(barInfo + 8 * info, n / kInfo & 1u, &abortFlag)) {
+                        ok = false;
+                        return;
+                    }
+                    word = lds32(words + ((info * NG + G) * kTileKeys + key) * 4);
+                    E = exponents[info][1];
+                }
+                if (!mbar_wait<Order::kLocal>(barTileFree + 8 * slot, slotPhase ^ 1u, &abortFlag)) {
+                    ok = false;
+                    return;
+                }
+                expand(src, slots + slot * kSlot, word, E);
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(barPackFree + 8 * pack);
+                    mbar_arrive(barTile + 8 * slot);
+                }
+            };
+            for (uint32_t x = begin; x < end && ok;) {
+                fill(w.t0, tile, true);
+                for (uint32_t i = 0; i < w.count && ok; ++i, ++tile) {
+                    if (i + 1 < w.count) fill(w.t0 + i + 1, tile + 1, true);
+                    if (ok) fill(w.t0 + i, tile, false);
+                }
+                x += w.count;
+                if (x < end) next_segment(w, x);
+            }
+        } else {
+            // ---------------- rows ----------------
+            const uint32_t quarter = warp & 3u, row = quarter * 32 + lane;
+            const uint32_t lanes = (quarter * 32) << 16;
+            uint32_t tile = 0, joins = 0;
+            bool ok = true;
+            Walk w = locate(begin);
+            for (uint32_t x = begin; x < end && ok;) {
+                const uint32_t token = row / group;
+                const bool there = token < w.q.tokens;
+                const uint32_t head = w.head * group + row % group;
+                const int p = w.q.p0 + (int)token, pLast = w.q.p0 + (int)w.q.tokens - 1;
+                // queries: f16 at a power of two of the row's largest value; runs of eight in the order of the tiles' codes
+                float toLog2;
+                {
+                    const uint4 *src = reinterpret_cast<const uint4 *>(a.q + (size_t)(w.q.firstRow + (there ? token : 0u)) * a.qStride + head * DIM);
+                    uint32_t largest = 0;
+#pragma unroll 8
+                    for (uint32_t i = 0; i < DIM / 8; ++i) {
+                        const uint4 v = there ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
+                        largest = __vmaxu2(largest, __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu)));
+                    }
+                    const uint32_t exponent = max(max(largest & 0xFFFFu, largest >> 16) >> 7, 7u);
+                    const float down = __uint_as_float((261u - exponent) << 23);  // the largest is 2^7 .. 2^8
+                    toLog2 = a.scale * 1.4426950408889634f * power_of_two((int)exponent - 134);
+#pragma unroll 1
+                    for (uint32_t c = 0; c < DIM / 64; ++c) {
+                        uint32_t o[32];
+#pragma unroll
+                        for (uint32_t i = 0; i < 8; ++i) {
+                            const uint4 v = there ? __ldg(src + 8 * c + i) : make_uint4(0u, 0u, 0u, 0u);
+                            o[4 * i] = pack_f16(low16(v.x) * down, low16(v.z) * down);
+                            o[4 * i + 1] = pack_f16(high16(v.x) * down, high16(v.z) * down);
+                            o[4 * i + 2] = pack_f16(low16(v.y) * down, low16(v.w) * down);
+                            o[4 * i + 3] = pack_f16(high16(v.y) * down, high16(v.w) * down);
+                        }
+                        tc_store_32cols(tmem + lanes + kColQ + 32 * c, o);
+                    }
+                    tc_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(barQ);
+                }
+                float top = -INFINITY, sum = 0.0f;
+                for (uint32_t i = 0; i < w.count; ++i, ++tile) {
+                    const uint32_t info = tile % kInfo;
+                    if (!(ok = mbar_wait_warp<false, Order::kLocal>(barS + 8 * (tile & 1u), tile >> 1 & 1u, &abortFlag))) break;
+                    tc_fence_after();
+                    const uint32_t s0 = tmem + lanes + kColS + (tile & 1u) * kTileKeys;
+                    uint32_t lo[32], hi[32];
+                    tc_load_32cols(s0, lo);
+                    tc_load_32cols(s0 + 32, hi);
+                    const int eK = exponents[info][0], eV = exponents[info][1];
+                    const uint32_t bad0 = broken[info][0], bad1 = broken[info][1], gone0 = hidden[info][0], gone1 = hidden[info][1];
+                    const int j0 = (int)key_at(w.q, w.t0 + i);
+                    tc_wait_ld();
+                    float *s = reinterpret_cast<float *>(lo), *u = reinterpret_cast<float *>(hi);
+                    const float f = toLog2 * power_of_two(eK);
+                    if (j0 + (int)kTileKeys - 1 > w.q.p0 || (a.window && (long long)j0 <= (long long)pLast - a.window && (uint32_t)j0 + kTileKeys > a.sinks) || (bad0 | bad1 | gone0 | gone1)) {
+                        const int most = p - j0;
+                        const long long least = a.window ? (long long)p - a.window - j0 : -1;  // sees c > least
+                        const long long sinks = a.window ? (long long)a.sinks - j0 : 0;        // or c < sinks
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) {
+                            const bool see0 = c <= most && (c > least || c < sinks) && !(gone0 >> c & 1u), see1 = c + 32 <= most && (c + 32 > least || c + 32 < sinks) && !(gone1 >> c & 1u);
+                            s[c] = !see0 ? -INFINITY : bad0 >> c & 1u ? NAN : s[c];
+                            u[c] = !see1 ? -INFINITY : bad1 >> c & 1u ? NAN : u[c];
+                        }
+                    }
+                    float most = fmaxf(s[0], u[0]);
+#pragma unroll
+                    for (int c = 1; c < 32; ++c) most = fmaxf(most, fmaxf(s[c], u[c]));
+                    most = fmaf(most, f, (float)eV);
+                    if (__any_sync(0xFFFFFFFFu, most > top + kLazy)) {
+                        const float next = fmaxf(top, most), down = top == -INFINITY ? 0.0f : exp2_fast(top - next);
+                        top = next;
+                        sum *= down;
+                        if (i) {  // O so far, once the products in flight are done
+                            if (!(ok = mbar_wait_warp<false, Order::kLocal>(barO + 8 * ((tile - 1) & 1u), (tile - 1) >> 1 & 1u, &abortFlag))) break;
+                            tc_fence_after();
+#pragma unroll 1
+                            for (uint32_t c = 0; c < DIM; c += 32) {
+                                uint32_t o[32];
+                                tc_load_32cols(tmem + lanes + kColO + c, o);
+                                tc_wait_ld();
+#pragma unroll
+                                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * down);
+                                tc_store_32cols(tmem + lanes + kColO + c, o);
+                            }
+                            tc_wait_st();
+                        }
+                    }
+                    const float shift = top == -INFINITY ? 0.0f : (float)eV - top;
+                    float part = 0.0f;
+                    uint32_t o[32];
+#pragma unroll
+                    for (int c = 0; c < 32; c += 2) {
+                        const float x0 = exp2_fast(fmaf(s[c], f, shift)), x1 = exp2_fast(fmaf(s[c + 1], f, shift));
+                        const float y0 = exp2_fast(fmaf(u[c], f, shift)), y1 = exp2_fast(fmaf(u[c + 1], f, shift));
+                        part += (x0 + x1) + (y0 + y1);
+                        o[c / 2] = pack_f16(x0, x1);
+                        o[16 + c / 2] = pack_f16(y0, y1);
+                    }
+                    sum = fmaf(part, power_of_two(-eV), sum);
+                    tc_store_32cols(s0, o);
+                    tc_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(barP + 8 * (tile & 1u));
+                }
+                if (!ok) break;
+
+                // ---- the unit's rows, or this CTA's part of them ----
+                if (!(ok = mbar_wait_warp<false, Order::kLocal>(barO + 8 * ((tile - 1) & 1u), (tile - 1) >> 1 & 1u, &abortFlag))) break;
+                tc_fence_after();
+                const bool whole = w.count == w.q.tiles;
+                const uint32_t part = 2 * cta + (w.t0 == 0 ? 1u : 0u);
+                uint16_t *out = a.out + (size_t)(w.q.firstRow + (there ? token : 0u)) * a.outStride + head * DIM;
+                auto write_32 = [&](uint32_t c, const float (&v)[32], float factor) {
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8)
+                        *reinterpret_cast<uint4 *>(out + c + i) = make_uint4(pack_bf16x2(v[i] * factor, v[i + 2] * factor), pack_bf16x2(v[i + 4] * factor, v[i + 6] * factor),
+                                                                             pack_bf16x2(v[i + 1] * factor, v[i + 3] * factor), pack_bf16x2(v[i + 5] * factor, v[i + 7] * factor));
+                };
+                const float factor = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll 1
+                for (uint32_t c = 0; c < DIM; c += 32) {
+                    uint32_t o[32];
+                    tc_load_32cols(tmem + lanes + kColO + c, o);
+                    tc_wait_ld();
+                    if (there && whole) {
+                        write_32(c, reinterpret_cast<const float(&)[32]>(o), factor);
+                    } else if (there) {
+                        float4 *to = reinterpret_cast<float4 *>(args.partials + ((size_t)part * kRows + row) * DIM + c);
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) to[k] = make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]), __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
+                    }
+                }
+                if (!whole) {
+                    if (there) args.stats[part * kRows + row] = make_float2(top, sum);
+                    const uint32_t c0 = cta_of(x - w.t0), c1 = cta_of(x - w.t0 + w.q.tiles - 1);
+                    auto meet = [&] {  // of the four warps
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(barJoin);
+                        ok = mbar_wait_warp<false, Order::kLocal>(barJoin, joins++ & 1u, &abortFlag);
+                        return ok;
+                    };
+                    __threadfence();
+                    if (!meet()) break;
+                    if (row == 0) {
+                        const uint32_t n = atomicAdd(args.arrived + c0, 1u);
+                        lastPart = n == c1 - c0;
+                        if (n == c1 - c0) args.arrived[c0] = 0u;
+                    }
+                    if (!meet()) break;
+                    if (lastPart && there) {
+                        __threadfence();
+                        auto part_of = [&](uint32_t c) { return 2 * c + (c == c0 ? 1u : 0u); };
+                        float all = -INFINITY, weights = 0.0f;
+                        for (uint32_t c = c0; c <= c1; ++c) all = fmaxf(all, __ldcg(args.stats + part_of(c) * kRows + row).x);
+                        auto weight_of = [&](const float2 &st) { return st.x == -INFINITY ? (st.y != st.y ? NAN : 0.0f) : exp2_fast(st.x - all); };
+                        for (uint32_t c = c0; c <= c1; ++c) {
+                            const float2 st = __ldcg(args.stats + part_of(c) * kRows + row);
+                            weights = fmaf(st.y, weight_of(st), weights);
+                        }
+                        const float last = weights == 0.0f ? 0.0f : 1.0f / weights;
+#pragma unroll 1
+                        for (uint32_t d = 0; d < DIM; d += 32) {
+                            float v[32];
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) v[k] = 0.0f;
+                            for (uint32_t c = c0; c <= c1; ++c) {
+                                const float g = weight_of(__ldcg(args.stats + part_of(c) * kRows + row));
+                                const float4 *from = reinterpret_cast<const float4 *>(args.partials + ((size_t)part_of(c) * kRows + row) * DIM + d);
+#pragma unroll
+                                for (int k = 0; k < 8; ++k) {
+                                    const float4 t = __ldcg(from + k);
+                                    v[4 * k] = fmaf(t.x, g, v[4 * k]), v[4 * k + 1] = fmaf(t.y, g, v[4 * k + 1]);
+                                    v[4 * k + 2] = fmaf(t.z, g, v[4 * k + 2]), v[4 * k + 3] = fmaf(t.w, g, v[4 * k + 3]);
+                                }
+                            }
+                            write_32(d, v, last);
+                        }
+                    }
+                    if (!meet()) break;  // (before the next unit's word in `lastPart`)
+                }
+                x += w.count;
+                if (x < end) next_segment(w, x);
+            }
+        }
+    }
+    // every role is done, or gave up after a bounded wait; copies and products in flight have landed before the ends
+    // they were waited for
+    tc_fence_before();
+    __syncthreads();
+    if (tid == 0 && abortFlag) *a.errorFlag = kFlagWait;
+    tc_fence_after();
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+}
+
+KernelSmemMemo tilesMemo[3];
+
+template <int DIM>
+bool launch_tiles(FFAttention *att, KernelSmemMemo &memo, const CUtensorMap &map, const TilesArgs &args, cudaStream_t stream, const char **error) {
+    if (!memo.prepare(k_attend_tiles<DIM>, att->device, tiles_smem(DIM), kTilesThreads, nullptr, error)) return false;
+    return launched(att, launch_pdl(k_attend_tiles<DIM>, dim3(att->smCount), dim3(kTilesThreads), tiles_smem(DIM), stream, map, args), "k_attend_tiles", error);
+}
+
+}  // namespace
+
+bool launch_attend_tiles(FFAttention *att, const AttendArgs &a, cudaStream_t stream, const char **error) {
+    const uint32_t dim = att->cfg.headDim;
+    TilesArgs args{a, att->partials, att->stats, att->arrived, (uint32_t)__builtin_ctz(att->cfg.pageTokens), kRows / (a.heads / a.kvHeads)};
+    CUtensorMap map;
+    if (!make_pages_map(&map, a, dim, error)) return false;
+    if (dim == 256) return launch_tiles<256>(att, tilesMemo[2], map, args, stream, error);
+    if (dim == 128) return launch_tiles<128>(att, tilesMemo[1], map, args, stream, error);
+    return launch_tiles<64>(att, tilesMemo[0], map, args, stream, error);
+}
+
+}  // namespace ff

@@ -6,88 +6,9 @@
 
 namespace ff {
 
-// ---- a warp a key ------------------------------------------------------------------------------
-
-// One CTA per (row, query head); its warps take the keys in turn, a key at a time, with a running maximum and sum, and
-// are joined at the end.
-template <int DIM>
-__global__ void __launch_bounds__(128) k_attend_simple(const AttendArgs a) {
-    constexpr int kValues = DIM / 32;  // of a lane: codes [kValues * lane, +kValues) of a head
-    __shared__ float shared[4][DIM + 2];
-    const uint32_t row = blockIdx.x / a.heads, head = blockIdx.x % a.heads, warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-    const uint32_t kvHead = head / (a.heads / a.kvHeads);
-    // the row's request
-    uint32_t r = 0;
-    while (r < a.requests && a.rowStart[r + 1] <= row) ++r;
-    float o[kValues], top = -INFINITY, sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kValues; ++i) o[i] = 0.0f;
-    if (r < a.requests) {
-        const int64_t rows = (int64_t)a.rowStart[r + 1] - a.rowStart[r], length = a.lengths[r];
-        const int64_t p = length - rows + (row - a.rowStart[r]);
-        float q[kValues];
-        for (int i = 0; i < kValues; ++i) q[i] = __uint_as_float((uint32_t)a.q[(size_t)row * a.qStride + head * DIM + lane * kValues + i] << 16);
-        const int64_t low = a.window ? p - a.window + 1 : 0;
-        for (int64_t j = warp; j <= p; j += 4) {
-            if (j < low && j >= a.sinks) j += (low - j) / 4 * 4;
-            if (j < low && j >= a.sinks) continue;
-            const uint32_t index = (uint32_t)(j / a.page.pageTokens), inPage = (uint32_t)(j % a.page.pageTokens);
-            const uint32_t page = index < a.tableStride ? a.blockTable[(size_t)r * a.tableStride + index] : FF_NO_PAGE;
-            if (page >= a.pageCount) {
-                if (lane == 0) *a.errorFlag = index < a.tableStride ? kFlagPage : kFlagTableRow;
-                continue;
-            }
-            const uint8_t *block = a.pages + (uint64_t)page * a.page.pageBytes + (uint64_t)kvHead * a.page.blockBytes;
-            float kv[2][kValues];
-#pragma unroll
-            for (int side = 0; side < 2; ++side) {
-                const uint8_t *part = block + side * a.page.values;
-                const uint32_t sb = *reinterpret_cast<const uint32_t *>(part + a.page.keyWords + inPage * a.page.wordBytes + lane * kValues / kGroup * 4);
-                const uint8_t *codes = part + inPage * a.page.codeBytes + lane * kValues / 2;
-#pragma unroll
-                for (int i = 0; i < kValues; ++i) {
-                    const float code = (float)(codes[i / 2] >> (4 * (i & 1)) & 15);
-                    kv[side][i] = fmaf(code, __uint_as_float(sb << 16), __uint_as_float(sb & 0xFFFF0000u));
-                }
-            }
-            float s = 0.0f;
-#pragma unroll
-            for (int i = 0; i < kValues; ++i) s = fmaf(q[i], kv[0][i], s);
-#pragma unroll
-            for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, d);
-            s *= a.scale;
-            const float next = fmaxf(top, s), keep = top == -INFINITY ? 0.0f : expf(top - next), w = expf(s - next);
-            sum = sum * keep + w;
-#pragma unroll
-            for (int i = 0; i < kValues; ++i) o[i] = fmaf(w, kv[1][i], o[i] * keep);
-            top = next;
-        }
-    }
-    for (int i = 0; i < kValues; ++i) shared[warp][lane * kValues + i] = o[i];
-    if (lane == 0) shared[warp][DIM] = top, shared[warp][DIM + 1] = sum;
-    __syncthreads();
-    float all = -INFINITY, total = 0.0f;
-    for (int w = 0; w < 4; ++w) all = fmaxf(all, shared[w][DIM]);
-    for (int w = 0; w < 4; ++w)
-        if (shared[w][DIM] != -INFINITY) total += shared[w][DIM + 1] * expf(shared[w][DIM] - all);
-    for (uint32_t i = threadIdx.x; i < DIM; i += 128) {
-        float v = 0.0f;
-        for (int w = 0; w < 4; ++w)
-            if (shared[w][DIM] != -INFINITY) v += shared[w][i] * expf(shared[w][DIM] - all);
-        v = total != 0.0f ? v / total : 0.0f;
-        uint32_t packed;
-        asm("cvt.rn.bf16x2.f32 %0, %1, %1;" : "=r"(packed) : "f"(v));
-        a.out[(size_t)row * a.outStride + head * DIM + i] = (uint16_t)packed;
-    }
-}
-
 bool launch_attend(FFAttention *att, const AttendArgs &a, cudaStream_t stream, const char **error) {
     if (a.maxRows <= 16) return launch_attend_rows(att, a, stream, error);
-    const dim3 grid(a.tokens * a.heads);
-    if (att->cfg.headDim == 64) k_attend_simple<64><<<grid, 128, 0, stream>>>(a);
-    else if (att->cfg.headDim == 128) k_attend_simple<128><<<grid, 128, 0, stream>>>(a);
-    else k_attend_simple<256><<<grid, 128, 0, stream>>>(a);
-    return launched(att, cudaSuccess, "k_attend", error);
+    return launch_attend_tiles(att, a, stream, error);
 }
 
 }  // namespace ff
@@ -207,8 +128,8 @@ FFAttention *ff_attention_create(int32_t deviceOrdinal, const FFAttentionConfig 
     alloc(&att->errorFlag, 1);
     alloc(&att->planCount, 1);
     att->rowsCtas = attend_rows_ctas(att->smCount);
-    alloc(&att->partials, (size_t)2 * att->rowsCtas * kPartialValues);
-    alloc(&att->stats, (size_t)2 * att->rowsCtas * kPartialColumns);
+    alloc(&att->partials, 2 * std::max((size_t)att->rowsCtas * kPartialValues, (size_t)att->smCount * kTileRows * config->headDim));
+    alloc(&att->stats, 2 * std::max((size_t)att->rowsCtas * kPartialColumns, (size_t)att->smCount * kTileRows));
     alloc(&att->arrived, att->rowsCtas);
     if (st == cudaSuccess) st = cudaDeviceSynchronize();
     if (st != cudaSuccess) {

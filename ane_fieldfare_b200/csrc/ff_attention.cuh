@@ -48,8 +48,9 @@ inline PageLayout page_layout(const FFAttentionConfig &c) {
     return l;
 }
 
-// Columns (rows times query heads of a key/value head) that a unit of few rows has at most, and their output values.
-constexpr uint32_t kPartialColumns = 32, kPartialValues = 4096;
+// Partial results of units that several CTAs share: columns (rows times query heads of a key/value head) of a unit, and
+// their output values, where requests have few rows (two CTAs an SM) and many (one).
+constexpr uint32_t kPartialColumns = 32, kPartialValues = 4096, kTileRows = 128;
 
 // Counts a launch and reports what it says.
 inline bool launched(FFAttention *att, cudaError_t status, const char *what, const char **error) {
@@ -94,6 +95,9 @@ bool launch_cache_read(FFAttention *att, const uint8_t *pages, uint32_t pageCoun
 // ff_attend_rows.cu
 uint32_t attend_rows_ctas(int smCount);
 bool launch_attend_rows(FFAttention *att, const AttendArgs &args, cudaStream_t stream, const char **error);
+
+// ff_attend_tiles.cu
+bool launch_attend_tiles(FFAttention *att, const AttendArgs &args, cudaStream_t stream, const char **error);
 
 // ff_attention.cu
 bool launch_attend(FFAttention *att, const AttendArgs &args, cudaStream_t stream, const char **error);
