@@ -34,7 +34,7 @@ struct RowsArgs {
     float *partials;      // [2 CTAs][columns][DIM]
     float2 *stats;        // [2 CTAs][columns] maximum (log2), sum
     uint32_t *arrived;    // [CTAs], zero between launches
-    uint32_t pageShift;
+    uint32_t pageShift, pieceShift;  // log2 of a page's tokens and of the keys of a tile on one page
 };
 
 __host__ __device__ constexpr uint32_t rows_stage_bytes(int dim) { return (kTileKeys * (dim + dim / 8) + 1023u) & ~1023u; }
@@ -43,13 +43,6 @@ __host__ __device__ constexpr uint32_t rows_smem(int dim, int nt) {
     return 1024u + rows_stages(dim) * rows_stage_bytes(dim) + 2u * 8u * nt * (dim + 4) * 4u;
 }
 
-// the NG scale words of a key
-template <int NG>
-__device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&w)[NG]) {
-    if (NG == 4) asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1 % NG]), "=r"(w[2 % NG]), "=r"(w[3 % NG]) : "r"(a));
-    else if (NG == 2) asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1 % NG]) : "r"(a));
-    else w[0] = lds32(a);
-}
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -59,11 +52,6 @@ __device__ __forceinline__ uint32_t transposed(uint32_t x) {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
-}
-__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
 }
 // a * b - c
 __device__ __forceinline__ uint32_t residual_f16x2(uint32_t a, uint32_t b, uint32_t c) {
@@ -97,11 +85,11 @@ __device__ __forceinline__ uint32_t key_of_row(uint32_t r) {
     return DIM == 128 ? (t & 1u) | (odd << 1) | ((t & 2u) << 1) : t | (odd << 2);
 }
 template <int DIM, int NT, bool SPLIT>
-__global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_attend_rows(const __grid_constant__ CUtensorMap map, const RowsArgs args) {
+__global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_attend_rows(const __grid_constant__ CUtensorMap mapCodes, const __grid_constant__ CUtensorMap mapWords, const RowsArgs args) {
     constexpr int NG = DIM / 64, CB = DIM / 2, WB = NG * 4;
     constexpr uint32_t kStage = rows_stage_bytes(DIM), kStages = rows_stages(DIM), kColumns = SPLIT ? 4 : 8 * NT;
     static_assert(!SPLIT || NT == 1, "four columns, each twice");
-    constexpr uint32_t kKeyWords = kTileKeys * CB * 2, kValueWords = kKeyWords + kTileKeys * WB;
+    constexpr uint32_t kKeyWords = kTileKeys * CB * 2;
     extern __shared__ uint8_t rowsSmem[];
     __shared__ __align__(8) uint64_t barriers[2 * 6];
     __shared__ uint32_t first[kRowsThreads + 1], warpSums[kConsumers + 1], holes[6];
@@ -226,8 +214,11 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
     if (warp == (uint32_t)kConsumers) {
         // ---------------- copies ----------------
         // A lane holds the page of one piece (the keys of a tile on one page): 32 pieces at a time, the next 32 in flight.
-        const uint32_t pieceKeys = min(kTileKeys, a.page.pageTokens), pieces = kTileKeys / pieceKeys;
-        const uint32_t tilesPer = 32u / pieces;  // tiles whose pieces a warp holds
+        // The warp runs as one and an elected lane issues: a copy in a branch that lanes take apart costs several hundred cycles,
+        // its operands go to the uniform registers by a loop over the lanes.
+        const uint32_t pieces = kTileKeys >> args.pieceShift, perTileShift = 6u - args.pieceShift;
+        const uint32_t tilesPer = 32u >> perTileShift;  // tiles whose pieces a warp holds
+        const uint32_t pieceCodes = 2u * CB << args.pieceShift, pieceWords = 2u * WB << args.pieceShift;
         uint32_t stage = 0, phase = 0;
         Walk w = locate(begin);
         uint32_t x = begin;
@@ -237,10 +228,10 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
             const int keysEnd = w.q.p0 + (int)w.q.rows;
             auto key_at = [&](uint32_t t) { return (t < w.q.tilesSink ? t : w.q.lowTile + t - w.q.tilesSink) * kTileKeys; };
             auto page_of = [&](uint32_t base) {
-                const uint32_t t = base + lane / pieces;
+                const uint32_t t = base + (lane >> perTileShift);
                 uint32_t page = FF_NO_PAGE;
                 if (t < t0 + count) {
-                    const uint32_t key = key_at(t) + lane % pieces * pieceKeys;
+                    const uint32_t key = key_at(t) + ((lane & (pieces - 1u)) << args.pieceShift);
                     if ((int)key < keysEnd) {
                         const uint32_t index = key >> args.pageShift;
                         if (index < a.tableStride) page = __ldg(a.blockTable + (size_t)w.r * a.tableStride + index);
@@ -256,29 +247,20 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
                 pagesNext = page_of(t + tilesPer);
                 const uint32_t many = min(tilesPer, t0 + count - t);
                 for (uint32_t i = 0; i < many; ++i) {
-                    // lane = 4 piece + kind: key codes, value codes, key words, value words
-                    const uint32_t piece = lane >> 2, kind = lane & 3u;
-                    const uint32_t page = __shfl_sync(0xFFFFFFFFu, pagesNow, (i * pieces + piece) & 31u);
-                    const bool live = piece < pieces && page < a.pageCount;
-                    const uint32_t lives = __ballot_sync(0xFFFFFFFFu, live);
+                    const uint32_t mine = __shfl_sync(0xFFFFFFFFu, pagesNow, (i << perTileShift) + (lane & (pieces - 1u)));
+                    const uint32_t lives = __ballot_sync(0xFFFFFFFFu, lane < pieces && mine < a.pageCount);
                     if (!mbar_try_wait(barEmpty + 8 * stage, phase ^ 1u) && !slot_wait_slow(barEmpty + 8 * stage, phase ^ 1u) && lane == 0) *a.errorFlag = kFlagWait;
                     __syncwarp();
-                    const uint32_t bar = barFull + 8 * stage, base = ring + stage * kStage;
-                    if (lane == 0) {
-                        uint32_t gone = 0;
-                        for (uint32_t p = 0; p < pieces; ++p) gone |= (lives >> (4 * p) & 1u ? 0u : 1u) << p;
-                        holes[stage] = gone;
-                        bar_expect(bar, (uint32_t)__popc(lives) / 4u * pieceKeys * 2u * (CB + WB));
+                    const uint32_t bar = barFull + 8 * stage, base = ring + stage * kStage, inTile = key_at(t + i) & (a.page.pageTokens - 1u);
+                    if (elect_one()) {
+                        holes[stage] = ~lives;
+                        bar_expect(bar, (uint32_t)__popc(lives) * (pieceCodes + pieceWords));
                     }
-                    __syncwarp();
-                    if (live) {
-                        const uint32_t inPage = (key_at(t + i) + piece * pieceKeys) & (a.page.pageTokens - 1u);
-                        const uint32_t block = page * a.kvHeads + head;
-                        if (kind < 2) {
-                            tma_load_4d(base + kind * (kTileKeys * CB) + piece * pieceKeys * CB, &map, 0, (int)inPage, (int)kind, (int)block, bar);
-                        } else {
-                            const uint8_t *src = a.pages + (uint64_t)block * a.page.blockBytes + (kind == 2 ? a.page.keyWords : a.page.valueWords) + inPage * WB;
-                            bulk_copy(base + (kind == 2 ? kKeyWords : kValueWords) + piece * pieceKeys * WB, src, pieceKeys * WB, bar);
+                    for (uint32_t p = 0; p < pieces; ++p) {
+                        const uint32_t block = __shfl_sync(0xFFFFFFFFu, mine, p) * a.kvHeads + head, at = (inTile + (p << args.pieceShift)) & (a.page.pageTokens - 1u);
+                        if ((lives >> p & 1u) && elect_one()) {
+                            tma_load_4d(base + p * pieceCodes, &mapCodes, 0, (int)at, 0, (int)block, bar);
+                            tma_load_3d(base + kKeyWords + p * pieceWords, &mapWords, (int)(at * NG), 0, (int)block, bar);
                         }
                     }
                     if (++stage == kStages) stage = 0, phase ^= 1u;
@@ -293,13 +275,17 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
 
     // ---------------- 16 keys of every tile ----------------
     const uint32_t g = lane >> 2, t = lane & 3u;
+    // A stage: [piece][keys, values][its keys][codes], then [piece][keys, values][its keys][words].
     const uint32_t keyA = 16 * warp + key_of_row<DIM>(g);  // the S fragments' rows: keys keyA and keyA + 8 of a tile
-    const uint32_t kOff = keyA * CB + ((t * 8) ^ chunk_flip<DIM>(keyA));
-    uint32_t vKey[2], vOff[2];  // the P fragments' keys 2t and 2t + 1, and those + 8
+    const uint32_t pieceAt = (16 * warp >> args.pieceShift) << args.pieceShift;  // first key of the warp's piece
+    const uint32_t kRow = keyA + pieceAt, vStep = 1u << args.pieceShift;         // (a piece's values lie behind its keys: rows pieceAt further)
+    const uint32_t kOff = kRow * CB + ((t * 8) ^ chunk_flip<DIM>(keyA));
+    uint32_t vKey[2], vRow[2], vOff[2];  // the P fragments' keys 2t and 2t + 1, and those + 8
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         vKey[i] = 16 * warp + key_of_row<DIM>(2 * t + i);
-        vOff[i] = vKey[i] * CB + ((g * 4) ^ chunk_flip<DIM>(vKey[i]));
+        vRow[i] = vKey[i] + pieceAt + vStep;
+        vOff[i] = vRow[i] * CB + ((g * 4) ^ chunk_flip<DIM>(vKey[i]));
     }
     uint32_t stage = 0, phase = 0;
     Walk w = locate(begin);
@@ -308,8 +294,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
         const uint32_t unitTiles = w.q.tiles, t0 = w.inRequest % unitTiles, unit = w.inRequest / unitTiles;
         const uint32_t head = unit / w.q.columnTiles, column0 = unit % w.q.columnTiles * kColumns;
         const uint32_t columns = w.q.rows * group, count = min(end - x, unitTiles - t0);
-        const uint32_t pieceKeys = min(kTileKeys, a.page.pageTokens);
-
+        
         // queries: f16 at a power of two of the column's largest value
         uint32_t qf[NG][4][NT][2];
         float qSum[NG][NT][2], toLog2[NT][2];
@@ -387,7 +372,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
             const uint32_t base = ring + stage * kStage;
             if (!mbar_try_wait(barFull + 8 * stage, phase) && !slot_wait_slow(barFull + 8 * stage, phase) && lane == 0) *a.errorFlag = kFlagWait;
             __syncwarp();
-            const bool hole = holes[stage] >> (16 * warp / pieceKeys) & 1u;
+            const bool hole = holes[stage] >> (16 * warp >> args.pieceShift) & 1u;
             // keys that not every row of the tile sees
             const bool careful = hole || j0 + 15 > pFirst || (a.window && (long long)j0 <= (long long)pLast - a.window && (uint32_t)j0 + 16u > a.sinks);
             auto sees = [&](int key, int p) {
@@ -397,7 +382,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
             // ---- value scales as f16 pairs of keys, at 2^-E ----
             uint32_t vWords[4][NG];  // keys 2t, 2t + 1, 2t + 8, 2t + 9
 #pragma unroll
-            for (int k = 0; k < 4; ++k) lds_words<NG>(base + kValueWords + (vKey[k & 1] + 8 * (k >> 1)) * WB, vWords[k]);
+            for (int k = 0; k < 4; ++k) lds_words<NG>(base + kKeyWords + (vRow[k & 1] + 8 * (k >> 1)) * WB, vWords[k]);
             if (careful) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
@@ -472,8 +457,8 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
 #pragma unroll
             for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
             uint32_t kWords[2][NG];
-            lds_words<NG>(base + kKeyWords + keyA * WB, kWords[0]);
-            lds_words<NG>(base + kKeyWords + (keyA + 8) * WB, kWords[1]);
+            lds_words<NG>(base + kKeyWords + kRow * WB, kWords[0]);
+            lds_words<NG>(base + kKeyWords + (kRow + 8) * WB, kWords[1]);
 #pragma unroll
             for (int G = 0; G < NG; ++G) {
                 const uint2 wa = lds64((base + kOff) ^ (uint32_t)(G * 32)), wb = lds64((base + kOff + 8 * CB) ^ (uint32_t)(G * 32));
@@ -508,7 +493,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         uint32_t words[NG];
-                        lds_words<NG>(base + kValueWords + (keyA + 8 * h) * WB, words);
+                        lds_words<NG>(base + kKeyWords + (kRow + vStep + 8 * h) * WB, words);
 #pragma unroll
                         for (int G = 0; G < NG; ++G) bad[h] |= is_broken(words[G]);
                     }
@@ -575,8 +560,8 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
                 uint32_t lo[2], hi[2];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const uint32_t wa = lds32((base + kTileKeys * CB + vOff[0] + 8 * h * CB) ^ (uint32_t)(G * 32));
-                    const uint32_t wb = lds32((base + kTileKeys * CB + vOff[1] + 8 * h * CB) ^ (uint32_t)(G * 32));
+                    const uint32_t wa = lds32((base + vOff[0] + 8 * h * CB) ^ (uint32_t)(G * 32));
+                    const uint32_t wb = lds32((base + vOff[1] + 8 * h * CB) ^ (uint32_t)(G * 32));
                     lo[h] = __byte_perm(wa, wb, 0x5410);
                     hi[h] = __byte_perm(wa, wb, 0x7632);
                 }
@@ -724,25 +709,32 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
 KernelSmemMemo rowsMemo[3][4];
 
 template <int DIM, int NT, bool SPLIT = false>
-bool launch_rows(FFAttention *att, KernelSmemMemo &memo, const CUtensorMap &map, const RowsArgs &args, cudaStream_t stream, const char **error) {
+bool launch_rows(FFAttention *att, KernelSmemMemo &memo, const CUtensorMap &codes, const CUtensorMap &words, const RowsArgs &args, cudaStream_t stream, const char **error) {
     const size_t smem = rows_smem(DIM, NT);
     int perSm = 0;
     if (!memo.prepare(k_attend_rows<DIM, NT, SPLIT>, att->device, smem, kRowsThreads, &perSm, error)) return false;
     const uint32_t grid = std::min((uint32_t)(att->smCount * std::max(1, perSm)), att->rowsCtas);
-    return launched(att, launch_pdl(k_attend_rows<DIM, NT, SPLIT>, dim3(grid), dim3(kRowsThreads), smem, stream, map, args), "k_attend_rows", error);
+    return launched(att, launch_pdl(k_attend_rows<DIM, NT, SPLIT>, dim3(grid), dim3(kRowsThreads), smem, stream, codes, words, args), "k_attend_rows", error);
 }
 
 }  // namespace
 
-bool make_pages_map(CUtensorMap *map, const AttendArgs &a, uint32_t dim, const char **error) {
-    const cuuint64_t dims[4] = {dim / 2, a.page.pageTokens, 2, (cuuint64_t)a.pageCount * a.kvHeads};
-    const cuuint64_t strides[3] = {dim / 2, a.page.values, a.page.blockBytes};
-    const cuuint32_t box[4] = {dim / 2, std::min(kTileKeys, a.page.pageTokens), 1, 1}, elem[4] = {1, 1, 1, 1};
+bool make_pages_maps(CUtensorMap *codes, CUtensorMap *words, const AttendArgs &a, uint32_t dim, uint32_t sides, const char **error) {
     const EncodeTiledFn encode = encode_tiled(error);
     if (!encode) return false;
-    const CUresult rc = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<uint8_t *>(a.pages), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                               dim == 256 ? CU_TENSOR_MAP_SWIZZLE_128B : dim == 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B,
-                               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const cuuint32_t piece = std::min(kTileKeys, a.page.pageTokens), groups = dim / kGroup, elem[4] = {1, 1, 1, 1};
+    const cuuint64_t blocks = (cuuint64_t)a.pageCount * a.kvHeads;
+    const cuuint64_t dims[4] = {dim / 2, a.page.pageTokens, 2, blocks}, strides[3] = {dim / 2, a.page.values, a.page.blockBytes};
+    const cuuint32_t box[4] = {dim / 2, piece, sides, 1};
+    CUresult rc = encode(codes, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<uint8_t *>(a.pages), dims, strides, box, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                         dim == 256 ? CU_TENSOR_MAP_SWIZZLE_128B : dim == 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (rc == CUDA_SUCCESS) {
+        const cuuint64_t wordDims[3] = {a.page.pageTokens * groups, 2, blocks}, wordStrides[2] = {a.page.values, a.page.blockBytes};
+        const cuuint32_t wordBox[3] = {piece * groups, 2, 1};
+        rc = encode(words, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<uint8_t *>(a.pages) + a.page.keyWords, wordDims, wordStrides, wordBox, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    }
     if (rc != CUDA_SUCCESS) return fail(error, "cuTensorMapEncodeTiled(cache pages) failed: " + std::to_string((int)rc));
     return true;
 }
@@ -751,25 +743,25 @@ uint32_t attend_rows_ctas(int smCount) { return 2u * (uint32_t)smCount; }
 
 bool launch_attend_rows(FFAttention *att, const AttendArgs &a, cudaStream_t stream, const char **error) {
     const uint32_t dim = att->cfg.headDim;
-    RowsArgs args{a, att->partials, att->stats, att->arrived, (uint32_t)__builtin_ctz(att->cfg.pageTokens)};
-    CUtensorMap map;
-    if (!make_pages_map(&map, a, dim, error)) return false;
+    RowsArgs args{a, att->partials, att->stats, att->arrived, (uint32_t)__builtin_ctz(att->cfg.pageTokens), (uint32_t)__builtin_ctz(std::min(kTileKeys, a.page.pageTokens))};
+    CUtensorMap codes, words;
+    if (!make_pages_maps(&codes, &words, a, dim, 2, error)) return false;
     const uint32_t columns = a.maxRows * (a.heads / a.kvHeads);
     if (dim == 256) {
-        if (columns <= 4) return launch_rows<256, 1, true>(att, rowsMemo[0][0], map, args, stream, error);
-        if (columns <= 8) return launch_rows<256, 1>(att, rowsMemo[0][1], map, args, stream, error);
-        return launch_rows<256, 2>(att, rowsMemo[0][2], map, args, stream, error);
+        if (columns <= 4) return launch_rows<256, 1, true>(att, rowsMemo[0][0], codes, words, args, stream, error);
+        if (columns <= 8) return launch_rows<256, 1>(att, rowsMemo[0][1], codes, words, args, stream, error);
+        return launch_rows<256, 2>(att, rowsMemo[0][2], codes, words, args, stream, error);
     }
     if (dim == 128) {
-        if (columns <= 4) return launch_rows<128, 1, true>(att, rowsMemo[1][0], map, args, stream, error);
-        if (columns <= 8) return launch_rows<128, 1>(att, rowsMemo[1][1], map, args, stream, error);
-        if (columns <= 16) return launch_rows<128, 2>(att, rowsMemo[1][2], map, args, stream, error);
-        return launch_rows<128, 4>(att, rowsMemo[1][3], map, args, stream, error);
+        if (columns <= 4) return launch_rows<128, 1, true>(att, rowsMemo[1][0], codes, words, args, stream, error);
+        if (columns <= 8) return launch_rows<128, 1>(att, rowsMemo[1][1], codes, words, args, stream, error);
+        if (columns <= 16) return launch_rows<128, 2>(att, rowsMemo[1][2], codes, words, args, stream, error);
+        return launch_rows<128, 4>(att, rowsMemo[1][3], codes, words, args, stream, error);
     }
-    if (columns <= 4) return launch_rows<64, 1, true>(att, rowsMemo[2][0], map, args, stream, error);
-    if (columns <= 8) return launch_rows<64, 1>(att, rowsMemo[2][1], map, args, stream, error);
-    if (columns <= 16) return launch_rows<64, 2>(att, rowsMemo[2][2], map, args, stream, error);
-    return launch_rows<64, 4>(att, rowsMemo[2][3], map, args, stream, error);
+    if (columns <= 4) return launch_rows<64, 1, true>(att, rowsMemo[2][0], codes, words, args, stream, error);
+    if (columns <= 8) return launch_rows<64, 1>(att, rowsMemo[2][1], codes, words, args, stream, error);
+    if (columns <= 16) return launch_rows<64, 2>(att, rowsMemo[2][2], codes, words, args, stream, error);
+    return launch_rows<64, 4>(att, rowsMemo[2][3], codes, words, args, stream, error);
 }
 
 }  // namespace ff

@@ -4,12 +4,15 @@
 // A unit of work is one row tile; its keys are tiles of 64, and all units' tiles end to end are cut into equal runs, one
 // per CTA, one CTA per SM.  A unit that several CTAs share is joined by whichever of them ends last, in the CTAs' order.
 //
-// Per key tile, warp by role: one copies packed codes and scale words; eight turn them into f16 tiles in shared memory
-// (128-byte swizzle, keys and values alike [64 values][key][128 bytes]); one issues the MMAs; four own a row a thread:
+// Per key tile, warp by role: two copy packed codes, keys' with the scale words and values'; one turns the tile's scale words into the pairs that
+// the expansion multiplies with; eight expand codes to f16 tiles in shared memory (128-byte swizzle, keys and values alike
+// [64 values][key][128 bytes]), four a slot, so that one group's waits stand behind the other's arithmetic; one issues the MMAs; two
+// warpgroups own a row a thread and take the tiles in turn:
 //   S = Q K^T   A: the rows' queries, in tensor memory for the whole unit (read from shared memory they would cost the
 //               128 bytes a cycle that dequantizing needs); B: the keys, K-major
 //   P = 2^(S f + E - M)   in registers, back into S's columns as f16
 //   O += P V    A: P; B: the values, N-major; O stays in tensor memory
+// A tile's warpgroup waits for the maximum M that the one before it settled on, not for its weights.
 // Tensor memory: Q dim/2, O dim, S two tiles of 64 columns: all 512 at dim 256.
 //
 // f16 holds 11 bits of keys, values and weights where bf16 would hold 8; its range is kept by powers of two: a row's
@@ -25,26 +28,29 @@ namespace ff {
 
 namespace {
 
-constexpr int kDequantWarps = 8, kSoftmaxWarps = 4;
-constexpr int kFirstDequant = 2, kFirstSoftmax = kFirstDequant + kDequantWarps;
-constexpr int kTilesThreads = 32 * (kFirstSoftmax + kSoftmaxWarps);
+// warps by role: copies of keys, MMAs, scales, copies of values; expansion; rows
+constexpr int kKeyCopyWarp = 0, kMmaWarp = 1, kScaleWarp = 2, kValueCopyWarp = 3, kDequantWarps = 8, kRowGroups = 2;
+constexpr int kFirstDequant = 4, kFirstRowWarp = kFirstDequant + kDequantWarps, kRowWarps = 4 * kRowGroups;
+constexpr int kTilesThreads = 32 * (kFirstRowWarp + kRowWarps);
+// registers a thread by role: together no more than the launch's 96 each
+constexpr int kRegsOthers = 64, kRegsRows = 144;
+static_assert(128 * kRegsOthers + 32 * kDequantWarps * kRegsOthers + 32 * kRowWarps * kRegsRows <= kTilesThreads * 96, "register split");
 constexpr uint32_t kRows = kTileRows;
-// Tiles whose scale words and exponents are kept.  Those of tile n + 8 are written once the keys of n + 6 are expanded, so once
-// the logits of n + 4 are formed, which are issued behind the products of the values of n + 2: tile n is done with.
-constexpr uint32_t kInfo = 8;
-constexpr uint32_t kSlots = 4, kPacked = 4;
+constexpr uint32_t kInfo = 4;   // tiles whose scales and exponents are kept
+constexpr uint32_t kSlots = 4, kPacked = 3;  // expanded tiles; packed ones, of keys and of values each
 
 struct TilesArgs {
     AttendArgs a;
     float *partials;      // [2 CTAs][rows][DIM]
     float2 *stats;        // [2 CTAs][rows]
     uint32_t *arrived;    // [CTAs], zero between launches
-    uint32_t pageShift, tileTokens;  // tokens of a row tile
+    uint32_t pageShift, pieceShift, tileTokens;  // log2 of a page's tokens and of the keys of a tile on one page; tokens of a row tile
 };
 
 __host__ __device__ constexpr uint32_t slot_bytes(int dim) { return kTileKeys * dim * 2; }
-__host__ __device__ constexpr uint32_t packed_bytes(int dim) { return (kTileKeys * (dim / 2 + 2 * (dim / 16)) + 1023u) & ~1023u; }  // codes, key words, value words
-__host__ __device__ constexpr uint32_t tiles_smem(int dim) { return 1024u + kSlots * slot_bytes(dim) + kPacked * packed_bytes(dim) + kInfo * kTileKeys * (dim / 64) * 4u; }
+__host__ __device__ constexpr uint32_t packed_bytes(int dim) { return (kTileKeys * dim / 2 + 1023u) & ~1023u; }
+__host__ __device__ constexpr uint32_t words_bytes(int dim) { return 2u * kTileKeys * (dim / 64) * 4u; }  // of a tile, keys' and values'
+__host__ __device__ constexpr uint32_t tiles_smem(int dim) { return 1024u + kSlots * slot_bytes(dim) + 2 * kPacked * packed_bytes(dim) + (kInfo + kPacked) * words_bytes(dim); }
 
 // K-major or N-major tile of f16 with the 128-byte swizzle: rows of 128 bytes, groups of eight 1024 bytes apart; N-major:
 // the next 64 values `lead` bytes further.
@@ -71,6 +77,23 @@ __device__ __forceinline__ void mma_a_tmem(uint32_t d, uint32_t a, uint64_t b, u
 __device__ __forceinline__ void commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
+// The bounded waits of ff_tc_device.cuh without a call: a kernel that divides its registers among the roles has none.
+template <bool kSleep>
+__device__ __forceinline__ bool wait_lane(uint32_t bar, uint32_t parity, volatile uint32_t *abortFlag) {
+    if (mbar_try_wait(bar, parity)) return true;
+#pragma unroll 1
+    for (uint32_t i = 0; i < kSpinLimit; ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (kSleep) __nanosleep(40);
+        if ((i & 255u) == 255u && *abortFlag) return false;
+    }
+    *abortFlag = 1u;
+    return false;
+}
+template <bool kSleep>
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile uint32_t *abortFlag) {
+    return __all_sync(0xFFFFFFFFu, wait_lane<kSleep>(bar, parity, abortFlag));
+}
 __device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c) {
     uint32_t r;
     asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
@@ -85,51 +108,53 @@ struct RowTileOf {
 };
 
 template <int DIM>
-__global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_constant__ CUtensorMap map, const TilesArgs args) {
+__global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_constant__ CUtensorMap mapCodes, const __grid_constant__ CUtensorMap mapWords, const TilesArgs args) {
     constexpr int NG = DIM / 64, CB = DIM / 2, WB = NG * 4;
     constexpr uint32_t kSlot = slot_bytes(DIM), kPack = packed_bytes(DIM);
-    constexpr uint32_t kKeyWords = kTileKeys * CB, kValueWords = kKeyWords + kTileKeys * WB;
-    constexpr uint32_t kSlotWarps = 2 * NG, kGroupsOfWarps = kDequantWarps / kSlotWarps;
+    constexpr uint32_t kWordSide = words_bytes(DIM) / 2, kUnits = kTileKeys * NG;  // of a slot: a key's group of 64 values
+    constexpr uint32_t kGroupWarps = DIM == 64 ? 2 : 4, kGroups = kDequantWarps / kGroupWarps, kUnitsEach = kUnits / (32 * kGroupWarps);
     constexpr uint32_t kColQ = 0, kColO = DIM / 2, kColS = kColO + DIM;
     extern __shared__ uint8_t tilesSmem[];
-    __shared__ __align__(8) uint64_t barriers[2 * kSlots + 2 * kPacked + 8 + kInfo + kGroupsOfWarps];
+    __shared__ __align__(8) uint64_t barriers[2 * kSlots + 4 * kPacked + 2 * kInfo + 2 + 2 + 2 + 1 + 1 + 8];
     __shared__ uint32_t tmemSlot, lastPart;
     __shared__ volatile uint32_t abortFlag;
     __shared__ uint32_t firstTile[kTilesThreads + 1], firstWork[kTilesThreads + 1], warpSums[32];
-    __shared__ uint32_t slotMax[kGroupsOfWarps][2][2][kSlotWarps];
     __shared__ uint32_t holes[kPacked], broken[kInfo][2], hidden[kInfo][2];
     __shared__ int exponents[kInfo][2];
+    __shared__ float topShared[kRows], sumShared[kRowGroups][kRows], refShared[kRowGroups][kRows];
     const AttendArgs &a = args.a;
     const uint32_t tid = threadIdx.x, warp = (uint32_t)warp_index(), lane = tid & 31u;
-    const uint32_t slots = (sm_addr(tilesSmem) + 1023u) & ~1023u, packed = slots + kSlots * kSlot, words = packed + kPacked * kPack;
+    const uint32_t slots = (sm_addr(tilesSmem) + 1023u) & ~1023u, packed = slots + kSlots * kSlot, scales = packed + 2 * kPacked * kPack, words = scales + kInfo * words_bytes(DIM);
     const uint32_t group = a.heads / a.kvHeads;
     const uint32_t bar0 = sm_addr(barriers);
-    const uint32_t barTile = bar0, barTileFree = bar0 + 8 * kSlots, barPack = barTileFree + 8 * kSlots, barPackFree = barPack + 8 * kPacked;
-    const uint32_t barS = barPackFree + 8 * kPacked, barP = barS + 16, barO = barP + 16, barQ = barO + 16;
-    const uint32_t barJoin = barQ + 8, barInfo = barJoin + 8, barMax = barInfo + 8 * kInfo;
+    const uint32_t barTile = bar0, barTileFree = barTile + 8 * kSlots, barPack = barTileFree + 8 * kSlots, barPackFree = barPack + 16 * kPacked;  // keys', then values'
+    const uint32_t barInfo = barPackFree + 16 * kPacked, barInfoFree = barInfo + 8 * kInfo;
+    const uint32_t barS = barInfoFree + 8 * kInfo, barP = barS + 16, barO = barP + 16, barQ = barO + 16, barJoin = barQ + 8, barTop = barJoin + 8;
     if (tid == 0) {
         abortFlag = 0;
         for (uint32_t s = 0; s < kSlots; ++s) {
-            mbar_init(barTile + 8 * s, kSlotWarps);
+            mbar_init(barTile + 8 * s, kGroupWarps);
             mbar_init(barTileFree + 8 * s, 1);
         }
-        for (uint32_t s = 0; s < kPacked; ++s) {
+        for (uint32_t s = 0; s < 2 * kPacked; ++s) {
             mbar_init(barPack + 8 * s, 1);
-            mbar_init(barPackFree + 8 * s, kSlotWarps);
+            mbar_init(barPackFree + 8 * s, kGroupWarps + (s < kPacked ? 1 : 0));  // (keys: and the scale warp)
+        }
+        for (uint32_t s = 0; s < kInfo; ++s) {
+            mbar_init(barInfo + 8 * s, 1);
+            mbar_init(barInfoFree + 8 * s, 1);
         }
         for (uint32_t s = 0; s < 2; ++s) {
             mbar_init(barS + 8 * s, 1);
-            mbar_init(barP + 8 * s, kSoftmaxWarps);
+            mbar_init(barP + 8 * s, 4);
+            mbar_init(barO + 8 * s, 1);
         }
-        mbar_init(barO, 1);
-        mbar_init(barO + 8, 1);
-        mbar_init(barQ, kSoftmaxWarps);
-        mbar_init(barJoin, kSoftmaxWarps);
-        for (uint32_t s = 0; s < kInfo; ++s) mbar_init(barInfo + 8 * s, kSlotWarps);
-        for (uint32_t s = 0; s < kGroupsOfWarps; ++s) mbar_init(barMax + 8 * s, kSlotWarps);
+        mbar_init(barQ, kRowWarps);
+        mbar_init(barJoin, kRowWarps);
+        for (uint32_t s = 0; s < 8; ++s) mbar_init(barTop + 8 * s, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 1) {
+    if (warp == (uint32_t)kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(sm_addr(&tmemSlot)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -288,23 +313,32 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
         set_segment(w, x);
     };
     auto key_at = [&](const RowTileOf &q, uint32_t t) { return (t < q.tilesSink ? t : q.lowTile + t - q.tilesSink) * kTileKeys; };
-    const uint32_t pieceKeys = min(kTileKeys, a.page.pageTokens), pieces = kTileKeys / pieceKeys;
+    const uint32_t pieceKeys = 1u << args.pieceShift, pieces = kTileKeys >> args.pieceShift;
 
-    if (begin < end) {
-        if (warp == 0) {
-            // ---------------- copies: K0, K1, V0, K2, V1, ... of every segment ----------------
+    if (warp < (uint32_t)kFirstRowWarp) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOthers));
+        if (begin >= end) {
+            // nothing
+        } else if (warp == (uint32_t)kKeyCopyWarp || warp == (uint32_t)kValueCopyWarp) {
+            // ---------------- copies ----------------
+            // The warp runs as one and an elected lane issues (a copy in a branch that lanes take apart costs several hundred
+            // cycles: its operands go to the uniform registers by a loop over the lanes); without a division in the loop, and keys
+            // and values by a warp each: with one for both its chain of latencies, 2300 cycles a tile, was the kernel's pace.
+            const uint32_t side = warp == (uint32_t)kKeyCopyWarp ? 0u : 1u;
+            const uint32_t full = barPack + 8 * kPacked * side, empty = barPackFree + 8 * kPacked * side, codes = packed + side * kPacked * kPack;
+            const uint32_t pieceCodes = CB << args.pieceShift, pieceWords = WB << args.pieceShift, pieceBytes = pieceCodes + (side ? 0u : 2u * pieceWords);
+            const uint32_t perTileShift = 6u - args.pieceShift, tilesPer = 32u >> perTileShift;  // pieces of a tile, as a shift; tiles whose pages a warp holds
             uint32_t stage = 0, phase = 0;
             bool ok = true;
             Walk w = locate(begin);
             for (uint32_t x = begin; x < end && ok;) {
                 const int keysEnd = w.q.p0 + (int)w.q.tokens;
-                const uint32_t tilesPer = 32u / pieces;
-                // a lane holds the page of one piece: of `tilesPer` tiles from `base` on, for keys and for values apart
+                // a lane holds the page of one piece of `tilesPer` tiles from `base` on
                 auto page_of = [&](uint32_t base) {
-                    const uint32_t t = base + lane / pieces;
+                    const uint32_t t = base + (lane >> perTileShift);
                     uint32_t page = FF_NO_PAGE;
                     if (t < w.t0 + w.count) {
-                        const uint32_t key = key_at(w.q, t) + lane % pieces * pieceKeys;
+                        const uint32_t key = key_at(w.q, t) + ((lane & (pieces - 1u)) << args.pieceShift);
                         if ((int)key < keysEnd) {
                             const uint32_t index = key >> args.pageShift;
                             if (index < a.tableStride) {
@@ -317,62 +351,42 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                     }
                     return page;
                 };
-                uint32_t pagesK = page_of(w.t0), pagesV = pagesK, nextK = page_of(w.t0 + tilesPer);
-                auto copy = [&](uint32_t t, bool key, uint32_t pagesNow) {
-                    // lane = 4 piece + kind: codes, key words, value words (values: codes alone)
-                    const uint32_t piece = lane >> 2, kind = lane & 3u;
-                    const uint32_t page = __shfl_sync(0xFFFFFFFFu, pagesNow, ((t - w.t0) % tilesPer * pieces + piece) & 31u);
-                    const bool live = piece < pieces && page < a.pageCount;
-                    const uint32_t lives = __ballot_sync(0xFFFFFFFFu, live);
-                    if (!mbar_wait_warp<true, Order::kLocal>(barPackFree + 8 * stage, phase ^ 1u, &abortFlag)) {
-                        ok = false;
-                        return;
-                    }
-                    const uint32_t bar = barPack + 8 * stage, base = packed + stage * kPack;
-                    if (lane == 0) {
-                        uint32_t gone = 0;
-                        for (uint32_t p = 0; p < pieces; ++p) gone |= (lives >> (4 * p) & 1u ? 0u : 1u) << p;
-                        holes[stage] = gone;
-                        mbar_expect_tx(bar, (uint32_t)__popc(lives) / 4u * pieceKeys * (key ? CB + 2 * WB : CB));
-                    }
-                    __syncwarp();
-                    if (live && kind < (key ? 3u : 1u)) {
-                        const uint32_t inPage = (key_at(w.q, t) + piece * pieceKeys) & (a.page.pageTokens - 1u);
-                        const uint32_t block = page * a.kvHeads + w.head;
-                        if (kind == 0) {
-                            tma_load_4d(base + piece * pieceKeys * CB, &map, 0, (int)inPage, key ? 0 : 1, (int)block, bar);
-                        } else {
-                            const uint8_t *src = a.pages + (uint64_t)block * a.page.blockBytes + (kind == 1 ? a.page.keyWords : a.page.valueWords) + inPage * WB;
-                            bulk_copy(base + (kind == 1 ? kKeyWords : kValueWords) + piece * pieceKeys * WB, src, pieceKeys * WB, bar);
+                const uint32_t tEnd = w.t0 + w.count;
+                uint32_t pagesNext = page_of(w.t0);
+                for (uint32_t base = w.t0; base < tEnd && ok; base += tilesPer) {
+                    const uint32_t pagesNow = pagesNext, many = min(tilesPer, tEnd - base);
+                    pagesNext = page_of(base + tilesPer);
+                    for (uint32_t i = 0; i < many; ++i) {
+                        const uint32_t mine = __shfl_sync(0xFFFFFFFFu, pagesNow, (i << perTileShift) + (lane & (pieces - 1u)));
+                        const uint32_t lives = __ballot_sync(0xFFFFFFFFu, lane < pieces && mine < a.pageCount);
+                        if (!(ok = wait_warp<true>(empty + 8 * stage, phase ^ 1u, &abortFlag))) break;
+                        const uint32_t bar = full + 8 * stage, inTile = key_at(w.q, base + i) & (a.page.pageTokens - 1u);
+                        const uint32_t toCodes = codes + stage * kPack, toWords = words + stage * words_bytes(DIM);
+                        if (elect_one()) {
+                            if (!side) holes[stage] = ~lives;
+                            mbar_expect_tx(bar, (uint32_t)__popc(lives) * pieceBytes);
                         }
-                    }
-                    if (++stage == kPacked) stage = 0, phase ^= 1u;
-                };
-                const uint32_t last = w.t0 + w.count - 1;
-                copy(w.t0, true, pagesK);
-                for (uint32_t t = w.t0; t <= last && ok; ++t) {
-                    if (t < last) {
-                        if ((t + 1 - w.t0) % tilesPer == 0) {
-                            pagesK = nextK;
-                            nextK = page_of(t + 1 + tilesPer);
+                        for (uint32_t p = 0; p < pieces; ++p) {
+                            const uint32_t block = __shfl_sync(0xFFFFFFFFu, mine, p) * a.kvHeads + w.head, at = (inTile + (p << args.pieceShift)) & (a.page.pageTokens - 1u);
+                            if ((lives >> p & 1u) && elect_one()) {
+                                tma_load_4d(toCodes + p * pieceCodes, &mapCodes, 0, (int)at, (int)side, (int)block, bar);
+                                if (!side) tma_load_3d(toWords + p * 2u * pieceWords, &mapWords, (int)(at * NG), 0, (int)block, bar);
+                            }
                         }
-                        copy(t + 1, true, pagesK);
+                        if (++stage == kPacked) stage = 0, phase ^= 1u;
                     }
-                    if (!ok) break;
-                    if ((t - w.t0) % tilesPer == 0 && t != w.t0) pagesV = pagesK;  // (keys are one tile ahead: the same pages)
-                    copy(t, false, pagesV);
                 }
                 x += w.count;
-                if (x < end) next_segment(w, x);
+                if (ok && x < end) next_segment(w, x);
             }
-        } else if (warp == 1) {
+        } else if (warp == (uint32_t)kMmaWarp) {
             // ---------------- MMAs ----------------
             uint32_t slot = 0, phase = 0, tile = 0, unitNo = 0;  // tile: key tiles so far (its S buffer, the barriers' parities)
             bool ok = true;
             Walk w = locate(begin);
             const uint32_t idescS = idesc_f16(kTileKeys, false), idescO = idesc_f16(DIM, true);
             auto scores = [&](uint32_t n) {  // S of the n-th tile, from the slot that is next
-                if (!mbar_wait_warp<false, Order::kLocal>(barTile + 8 * slot, phase, &abortFlag)) return false;
+                if (!wait_warp<false>(barTile + 8 * slot, phase, &abortFlag)) return false;
                 tc_fence_after();
                 const uint64_t desc = desc_sw128(slots + slot * kSlot, 16);
                 const uint32_t d = tmem + kColS + (n & 1u) * kTileKeys;
@@ -388,13 +402,13 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                 return true;
             };
             for (uint32_t x = begin; x < end && ok;) {
-                ok = mbar_wait_warp<false, Order::kLocal>(barQ, unitNo & 1u, &abortFlag);
+                ok = wait_warp<false>(barQ, unitNo & 1u, &abortFlag);
                 tc_fence_after();
                 ok = ok && scores(tile);
                 for (uint32_t i = 0; i < w.count && ok; ++i, ++tile) {
                     if (i + 1 < w.count && !(ok = scores(tile + 1))) break;
-                    if (!(ok = mbar_wait_warp<false, Order::kLocal>(barTile + 8 * slot, phase, &abortFlag))) break;
-                    if (!(ok = mbar_wait_warp<false, Order::kLocal>(barP + 8 * (tile & 1u), tile >> 1 & 1u, &abortFlag))) break;
+                    if (!(ok = wait_warp<false>(barTile + 8 * slot, phase, &abortFlag))) break;
+                    if (!(ok = wait_warp<false>(barP + 8 * (tile & 1u), tile >> 1 & 1u, &abortFlag))) break;
                     tc_fence_after();
                     const uint64_t desc = desc_sw128(slots + slot * kSlot, kTileKeys * 128);
                     const uint32_t p = tmem + kColS + (tile & 1u) * kTileKeys;
@@ -403,6 +417,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                         for (uint32_t k = 0; k < kTileKeys / 16; ++k) mma_a_tmem(tmem + kColO, p + 8 * k, desc + k * (2048 >> 4), idescO, (i | k) != 0);
                         commit(barTileFree + 8 * slot);
                         commit(barO + 8 * (tile & 1u));
+                        commit(barInfoFree + 8 * (tile % kInfo));  // weights formed, values expanded: nobody looks at the tile's scales any more
                     }
                     __syncwarp();
                     if (++slot == kSlots) slot = 0, phase ^= 1u;
@@ -411,104 +426,116 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                 x += w.count;
                 if (x < end) next_segment(w, x);
             }
-        } else if (warp < (uint32_t)kFirstSoftmax) {
-            // ---------------- dequantizing ----------------
-            // 2 NG warps a slot, a thread one group of 64 values of one key; with fewer values a head, groups of warps take
-            // slots in turn.
-            const uint32_t dw = warp - kFirstDequant, grp = dw / kSlotWarps, inGroup = dw % kSlotWarps;
-            const uint32_t unit = inGroup * 32 + lane, key = unit % kTileKeys, G = unit / kTileKeys;  // (a warp's keys follow one another)
-            const uint32_t codesAt = key * CB, flip = chunk_flip<DIM>(key);
-            uint32_t item = 0, tile = 0, keySlots = 0;  // slots filled by all groups; key tiles so far; key slots of this group
+        } else if (warp == (uint32_t)kScaleWarp) {
+            // ---------------- scales: a lane two keys of a tile ----------------
+            // What no row sees is nothing; a visible key with a value that is no number is marked, and so is one whose page is
+            // outside the cache.  A group's word for the expansion: f16 scale * 2^(24 - E) | f16 bias * 2^-E, the largest of
+            // 16 scale and |bias| of the tile 2^-6 .. 2^-5.
+            uint32_t tile = 0;
             bool ok = true;
             Walk w = locate(begin);
-            auto expand = [&](uint32_t src, uint32_t dst, uint32_t word, int E) {
-                const float f = power_of_two(-E);
-                const float s = low16(word) * f, b = high16(word) * f;
-                const uint32_t s0 = pack_f16(s * 0x1p24f, s * 0x1p24f), s1 = pack_f16(s * 0x1p20f, s * 0x1p20f), bb = pack_f16(b, b);
-                const uint32_t to = dst + G * (kTileKeys * 128) + key * 128;
+            for (uint32_t x = begin; x < end && ok;) {
+                const int pLast = w.q.p0 + (int)w.q.tokens - 1;
+                for (uint32_t i = 0; i < w.count; ++i, ++tile) {
+                    const uint32_t at = tile % kPacked, info = tile % kInfo;
+                    if (!(ok = wait_warp<true>(barPack + 8 * at, tile / kPacked & 1u, &abortFlag))) break;
+                    const uint32_t gone = holes[at];
+                    uint32_t v[2][2][NG];  // [keys, values][lane's key][group]
+                    uint32_t bad[2], out[2];
 #pragma unroll
-                for (uint32_t h = 0; h < 2; ++h) {
-                    const uint4 v = lds128(src + codesAt + ((G * 32 + 16 * h) ^ flip));
-                    const uint32_t c[4] = {v.x, v.y, v.z, v.w};
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t key = lane + 32 * h;
+                        const int j = (int)(key_at(w.q, w.t0 + i) + key), p = max(j, w.q.p0);  // of the rows that may see it, the one whose window goes back furthest
+                        const bool hole = gone >> (key >> args.pieceShift) & 1u;
+                        const bool seen = p <= pLast && (!a.window || (long long)j > (long long)p - a.window || (uint32_t)j < a.sinks);
+                        bool none = false;
 #pragma unroll
-                    for (uint32_t i = 0; i < 4; ++i) {
-                        const uint32_t upper = c[i] >> 8;
-                        sts128(to + (((4 * h + i) ^ (key & 7u)) << 4), fma_f16x2(c[i] & 0x000F000Fu, s0, bb), fma_f16x2(c[i] & 0x00F000F0u, s1, bb),
-                               fma_f16x2(upper & 0x000F000Fu, s0, bb), fma_f16x2(upper & 0x00F000F0u, s1, bb));
+                        for (int side = 0; side < 2; ++side) {
+                            // (of a piece: the keys' words, then the values')
+                            lds_words<NG>(words + at * words_bytes(DIM) + (((key >> args.pieceShift) * 2 + side) << args.pieceShift) * WB + (key & (pieceKeys - 1u)) * WB, v[side][h]);
+#pragma unroll
+                            for (int G = 0; G < NG; ++G) none |= is_broken(v[side][h][G]);
+                        }
+                        bad[h] = __ballot_sync(0xFFFFFFFFu, seen && !hole && none);
+                        out[h] = __ballot_sync(0xFFFFFFFFu, seen && hole);
+                        if (!seen || hole || none)
+#pragma unroll
+                            for (int side = 0; side < 2; ++side)
+#pragma unroll
+                                for (int G = 0; G < NG; ++G) v[side][h][G] = 0u;
                     }
-                }
-            };
-            auto fill = [&](uint32_t t, uint32_t n, bool isKey) {  // tile t of the segment, the n-th of the CTA
-                if (item % kGroupsOfWarps != grp) {
-                    ++item;
-                    return;
-                }
-                const uint32_t slot = item % kSlots, slotPhase = item / kSlots & 1u, pack = item % kPacked, packPhase = item / kPacked & 1u;
-                ++item;
-                if (!mbar_wait<Order::kLocal>(barPack + 8 * pack, packPhase, &abortFlag)) {
-                    ok = false;
-                    return;
-                }
-                const uint32_t src = packed + pack * kPack, info = n % kInfo;
-                uint32_t word;
-                int E;
-                if (isKey) {
-                    // the tile's scale words, keys' and values': what no row sees is nothing, what is no number is marked
-                    word = lds32(src + kKeyWords + key * WB + G * 4);
-                    uint32_t value = lds32(src + kValueWords + key * WB + G * 4);
-                    const int j = (int)(key_at(w.q, t) + key), pLast = w.q.p0 + (int)w.q.tokens - 1, p = max(j, w.q.p0);
-                    const bool hole = holes[pack] >> (key / pieceKeys) & 1u;
-                    const bool seen = p <= pLast && (!a.window || (long long)j > (long long)p - a.window || (uint32_t)j < a.sinks);
-                    const bool bad = seen && !hole && (is_broken(word) || is_broken(value));
-                    if (!seen || hole || bad) word = value = 0u;
-                    const uint32_t most = __reduce_max_sync(0xFFFFFFFFu, word_exponent(word)), mostValue = __reduce_max_sync(0xFFFFFFFFu, word_exponent(value));
-                    const uint32_t marked = __ballot_sync(0xFFFFFFFFu, bad), gone = __ballot_sync(0xFFFFFFFFu, seen && hole);
-                    // (what is kept of the tile kInfo back is used: its values are multiplied.  The maxima of the key slot two
-                    // back are read: every warp has been at the barrier of the one between.)
-                    const uint32_t turn = keySlots & 1u;
-                    if (inGroup < 2 && lane == 0) {
-                        broken[info][inGroup] = 0u;
-                        hidden[info][inGroup] = gone;
-                    }
-                    if (lane == 0) {
-                        slotMax[grp][turn][0][inGroup] = most;
-                        slotMax[grp][turn][1][inGroup] = mostValue;
-                    }
-                    asm volatile("st.shared.u32 [%0], %1;" ::"r"(words + ((info * NG + G) * kTileKeys + key) * 4), "r"(value) : "memory");
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(barMax + 8 * grp);
-                    if (!mbar_wait<Order::kLocal>(barMax + 8 * grp, keySlots & 1u, &abortFlag)) {
-                        ok = false;
-                        return;
-                    }
-                    ++keySlots;
-                    uint32_t top = 0, topValue = 0;
+                    if (lane == 0) mbar_arrive(barPackFree + 8 * at);
+                    if (!(ok = wait_warp<true>(barInfoFree + 8 * info, tile / kInfo & 1u ^ 1u, &abortFlag))) break;
 #pragma unroll
-                    for (uint32_t i = 0; i < kSlotWarps; ++i) {
-                        top = max(top, slotMax[grp][turn][0][i]);
-                        topValue = max(topValue, slotMax[grp][turn][1][i]);
-                    }
-                    E = min(max((int)top - 127 + 6, -120), 120);  // the largest is 2^-6 .. 2^-5
-                    if (marked && lane == 0) atomicOr(&broken[info][inGroup & 1u], marked);
-                    if (inGroup == 0 && lane == 0) {
-                        exponents[info][0] = E;
-                        exponents[info][1] = min(max((int)topValue - 127 + 6, -120), 120);
+                    for (int side = 0; side < 2; ++side) {
+                        uint32_t most = 0;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int G = 0; G < NG; ++G) most = max(most, word_exponent(v[side][h][G]));
+                        most = __reduce_max_sync(0xFFFFFFFFu, most);
+                        const int E = min(max((int)most - 127 + 6, -120), 120);
+                        const float f = power_of_two(-E);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h)
+#pragma unroll
+                            for (int G = 0; G < NG; ++G)
+                                sts32(scales + info * words_bytes(DIM) + side * kWordSide + (G * kTileKeys + lane + 32 * h) * 4,
+                                      pack_f16(low16(v[side][h][G]) * f * 0x1p24f, high16(v[side][h][G]) * f));
+                        if (lane == 0) {
+                            exponents[info][side] = E;
+                            broken[info][side] = bad[side];
+                            hidden[info][side] = out[side];
+                        }
                     }
                     __syncwarp();
                     if (lane == 0) mbar_arrive(barInfo + 8 * info);
-                } else {
-                    if (!mbar_wait<Order::kLocal>(barInfo + 8 * info, n / kInfo & 1u, &abortFlag)) {
-                        ok = false;
-                        return;
-                    }
-                    word = lds32(words + ((info * NG + G) * kTileKeys + key) * 4);
-                    E = exponents[info][1];
                 }
-                if (!mbar_wait<Order::kLocal>(barTileFree + 8 * slot, slotPhase ^ 1u, &abortFlag)) {
+                x += w.count;
+                if (ok && x < end) next_segment(w, x);
+            }
+        } else if (warp >= (uint32_t)kFirstDequant) {
+            // ---------------- expansion: the groups of warps take slots K0, K1, V0, K2, V1, ... in turn ----------------
+            const uint32_t dw = warp - kFirstDequant, grp = dw / kGroupWarps, inGroup = dw % kGroupWarps;
+            uint32_t item = 0, tile = 0;  // slots filled by all groups; key tiles so far
+            bool ok = true;
+            auto fill = [&](uint32_t n, uint32_t side) {  // keys or values of the CTA's n-th tile
+                const uint32_t slot = item % kSlots, slotPhase = item / kSlots & 1u, pack = n % kPacked + side * kPacked, packPhase = n / kPacked & 1u, info = n % kInfo;
+                if (!wait_lane<false>(barInfo + 8 * info, n / kInfo & 1u, &abortFlag) ||
+                    !wait_lane<false>(barPack + 8 * pack, packPhase, &abortFlag)) {
                     ok = false;
                     return;
                 }
-                expand(src, slots + slot * kSlot, word, E);
+                uint32_t word[kUnitsEach];
+                uint4 v[kUnitsEach][2];
+#pragma unroll
+                for (uint32_t e = 0; e < kUnitsEach; ++e) {
+                    const uint32_t unit = e * (32 * kGroupWarps) + inGroup * 32 + lane, key = unit % kTileKeys, G = unit / kTileKeys;
+                    word[e] = lds32(scales + info * words_bytes(DIM) + side * kWordSide + unit * 4);
+#pragma unroll
+                    for (uint32_t h = 0; h < 2; ++h) v[e][h] = lds128(packed + pack * kPack + key * CB + ((G * 32 + 16 * h) ^ chunk_flip<DIM>(key)));
+                }
+                if (!wait_lane<false>(barTileFree + 8 * slot, slotPhase ^ 1u, &abortFlag)) {
+                    ok = false;
+                    return;
+                }
+#pragma unroll
+                for (uint32_t e = 0; e < kUnitsEach; ++e) {
+                    const uint32_t unit = e * (32 * kGroupWarps) + inGroup * 32 + lane, key = unit % kTileKeys, G = unit / kTileKeys;
+                    const uint32_t s0 = __byte_perm(word[e], word[e], 0x1010), bb = __byte_perm(word[e], word[e], 0x3232), s1 = mul_f16x2(s0, 0x2C002C00u);  // 2^-4
+                    const uint32_t to = slots + slot * kSlot + G * (kTileKeys * 128) + key * 128;
+#pragma unroll
+                    for (uint32_t h = 0; h < 2; ++h) {
+                        const uint32_t c[4] = {v[e][h].x, v[e][h].y, v[e][h].z, v[e][h].w};
+#pragma unroll
+                        for (uint32_t i = 0; i < 4; ++i) {
+                            const uint32_t upper = c[i] >> 8;
+                            sts128(to + (((4 * h + i) ^ (key & 7u)) << 4), fma_f16x2(c[i] & 0x000F000Fu, s0, bb), fma_f16x2(c[i] & 0x00F000F0u, s1, bb),
+                                   fma_f16x2(upper & 0x000F000Fu, s0, bb), fma_f16x2(upper & 0x00F000F0u, s1, bb));
+                        }
+                    }
+                }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) {
@@ -516,18 +543,24 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                     mbar_arrive(barTile + 8 * slot);
                 }
             };
+            Walk w = locate(begin);
             for (uint32_t x = begin; x < end && ok;) {
-                fill(w.t0, tile, true);
-                for (uint32_t i = 0; i < w.count && ok; ++i, ++tile) {
-                    if (i + 1 < w.count) fill(w.t0 + i + 1, tile + 1, true);
-                    if (ok) fill(w.t0 + i, tile, false);
+                // a segment of n tiles is 2 n slots: K0, then for every tile i the keys of i + 1 (all but the last) and the values of i
+                for (uint32_t k = 0; k < 2 * w.count && ok; ++k, ++item) {
+                    if (item % kGroups != grp) continue;
+                    const bool isKey = k == 0 || (k % 2 == 1 && k != 2 * w.count - 1);
+                    fill(tile + (isKey ? (k + 1) / 2 : (k == 2 * w.count - 1 ? w.count - 1 : k / 2 - 1)), isKey ? 0u : 1u);
                 }
+                tile += w.count;
                 x += w.count;
                 if (x < end) next_segment(w, x);
             }
-        } else {
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsRows));
+        if (begin < end) {
             // ---------------- rows ----------------
-            const uint32_t quarter = warp & 3u, row = quarter * 32 + lane;
+            const uint32_t wg = (warp - kFirstRowWarp) / 4, quarter = warp & 3u, row = quarter * 32 + lane;
             const uint32_t lanes = (quarter * 32) << 16;
             uint32_t tile = 0, joins = 0;
             bool ok = true;
@@ -537,7 +570,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                 const bool there = token < w.q.tokens;
                 const uint32_t head = w.head * group + row % group;
                 const int p = w.q.p0 + (int)token, pLast = w.q.p0 + (int)w.q.tokens - 1;
-                // queries: f16 at a power of two of the row's largest value; runs of eight in the order of the tiles' codes
+                // queries: f16 at a power of two of the row's largest value; runs of eight in the order of the tiles' codes;
+                // either warpgroup half of them
                 float toLog2;
                 {
                     const uint4 *src = reinterpret_cast<const uint4 *>(a.q + (size_t)(w.q.firstRow + (there ? token : 0u)) * a.qStride + head * DIM);
@@ -551,29 +585,30 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                     const float down = __uint_as_float((261u - exponent) << 23);  // the largest is 2^7 .. 2^8
                     toLog2 = a.scale * 1.4426950408889634f * power_of_two((int)exponent - 134);
 #pragma unroll 1
-                    for (uint32_t c = 0; c < DIM / 64; ++c) {
-                        uint32_t o[32];
+                    for (uint32_t c = wg; c < DIM / 32; c += kRowGroups) {
+                        uint32_t o[16];
 #pragma unroll
-                        for (uint32_t i = 0; i < 8; ++i) {
-                            const uint4 v = there ? __ldg(src + 8 * c + i) : make_uint4(0u, 0u, 0u, 0u);
+                        for (uint32_t i = 0; i < 4; ++i) {
+                            const uint4 v = there ? __ldg(src + 4 * c + i) : make_uint4(0u, 0u, 0u, 0u);
                             o[4 * i] = pack_f16(low16(v.x) * down, low16(v.z) * down);
                             o[4 * i + 1] = pack_f16(high16(v.x) * down, high16(v.z) * down);
                             o[4 * i + 2] = pack_f16(low16(v.y) * down, low16(v.w) * down);
                             o[4 * i + 3] = pack_f16(high16(v.y) * down, high16(v.w) * down);
                         }
-                        tc_store_32cols(tmem + lanes + kColQ + 32 * c, o);
+                        tc_store_16cols(tmem + lanes + kColQ + 16 * c, o);
                     }
                     tc_wait_st();
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(barQ);
                 }
-                float top = -INFINITY, sum = 0.0f;
-                for (uint32_t i = 0; i < w.count; ++i, ++tile) {
+                float ref = -INFINITY, sum = 0.0f;  // the warpgroup's part of the weights' sum, at 2^ref
+                uint32_t i = (tile ^ wg) & 1u;      // the segment's first tile of this warpgroup
+                for (tile += i; i < w.count; i += 2, tile += 2) {
                     const uint32_t info = tile % kInfo;
-                    if (!(ok = mbar_wait_warp<false, Order::kLocal>(barS + 8 * (tile & 1u), tile >> 1 & 1u, &abortFlag))) break;
+                    if (!(ok = wait_warp<false>(barS + 8 * wg, tile >> 1 & 1u, &abortFlag))) break;
                     tc_fence_after();
-                    const uint32_t s0 = tmem + lanes + kColS + (tile & 1u) * kTileKeys;
+                    const uint32_t s0 = tmem + lanes + kColS + wg * kTileKeys;
                     uint32_t lo[32], hi[32];
                     tc_load_32cols(s0, lo);
                     tc_load_32cols(s0 + 32, hi);
@@ -584,9 +619,9 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                     float *s = reinterpret_cast<float *>(lo), *u = reinterpret_cast<float *>(hi);
                     const float f = toLog2 * power_of_two(eK);
                     if (j0 + (int)kTileKeys - 1 > w.q.p0 || (a.window && (long long)j0 <= (long long)pLast - a.window && (uint32_t)j0 + kTileKeys > a.sinks) || (bad0 | bad1 | gone0 | gone1)) {
+                        // the keys c of the tile that this row sees: up to `most`, above `least` or below `sinks`
                         const int most = p - j0;
-                        const long long least = a.window ? (long long)p - a.window - j0 : -1;  // sees c > least
-                        const long long sinks = a.window ? (long long)a.sinks - j0 : 0;        // or c < sinks
+                        const int least = a.window ? (int)max((long long)p - a.window - j0, -1ll) : -1, sinks = a.window ? (int)min(max((long long)a.sinks - j0, 0ll), 64ll) : 0;
 #pragma unroll
                         for (int c = 0; c < 32; ++c) {
                             const bool see0 = c <= most && (c > least || c < sinks) && !(gone0 >> c & 1u), see1 = c + 32 <= most && (c + 32 > least || c + 32 < sinks) && !(gone1 >> c & 1u);
@@ -598,48 +633,72 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
 #pragma unroll
                     for (int c = 1; c < 32; ++c) most = fmaxf(most, fmaxf(s[c], u[c]));
                     most = fmaf(most, f, (float)eV);
+                    // the maximum that the tile before settled on
+                    float top = -INFINITY;
+                    if (i) {
+                        if (!(ok = wait_warp<false>(barTop + 8 * ((wg ^ 1u) * 4 + quarter), (tile - 1) >> 1 & 1u, &abortFlag))) break;
+                        top = topShared[row];
+                    }
                     if (__any_sync(0xFFFFFFFFu, most > top + kLazy)) {
                         const float next = fmaxf(top, most), down = top == -INFINITY ? 0.0f : exp2_fast(top - next);
                         top = next;
-                        sum *= down;
                         if (i) {  // O so far, once the products in flight are done
-                            if (!(ok = mbar_wait_warp<false, Order::kLocal>(barO + 8 * ((tile - 1) & 1u), (tile - 1) >> 1 & 1u, &abortFlag))) break;
+                            if (!(ok = wait_warp<false>(barO + 8 * (wg ^ 1u), (tile - 1) >> 1 & 1u, &abortFlag))) break;
                             tc_fence_after();
 #pragma unroll 1
-                            for (uint32_t c = 0; c < DIM; c += 32) {
-                                uint32_t o[32];
-                                tc_load_32cols(tmem + lanes + kColO + c, o);
+                            for (uint32_t c = 0; c < DIM; c += 16) {
+                                uint32_t o[16];
+                                tc_load_16cols(tmem + lanes + kColO + c, o);
                                 tc_wait_ld();
 #pragma unroll
-                                for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * down);
-                                tc_store_32cols(tmem + lanes + kColO + c, o);
+                                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * down);
+                                tc_store_16cols(tmem + lanes + kColO + c, o);
                             }
                             tc_wait_st();
                         }
                     }
+                    topShared[row] = top;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(barTop + 8 * (wg * 4 + quarter));
+                    if (ref != top) sum *= ref == -INFINITY ? 0.0f : exp2_fast(ref - top), ref = top;
                     const float shift = top == -INFINITY ? 0.0f : (float)eV - top;
                     float part = 0.0f;
-                    uint32_t o[32];
+                    auto weigh = [&](const float *v, uint32_t to) {  // 32 logits: weights to 16 columns
+                        uint32_t o[16];
 #pragma unroll
-                    for (int c = 0; c < 32; c += 2) {
-                        const float x0 = exp2_fast(fmaf(s[c], f, shift)), x1 = exp2_fast(fmaf(s[c + 1], f, shift));
-                        const float y0 = exp2_fast(fmaf(u[c], f, shift)), y1 = exp2_fast(fmaf(u[c + 1], f, shift));
-                        part += (x0 + x1) + (y0 + y1);
-                        o[c / 2] = pack_f16(x0, x1);
-                        o[16 + c / 2] = pack_f16(y0, y1);
-                    }
+                        for (int c = 0; c < 32; c += 2) {
+                            const float x0 = exp2_fast(fmaf(v[c], f, shift)), x1 = exp2_fast(fmaf(v[c + 1], f, shift));
+                            part += x0 + x1;
+                            o[c / 2] = pack_f16(x0, x1);
+                        }
+                        tc_store_16cols(to, o);
+                    };
+                    weigh(s, s0);
+                    weigh(u, s0 + 16);
                     sum = fmaf(part, power_of_two(-eV), sum);
-                    tc_store_32cols(s0, o);
                     tc_wait_st();
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(barP + 8 * (tile & 1u));
+                    if (lane == 0) mbar_arrive(barP + 8 * wg);
                 }
                 if (!ok) break;
+                tile = tile - i + w.count;
 
-                // ---- the unit's rows, or this CTA's part of them ----
-                if (!(ok = mbar_wait_warp<false, Order::kLocal>(barO + 8 * ((tile - 1) & 1u), (tile - 1) >> 1 & 1u, &abortFlag))) break;
+                // ---- the unit's rows, or this CTA's part of them: either warpgroup every second 32 values ----
+                auto meet = [&] {  // of both warpgroups
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(barJoin);
+                    ok = wait_warp<false>(barJoin, joins++ & 1u, &abortFlag);
+                    return ok;
+                };
+                sumShared[wg][row] = sum;
+                refShared[wg][row] = ref;
+                if (!meet() || !(ok = wait_warp<false>(barO + 8 * ((tile - 1) & 1u), (tile - 1) >> 1 & 1u, &abortFlag))) break;
                 tc_fence_after();
+                const float top = topShared[row];
+                sum = 0.0f;
+#pragma unroll
+                for (int k = 0; k < kRowGroups; ++k) sum += refShared[k][row] == -INFINITY ? sumShared[k][row] : sumShared[k][row] * exp2_fast(refShared[k][row] - top);
                 const bool whole = w.count == w.q.tiles;
                 const uint32_t part = 2 * cta + (w.t0 == 0 ? 1u : 0u);
                 uint16_t *out = a.out + (size_t)(w.q.firstRow + (there ? token : 0u)) * a.outStride + head * DIM;
@@ -651,7 +710,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                 };
                 const float factor = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll 1
-                for (uint32_t c = 0; c < DIM; c += 32) {
+                for (uint32_t c = 32 * wg; c < DIM; c += 32 * kRowGroups) {
                     uint32_t o[32];
                     tc_load_32cols(tmem + lanes + kColO + c, o);
                     tc_wait_ld();
@@ -663,18 +722,13 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                         for (int k = 0; k < 8; ++k) to[k] = make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]), __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
                     }
                 }
+                tc_fence_before();  // (the next unit's products overwrite O once both warpgroups have brought their queries)
                 if (!whole) {
-                    if (there) args.stats[part * kRows + row] = make_float2(top, sum);
+                    if (there && wg == 0) args.stats[part * kRows + row] = make_float2(top, sum);
                     const uint32_t c0 = cta_of(x - w.t0), c1 = cta_of(x - w.t0 + w.q.tiles - 1);
-                    auto meet = [&] {  // of the four warps
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(barJoin);
-                        ok = mbar_wait_warp<false, Order::kLocal>(barJoin, joins++ & 1u, &abortFlag);
-                        return ok;
-                    };
                     __threadfence();
                     if (!meet()) break;
-                    if (row == 0) {
+                    if (wg == 0 && row == 0) {
                         const uint32_t n = atomicAdd(args.arrived + c0, 1u);
                         lastPart = n == c1 - c0;
                         if (n == c1 - c0) args.arrived[c0] = 0u;
@@ -692,7 +746,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                         }
                         const float last = weights == 0.0f ? 0.0f : 1.0f / weights;
 #pragma unroll 1
-                        for (uint32_t d = 0; d < DIM; d += 32) {
+                        for (uint32_t d = 32 * wg; d < DIM; d += 32 * kRowGroups) {
                             float v[32];
 #pragma unroll
                             for (int k = 0; k < 32; ++k) v[k] = 0.0f;
@@ -709,8 +763,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                             write_32(d, v, last);
                         }
                     }
-                    if (!meet()) break;  // (before the next unit's word in `lastPart`)
                 }
+                if (!meet()) break;  // (before the next unit's words in shared memory)
                 x += w.count;
                 if (x < end) next_segment(w, x);
             }
@@ -722,27 +776,27 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
     __syncthreads();
     if (tid == 0 && abortFlag) *a.errorFlag = kFlagWait;
     tc_fence_after();
-    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    if (warp == (uint32_t)kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
 KernelSmemMemo tilesMemo[3];
 
 template <int DIM>
-bool launch_tiles(FFAttention *att, KernelSmemMemo &memo, const CUtensorMap &map, const TilesArgs &args, cudaStream_t stream, const char **error) {
+bool launch_tiles(FFAttention *att, KernelSmemMemo &memo, const CUtensorMap &codes, const CUtensorMap &words, const TilesArgs &args, cudaStream_t stream, const char **error) {
     if (!memo.prepare(k_attend_tiles<DIM>, att->device, tiles_smem(DIM), kTilesThreads, nullptr, error)) return false;
-    return launched(att, launch_pdl(k_attend_tiles<DIM>, dim3(att->smCount), dim3(kTilesThreads), tiles_smem(DIM), stream, map, args), "k_attend_tiles", error);
+    return launched(att, launch_pdl(k_attend_tiles<DIM>, dim3(att->smCount), dim3(kTilesThreads), tiles_smem(DIM), stream, codes, words, args), "k_attend_tiles", error);
 }
 
 }  // namespace
 
 bool launch_attend_tiles(FFAttention *att, const AttendArgs &a, cudaStream_t stream, const char **error) {
     const uint32_t dim = att->cfg.headDim;
-    TilesArgs args{a, att->partials, att->stats, att->arrived, (uint32_t)__builtin_ctz(att->cfg.pageTokens), kRows / (a.heads / a.kvHeads)};
-    CUtensorMap map;
-    if (!make_pages_map(&map, a, dim, error)) return false;
-    if (dim == 256) return launch_tiles<256>(att, tilesMemo[2], map, args, stream, error);
-    if (dim == 128) return launch_tiles<128>(att, tilesMemo[1], map, args, stream, error);
-    return launch_tiles<64>(att, tilesMemo[0], map, args, stream, error);
+    TilesArgs args{a, att->partials, att->stats, att->arrived, (uint32_t)__builtin_ctz(att->cfg.pageTokens), (uint32_t)__builtin_ctz(std::min(kTileKeys, a.page.pageTokens)), kRows / (a.heads / a.kvHeads)};
+    CUtensorMap codes, words;
+    if (!make_pages_maps(&codes, &words, a, dim, 1, error)) return false;
+    if (dim == 256) return launch_tiles<256>(att, tilesMemo[2], codes, words, args, stream, error);
+    if (dim == 128) return launch_tiles<128>(att, tilesMemo[1], codes, words, args, stream, error);
+    return launch_tiles<64>(att, tilesMemo[0], codes, words, args, stream, error);
 }
 
 }  // namespace ff

@@ -31,8 +31,21 @@ __device__ __forceinline__ uint4 lds128(uint32_t a) {
     asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
     return v;
 }
+__device__ __forceinline__ void sts32(uint32_t a, uint32_t x) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(a), "r"(x) : "memory"); }
 __device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
     asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
+}
+// the NG scale words of a key
+template <int NG>
+__device__ __forceinline__ void lds_words(uint32_t a, uint32_t (&w)[NG]) {
+    if (NG == 4) asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1 % NG]), "=r"(w[2 % NG]), "=r"(w[3 % NG]) : "r"(a));
+    else if (NG == 2) asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1 % NG]) : "r"(a));
+    else w[0] = lds32(a);
+}
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
 }
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
@@ -64,7 +77,8 @@ __device__ __forceinline__ uint32_t chunk_flip(uint32_t key) {
     return DIM == 256 ? (key & 7u) << 4 : DIM == 128 ? ((key >> 1) & 3u) << 4 : ((key >> 2) & 1u) << 4;
 }
 
-// Codes of the cache's pages as a tensor [blocks][keys, values][tokens][bytes]; a box is (part of) a tile on one page.
-bool make_pages_map(CUtensorMap *map, const AttendArgs &a, uint32_t dim, const char **error);
+// The cache's pages as tensors: codes [blocks][keys, values][tokens][bytes], a box the part of a tile that lies on one page, of
+// `sides` of the two; scale words [blocks][keys, values][words], a box both sides of such a part.
+bool make_pages_maps(CUtensorMap *codes, CUtensorMap *words, const AttendArgs &a, uint32_t dim, uint32_t sides, const char **error);
 
 }  // namespace ff
