@@ -39,7 +39,7 @@ class AttentionContext:
         self._handle = lib.ff_attention_create(device, ctypes.byref(self.config), ctypes.byref(err))
         if not self._handle:
             raise FieldfareError(err.value.decode() if err.value else "ff_attention_create failed")
-        self.device = torch.device("cuda", device)
+        self.device, self._ordinal = torch.device("cuda", device), device
         self.heads, self.kvHeads, self.headDim, self.pageTokens = heads, kvHeads, headDim, pageTokens
         self.maxRequests, self.maxTokens = maxRequests, maxTokens
         self.pageBytes = lib.ff_cache_page_bytes(ctypes.byref(self.config))
@@ -69,31 +69,43 @@ class AttentionContext:
 
     # -- arguments ---------------------------------------------------------------------------------
 
-    def _ints(self, t: torch.Tensor, what: str) -> int:
-        if t.dtype != torch.int32 or t.device != self.device or not t.is_contiguous():
-            raise ValueError(f"{what} must be a contiguous int32 tensor on {self.device}")
-        return t.data_ptr()
+    # (A step of small calls is bound by the host: `get_device` and `is` cost a fifth of comparing torch.device objects, one
+    # look at shape and strides a third of four.)
+
+    def _ints(self, **tensors: torch.Tensor):
+        """Refuses what is not a contiguous int32 tensor on the device."""
+        i32, ordinal = torch.int32, self._ordinal
+        for t in tensors.values():
+            if t.dtype is not i32 or t.get_device() != ordinal or not t.is_contiguous():
+                what = next(name for name, u in tensors.items() if u is t)
+                raise ValueError(f"{what} must be a contiguous int32 tensor on {self.device}")
 
     def _heads(self, t: torch.Tensor, heads: int, tokens: int, what: str) -> tuple:
         """(pointer, elements between rows) of bf16 [tokens][heads][headDim], the heads of a row side by side."""
-        if t.dtype != torch.bfloat16 or t.device != self.device:
+        dim = self.headDim
+        if t.dtype is not torch.bfloat16 or t.get_device() != self._ordinal:
             raise ValueError(f"{what} must be bf16 on {self.device}")
-        if tuple(t.shape) != (tokens, heads, self.headDim) or (tokens and (t.stride(2) != 1 or (heads > 1 and t.stride(1) != self.headDim))):
-            raise ValueError(f"{what} must be [{tokens}][{heads}][{self.headDim}] with the heads of a row side by side")
-        return t.data_ptr(), t.stride(0) if tokens > 1 else heads * self.headDim
+        if t.shape != (tokens, heads, dim):
+            raise ValueError(f"{what} must be [{tokens}][{heads}][{dim}]")
+        row, head, value = t.stride()
+        if tokens and (value != 1 or (head != dim and heads > 1)):
+            raise ValueError(f"{what} must have the heads of a row side by side")
+        return t.data_ptr(), row if tokens > 1 else heads * dim
 
     def _cache(self, pages: torch.Tensor) -> tuple:
-        if pages.dtype != torch.uint8 or pages.device != self.device or not pages.is_contiguous() or pages.dim() < 1 or (
-                pages.numel() != pages.shape[0] * self.pageBytes):
+        count = pages.shape[0] if pages.dim() else 0
+        if (pages.dtype is not torch.uint8 or pages.get_device() != self._ordinal or not pages.is_contiguous()
+                or pages.numel() != count * self.pageBytes):
             raise ValueError(f"a cache is contiguous uint8 [pages][kvHeads][...] with {self.pageBytes} bytes a page on {self.device}")
-        return pages.data_ptr(), pages.shape[0]
+        return pages.data_ptr(), count
 
     def _rope(self, table: Optional[torch.Tensor], interleaved: bool) -> FFRope:
         if table is None:
             return FFRope(None, 0, 0, int(interleaved))
-        if table.dtype != torch.float32 or table.device != self.device or not table.is_contiguous() or table.dim() != 3 or table.shape[2] != 2:
+        shape = table.shape
+        if table.dtype is not torch.float32 or table.get_device() != self._ordinal or not table.is_contiguous() or len(shape) != 3 or shape[2] != 2:
             raise ValueError(f"a rotary table is fp32 [positions][rotaryDim/2][2] on {self.device}")
-        return FFRope(table.data_ptr(), table.shape[0], 2 * table.shape[1], int(interleaved))
+        return FFRope(table.data_ptr(), shape[0], 2 * shape[1], int(interleaved))
 
     # -- the cache ---------------------------------------------------------------------------------
 
@@ -107,15 +119,17 @@ class AttentionContext:
         """Request r goes from oldLengths[r] to newLengths[r] tokens: pages given back and taken (blockTable [requests]
         [pages], the stack freePages with freeCount [1] entries; freeCountOut may be freeCount), and a row for every new
         token: rowStart [requests + 1], positions and slots [rows]."""
-        requests = oldLengths.numel()
-        if newLengths.numel() != requests or blockTable.dim() != 2 or blockTable.shape[0] != requests or rowStart.numel() != requests + 1:
+        requests, rows = oldLengths.numel(), slots.numel()
+        shape = blockTable.shape
+        if newLengths.numel() != requests or len(shape) != 2 or shape[0] != requests or rowStart.numel() != requests + 1:
             raise ValueError("lengths, blockTable and rowStart must agree on the number of requests")
-        if positions.numel() != slots.numel() or freeCount.numel() != 1 or freeCountOut.numel() != 1:
+        if positions.numel() != rows or freeCount.numel() != 1 or freeCountOut.numel() != 1:
             raise ValueError("one position and one slot per row; one word for the stack's height")
-        call("ff_cache_plan", self.handle, self._ints(oldLengths, "oldLengths"), self._ints(newLengths, "newLengths"), requests,
-             self._ints(blockTable, "blockTable"), blockTable.shape[1], self._ints(freePages, "freePages"), freePages.numel(),
-             self._ints(freeCount, "freeCount"), self._ints(freeCountOut, "freeCountOut"), self._ints(rowStart, "rowStart"),
-             self._ints(positions, "positions"), self._ints(slots, "slots"), slots.numel(), _stream(stream))
+        self._ints(oldLengths=oldLengths, newLengths=newLengths, blockTable=blockTable, freePages=freePages, freeCount=freeCount,
+                   freeCountOut=freeCountOut, rowStart=rowStart, positions=positions, slots=slots)
+        call("ff_cache_plan", self.handle, oldLengths.data_ptr(), newLengths.data_ptr(), requests, blockTable.data_ptr(), shape[1],
+             freePages.data_ptr(), freePages.numel(), freeCount.data_ptr(), freeCountOut.data_ptr(), rowStart.data_ptr(),
+             positions.data_ptr(), slots.data_ptr(), rows, _stream(stream))
 
     def ropeTable(self, positions: int, *, base: float = 10000.0, rotaryDim: Optional[int] = None, scaling: str = "none",
                   factor: float = 1.0, lowTurns: float = 1.0, highTurns: float = 4.0, originalContext: float = 8192.0,
@@ -138,7 +152,8 @@ class AttentionContext:
         if y is None:
             y = torch.empty((tokens, heads, self.headDim), dtype=torch.bfloat16, device=self.device)
         rope = self._rope(table, interleaved)
-        call("ff_rope", self.handle, *self._heads(x, heads, tokens, "x"), ctypes.byref(rope), self._ints(positions, "positions"), heads, tokens,
+        self._ints(positions=positions)
+        call("ff_rope", self.handle, *self._heads(x, heads, tokens, "x"), ctypes.byref(rope), positions.data_ptr(), heads, tokens,
              *self._heads(y, heads, tokens, "y"), _stream(stream))
         return y
 
@@ -156,8 +171,9 @@ class AttentionContext:
                 qOut = torch.empty((tokens, self.heads, self.headDim), dtype=torch.bfloat16, device=self.device)
             query, out = self._heads(q, self.heads, tokens, "q"), self._heads(qOut, self.heads, tokens, "qOut")
         rope = self._rope(table, interleaved)
+        self._ints(positions=positions, slots=slots)
         call("ff_cache_append", self.handle, *query, *self._heads(k, self.kvHeads, tokens, "k"), *self._heads(v, self.kvHeads, tokens, "v"),
-             ctypes.byref(rope), self._ints(positions, "positions"), self._ints(slots, "slots"), tokens, *out, *self._cache(pages),
+             ctypes.byref(rope), positions.data_ptr(), slots.data_ptr(), tokens, *out, *self._cache(pages),
              _stream(stream))
         return qOut
 
@@ -166,14 +182,16 @@ class AttentionContext:
         """(keys, values) that slots hold, bf16 [slots][kvHeads][headDim]; zeros for NO_SLOT."""
         tokens = slots.numel()
         shape = (tokens, self.kvHeads, self.headDim)
-        out = [torch.empty(shape, dtype=torch.bfloat16, device=self.device) if t is None else t for t in (k, v)]
-        for t in out:
-            if not t.is_contiguous():
-                raise ValueError("k and v must be contiguous")
-            self._heads(t, self.kvHeads, tokens, "k and v")
-        call("ff_cache_read", self.handle, *self._cache(pages), self._ints(slots, "slots"), tokens, out[0].data_ptr(), out[1].data_ptr(),
-             _stream(stream))
-        return tuple(out)
+        if k is None:
+            k = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
+        if v is None:
+            v = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
+        if not (k.is_contiguous() and v.is_contiguous()):
+            raise ValueError("k and v must be contiguous")
+        self._ints(slots=slots)
+        call("ff_cache_read", self.handle, *self._cache(pages), slots.data_ptr(), tokens, self._heads(k, self.kvHeads, tokens, "k")[0],
+             self._heads(v, self.kvHeads, tokens, "v")[0], _stream(stream))
+        return k, v
 
     # -- attention ---------------------------------------------------------------------------------
 
@@ -183,15 +201,15 @@ class AttentionContext:
         """Rows rowStart[r] .. rowStart[r + 1] - 1 of q over request r's `lengths[r]` cached keys, their own among them;
         maxRows: no request has more rows.  window 0: every key up to the row's own; otherwise the last `window` of them
         and the first `sinks`."""
-        tokens, requests = q.shape[0], lengths.numel()
-        if rowStart.numel() != requests + 1 or blockTable.dim() != 2 or blockTable.shape[0] != requests:
+        tokens, requests, shape = q.shape[0], lengths.numel(), blockTable.shape
+        if rowStart.numel() != requests + 1 or len(shape) != 2 or shape[0] != requests:
             raise ValueError("lengths, blockTable and rowStart must agree on the number of requests")
         if window < 0 or sinks < 0 or maxRows < 0:
             raise ValueError("window, sinks and maxRows must not be negative")
         if out is None:
             out = torch.empty((tokens, self.heads, self.headDim), dtype=torch.bfloat16, device=self.device)
-        call("ff_attention", self.handle, *self._heads(q, self.heads, tokens, "q"), tokens, *self._cache(pages),
-             self._ints(blockTable, "blockTable"), blockTable.shape[1], self._ints(rowStart, "rowStart"), self._ints(lengths, "lengths"),
-             requests, maxRows, self.headDim ** -0.5 if scale is None else scale, window, sinks,
+        self._ints(blockTable=blockTable, rowStart=rowStart, lengths=lengths)
+        call("ff_attention", self.handle, *self._heads(q, self.heads, tokens, "q"), tokens, *self._cache(pages), blockTable.data_ptr(), shape[1],
+             rowStart.data_ptr(), lengths.data_ptr(), requests, maxRows, self.headDim ** -0.5 if scale is None else scale, window, sinks,
              *self._heads(out, self.heads, tokens, "out"), _stream(stream))
         return out

@@ -7,12 +7,14 @@
 // Per key tile, warp by role: two copy packed codes, keys' with the scale words and values'; one turns the tile's scale words into the pairs that
 // the expansion multiplies with; eight expand codes to f16 tiles in shared memory (128-byte swizzle, keys and values alike
 // [64 values][key][128 bytes]), four a slot, so that one group's waits stand behind the other's arithmetic; one issues the MMAs; two
-// warpgroups own a row a thread and take the tiles in turn:
+// warpgroups own half of a row's keys a thread:
 //   S = Q K^T   A: the rows' queries, in tensor memory for the whole unit (read from shared memory they would cost the
 //               128 bytes a cycle that dequantizing needs); B: the keys, K-major
 //   P = 2^(S f + E - M)   in registers, back into S's columns as f16
 //   O += P V    A: P; B: the values, N-major; O stays in tensor memory
-// A tile's warpgroup waits for the maximum M that the one before it settled on, not for its weights.
+// The halves exchange their maxima while they form the weights with the M there is; M moves only where a row passes it by 2^8.
+// (A row a thread, with the tiles taken in turn by the two warpgroups: 2000 cycles from S to P, which two tiles of S cannot
+// hide; now 900.)
 // Tensor memory: Q dim/2, O dim, S two tiles of 64 columns: all 512 at dim 256.
 //
 // f16 holds 11 bits of keys, values and weights where bf16 would hold 8; its range is kept by powers of two: a row's
@@ -115,13 +117,14 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
     constexpr uint32_t kGroupWarps = DIM == 64 ? 2 : 4, kGroups = kDequantWarps / kGroupWarps, kUnitsEach = kUnits / (32 * kGroupWarps);
     constexpr uint32_t kColQ = 0, kColO = DIM / 2, kColS = kColO + DIM;
     extern __shared__ uint8_t tilesSmem[];
-    __shared__ __align__(8) uint64_t barriers[2 * kSlots + 4 * kPacked + 2 * kInfo + 2 + 2 + 2 + 1 + 1 + 8];
+    __shared__ __align__(8) uint64_t barriers[2 * kSlots + 4 * kPacked + 2 * kInfo + 2 + 2 + 2 + 1 + 1 + 4];
     __shared__ uint32_t tmemSlot, lastPart;
     __shared__ volatile uint32_t abortFlag;
     __shared__ uint32_t firstTile[kTilesThreads + 1], firstWork[kTilesThreads + 1], warpSums[32];
     __shared__ uint32_t holes[kPacked], broken[kInfo][2], hidden[kInfo][2];
     __shared__ int exponents[kInfo][2];
-    __shared__ float topShared[kRows], sumShared[kRowGroups][kRows], refShared[kRowGroups][kRows];
+    __shared__ float mostShared[2][kRowGroups][kRows], sumShared[kRowGroups][kRows];
+    __shared__ uint32_t aboveShared[2][kRowGroups][4];
     const AttendArgs &a = args.a;
     const uint32_t tid = threadIdx.x, warp = (uint32_t)warp_index(), lane = tid & 31u;
     const uint32_t slots = (sm_addr(tilesSmem) + 1023u) & ~1023u, packed = slots + kSlots * kSlot, scales = packed + 2 * kPacked * kPack, words = scales + kInfo * words_bytes(DIM);
@@ -146,12 +149,12 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
         }
         for (uint32_t s = 0; s < 2; ++s) {
             mbar_init(barS + 8 * s, 1);
-            mbar_init(barP + 8 * s, 4);
+            mbar_init(barP + 8 * s, kRowWarps);
             mbar_init(barO + 8 * s, 1);
         }
         mbar_init(barQ, kRowWarps);
         mbar_init(barJoin, kRowWarps);
-        for (uint32_t s = 0; s < 8; ++s) mbar_init(barTop + 8 * s, 1);
+        for (uint32_t s = 0; s < 4; ++s) mbar_init(barTop + 8 * s, kRowGroups);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == (uint32_t)kMmaWarp) {
@@ -602,87 +605,84 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                     __syncwarp();
                     if (lane == 0) mbar_arrive(barQ);
                 }
-                float ref = -INFINITY, sum = 0.0f;  // the warpgroup's part of the weights' sum, at 2^ref
-                uint32_t i = (tile ^ wg) & 1u;      // the segment's first tile of this warpgroup
-                for (tile += i; i < w.count; i += 2, tile += 2) {
-                    const uint32_t info = tile % kInfo;
-                    if (!(ok = wait_warp<false>(barS + 8 * wg, tile >> 1 & 1u, &abortFlag))) break;
+                float top = -INFINITY, sum = 0.0f;  // the row's maximum; the sum of this half's weights, at 2^top
+                for (uint32_t i = 0; i < w.count; ++i, ++tile) {
+                    const uint32_t info = tile % kInfo, turn = tile & 1u;
+                    if (!(ok = wait_warp<false>(barS + 8 * turn, tile >> 1 & 1u, &abortFlag))) break;
                     tc_fence_after();
-                    const uint32_t s0 = tmem + lanes + kColS + wg * kTileKeys;
-                    uint32_t lo[32], hi[32];
-                    tc_load_32cols(s0, lo);
-                    tc_load_32cols(s0 + 32, hi);
+                    const uint32_t s0 = tmem + lanes + kColS + turn * kTileKeys;
+                    uint32_t bits[32];
+                    tc_load_32cols(s0 + 32 * wg, bits);
                     const int eK = exponents[info][0], eV = exponents[info][1];
-                    const uint32_t bad0 = broken[info][0], bad1 = broken[info][1], gone0 = hidden[info][0], gone1 = hidden[info][1];
-                    const int j0 = (int)key_at(w.q, w.t0 + i);
+                    const uint32_t bad = broken[info][wg], gone = hidden[info][wg];
+                    const int tileKey = (int)key_at(w.q, w.t0 + i), j0 = tileKey + 32 * (int)wg;
                     tc_wait_ld();
-                    float *s = reinterpret_cast<float *>(lo), *u = reinterpret_cast<float *>(hi);
+                    float *s = reinterpret_cast<float *>(bits);
                     const float f = toLog2 * power_of_two(eK);
-                    if (j0 + (int)kTileKeys - 1 > w.q.p0 || (a.window && (long long)j0 <= (long long)pLast - a.window && (uint32_t)j0 + kTileKeys > a.sinks) || (bad0 | bad1 | gone0 | gone1)) {
-                        // the keys c of the tile that this row sees: up to `most`, above `least` or below `sinks`
+                    if (j0 + 31 > w.q.p0 || (a.window && (long long)j0 <= (long long)pLast - a.window && (uint32_t)j0 + 32u > a.sinks) || (bad | gone)) {
+                        // the keys c of this half that the row sees: up to `most`, above `least` or below `sinks`
                         const int most = p - j0;
-                        const int least = a.window ? (int)max((long long)p - a.window - j0, -1ll) : -1, sinks = a.window ? (int)min(max((long long)a.sinks - j0, 0ll), 64ll) : 0;
+                        const int least = a.window ? (int)max((long long)p - a.window - j0, -1ll) : -1, sinks = a.window ? (int)min(max((long long)a.sinks - j0, 0ll), 32ll) : 0;
 #pragma unroll
                         for (int c = 0; c < 32; ++c) {
-                            const bool see0 = c <= most && (c > least || c < sinks) && !(gone0 >> c & 1u), see1 = c + 32 <= most && (c + 32 > least || c + 32 < sinks) && !(gone1 >> c & 1u);
-                            s[c] = !see0 ? -INFINITY : bad0 >> c & 1u ? NAN : s[c];
-                            u[c] = !see1 ? -INFINITY : bad1 >> c & 1u ? NAN : u[c];
+                            const bool sees = c <= most && (c > least || c < sinks) && !(gone >> c & 1u);
+                            s[c] = !sees ? -INFINITY : bad >> c & 1u ? NAN : s[c];
                         }
                     }
-                    float most = fmaxf(s[0], u[0]);
+                    float most = s[0], most2 = s[1];
 #pragma unroll
-                    for (int c = 1; c < 32; ++c) most = fmaxf(most, fmaxf(s[c], u[c]));
-                    most = fmaf(most, f, (float)eV);
-                    // the maximum that the tile before settled on
-                    float top = -INFINITY;
-                    if (i) {
-                        if (!(ok = wait_warp<false>(barTop + 8 * ((wg ^ 1u) * 4 + quarter), (tile - 1) >> 1 & 1u, &abortFlag))) break;
-                        top = topShared[row];
-                    }
-                    if (__any_sync(0xFFFFFFFFu, most > top + kLazy)) {
-                        const float next = fmaxf(top, most), down = top == -INFINITY ? 0.0f : exp2_fast(top - next);
-                        top = next;
-                        if (i) {  // O so far, once the products in flight are done
-                            if (!(ok = wait_warp<false>(barO + 8 * (wg ^ 1u), (tile - 1) >> 1 & 1u, &abortFlag))) break;
-                            tc_fence_after();
-#pragma unroll 1
-                            for (uint32_t c = 0; c < DIM; c += 16) {
-                                uint32_t o[16];
-                                tc_load_16cols(tmem + lanes + kColO + c, o);
-                                tc_wait_ld();
-#pragma unroll
-                                for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * down);
-                                tc_store_16cols(tmem + lanes + kColO + c, o);
-                            }
-                            tc_wait_st();
-                        }
-                    }
-                    topShared[row] = top;
+                    for (int c = 2; c < 32; c += 2) most = fmaxf(most, s[c]), most2 = fmaxf(most2, s[c + 1]);
+                    most = fmaf(fmaxf(most, most2), f, (float)eV);
+                    // Either half's maximum; the weights are formed meanwhile, and once more where a row of either half passes
+                    // its maximum by more than kLazy.
+                    const bool above = __any_sync(0xFFFFFFFFu, most > top + kLazy);
+                    mostShared[turn][wg][row] = most;
+                    if (lane == 0) aboveShared[turn][wg][quarter] = above;
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(barTop + 8 * (wg * 4 + quarter));
-                    if (ref != top) sum *= ref == -INFINITY ? 0.0f : exp2_fast(ref - top), ref = top;
-                    const float shift = top == -INFINITY ? 0.0f : (float)eV - top;
-                    float part = 0.0f;
-                    auto weigh = [&](const float *v, uint32_t to) {  // 32 logits: weights to 16 columns
-                        uint32_t o[16];
+                    if (lane == 0) mbar_arrive(barTop + 8 * quarter);
+                    float part;
+                    uint32_t o[16];
+                    auto weigh = [&] {
+                        const float shift = top == -INFINITY ? 0.0f : (float)eV - top;
+                        float part2 = 0.0f;
+                        part = 0.0f;
 #pragma unroll
                         for (int c = 0; c < 32; c += 2) {
-                            const float x0 = exp2_fast(fmaf(v[c], f, shift)), x1 = exp2_fast(fmaf(v[c + 1], f, shift));
-                            part += x0 + x1;
+                            const float x0 = exp2_fast(fmaf(s[c], f, shift)), x1 = exp2_fast(fmaf(s[c + 1], f, shift));
+                            part += x0, part2 += x1;
                             o[c / 2] = pack_f16(x0, x1);
                         }
-                        tc_store_16cols(to, o);
+                        part += part2;
                     };
-                    weigh(s, s0);
-                    weigh(u, s0 + 16);
+                    if (!above) weigh();
+                    if (!(ok = wait_warp<false>(barTop + 8 * quarter, tile & 1u, &abortFlag))) break;
+                    if (above || aboveShared[turn][wg ^ 1u][quarter]) {
+                        const float next = fmaxf(top, fmaxf(most, mostShared[turn][wg ^ 1u][row])), down = top == -INFINITY ? 0.0f : exp2_fast(top - next);
+                        top = next;
+                        sum *= down;
+                        if (i) {  // half of O so far, once the products in flight are done
+                            if (!(ok = wait_warp<false>(barO + 8 * (turn ^ 1u), (tile - 1) >> 1 & 1u, &abortFlag))) break;
+                            tc_fence_after();
+#pragma unroll 1
+                            for (uint32_t c = 16 * wg; c < DIM; c += 32) {
+                                uint32_t v[16];
+                                tc_load_16cols(tmem + lanes + kColO + c, v);
+                                tc_wait_ld();
+#pragma unroll
+                                for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * down);
+                                tc_store_16cols(tmem + lanes + kColO + c, v);
+                            }
+                        }
+                        weigh();
+                    }
+                    tc_store_16cols(s0 + 16 * wg, o);
                     sum = fmaf(part, power_of_two(-eV), sum);
                     tc_wait_st();
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(barP + 8 * wg);
+                    if (lane == 0) mbar_arrive(barP + 8 * turn);
                 }
                 if (!ok) break;
-                tile = tile - i + w.count;
 
                 // ---- the unit's rows, or this CTA's part of them: either warpgroup every second 32 values ----
                 auto meet = [&] {  // of both warpgroups
@@ -692,13 +692,9 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                     return ok;
                 };
                 sumShared[wg][row] = sum;
-                refShared[wg][row] = ref;
                 if (!meet() || !(ok = wait_warp<false>(barO + 8 * ((tile - 1) & 1u), (tile - 1) >> 1 & 1u, &abortFlag))) break;
                 tc_fence_after();
-                const float top = topShared[row];
-                sum = 0.0f;
-#pragma unroll
-                for (int k = 0; k < kRowGroups; ++k) sum += refShared[k][row] == -INFINITY ? sumShared[k][row] : sumShared[k][row] * exp2_fast(refShared[k][row] - top);
+                sum = sumShared[0][row] + sumShared[1][row];
                 const bool whole = w.count == w.q.tiles;
                 const uint32_t part = 2 * cta + (w.t0 == 0 ? 1u : 0u);
                 uint16_t *out = a.out + (size_t)(w.q.firstRow + (there ? token : 0u)) * a.outStride + head * DIM;

@@ -242,134 +242,157 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     return r;
 }
 
-// A warp takes 256 values at a time: 256 / DIM heads of one row, eight values a lane.  Its cosines and sines stay in
-// registers for all the heads it takes.  Bound by the bytes of the rows.
-template <int DIM, bool INTERLEAVED>
-__global__ void __launch_bounds__(128) k_rope_rows(const RopeArgs a) {
+// the lesser, the greater of two pairs of bf16; NaN if either is
+__device__ __forceinline__ uint32_t min_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
+// A warp takes 256 values at a time, 256 / DIM heads of one row, eight values a lane, BATCH such steps' loads in flight.  Its
+// cosines and sines stay in registers for all the heads it takes.  Bound by the bytes of the rows.
+template <int DIM, bool INTERLEAVED, int BATCH>
+__global__ void __launch_bounds__(128, 8) k_rope_rows(const RopeArgs a) {
     constexpr uint32_t kLanes = DIM / 8, kHeads = 32 / kLanes;
     const uint32_t lane = threadIdx.x & 31u, inHead = lane % kLanes, headInWarp = lane / kLanes;
     const uint32_t unit = blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5);
-    const uint32_t token = unit / a.unitsPerToken, part = unit % a.unitsPerToken;
+    const uint32_t token = unit / a.unitsPerToken, part = unit - token * a.unitsPerToken;
     pdl_enter();
     if (token >= a.tokens) return;
-    const uint32_t qHeads = a.rows.q ? a.rows.qHeads : 0u, kHeadsTotal = a.rows.k ? a.kvHeads : 0u;
-    const uint32_t allHeads = qHeads + 2u * kHeadsTotal;
-    const uint32_t slot = a.slots ? __ldg(a.slots + token) : 0u;
+    const uint32_t qHeads = a.rows.q ? a.rows.qHeads : 0u, kEnd = qHeads + (a.rows.k ? a.kvHeads : 0u), allHeads = 2u * kEnd - qHeads;
+    const uint32_t firstHead = part * a.headsPerUnit, endHead = min(firstHead + a.headsPerUnit, allHeads);
 
+    // where head h of the row lies: queries, keys, values
+    auto source = [&](uint32_t h) {
+        const uint16_t *src = h < qHeads ? a.rows.q + (size_t)token * a.rows.qStride + h * DIM
+                              : h < kEnd ? a.rows.k + (size_t)token * a.rows.kStride + (h - qHeads) * DIM
+                                         : a.rows.v + (size_t)token * a.rows.vStride + (h - kEnd) * DIM;
+        return *reinterpret_cast<const uint4 *>(src + inHead * 8u);  // (qOut may be q: no read-only load)
+    };
+    uint4 loaded[BATCH];
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) {
+        const uint32_t h = firstHead + b * kHeads + headInWarp;
+        loaded[b] = h < endHead ? source(h) : make_uint4(0u, 0u, 0u, 0u);
+    }
+    const uint32_t slot = a.slots ? __ldg(a.slots + token) : 0u;
     float c[8], s[8];
-    const bool turns = inHead * 8u < a.rotaryDim;
+    const uint32_t half = a.rotaryDim / 2;
+    const bool turns = inHead * 8u < a.rotaryDim, second = !INTERLEAVED && inHead * 8u >= half;
     if (turns) {
         uint32_t position = __ldg(a.positions + token);
         if (position >= a.tablePositions) {
             if (lane == 0) *a.errorFlag = kFlagPosition;
             position = 0;
         }
-        const uint32_t half = a.rotaryDim / 2;
-        const float4 *row = reinterpret_cast<const float4 *>(a.table + (size_t)position * a.rotaryDim);
-        if (INTERLEAVED) {
+        const float4 *row = reinterpret_cast<const float4 *>(a.table + (size_t)position * a.rotaryDim) + (INTERLEAVED ? inHead * 2 : (inHead * 8u - (second ? half : 0u)) / 2);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const float4 v = __ldg(row + inHead * 2 + i);
-                c[2 * i] = v.x, s[2 * i] = v.y, c[2 * i + 1] = v.z, s[2 * i + 1] = v.w;
-            }
-        } else {
-            const uint32_t first = inHead * 8u % half;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float4 v = __ldg(row + first / 2 + i);
-                c[2 * i] = v.x, s[2 * i] = v.y, c[2 * i + 1] = v.z, s[2 * i + 1] = v.w;
-            }
+        for (int i = 0; i < (INTERLEAVED ? 2 : 4); ++i) {
+            const float4 v = __ldg(row + i);
+            c[2 * i] = v.x, s[2 * i] = v.y, c[2 * i + 1] = v.z, s[2 * i + 1] = v.w;
         }
+        if (!INTERLEAVED && !second)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s[i] = -s[i];  // a c - b s for the first of a pair, b c + a s for the second
     }
-    const uint32_t firstHead = part * a.headsPerUnit, endHead = min(firstHead + a.headsPerUnit, allHeads);
-    for (uint32_t h0 = firstHead; h0 < endHead; h0 += kHeads) {
-        const uint32_t h = h0 + headInWarp;
-        const bool live = h < endHead;
-        const bool isQ = h < qHeads, isK = !isQ && h < qHeads + kHeadsTotal;
-        const uint32_t head = isQ ? h : isK ? h - qHeads : h - qHeads - kHeadsTotal;
-        uint32_t x[4] = {0u, 0u, 0u, 0u};
-        if (live) {
-            const uint16_t *src = isQ ? a.rows.q + (size_t)token * a.rows.qStride
-                                      : isK ? a.rows.k + (size_t)token * a.rows.kStride : a.rows.v + (size_t)token * a.rows.vStride;
-            const uint4 v = *reinterpret_cast<const uint4 *>(src + head * DIM + inHead * 8u);  // (qOut may be q)
-            x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+    const uint32_t inPage = slot & (a.page.pageTokens - 1u);
+    uint8_t *page = a.pages + (uint64_t)(slot >> a.pageShift) * a.page.pageBytes;
+    const bool placed = slot < a.slotCount;
+    if (!placed && slot != FF_NO_SLOT && endHead > qHeads && lane == 0) *a.errorFlag = kFlagPage;
+
+    for (uint32_t h0 = firstHead; h0 < endHead; h0 += BATCH * kHeads) {
+        uint4 now[BATCH];
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b) {
+            now[b] = loaded[b];
+            const uint32_t h = h0 + (BATCH + b) * kHeads + headInWarp;
+            if (h < endHead) loaded[b] = source(h);
         }
-        const bool rotates = turns && (isQ || isK);
-        if (INTERLEAVED) {
-            if (rotates) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float p = bf16_low(x[i]), q = bf16_high(x[i]);
-                    x[i] = pack_bf16(__fsub_rn(__fmul_rn(p, c[i]), __fmul_rn(q, s[i])), __fadd_rn(__fmul_rn(p, s[i]), __fmul_rn(q, c[i])));
-                }
-            }
-        } else {
-            // the partner's values lie rotaryDim / 16 lanes away
-            const uint32_t half = a.rotaryDim / 2, away = half / 8u;
-            const bool second = inHead * 8u >= half;
-            const uint32_t from = turns ? (second ? lane - away : lane + away) : lane;
-            uint32_t y[4];
+        for (int b = 0; b < BATCH; ++b) {
+            const uint32_t h = h0 + b * kHeads + headInWarp;
+            if (h0 + b * kHeads >= endHead) break;
+            const bool live = h < endHead, isQ = h < qHeads, isK = !isQ && h < kEnd;
+            uint32_t x[4] = {now[b].x, now[b].y, now[b].z, now[b].w};
+            const bool rotates = turns && (isQ || isK);
+            if (INTERLEAVED) {
+                if (rotates) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) y[i] = __shfl_sync(0xFFFFFFFFu, x[i], from);
-            if (rotates) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float o[2];
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const float own = j ? bf16_high(x[i]) : bf16_low(x[i]), other = j ? bf16_high(y[i]) : bf16_low(y[i]);
-                        const float cs = __fmul_rn(own, c[2 * i + j]), sn = __fmul_rn(other, s[2 * i + j]);
-                        o[j] = second ? __fadd_rn(sn, cs) : __fsub_rn(cs, sn);
+                    for (int i = 0; i < 4; ++i) {
+                        const float p = bf16_low(x[i]), q = bf16_high(x[i]);
+                        x[i] = pack_bf16(__fsub_rn(__fmul_rn(p, c[i]), __fmul_rn(q, s[i])), __fadd_rn(__fmul_rn(p, s[i]), __fmul_rn(q, c[i])));
                     }
-                    x[i] = pack_bf16(o[0], o[1]);
+                }
+            } else if (__any_sync(0xFFFFFFFFu, rotates)) {
+                // the partner's values lie rotaryDim / 16 lanes away
+                const uint32_t away = half / 8u, from = turns ? (second ? lane - away : lane + away) : lane;
+                uint32_t y[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[i] = __shfl_sync(0xFFFFFFFFu, x[i], from);
+                if (rotates) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        float o[2];
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            const float own = j ? bf16_high(x[i]) : bf16_low(x[i]), other = j ? bf16_high(y[i]) : bf16_low(y[i]);
+                            o[j] = __fadd_rn(__fmul_rn(own, c[2 * i + j]), __fmul_rn(other, s[2 * i + j]));
+                        }
+                        x[i] = pack_bf16(o[0], o[1]);
+                    }
                 }
             }
-        }
-        if (live && isQ)
-            *reinterpret_cast<uint4 *>(a.rows.qOut + (size_t)token * a.rows.qOutStride + head * DIM + inHead * 8u) = make_uint4(x[0], x[1], x[2], x[3]);
-        // keys and values: quantized, eight lanes a group
-        if (__any_sync(0xFFFFFFFFu, live && !isQ)) {
-            float f[8];
+            if (live && isQ)
+                *reinterpret_cast<uint4 *>(a.rows.qOut + (size_t)token * a.rows.qOutStride + h * DIM + inHead * 8u) = make_uint4(x[0], x[1], x[2], x[3]);
+            // keys and values: quantized, eight lanes a group
+            if (__any_sync(0xFFFFFFFFu, live && !isQ)) {
+                uint32_t least = min_bf16x2(min_bf16x2(x[0], x[1]), min_bf16x2(x[2], x[3])), most = max_bf16x2(max_bf16x2(x[0], x[1]), max_bf16x2(x[2], x[3]));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) f[2 * i] = bf16_low(x[i]), f[2 * i + 1] = bf16_high(x[i]);
-            float low = f[0], high = f[0];
-            bool finite = true;
+                for (int d = 1; d < 8; d <<= 1) {
+                    least = min_bf16x2(least, __shfl_xor_sync(0xFFFFFFFFu, least, d));
+                    most = max_bf16x2(most, __shfl_xor_sync(0xFFFFFFFFu, most, d));
+                }
+                const uint32_t both = min_bf16x2(least, least >> 16), top = max_bf16x2(most, most >> 16);  // (their low halves)
+                const float low = bf16_low(both), high = bf16_low(top);
+                const uint32_t scaleBits = pack_bf16(__fdiv_rn(__fsub_rn(high, low), 15.0f), low);  // scale | bias
+                const float scale = bf16_low(scaleBits);
+                // a value that is no number is the minimum or the maximum, or makes both NaN, and the range with them
+                const bool finite = scale < INFINITY;
+                const float inverse = scale > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f;
+                float code[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                low = fminf(low, f[i]);
-                high = fmaxf(high, f[i]);
-                finite &= fabsf(f[i]) < INFINITY;
-            }
+                for (int i = 0; i < 8; ++i) code[i] = __fmul_rn(__fsub_rn(i % 2 ? bf16_high(x[i / 2]) : bf16_low(x[i / 2]), low), inverse);
+                // The scale is within 2^-9 of a fifteenth of the range, so no code reaches 15.5, but for scales without all their
+                // bits or with a reciprocal that overflows (0 * inf stays below code 0, the rest is code 15).
+                if (__any_sync(0xFFFFFFFFu, scale < 0x1p-118f))
 #pragma unroll
-            for (int d = 1; d < 8; d <<= 1) {
-                low = fminf(low, __shfl_xor_sync(0xFFFFFFFFu, low, d));
-                high = fmaxf(high, __shfl_xor_sync(0xFFFFFFFFu, high, d));
-                finite &= __shfl_xor_sync(0xFFFFFFFFu, (int)finite, d) != 0;
-            }
-            const uint32_t scaleBits = pack_bf16(__fdiv_rn(__fsub_rn(high, low), 15.0f), low);  // scale | bias
-            const float scale = bf16_low(scaleBits);
-            finite &= scale < INFINITY;
-            const float inverse = scale > 0.0f ? __fdiv_rn(1.0f, scale) : 0.0f;
-            uint32_t word = 0;
+                    for (int i = 0; i < 8; ++i) code[i] = fminf(fmaxf(code[i], 0.0f), 15.0f);
+                // rounded to whole numbers by adding 1.5 * 2^23, whose bits add up to a constant
+                uint32_t word = 0u;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                // (a scale so small that its reciprocal overflows: 0 * inf stays below code 0, the rest is code 15)
-                const float code = fminf(fmaxf(rintf(__fmul_rn(__fsub_rn(f[i], low), inverse)), 0.0f), 15.0f);
-                word |= (finite ? (uint32_t)code : 0u) << (4 * i);
-            }
-            if (live && !isQ && slot != FF_NO_SLOT) {
-                if (slot < a.slotCount) {
-                    const uint32_t inPage = slot & (a.page.pageTokens - 1u);
-                    uint8_t *block = a.pages + (uint64_t)(slot >> a.pageShift) * a.page.pageBytes + (uint64_t)head * a.page.blockBytes + (isK ? 0u : a.page.values);
-                    *reinterpret_cast<uint32_t *>(block + inPage * a.page.codeBytes + inHead * 4u) = word;
+                for (int i = 7; i >= 0; --i) word = word * 16u + __float_as_uint(__fadd_rn(code[i], 12582912.0f));
+                word -= 0x4B400000u * 0x11111111u;
+                if (live && !isQ && placed) {
+                    uint8_t *block = page + (uint64_t)(isK ? h - qHeads : h - kEnd) * a.page.blockBytes + (isK ? 0u : a.page.values);
+                    *reinterpret_cast<uint32_t *>(block + inPage * a.page.codeBytes + inHead * 4u) = finite ? word : 0u;
                     if ((inHead & 7u) == 0u)
                         *reinterpret_cast<uint32_t *>(block + a.page.keyWords + inPage * a.page.wordBytes + (inHead >> 3) * 4u) = finite ? scaleBits : 0x7FC07FC0u;
-                } else if (inHead == 0u) {
-                    *a.errorFlag = kFlagPage;
                 }
             }
         }
     }
+}
+
+template <int DIM>
+static cudaError_t start_rope(const RopeArgs &a, bool interleaved, bool many, dim3 grid, cudaStream_t stream) {
+    const dim3 block(128);
+    if (many) return interleaved ? launch_pdl(k_rope_rows<DIM, true, 2>, grid, block, 0, stream, a) : launch_pdl(k_rope_rows<DIM, false, 2>, grid, block, 0, stream, a);
+    return interleaved ? launch_pdl(k_rope_rows<DIM, true, 1>, grid, block, 0, stream, a) : launch_pdl(k_rope_rows<DIM, false, 1>, grid, block, 0, stream, a);
 }
 
 bool launch_rope_rows(FFAttention *att, const RopeRows &rows, const FFRope &rope, const uint32_t *positions, const uint32_t *slots,
@@ -392,15 +415,15 @@ bool launch_rope_rows(FFAttention *att, const RopeRows &rows, const FFRope &rope
     a.errorFlag = att->errorFlag;
     const uint32_t perWarp = 256u / cfg.headDim;
     const uint32_t heads = (rows.q ? rows.qHeads : 0u) + (rows.k ? 2u * cfg.kvHeads : 0u);
-    a.headsPerUnit = perWarp;
+    // Steps of a warp: as many as leave every SM 32 warps, up to eight.
+    uint32_t steps = 1;
+    while (steps < 8 && (uint64_t)tokens * ((heads + 2 * steps * perWarp - 1) / (2 * steps * perWarp)) >= (uint64_t)att->smCount * 32) steps *= 2;
+    a.headsPerUnit = steps * perWarp;
     a.unitsPerToken = (heads + a.headsPerUnit - 1) / a.headsPerUnit;
-    const uint64_t units = (uint64_t)tokens * a.unitsPerToken;
-    const dim3 grid((uint32_t)((units + 3) / 4)), block(128);
+    const dim3 grid((uint32_t)(((uint64_t)tokens * a.unitsPerToken + 3) / 4));
     const bool interleaved = rope.layout == FF_ROPE_INTERLEAVED;
-    cudaError_t st;
-    if (cfg.headDim == 64) st = interleaved ? launch_pdl(k_rope_rows<64, true>, grid, block, 0, stream, a) : launch_pdl(k_rope_rows<64, false>, grid, block, 0, stream, a);
-    else if (cfg.headDim == 128) st = interleaved ? launch_pdl(k_rope_rows<128, true>, grid, block, 0, stream, a) : launch_pdl(k_rope_rows<128, false>, grid, block, 0, stream, a);
-    else st = interleaved ? launch_pdl(k_rope_rows<256, true>, grid, block, 0, stream, a) : launch_pdl(k_rope_rows<256, false>, grid, block, 0, stream, a);
+    const cudaError_t st = cfg.headDim == 64 ? start_rope<64>(a, interleaved, steps > 1, grid, stream)
+                           : cfg.headDim == 128 ? start_rope<128>(a, interleaved, steps > 1, grid, stream) : start_rope<256>(a, interleaved, steps > 1, grid, stream);
     return launched(att, st, "k_rope_rows", error);
 }
 
@@ -410,39 +433,46 @@ struct ReadArgs {
     const uint8_t *pages;
     const uint32_t *slots;
     uint16_t *k, *v;
-    uint32_t tokens, kvHeads, slotCount, pageShift, dim;
+    uint32_t tokens, kvHeads, slotCount, pageShift, unitsPerToken;
     PageLayout page;
     uint32_t *errorFlag;
 };
 
-// Eight values a thread.  Bound by the bytes written.
-__global__ void __launch_bounds__(256) k_cache_read(const ReadArgs a) {
+// A warp takes 256 values at a time of one row, eight a lane, four such steps.  Bound by the bytes written.
+template <int DIM>
+__global__ void __launch_bounds__(128) k_cache_read(const ReadArgs a) {
+    constexpr uint32_t kLanes = DIM / 8, kHeads = 32 / kLanes, kSteps = 4;
+    const uint32_t lane = threadIdx.x & 31u, inHead = lane % kLanes, headInWarp = lane / kLanes;
+    const uint32_t unit = blockIdx.x * (blockDim.x / 32) + (threadIdx.x >> 5);
+    const uint32_t token = unit / a.unitsPerToken, part = unit - token * a.unitsPerToken;
     pdl_enter();
-    const uint32_t perHead = a.dim / 8, perRow = a.kvHeads * perHead, kinds = (a.k ? 1u : 0u) + (a.v ? 1u : 0u);
-    const uint64_t total = (uint64_t)a.tokens * perRow * kinds;
-    for (uint64_t i = (uint64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (uint64_t)gridDim.x * blockDim.x) {
-        const uint32_t inRow = (uint32_t)(i % perRow);
-        const uint64_t rest = i / perRow;
-        const uint32_t token = (uint32_t)(rest / kinds);
-        const bool key = a.k && rest % kinds == 0;
-        const uint32_t head = inRow / perHead, at = inRow % perHead;
-        const uint32_t slot = __ldg(a.slots + token);
-        uint4 o = make_uint4(0u, 0u, 0u, 0u);
-        if (slot < a.slotCount) {
-            const uint32_t inPage = slot & (a.page.pageTokens - 1u);
-            const uint8_t *block = a.pages + (uint64_t)(slot >> a.pageShift) * a.page.pageBytes + (uint64_t)head * a.page.blockBytes + (key ? 0u : a.page.values);
-            const uint32_t w = *reinterpret_cast<const uint32_t *>(block + inPage * a.page.codeBytes + at * 4u);
-            const uint32_t sb = *reinterpret_cast<const uint32_t *>(block + a.page.keyWords + inPage * a.page.wordBytes + (at >> 3) * 4u);
-            const float scale = bf16_low(sb), bias = bf16_high(sb);
-            float f[8];
+    if (token >= a.tokens) return;
+    const uint32_t keys = a.k ? a.kvHeads : 0u, all = keys + (a.v ? a.kvHeads : 0u);
+    const uint32_t slot = __ldg(a.slots + token), inPage = slot & (a.page.pageTokens - 1u);
+    const uint8_t *page = a.pages + (uint64_t)(slot >> a.pageShift) * a.page.pageBytes;
+    const bool placed = slot < a.slotCount;
+    if (!placed && slot != FF_NO_SLOT && lane == 0) *a.errorFlag = kFlagPage;
+    uint32_t w[kSteps], sb[kSteps];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) f[j] = __fadd_rn(__fmul_rn((float)((w >> (4 * j)) & 15u), scale), bias);
-            o = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
-        } else if (slot != FF_NO_SLOT) {
-            *a.errorFlag = kFlagPage;
+    for (uint32_t i = 0; i < kSteps; ++i) {
+        const uint32_t h = (part * kSteps + i) * kHeads + headInWarp;
+        w[i] = sb[i] = 0u;
+        if (h < all && placed) {
+            const uint8_t *block = page + (uint64_t)(h < keys ? h : h - keys) * a.page.blockBytes + (h < keys ? 0u : a.page.values);
+            w[i] = *reinterpret_cast<const uint32_t *>(block + inPage * a.page.codeBytes + inHead * 4u);
+            sb[i] = *reinterpret_cast<const uint32_t *>(block + a.page.keyWords + inPage * a.page.wordBytes + (inHead >> 3) * 4u);
         }
-        uint16_t *out = key ? a.k : a.v;
-        *reinterpret_cast<uint4 *>(out + ((uint64_t)token * perRow + inRow) * 8u) = o;
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kSteps; ++i) {
+        const uint32_t h = (part * kSteps + i) * kHeads + headInWarp;
+        if (h >= all) break;
+        const float scale = bf16_low(sb[i]), bias = bf16_high(sb[i]);
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = __fadd_rn(__fmul_rn((float)((w[i] >> (4 * j)) & 15u), scale), bias);
+        uint16_t *out = (h < keys ? a.k : a.v) + ((uint64_t)token * a.kvHeads + (h < keys ? h : h - keys)) * DIM;
+        *reinterpret_cast<uint4 *>(out + inHead * 8u) = make_uint4(pack_bf16(f[0], f[1]), pack_bf16(f[2], f[3]), pack_bf16(f[4], f[5]), pack_bf16(f[6], f[7]));
     }
 }
 
@@ -450,10 +480,12 @@ bool launch_cache_read(FFAttention *att, const uint8_t *pages, uint32_t pageCoun
                        uint16_t *v, cudaStream_t stream, const char **error) {
     if (tokens == 0 || (!k && !v)) return true;
     const FFAttentionConfig &cfg = att->cfg;
-    ReadArgs a{pages, slots, k, v, tokens, cfg.kvHeads, pageCount * cfg.pageTokens, shift_of(cfg.pageTokens), cfg.headDim, page_layout(cfg), att->errorFlag};
-    const uint64_t total = (uint64_t)tokens * cfg.kvHeads * (cfg.headDim / 8) * ((k ? 1 : 0) + (v ? 1 : 0));
-    const uint32_t grid = (uint32_t)std::min<uint64_t>((total + 255) / 256, (uint64_t)att->smCount * 32);
-    return launched(att, launch_pdl(k_cache_read, dim3(grid), dim3(256), 0, stream, a), "k_cache_read", error);
+    const uint32_t perUnit = 4u * 256u / cfg.headDim, heads = cfg.kvHeads * ((k ? 1u : 0u) + (v ? 1u : 0u));
+    ReadArgs a{pages, slots, k, v, tokens, cfg.kvHeads, pageCount * cfg.pageTokens, shift_of(cfg.pageTokens), (heads + perUnit - 1) / perUnit, page_layout(cfg), att->errorFlag};
+    const dim3 grid((uint32_t)(((uint64_t)tokens * a.unitsPerToken + 3) / 4)), block(128);
+    const cudaError_t st = cfg.headDim == 64 ? launch_pdl(k_cache_read<64>, grid, block, 0, stream, a)
+                           : cfg.headDim == 128 ? launch_pdl(k_cache_read<128>, grid, block, 0, stream, a) : launch_pdl(k_cache_read<256>, grid, block, 0, stream, a);
+    return launched(att, st, "k_cache_read", error);
 }
 
 }  // namespace ff
