@@ -6,8 +6,8 @@
 // batch leaves no SM with more than another.  A unit that several CTAs share is joined by whichever of them ends last,
 // in the CTAs' order: the same bits every time, and nothing waits.
 //
-// In a CTA one warp copies (TMA boxes of codes, bulk copies of scale words, a ring of tiles); four warps take 16 keys of
-// a tile each, with a maximum, sum and output of their own, joined at the end of a unit.  Per 16 keys:
+// In a CTA one warp copies (TMA boxes of codes, bulk copies of scale words, a ring of tiles); four warps take 32 keys of
+// every second tile each, with a maximum, sum and output of their own, joined at the end of a unit.  Per 16 keys:
 //   S = K q   codes as they lie are the A operand: a nibble masked in place IS an f16, the subnormal code * 2^-24 or
 //             * 2^-20, exact, so a word of eight codes costs five instructions.  q is B, in f16 at a power of two of its
 //             own (bf16 fits f16's 11 bits; what lies 2^-28 below the largest is lost).  Per group of 64 the 32-bit sum
@@ -25,9 +25,9 @@ namespace ff {
 
 namespace {
 
-constexpr int kConsumers = 4;                      // warps that compute, 16 keys of a tile each
+constexpr int kConsumers = 4;                      // warps that compute: two a tile, 32 keys each
 constexpr int kRowsThreads = 32 * (kConsumers + 1);
-static_assert(kTileKeys == 16 * kConsumers, "a warp takes 16 keys");
+static_assert(kTileKeys == 64 && kConsumers == 4, "two warps a tile, 32 keys each");
 
 struct RowsArgs {
     AttendArgs a;
@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
     if (tid == 0) {
         for (uint32_t s = 0; s < kStages; ++s) {
             bar_init(barFull + 8 * s, 1);
-            bar_init(barEmpty + 8 * s, kConsumers);
+            bar_init(barEmpty + 8 * s, kConsumers / 2);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -275,19 +275,30 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
 
     // ---------------- 16 keys of every tile ----------------
     const uint32_t g = lane >> 2, t = lane & 3u;
-    // A stage: [piece][keys, values][its keys][codes], then [piece][keys, values][its keys][words].
-    const uint32_t keyA = 16 * warp + key_of_row<DIM>(g);  // the S fragments' rows: keys keyA and keyA + 8 of a tile
-    const uint32_t pieceAt = (16 * warp >> args.pieceShift) << args.pieceShift;  // first key of the warp's piece
-    const uint32_t kRow = keyA + pieceAt, vStep = 1u << args.pieceShift;         // (a piece's values lie behind its keys: rows pieceAt further)
-    const uint32_t kOff = kRow * CB + ((t * 8) ^ chunk_flip<DIM>(keyA));
-    uint32_t vKey[2], vRow[2], vOff[2];  // the P fragments' keys 2t and 2t + 1, and those + 8
+    // A stage: [piece][keys, values][its keys][codes], then [piece][keys, values][its keys][words].  Warps 0 and 1 take half of
+    // every second tile each, warps 2 and 3 of the others: 32 keys at a time as two subtiles of 16, for whose loads and products
+    // there is then other work to do, and one round of everything that is done once.
+    const uint32_t warpKey = 32 * (warp & 1u);
+    const uint32_t keyA = key_of_row<DIM>(g);  // the S fragments' rows: keys keyA and keyA + 8 of a subtile
+    const uint32_t vStep = 1u << args.pieceShift;
+    uint32_t subRow[2];  // first row of a subtile's keys: a piece's values lie behind its keys
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        vKey[i] = 16 * warp + key_of_row<DIM>(2 * t + i);
-        vRow[i] = vKey[i] + pieceAt + vStep;
-        vOff[i] = vRow[i] * CB + ((g * 4) ^ chunk_flip<DIM>(vKey[i]));
+    for (int sub = 0; sub < 2; ++sub) {
+        const uint32_t key = warpKey + 16 * sub;
+        subRow[sub] = key + ((key >> args.pieceShift) << args.pieceShift);
     }
-    uint32_t stage = 0, phase = 0;
+    const uint32_t kOff = keyA * CB + ((t * 8) ^ chunk_flip<DIM>(keyA));
+    uint32_t vOff[2];  // the P fragments' keys 2t and 2t + 1; those + 8 follow
+#pragma unroll
+    for (int i = 0; i < 2; ++i) vOff[i] = (key_of_row<DIM>(2 * t + i) + vStep) * CB + ((g * 4) ^ chunk_flip<DIM>(key_of_row<DIM>(2 * t + i)));
+    // Value scales are converted once, a pair of keys (rows 2j, 2j + 1 of a subtile) and group to a lane, and handed round:
+    // lane (and element e) = subtile * 8 + j, group = 2 e + lane / 16 (dim 64: lanes from 16 on repeat)
+    constexpr int kPairs = NG == 4 ? 2 : 1;
+    const uint32_t pairSub = (lane >> 3) & 1u, pairRow = 2 * (lane & 7u), pairGroup = NG == 1 ? 0u : lane >> 4;
+    uint32_t pairKey[2];  // in the warp's 32
+#pragma unroll
+    for (int i = 0; i < 2; ++i) pairKey[i] = 16 * pairSub + (pairRow & 8u) + key_of_row<DIM>((pairRow & 7u) + i);
+    const uint32_t pairWord = (subRow[0] + vStep + (pairSub ? subRow[1] - subRow[0] - 16 : 0u)) * WB + pairGroup * 4;  // + pairKey * WB
     Walk w = locate(begin);
     uint32_t x = begin;
     while (x < end) {
@@ -345,8 +356,9 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
                 const uint32_t from = (2 * t + c) * 4;
 #pragma unroll
                 for (int G = 0; G < NG; ++G) qSum[G][n][c] = __shfl_sync(0xFFFFFFFFu, mine[G], from) * 0x1p-24f;
-                const int e = (int)__shfl_sync(0xFFFFFFFFu, exponent, from) - 140;  // q = f16 * 2^e; the codes are 2^-24 of theirs
-                toLog2[n][c] = a.scale * 1.4426950408889634f * power_of_two(e + 4);
+                // q = f16 * 2^(exponent - 140), the codes are 2^-24 of theirs
+                const int e = (int)__shfl_sync(0xFFFFFFFFu, exponent, from) - 116, half = e >> 1;
+                toLog2[n][c] = a.scale * 1.4426950408889634f * power_of_two(half) * power_of_two(e - half);
             }
         }
 
@@ -366,72 +378,63 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
         }
         const int pFirst = w.q.p0 + (int)(column0 / group), pLast = w.q.p0 + (int)((min(columns, column0 + kColumns) - 1) / group);
 
-        for (uint32_t i = t0; i < t0 + count; ++i) {
+        // tiles are counted over the CTA's run: their stage, and the warps that take them
+        const uint32_t n0 = x - begin;
+        for (uint32_t i = t0 + ((n0 ^ (warp >> 1)) & 1u); i < t0 + count; i += 2) {
+            const uint32_t number = n0 + i - t0, stage = number % kStages, phase = number / kStages & 1u;
             const uint32_t tileKey = (i < w.q.tilesSink ? i : w.q.lowTile + i - w.q.tilesSink) * kTileKeys;
-            const int j0 = (int)(tileKey + 16 * warp);
+            const int j0 = (int)(tileKey + warpKey);
             const uint32_t base = ring + stage * kStage;
             if (!mbar_try_wait(barFull + 8 * stage, phase) && !slot_wait_slow(barFull + 8 * stage, phase) && lane == 0) *a.errorFlag = kFlagWait;
             __syncwarp();
-            const bool hole = holes[stage] >> (16 * warp >> args.pieceShift) & 1u;
+            const uint32_t gone = holes[stage], hole0 = gone >> (warpKey >> args.pieceShift) & 1u, hole1 = gone >> ((warpKey + 16) >> args.pieceShift) & 1u;
             // keys that not every row of the tile sees
-            const bool careful = hole || j0 + 15 > pFirst || (a.window && (long long)j0 <= (long long)pLast - a.window && (uint32_t)j0 + 16u > a.sinks);
+            const bool careful = (hole0 | hole1) || j0 + 31 > pFirst || (a.window && (long long)j0 <= (long long)pLast - a.window && (uint32_t)j0 + 32u > a.sinks);
             auto sees = [&](int key, int p) {
-                return !hole && key <= p && (!a.window || (long long)key > (long long)p - a.window || (uint32_t)key < a.sinks);
+                return key <= p && (!a.window || (long long)key > (long long)p - a.window || (uint32_t)key < a.sinks) && !((uint32_t)(key - j0) < 16u ? hole0 : hole1);
             };
 
             // ---- value scales as f16 pairs of keys, at 2^-E ----
-            uint32_t vWords[4][NG];  // keys 2t, 2t + 1, 2t + 8, 2t + 9
+            uint32_t pairs[kPairs][2];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) lds_words<NG>(base + kKeyWords + (vRow[k & 1] + 8 * (k >> 1)) * WB, vWords[k]);
+            for (int e = 0; e < kPairs; ++e)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) pairs[e][k] = lds32(base + kKeyWords + pairWord + pairKey[k] * WB + 8 * e);
             if (careful) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int key = (int)tileKey + (int)vKey[k & 1] + 8 * (k >> 1);
-                    const int p = max(key, pFirst);  // of the rows that may see it, the one whose window goes back furthest
+                for (int k = 0; k < 2; ++k) {
+                    const int key = j0 + (int)pairKey[k], p = max(key, pFirst);  // of the rows that may see it, the one whose window goes back furthest
                     if (p > pLast || !sees(key, p))
 #pragma unroll
-                        for (int G = 0; G < NG; ++G) vWords[k][G] = 0u;
+                        for (int e = 0; e < kPairs; ++e) pairs[e][k] = 0u;
                 }
             }
-            uint32_t vScale[NG][2], vBias[2];
+            uint32_t pairScale[kPairs], pairBias[kPairs];
             auto convert = [&] {
                 const float f = power_of_two(-E);
                 uint32_t most = 0;
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                    for (int G = 0; G < NG; ++G) {
-                        vScale[G][h] = pack_f16(low16(vWords[2 * h][G]) * f, low16(vWords[2 * h + 1][G]) * f);
-                        most = max_f16x2(most, vScale[G][h]);
-                    }
-                    uint32_t b0 = 0, b1 = 0;
-#pragma unroll
-                    for (int G = 0; G < NG; ++G)
-                        if (g == (uint32_t)G) b0 = vWords[2 * h][G], b1 = vWords[2 * h + 1][G];
-                    vBias[h] = pack_f16(high16(b0) * f, high16(b1) * f);
-                    most = max_f16x2(most, vBias[h] & 0x7FFF7FFFu);
+                for (int e = 0; e < kPairs; ++e) {
+                    pairScale[e] = pack_f16(low16(pairs[e][0]) * f, low16(pairs[e][1]) * f);
+                    pairBias[e] = pack_f16(high16(pairs[e][0]) * f, high16(pairs[e][1]) * f);
+                    most = max_f16x2(most, max_f16x2(pairScale[e], pairBias[e] & 0x7FFF7FFFu));
                 }
                 // beyond 2^6, or NaN
                 const __half2 m = *reinterpret_cast<const __half2 *>(&most);
                 return !(__low2float(m) <= 64.0f && __high2float(m) <= 64.0f);
             };
-            bool brokenKeys = false;
+            uint32_t broken[2] = {0u, 0u};  // lanes whose pair's first, second key has a value that is no number
             if (__any_sync(0xFFFFFFFFu, convert())) {
                 uint32_t most = 0;
-                bool broken = false;
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    bool bad = false;
+                for (int e = 0; e < kPairs; ++e)
 #pragma unroll
-                    for (int G = 0; G < NG; ++G) bad |= is_broken(vWords[k][G]);
-                    broken |= bad;
-#pragma unroll
-                    for (int G = 0; G < NG; ++G) {
-                        if (bad) vWords[k][G] = 0u;
-                        most = max(most, word_exponent(vWords[k][G]));
+                    for (int k = 0; k < 2; ++k) {
+                        const bool bad = is_broken(pairs[e][k]);
+                        broken[k] |= __ballot_sync(0xFFFFFFFFu, bad);
+                        if (bad) pairs[e][k] = 0u;
+                        most = max(most, word_exponent(pairs[e][k]));
                     }
-                }
-                brokenKeys = __any_sync(0xFFFFFFFFu, broken);
                 most = __reduce_max_sync(0xFFFFFFFFu, most);
                 const int raised = min(max((int)most - 127 - 5, E), 120);
                 if (raised > E) {
@@ -453,59 +456,56 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
             }
 
             // ---- logits ----
-            float s[NT][4];
+            float s[2][NT][4];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
-            uint32_t kWords[2][NG];
-            lds_words<NG>(base + kKeyWords + kRow * WB, kWords[0]);
-            lds_words<NG>(base + kKeyWords + (kRow + 8) * WB, kWords[1]);
+            for (int sub = 0; sub < 2; ++sub) {
+                uint32_t kWords[2][NG];
+                lds_words<NG>(base + kKeyWords + (subRow[sub] + keyA) * WB, kWords[0]);
+                lds_words<NG>(base + kKeyWords + (subRow[sub] + keyA + 8) * WB, kWords[1]);
+                const uint32_t row = base + subRow[sub] * CB + kOff;
 #pragma unroll
-            for (int G = 0; G < NG; ++G) {
-                const uint2 wa = lds64((base + kOff) ^ (uint32_t)(G * 32)), wb = lds64((base + kOff + 8 * CB) ^ (uint32_t)(G * 32));
-                const uint32_t ax = wa.x >> 8, ay = wa.y >> 8, bx = wb.x >> 8, by = wb.y >> 8;
-                float acc[NT][4];
+                for (int n = 0; n < NT; ++n) s[sub][n][0] = s[sub][n][1] = s[sub][n][2] = s[sub][n][3] = 0.0f;
 #pragma unroll
-                for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
+                for (int G = 0; G < NG; ++G) {
+                    const uint2 wa = lds64(row ^ (uint32_t)(G * 32)), wb = lds64((row ^ (uint32_t)(G * 32)) + 8 * CB);
+                    const uint32_t ax = wa.x >> 8, ay = wa.y >> 8, bx = wb.x >> 8, by = wb.y >> 8;
+                    float acc[NT][4];
 #pragma unroll
-                for (int n = 0; n < NT; ++n) mma_f16(acc[n], nibbles<0>(wa.x, ax), nibbles<0>(wb.x, bx), nibbles<0>(wa.y, ay), nibbles<0>(wb.y, by), qf[G][0][n][0], qf[G][0][n][1]);
+                    for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
 #pragma unroll
-                for (int n = 0; n < NT; ++n) mma_f16(acc[n], nibbles<1>(wa.x, ax), nibbles<1>(wb.x, bx), nibbles<1>(wa.y, ay), nibbles<1>(wb.y, by), qf[G][1][n][0], qf[G][1][n][1]);
+                    for (int n = 0; n < NT; ++n) mma_f16(acc[n], nibbles<0>(wa.x, ax), nibbles<0>(wb.x, bx), nibbles<0>(wa.y, ay), nibbles<0>(wb.y, by), qf[G][0][n][0], qf[G][0][n][1]);
 #pragma unroll
-                for (int n = 0; n < NT; ++n) mma_f16(acc[n], nibbles<2>(wa.x, ax), nibbles<2>(wb.x, bx), nibbles<2>(wa.y, ay), nibbles<2>(wb.y, by), qf[G][2][n][0], qf[G][2][n][1]);
+                    for (int n = 0; n < NT; ++n) mma_f16(acc[n], nibbles<1>(wa.x, ax), nibbles<1>(wb.x, bx), nibbles<1>(wa.y, ay), nibbles<1>(wb.y, by), qf[G][1][n][0], qf[G][1][n][1]);
 #pragma unroll
-                for (int n = 0; n < NT; ++n) mma_f16(acc[n], nibbles<3>(wa.x, ax), nibbles<3>(wb.x, bx), nibbles<3>(wa.y, ay), nibbles<3>(wb.y, by), qf[G][3][n][0], qf[G][3][n][1]);
-                const float sa = low16(kWords[0][G]), ba = high16(kWords[0][G]), sb = low16(kWords[1][G]), bb = high16(kWords[1][G]);
+                    for (int n = 0; n < NT; ++n) mma_f16(acc[n], nibbles<2>(wa.x, ax), nibbles<2>(wb.x, bx), nibbles<2>(wa.y, ay), nibbles<2>(wb.y, by), qf[G][2][n][0], qf[G][2][n][1]);
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    s[n][0] = fmaf(sa, acc[n][0], fmaf(ba, qSum[G][n][0], s[n][0]));
-                    s[n][1] = fmaf(sa, acc[n][1], fmaf(ba, qSum[G][n][1], s[n][1]));
-                    s[n][2] = fmaf(sb, acc[n][2], fmaf(bb, qSum[G][n][0], s[n][2]));
-                    s[n][3] = fmaf(sb, acc[n][3], fmaf(bb, qSum[G][n][1], s[n][3]));
-                }
-            }
+                    for (int n = 0; n < NT; ++n) mma_f16(acc[n], nibbles<3>(wa.x, ax), nibbles<3>(wb.x, bx), nibbles<3>(wa.y, ay), nibbles<3>(wb.y, by), qf[G][3][n][0], qf[G][3][n][1]);
+                    const float sa = low16(kWords[0][G]), ba = high16(kWords[0][G]), sb = low16(kWords[1][G]), bb = high16(kWords[1][G]);
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int k = 0; k < 4; ++k) s[n][k] = (s[n][k] * 0x1p20f) * toLog2[n][k & 1];
-            if (careful || brokenKeys) {
-                bool bad[2] = {false, false};
-                if (brokenKeys) {
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        uint32_t words[NG];
-                        lds_words<NG>(base + kKeyWords + (kRow + vStep + 8 * h) * WB, words);
-#pragma unroll
-                        for (int G = 0; G < NG; ++G) bad[h] |= is_broken(words[G]);
+                    for (int n = 0; n < NT; ++n) {
+                        s[sub][n][0] = fmaf(sa, acc[n][0], fmaf(ba, qSum[G][n][0], s[sub][n][0]));
+                        s[sub][n][1] = fmaf(sa, acc[n][1], fmaf(ba, qSum[G][n][1], s[sub][n][1]));
+                        s[sub][n][2] = fmaf(sb, acc[n][2], fmaf(bb, qSum[G][n][0], s[sub][n][2]));
+                        s[sub][n][3] = fmaf(sb, acc[n][3], fmaf(bb, qSum[G][n][1], s[sub][n][3]));
                     }
                 }
+            }
+            if (careful || (broken[0] | broken[1])) {
+                // a row r of a subtile is the first or second key of pair r / 2
+                const uint32_t marks0 = broken[0] | (broken[0] >> 16), marks1 = broken[1] | (broken[1] >> 16);
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+                for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const uint32_t column = column0 + 8 * n + (2 * t + (k & 1)) % kColumns;
-                        const int p = w.q.p0 + (int)(column / group);
-                        if (!sees((int)tileKey + (int)keyA + 8 * (k >> 1), p)) s[n][k] = -INFINITY;
-                        else if (bad[k >> 1]) s[n][k] = NAN;
+                    for (int h = 0; h < 2; ++h) {
+                        const bool bad = (g & 1u ? marks1 : marks0) >> (8 * sub + 4 * h + (g >> 1)) & 1u;
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int c = 0; c < 2; ++c) {
+                                const uint32_t column = column0 + 8 * n + (2 * t + c) % kColumns;
+                                if (!sees(j0 + 16 * sub + 8 * h + (int)keyA, w.q.p0 + (int)(column / group))) s[sub][n][2 * h + c] = -INFINITY;
+                                else if (bad) s[sub][n][2 * h + c] = NAN;
+                            }
                     }
             }
 
@@ -516,12 +516,12 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
             for (int n = 0; n < NT; ++n)
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    float m = fmaxf(s[n][c], s[n][c + 2]);
+                    float m = fmaxf(fmaxf(s[0][n][c], s[0][n][c + 2]), fmaxf(s[1][n][c], s[1][n][c + 2]));
                     m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 4));
                     m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 8));
                     m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 16));
-                    most[n][c] = m;
-                    above |= m > top[n][c] + kLazy;
+                    most[n][c] = m * toLog2[n][c];
+                    above |= most[n][c] > top[n][c] + kLazy;
                 }
             if (__any_sync(0xFFFFFFFFu, above)) {
 #pragma unroll
@@ -543,49 +543,66 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
                     for (int k = 0; k < 4; ++k) extra[n][k] *= f[k & 1];
                 }
             }
-            uint32_t p[NT][2];
+            uint32_t p[2][NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const float m0 = top[n][0] == -INFINITY ? 0.0f : top[n][0], m1 = top[n][1] == -INFINITY ? 0.0f : top[n][1];
-                p[n][0] = transposed(pack_f16(exp2_fast(s[n][0] - m0), exp2_fast(s[n][1] - m1)));
-                p[n][1] = transposed(pack_f16(exp2_fast(s[n][2] - m0), exp2_fast(s[n][3] - m1)));
+#pragma unroll
+                for (int sub = 0; sub < 2; ++sub)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        p[sub][n][h] = transposed(pack_f16(exp2_fast(fmaf(s[sub][n][2 * h], toLog2[n][0], -m0)), exp2_fast(fmaf(s[sub][n][2 * h + 1], toLog2[n][1], -m1))));
             }
 
             // ---- values; row 8 of the last product adds up the weights, rows 0 .. NG - 1 the biases ----
             const uint32_t ones = g == 0 ? 0x3C003C00u : 0u;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) mma_f16(extra[n], vBias[0], ones, vBias[1], ones, p[n][0], p[n][1]);
-#pragma unroll
-            for (int G = 0; G < NG; ++G) {
-                uint32_t lo[2], hi[2];
+            for (int sub = 0; sub < 2; ++sub) {
+                uint32_t bias[2];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const uint32_t wa = lds32((base + vOff[0] + 8 * h * CB) ^ (uint32_t)(G * 32));
-                    const uint32_t wb = lds32((base + vOff[1] + 8 * h * CB) ^ (uint32_t)(G * 32));
-                    lo[h] = __byte_perm(wa, wb, 0x5410);
-                    hi[h] = __byte_perm(wa, wb, 0x7632);
+                    const uint32_t from = (NG == 1 ? 0u : (g & 1u) * 16) + 8 * sub + 4 * h + t;
+                    bias[h] = __shfl_sync(0xFFFFFFFFu, pairBias[0], from);
+                    if (NG == 4) {
+                        const uint32_t other = __shfl_sync(0xFFFFFFFFu, pairBias[kPairs - 1], from);
+                        if (g & 2u) bias[h] = other;
+                    }
+                    if (g >= (uint32_t)NG) bias[h] = 0u;
                 }
-                const uint32_t lo0 = lo[0] >> 8, lo1 = lo[1] >> 8, hi0 = hi[0] >> 8, hi1 = hi[1] >> 8;
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    uint32_t b0 = mul_f16x2(p[n][0], vScale[G][0]), b1 = mul_f16x2(p[n][1], vScale[G][1]);
-                    const uint32_t rest0 = residual_f16x2(p[n][0], vScale[G][0], b0), rest1 = residual_f16x2(p[n][1], vScale[G][1], b1);
-                    if (SPLIT && g >= 4) b0 = rest0, b1 = rest1;
-                    mma_f16(o[G][0][n], nibbles<0>(lo[0], lo0), nibbles<0>(hi[0], hi0), nibbles<0>(lo[1], lo1), nibbles<0>(hi[1], hi1), b0, b1);
-                    mma_f16(o[G][1][n], nibbles<1>(lo[0], lo0), nibbles<1>(hi[0], hi0), nibbles<1>(lo[1], lo1), nibbles<1>(hi[1], hi1), b0, b1);
-                    mma_f16(o[G][2][n], nibbles<2>(lo[0], lo0), nibbles<2>(hi[0], hi0), nibbles<2>(lo[1], lo1), nibbles<2>(hi[1], hi1), b0, b1);
-                    mma_f16(o[G][3][n], nibbles<3>(lo[0], lo0), nibbles<3>(hi[0], hi0), nibbles<3>(lo[1], lo1), nibbles<3>(hi[1], hi1), b0, b1);
-                    if (!SPLIT) {
-                        mma_f16(o[G][0][n], nibbles<0>(lo[0], lo0), nibbles<0>(hi[0], hi0), nibbles<0>(lo[1], lo1), nibbles<0>(hi[1], hi1), rest0, rest1);
-                        mma_f16(o[G][1][n], nibbles<1>(lo[0], lo0), nibbles<1>(hi[0], hi0), nibbles<1>(lo[1], lo1), nibbles<1>(hi[1], hi1), rest0, rest1);
-                        mma_f16(o[G][2][n], nibbles<2>(lo[0], lo0), nibbles<2>(hi[0], hi0), nibbles<2>(lo[1], lo1), nibbles<2>(hi[1], hi1), rest0, rest1);
-                        mma_f16(o[G][3][n], nibbles<3>(lo[0], lo0), nibbles<3>(hi[0], hi0), nibbles<3>(lo[1], lo1), nibbles<3>(hi[1], hi1), rest0, rest1);
+                for (int n = 0; n < NT; ++n) mma_f16(extra[n], bias[0], ones, bias[1], ones, p[sub][n][0], p[sub][n][1]);
+                const uint32_t rows0 = base + subRow[sub] * CB + vOff[0], rows1 = base + subRow[sub] * CB + vOff[1];
+#pragma unroll
+                for (int G = 0; G < NG; ++G) {
+                    uint32_t lo[2], hi[2], scale[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const uint32_t wa = lds32((rows0 ^ (uint32_t)(G * 32)) + 8 * h * CB), wb = lds32((rows1 ^ (uint32_t)(G * 32)) + 8 * h * CB);
+                        lo[h] = __byte_perm(wa, wb, 0x5410);
+                        hi[h] = __byte_perm(wa, wb, 0x7632);
+                        scale[h] = __shfl_sync(0xFFFFFFFFu, pairScale[NG == 4 ? G / 2 : 0], (G & 1) * 16 + 8 * sub + 4 * h + t);
+                    }
+                    const uint32_t lo0 = lo[0] >> 8, lo1 = lo[1] >> 8, hi0 = hi[0] >> 8, hi1 = hi[1] >> 8;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        uint32_t b0 = mul_f16x2(p[sub][n][0], scale[0]), b1 = mul_f16x2(p[sub][n][1], scale[1]);
+                        const uint32_t rest0 = residual_f16x2(p[sub][n][0], scale[0], b0), rest1 = residual_f16x2(p[sub][n][1], scale[1], b1);
+                        if (SPLIT && g >= 4) b0 = rest0, b1 = rest1;
+                        mma_f16(o[G][0][n], nibbles<0>(lo[0], lo0), nibbles<0>(hi[0], hi0), nibbles<0>(lo[1], lo1), nibbles<0>(hi[1], hi1), b0, b1);
+                        mma_f16(o[G][1][n], nibbles<1>(lo[0], lo0), nibbles<1>(hi[0], hi0), nibbles<1>(lo[1], lo1), nibbles<1>(hi[1], hi1), b0, b1);
+                        mma_f16(o[G][2][n], nibbles<2>(lo[0], lo0), nibbles<2>(hi[0], hi0), nibbles<2>(lo[1], lo1), nibbles<2>(hi[1], hi1), b0, b1);
+                        mma_f16(o[G][3][n], nibbles<3>(lo[0], lo0), nibbles<3>(hi[0], hi0), nibbles<3>(lo[1], lo1), nibbles<3>(hi[1], hi1), b0, b1);
+                        if (!SPLIT) {
+                            mma_f16(o[G][0][n], nibbles<0>(lo[0], lo0), nibbles<0>(hi[0], hi0), nibbles<0>(lo[1], lo1), nibbles<0>(hi[1], hi1), rest0, rest1);
+                            mma_f16(o[G][1][n], nibbles<1>(lo[0], lo0), nibbles<1>(hi[0], hi0), nibbles<1>(lo[1], lo1), nibbles<1>(hi[1], hi1), rest0, rest1);
+                            mma_f16(o[G][2][n], nibbles<2>(lo[0], lo0), nibbles<2>(hi[0], hi0), nibbles<2>(lo[1], lo1), nibbles<2>(hi[1], hi1), rest0, rest1);
+                            mma_f16(o[G][3][n], nibbles<3>(lo[0], lo0), nibbles<3>(hi[0], hi0), nibbles<3>(lo[1], lo1), nibbles<3>(hi[1], hi1), rest0, rest1);
+                        }
                     }
                 }
             }
             __syncwarp();
             if (lane == 0) mbar_arrive(barEmpty + 8 * stage);
-            if (++stage == kStages) stage = 0, phase ^= 1u;
         }
 
         // ---- the warps' outputs joined ----
