@@ -27,6 +27,7 @@ namespace {
 
 constexpr int kConsumers = 4;                      // warps that compute: two a tile, 32 keys each
 constexpr int kRowsThreads = 32 * (kConsumers + 1);
+constexpr uint32_t kUnitCost = 8;                 // tiles' time that a unit takes besides its tiles
 static_assert(kTileKeys == 64 && kConsumers == 4, "two warps a tile, 32 keys each");
 
 struct RowsArgs {
@@ -96,6 +97,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
     __shared__ float2 joinStats[kConsumers][kColumns];
     __shared__ float joinBias[kConsumers][NG][kColumns];
     __shared__ uint32_t lastPart;
+    __shared__ RowsRequest known[kRowsThreads];
     const AttendArgs &a = args.a;
     const uint32_t tid = threadIdx.x, warp = (uint32_t)warp_index(), lane = tid & 31u;
     const uint32_t ring = (sm_addr(rowsSmem) + 1023u) & ~1023u;
@@ -112,7 +114,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
     pdl_enter();
 
     // ---- the plan: how many tiles each request is, and this CTA's run of them ----
-    auto request_of = [&](uint32_t r) {
+    auto look_up = [&](uint32_t r) {
         RowsRequest q{};
         const uint32_t begin = min(__ldg(a.rowStart + r), a.tokens), end = min(__ldg(a.rowStart + r + 1), a.tokens);
         const uint32_t rows = end > begin ? end - begin : 0u;
@@ -131,12 +133,17 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
         q.tiles = max(1u, q.tilesSink + ends - q.lowTile);  // (a request without keys: one tile that nobody sees)
         return q;
     };
+    // A unit costs its tiles and kUnitCost more: its queries, joins and output take as long.  (Cut by tiles alone, the CTAs with the
+    // short requests of a ragged batch took 94 us where the others took 62.)
+    auto unit_cost = [](const RowsRequest &q) { return q.rows ? q.tiles + kUnitCost : 0u; };
     const uint32_t run = (a.requests + kRowsThreads - 1) / kRowsThreads;
+    auto request_of = [&](uint32_t r) { return run == 1 ? known[r] : look_up(r); };  // (a batch of up to 160 is looked up once)
     const uint32_t r0 = min(tid * run, a.requests), r1 = min(r0 + run, a.requests);
     uint32_t sum = 0;
     for (uint32_t r = r0; r < r1; ++r) {
-        const RowsRequest q = request_of(r);
-        sum += q.tiles * q.columnTiles * a.kvHeads;
+        const RowsRequest q = look_up(r);
+        if (run == 1) known[r] = q;
+        sum += unit_cost(q) * q.columnTiles * a.kvHeads;
     }
     uint32_t scan = sum;
 #pragma unroll
@@ -174,16 +181,25 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
         }
     }
     if (total == 0) return;
-    const uint32_t ctas = min(gridDim.x, total), cta = blockIdx.x;
+    const uint32_t ctas = min(gridDim.x, max(1u, total / 3u)), cta = blockIdx.x;
     if (cta >= ctas) return;
     auto start_of = [&](uint32_t c) { return (uint32_t)((unsigned long long)c * total / ctas); };
     auto cta_of = [&](uint32_t x) { return (uint32_t)((((unsigned long long)x + 1) * ctas - 1) / total); };
     const uint32_t begin = start_of(cta), end = start_of(cta + 1);
 
-    // Where the run stands: request, head, column tile, tile.
+    // Where the run stands: a request's unit, whose tile i stands at x = first + kUnitCost + i; and the tiles of it that are
+    // this CTA's.
     struct Walk {
-        uint32_t r, inRequest, x;  // request, units' tiles before x within it
+        uint32_t r, unit, first;
         RowsRequest q;
+        uint32_t t0, count, head, column0;
+    };
+    auto take = [&](Walk &w) {
+        const uint32_t tile0 = w.first + kUnitCost;
+        w.t0 = begin > tile0 ? min(begin - tile0, w.q.tiles) : 0u;
+        w.count = (end > tile0 ? min(end - tile0, w.q.tiles) : 0u) - w.t0;
+        w.head = w.unit / w.q.columnTiles;
+        w.column0 = w.unit % w.q.columnTiles * kColumns;
     };
     auto locate = [&](uint32_t x) {
         uint32_t low = 0, high = kRowsThreads;
@@ -193,22 +209,30 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
             else high = mid;
         }
         Walk w;
-        w.x = x;
         uint32_t n = x - first[low];
         for (w.r = low * run;; ++w.r) {
             w.q = request_of(w.r);
-            const uint32_t mine = w.q.tiles * w.q.columnTiles * a.kvHeads;
+            const uint32_t mine = unit_cost(w.q) * w.q.columnTiles * a.kvHeads;
             if (n < mine) break;
             n -= mine;
         }
-        w.inRequest = n;
+        w.unit = n / unit_cost(w.q);
+        w.first = x - n % unit_cost(w.q);
+        take(w);
         return w;
     };
-    auto next_request = [&](Walk &w) {
-        w.inRequest = 0;
-        do {
-            w.q = request_of(++w.r);
-        } while (w.q.rows == 0);
+    // the unit behind; false past the run's end
+    auto next_unit = [&](Walk &w) {
+        w.first += unit_cost(w.q);
+        if (w.first >= end) return false;
+        if (++w.unit == w.q.columnTiles * a.kvHeads) {
+            w.unit = 0;
+            do {
+                w.q = request_of(++w.r);
+            } while (w.q.rows == 0);
+        }
+        take(w);
+        return true;
     };
 
     if (warp == (uint32_t)kConsumers) {
@@ -221,10 +245,9 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
         const uint32_t pieceCodes = 2u * CB << args.pieceShift, pieceWords = 2u * WB << args.pieceShift;
         uint32_t stage = 0, phase = 0;
         Walk w = locate(begin);
-        uint32_t x = begin;
-        while (x < end) {
-            const uint32_t unitTiles = w.q.tiles, t0 = w.inRequest % unitTiles, head = w.inRequest / unitTiles / w.q.columnTiles;
-            const uint32_t count = min(end - x, unitTiles - t0);
+        do {
+            const uint32_t t0 = w.t0, count = w.count, head = w.head;
+            if (count == 0) continue;
             const int keysEnd = w.q.p0 + (int)w.q.rows;
             auto key_at = [&](uint32_t t) { return (t < w.q.tilesSink ? t : w.q.lowTile + t - w.q.tilesSink) * kTileKeys; };
             auto page_of = [&](uint32_t base) {
@@ -266,10 +289,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
                     if (++stage == kStages) stage = 0, phase ^= 1u;
                 }
             }
-            x += count;
-            w.inRequest += count;
-            if (x < end && w.inRequest == unitTiles * w.q.columnTiles * a.kvHeads) next_request(w);
-        }
+        } while (next_unit(w));
         return;
     }
 
@@ -300,12 +320,11 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
     for (int i = 0; i < 2; ++i) pairKey[i] = 16 * pairSub + (pairRow & 8u) + key_of_row<DIM>((pairRow & 7u) + i);
     const uint32_t pairWord = (subRow[0] + vStep + (pairSub ? subRow[1] - subRow[0] - 16 : 0u)) * WB + pairGroup * 4;  // + pairKey * WB
     Walk w = locate(begin);
-    uint32_t x = begin;
-    while (x < end) {
-        const uint32_t unitTiles = w.q.tiles, t0 = w.inRequest % unitTiles, unit = w.inRequest / unitTiles;
-        const uint32_t head = unit / w.q.columnTiles, column0 = unit % w.q.columnTiles * kColumns;
-        const uint32_t columns = w.q.rows * group, count = min(end - x, unitTiles - t0);
-        
+    uint32_t n0 = 0;  // tiles so far: they are counted over the CTA's run, for their stage and the warps that take them
+    do {
+        const uint32_t t0 = w.t0, count = w.count, head = w.head, column0 = w.column0, unitTiles = w.q.tiles;
+        if (count == 0) continue;  // (the run begins or ends in front of the unit's first tile)
+        const uint32_t columns = w.q.rows * group;
         // queries: f16 at a power of two of the column's largest value
         uint32_t qf[NG][4][NT][2];
         float qSum[NG][NT][2], toLog2[NT][2];
@@ -378,8 +397,6 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
         }
         const int pFirst = w.q.p0 + (int)(column0 / group), pLast = w.q.p0 + (int)((min(columns, column0 + kColumns) - 1) / group);
 
-        // tiles are counted over the CTA's run: their stage, and the warps that take them
-        const uint32_t n0 = x - begin;
         for (uint32_t i = t0 + ((n0 ^ (warp >> 1)) & 1u); i < t0 + count; i += 2) {
             const uint32_t number = n0 + i - t0, stage = number % kStages, phase = number / kStages & 1u;
             const uint32_t tileKey = (i < w.q.tilesSink ? i : w.q.lowTile + i - w.q.tilesSink) * kTileKeys;
@@ -657,7 +674,6 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
 
         // ---- the unit's rows, or this CTA's part of them ----
         const uint32_t used = min(kColumns, columns - column0);
-        const uint32_t unitBegin = x - t0, unitEnd = unitBegin + unitTiles;
         const bool whole = count == unitTiles;
         const uint32_t slot = 2 * cta + (t0 == 0 ? 1u : 0u);
         for (uint32_t e = tid; e < used * (DIM / 4); e += 32 * kConsumers) {
@@ -681,31 +697,50 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
             }
         }
         if (!whole) {
-            const uint32_t c0 = cta_of(unitBegin), c1 = cta_of(unitEnd - 1);
-            __threadfence();
+            const uint32_t c0 = cta_of(w.first + kUnitCost), c1 = cta_of(w.first + kUnitCost + unitTiles - 1);
             named_barrier(1, 32 * kConsumers);
             if (tid == 0) {
+                __threadfence();  // (cumulative: for the parts that the barrier made this thread see)
                 const uint32_t n = atomicAdd(args.arrived + c0, 1u);
+                __threadfence();
                 lastPart = n == c1 - c0;
                 if (n == c1 - c0) args.arrived[c0] = 0u;
             }
             named_barrier(1, 32 * kConsumers);
             if (lastPart) {
-                __threadfence();
                 for (uint32_t e = tid; e < used * (DIM / 4); e += 32 * kConsumers) {
                     const uint32_t column = e / (DIM / 4), at = e % (DIM / 4) * 4;
                     auto slot_of = [&](uint32_t c) { return 2 * c + (c == c0 ? 1u : 0u); };
-                    float all = -INFINITY;
-                    for (uint32_t c = c0; c <= c1; ++c) all = fmaxf(all, __ldcg(args.stats + slot_of(c) * kColumns + column).x);
-                    float weights = 0.0f;
+                    // kAtOnce parts' loads in flight: one after the other they took 10 us for 37 parts
+                    constexpr uint32_t kAtOnce = 12;
+                    float all = -INFINITY, weights = 0.0f;
                     float4 sum4 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-                    for (uint32_t c = c0; c <= c1; ++c) {
-                        const float2 st = __ldcg(args.stats + slot_of(c) * kColumns + column);
-                        const float4 v = __ldcg(reinterpret_cast<const float4 *>(args.partials + ((size_t)slot_of(c) * kColumns + column) * DIM + at));
-                        const float f = st.x == -INFINITY ? (st.y != st.y ? NAN : 0.0f) : exp2_fast(st.x - all);
-                        weights = fmaf(st.y, f, weights);
-                        sum4.x = fmaf(v.x, f, sum4.x), sum4.y = fmaf(v.y, f, sum4.y), sum4.z = fmaf(v.z, f, sum4.z), sum4.w = fmaf(v.w, f, sum4.w);
+                    for (uint32_t first = c0; first <= c1; first += kAtOnce) {
+                        float2 st[kAtOnce];
+                        float4 v[kAtOnce];
+#pragma unroll
+                        for (uint32_t k = 0; k < kAtOnce; ++k) {
+                            const uint32_t c = first + k;
+                            st[k] = make_float2(-INFINITY, 0.0f);
+                            v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                            if (c <= c1) {
+                                st[k] = __ldcg(args.stats + slot_of(c) * kColumns + column);
+                                v[k] = __ldcg(reinterpret_cast<const float4 *>(args.partials + ((size_t)slot_of(c) * kColumns + column) * DIM + at));
+                            }
+                        }
+                        float next = all;
+#pragma unroll
+                        for (uint32_t k = 0; k < kAtOnce; ++k) next = fmaxf(next, st[k].x);
+                        const float keep = all == -INFINITY ? (weights != weights ? NAN : 0.0f) : exp2_fast(all - next);
+                        all = next;
+                        weights *= keep;
+                        sum4.x *= keep, sum4.y *= keep, sum4.z *= keep, sum4.w *= keep;
+#pragma unroll
+                        for (uint32_t k = 0; k < kAtOnce; ++k) {
+                            const float f = st[k].x == -INFINITY ? (st[k].y != st[k].y ? NAN : 0.0f) : exp2_fast(st[k].x - all);
+                            weights = fmaf(st[k].y, f, weights);
+                            sum4.x = fmaf(v[k].x, f, sum4.x), sum4.y = fmaf(v[k].y, f, sum4.y), sum4.z = fmaf(v[k].z, f, sum4.z), sum4.w = fmaf(v[k].w, f, sum4.w);
+                        }
                     }
                     const float f = weights == 0.0f ? 0.0f : 1.0f / weights;
                     const uint32_t global = column0 + column;
@@ -714,13 +749,9 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
                 }
             }
         }
-        x += count;
-        w.inRequest += count;
-        if (x < end) {
-            named_barrier(1, 32 * kConsumers);  // the joining buffers are free
-            if (w.inRequest == unitTiles * w.q.columnTiles * a.kvHeads) next_request(w);
-        }
-    }
+        n0 += count;
+        named_barrier(1, 32 * kConsumers);  // the joining buffers are free
+    } while (next_unit(w));
 }
 
 KernelSmemMemo rowsMemo[3][4];

@@ -704,6 +704,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                         *reinterpret_cast<uint4 *>(out + c + i) = make_uint4(pack_bf16x2(v[i] * factor, v[i + 2] * factor), pack_bf16x2(v[i + 4] * factor, v[i + 6] * factor),
                                                                              pack_bf16x2(v[i + 1] * factor, v[i + 3] * factor), pack_bf16x2(v[i + 5] * factor, v[i + 7] * factor));
                 };
+                // a part's values, four of a row behind four of the next
+                auto part_at = [&](uint32_t n, uint32_t c) { return reinterpret_cast<float4 *>(args.partials) + ((size_t)n * (DIM / 4) + c / 4) * kRows + row; };
                 const float factor = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll 1
                 for (uint32_t c = 32 * wg; c < DIM; c += 32 * kRowGroups) {
@@ -713,9 +715,9 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                     if (there && whole) {
                         write_32(c, reinterpret_cast<const float(&)[32]>(o), factor);
                     } else if (there) {
-                        float4 *to = reinterpret_cast<float4 *>(args.partials + ((size_t)part * kRows + row) * DIM + c);
+                        float4 *to = part_at(part, c);
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) to[k] = make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]), __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
+                        for (int k = 0; k < 8; ++k) to[k * kRows] = make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]), __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
                     }
                 }
                 tc_fence_before();  // (the next unit's products overwrite O once both warpgroups have brought their queries)
@@ -734,8 +736,10 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                         __threadfence();
                         auto part_of = [&](uint32_t c) { return 2 * c + (c == c0 ? 1u : 0u); };
                         float all = -INFINITY, weights = 0.0f;
+#pragma unroll 8
                         for (uint32_t c = c0; c <= c1; ++c) all = fmaxf(all, __ldcg(args.stats + part_of(c) * kRows + row).x);
                         auto weight_of = [&](const float2 &st) { return st.x == -INFINITY ? (st.y != st.y ? NAN : 0.0f) : exp2_fast(st.x - all); };
+#pragma unroll 8
                         for (uint32_t c = c0; c <= c1; ++c) {
                             const float2 st = __ldcg(args.stats + part_of(c) * kRows + row);
                             weights = fmaf(st.y, weight_of(st), weights);
@@ -746,12 +750,13 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                             float v[32];
 #pragma unroll
                             for (int k = 0; k < 32; ++k) v[k] = 0.0f;
+#pragma unroll 2
                             for (uint32_t c = c0; c <= c1; ++c) {
                                 const float g = weight_of(__ldcg(args.stats + part_of(c) * kRows + row));
-                                const float4 *from = reinterpret_cast<const float4 *>(args.partials + ((size_t)part_of(c) * kRows + row) * DIM + d);
+                                const float4 *from = part_at(part_of(c), d);
 #pragma unroll
                                 for (int k = 0; k < 8; ++k) {
-                                    const float4 t = __ldcg(from + k);
+                                    const float4 t = __ldcg(from + k * kRows);
                                     v[4 * k] = fmaf(t.x, g, v[4 * k]), v[4 * k + 1] = fmaf(t.y, g, v[4 * k + 1]);
                                     v[4 * k + 2] = fmaf(t.z, g, v[4 * k + 2]), v[4 * k + 3] = fmaf(t.w, g, v[4 * k + 3]);
                                 }
