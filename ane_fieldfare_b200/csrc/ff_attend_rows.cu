@@ -27,6 +27,7 @@ namespace {
 
 constexpr int kConsumers = 4;                      // warps that compute: two a tile, 32 keys each
 constexpr int kRowsThreads = 32 * (kConsumers + 1);
+constexpr float kNone = -1e30f;                    // the maximum of no logit: any is above it, and 2^(it - any) is 0
 constexpr uint32_t kUnitCost = 8;                 // tiles' time that a unit takes besides its tiles
 static_assert(kTileKeys == 64 && kConsumers == 4, "two warps a tile, 32 keys each");
 
@@ -48,6 +49,12 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// the first product of a sum
+__device__ __forceinline__ void mma_f16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 __device__ __forceinline__ uint32_t transposed(uint32_t x) {
     uint32_t y;
@@ -307,10 +314,13 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
         const uint32_t key = warpKey + 16 * sub;
         subRow[sub] = key + ((key >> args.pieceShift) << args.pieceShift);
     }
-    const uint32_t kOff = keyA * CB + ((t * 8) ^ chunk_flip<DIM>(keyA));
-    uint32_t vOff[2];  // the P fragments' keys 2t and 2t + 1; those + 8 follow
+    uint32_t kOff[NG], vOff[2][NG];  // in a subtile, by group; the P fragments' keys 2t and 2t + 1; those + 8 follow
 #pragma unroll
-    for (int i = 0; i < 2; ++i) vOff[i] = (key_of_row<DIM>(2 * t + i) + vStep) * CB + ((g * 4) ^ chunk_flip<DIM>(key_of_row<DIM>(2 * t + i)));
+    for (int G = 0; G < NG; ++G) {
+        kOff[G] = keyA * CB + ((G * 32 + t * 8) ^ chunk_flip<DIM>(keyA));
+#pragma unroll
+        for (int i = 0; i < 2; ++i) vOff[i][G] = (key_of_row<DIM>(2 * t + i) + vStep) * CB + ((G * 32 + g * 4) ^ chunk_flip<DIM>(key_of_row<DIM>(2 * t + i)));
+    }
     // Value scales are converted once, a pair of keys (rows 2j, 2j + 1 of a subtile) and group to a lane, and handed round:
     // lane (and element e) = subtile * 8 + j, group = 2 e + lane / 16 (dim 64: lanes from 16 on repeat)
     constexpr int kPairs = NG == 4 ? 2 : 1;
@@ -383,6 +393,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
 
         float o[NG][4][NT][4], extra[NT][4], top[NT][2];
         int E = -120;
+        float toE = power_of_two(120);  // 2^-E
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
 #pragma unroll
@@ -393,7 +404,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
                     for (int i = 0; i < 4; ++i) o[G][v][n][i] = 0.0f;
 #pragma unroll
             for (int i = 0; i < 4; ++i) extra[n][i] = 0.0f;
-            top[n][0] = top[n][1] = -INFINITY;
+            top[n][0] = top[n][1] = kNone;
         }
         const int pFirst = w.q.p0 + (int)(column0 / group), pLast = w.q.p0 + (int)((min(columns, column0 + kColumns) - 1) / group);
 
@@ -428,7 +439,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
             }
             uint32_t pairScale[kPairs], pairBias[kPairs];
             auto convert = [&] {
-                const float f = power_of_two(-E);
+                const float f = toE;
                 uint32_t most = 0;
 #pragma unroll
                 for (int e = 0; e < kPairs; ++e) {
@@ -436,9 +447,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
                     pairBias[e] = pack_f16(high16(pairs[e][0]) * f, high16(pairs[e][1]) * f);
                     most = max_f16x2(most, max_f16x2(pairScale[e], pairBias[e] & 0x7FFF7FFFu));
                 }
-                // beyond 2^6, or NaN
-                const __half2 m = *reinterpret_cast<const __half2 *>(&most);
-                return !(__low2float(m) <= 64.0f && __high2float(m) <= 64.0f);
+                return __vmaxu2(most, 0x54005400u) != 0x54005400u;  // beyond 2^6, or NaN
             };
             uint32_t broken[2] = {0u, 0u};  // lanes whose pair's first, second key has a value that is no number
             if (__any_sync(0xFFFFFFFFu, convert())) {
@@ -468,6 +477,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
                         extra[n][1] *= f;
                     }
                     E = raised;
+                    toE = power_of_two(-E);
                 }
                 convert();
             }
@@ -479,18 +489,16 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
                 uint32_t kWords[2][NG];
                 lds_words<NG>(base + kKeyWords + (subRow[sub] + keyA) * WB, kWords[0]);
                 lds_words<NG>(base + kKeyWords + (subRow[sub] + keyA + 8) * WB, kWords[1]);
-                const uint32_t row = base + subRow[sub] * CB + kOff;
+                const uint32_t row = base + subRow[sub] * CB;
 #pragma unroll
                 for (int n = 0; n < NT; ++n) s[sub][n][0] = s[sub][n][1] = s[sub][n][2] = s[sub][n][3] = 0.0f;
 #pragma unroll
                 for (int G = 0; G < NG; ++G) {
-                    const uint2 wa = lds64(row ^ (uint32_t)(G * 32)), wb = lds64((row ^ (uint32_t)(G * 32)) + 8 * CB);
+                    const uint2 wa = lds64(row + kOff[G]), wb = lds64(row + kOff[G] + 8 * CB);
                     const uint32_t ax = wa.x >> 8, ay = wa.y >> 8, bx = wb.x >> 8, by = wb.y >> 8;
                     float acc[NT][4];
 #pragma unroll
-                    for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) mma_f16(acc[n], nibbles<0>(wa.x, ax), nibbles<0>(wb.x, bx), nibbles<0>(wa.y, ay), nibbles<0>(wb.y, by), qf[G][0][n][0], qf[G][0][n][1]);
+                    for (int n = 0; n < NT; ++n) mma_f16_first(acc[n], nibbles<0>(wa.x, ax), nibbles<0>(wb.x, bx), nibbles<0>(wa.y, ay), nibbles<0>(wb.y, by), qf[G][0][n][0], qf[G][0][n][1]);
 #pragma unroll
                     for (int n = 0; n < NT; ++n) mma_f16(acc[n], nibbles<1>(wa.x, ax), nibbles<1>(wb.x, bx), nibbles<1>(wa.y, ay), nibbles<1>(wb.y, by), qf[G][1][n][0], qf[G][1][n][1]);
 #pragma unroll
@@ -547,7 +555,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
 #pragma unroll
                     for (int c = 0; c < 2; ++c) {
                         const float next = fmaxf(top[n][c], most[n][c]);
-                        f[c] = top[n][c] == -INFINITY ? 0.0f : exp2_fast(top[n][c] - next);
+                        f[c] = exp2_fast(top[n][c] - next);
                         top[n][c] = next;
                     }
 #pragma unroll
@@ -563,12 +571,11 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
             uint32_t p[2][NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-                const float m0 = top[n][0] == -INFINITY ? 0.0f : top[n][0], m1 = top[n][1] == -INFINITY ? 0.0f : top[n][1];
 #pragma unroll
                 for (int sub = 0; sub < 2; ++sub)
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
-                        p[sub][n][h] = transposed(pack_f16(exp2_fast(fmaf(s[sub][n][2 * h], toLog2[n][0], -m0)), exp2_fast(fmaf(s[sub][n][2 * h + 1], toLog2[n][1], -m1))));
+                        p[sub][n][h] = transposed(pack_f16(exp2_fast(fmaf(s[sub][n][2 * h], toLog2[n][0], -top[n][0])), exp2_fast(fmaf(s[sub][n][2 * h + 1], toLog2[n][1], -top[n][1]))));
             }
 
             // ---- values; row 8 of the last product adds up the weights, rows 0 .. NG - 1 the biases ----
@@ -588,13 +595,13 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
                 }
 #pragma unroll
                 for (int n = 0; n < NT; ++n) mma_f16(extra[n], bias[0], ones, bias[1], ones, p[sub][n][0], p[sub][n][1]);
-                const uint32_t rows0 = base + subRow[sub] * CB + vOff[0], rows1 = base + subRow[sub] * CB + vOff[1];
+                const uint32_t row = base + subRow[sub] * CB;
 #pragma unroll
                 for (int G = 0; G < NG; ++G) {
                     uint32_t lo[2], hi[2], scale[2];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
-                        const uint32_t wa = lds32((rows0 ^ (uint32_t)(G * 32)) + 8 * h * CB), wb = lds32((rows1 ^ (uint32_t)(G * 32)) + 8 * h * CB);
+                        const uint32_t wa = lds32(row + vOff[0][G] + 8 * h * CB), wb = lds32(row + vOff[1][G] + 8 * h * CB);
                         lo[h] = __byte_perm(wa, wb, 0x5410);
                         hi[h] = __byte_perm(wa, wb, 0x7632);
                         scale[h] = __shfl_sync(0xFFFFFFFFu, pairScale[NG == 4 ? G / 2 : 0], (G & 1) * 16 + 8 * sub + 4 * h + t);
@@ -653,7 +660,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
                         float all = joinStats[0][column].x;
 #pragma unroll
                         for (int k = 1; k < kConsumers; ++k) all = fmaxf(all, joinStats[k][column].x);
-                        const float f = top[n][c] == -INFINITY ? 0.0f : exp2_fast(top[n][c] - all);
+                        const float f = exp2_fast(top[n][c] - all);
 #pragma unroll
                         for (int G = 0; G < NG; ++G) {
                             const float bias = joinBias[warp][G][column];
@@ -684,7 +691,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
 #pragma unroll
             for (int k = 1; k < kConsumers; ++k) all = fmaxf(all, joinStats[k][column].x);
 #pragma unroll
-            for (int k = 0; k < kConsumers; ++k) weights += joinStats[k][column].x == -INFINITY ? (joinStats[k][column].y != joinStats[k][column].y ? NAN : 0.0f) : joinStats[k][column].y * exp2_fast(joinStats[k][column].x - all);
+            for (int k = 0; k < kConsumers; ++k) weights += joinStats[k][column].y * exp2_fast(joinStats[k][column].x - all);
             const float4 sum4 = make_float4(u.x + v.x, u.y + v.y, u.z + v.z, u.w + v.w);
             if (whole) {
                 const float f = weights == 0.0f ? 0.0f : 1.0f / weights;
@@ -713,7 +720,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
                     auto slot_of = [&](uint32_t c) { return 2 * c + (c == c0 ? 1u : 0u); };
                     // kAtOnce parts' loads in flight: one after the other they took 10 us for 37 parts
                     constexpr uint32_t kAtOnce = 12;
-                    float all = -INFINITY, weights = 0.0f;
+                    float all = kNone, weights = 0.0f;
                     float4 sum4 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                     for (uint32_t first = c0; first <= c1; first += kAtOnce) {
                         float2 st[kAtOnce];
@@ -721,7 +728,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
 #pragma unroll
                         for (uint32_t k = 0; k < kAtOnce; ++k) {
                             const uint32_t c = first + k;
-                            st[k] = make_float2(-INFINITY, 0.0f);
+                            st[k] = make_float2(kNone, 0.0f);
                             v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
                             if (c <= c1) {
                                 st[k] = __ldcg(args.stats + slot_of(c) * kColumns + column);
@@ -731,13 +738,13 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
                         float next = all;
 #pragma unroll
                         for (uint32_t k = 0; k < kAtOnce; ++k) next = fmaxf(next, st[k].x);
-                        const float keep = all == -INFINITY ? (weights != weights ? NAN : 0.0f) : exp2_fast(all - next);
+                        const float keep = exp2_fast(all - next);
                         all = next;
                         weights *= keep;
                         sum4.x *= keep, sum4.y *= keep, sum4.z *= keep, sum4.w *= keep;
 #pragma unroll
                         for (uint32_t k = 0; k < kAtOnce; ++k) {
-                            const float f = st[k].x == -INFINITY ? (st[k].y != st[k].y ? NAN : 0.0f) : exp2_fast(st[k].x - all);
+                            const float f = exp2_fast(st[k].x - all);
                             weights = fmaf(st[k].y, f, weights);
                             sum4.x = fmaf(v[k].x, f, sum4.x), sum4.y = fmaf(v[k].y, f, sum4.y), sum4.z = fmaf(v[k].z, f, sum4.z), sum4.w = fmaf(v[k].w, f, sum4.w);
                         }
