@@ -27,7 +27,6 @@ namespace {
 
 constexpr int kConsumers = 4;                      // warps that compute: two a tile, 32 keys each
 constexpr int kRowsThreads = 32 * (kConsumers + 1);
-constexpr float kNone = -1e30f;                    // the maximum of no logit: any is above it, and 2^(it - any) is 0
 constexpr uint32_t kUnitCost = 8;                 // tiles' time that a unit takes besides its tiles
 static_assert(kTileKeys == 64 && kConsumers == 4, "two warps a tile, 32 keys each");
 

@@ -124,6 +124,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
     __shared__ uint32_t holes[kPacked], broken[kInfo][2], hidden[kInfo][2];
     __shared__ int exponents[kInfo][2];
     __shared__ float mostShared[2][kRowGroups][kRows], sumShared[kRowGroups][kRows];
+    __shared__ uint32_t largestShared[kRowGroups][kRows];
     __shared__ uint32_t aboveShared[2][kRowGroups][4];
     const AttendArgs &a = args.a;
     const uint32_t tid = threadIdx.x, warp = (uint32_t)warp_index(), lane = tid & 31u;
@@ -573,39 +574,49 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                 const bool there = token < w.q.tokens;
                 const uint32_t head = w.head * group + row % group;
                 const int p = w.q.p0 + (int)token, pLast = w.q.p0 + (int)w.q.tokens - 1;
-                // queries: f16 at a power of two of the row's largest value; runs of eight in the order of the tiles' codes;
-                // either warpgroup half of them
+                auto meet = [&] {  // of both warpgroups
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(barJoin);
+                    ok = wait_warp<false>(barJoin, joins++ & 1u, &abortFlag);
+                    return ok;
+                };
+                // queries: f16 at a power of two of the row's largest value; runs of eight in the order of the tiles' codes; either
+                // warpgroup half of a row, all its loads in flight
                 float toLog2;
                 {
-                    const uint4 *src = reinterpret_cast<const uint4 *>(a.q + (size_t)(w.q.firstRow + (there ? token : 0u)) * a.qStride + head * DIM);
+                    const uint4 *src = reinterpret_cast<const uint4 *>(a.q + (size_t)(w.q.firstRow + (there ? token : 0u)) * a.qStride + head * DIM) + wg * (DIM / 16);
+                    uint4 v[DIM / 16];
                     uint32_t largest = 0;
-#pragma unroll 8
-                    for (uint32_t i = 0; i < DIM / 8; ++i) {
-                        const uint4 v = there ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
-                        largest = __vmaxu2(largest, __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu)));
-                    }
-                    const uint32_t exponent = max(max(largest & 0xFFFFu, largest >> 16) >> 7, 7u);
+#pragma unroll
+                    for (uint32_t i = 0; i < DIM / 16; ++i) v[i] = there ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+                    for (uint32_t i = 0; i < DIM / 16; ++i)
+                        largest = __vmaxu2(largest, __vmaxu2(__vmaxu2(v[i].x & 0x7FFF7FFFu, v[i].y & 0x7FFF7FFFu), __vmaxu2(v[i].z & 0x7FFF7FFFu, v[i].w & 0x7FFF7FFFu)));
+                    largest = max(largest & 0xFFFFu, largest >> 16) >> 7;
+                    largestShared[wg][row] = largest;
+                    if (!meet()) break;
+                    const uint32_t exponent = max(max(largest, largestShared[wg ^ 1u][row]), 7u);
                     const float down = __uint_as_float((261u - exponent) << 23);  // the largest is 2^7 .. 2^8
                     toLog2 = a.scale * 1.4426950408889634f * power_of_two((int)exponent - 134);
-#pragma unroll 1
-                    for (uint32_t c = wg; c < DIM / 32; c += kRowGroups) {
+#pragma unroll
+                    for (uint32_t c = 0; c < DIM / 64; ++c) {
                         uint32_t o[16];
 #pragma unroll
                         for (uint32_t i = 0; i < 4; ++i) {
-                            const uint4 v = there ? __ldg(src + 4 * c + i) : make_uint4(0u, 0u, 0u, 0u);
-                            o[4 * i] = pack_f16(low16(v.x) * down, low16(v.z) * down);
-                            o[4 * i + 1] = pack_f16(high16(v.x) * down, high16(v.z) * down);
-                            o[4 * i + 2] = pack_f16(low16(v.y) * down, low16(v.w) * down);
-                            o[4 * i + 3] = pack_f16(high16(v.y) * down, high16(v.w) * down);
+                            const uint4 u = v[4 * c + i];
+                            o[4 * i] = pack_f16(low16(u.x) * down, low16(u.z) * down);
+                            o[4 * i + 1] = pack_f16(high16(u.x) * down, high16(u.z) * down);
+                            o[4 * i + 2] = pack_f16(low16(u.y) * down, low16(u.w) * down);
+                            o[4 * i + 3] = pack_f16(high16(u.y) * down, high16(u.w) * down);
                         }
-                        tc_store_16cols(tmem + lanes + kColQ + 16 * c, o);
+                        tc_store_16cols(tmem + lanes + kColQ + wg * (DIM / 4) + 16 * c, o);
                     }
                     tc_wait_st();
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) mbar_arrive(barQ);
                 }
-                float top = -INFINITY, sum = 0.0f;  // the row's maximum; the sum of this half's weights, at 2^top
+                float top = kNone, sum = 0.0f;  // the row's maximum; the sum of this half's weights, at 2^top
                 for (uint32_t i = 0; i < w.count; ++i, ++tile) {
                     const uint32_t info = tile % kInfo, turn = tile & 1u;
                     if (!(ok = wait_warp<false>(barS + 8 * turn, tile >> 1 & 1u, &abortFlag))) break;
@@ -643,7 +654,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                     float part;
                     uint32_t o[16];
                     auto weigh = [&] {
-                        const float shift = top == -INFINITY ? 0.0f : (float)eV - top;
+                        const float shift = (float)eV - top;
                         float part2 = 0.0f;
                         part = 0.0f;
 #pragma unroll
@@ -657,7 +668,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                     if (!above) weigh();
                     if (!(ok = wait_warp<false>(barTop + 8 * quarter, tile & 1u, &abortFlag))) break;
                     if (above || aboveShared[turn][wg ^ 1u][quarter]) {
-                        const float next = fmaxf(top, fmaxf(most, mostShared[turn][wg ^ 1u][row])), down = top == -INFINITY ? 0.0f : exp2_fast(top - next);
+                        const float next = fmaxf(top, fmaxf(most, mostShared[turn][wg ^ 1u][row])), down = exp2_fast(top - next);
                         top = next;
                         sum *= down;
                         if (i) {  // half of O so far, once the products in flight are done
@@ -685,12 +696,6 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                 if (!ok) break;
 
                 // ---- the unit's rows, or this CTA's part of them: either warpgroup every second 32 values ----
-                auto meet = [&] {  // of both warpgroups
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(barJoin);
-                    ok = wait_warp<false>(barJoin, joins++ & 1u, &abortFlag);
-                    return ok;
-                };
                 sumShared[wg][row] = sum;
                 if (!meet() || !(ok = wait_warp<false>(barO + 8 * ((tile - 1) & 1u), (tile - 1) >> 1 & 1u, &abortFlag))) break;
                 tc_fence_after();
@@ -724,44 +729,64 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                 if (!whole) {
                     if (there && wg == 0) args.stats[part * kRows + row] = make_float2(top, sum);
                     const uint32_t c0 = cta_of(x - w.t0), c1 = cta_of(x - w.t0 + w.q.tiles - 1);
-                    __threadfence();
                     if (!meet()) break;
                     if (wg == 0 && row == 0) {
+                        __threadfence();  // (cumulative: for the parts that the barrier made this thread see)
                         const uint32_t n = atomicAdd(args.arrived + c0, 1u);
+                        __threadfence();
                         lastPart = n == c1 - c0;
                         if (n == c1 - c0) args.arrived[c0] = 0u;
                     }
                     if (!meet()) break;
-                    if (lastPart && there) {
+                    if (lastPart) {
                         __threadfence();
                         auto part_of = [&](uint32_t c) { return 2 * c + (c == c0 ? 1u : 0u); };
-                        float all = -INFINITY, weights = 0.0f;
-#pragma unroll 8
-                        for (uint32_t c = c0; c <= c1; ++c) all = fmaxf(all, __ldcg(args.stats + part_of(c) * kRows + row).x);
-                        auto weight_of = [&](const float2 &st) { return st.x == -INFINITY ? (st.y != st.y ? NAN : 0.0f) : exp2_fast(st.x - all); };
-#pragma unroll 8
-                        for (uint32_t c = c0; c <= c1; ++c) {
-                            const float2 st = __ldcg(args.stats + part_of(c) * kRows + row);
-                            weights = fmaf(st.y, weight_of(st), weights);
-                        }
-                        const float last = weights == 0.0f ? 0.0f : 1.0f / weights;
-#pragma unroll 1
-                        for (uint32_t d = 32 * wg; d < DIM; d += 32 * kRowGroups) {
-                            float v[32];
+                        // a warp 32 rows and eight of their values at a time, kAtOnce parts' loads in flight
+                        constexpr uint32_t kAtOnce = 6;
+                        const uint32_t used = w.q.tokens * group, blocks = (used + 31) / 32;
+                        for (uint32_t item = warp - kFirstRowWarp; item < blocks * (DIM / 8); item += kRowWarps) {
+                            const uint32_t mine = item % blocks * 32 + lane, d = item / blocks * 8;
+                            if (mine >= used) continue;
+                            float all = kNone, weights = 0.0f, v[8];
 #pragma unroll
-                            for (int k = 0; k < 32; ++k) v[k] = 0.0f;
-#pragma unroll 2
-                            for (uint32_t c = c0; c <= c1; ++c) {
-                                const float g = weight_of(__ldcg(args.stats + part_of(c) * kRows + row));
-                                const float4 *from = part_at(part_of(c), d);
+                            for (int k = 0; k < 8; ++k) v[k] = 0.0f;
+                            for (uint32_t from = c0; from <= c1; from += kAtOnce) {
+                                float2 st[kAtOnce];
+                                float4 t[kAtOnce][2];
 #pragma unroll
-                                for (int k = 0; k < 8; ++k) {
-                                    const float4 t = __ldcg(from + k * kRows);
-                                    v[4 * k] = fmaf(t.x, g, v[4 * k]), v[4 * k + 1] = fmaf(t.y, g, v[4 * k + 1]);
-                                    v[4 * k + 2] = fmaf(t.z, g, v[4 * k + 2]), v[4 * k + 3] = fmaf(t.w, g, v[4 * k + 3]);
+                                for (uint32_t k = 0; k < kAtOnce; ++k) {
+                                    const uint32_t n = part_of(from + k);
+                                    st[k] = make_float2(kNone, 0.0f);
+                                    t[k][0] = t[k][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                                    if (from + k <= c1) {
+                                        st[k] = __ldcg(args.stats + n * kRows + mine);
+                                        const float4 *at = reinterpret_cast<const float4 *>(args.partials) + ((size_t)n * (DIM / 4) + d / 4) * kRows + mine;
+                                        t[k][0] = __ldcg(at);
+                                        t[k][1] = __ldcg(at + kRows);
+                                    }
+                                }
+                                float next = all;
+#pragma unroll
+                                for (uint32_t k = 0; k < kAtOnce; ++k) next = fmaxf(next, st[k].x);
+                                const float keep = exp2_fast(all - next);
+                                all = next;
+                                weights *= keep;
+#pragma unroll
+                                for (int k = 0; k < 8; ++k) v[k] *= keep;
+#pragma unroll
+                                for (uint32_t k = 0; k < kAtOnce; ++k) {
+                                    const float g = exp2_fast(st[k].x - all);
+                                    weights = fmaf(st[k].y, g, weights);
+#pragma unroll
+                                    for (int h = 0; h < 2; ++h) {
+                                        v[4 * h] = fmaf(t[k][h].x, g, v[4 * h]), v[4 * h + 1] = fmaf(t[k][h].y, g, v[4 * h + 1]);
+                                        v[4 * h + 2] = fmaf(t[k][h].z, g, v[4 * h + 2]), v[4 * h + 3] = fmaf(t[k][h].w, g, v[4 * h + 3]);
+                                    }
                                 }
                             }
-                            write_32(d, v, last);
+                            const float f = weights == 0.0f ? 0.0f : 1.0f / weights;
+                            *reinterpret_cast<uint4 *>(a.out + (size_t)(w.q.firstRow + mine / group) * a.outStride + (w.head * group + mine % group) * DIM + d) =
+                                make_uint4(pack_bf16x2(v[0] * f, v[2] * f), pack_bf16x2(v[4] * f, v[6] * f), pack_bf16x2(v[1] * f, v[3] * f), pack_bf16x2(v[5] * f, v[7] * f));
                         }
                     }
                 }

@@ -9,6 +9,7 @@
 namespace ff {
 
 constexpr float kLazy = 8.0f;  // log2 by which a logit may pass the running maximum before outputs are rescaled
+constexpr float kNone = -1e30f;  // the maximum of no logit: any is above it, and 2^(it - any) is 0
 constexpr uint32_t kTileKeys = 64;
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, int w, uint32_t bar) {
