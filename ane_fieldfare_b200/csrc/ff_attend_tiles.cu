@@ -7,14 +7,14 @@
 // Per key tile, warp by role: two copy packed codes, keys' with the scale words and values'; one turns the tile's scale words into the pairs that
 // the expansion multiplies with; eight expand codes to f16 tiles in shared memory (128-byte swizzle, keys and values alike
 // [64 values][key][128 bytes]), four a slot, so that one group's waits stand behind the other's arithmetic; one issues the MMAs; two
-// warpgroups own half of a row's keys a thread:
+// warpgroups own a row a thread and take the tiles in turn:
 //   S = Q K^T   A: the rows' queries, in tensor memory for the whole unit (read from shared memory they would cost the
 //               128 bytes a cycle that dequantizing needs); B: the keys, K-major
 //   P = 2^(S f + E - M)   in registers, back into S's columns as f16
 //   O += P V    A: P; B: the values, N-major; O stays in tensor memory
-// The halves exchange their maxima while they form the weights with the M there is; M moves only where a row passes it by 2^8.
-// (A row a thread, with the tiles taken in turn by the two warpgroups: 2000 cycles from S to P, which two tiles of S cannot
-// hide; now 900.)
+// A tile's warpgroup waits for the maximum M that the one before it settled on, not for its weights; M moves, and O with it, only
+// where a row passes it by 2^8.  (Both warpgroups on each tile, half a row a thread, were slower: what a tile costs besides its
+// arithmetic was paid twice.)
 // Tensor memory: Q dim/2, O dim, S two tiles of 64 columns: all 512 at dim 256.
 //
 // f16 holds 11 bits of keys, values and weights where bf16 would hold 8; its range is kept by powers of two: a row's
@@ -96,6 +96,24 @@ template <bool kSleep>
 __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile uint32_t *abortFlag) {
     return __all_sync(0xFFFFFFFFu, wait_lane<kSleep>(bar, parity, abortFlag));
 }
+// two fp32 operations an instruction
+__device__ __forceinline__ unsigned long long pair_f32(float a, float b) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float first_f32(unsigned long long v) { return __uint_as_float((uint32_t)v); }
+__device__ __forceinline__ float second_f32(unsigned long long v) { return __uint_as_float((uint32_t)(v >> 32)); }
+__device__ __forceinline__ unsigned long long fma_f32x2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ unsigned long long add_f32x2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
 __device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c) {
     uint32_t r;
     asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
@@ -117,15 +135,14 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
     constexpr uint32_t kGroupWarps = DIM == 64 ? 2 : 4, kGroups = kDequantWarps / kGroupWarps, kUnitsEach = kUnits / (32 * kGroupWarps);
     constexpr uint32_t kColQ = 0, kColO = DIM / 2, kColS = kColO + DIM;
     extern __shared__ uint8_t tilesSmem[];
-    __shared__ __align__(8) uint64_t barriers[2 * kSlots + 4 * kPacked + 2 * kInfo + 2 + 2 + 2 + 1 + 1 + 4];
+    __shared__ __align__(8) uint64_t barriers[2 * kSlots + 4 * kPacked + 2 * kInfo + 2 + 4 + 2 + 1 + 1 + 8];
     __shared__ uint32_t tmemSlot, lastPart;
     __shared__ volatile uint32_t abortFlag;
     __shared__ uint32_t firstTile[kTilesThreads + 1], firstWork[kTilesThreads + 1], warpSums[32];
     __shared__ uint32_t holes[kPacked], broken[kInfo][2], hidden[kInfo][2];
-    __shared__ int exponents[kInfo][2];
-    __shared__ float mostShared[2][kRowGroups][kRows], sumShared[kRowGroups][kRows];
+    __shared__ float4 tileInfo[kInfo];
+    __shared__ float topShared[kRows], sumShared[kRowGroups][kRows], refShared[kRowGroups][kRows];
     __shared__ uint32_t largestShared[kRowGroups][kRows];
-    __shared__ uint32_t aboveShared[2][kRowGroups][4];
     const AttendArgs &a = args.a;
     const uint32_t tid = threadIdx.x, warp = (uint32_t)warp_index(), lane = tid & 31u;
     const uint32_t slots = (sm_addr(tilesSmem) + 1023u) & ~1023u, packed = slots + kSlots * kSlot, scales = packed + 2 * kPacked * kPack, words = scales + kInfo * words_bytes(DIM);
@@ -133,7 +150,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
     const uint32_t bar0 = sm_addr(barriers);
     const uint32_t barTile = bar0, barTileFree = barTile + 8 * kSlots, barPack = barTileFree + 8 * kSlots, barPackFree = barPack + 16 * kPacked;  // keys', then values'
     const uint32_t barInfo = barPackFree + 16 * kPacked, barInfoFree = barInfo + 8 * kInfo;
-    const uint32_t barS = barInfoFree + 8 * kInfo, barP = barS + 16, barO = barP + 16, barQ = barO + 16, barJoin = barQ + 8, barTop = barJoin + 8;
+    const uint32_t barS = barInfoFree + 8 * kInfo, barP = barS + 16, barO = barP + 32, barQ = barO + 16, barJoin = barQ + 8, barTop = barJoin + 8;
     if (tid == 0) {
         abortFlag = 0;
         for (uint32_t s = 0; s < kSlots; ++s) {
@@ -150,12 +167,13 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
         }
         for (uint32_t s = 0; s < 2; ++s) {
             mbar_init(barS + 8 * s, 1);
-            mbar_init(barP + 8 * s, kRowWarps);
+            mbar_init(barP + 16 * s, 4);  // the first 32 keys' weights
+            mbar_init(barP + 16 * s + 8, 4);
             mbar_init(barO + 8 * s, 1);
         }
         mbar_init(barQ, kRowWarps);
         mbar_init(barJoin, kRowWarps);
-        for (uint32_t s = 0; s < 4; ++s) mbar_init(barTop + 8 * s, kRowGroups);
+        for (uint32_t s = 0; s < 8; ++s) mbar_init(barTop + 8 * s, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == (uint32_t)kMmaWarp) {
@@ -412,13 +430,20 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                 for (uint32_t i = 0; i < w.count && ok; ++i, ++tile) {
                     if (i + 1 < w.count && !(ok = scores(tile + 1))) break;
                     if (!(ok = wait_warp<false>(barTile + 8 * slot, phase, &abortFlag))) break;
-                    if (!(ok = wait_warp<false>(barP + 8 * (tile & 1u), tile >> 1 & 1u, &abortFlag))) break;
+                    if (!(ok = wait_warp<false>(barP + 16 * (tile & 1u), tile >> 1 & 1u, &abortFlag))) break;
                     tc_fence_after();
                     const uint64_t desc = desc_sw128(slots + slot * kSlot, kTileKeys * 128);
                     const uint32_t p = tmem + kColS + (tile & 1u) * kTileKeys;
                     if (elect_one()) {
 #pragma unroll
-                        for (uint32_t k = 0; k < kTileKeys / 16; ++k) mma_a_tmem(tmem + kColO, p + 8 * k, desc + k * (2048 >> 4), idescO, (i | k) != 0);
+                        for (uint32_t k = 0; k < kTileKeys / 32; ++k) mma_a_tmem(tmem + kColO, p + 8 * k, desc + k * (2048 >> 4), idescO, (i | k) != 0);
+                    }
+                    __syncwarp();
+                    if (!(ok = wait_warp<false>(barP + 16 * (tile & 1u) + 8, tile >> 1 & 1u, &abortFlag))) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+#pragma unroll
+                        for (uint32_t k = kTileKeys / 32; k < kTileKeys / 16; ++k) mma_a_tmem(tmem + kColO, p + 8 * k, desc + k * (2048 >> 4), idescO, 1u);
                         commit(barTileFree + 8 * slot);
                         commit(barO + 8 * (tile & 1u));
                         commit(barInfoFree + 8 * (tile % kInfo));  // weights formed, values expanded: nobody looks at the tile's scales any more
@@ -431,7 +456,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                 if (x < end) next_segment(w, x);
             }
         } else if (warp == (uint32_t)kScaleWarp) {
-            // ---------------- scales: a lane two keys of a tile ----------------
+            // ---------------- scales: a lane two neighbouring keys of a tile ----------------
             // What no row sees is nothing; a visible key with a value that is no number is marked, and so is one whose page is
             // outside the cache.  A group's word for the expansion: f16 scale * 2^(24 - E) | f16 bias * 2^-E, the largest of
             // 16 scale and |bias| of the tile 2^-6 .. 2^-5.
@@ -442,59 +467,71 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                 const int pLast = w.q.p0 + (int)w.q.tokens - 1;
                 for (uint32_t i = 0; i < w.count; ++i, ++tile) {
                     const uint32_t at = tile % kPacked, info = tile % kInfo;
+                    const int j0 = (int)key_at(w.q, w.t0 + i);
                     if (!(ok = wait_warp<true>(barPack + 8 * at, tile / kPacked & 1u, &abortFlag))) break;
-                    const uint32_t gone = holes[at];
-                    uint32_t v[2][2][NG];  // [keys, values][lane's key][group]
-                    uint32_t bad[2], out[2];
+                    // keys that some row does not see, or on a page outside the cache
+                    const uint32_t gone = holes[at] & ((1u << pieces) - 1u);
+                    const bool unseen = gone || j0 + (int)kTileKeys - 1 > w.q.p0 || (a.window && (long long)j0 <= (long long)pLast - a.window && (uint32_t)j0 + kTileKeys > a.sinks);
+                    uint32_t v[2][2][NG];  // [keys, values][the lane's key][group]
+                    const uint32_t key0 = 2 * lane, from = words + at * words_bytes(DIM) + (((key0 >> args.pieceShift) * 2) << args.pieceShift) * WB + (key0 & (pieceKeys - 1u)) * WB;  // of a piece: keys' words, then values'
+                    uint32_t most[2] = {0u, 0u};  // magnitudes of scales and biases
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint32_t key = lane + 32 * h;
-                        const int j = (int)(key_at(w.q, w.t0 + i) + key), p = max(j, w.q.p0);  // of the rows that may see it, the one whose window goes back furthest
-                        const bool hole = gone >> (key >> args.pieceShift) & 1u;
-                        const bool seen = p <= pLast && (!a.window || (long long)j > (long long)p - a.window || (uint32_t)j < a.sinks);
-                        bool none = false;
+                    for (int side = 0; side < 2; ++side)
 #pragma unroll
-                        for (int side = 0; side < 2; ++side) {
-                            // (of a piece: the keys' words, then the values')
-                            lds_words<NG>(words + at * words_bytes(DIM) + (((key >> args.pieceShift) * 2 + side) << args.pieceShift) * WB + (key & (pieceKeys - 1u)) * WB, v[side][h]);
+                        for (int h = 0; h < 2; ++h) {
+                            lds_words<NG>(from + ((side << args.pieceShift) + h) * WB, v[side][h]);
 #pragma unroll
-                            for (int G = 0; G < NG; ++G) none |= is_broken(v[side][h][G]);
+                            for (int G = 0; G < NG; ++G) most[side] = __vmaxu2(most[side], v[side][h][G] & 0x7FFF7FFFu);
                         }
-                        bad[h] = __ballot_sync(0xFFFFFFFFu, seen && !hole && none);
-                        out[h] = __ballot_sync(0xFFFFFFFFu, seen && hole);
-                        if (!seen || hole || none)
+                    auto none = [](uint32_t m) { return max(m & 0xFFFFu, m >> 16) >= 0x7F80u; };
+                    uint32_t bad[2] = {0u, 0u}, out[2] = {0u, 0u};  // bit l: key 2 l, key 2 l + 1
+                    if (__any_sync(0xFFFFFFFFu, unseen || none(most[0]) || none(most[1]))) {
+                        most[0] = most[1] = 0u;
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int j = j0 + (int)key0 + h, p = max(j, w.q.p0);  // of the rows that may see it, the one whose window goes back furthest
+                            const bool hole = gone >> (key0 >> args.pieceShift) & 1u;
+                            const bool seen = p <= pLast && (!a.window || (long long)j > (long long)p - a.window || (uint32_t)j < a.sinks);
+                            bool broke = false;
 #pragma unroll
                             for (int side = 0; side < 2; ++side)
 #pragma unroll
-                                for (int G = 0; G < NG; ++G) v[side][h][G] = 0u;
-                    }
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(barPackFree + 8 * at);
-                    if (!(ok = wait_warp<true>(barInfoFree + 8 * info, tile / kInfo & 1u ^ 1u, &abortFlag))) break;
+                                for (int G = 0; G < NG; ++G) broke |= is_broken(v[side][h][G]);
+                            bad[h] = __ballot_sync(0xFFFFFFFFu, seen && !hole && broke);
+                            out[h] = __ballot_sync(0xFFFFFFFFu, seen && hole);
 #pragma unroll
-                    for (int side = 0; side < 2; ++side) {
-                        uint32_t most = 0;
+                            for (int side = 0; side < 2; ++side)
 #pragma unroll
-                        for (int h = 0; h < 2; ++h)
-#pragma unroll
-                            for (int G = 0; G < NG; ++G) most = max(most, word_exponent(v[side][h][G]));
-                        most = __reduce_max_sync(0xFFFFFFFFu, most);
-                        const int E = min(max((int)most - 127 + 6, -120), 120);
-                        const float f = power_of_two(-E);
-#pragma unroll
-                        for (int h = 0; h < 2; ++h)
-#pragma unroll
-                            for (int G = 0; G < NG; ++G)
-                                sts32(scales + info * words_bytes(DIM) + side * kWordSide + (G * kTileKeys + lane + 32 * h) * 4,
-                                      pack_f16(low16(v[side][h][G]) * f * 0x1p24f, high16(v[side][h][G]) * f));
-                        if (lane == 0) {
-                            exponents[info][side] = E;
-                            broken[info][side] = bad[side];
-                            hidden[info][side] = out[side];
+                                for (int G = 0; G < NG; ++G) {
+                                    if (!seen || hole || broke) v[side][h][G] = 0u;
+                                    most[side] = __vmaxu2(most[side], v[side][h][G] & 0x7FFF7FFFu);
+                                }
                         }
                     }
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(barInfo + 8 * info);
+                    if (lane == 0) mbar_arrive(barPackFree + 8 * at);
+                    int exponent[2];
+#pragma unroll
+                    for (int side = 0; side < 2; ++side) {
+                        const uint32_t largest = __reduce_max_sync(0xFFFFFFFFu, max(((most[side] & 0xFFFFu) >> 7) + 4u, most[side] >> 23));
+                        exponent[side] = min(max((int)largest - 127 + 6, -100), 120);
+                    }
+                    if (!(ok = wait_warp<true>(barInfoFree + 8 * info, tile / kInfo & 1u ^ 1u, &abortFlag))) break;
+#pragma unroll
+                    for (int side = 0; side < 2; ++side) {
+                        const float toBias = power_of_two(-exponent[side]), toScale = power_of_two(24 - exponent[side]);
+#pragma unroll
+                        for (int G = 0; G < NG; ++G)
+                            sts64(scales + info * words_bytes(DIM) + side * kWordSide + (G * kTileKeys + key0) * 4, pack_f16(low16(v[side][0][G]) * toScale, high16(v[side][0][G]) * toBias),
+                                  pack_f16(low16(v[side][1][G]) * toScale, high16(v[side][1][G]) * toBias));
+                    }
+                    __syncwarp();
+                    if (lane == 0) {
+                        tileInfo[info] = make_float4(power_of_two(exponent[0]), (float)exponent[1], power_of_two(-exponent[1]), unseen || (bad[0] | bad[1]) ? 1.0f : 0.0f);
+                        broken[info][0] = bad[0], broken[info][1] = bad[1];
+                        hidden[info][0] = out[0], hidden[info][1] = out[1];
+                        mbar_arrive(barInfo + 8 * info);
+                    }
                 }
                 x += w.count;
                 if (ok && x < end) next_segment(w, x);
@@ -573,7 +610,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                 const uint32_t token = row / group;
                 const bool there = token < w.q.tokens;
                 const uint32_t head = w.head * group + row % group;
-                const int p = w.q.p0 + (int)token, pLast = w.q.p0 + (int)w.q.tokens - 1;
+                const int p = w.q.p0 + (int)token;
                 auto meet = [&] {  // of both warpgroups
                     __syncwarp();
                     if (lane == 0) mbar_arrive(barJoin);
@@ -616,66 +653,55 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                     __syncwarp();
                     if (lane == 0) mbar_arrive(barQ);
                 }
-                float top = kNone, sum = 0.0f;  // the row's maximum; the sum of this half's weights, at 2^top
-                for (uint32_t i = 0; i < w.count; ++i, ++tile) {
-                    const uint32_t info = tile % kInfo, turn = tile & 1u;
-                    if (!(ok = wait_warp<false>(barS + 8 * turn, tile >> 1 & 1u, &abortFlag))) break;
+                float ref = kNone, sum = 0.0f;  // the warpgroup's part of the weights' sum, at 2^ref
+                uint32_t i = (tile ^ wg) & 1u;  // the segment's first tile of this warpgroup
+                for (tile += i; i < w.count; i += 2, tile += 2) {
+                    const uint32_t info = tile % kInfo;
+                    if (!(ok = wait_warp<false>(barS + 8 * wg, tile >> 1 & 1u, &abortFlag))) break;
                     tc_fence_after();
-                    const uint32_t s0 = tmem + lanes + kColS + turn * kTileKeys;
-                    uint32_t bits[32];
-                    tc_load_32cols(s0 + 32 * wg, bits);
-                    const int eK = exponents[info][0], eV = exponents[info][1];
-                    const uint32_t bad = broken[info][wg], gone = hidden[info][wg];
-                    const int tileKey = (int)key_at(w.q, w.t0 + i), j0 = tileKey + 32 * (int)wg;
+                    const uint32_t s0 = tmem + lanes + kColS + wg * kTileKeys;
+                    uint32_t lo[32], hi[32];
+                    tc_load_32cols(s0, lo);
+                    tc_load_32cols(s0 + 32, hi);
+                    const float4 about = tileInfo[info];  // 2^eK, eV, 2^-eV, whether some row does not see some key
                     tc_wait_ld();
-                    float *s = reinterpret_cast<float *>(bits);
-                    const float f = toLog2 * power_of_two(eK);
-                    if (j0 + 31 > w.q.p0 || (a.window && (long long)j0 <= (long long)pLast - a.window && (uint32_t)j0 + 32u > a.sinks) || (bad | gone)) {
-                        // the keys c of this half that the row sees: up to `most`, above `least` or below `sinks`
-                        const int most = p - j0;
-                        const int least = a.window ? (int)max((long long)p - a.window - j0, -1ll) : -1, sinks = a.window ? (int)min(max((long long)a.sinks - j0, 0ll), 32ll) : 0;
+                    float *s = reinterpret_cast<float *>(lo), *u = reinterpret_cast<float *>(hi);
+                    if (about.w != 0.0f) {
+                        // the keys c of the tile that the row sees: up to `most`, above `least` or below `sinks`
+                        const uint32_t bad0 = broken[info][0], bad1 = broken[info][1], gone0 = hidden[info][0], gone1 = hidden[info][1];
+                        const int j0 = (int)key_at(w.q, w.t0 + i), most = p - j0;
+                        const int least = a.window ? (int)max((long long)p - a.window - j0, -1ll) : -1, sinks = a.window ? (int)min(max((long long)a.sinks - j0, 0ll), 64ll) : 0;
 #pragma unroll
                         for (int c = 0; c < 32; ++c) {
-                            const bool sees = c <= most && (c > least || c < sinks) && !(gone >> c & 1u);
-                            s[c] = !sees ? -INFINITY : bad >> c & 1u ? NAN : s[c];
+                            const uint32_t bad = c % 2 ? bad1 : bad0, gone = c % 2 ? gone1 : gone0;  // bit l: key 2 l, key 2 l + 1
+                            const bool see0 = c <= most && (c > least || c < sinks) && !(gone >> (c / 2) & 1u), see1 = c + 32 <= most && (c + 32 > least || c + 32 < sinks) && !(gone >> (16 + c / 2) & 1u);
+                            s[c] = !see0 ? -INFINITY : bad >> (c / 2) & 1u ? NAN : s[c];
+                            u[c] = !see1 ? -INFINITY : bad >> (16 + c / 2) & 1u ? NAN : u[c];
                         }
                     }
-                    float most = s[0], most2 = s[1];
+                    float most[4] = {s[0], s[1], u[0], u[1]};
 #pragma unroll
-                    for (int c = 2; c < 32; c += 2) most = fmaxf(most, s[c]), most2 = fmaxf(most2, s[c + 1]);
-                    most = fmaf(fmaxf(most, most2), f, (float)eV);
-                    // Either half's maximum; the weights are formed meanwhile, and once more where a row of either half passes
-                    // its maximum by more than kLazy.
-                    const bool above = __any_sync(0xFFFFFFFFu, most > top + kLazy);
-                    mostShared[turn][wg][row] = most;
-                    if (lane == 0) aboveShared[turn][wg][quarter] = above;
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(barTop + 8 * quarter);
-                    float part;
-                    uint32_t o[16];
-                    auto weigh = [&] {
-                        const float shift = (float)eV - top;
-                        float part2 = 0.0f;
-                        part = 0.0f;
-#pragma unroll
-                        for (int c = 0; c < 32; c += 2) {
-                            const float x0 = exp2_fast(fmaf(s[c], f, shift)), x1 = exp2_fast(fmaf(s[c + 1], f, shift));
-                            part += x0, part2 += x1;
-                            o[c / 2] = pack_f16(x0, x1);
-                        }
-                        part += part2;
-                    };
-                    if (!above) weigh();
-                    if (!(ok = wait_warp<false>(barTop + 8 * quarter, tile & 1u, &abortFlag))) break;
-                    if (above || aboveShared[turn][wg ^ 1u][quarter]) {
-                        const float next = fmaxf(top, fmaxf(most, mostShared[turn][wg ^ 1u][row])), down = exp2_fast(top - next);
+                    for (int c = 2; c < 32; c += 4) {
+                        most[0] = fmaxf(fmaxf(most[0], s[c]), s[c + 2 < 32 ? c + 2 : c]);
+                        most[1] = fmaxf(fmaxf(most[1], s[c + 1]), s[c + 3 < 32 ? c + 3 : c + 1]);
+                        most[2] = fmaxf(fmaxf(most[2], u[c]), u[c + 2 < 32 ? c + 2 : c]);
+                        most[3] = fmaxf(fmaxf(most[3], u[c + 1]), u[c + 3 < 32 ? c + 3 : c + 1]);
+                    }
+                    const float f = toLog2 * about.x, peak = fmaf(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])), f, about.y);
+                    // the maximum that the tile before settled on
+                    float top = kNone;
+                    if (i) {
+                        if (!(ok = wait_warp<false>(barTop + 8 * ((wg ^ 1u) * 4 + quarter), (tile - 1) >> 1 & 1u, &abortFlag))) break;
+                        top = topShared[row];
+                    }
+                    if (__any_sync(0xFFFFFFFFu, peak > top + kLazy)) {
+                        const float next = fmaxf(top, peak), down = exp2_fast(top - next);
                         top = next;
-                        sum *= down;
-                        if (i) {  // half of O so far, once the products in flight are done
-                            if (!(ok = wait_warp<false>(barO + 8 * (turn ^ 1u), (tile - 1) >> 1 & 1u, &abortFlag))) break;
+                        if (i) {  // O so far, once the products in flight are done
+                            if (!(ok = wait_warp<false>(barO + 8 * (wg ^ 1u), (tile - 1) >> 1 & 1u, &abortFlag))) break;
                             tc_fence_after();
 #pragma unroll 1
-                            for (uint32_t c = 16 * wg; c < DIM; c += 32) {
+                            for (uint32_t c = 0; c < DIM; c += 16) {
                                 uint32_t v[16];
                                 tc_load_16cols(tmem + lanes + kColO + c, v);
                                 tc_wait_ld();
@@ -683,23 +709,53 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                                 for (int k = 0; k < 16; ++k) v[k] = __float_as_uint(__uint_as_float(v[k]) * down);
                                 tc_store_16cols(tmem + lanes + kColO + c, v);
                             }
+                            tc_wait_st();
                         }
-                        weigh();
                     }
-                    tc_store_16cols(s0 + 16 * wg, o);
-                    sum = fmaf(part, power_of_two(-eV), sum);
+                    topShared[row] = top;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(barTop + 8 * (wg * 4 + quarter));
+                    sum *= exp2_fast(ref - top);
+                    ref = top;
+                    const float shift = about.y - top;
+                    const unsigned long long f2 = pair_f32(f, f), shift2 = pair_f32(shift, shift);
+                    unsigned long long part = pair_f32(0.0f, 0.0f), part2 = part;
+                    auto weigh = [&](const float *v, uint32_t to) {  // 32 logits: weights to 16 columns
+                        uint32_t o[16];
+#pragma unroll
+                        for (int c = 0; c < 32; c += 4) {
+                            const unsigned long long x = fma_f32x2(pair_f32(v[c], v[c + 1]), f2, shift2), y = fma_f32x2(pair_f32(v[c + 2], v[c + 3]), f2, shift2);
+                            const float x0 = exp2_fast(first_f32(x)), x1 = exp2_fast(second_f32(x)), y0 = exp2_fast(first_f32(y)), y1 = exp2_fast(second_f32(y));
+                            part = add_f32x2(part, pair_f32(x0, x1));
+                            part2 = add_f32x2(part2, pair_f32(y0, y1));
+                            o[c / 2] = pack_f16(x0, x1);
+                            o[c / 2 + 1] = pack_f16(y0, y1);
+                        }
+                        tc_store_16cols(to, o);
+                    };
+                    weigh(s, s0);
                     tc_wait_st();
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(barP + 8 * turn);
+                    if (lane == 0) mbar_arrive(barP + 16 * wg);  // (the products of the first 32 keys may begin)
+                    weigh(u, s0 + 16);
+                    part = add_f32x2(part, part2);
+                    sum = fmaf(first_f32(part) + second_f32(part), about.z, sum);
+                    tc_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(barP + 16 * wg + 8);
                 }
                 if (!ok) break;
+                tile = tile - i + w.count;
 
                 // ---- the unit's rows, or this CTA's part of them: either warpgroup every second 32 values ----
                 sumShared[wg][row] = sum;
+                refShared[wg][row] = ref;
                 if (!meet() || !(ok = wait_warp<false>(barO + 8 * ((tile - 1) & 1u), (tile - 1) >> 1 & 1u, &abortFlag))) break;
                 tc_fence_after();
-                sum = sumShared[0][row] + sumShared[1][row];
+                const float top = topShared[row];
+                sum = sumShared[0][row] * exp2_fast(refShared[0][row] - top) + sumShared[1][row] * exp2_fast(refShared[1][row] - top);
                 const bool whole = w.count == w.q.tiles;
                 const uint32_t part = 2 * cta + (w.t0 == 0 ? 1u : 0u);
                 uint16_t *out = a.out + (size_t)(w.q.firstRow + (there ? token : 0u)) * a.outStride + head * DIM;
