@@ -5,7 +5,7 @@
 // per CTA, one CTA per SM.  A unit that several CTAs share is joined by whichever of them ends last, in the CTAs' order.
 //
 // Per key tile, warp by role: two copy packed codes, keys' with the scale words and values'; one turns the tile's scale words into the pairs that
-// the expansion multiplies with; eight expand codes to f16 tiles in shared memory (128-byte swizzle, keys and values alike
+// the expansion multiplies with; sixteen expand codes to f16 tiles in shared memory (128-byte swizzle, keys and values alike
 // [64 values][key][128 bytes]), four a slot, so that one group's waits stand behind the other's arithmetic; one issues the MMAs; two
 // warpgroups own a row a thread and take the tiles in turn:
 //   S = Q K^T   A: the rows' queries, in tensor memory for the whole unit (read from shared memory they would cost the
@@ -31,12 +31,12 @@ namespace ff {
 namespace {
 
 // warps by role: copies of keys, MMAs, scales, copies of values; expansion; rows
-constexpr int kKeyCopyWarp = 0, kMmaWarp = 1, kScaleWarp = 2, kValueCopyWarp = 3, kDequantWarps = 8, kRowGroups = 2;
+constexpr int kKeyCopyWarp = 0, kMmaWarp = 1, kScaleWarp = 2, kValueCopyWarp = 3, kDequantWarps = 16, kRowGroups = 2;
 constexpr int kFirstDequant = 4, kFirstRowWarp = kFirstDequant + kDequantWarps, kRowWarps = 4 * kRowGroups;
 constexpr int kTilesThreads = 32 * (kFirstRowWarp + kRowWarps);
-// registers a thread by role: together no more than the launch's 96 each
-constexpr int kRegsOthers = 64, kRegsRows = 144;
-static_assert(128 * kRegsOthers + 32 * kDequantWarps * kRegsOthers + 32 * kRowWarps * kRegsRows <= kTilesThreads * 96, "register split");
+// registers a thread by role: together no more than the launch's 72 each
+constexpr int kRegsOthers = 48, kRegsRows = 128;
+static_assert(128 * kRegsOthers + 32 * kDequantWarps * kRegsOthers + 32 * kRowWarps * kRegsRows <= kTilesThreads * 72, "register split");
 constexpr uint32_t kRows = kTileRows;
 constexpr uint32_t kInfo = 4;   // tiles whose scales and exponents are kept
 constexpr uint32_t kSlots = 4, kPacked = 3;  // expanded tiles; packed ones, of keys and of values each
@@ -79,12 +79,13 @@ __device__ __forceinline__ void mma_a_tmem(uint32_t d, uint32_t a, uint64_t b, u
 __device__ __forceinline__ void commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
+constexpr uint32_t kWaitLimit = 1u << 20;
 // The bounded waits of ff_tc_device.cuh without a call: a kernel that divides its registers among the roles has none.
 template <bool kSleep>
 __device__ __forceinline__ bool wait_lane(uint32_t bar, uint32_t parity, volatile uint32_t *abortFlag) {
     if (mbar_try_wait(bar, parity)) return true;
 #pragma unroll 1
-    for (uint32_t i = 0; i < kSpinLimit; ++i) {
+    for (uint32_t i = 0; i < kWaitLimit; ++i) {
         if (mbar_try_wait(bar, parity)) return true;
         if (kSleep) __nanosleep(40);
         if ((i & 255u) == 255u && *abortFlag) return false;
@@ -132,7 +133,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
     constexpr int NG = DIM / 64, CB = DIM / 2, WB = NG * 4;
     constexpr uint32_t kSlot = slot_bytes(DIM), kPack = packed_bytes(DIM);
     constexpr uint32_t kWordSide = words_bytes(DIM) / 2, kUnits = kTileKeys * NG;  // of a slot: a key's group of 64 values
-    constexpr uint32_t kGroupWarps = DIM == 64 ? 2 : 4, kGroups = kDequantWarps / kGroupWarps, kUnitsEach = kUnits / (32 * kGroupWarps);
+    // (no more groups than slots: one that waited for a slot two rounds ahead would take one round's parity for the other's)
+    constexpr uint32_t kGroupWarps = DIM == 64 ? 2 : 4, kGroups = kDequantWarps / kGroupWarps < kSlots ? kDequantWarps / kGroupWarps : kSlots, kUnitsEach = kUnits / (32 * kGroupWarps);
     constexpr uint32_t kColQ = 0, kColO = DIM / 2, kColS = kColO + DIM;
     extern __shared__ uint8_t tilesSmem[];
     __shared__ __align__(8) uint64_t barriers[2 * kSlots + 4 * kPacked + 2 * kInfo + 2 + 4 + 2 + 1 + 1 + 8];
