@@ -38,6 +38,10 @@ constexpr int kTilesThreads = 32 * (kFirstRowWarp + kRowWarps);
 constexpr int kRegsOthers = 48, kRegsRows = 128;
 static_assert(128 * kRegsOthers + 32 * kDequantWarps * kRegsOthers + 32 * kRowWarps * kRegsRows <= kTilesThreads * 72, "register split");
 constexpr uint32_t kRows = kTileRows;
+// Weights are held times 2^6 (as is their sum): with the 2^8 that a logit may pass the maximum by they stay within f16, and what
+// is 2^-30 of the largest is still something.
+constexpr float kWeightScale = 6.0f;
+constexpr uint32_t kUnitCost = 8;  // tiles' time that a unit takes besides its tiles
 constexpr uint32_t kInfo = 4;   // tiles whose scales and exponents are kept
 constexpr uint32_t kSlots = 4, kPacked = 3;  // expanded tiles; packed ones, of keys and of values each
 
@@ -143,6 +147,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
     __shared__ uint32_t firstTile[kTilesThreads + 1], firstWork[kTilesThreads + 1], warpSums[32];
     __shared__ uint32_t holes[kPacked], broken[kInfo][2], hidden[kInfo][2];
     __shared__ float4 tileInfo[kInfo];
+    __shared__ uint3 known[kTilesThreads];
     __shared__ float topShared[kRows], sumShared[kRowGroups][kRows], refShared[kRowGroups][kRows];
     __shared__ uint32_t largestShared[kRowGroups][kRows];
     const AttendArgs &a = args.a;
@@ -189,18 +194,22 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
     pdl_enter();
 
     // ---- the plan: row tiles of the requests, key tiles of those, this CTA's run ----
-    auto rows_of = [&](uint32_t r) {
+    // A request: its first row, rows, length; looked up once where there is a thread for each.
+    const uint32_t run = (a.requests + kTilesThreads - 1) / kTilesThreads;
+    auto look_up = [&](uint32_t r) {
         const uint32_t begin = min(__ldg(a.rowStart + r), a.tokens), end = min(__ldg(a.rowStart + r + 1), a.tokens);
-        return end > begin ? min(end - begin, a.maxRows) : 0u;
+        return make_uint3(begin, end > begin ? end - begin : 0u, min(__ldg(a.lengths + r), 0x7FFFFFFFu));
     };
+    auto request = [&](uint32_t r) { return run == 1 ? known[r] : look_up(r); };
+    auto row_tiles_of = [&](uint32_t r) { return (min(request(r).y, a.maxRows) + args.tileTokens - 1) / args.tileTokens; };
     auto row_tile = [&](uint32_t r, uint32_t i) {
         RowTileOf q;
-        const uint32_t begin = min(__ldg(a.rowStart + r), a.tokens), end = min(__ldg(a.rowStart + r + 1), a.tokens);
-        const uint32_t rows = end > begin ? end - begin : 0u, used = min(rows, a.maxRows);
+        const uint3 of = request(r);
+        const uint32_t used = min(of.y, a.maxRows);
         q.r = r;
-        q.firstRow = begin + i * args.tileTokens;
+        q.firstRow = of.x + i * args.tileTokens;
         q.tokens = min(args.tileTokens, used - i * args.tileTokens);
-        q.p0 = (int)min(__ldg(a.lengths + r), 0x7FFFFFFFu) - (int)rows + (int)(i * args.tileTokens);
+        q.p0 = (int)of.z - (int)of.y + (int)(i * args.tileTokens);
         const uint32_t ends = ((uint32_t)max(0, q.p0 + (int)q.tokens) + kTileKeys - 1) / kTileKeys;
         q.lowTile = q.tilesSink = 0;
         if (a.window) {
@@ -220,12 +229,15 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
         }
         if (lane == 31u) warpSums[warp] = scan;
         __syncthreads();
-        uint32_t before = 0, total = 0;
-        for (uint32_t w = 0; w < kTilesThreads / 32; ++w) {
-            if (w < warp) before += warpSums[w];
-            total += warpSums[w];
+        const uint32_t mine = lane < kTilesThreads / 32 ? warpSums[lane] : 0u;
+        uint32_t sums = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, sums, d);
+            if (lane >= (uint32_t)d) sums += v;
         }
-        first[tid] = before + scan - sum;
+        const uint32_t total = __shfl_sync(0xFFFFFFFFu, sums, 31);
+        first[tid] = __shfl_sync(0xFFFFFFFFu, sums - mine, warp) + scan - sum;
         if (tid == 0) first[kTilesThreads] = total;
         __syncthreads();
         return total;
@@ -239,10 +251,13 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
         }
         return low;
     };
-    const uint32_t run = (a.requests + kTilesThreads - 1) / kTilesThreads;
     const uint32_t r0 = min(tid * run, a.requests), r1 = min(r0 + run, a.requests);
     uint32_t mineTiles = 0;
-    for (uint32_t r = r0; r < r1; ++r) mineTiles += (rows_of(r) + args.tileTokens - 1) / args.tileTokens;
+    for (uint32_t r = r0; r < r1; ++r) {
+        const uint3 of = look_up(r);
+        if (run == 1) known[r] = of;
+        mineTiles += (min(of.y, a.maxRows) + args.tileTokens - 1) / args.tileTokens;
+    }
     const uint32_t rowTiles = block_scan(mineTiles, firstTile);
     // the n-th row tile
     struct Place {
@@ -253,7 +268,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
         n -= firstTile[low];
         Place p{low * run, 0u, 0u};
         for (;; ++p.r) {
-            p.count = (rows_of(p.r) + args.tileTokens - 1) / args.tileTokens;
+            p.count = row_tiles_of(p.r);
             if (n < p.count) break;
             n -= p.count;
         }
@@ -265,7 +280,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
         p.i = 0;
         do {
             ++p.r;
-            p.count = (rows_of(p.r) + args.tileTokens - 1) / args.tileTokens;
+            p.count = row_tiles_of(p.r);
         } while (p.count == 0);
     };
     const uint32_t perThread = (rowTiles + kTilesThreads - 1) / kTilesThreads;
@@ -274,7 +289,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
     if (n0 < n1) {
         Place p = place_of(n0);
         for (uint32_t n = n0; n < n1; ++n) {
-            work += row_tile(p.r, p.i).tiles * a.kvHeads;
+            work += (row_tile(p.r, p.i).tiles + kUnitCost) * a.kvHeads;
             if (n + 1 < n1) advance(p);
         }
     }
@@ -297,44 +312,54 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
             }
         }
     }
-    const uint32_t ctas = min(gridDim.x, total), cta = blockIdx.x;
+    const uint32_t ctas = min(gridDim.x, max(1u, total / 2u)), cta = blockIdx.x;
     auto start_of = [&](uint32_t c) { return (uint32_t)((unsigned long long)c * total / ctas); };
     auto cta_of = [&](uint32_t x) { return (uint32_t)((((unsigned long long)x + 1) * ctas - 1) / total); };
-    const uint32_t begin = cta < ctas ? start_of(cta) : 0u, end = cta < ctas ? start_of(cta + 1) : 0u;
+    const uint32_t begin = cta < ctas && total ? start_of(cta) : 0u, end = cta < ctas && total ? start_of(cta + 1) : 0u;
 
-    // The run's segments: consecutive key tiles of one unit.
+    // The run's segments: consecutive key tiles of one unit, whose tile i stands at x = first + kUnitCost + i.  A unit costs its
+    // tiles and kUnitCost more: its queries, first logits and output take as long.
     struct Walk {
         Place place;
         RowTileOf q;
-        uint32_t inTile, head, t0, count;  // inTile: work of the row tile before this; segment [t0, t0 + count)
+        uint32_t first, head, t0, count;  // segment [t0, t0 + count)
     };
-    auto set_segment = [&](Walk &w, uint32_t x) {
-        w.head = w.inTile / w.q.tiles;
-        w.t0 = w.inTile % w.q.tiles;
-        w.count = min(end - x, w.q.tiles - w.t0);
+    auto take = [&](Walk &w) {
+        const uint32_t tile0 = w.first + kUnitCost;
+        w.t0 = begin > tile0 ? min(begin - tile0, w.q.tiles) : 0u;
+        w.count = (end > tile0 ? min(end - tile0, w.q.tiles) : 0u) - w.t0;
     };
-    auto locate = [&](uint32_t x) {
-        Walk w;
-        const uint32_t low = search(firstWork, x);
-        w.place = place_of(low * perThread);
-        uint32_t n = x - firstWork[low];
-        for (;; advance(w.place)) {
-            w.q = row_tile(w.place.r, w.place.i);
-            if (n < w.q.tiles * a.kvHeads) break;
-            n -= w.q.tiles * a.kvHeads;
-        }
-        w.inTile = n;
-        set_segment(w, x);
-        return w;
-    };
-    auto next_segment = [&](Walk &w, uint32_t x) {  // x: where the last one ended, below `end`
-        w.inTile += w.count;
-        if (w.inTile == w.q.tiles * a.kvHeads) {
+    auto next_unit = [&](Walk &w) {
+        w.first += w.q.tiles + kUnitCost;
+        if (w.first >= end) return false;
+        if (++w.head == a.kvHeads) {
+            w.head = 0;
             advance(w.place);
             w.q = row_tile(w.place.r, w.place.i);
-            w.inTile = 0;
         }
-        set_segment(w, x);
+        take(w);
+        return true;
+    };
+    // the segment behind; false past the run's end (a run may begin or end in front of a unit's first tile)
+    auto next_segment = [&](Walk &w) {
+        do {
+            if (!next_unit(w)) return false;
+        } while (w.count == 0);
+        return true;
+    };
+    auto first_segment = [&](Walk &w) {
+        const uint32_t low = search(firstWork, begin);
+        w.place = place_of(low * perThread);
+        uint32_t n = begin - firstWork[low];
+        for (;; advance(w.place)) {
+            w.q = row_tile(w.place.r, w.place.i);
+            if (n < (w.q.tiles + kUnitCost) * a.kvHeads) break;
+            n -= (w.q.tiles + kUnitCost) * a.kvHeads;
+        }
+        w.head = n / (w.q.tiles + kUnitCost);
+        w.first = begin - n % (w.q.tiles + kUnitCost);
+        take(w);
+        return w.count != 0 || next_segment(w);
     };
     auto key_at = [&](const RowTileOf &q, uint32_t t) { return (t < q.tilesSink ? t : q.lowTile + t - q.tilesSink) * kTileKeys; };
     const uint32_t pieceKeys = 1u << args.pieceShift, pieces = kTileKeys >> args.pieceShift;
@@ -354,8 +379,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
             const uint32_t perTileShift = 6u - args.pieceShift, tilesPer = 32u >> perTileShift;  // pieces of a tile, as a shift; tiles whose pages a warp holds
             uint32_t stage = 0, phase = 0;
             bool ok = true;
-            Walk w = locate(begin);
-            for (uint32_t x = begin; x < end && ok;) {
+            Walk w;
+            for (bool more = first_segment(w); more && ok; more = ok && next_segment(w)) {
                 const int keysEnd = w.q.p0 + (int)w.q.tokens;
                 // a lane holds the page of one piece of `tilesPer` tiles from `base` on
                 auto page_of = [&](uint32_t base) {
@@ -400,14 +425,12 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                         if (++stage == kPacked) stage = 0, phase ^= 1u;
                     }
                 }
-                x += w.count;
-                if (ok && x < end) next_segment(w, x);
             }
         } else if (warp == (uint32_t)kMmaWarp) {
             // ---------------- MMAs ----------------
             uint32_t slot = 0, phase = 0, tile = 0, unitNo = 0;  // tile: key tiles so far (its S buffer, the barriers' parities)
             bool ok = true;
-            Walk w = locate(begin);
+            Walk w;
             const uint32_t idescS = idesc_f16(kTileKeys, false), idescO = idesc_f16(DIM, true);
             auto scores = [&](uint32_t n) {  // S of the n-th tile, from the slot that is next
                 if (!wait_warp<false>(barTile + 8 * slot, phase, &abortFlag)) return false;
@@ -425,7 +448,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                 if (++slot == kSlots) slot = 0, phase ^= 1u;
                 return true;
             };
-            for (uint32_t x = begin; x < end && ok;) {
+            for (bool more = first_segment(w); more && ok; more = ok && next_segment(w)) {
                 ok = wait_warp<false>(barQ, unitNo & 1u, &abortFlag);
                 tc_fence_after();
                 ok = ok && scores(tile);
@@ -454,8 +477,6 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                     if (++slot == kSlots) slot = 0, phase ^= 1u;
                 }
                 ++unitNo;
-                x += w.count;
-                if (x < end) next_segment(w, x);
             }
         } else if (warp == (uint32_t)kScaleWarp) {
             // ---------------- scales: a lane two neighbouring keys of a tile ----------------
@@ -464,8 +485,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
             // 16 scale and |bias| of the tile 2^-6 .. 2^-5.
             uint32_t tile = 0;
             bool ok = true;
-            Walk w = locate(begin);
-            for (uint32_t x = begin; x < end && ok;) {
+            Walk w;
+            for (bool more = first_segment(w); more && ok; more = ok && next_segment(w)) {
                 const int pLast = w.q.p0 + (int)w.q.tokens - 1;
                 for (uint32_t i = 0; i < w.count; ++i, ++tile) {
                     const uint32_t at = tile % kPacked, info = tile % kInfo;
@@ -535,8 +556,6 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                         mbar_arrive(barInfo + 8 * info);
                     }
                 }
-                x += w.count;
-                if (ok && x < end) next_segment(w, x);
             }
         } else if (warp >= (uint32_t)kFirstDequant) {
             // ---------------- expansion: the groups of warps take slots K0, K1, V0, K2, V1, ... in turn ----------------
@@ -586,8 +605,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                     mbar_arrive(barTile + 8 * slot);
                 }
             };
-            Walk w = locate(begin);
-            for (uint32_t x = begin; x < end && ok;) {
+            Walk w;
+            for (bool more = first_segment(w); more && ok; more = ok && next_segment(w)) {
                 // a segment of n tiles is 2 n slots: K0, then for every tile i the keys of i + 1 (all but the last) and the values of i
                 for (uint32_t k = 0; k < 2 * w.count && ok; ++k, ++item) {
                     if (item % kGroups != grp) continue;
@@ -595,8 +614,6 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                     fill(tile + (isKey ? (k + 1) / 2 : (k == 2 * w.count - 1 ? w.count - 1 : k / 2 - 1)), isKey ? 0u : 1u);
                 }
                 tile += w.count;
-                x += w.count;
-                if (x < end) next_segment(w, x);
             }
         }
     } else {
@@ -607,8 +624,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
             const uint32_t lanes = (quarter * 32) << 16;
             uint32_t tile = 0, joins = 0;
             bool ok = true;
-            Walk w = locate(begin);
-            for (uint32_t x = begin; x < end && ok;) {
+            Walk w;
+            for (bool more = first_segment(w); more && ok; more = ok && next_segment(w)) {
                 const uint32_t token = row / group;
                 const bool there = token < w.q.tokens;
                 const uint32_t head = w.head * group + row % group;
@@ -719,7 +736,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                     if (lane == 0) mbar_arrive(barTop + 8 * (wg * 4 + quarter));
                     sum *= exp2_fast(ref - top);
                     ref = top;
-                    const float shift = about.y - top;
+                    const float shift = about.y - top + kWeightScale;
                     const unsigned long long f2 = pair_f32(f, f), shift2 = pair_f32(shift, shift);
                     unsigned long long part = pair_f32(0.0f, 0.0f), part2 = part;
                     auto weigh = [&](const float *v, uint32_t to) {  // 32 logits: weights to 16 columns
@@ -786,7 +803,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                 tc_fence_before();  // (the next unit's products overwrite O once both warpgroups have brought their queries)
                 if (!whole) {
                     if (there && wg == 0) args.stats[part * kRows + row] = make_float2(top, sum);
-                    const uint32_t c0 = cta_of(x - w.t0), c1 = cta_of(x - w.t0 + w.q.tiles - 1);
+                    const uint32_t c0 = cta_of(w.first + kUnitCost), c1 = cta_of(w.first + kUnitCost + w.q.tiles - 1);
                     if (!meet()) break;
                     if (wg == 0 && row == 0) {
                         __threadfence();  // (cumulative: for the parts that the barrier made this thread see)
@@ -799,29 +816,26 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                     if (lastPart) {
                         __threadfence();
                         auto part_of = [&](uint32_t c) { return 2 * c + (c == c0 ? 1u : 0u); };
-                        // a warp 32 rows and eight of their values at a time, kAtOnce parts' loads in flight
-                        constexpr uint32_t kAtOnce = 6;
+                        // a warp 32 rows and four times eight of their values at a time, two parts' loads in flight
+                        constexpr uint32_t kAtOnce = 2, kValues = 4;
                         const uint32_t used = w.q.tokens * group, blocks = (used + 31) / 32;
-                        for (uint32_t item = warp - kFirstRowWarp; item < blocks * (DIM / 8); item += kRowWarps) {
-                            const uint32_t mine = item % blocks * 32 + lane, d = item / blocks * 8;
+                        for (uint32_t item = warp - kFirstRowWarp; item < blocks * (DIM / 8 / kValues); item += kRowWarps) {
+                            const uint32_t mine = item % blocks * 32 + lane, d = item / blocks * (8 * kValues);
                             if (mine >= used) continue;
-                            float all = kNone, weights = 0.0f, v[8];
+                            float all = kNone, weights = 0.0f, v[8 * kValues];
 #pragma unroll
-                            for (int k = 0; k < 8; ++k) v[k] = 0.0f;
+                            for (uint32_t k = 0; k < 8 * kValues; ++k) v[k] = 0.0f;
+#pragma unroll 1
                             for (uint32_t from = c0; from <= c1; from += kAtOnce) {
                                 float2 st[kAtOnce];
-                                float4 t[kAtOnce][2];
+                                float4 t[kAtOnce][2 * kValues];
 #pragma unroll
                                 for (uint32_t k = 0; k < kAtOnce; ++k) {
-                                    const uint32_t n = part_of(from + k);
-                                    st[k] = make_float2(kNone, 0.0f);
-                                    t[k][0] = t[k][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                                    if (from + k <= c1) {
-                                        st[k] = __ldcg(args.stats + n * kRows + mine);
-                                        const float4 *at = reinterpret_cast<const float4 *>(args.partials) + ((size_t)n * (DIM / 4) + d / 4) * kRows + mine;
-                                        t[k][0] = __ldcg(at);
-                                        t[k][1] = __ldcg(at + kRows);
-                                    }
+                                    const uint32_t n = part_of(min(from + k, c1));
+                                    st[k] = __ldcg(args.stats + n * kRows + mine);
+                                    const float4 *at = reinterpret_cast<const float4 *>(args.partials) + ((size_t)n * (DIM / 4) + d / 4) * kRows + mine;
+#pragma unroll
+                                    for (uint32_t h = 0; h < 2 * kValues; ++h) t[k][h] = __ldcg(at + h * kRows);
                                 }
                                 float next = all;
 #pragma unroll
@@ -830,27 +844,29 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                                 all = next;
                                 weights *= keep;
 #pragma unroll
-                                for (int k = 0; k < 8; ++k) v[k] *= keep;
+                                for (uint32_t k = 0; k < 8 * kValues; ++k) v[k] *= keep;
 #pragma unroll
                                 for (uint32_t k = 0; k < kAtOnce; ++k) {
+                                    if (from + k > c1) break;
                                     const float g = exp2_fast(st[k].x - all);
                                     weights = fmaf(st[k].y, g, weights);
 #pragma unroll
-                                    for (int h = 0; h < 2; ++h) {
+                                    for (uint32_t h = 0; h < 2 * kValues; ++h) {
                                         v[4 * h] = fmaf(t[k][h].x, g, v[4 * h]), v[4 * h + 1] = fmaf(t[k][h].y, g, v[4 * h + 1]);
                                         v[4 * h + 2] = fmaf(t[k][h].z, g, v[4 * h + 2]), v[4 * h + 3] = fmaf(t[k][h].w, g, v[4 * h + 3]);
                                     }
                                 }
                             }
                             const float f = weights == 0.0f ? 0.0f : 1.0f / weights;
-                            *reinterpret_cast<uint4 *>(a.out + (size_t)(w.q.firstRow + mine / group) * a.outStride + (w.head * group + mine % group) * DIM + d) =
-                                make_uint4(pack_bf16x2(v[0] * f, v[2] * f), pack_bf16x2(v[4] * f, v[6] * f), pack_bf16x2(v[1] * f, v[3] * f), pack_bf16x2(v[5] * f, v[7] * f));
+                            uint16_t *to = a.out + (size_t)(w.q.firstRow + mine / group) * a.outStride + (w.head * group + mine % group) * DIM + d;
+#pragma unroll
+                            for (uint32_t k = 0; k < 8 * kValues; k += 8)
+                                *reinterpret_cast<uint4 *>(to + k) = make_uint4(pack_bf16x2(v[k] * f, v[k + 2] * f), pack_bf16x2(v[k + 4] * f, v[k + 6] * f),
+                                                                                pack_bf16x2(v[k + 1] * f, v[k + 3] * f), pack_bf16x2(v[k + 5] * f, v[k + 7] * f));
                         }
                     }
                 }
                 if (!meet()) break;  // (before the next unit's words in shared memory)
-                x += w.count;
-                if (x < end) next_segment(w, x);
             }
         }
     }
