@@ -34,7 +34,7 @@ struct RowsArgs {
     AttendArgs a;
     float *partials;      // [2 CTAs][columns][DIM]
     float2 *stats;        // [2 CTAs][columns] maximum (log2), sum
-    uint32_t *arrived;    // [CTAs], zero between launches
+    uint32_t *arrived;    // [3][CTAs], zero between launches: of a unit, of its first group of parts, of another group
     uint32_t pageShift, pieceShift;  // log2 of a page's tokens and of the keys of a tile on one page
 };
 
@@ -682,6 +682,12 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
         const uint32_t used = min(kColumns, columns - column0);
         const bool whole = count == unitTiles;
         const uint32_t slot = 2 * cta + (t0 == 0 ? 1u : 0u);
+        auto write = [&](uint32_t column, uint32_t at, const float4 &v, float weights) {
+            const float f = weights == 0.0f ? 0.0f : 1.0f / weights;
+            const uint32_t global = column0 + column;
+            uint16_t *to = a.out + (size_t)(w.q.firstRow + global / group) * a.outStride + (head * group + global % group) * DIM + at;
+            *reinterpret_cast<uint2 *>(to) = make_uint2(pack_bf16x2(v.x * f, v.y * f), pack_bf16x2(v.z * f, v.w * f));
+        };
         for (uint32_t e = tid; e < used * (DIM / 4); e += 32 * kConsumers) {
             const uint32_t column = e / (DIM / 4), at = e % (DIM / 4) * 4;
             const float4 u = *reinterpret_cast<const float4 *>(joined + column * (DIM + 4) + at);
@@ -693,45 +699,47 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
             for (int k = 0; k < kConsumers; ++k) weights += joinStats[k][column].y * exp2_fast(joinStats[k][column].x - all);
             const float4 sum4 = make_float4(u.x + v.x, u.y + v.y, u.z + v.z, u.w + v.w);
             if (whole) {
-                const float f = weights == 0.0f ? 0.0f : 1.0f / weights;
-                const uint32_t global = column0 + column;
-                uint16_t *to = a.out + (size_t)(w.q.firstRow + global / group) * a.outStride + (head * group + global % group) * DIM + at;
-                *reinterpret_cast<uint2 *>(to) = make_uint2(pack_bf16x2(sum4.x * f, sum4.y * f), pack_bf16x2(sum4.z * f, sum4.w * f));
+                write(column, at, sum4, weights);
             } else {
                 *reinterpret_cast<float4 *>(args.partials + ((size_t)slot * kColumns + column) * DIM + at) = sum4;
                 if (at == 0) args.stats[slot * kColumns + column] = make_float2(all, weights);
             }
         }
         if (!whole) {
-            const uint32_t c0 = cta_of(w.first + kUnitCost), c1 = cta_of(w.first + kUnitCost + unitTiles - 1);
-            named_barrier(1, 32 * kConsumers);
-            if (tid == 0) {
-                __threadfence();  // (cumulative: for the parts that the barrier made this thread see)
-                const uint32_t n = atomicAdd(args.arrived + c0, 1u);
-                __threadfence();
-                lastPart = n == c1 - c0;
-                if (n == c1 - c0) args.arrived[c0] = 0u;
-            }
-            named_barrier(1, 32 * kConsumers);
-            if (lastPart) {
+            const uint32_t c0 = cta_of(w.first + kUnitCost), c1 = cta_of(w.first + kUnitCost + unitTiles - 1), parts = c1 - c0 + 1;
+            // whether this is the last of `expected` CTAs; then what they wrote is there
+            auto arrive = [&](uint32_t *counter, uint32_t expected) {
+                named_barrier(1, 32 * kConsumers);
+                if (tid == 0) {
+                    __threadfence();  // (cumulative: for the parts that the barrier made this thread see)
+                    const uint32_t n = atomicAdd(counter, 1u);
+                    __threadfence();
+                    lastPart = n == expected - 1;
+                    if (n == expected - 1) *counter = 0u;
+                }
+                named_barrier(1, 32 * kConsumers);
+                return lastPart != 0u;
+            };
+            // parts of CTAs from, from + step, ... joined, into the unit's rows or the first one's place
+            auto join = [&](uint32_t from, uint32_t count, uint32_t step, bool last) {
+                auto slot_of = [&](uint32_t c) { return 2 * c + (c == c0 ? 1u : 0u); };
                 for (uint32_t e = tid; e < used * (DIM / 4); e += 32 * kConsumers) {
                     const uint32_t column = e / (DIM / 4), at = e % (DIM / 4) * 4;
-                    auto slot_of = [&](uint32_t c) { return 2 * c + (c == c0 ? 1u : 0u); };
                     // kAtOnce parts' loads in flight: one after the other they took 10 us for 37 parts
-                    constexpr uint32_t kAtOnce = 12;
+                    constexpr uint32_t kAtOnce = 10;
                     float all = kNone, weights = 0.0f;
                     float4 sum4 = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    for (uint32_t first = c0; first <= c1; first += kAtOnce) {
+                    for (uint32_t k0 = 0; k0 < count; k0 += kAtOnce) {
                         float2 st[kAtOnce];
                         float4 v[kAtOnce];
 #pragma unroll
                         for (uint32_t k = 0; k < kAtOnce; ++k) {
-                            const uint32_t c = first + k;
                             st[k] = make_float2(kNone, 0.0f);
                             v[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                            if (c <= c1) {
-                                st[k] = __ldcg(args.stats + slot_of(c) * kColumns + column);
-                                v[k] = __ldcg(reinterpret_cast<const float4 *>(args.partials + ((size_t)slot_of(c) * kColumns + column) * DIM + at));
+                            if (k0 + k < count) {
+                                const uint32_t slot = slot_of(from + (k0 + k) * step);
+                                st[k] = __ldcg(args.stats + slot * kColumns + column);
+                                v[k] = __ldcg(reinterpret_cast<const float4 *>(args.partials + ((size_t)slot * kColumns + column) * DIM + at));
                             }
                         }
                         float next = all;
@@ -748,11 +756,32 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
                             sum4.x = fmaf(v[k].x, f, sum4.x), sum4.y = fmaf(v[k].y, f, sum4.y), sum4.z = fmaf(v[k].z, f, sum4.z), sum4.w = fmaf(v[k].w, f, sum4.w);
                         }
                     }
-                    const float f = weights == 0.0f ? 0.0f : 1.0f / weights;
-                    const uint32_t global = column0 + column;
-                    uint16_t *to = a.out + (size_t)(w.q.firstRow + global / group) * a.outStride + (head * group + global % group) * DIM + at;
-                    *reinterpret_cast<uint2 *>(to) = make_uint2(pack_bf16x2(sum4.x * f, sum4.y * f), pack_bf16x2(sum4.z * f, sum4.w * f));
+                    if (last) {
+                        write(column, at, sum4, weights);
+                    } else {
+                        *reinterpret_cast<float4 *>(args.partials + ((size_t)slot_of(from) * kColumns + column) * DIM + at) = sum4;
+                        if (at == 0) joinStats[0][column] = make_float2(all, weights);
+                    }
                 }
+                if (!last) {
+                    named_barrier(1, 32 * kConsumers);  // (the first one's maxima have been read)
+                    if (tid < used) args.stats[slot_of(from) * kColumns + tid] = joinStats[0][tid];
+                }
+            };
+            // by groups of 16 first where there are more: one CTA would take 100 us for 296 parts (a CTA is the first of one unit
+            // and inside another at most: a group's counter goes by which)
+            constexpr uint32_t kGroupParts = 16;
+            const uint32_t groups = (parts + kGroupParts - 1) / kGroupParts, group0 = c0 + (cta - c0) / kGroupParts * kGroupParts;
+            bool last = groups == 1;
+            uint32_t *counter = args.arrived + (last ? 0 : group0 == c0 ? 1 : 2) * gridDim.x + group0;
+            uint32_t from = group0, many = min(kGroupParts, c1 - group0 + 1), step = 1;
+#pragma unroll 1
+            while (arrive(counter, many)) {
+                join(from, many, step, last);
+                if (last) break;
+                last = true;
+                counter = args.arrived + c0;
+                from = c0, many = groups, step = kGroupParts;
             }
         }
         n0 += count;
@@ -760,7 +789,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
     } while (next_unit(w));
 }
 
-KernelSmemMemo rowsMemo[3][4];
+KernelSmemMemo rowsMemo[3][3];
 
 template <int DIM, int NT, bool SPLIT = false>
 bool launch_rows(FFAttention *att, KernelSmemMemo &memo, const CUtensorMap &codes, const CUtensorMap &words, const RowsArgs &args, cudaStream_t stream, const char **error) {
@@ -809,13 +838,11 @@ bool launch_attend_rows(FFAttention *att, const AttendArgs &a, cudaStream_t stre
     if (dim == 128) {
         if (columns <= 4) return launch_rows<128, 1, true>(att, rowsMemo[1][0], codes, words, args, stream, error);
         if (columns <= 8) return launch_rows<128, 1>(att, rowsMemo[1][1], codes, words, args, stream, error);
-        if (columns <= 16) return launch_rows<128, 2>(att, rowsMemo[1][2], codes, words, args, stream, error);
-        return launch_rows<128, 4>(att, rowsMemo[1][3], codes, words, args, stream, error);
+        return launch_rows<128, 2>(att, rowsMemo[1][2], codes, words, args, stream, error);
     }
     if (columns <= 4) return launch_rows<64, 1, true>(att, rowsMemo[2][0], codes, words, args, stream, error);
     if (columns <= 8) return launch_rows<64, 1>(att, rowsMemo[2][1], codes, words, args, stream, error);
-    if (columns <= 16) return launch_rows<64, 2>(att, rowsMemo[2][2], codes, words, args, stream, error);
-    return launch_rows<64, 4>(att, rowsMemo[2][3], codes, words, args, stream, error);
+    return launch_rows<64, 2>(att, rowsMemo[2][2], codes, words, args, stream, error);
 }
 
 }  // namespace ff

@@ -49,7 +49,7 @@ struct TilesArgs {
     AttendArgs a;
     float *partials;      // [2 CTAs][rows][DIM]
     float2 *stats;        // [2 CTAs][rows]
-    uint32_t *arrived;    // [CTAs], zero between launches
+    uint32_t *arrived;    // [3][CTAs], zero between launches: of a unit, of its first group of parts, of another group
     uint32_t pageShift, pieceShift, tileTokens;  // log2 of a page's tokens and of the keys of a tile on one page; tokens of a row tile
 };
 
@@ -803,39 +803,43 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                 tc_fence_before();  // (the next unit's products overwrite O once both warpgroups have brought their queries)
                 if (!whole) {
                     if (there && wg == 0) args.stats[part * kRows + row] = make_float2(top, sum);
-                    const uint32_t c0 = cta_of(w.first + kUnitCost), c1 = cta_of(w.first + kUnitCost + w.q.tiles - 1);
-                    if (!meet()) break;
-                    if (wg == 0 && row == 0) {
-                        __threadfence();  // (cumulative: for the parts that the barrier made this thread see)
-                        const uint32_t n = atomicAdd(args.arrived + c0, 1u);
-                        __threadfence();
-                        lastPart = n == c1 - c0;
-                        if (n == c1 - c0) args.arrived[c0] = 0u;
-                    }
-                    if (!meet()) break;
-                    if (lastPart) {
-                        __threadfence();
+                    const uint32_t c0 = cta_of(w.first + kUnitCost), c1 = cta_of(w.first + kUnitCost + w.q.tiles - 1), parts = c1 - c0 + 1;
+                    // whether this is the last of `expected` CTAs; then what they wrote is there
+                    auto arrive = [&](uint32_t *counter, uint32_t expected) {
+                        if (!meet()) return false;
+                        if (wg == 0 && row == 0) {
+                            __threadfence();  // (cumulative: for the parts that the barrier made this thread see)
+                            const uint32_t n = atomicAdd(counter, 1u);
+                            __threadfence();
+                            lastPart = n == expected - 1;
+                            if (n == expected - 1) *counter = 0u;
+                        }
+                        return meet() && lastPart != 0u;
+                    };
+                    // parts of CTAs from, from + step, ... joined, into the unit's rows or the first one's place: a warp 32 rows and
+                    // four times eight of their values at a time, two parts' loads in flight
+                    auto join = [&](uint32_t from, uint32_t count, uint32_t step, bool last) {
                         auto part_of = [&](uint32_t c) { return 2 * c + (c == c0 ? 1u : 0u); };
-                        // a warp 32 rows and four times eight of their values at a time, two parts' loads in flight
                         constexpr uint32_t kAtOnce = 2, kValues = 4;
                         const uint32_t used = w.q.tokens * group, blocks = (used + 31) / 32;
+#pragma unroll 1
                         for (uint32_t item = warp - kFirstRowWarp; item < blocks * (DIM / 8 / kValues); item += kRowWarps) {
                             const uint32_t mine = item % blocks * 32 + lane, d = item / blocks * (8 * kValues);
                             if (mine >= used) continue;
                             float all = kNone, weights = 0.0f, v[8 * kValues];
 #pragma unroll
                             for (uint32_t k = 0; k < 8 * kValues; ++k) v[k] = 0.0f;
+                            auto place = [&](uint32_t n) { return reinterpret_cast<float4 *>(args.partials) + ((size_t)n * (DIM / 4) + d / 4) * kRows + mine; };
 #pragma unroll 1
-                            for (uint32_t from = c0; from <= c1; from += kAtOnce) {
+                            for (uint32_t k0 = 0; k0 < count; k0 += kAtOnce) {
                                 float2 st[kAtOnce];
                                 float4 t[kAtOnce][2 * kValues];
 #pragma unroll
                                 for (uint32_t k = 0; k < kAtOnce; ++k) {
-                                    const uint32_t n = part_of(min(from + k, c1));
+                                    const uint32_t n = part_of(from + min(k0 + k, count - 1) * step);
                                     st[k] = __ldcg(args.stats + n * kRows + mine);
-                                    const float4 *at = reinterpret_cast<const float4 *>(args.partials) + ((size_t)n * (DIM / 4) + d / 4) * kRows + mine;
 #pragma unroll
-                                    for (uint32_t h = 0; h < 2 * kValues; ++h) t[k][h] = __ldcg(at + h * kRows);
+                                    for (uint32_t h = 0; h < 2 * kValues; ++h) t[k][h] = __ldcg(place(n) + h * kRows);
                                 }
                                 float next = all;
 #pragma unroll
@@ -847,7 +851,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                                 for (uint32_t k = 0; k < 8 * kValues; ++k) v[k] *= keep;
 #pragma unroll
                                 for (uint32_t k = 0; k < kAtOnce; ++k) {
-                                    if (from + k > c1) break;
+                                    if (k0 + k >= count) break;
                                     const float g = exp2_fast(st[k].x - all);
                                     weights = fmaf(st[k].y, g, weights);
 #pragma unroll
@@ -857,14 +861,38 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                                     }
                                 }
                             }
-                            const float f = weights == 0.0f ? 0.0f : 1.0f / weights;
-                            uint16_t *to = a.out + (size_t)(w.q.firstRow + mine / group) * a.outStride + (w.head * group + mine % group) * DIM + d;
+                            if (last) {
+                                const float f = weights == 0.0f ? 0.0f : 1.0f / weights;
+                                uint16_t *to = a.out + (size_t)(w.q.firstRow + mine / group) * a.outStride + (w.head * group + mine % group) * DIM + d;
 #pragma unroll
-                            for (uint32_t k = 0; k < 8 * kValues; k += 8)
-                                *reinterpret_cast<uint4 *>(to + k) = make_uint4(pack_bf16x2(v[k] * f, v[k + 2] * f), pack_bf16x2(v[k + 4] * f, v[k + 6] * f),
-                                                                                pack_bf16x2(v[k + 1] * f, v[k + 3] * f), pack_bf16x2(v[k + 5] * f, v[k + 7] * f));
+                                for (uint32_t k = 0; k < 8 * kValues; k += 8)
+                                    *reinterpret_cast<uint4 *>(to + k) = make_uint4(pack_bf16x2(v[k] * f, v[k + 2] * f), pack_bf16x2(v[k + 4] * f, v[k + 6] * f),
+                                                                                    pack_bf16x2(v[k + 1] * f, v[k + 3] * f), pack_bf16x2(v[k + 5] * f, v[k + 7] * f));
+                            } else {
+#pragma unroll
+                                for (uint32_t h = 0; h < 2 * kValues; ++h) place(part_of(from))[h * kRows] = make_float4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]);
+                                if (d == 0) refShared[0][mine] = all, sumShared[0][mine] = weights;
+                            }
                         }
+                        if (last || !meet()) return;  // (the first one's maxima have been read)
+                        if (wg == 0 && row < used) args.stats[part_of(from) * kRows + row] = make_float2(refShared[0][row], sumShared[0][row]);
+                    };
+                    // by groups of 16 first where there are more (a CTA is the first of one unit and inside another at most: a
+                    // group's counter goes by which)
+                    constexpr uint32_t kGroupParts = 16;
+                    const uint32_t groups = (parts + kGroupParts - 1) / kGroupParts, group0 = c0 + (cta - c0) / kGroupParts * kGroupParts;
+                    bool last = groups == 1;
+                    uint32_t *counter = args.arrived + (last ? 0 : group0 == c0 ? 1 : 2) * gridDim.x + group0;
+                    uint32_t from = group0, count = min(kGroupParts, c1 - group0 + 1), step = 1;
+#pragma unroll 1
+                    while (arrive(counter, count)) {
+                        join(from, count, step, last);
+                        if (last || !ok) break;
+                        last = true;
+                        counter = args.arrived + c0;
+                        from = c0, count = groups, step = kGroupParts;
                     }
+                    if (!ok) break;
                 }
                 if (!meet()) break;  // (before the next unit's words in shared memory)
             }

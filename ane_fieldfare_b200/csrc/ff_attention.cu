@@ -7,7 +7,10 @@
 namespace ff {
 
 bool launch_attend(FFAttention *att, const AttendArgs &a, cudaStream_t stream, const char **error) {
-    if (a.maxRows <= 16) return launch_attend_rows(att, a, stream, error);
+    // Columns of a key/value head: up to 16 as columns of mma.sync, which then take as long as the cache's bytes; more as rows of
+    // tcgen05.mma.  us as columns / as rows: 16 columns of 128, 64 requests of up to 16384 keys 43 / 67; 10 of 256, 8 x 4000 keys
+    // 57 / 53; 32 of 256, 20000 keys 66 / 41; 32 of 128, 16 requests of up to 3000 keys 44 / 30.
+    if (a.maxRows * (a.heads / a.kvHeads) <= 16) return launch_attend_rows(att, a, stream, error);
     return launch_attend_tiles(att, a, stream, error);
 }
 
@@ -130,7 +133,7 @@ FFAttention *ff_attention_create(int32_t deviceOrdinal, const FFAttentionConfig 
     att->rowsCtas = attend_rows_ctas(att->smCount);
     alloc(&att->partials, 2 * std::max((size_t)att->rowsCtas * kPartialValues, (size_t)att->smCount * kTileRows * config->headDim));
     alloc(&att->stats, 2 * std::max((size_t)att->rowsCtas * kPartialColumns, (size_t)att->smCount * kTileRows));
-    alloc(&att->arrived, att->rowsCtas);
+    alloc(&att->arrived, 3 * att->rowsCtas);
     if (st == cudaSuccess) st = cudaDeviceSynchronize();
     if (st != cudaSuccess) {
         fail(error, std::string("attention scratch: ") + cudaGetErrorString(st));

@@ -50,7 +50,7 @@ inline PageLayout page_layout(const FFAttentionConfig &c) {
 
 // Partial results of units that several CTAs share: columns (rows times query heads of a key/value head) of a unit, and
 // their output values, where requests have few rows (two CTAs an SM) and many (one).
-constexpr uint32_t kPartialColumns = 32, kPartialValues = 4096, kTileRows = 128;
+constexpr uint32_t kPartialColumns = 16, kPartialValues = 4096, kTileRows = 128;
 
 // Counts a launch and reports what it says.
 inline bool launched(FFAttention *att, cudaError_t status, const char *what, const char **error) {

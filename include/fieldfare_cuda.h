@@ -556,9 +556,9 @@ bool ff_cache_read(FFAttention *attention, const void *pages, uint32_t pageCount
  *   lengths[r] keys of request r, its rows' included; its row i stands at position lengths[r] - rows + i
  * A row at position p sees key j <= p if window is 0, j > p - window, or j < sinks.  out [tokens][heads][headDim]
  * (rows outStride apart) = softmax(scale q.k) v; a row that sees no key, and rows behind the last request's, are zero.
- * maxRows: no request has more rows (it chooses the kernel; rows past it are zero, flag 15).  Up to 16 rows a request
- * decode and verify blocks are split over the keys, so that one request fills the GPU; longer ones run on the
- * 5th-generation tensor cores.  Keys on a page outside the cache are not seen (flag 16). */
+ * maxRows: no request has more rows (it chooses the kernel; rows past it are zero, flag 15).  Up to 16 columns (rows times
+ * heads/kvHeads) run on mma.sync on the codes as they lie, more on the 5th-generation tensor cores; either way the keys are
+ * split over the CTAs, so that one request fills the GPU.  Keys on a page outside the cache are not seen (flag 16). */
 bool ff_attention(FFAttention *attention, const uint16_t *q, uint32_t qStride, uint32_t tokens, const void *pages,
                   uint32_t pageCount, const uint32_t *blockTable, uint32_t tableStride, const uint32_t *rowStart,
                   const uint32_t *lengths, uint32_t requests, uint32_t maxRows, float scale, uint32_t window,
