@@ -125,6 +125,18 @@ __device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c
     return r;
 }
 
+// the n lowest bits of 64
+__device__ __forceinline__ unsigned long long first_bits(long long n) { return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1ull; }
+// bit l to bit 2 l
+__device__ __forceinline__ unsigned long long spread_bits(uint32_t v) {
+    unsigned long long x = v;
+    x = (x | x << 16) & 0x0000FFFF0000FFFFull;
+    x = (x | x << 8) & 0x00FF00FF00FF00FFull;
+    x = (x | x << 4) & 0x0F0F0F0F0F0F0F0Full;
+    x = (x | x << 2) & 0x3333333333333333ull;
+    return (x | x << 1) & 0x5555555555555555ull;
+}
+
 // A row tile of a request as the kernel sees it.
 struct RowTileOf {
     uint32_t r, firstRow, tokens;          // its request, first row of q, tokens
@@ -145,7 +157,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
     __shared__ uint32_t tmemSlot, lastPart;
     __shared__ volatile uint32_t abortFlag;
     __shared__ uint32_t firstTile[kTilesThreads + 1], firstWork[kTilesThreads + 1], warpSums[32];
-    __shared__ uint32_t holes[kPacked], broken[kInfo][2], hidden[kInfo][2];
+    __shared__ uint32_t holes[kPacked], hidden[kInfo][2];
     __shared__ float4 tileInfo[kInfo];
     __shared__ uint3 known[kTilesThreads];
     __shared__ float topShared[kRows], sumShared[kRowGroups][kRows], refShared[kRowGroups][kRows];
@@ -480,8 +492,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
             }
         } else if (warp == (uint32_t)kScaleWarp) {
             // ---------------- scales: a lane two neighbouring keys of a tile ----------------
-            // What no row sees is nothing; a visible key with a value that is no number is marked, and so is one whose page is
-            // outside the cache.  A group's word for the expansion: f16 scale * 2^(24 - E) | f16 bias * 2^-E, the largest of
+            // What no row sees is nothing; a visible key with a value (or a value of its value) that is no number is NaN, its value
+            // nothing; keys whose page is outside the cache are marked.  A group's word for the expansion: f16 scale * 2^(24 - E) | f16 bias * 2^-E, the largest of
             // 16 scale and |bias| of the tile 2^-6 .. 2^-5.
             uint32_t tile = 0;
             bool ok = true;
@@ -507,7 +519,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                             for (int G = 0; G < NG; ++G) most[side] = __vmaxu2(most[side], v[side][h][G] & 0x7FFF7FFFu);
                         }
                     auto none = [](uint32_t m) { return max(m & 0xFFFFu, m >> 16) >= 0x7F80u; };
-                    uint32_t bad[2] = {0u, 0u}, out[2] = {0u, 0u};  // bit l: key 2 l, key 2 l + 1
+                    uint32_t out[2] = {0u, 0u};  // bit l: key 2 l, key 2 l + 1
                     if (__any_sync(0xFFFFFFFFu, unseen || none(most[0]) || none(most[1]))) {
                         most[0] = most[1] = 0u;
 #pragma unroll
@@ -520,7 +532,6 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                             for (int side = 0; side < 2; ++side)
 #pragma unroll
                                 for (int G = 0; G < NG; ++G) broke |= is_broken(v[side][h][G]);
-                            bad[h] = __ballot_sync(0xFFFFFFFFu, seen && !hole && broke);
                             out[h] = __ballot_sync(0xFFFFFFFFu, seen && hole);
 #pragma unroll
                             for (int side = 0; side < 2; ++side)
@@ -529,6 +540,10 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                                     if (!seen || hole || broke) v[side][h][G] = 0u;
                                     most[side] = __vmaxu2(most[side], v[side][h][G] & 0x7FFF7FFFu);
                                 }
+                            // (the key of either makes its column of S NaN, which only rows that see it take)
+                            if (seen && !hole && broke)
+#pragma unroll
+                                for (int G = 0; G < NG; ++G) v[0][h][G] = 0x7FC07FC0u;
                         }
                     }
                     __syncwarp();
@@ -550,8 +565,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                     }
                     __syncwarp();
                     if (lane == 0) {
-                        tileInfo[info] = make_float4(power_of_two(exponent[0]), (float)exponent[1], power_of_two(-exponent[1]), unseen || (bad[0] | bad[1]) ? 1.0f : 0.0f);
-                        broken[info][0] = bad[0], broken[info][1] = bad[1];
+                        tileInfo[info] = make_float4(power_of_two(exponent[0]), (float)exponent[1], power_of_two(-exponent[1]), unseen ? 1.0f : 0.0f);
                         hidden[info][0] = out[0], hidden[info][1] = out[1];
                         mbar_arrive(barInfo + 8 * info);
                     }
@@ -569,32 +583,29 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                     ok = false;
                     return;
                 }
-                uint32_t word[kUnitsEach];
-                uint4 v[kUnitsEach][2];
-#pragma unroll
-                for (uint32_t e = 0; e < kUnitsEach; ++e) {
-                    const uint32_t unit = e * (32 * kGroupWarps) + inGroup * 32 + lane, key = unit % kTileKeys, G = unit / kTileKeys;
-                    word[e] = lds32(scales + info * words_bytes(DIM) + side * kWordSide + unit * 4);
-#pragma unroll
-                    for (uint32_t h = 0; h < 2; ++h) v[e][h] = lds128(packed + pack * kPack + key * CB + ((G * 32 + 16 * h) ^ chunk_flip<DIM>(key)));
-                }
                 if (!wait_lane<false>(barTileFree + 8 * slot, slotPhase ^ 1u, &abortFlag)) {
                     ok = false;
                     return;
                 }
-#pragma unroll
+#pragma unroll 1
                 for (uint32_t e = 0; e < kUnitsEach; ++e) {
                     const uint32_t unit = e * (32 * kGroupWarps) + inGroup * 32 + lane, key = unit % kTileKeys, G = unit / kTileKeys;
-                    const uint32_t s0 = __byte_perm(word[e], word[e], 0x1010), bb = __byte_perm(word[e], word[e], 0x3232), s1 = mul_f16x2(s0, 0x2C002C00u);  // 2^-4
+                    const uint32_t word = lds32(scales + info * words_bytes(DIM) + side * kWordSide + unit * 4);
+                    const uint32_t from = packed + pack * kPack + key * CB;
+                    const uint4 v[2] = {lds128(from + ((G * 32) ^ chunk_flip<DIM>(key))), lds128(from + ((G * 32 + 16) ^ chunk_flip<DIM>(key)))};
+                    const uint32_t s0 = __byte_perm(word, word, 0x1010), bb = __byte_perm(word, word, 0x3232), s1 = mul_f16x2(s0, 0x2C002C00u);  // 2^-4
                     const uint32_t to = slots + slot * kSlot + G * (kTileKeys * 128) + key * 128;
 #pragma unroll
                     for (uint32_t h = 0; h < 2; ++h) {
-                        const uint32_t c[4] = {v[e][h].x, v[e][h].y, v[e][h].z, v[e][h].w};
+                        // Four runs of eight values; a chunk is their values n and n + 4.  (In this order four lanes hold a row of
+                        // 32 values in tensor memory, a run each: queries come, and outputs go, 64 bytes of a row at a time.)
+                        const uint32_t c[4] = {v[h].x, v[h].y, v[h].z, v[h].w};
+                        const uint32_t upper[4] = {c[0] >> 8, c[1] >> 8, c[2] >> 8, c[3] >> 8};
 #pragma unroll
-                        for (uint32_t i = 0; i < 4; ++i) {
-                            const uint32_t upper = c[i] >> 8;
-                            sts128(to + (((4 * h + i) ^ (key & 7u)) << 4), fma_f16x2(c[i] & 0x000F000Fu, s0, bb), fma_f16x2(c[i] & 0x00F000F0u, s1, bb),
-                                   fma_f16x2(upper & 0x000F000Fu, s0, bb), fma_f16x2(upper & 0x00F000F0u, s1, bb));
+                        for (uint32_t n = 0; n < 4; ++n) {
+                            const uint32_t *w4 = n < 2 ? c : upper, mask = n % 2 ? 0x00F000F0u : 0x000F000Fu, scale = n % 2 ? s1 : s0;
+                            sts128(to + (((4 * h + n) ^ (key & 7u)) << 4), fma_f16x2(w4[0] & mask, scale, bb), fma_f16x2(w4[1] & mask, scale, bb),
+                                   fma_f16x2(w4[2] & mask, scale, bb), fma_f16x2(w4[3] & mask, scale, bb));
                         }
                     }
                 }
@@ -624,11 +635,16 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
             const uint32_t lanes = (quarter * 32) << 16;
             uint32_t tile = 0, joins = 0;
             bool ok = true;
+            uint32_t mineRows[4];  // token << 16 | head of the rows lane / 4 + 8 k of the warp's 32
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t r = quarter * 32 + 8 * k + (lane >> 2);
+                mineRows[k] = (r / group) << 16 | r % group;
+            }
             Walk w;
             for (bool more = first_segment(w); more && ok; more = ok && next_segment(w)) {
                 const uint32_t token = row / group;
                 const bool there = token < w.q.tokens;
-                const uint32_t head = w.head * group + row % group;
                 const int p = w.q.p0 + (int)token;
                 auto meet = [&] {  // of both warpgroups
                     __syncwarp();
@@ -636,36 +652,50 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                     ok = wait_warp<false>(barJoin, joins++ & 1u, &abortFlag);
                     return ok;
                 };
-                // queries: f16 at a power of two of the row's largest value; runs of eight in the order of the tiles' codes; either
-                // warpgroup half of a row, all its loads in flight
+                // queries: f16 at a power of two of the row's largest value; either warpgroup half of a row, all its loads in flight,
+                // four lanes a row of 64 bytes
                 float toLog2;
                 {
-                    const uint4 *src = reinterpret_cast<const uint4 *>(a.q + (size_t)(w.q.firstRow + (there ? token : 0u)) * a.qStride + head * DIM) + wg * (DIM / 16);
-                    uint4 v[DIM / 16];
-                    uint32_t largest = 0;
+                    constexpr int kBlocks = DIM / 64;  // of 32 values in half a row
+                    uint4 v[4][kBlocks];
 #pragma unroll
-                    for (uint32_t i = 0; i < DIM / 16; ++i) v[i] = there ? __ldg(src + i) : make_uint4(0u, 0u, 0u, 0u);
+                    for (int k = 0; k < 4; ++k) {
+                        const uint32_t tok = mineRows[k] >> 16;
+                        const uint4 *src = reinterpret_cast<const uint4 *>(a.q + (size_t)(w.q.firstRow + tok) * a.qStride + (w.head * group + (mineRows[k] & 0xFFFFu)) * DIM + wg * (DIM / 2)) + (lane & 3u);
 #pragma unroll
-                    for (uint32_t i = 0; i < DIM / 16; ++i)
-                        largest = __vmaxu2(largest, __vmaxu2(__vmaxu2(v[i].x & 0x7FFF7FFFu, v[i].y & 0x7FFF7FFFu), __vmaxu2(v[i].z & 0x7FFF7FFFu, v[i].w & 0x7FFF7FFFu)));
-                    largest = max(largest & 0xFFFFu, largest >> 16) >> 7;
-                    largestShared[wg][row] = largest;
+                        for (int i = 0; i < kBlocks; ++i) v[k][i] = tok < w.q.tokens ? __ldg(src + 4 * i) : make_uint4(0u, 0u, 0u, 0u);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        uint32_t largest = 0;
+#pragma unroll
+                        for (int i = 0; i < kBlocks; ++i)
+                            largest = __vmaxu2(largest, __vmaxu2(__vmaxu2(v[k][i].x & 0x7FFF7FFFu, v[k][i].y & 0x7FFF7FFFu), __vmaxu2(v[k][i].z & 0x7FFF7FFFu, v[k][i].w & 0x7FFF7FFFu)));
+                        largest = __vmaxu2(largest, __shfl_xor_sync(0xFFFFFFFFu, largest, 1));
+                        largest = __vmaxu2(largest, __shfl_xor_sync(0xFFFFFFFFu, largest, 2));
+                        if ((lane & 3u) == 0u) largestShared[wg][quarter * 32 + 8 * k + (lane >> 2)] = max(largest & 0xFFFFu, largest >> 16) >> 7;
+                    }
                     if (!meet()) break;
-                    const uint32_t exponent = max(max(largest, largestShared[wg ^ 1u][row]), 7u);
-                    const float down = __uint_as_float((261u - exponent) << 23);  // the largest is 2^7 .. 2^8
-                    toLog2 = a.scale * 1.4426950408889634f * power_of_two((int)exponent - 134);
+                    auto exponent_of = [&](uint32_t r) { return max(max(largestShared[0][r], largestShared[1][r]), 7u); };
+                    toLog2 = a.scale * 1.4426950408889634f * power_of_two((int)exponent_of(row) - 134);
 #pragma unroll
-                    for (uint32_t c = 0; c < DIM / 64; ++c) {
-                        uint32_t o[16];
+                    for (int half = 0; half < 2; ++half) {
+                        float down[2];
 #pragma unroll
-                        for (uint32_t i = 0; i < 4; ++i) {
-                            const uint4 u = v[4 * c + i];
-                            o[4 * i] = pack_f16(low16(u.x) * down, low16(u.z) * down);
-                            o[4 * i + 1] = pack_f16(high16(u.x) * down, high16(u.z) * down);
-                            o[4 * i + 2] = pack_f16(low16(u.y) * down, low16(u.w) * down);
-                            o[4 * i + 3] = pack_f16(high16(u.y) * down, high16(u.w) * down);
+                        for (int k = 0; k < 2; ++k) down[k] = __uint_as_float((261u - exponent_of(quarter * 32 + 16 * half + 8 * k + (lane >> 2))) << 23);  // the largest is 2^7 .. 2^8
+#pragma unroll
+                        for (int i = 0; i < kBlocks; ++i) {
+                            uint32_t o[8];  // columns 4 j + lane % 4 of rows lane / 4 and lane / 4 + 8
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) {
+                                const uint4 u = v[2 * half + k][i];
+                                o[k] = pack_f16(low16(u.x) * down[k], low16(u.z) * down[k]);
+                                o[2 + k] = pack_f16(high16(u.x) * down[k], high16(u.z) * down[k]);
+                                o[4 + k] = pack_f16(low16(u.y) * down[k], low16(u.w) * down[k]);
+                                o[6 + k] = pack_f16(high16(u.y) * down[k], high16(u.w) * down[k]);
+                            }
+                            tc_store_16x16(tmem + lanes + (half << 20) + kColQ + wg * (DIM / 4) + 16 * i, o);
                         }
-                        tc_store_16cols(tmem + lanes + kColQ + wg * (DIM / 4) + 16 * c, o);
                     }
                     tc_wait_st();
                     tc_fence_before();
@@ -686,16 +716,17 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                     tc_wait_ld();
                     float *s = reinterpret_cast<float *>(lo), *u = reinterpret_cast<float *>(hi);
                     if (about.w != 0.0f) {
-                        // the keys c of the tile that the row sees: up to `most`, above `least` or below `sinks`
-                        const uint32_t bad0 = broken[info][0], bad1 = broken[info][1], gone0 = hidden[info][0], gone1 = hidden[info][1];
-                        const int j0 = (int)key_at(w.q, w.t0 + i), most = p - j0;
-                        const int least = a.window ? (int)max((long long)p - a.window - j0, -1ll) : -1, sinks = a.window ? (int)min(max((long long)a.sinks - j0, 0ll), 64ll) : 0;
+                        // the keys that the row sees: up to its own, and above the window's end or below the last sink
+                        const uint32_t gone0 = hidden[info][0], gone1 = hidden[info][1];
+                        const long long j0 = key_at(w.q, w.t0 + i);
+                        unsigned long long sees = first_bits(p - j0 + 1);
+                        if (a.window) sees &= ~first_bits(p - j0 - a.window + 1) | first_bits((long long)a.sinks - j0);
+                        if (gone0 | gone1) sees &= ~(spread_bits(gone0) | spread_bits(gone1) << 1);
+                        const uint32_t sees0 = (uint32_t)sees, sees1 = (uint32_t)(sees >> 32);
 #pragma unroll
                         for (int c = 0; c < 32; ++c) {
-                            const uint32_t bad = c % 2 ? bad1 : bad0, gone = c % 2 ? gone1 : gone0;  // bit l: key 2 l, key 2 l + 1
-                            const bool see0 = c <= most && (c > least || c < sinks) && !(gone >> (c / 2) & 1u), see1 = c + 32 <= most && (c + 32 > least || c + 32 < sinks) && !(gone >> (16 + c / 2) & 1u);
-                            s[c] = !see0 ? -INFINITY : bad >> (c / 2) & 1u ? NAN : s[c];
-                            u[c] = !see1 ? -INFINITY : bad >> (16 + c / 2) & 1u ? NAN : u[c];
+                            s[c] = sees0 >> c & 1u ? s[c] : -INFINITY;
+                            u[c] = sees1 >> c & 1u ? u[c] : -INFINITY;
                         }
                     }
                     float most[4] = {s[0], s[1], u[0], u[1]};
@@ -777,27 +808,41 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                 sum = sumShared[0][row] * exp2_fast(refShared[0][row] - top) + sumShared[1][row] * exp2_fast(refShared[1][row] - top);
                 const bool whole = w.count == w.q.tiles;
                 const uint32_t part = 2 * cta + (w.t0 == 0 ? 1u : 0u);
-                uint16_t *out = a.out + (size_t)(w.q.firstRow + (there ? token : 0u)) * a.outStride + head * DIM;
-                auto write_32 = [&](uint32_t c, const float (&v)[32], float factor) {
-#pragma unroll
-                    for (int i = 0; i < 32; i += 8)
-                        *reinterpret_cast<uint4 *>(out + c + i) = make_uint4(pack_bf16x2(v[i] * factor, v[i + 2] * factor), pack_bf16x2(v[i + 4] * factor, v[i + 6] * factor),
-                                                                             pack_bf16x2(v[i + 1] * factor, v[i + 3] * factor), pack_bf16x2(v[i + 5] * factor, v[i + 7] * factor));
-                };
-                // a part's values, four of a row behind four of the next
-                auto part_at = [&](uint32_t n, uint32_t c) { return reinterpret_cast<float4 *>(args.partials) + ((size_t)n * (DIM / 4) + c / 4) * kRows + row; };
                 const float factor = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll 1
-                for (uint32_t c = 32 * wg; c < DIM; c += 32 * kRowGroups) {
-                    uint32_t o[32];
-                    tc_load_32cols(tmem + lanes + kColO + c, o);
-                    tc_wait_ld();
-                    if (there && whole) {
-                        write_32(c, reinterpret_cast<const float(&)[32]>(o), factor);
-                    } else if (there) {
-                        float4 *to = part_at(part, c);
+                if (whole) {
+                    // four lanes 64 bytes of a row
+                    float factors[4];
+                    uint16_t *to[4];
 #pragma unroll
-                        for (int k = 0; k < 8; ++k) to[k * kRows] = make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]), __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
+                    for (int k = 0; k < 4; ++k) {
+                        factors[k] = __shfl_sync(0xFFFFFFFFu, factor, 8 * k + (lane >> 2));
+                        to[k] = a.out + (size_t)(w.q.firstRow + (mineRows[k] >> 16)) * a.outStride + (w.head * group + (mineRows[k] & 0xFFFFu)) * DIM + 8 * (lane & 3u);
+                    }
+#pragma unroll 1
+                    for (uint32_t c = 32 * wg; c < DIM; c += 32 * kRowGroups) {
+                        uint32_t o[2][16];
+                        tc_load_16x32(tmem + lanes + kColO + c, o[0]);
+                        tc_load_16x32(tmem + lanes + (1u << 20) + kColO + c, o[1]);
+                        tc_wait_ld();
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const uint32_t *u = o[k >> 1] + 2 * (k & 1);  // u[4 j], u[4 j + 1]: values j and j + 4 of the lane's run
+                            auto at = [&](int n) { return __uint_as_float(u[4 * (n & 3) + (n >> 2)]) * factors[k]; };
+                            if ((mineRows[k] >> 16) < w.q.tokens)
+                                *reinterpret_cast<uint4 *>(to[k] + c) = make_uint4(pack_bf16x2(at(0), at(1)), pack_bf16x2(at(2), at(3)), pack_bf16x2(at(4), at(5)), pack_bf16x2(at(6), at(7)));
+                        }
+                    }
+                } else {
+                    // (a part's values, four of a row behind four of the next, in the order of O's columns)
+#pragma unroll 1
+                    for (uint32_t c = 32 * wg; c < DIM; c += 32 * kRowGroups) {
+                        uint32_t o[32];
+                        tc_load_32cols(tmem + lanes + kColO + c, o);
+                        tc_wait_ld();
+                        float4 *at = reinterpret_cast<float4 *>(args.partials) + ((size_t)part * (DIM / 4) + c / 4) * kRows + row;
+                        if (there)
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) at[k * kRows] = make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]), __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3]));
                     }
                 }
                 tc_fence_before();  // (the next unit's products overwrite O once both warpgroups have brought their queries)
@@ -817,7 +862,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                         return meet() && lastPart != 0u;
                     };
                     // parts of CTAs from, from + step, ... joined, into the unit's rows or the first one's place: a warp 32 rows and
-                    // four times eight of their values at a time, two parts' loads in flight
+                    // 32 of their values at a time, two parts' loads in flight
                     auto join = [&](uint32_t from, uint32_t count, uint32_t step, bool last) {
                         auto part_of = [&](uint32_t c) { return 2 * c + (c == c0 ? 1u : 0u); };
                         constexpr uint32_t kAtOnce = 2, kValues = 4;
@@ -865,9 +910,9 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                                 const float f = weights == 0.0f ? 0.0f : 1.0f / weights;
                                 uint16_t *to = a.out + (size_t)(w.q.firstRow + mine / group) * a.outStride + (w.head * group + mine % group) * DIM + d;
 #pragma unroll
-                                for (uint32_t k = 0; k < 8 * kValues; k += 8)
-                                    *reinterpret_cast<uint4 *>(to + k) = make_uint4(pack_bf16x2(v[k] * f, v[k + 2] * f), pack_bf16x2(v[k + 4] * f, v[k + 6] * f),
-                                                                                    pack_bf16x2(v[k + 1] * f, v[k + 3] * f), pack_bf16x2(v[k + 5] * f, v[k + 7] * f));
+                                for (uint32_t k = 0; k < 4; ++k)  // value n of run k: column 8 (n % 4) + 2 k + n / 4
+                                    *reinterpret_cast<uint4 *>(to + 8 * k) = make_uint4(pack_bf16x2(v[2 * k] * f, v[8 + 2 * k] * f), pack_bf16x2(v[16 + 2 * k] * f, v[24 + 2 * k] * f),
+                                                                                        pack_bf16x2(v[2 * k + 1] * f, v[9 + 2 * k] * f), pack_bf16x2(v[17 + 2 * k] * f, v[25 + 2 * k] * f));
                             } else {
 #pragma unroll
                                 for (uint32_t h = 0; h < 2 * kValues; ++h) place(part_of(from))[h * kRows] = make_float4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]);
