@@ -72,12 +72,12 @@ class AttentionContext:
     # (A step of small calls is bound by the host: `get_device` and `is` cost a fifth of comparing torch.device objects, one
     # look at shape and strides a third of four.)
 
-    def _ints(self, **tensors: torch.Tensor):
+    def _ints(self, names: str, *tensors: torch.Tensor):
         """Refuses what is not a contiguous int32 tensor on the device."""
         i32, ordinal = torch.int32, self._ordinal
-        for t in tensors.values():
+        for t in tensors:
             if t.dtype is not i32 or t.get_device() != ordinal or not t.is_contiguous():
-                what = next(name for name, u in tensors.items() if u is t)
+                what = next(name for name, u in zip(names.split(), tensors) if u is t)
                 raise ValueError(f"{what} must be a contiguous int32 tensor on {self.device}")
 
     def _heads(self, t: torch.Tensor, heads: int, tokens: int, what: str) -> tuple:
@@ -125,8 +125,8 @@ class AttentionContext:
             raise ValueError("lengths, blockTable and rowStart must agree on the number of requests")
         if positions.numel() != rows or freeCount.numel() != 1 or freeCountOut.numel() != 1:
             raise ValueError("one position and one slot per row; one word for the stack's height")
-        self._ints(oldLengths=oldLengths, newLengths=newLengths, blockTable=blockTable, freePages=freePages, freeCount=freeCount,
-                   freeCountOut=freeCountOut, rowStart=rowStart, positions=positions, slots=slots)
+        self._ints("oldLengths newLengths blockTable freePages freeCount freeCountOut rowStart positions slots", oldLengths, newLengths,
+                   blockTable, freePages, freeCount, freeCountOut, rowStart, positions, slots)
         call("ff_cache_plan", self.handle, oldLengths.data_ptr(), newLengths.data_ptr(), requests, blockTable.data_ptr(), shape[1],
              freePages.data_ptr(), freePages.numel(), freeCount.data_ptr(), freeCountOut.data_ptr(), rowStart.data_ptr(),
              positions.data_ptr(), slots.data_ptr(), rows, _stream(stream))
@@ -152,7 +152,7 @@ class AttentionContext:
         if y is None:
             y = torch.empty((tokens, heads, self.headDim), dtype=torch.bfloat16, device=self.device)
         rope = self._rope(table, interleaved)
-        self._ints(positions=positions)
+        self._ints("positions", positions)
         call("ff_rope", self.handle, *self._heads(x, heads, tokens, "x"), ctypes.byref(rope), positions.data_ptr(), heads, tokens,
              *self._heads(y, heads, tokens, "y"), _stream(stream))
         return y
@@ -171,7 +171,7 @@ class AttentionContext:
                 qOut = torch.empty((tokens, self.heads, self.headDim), dtype=torch.bfloat16, device=self.device)
             query, out = self._heads(q, self.heads, tokens, "q"), self._heads(qOut, self.heads, tokens, "qOut")
         rope = self._rope(table, interleaved)
-        self._ints(positions=positions, slots=slots)
+        self._ints("positions slots", positions, slots)
         call("ff_cache_append", self.handle, *query, *self._heads(k, self.kvHeads, tokens, "k"), *self._heads(v, self.kvHeads, tokens, "v"),
              ctypes.byref(rope), positions.data_ptr(), slots.data_ptr(), tokens, *out, *self._cache(pages),
              _stream(stream))
@@ -188,7 +188,7 @@ class AttentionContext:
             v = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
         if not (k.is_contiguous() and v.is_contiguous()):
             raise ValueError("k and v must be contiguous")
-        self._ints(slots=slots)
+        self._ints("slots", slots)
         call("ff_cache_read", self.handle, *self._cache(pages), slots.data_ptr(), tokens, self._heads(k, self.kvHeads, tokens, "k")[0],
              self._heads(v, self.kvHeads, tokens, "v")[0], _stream(stream))
         return k, v
@@ -208,7 +208,7 @@ class AttentionContext:
             raise ValueError("window, sinks and maxRows must not be negative")
         if out is None:
             out = torch.empty((tokens, self.heads, self.headDim), dtype=torch.bfloat16, device=self.device)
-        self._ints(blockTable=blockTable, rowStart=rowStart, lengths=lengths)
+        self._ints("blockTable rowStart lengths", blockTable, rowStart, lengths)
         call("ff_attention", self.handle, *self._heads(q, self.heads, tokens, "q"), tokens, *self._cache(pages), blockTable.data_ptr(), shape[1],
              rowStart.data_ptr(), lengths.data_ptr(), requests, maxRows, self.headDim ** -0.5 if scale is None else scale, window, sinks,
              *self._heads(out, self.heads, tokens, "out"), _stream(stream))
