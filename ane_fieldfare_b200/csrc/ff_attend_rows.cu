@@ -1,4 +1,4 @@
-// Attention of few rows a request (decode steps, verify blocks) over the paged INT4 cache: bound by the cache's bytes.
+// Attention of up to 16 columns a key/value head (decode steps, short verify blocks) over the paged INT4 cache.
 //
 // The columns of a request's key/value head are its rows times the query heads that share the head; they stand in
 // tiles of 8 NT.  A unit of work is one (request, key/value head, column tile); its keys are tiles of 64, and all
@@ -15,7 +15,16 @@
 //   O += V p  codes of two keys are merged by a byte permute; the value scale goes into p (f16, one rounding more), at a
 //             power of two E that keeps the largest scale and bias of the unit so far within f16 (raised like the
 //             running maximum); one more MMA adds up p * bias per group and p itself.
-// Logits are then exact but for 32-bit sums; weights carry two roundings to 11 bits.
+// Logits are then exact but for 32-bit sums.  A weight is rounded to 11 bits once, for sum and output alike; times the value scale it
+// would be rounded again, so that the codes' and the biases' part of a value that is near zero would not cancel: what that
+// rounding leaves goes through a second product (up to four columns: through the four columns that a tile of eight has to spare).
+// A weight below 2^-24 of the largest of its warp's keys so far is lost.
+//
+// Bound by the cache's bytes and by latency.  131072 keys of 8 heads of 128 (151 MB) take 45 us, 3.3 TB/s or 51 % of a copy's
+// rate; with the arithmetic left out 33 us.  A warp executes 611 instructions for 32 keys of 128, all of the kernel's counted.  64
+// ragged requests (261 MB) take 75 us, 3.5 TB/s, at 46 % of the issue slots, and 53 us with the arithmetic left out.  Three CTAs an SM
+// with fewer registers a thread: 131072 keys 48.4 us where two take 44.3, ragged 73.4 and 73.1.  2000 keys of 8 heads of 256 are 13.5 us of
+// waits one after another: look-up of the requests 1.0, queries 1.7, tiles 3.4, joins in the CTA 1 and of the parts 2.
 #include <algorithm>
 #include <string>
 
@@ -140,7 +149,8 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
         return q;
     };
     // A unit costs its tiles and kUnitCost more: its queries, joins and output take as long.  (Cut by tiles alone, the CTAs with the
-    // short requests of a ragged batch took 94 us where the others took 62.)
+    // short requests of a ragged batch took 94 us where the others took 62.  kUnitCost 1, 3, 6, 8, 10, 14: ragged 90, 81, 72, 73,
+    // 74, 78 us, 4 x 16 rows in a window 42, 39, 36, 35, 37, 37; 1 and 3 with CTAs of two tiles or more, the others of three.)
     auto unit_cost = [](const RowsRequest &q) { return q.rows ? q.tiles + kUnitCost : 0u; };
     const uint32_t run = (a.requests + kRowsThreads - 1) / kRowsThreads;
     auto request_of = [&](uint32_t r) { return run == 1 ? known[r] : look_up(r); };  // (a batch of up to 160 is looked up once)
@@ -299,7 +309,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
         return;
     }
 
-    // ---------------- 16 keys of every tile ----------------
+    // ---------------- 32 keys of every second tile ----------------
     const uint32_t g = lane >> 2, t = lane & 3u;
     // A stage: [piece][keys, values][its keys][codes], then [piece][keys, values][its keys][words].  Warps 0 and 1 take half of
     // every second tile each, warps 2 and 3 of the others: 32 keys at a time as two subtiles of 16, for whose loads and products

@@ -1,4 +1,4 @@
-// Attention of many rows a request (prefill chunks) over the paged INT4 cache, on tcgen05: bound by the tensor core.
+// Attention of more than 16 columns a key/value head (verify blocks, prefill chunks) over the paged INT4 cache, on tcgen05.
 //
 // A row tile is up to 128 rows of one request and key/value head (tokens times the query heads that share the head).
 // A unit of work is one row tile; its keys are tiles of 64, and all units' tiles end to end are cut into equal runs, one
@@ -8,8 +8,8 @@
 // the expansion multiplies with; sixteen expand codes to f16 tiles in shared memory (128-byte swizzle, keys and values alike
 // [64 values][key][128 bytes]), four a slot, so that one group's waits stand behind the other's arithmetic; one issues the MMAs; two
 // warpgroups own a row a thread and take the tiles in turn:
-//   S = Q K^T   A: the rows' queries, in tensor memory for the whole unit (read from shared memory they would cost the
-//               128 bytes a cycle that dequantizing needs); B: the keys, K-major
+//   S = Q K^T   A: the rows' queries, in tensor memory for the whole unit (from shared memory an MMA of 64 keys takes 73
+//               cycles, from tensor memory 33); B: the keys, K-major
 //   P = 2^(S f + E - M)   in registers, back into S's columns as f16
 //   O += P V    A: P; B: the values, N-major; O stays in tensor memory
 // A tile's warpgroup waits for the maximum M that the one before it settled on, not for its weights; M moves, and O with it, only
@@ -19,8 +19,16 @@
 //
 // f16 holds 11 bits of keys, values and weights where bf16 would hold 8; its range is kept by powers of two: a row's
 // own for the queries, a tile's own for keys (taken back with the logits) and for values (E, part of the exponent of P and
-// of the maximum M that P stays below 2^8 of).  A code masked in place is the f16 code * 2^-24 or * 2^-20, and one FMA
-// with scale times 2^24 or 2^20 and the bias rounds once: nine instructions a word of eight codes.
+// of the maximum M that P stays below 2^14 of; keys and values of 2^116 and more are out of its reach).  A weight below 2^-30 of the largest of
+// its part of the keys is lost.  A code masked in place is the f16 code * 2^-24 or * 2^-20, and one FMA with scale times 2^24 or
+// 2^20 and the bias rounds once: nine instructions a word of eight codes.
+//
+// 4096 rows of 16 heads of 256 over 36864 keys take 2.19 ms, 1.07 PFLOP/s: 66 % of the burst bf16 rate, 78 % of the sustained one
+// (at 36864 keys the power limit holds the clock below its maximum).  A tile takes 1.16 us.  Its MMAs alone are 1077 cycles: 16 of
+// 32.8 and 4 of 138, each form timed by itself.  The tensor pipe is active 45 % of the time at 8192 keys: S of a tile waits in one of
+// two buffers until its weights are formed, and tensor memory has no third at 256 values a head.  4096 rows in a window of 1024 take
+// 143 us: 19 tiles a unit, beside which queries, first logits, output and parts of units count; five ragged requests of up to
+// 613 rows with 14 heads of 64 27.5 us.
 #include <algorithm>
 #include <string>
 
@@ -34,7 +42,8 @@ namespace {
 constexpr int kKeyCopyWarp = 0, kMmaWarp = 1, kScaleWarp = 2, kValueCopyWarp = 3, kDequantWarps = 16, kRowGroups = 2;
 constexpr int kFirstDequant = 4, kFirstRowWarp = kFirstDequant + kDequantWarps, kRowWarps = 4 * kRowGroups;
 constexpr int kTilesThreads = 32 * (kFirstRowWarp + kRowWarps);
-// registers a thread by role: together no more than the launch's 72 each
+// registers a thread by role: together no more than the launch's 72 each (4096 rows over 36864 keys, in one run: eight
+// expanding warps 2.34 ms, twelve 2.12 to 2.14, sixteen 2.01; a later run at another clock took 2.19)
 constexpr int kRegsOthers = 48, kRegsRows = 128;
 static_assert(128 * kRegsOthers + 32 * kDequantWarps * kRegsOthers + 32 * kRowWarps * kRegsRows <= kTilesThreads * 72, "register split");
 constexpr uint32_t kRows = kTileRows;

@@ -13,7 +13,8 @@ namespace ff {
 // pages and the table entries.  The k-th page taken is the k-th from the top of the stack as it stands with the
 // returned pages on it; where that is a returned page its id is read from the table entry it came from, which
 // nothing writes: a request either grows or shrinks.  So no value passes through memory that this launch writes.
-// Bound by latency: two rounds of loads, a scan, a search of eleven steps.
+// Bound by latency: two rounds of loads, a scan, a search of ten steps; 4.0 us for 16 requests of a decode step, 6.3 us for 1000
+// requests that grow, shrink and end (in a graph; a call from Python is 8.5 us of the host's time).
 constexpr int kPlanThreads = 1024;
 
 struct PlanArgs {
@@ -255,7 +256,10 @@ __device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
 }
 
 // A warp takes 256 values at a time, 256 / DIM heads of one row, eight values a lane, BATCH such steps' loads in flight.  Its
-// cosines and sines stay in registers for all the heads it takes.  Bound by the bytes of the rows.
+// cosines and sines stay in registers for all the heads it takes.  Bound by issue slots and the bytes of the rows together: 4096 rows
+// of 16 query and 2 x 8 key/value heads of 256 are 113 MB and take 29.6 us (3.8 TB/s, 58 % of a copy's rate) at 62 % of the issue
+// slots, 175 warp instructions for 256 values.  Two steps' loads in flight at 64 registers 29.6 us; four at 64 registers 38.3, four at 92
+// (a quarter of the SM's warps) 38.9.
 template <int DIM, bool INTERLEAVED, int BATCH>
 __global__ void __launch_bounds__(128, 8) k_rope_rows(const RopeArgs a) {
     constexpr uint32_t kLanes = DIM / 8, kHeads = 32 / kLanes;
@@ -438,7 +442,8 @@ struct ReadArgs {
     uint32_t *errorFlag;
 };
 
-// A warp takes 256 values at a time of one row, eight a lane, four such steps.  Bound by the bytes written.
+// A warp takes 256 values at a time of one row, eight a lane, four such steps.  Bound by the bytes written: 4096 rows of 2 x 8 heads of
+// 256, 43 MB, in 8.6 us (5.0 TB/s).
 template <int DIM>
 __global__ void __launch_bounds__(128) k_cache_read(const ReadArgs a) {
     constexpr uint32_t kLanes = DIM / 8, kHeads = 32 / kLanes, kSteps = 4;
