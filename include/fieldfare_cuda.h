@@ -558,7 +558,9 @@ bool ff_cache_read(FFAttention *attention, const void *pages, uint32_t pageCount
  * (rows outStride apart) = softmax(scale q.k) v; a row that sees no key, and rows behind the last request's, are zero.
  * maxRows: no request has more rows (it chooses the kernel; rows past it are zero, flag 15).  Up to 16 columns (rows times
  * heads/kvHeads) run on mma.sync on the codes as they lie, more on the 5th-generation tensor cores; either way the keys are
- * split over the CTAs, so that one request fills the GPU.  Keys on a page outside the cache are not seen (flag 16). */
+ * split over the CTAs, so that one request fills the GPU.  Keys on a page outside the cache are not seen (flag 16).
+ * Sums are fp32, factors f16 at powers of two of their own: weights below 2^-24 of the largest of their part of the keys may count
+ * as zero; keys and values from 2^116 on and queries from 2^110 on may give results that are not finite. */
 bool ff_attention(FFAttention *attention, const uint16_t *q, uint32_t qStride, uint32_t tokens, const void *pages,
                   uint32_t pageCount, const uint32_t *blockTable, uint32_t tableStride, const uint32_t *rowStart,
                   const uint32_t *lengths, uint32_t requests, uint32_t maxRows, float scale, uint32_t window,
