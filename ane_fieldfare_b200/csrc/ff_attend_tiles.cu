@@ -53,6 +53,8 @@ constexpr float kWeightScale = 6.0f;
 constexpr uint32_t kUnitCost = 8;  // tiles' time that a unit takes besides its tiles
 constexpr uint32_t kInfo = 4;   // tiles whose scales and exponents are kept
 constexpr uint32_t kSlots = 4, kPacked = 3;  // expanded tiles; packed ones, of keys and of values each
+// The values of tile m are item 2 m + 1 or 2 m + 2 of the expansion: those kPacked tiles before them are at least kSlots items before.
+static_assert(2 * kPacked - 1 >= kSlots, "a free slot says that the ring's place was read");
 
 struct TilesArgs {
     AttendArgs a;
@@ -587,12 +589,14 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
             bool ok = true;
             auto fill = [&](uint32_t n, uint32_t side) {  // keys or values of the CTA's n-th tile
                 const uint32_t slot = item % kSlots, slotPhase = item / kSlots & 1u, pack = n % kPacked + side * kPacked, packPhase = n / kPacked & 1u, info = n % kInfo;
-                if (!wait_lane<false>(barInfo + 8 * info, n / kInfo & 1u, &abortFlag) ||
-                    !wait_lane<false>(barPack + 8 * pack, packPhase, &abortFlag)) {
+                if (!wait_lane<false>(barInfo + 8 * info, n / kInfo & 1u, &abortFlag)) {
                     ok = false;
                     return;
                 }
-                if (!wait_lane<false>(barTileFree + 8 * slot, slotPhase ^ 1u, &abortFlag)) {
+                // The slot before the codes: it is free when the item kSlots before this one has been multiplied, and with it the
+                // values that lay in this place of the packed ring before.  Waiting for the codes first, a group that is ahead of the one
+                // that expands those (copies land in any order) would take the parity of the round before last for its own.
+                if (!wait_lane<false>(barTileFree + 8 * slot, slotPhase ^ 1u, &abortFlag) || !wait_lane<false>(barPack + 8 * pack, packPhase, &abortFlag)) {
                     ok = false;
                     return;
                 }

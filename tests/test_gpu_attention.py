@@ -298,6 +298,16 @@ def test_one_long_request_is_split_and_joined(dim, rows):
     b.check(b.attend(700, 5), 700, 5)
 
 
+@pytest.mark.parametrize("dim,page", [(64, 16), (64, 64), (128, 16), (256, 16)])
+def test_many_tiles_a_cta(dim, page):
+    """The rings of the kernel for many rows go round several times, with tiles whose pieces lie on several pages."""
+    b = Batch(16, 2, dim, page, [1500, 700], [260, 130])
+    want = b.attend().clone()
+    b.check(want)
+    for _ in range(20):
+        assert torch.equal(b.attend(), want)
+
+
 @pytest.mark.parametrize("rows", [[1, 1, 0], [5, 16, 0], [30, 2, 0]])
 def test_rows_without_keys_and_spare_rows_are_zero(rows):
     b = Batch(4, 2, 128, 16, [40, 33, 0], rows, extraRows=5)
