@@ -36,6 +36,7 @@ namespace {
 
 constexpr int kConsumers = 4;                      // warps that compute: two a tile, 32 keys each
 constexpr int kRowsThreads = 32 * (kConsumers + 1);
+constexpr uint32_t kWaitLimit = 1u << 20;
 constexpr uint32_t kUnitCost = 8;                 // tiles' time that a unit takes besides its tiles
 static_assert(kTileKeys == 64 && kConsumers == 4, "two warps a tile, 32 keys each");
 
@@ -86,6 +87,16 @@ __device__ __forceinline__ uint32_t nibbles(uint32_t w, uint32_t upper) {
     return (U < 2 ? w : upper) & (U % 2 ? 0x00F000F0u : 0x000F000Fu);
 }
 
+// The rest of a wait whose first look found nothing: up to a limit, or until another warp of the CTA has given up.
+__device__ __noinline__ void wait_rows(uint32_t bar, uint32_t parity, volatile uint32_t *abortFlag) {
+#pragma unroll 1
+    for (uint32_t i = 0; i < kWaitLimit; ++i) {
+        if ((i & 255u) == 0u && *abortFlag) return;
+        if (mbar_try_wait(bar, parity)) return;
+    }
+    *abortFlag = 1u;
+}
+
 // One request as the kernel sees it.
 struct RowsRequest {
     uint32_t firstRow, rows, tilesSink, lowTile, tiles, columnTiles;
@@ -112,6 +123,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
     __shared__ float2 joinStats[kConsumers][kColumns];
     __shared__ float joinBias[kConsumers][NG][kColumns];
     __shared__ uint32_t lastPart;
+    __shared__ volatile uint32_t abortFlag;  // a wait was given up: nothing more is copied, what there is to multiply and join goes on
     __shared__ RowsRequest known[kRowsThreads];
     const AttendArgs &a = args.a;
     const uint32_t tid = threadIdx.x, warp = (uint32_t)warp_index(), lane = tid & 31u;
@@ -120,6 +132,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
     const uint32_t group = a.heads / a.kvHeads;
     const uint32_t barFull = sm_addr(barriers), barEmpty = barFull + 8 * kStages;
     if (tid == 0) {
+        abortFlag = 0;
         for (uint32_t s = 0; s < kStages; ++s) {
             bar_init(barFull + 8 * s, 1);
             bar_init(barEmpty + 8 * s, kConsumers / 2);
@@ -260,6 +273,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
         const uint32_t tilesPer = 32u >> perTileShift;  // tiles whose pieces a warp holds
         const uint32_t pieceCodes = 2u * CB << args.pieceShift, pieceWords = 2u * WB << args.pieceShift;
         uint32_t stage = 0, phase = 0;
+        bool ok = true;
         Walk w = locate(begin);
         do {
             const uint32_t t0 = w.t0, count = w.count, head = w.head;
@@ -281,15 +295,15 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
                 return page;
             };
             uint32_t pagesNext = page_of(t0);
-            for (uint32_t t = t0; t < t0 + count; t += tilesPer) {
+            for (uint32_t t = t0; t < t0 + count && ok; t += tilesPer) {
                 const uint32_t pagesNow = pagesNext;
                 pagesNext = page_of(t + tilesPer);
                 const uint32_t many = min(tilesPer, t0 + count - t);
                 for (uint32_t i = 0; i < many; ++i) {
                     const uint32_t mine = __shfl_sync(0xFFFFFFFFu, pagesNow, (i << perTileShift) + (lane & (pieces - 1u)));
                     const uint32_t lives = __ballot_sync(0xFFFFFFFFu, lane < pieces && mine < a.pageCount);
-                    if (!mbar_try_wait(barEmpty + 8 * stage, phase ^ 1u) && !slot_wait_slow(barEmpty + 8 * stage, phase ^ 1u) && lane == 0) *a.errorFlag = kFlagWait;
-                    __syncwarp();
+                    if (!mbar_try_wait(barEmpty + 8 * stage, phase ^ 1u)) wait_rows(barEmpty + 8 * stage, phase ^ 1u, &abortFlag);
+                    if (!(ok = __all_sync(0xFFFFFFFFu, abortFlag == 0u))) break;  // (a stage may still wait for its copies)
                     const uint32_t bar = barFull + 8 * stage, base = ring + stage * kStage, inTile = key_at(t + i) & (a.page.pageTokens - 1u);
                     if (elect_one()) {
                         holes[stage] = ~lives;
@@ -305,7 +319,14 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
                     if (++stage == kStages) stage = 0, phase ^= 1u;
                 }
             }
-        } while (next_unit(w));
+        } while (ok && next_unit(w));
+        // also where a consumer gave up: no copy is in flight when the CTA ends
+        for (uint32_t s = 0; s < kStages; ++s) {
+            const uint32_t parity = s < stage ? phase : phase ^ 1u;
+#pragma unroll 1
+            for (uint32_t i = 0; i < kWaitLimit && !mbar_try_wait(barFull + 8 * s, parity); ++i) __nanosleep(40);
+        }
+        if (lane == 0 && abortFlag) *a.errorFlag = kFlagWait;
         return;
     }
 
@@ -422,7 +443,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
             const uint32_t tileKey = (i < w.q.tilesSink ? i : w.q.lowTile + i - w.q.tilesSink) * kTileKeys;
             const int j0 = (int)(tileKey + warpKey);
             const uint32_t base = ring + stage * kStage;
-            if (!mbar_try_wait(barFull + 8 * stage, phase) && !slot_wait_slow(barFull + 8 * stage, phase) && lane == 0) *a.errorFlag = kFlagWait;
+            if (!mbar_try_wait(barFull + 8 * stage, phase)) wait_rows(barFull + 8 * stage, phase, &abortFlag);
             __syncwarp();
             const uint32_t gone = holes[stage], hole0 = gone >> (warpKey >> args.pieceShift) & 1u, hole1 = gone >> ((warpKey + 16) >> args.pieceShift) & 1u;
             // keys that not every row of the tile sees
@@ -797,6 +818,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
         n0 += count;
         named_barrier(1, 32 * kConsumers);  // the joining buffers are free
     } while (next_unit(w));
+    if (lane == 0 && abortFlag) *a.errorFlag = kFlagWait;
 }
 
 KernelSmemMemo rowsMemo[3][3];

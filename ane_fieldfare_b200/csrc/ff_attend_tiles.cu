@@ -112,6 +112,12 @@ template <bool kSleep>
 __device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile uint32_t *abortFlag) {
     return __all_sync(0xFFFFFFFFu, wait_lane<kSleep>(bar, parity, abortFlag));
 }
+// The last wait of a role for what it issued, also after another one gave up.
+__device__ __forceinline__ void landed(uint32_t bar, uint32_t parity) {
+#pragma unroll 1
+    for (uint32_t i = 0; i < kWaitLimit && !mbar_try_wait(bar, parity); ++i) __nanosleep(40);
+    __syncwarp();
+}
 // two fp32 operations an instruction
 __device__ __forceinline__ unsigned long long pair_f32(float a, float b) {
     unsigned long long r;
@@ -164,7 +170,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
     constexpr uint32_t kGroupWarps = DIM == 64 ? 2 : 4, kGroups = kDequantWarps / kGroupWarps < kSlots ? kDequantWarps / kGroupWarps : kSlots, kUnitsEach = kUnits / (32 * kGroupWarps);
     constexpr uint32_t kColQ = 0, kColO = DIM / 2, kColS = kColO + DIM;
     extern __shared__ uint8_t tilesSmem[];
-    __shared__ __align__(8) uint64_t barriers[2 * kSlots + 4 * kPacked + 2 * kInfo + 2 + 4 + 2 + 1 + 1 + 8];
+    __shared__ __align__(8) uint64_t barriers[2 * kSlots + 4 * kPacked + 2 * kInfo + 2 + 4 + 2 + 1 + 1 + 8 + 1];
     __shared__ uint32_t tmemSlot, lastPart;
     __shared__ volatile uint32_t abortFlag;
     __shared__ uint32_t firstTile[kTilesThreads + 1], firstWork[kTilesThreads + 1], warpSums[32];
@@ -180,7 +186,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
     const uint32_t bar0 = sm_addr(barriers);
     const uint32_t barTile = bar0, barTileFree = barTile + 8 * kSlots, barPack = barTileFree + 8 * kSlots, barPackFree = barPack + 16 * kPacked;  // keys', then values'
     const uint32_t barInfo = barPackFree + 16 * kPacked, barInfoFree = barInfo + 8 * kInfo;
-    const uint32_t barS = barInfoFree + 8 * kInfo, barP = barS + 16, barO = barP + 32, barQ = barO + 16, barJoin = barQ + 8, barTop = barJoin + 8;
+    const uint32_t barS = barInfoFree + 8 * kInfo, barP = barS + 16, barO = barP + 32, barQ = barO + 16, barJoin = barQ + 8, barTop = barJoin + 8, barDone = barTop + 64;
     if (tid == 0) {
         abortFlag = 0;
         for (uint32_t s = 0; s < kSlots; ++s) {
@@ -204,6 +210,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
         mbar_init(barQ, kRowWarps);
         mbar_init(barJoin, kRowWarps);
         for (uint32_t s = 0; s < 8; ++s) mbar_init(barTop + 8 * s, 1);
+        mbar_init(barDone, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == (uint32_t)kMmaWarp) {
@@ -449,6 +456,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                     }
                 }
             }
+            // whatever the other roles did: no copy is in flight when the CTA ends
+            for (uint32_t s = 0; s < kPacked; ++s) landed(full + 8 * s, s < stage ? phase : phase ^ 1u);
         } else if (warp == (uint32_t)kMmaWarp) {
             // ---------------- MMAs ----------------
             uint32_t slot = 0, phase = 0, tile = 0, unitNo = 0;  // tile: key tiles so far (its S buffer, the barriers' parities)
@@ -501,6 +510,10 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                 }
                 ++unitNo;
             }
+            // nor any product, when tensor memory goes back
+            if (elect_one()) commit(barDone);
+            __syncwarp();
+            landed(barDone, 0);
         } else if (warp == (uint32_t)kScaleWarp) {
             // ---------------- scales: a lane two neighbouring keys of a tile ----------------
             // What no row sees is nothing; a visible key with a value (or a value of its value) that is no number is NaN, its value
@@ -589,17 +602,12 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
             bool ok = true;
             auto fill = [&](uint32_t n, uint32_t side) {  // keys or values of the CTA's n-th tile
                 const uint32_t slot = item % kSlots, slotPhase = item / kSlots & 1u, pack = n % kPacked + side * kPacked, packPhase = n / kPacked & 1u, info = n % kInfo;
-                if (!wait_lane<false>(barInfo + 8 * info, n / kInfo & 1u, &abortFlag)) {
-                    ok = false;
-                    return;
-                }
                 // The slot before the codes: it is free when the item kSlots before this one has been multiplied, and with it the
                 // values that lay in this place of the packed ring before.  Waiting for the codes first, a group that is ahead of the one
                 // that expands those (copies land in any order) would take the parity of the round before last for its own.
-                if (!wait_lane<false>(barTileFree + 8 * slot, slotPhase ^ 1u, &abortFlag) || !wait_lane<false>(barPack + 8 * pack, packPhase, &abortFlag)) {
-                    ok = false;
-                    return;
-                }
+                // (A lane that gives up goes on with what lies there, so that the warp ends the item as one.)
+                bool mine = wait_lane<false>(barInfo + 8 * info, n / kInfo & 1u, &abortFlag);
+                mine = mine && wait_lane<false>(barTileFree + 8 * slot, slotPhase ^ 1u, &abortFlag) && wait_lane<false>(barPack + 8 * pack, packPhase, &abortFlag);
 #pragma unroll 1
                 for (uint32_t e = 0; e < kUnitsEach; ++e) {
                     const uint32_t unit = e * (32 * kGroupWarps) + inGroup * 32 + lane, key = unit % kTileKeys, G = unit / kTileKeys;
@@ -623,8 +631,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                     }
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) {
+                ok = __all_sync(0xFFFFFFFFu, mine);
+                if (lane == 0 && ok) {
                     mbar_arrive(barPackFree + 8 * pack);
                     mbar_arrive(barTile + 8 * slot);
                 }
@@ -956,8 +964,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
             }
         }
     }
-    // every role is done, or gave up after a bounded wait; copies and products in flight have landed before the ends
-    // they were waited for
+    // every role is done, or gave up after a bounded wait; copies and products have landed
     tc_fence_before();
     __syncthreads();
     if (tid == 0 && abortFlag) *a.errorFlag = kFlagWait;
