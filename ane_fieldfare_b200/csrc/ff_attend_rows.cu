@@ -152,7 +152,8 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
         q.rows = min(rows, a.maxRows);
         if (q.rows == 0) return q;
         q.columnTiles = (q.rows * group + kColumns - 1) / kColumns;
-        const uint32_t ends = ((uint32_t)max(0, q.p0 + (int)q.rows) + kTileKeys - 1) / kTileKeys;
+        const uint32_t last = (uint32_t)max(0, q.p0 + (int)q.rows), ends = (min(last, a.tableKeys) + kTileKeys - 1) / kTileKeys;
+        if (last > a.tableKeys) *a.errorFlag = kFlagTableRow;  // (and what the row has no room for is not walked)
         if (a.window) {
             const uint32_t low = (uint32_t)max((long long)0, (long long)q.p0 - (long long)a.window + 1);
             q.lowTile = min(low / kTileKeys, ends);

@@ -240,7 +240,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
         q.firstRow = of.x + i * args.tileTokens;
         q.tokens = min(args.tileTokens, used - i * args.tileTokens);
         q.p0 = (int)of.z - (int)of.y + (int)(i * args.tileTokens);
-        const uint32_t ends = ((uint32_t)max(0, q.p0 + (int)q.tokens) + kTileKeys - 1) / kTileKeys;
+        const uint32_t last = (uint32_t)max(0, q.p0 + (int)q.tokens), ends = (min(last, a.tableKeys) + kTileKeys - 1) / kTileKeys;
+        if (last > a.tableKeys) *a.errorFlag = kFlagTableRow;  // (and what the row has no room for is not walked)
         q.lowTile = q.tilesSink = 0;
         if (a.window) {
             const uint32_t low = (uint32_t)max((long long)0, (long long)q.p0 - (long long)a.window + 1);

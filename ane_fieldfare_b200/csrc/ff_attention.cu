@@ -255,8 +255,9 @@ bool ff_attention(FFAttention *att, const uint16_t *q, uint32_t qStride, uint32_
     if (tableStride == 0 || maxRows == 0) return fail(error, "tableStride and maxRows must be positive");
     if (!(scale > 0.0f && scale < INFINITY)) return fail(error, "scale must be positive and finite");
     if (sinks && !window) return fail(error, "sinks need a window");
-    AttendArgs a{q, out, qStride, outStride, tokens, static_cast<const uint8_t *>(pages), pageCount, tableStride, blockTable, rowStart, lengths,
-                 requests, std::min(maxRows, std::max(1u, tokens)), scale, window, sinks, c.heads, c.kvHeads, page_layout(c), att->errorFlag};
+    AttendArgs a{q, out, qStride, outStride, tokens, static_cast<const uint8_t *>(pages), pageCount, tableStride,
+                 (uint32_t)std::min<uint64_t>((uint64_t)tableStride * c.pageTokens, UINT32_MAX), blockTable, rowStart, lengths, requests,
+                 std::min(maxRows, std::max(1u, tokens)), scale, window, sinks, c.heads, c.kvHeads, page_layout(c), att->errorFlag};
     return launch_attend(att, a, static_cast<cudaStream_t>(stream), error);
 }
 

@@ -65,7 +65,7 @@ struct AttendArgs {
     uint16_t *out;
     uint32_t qStride, outStride, tokens;
     const uint8_t *pages;
-    uint32_t pageCount, tableStride;
+    uint32_t pageCount, tableStride, tableKeys;  // tableKeys: those that a row of the block table has room for
     const uint32_t *blockTable, *rowStart, *lengths;
     uint32_t requests, maxRows;
     float scale;

@@ -487,6 +487,25 @@ def test_pages_outside_the_cache_are_not_read(rows):
     assert b.ctx.info().deviceErrorFlag == 14
 
 
+@pytest.mark.parametrize("rows", [1, 7, 40])
+@pytest.mark.parametrize("requests,length", [(1, 113), (1, 100_000), (3, -1), (64, -1)])
+def test_a_length_past_the_table_row_ends_with_it(rows, requests, length):
+    """The keys that the table has room for are seen, those behind it do not exist and take no time."""
+    heads, kvHeads, dim, page = 8, 8, 64, 16
+    b = Batch(heads, kvHeads, dim, page, [112] * requests, [rows] * requests, tableExtra=0)
+    keys, values = R.unpack(b.cache.cpu().numpy(), kvHeads, dim, page)
+    b.lengths = [length] * requests
+    for window, sinks in ((0, 0), (1 << 30, 3), (64, 3)):
+        p = [(length if length > 0 else 2 ** 31 - 1) - rows + i for i in range(rows)] * requests
+        mine = [b.slots[n // rows] for n in range(requests * rows)]
+        seen = [[s for j, s in enumerate(mine[n]) if j <= p[n] and (not window or j > p[n] - window or j < sinks)] for n in range(requests * rows)]
+        want, bound = R.attention(numbers(b.q), keys, values, seen, [len(s) for s in seen], [1] * len(seen), 0, 0, dim ** -0.5)
+        got = numbers(b.attend(window, sinks))
+        assert np.all(np.abs(got - want) <= 2.0 ** -8 * np.abs(want) + bound)
+        assert b.ctx.info().deviceErrorFlag == 14
+        b.ctx.resetDeviceError()
+
+
 # ---- refusals --------------------------------------------------------------------------------------
 
 
