@@ -153,7 +153,6 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
         if (q.rows == 0) return q;
         q.columnTiles = (q.rows * group + kColumns - 1) / kColumns;
         const uint32_t last = (uint32_t)max(0, q.p0 + (int)q.rows), ends = (min(last, a.tableKeys) + kTileKeys - 1) / kTileKeys;
-        if (last > a.tableKeys) *a.errorFlag = kFlagTableRow;  // (and what the row has no room for is not walked)
         if (a.window) {
             const uint32_t low = (uint32_t)max((long long)0, (long long)q.p0 - (long long)a.window + 1);
             q.lowTile = min(low / kTileKeys, ends);
@@ -169,17 +168,21 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
     const uint32_t run = (a.requests + kRowsThreads - 1) / kRowsThreads;
     auto request_of = [&](uint32_t r) { return run == 1 ? known[r] : look_up(r); };  // (a batch of up to 160 is looked up once)
     const uint32_t r0 = min(tid * run, a.requests), r1 = min(r0 + run, a.requests);
+    // rowStart goes back, to rows that several requests would write: such a call is refused like one with too much work
+    auto goes_back = [&](uint32_t r) { return __ldg(a.rowStart + r + 1) < __ldg(a.rowStart + r); };
     uint32_t sum = 0;
     for (uint32_t r = r0; r < r1; ++r) {
         const RowsRequest q = look_up(r);
         if (run == 1) known[r] = q;
-        sum += unit_cost(q) * q.columnTiles * a.kvHeads;
+        if (q.rows && q.p0 + (int)q.rows > 0 && (uint32_t)(q.p0 + (int)q.rows) > a.tableKeys) *a.errorFlag = kFlagTableRow;  // (what the row has no room for is not walked)
+        sum = add_work(sum, work_of(unit_cost(q), q.columnTiles * a.kvHeads));
+        if (goes_back(r)) sum = kTooMuch;
     }
     uint32_t scan = sum;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
         const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, scan, d);
-        if (lane >= (uint32_t)d) scan += v;
+        if (lane >= (uint32_t)d) scan = add_work(scan, v);
     }
     if (lane == 31u) warpSums[warp] = scan;
     __syncthreads();
@@ -187,21 +190,26 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
 #pragma unroll
     for (uint32_t w = 0; w <= (uint32_t)kConsumers; ++w) {
         if (w < warp) before += warpSums[w];
-        total += warpSums[w];
+        total = add_work(total, warpSums[w]);
     }
+    const bool refused = total == kTooMuch;  // (the places of units are nothing then)
     first[tid] = before + scan - sum;
     if (tid == 0) first[kRowsThreads] = total;
     __syncthreads();
 
     // rows that no unit writes: behind the last request's, and past maxRows
     {
-        const uint32_t covered = a.requests ? min(__ldg(a.rowStart + a.requests), a.tokens) : 0u;
+        const uint32_t covered = a.requests && !refused ? min(__ldg(a.rowStart + a.requests), a.tokens) : 0u;
         const uint32_t perRow = a.heads * DIM / 8;
         for (uint32_t row = covered + blockIdx.x; row < a.tokens; row += gridDim.x)
             for (uint32_t i = tid; i < perRow; i += kRowsThreads) *reinterpret_cast<uint4 *>(a.out + (size_t)row * a.outStride + i * 8) = make_uint4(0u, 0u, 0u, 0u);
         if (blockIdx.x == 0) {
+            if (tid == 0 && refused) *a.errorFlag = kFlagWork;
+            __syncthreads();
             if (tid == 0 && a.requests && __ldg(a.rowStart + a.requests) > a.tokens) *a.errorFlag = kFlagRows;
             for (uint32_t r = r0; r < r1; ++r) {
+                if (goes_back(r)) *a.errorFlag = kFlagRows;
+                if (refused) continue;
                 const uint32_t begin = min(__ldg(a.rowStart + r), a.tokens), end = min(__ldg(a.rowStart + r + 1), a.tokens);
                 for (uint32_t row = begin + a.maxRows; row < end; ++row) {
                     *a.errorFlag = kFlagRows;
@@ -210,7 +218,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
             }
         }
     }
-    if (total == 0) return;
+    if (total == 0 || refused) return;
     const uint32_t ctas = min(gridDim.x, max(1u, total / 3u)), cta = blockIdx.x;
     if (cta >= ctas) return;
     auto start_of = [&](uint32_t c) { return (uint32_t)((unsigned long long)c * total / ctas); };

@@ -241,7 +241,6 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
         q.tokens = min(args.tileTokens, used - i * args.tileTokens);
         q.p0 = (int)of.z - (int)of.y + (int)(i * args.tileTokens);
         const uint32_t last = (uint32_t)max(0, q.p0 + (int)q.tokens), ends = (min(last, a.tableKeys) + kTileKeys - 1) / kTileKeys;
-        if (last > a.tableKeys) *a.errorFlag = kFlagTableRow;  // (and what the row has no room for is not walked)
         q.lowTile = q.tilesSink = 0;
         if (a.window) {
             const uint32_t low = (uint32_t)max((long long)0, (long long)q.p0 - (long long)a.window + 1);
@@ -256,7 +255,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
             const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, scan, d);
-            if (lane >= (uint32_t)d) scan += v;
+            if (lane >= (uint32_t)d) scan = add_work(scan, v);
         }
         if (lane == 31u) warpSums[warp] = scan;
         __syncthreads();
@@ -265,7 +264,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
             const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, sums, d);
-            if (lane >= (uint32_t)d) sums += v;
+            if (lane >= (uint32_t)d) sums = add_work(sums, v);
         }
         const uint32_t total = __shfl_sync(0xFFFFFFFFu, sums, 31);
         first[tid] = __shfl_sync(0xFFFFFFFFu, sums - mine, warp) + scan - sum;
@@ -283,13 +282,17 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
         return low;
     };
     const uint32_t r0 = min(tid * run, a.requests), r1 = min(r0 + run, a.requests);
+    // rowStart goes back, to rows that several requests would write: such a call is refused like one with too much work
+    auto goes_back = [&](uint32_t r) { return __ldg(a.rowStart + r + 1) < __ldg(a.rowStart + r); };
     uint32_t mineTiles = 0;
     for (uint32_t r = r0; r < r1; ++r) {
         const uint3 of = look_up(r);
         if (run == 1) known[r] = of;
-        mineTiles += (min(of.y, a.maxRows) + args.tileTokens - 1) / args.tileTokens;
+        mineTiles = goes_back(r) ? kTooMuch : add_work(mineTiles, (min(of.y, a.maxRows) + args.tileTokens - 1) / args.tileTokens);
+        if (of.y && (int)of.z - (int)of.y + (int)min(of.y, a.maxRows) > 0 && of.z - of.y + min(of.y, a.maxRows) > a.tableKeys) *a.errorFlag = kFlagTableRow;  // (what the row has no room for is not walked)
     }
-    const uint32_t rowTiles = block_scan(mineTiles, firstTile);
+    const uint32_t allTiles = block_scan(mineTiles, firstTile);
+    const uint32_t rowTiles = allTiles == kTooMuch ? 0u : allTiles;
     // the n-th row tile
     struct Place {
         uint32_t r, i, count;  // request, row tile of it, row tiles that it has
@@ -320,21 +323,27 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
     if (n0 < n1) {
         Place p = place_of(n0);
         for (uint32_t n = n0; n < n1; ++n) {
-            work += (row_tile(p.r, p.i).tiles + kUnitCost) * a.kvHeads;
+            work = add_work(work, work_of(row_tile(p.r, p.i).tiles + kUnitCost, a.kvHeads));
             if (n + 1 < n1) advance(p);
         }
     }
-    const uint32_t total = block_scan(work, firstWork);
+    const uint32_t allWork = block_scan(work, firstWork);
+    const bool refused = allTiles == kTooMuch || allWork == kTooMuch;  // (the places of units are nothing then)
+    const uint32_t total = refused ? 0u : allWork;
 
     // rows that no unit writes: behind the last request's, and past maxRows
     {
-        const uint32_t covered = a.requests ? min(__ldg(a.rowStart + a.requests), a.tokens) : 0u;
+        const uint32_t covered = a.requests && !refused ? min(__ldg(a.rowStart + a.requests), a.tokens) : 0u;
         const uint32_t perRow = a.heads * DIM / 8;
         for (uint32_t row = covered + blockIdx.x; row < a.tokens; row += gridDim.x)
             for (uint32_t i = tid; i < perRow; i += kTilesThreads) *reinterpret_cast<uint4 *>(a.out + (size_t)row * a.outStride + i * 8) = make_uint4(0u, 0u, 0u, 0u);
         if (blockIdx.x == 0) {
+            if (tid == 0 && refused) *a.errorFlag = kFlagWork;
+            __syncthreads();
             if (tid == 0 && a.requests && __ldg(a.rowStart + a.requests) > a.tokens) *a.errorFlag = kFlagRows;
             for (uint32_t r = r0; r < r1; ++r) {
+                if (goes_back(r)) *a.errorFlag = kFlagRows;
+                if (refused) continue;
                 const uint32_t begin = min(__ldg(a.rowStart + r), a.tokens), end = min(__ldg(a.rowStart + r + 1), a.tokens);
                 for (uint32_t row = begin + a.maxRows; row < end; ++row) {
                     *a.errorFlag = kFlagRows;

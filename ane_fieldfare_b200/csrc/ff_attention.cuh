@@ -26,6 +26,7 @@ enum AttentionFlag : uint32_t {
     kFlagPage = 16,
     kFlagWait = 17,
     kFlagPosition = 18,
+    kFlagWork = 19,
 };
 
 // A block: one key/value head of one page.  Offsets in bytes from its start.

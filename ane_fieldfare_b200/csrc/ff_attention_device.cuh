@@ -78,6 +78,11 @@ __device__ __forceinline__ uint32_t chunk_flip(uint32_t key) {
     return DIM == 256 ? (key & 7u) << 4 : DIM == 128 ? ((key >> 1) & 3u) << 4 : ((key >> 2) & 1u) << 4;
 }
 
+// Work is counted in tiles, in 32 bits; what does not fit (seconds of the GPU's time) stays at the largest number, kTooMuch.
+constexpr uint32_t kTooMuch = 0xFFFFFFFFu;
+__device__ __forceinline__ uint32_t add_work(uint32_t a, uint32_t b) { return a + b < a ? kTooMuch : a + b; }
+__device__ __forceinline__ uint32_t work_of(uint32_t tiles, uint32_t units) { return __umulhi(tiles, units) ? kTooMuch : tiles * units; }
+
 // The cache's pages as tensors: codes [blocks][keys, values][tokens][bytes], a box the part of a tile that lies on one page, of
 // `sides` of the two; scale words [blocks][keys, values][words], a box both sides of such a part.
 bool make_pages_maps(CUtensorMap *codes, CUtensorMap *words, const AttendArgs &a, uint32_t dim, uint32_t sides, const char **error);

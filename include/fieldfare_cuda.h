@@ -479,8 +479,10 @@ void ff_attention_destroy(FFAttention *attention);
 FFAttentionInfo ff_attention_get_info(const FFAttention *attention);
 /* Waits for the device and clears the flag that FFAttentionInfo reports.  It is sticky; a kernel sets it to
  * 13: no free page was left, 14: a request is longer than its block table row, 15: more rows than the
- * arrays hold, 16: a page or slot outside the cache, 17: a wait was given up, 18: a position outside the
- * rotary table.  What such an entry names is left out; nothing outside the arrays is touched. */
+ * arrays hold, or a rowStart that goes back (every row is zero then), 16: a page or slot outside the cache, 17: a wait was
+ * given up, 18: a position outside the rotary table, 19: more work in a call of ff_attention than 2^32 tiles of 64 keys,
+ * counted for every head and tile of rows (every row is zero then).  What such an entry names is left out; nothing outside
+ * the arrays is touched. */
 bool ff_attention_reset_device_error(FFAttention *attention, const char **error);
 /* Bytes of one page of one layer; 0 for a configuration that ff_attention_create refuses. */
 uint64_t ff_cache_page_bytes(const FFAttentionConfig *config);

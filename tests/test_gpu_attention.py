@@ -506,6 +506,28 @@ def test_a_length_past_the_table_row_ends_with_it(rows, requests, length):
         b.ctx.resetDeviceError()
 
 
+@pytest.mark.parametrize("rows", [1, 40])
+def test_row_starts_that_go_back_are_reported(rows):
+    b = Batch(4, 2, 64, 16, [100, 90, 80], [rows] * 3)
+    args = ints(b.table), ints([0, 2 * rows, rows, 3 * rows]), ints(b.lengths), 2 * rows
+    out = b.ctx.attend(b.q, b.cache, *args, out=torch.full_like(b.q, 7.0))
+    assert not out.any()
+    assert b.ctx.info().deviceErrorFlag == 15
+    b.ctx.resetDeviceError()
+    b.check(b.attend())
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_more_work_than_a_call_counts_is_reported(rows):
+    """1024 heads over a table of 2^31 keys, none of them there: 2^35 tiles."""
+    ctx = context(1024, 1024, 64, 16, requests=1, tokens=rows)
+    q = rows_of(generator(), rows, 1024, 64)
+    table = torch.full((1, 1 << 27), -1, dtype=torch.int32, device="cuda")
+    out = ctx.attend(q, ctx.newCache(1), table, ints([0, rows]), ints([2 ** 31 - 1]), rows, out=torch.full_like(q, 7.0))
+    assert not out.any()
+    assert ctx.info().deviceErrorFlag == 19
+
+
 # ---- refusals --------------------------------------------------------------------------------------
 
 
