@@ -176,6 +176,7 @@ bool ff_cache_plan(FFAttention *att, const uint32_t *oldLengths, const uint32_t 
                           reinterpret_cast<uintptr_t>(rowStart) | reinterpret_cast<uintptr_t>(positions) | reinterpret_cast<uintptr_t>(slots);
     if (all & 3u) return fail(error, "arrays must be 4-byte aligned");
     if (tableStride == 0) return fail(error, "tableStride must be positive");
+    if ((uint64_t)requests * tableStride > 1u << 30) return fail(error, "the block table has more than 2^30 entries");
     if ((uint64_t)pageCount * att->cfg.pageTokens >= FF_NO_SLOT) return fail(error, "the cache has more slots than 32 bits name");
     return launch_cache_plan(att, oldLengths, newLengths, requests, blockTable, tableStride, freePages, pageCount, freeCountIn, freeCountOut,
                              rowStart, positions, slots, rows, static_cast<cudaStream_t>(stream), error);

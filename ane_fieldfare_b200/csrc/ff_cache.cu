@@ -30,6 +30,11 @@ struct PlanArgs {
     uint32_t *done, *errorFlag;
 };
 
+// Rows are counted up to here, what is more stays there: more than the arrays hold by far (2^24), and two counts add up in 32
+// bits.  (A length that is none, as -1, would make the sums wrap.)  Pages are at most the table's entries, which are no more.
+constexpr uint32_t kMost = 1u << 30;
+__device__ __forceinline__ uint32_t add_counts(uint32_t a, uint32_t b) { return min(a + b, kMost); }
+
 struct PlanRequest {
     uint32_t rows, had, has;  // new rows; pages before and after, as far as the table row goes
     uint32_t oldLength;
@@ -42,7 +47,7 @@ __device__ __forceinline__ PlanRequest plan_request(const PlanArgs &a, uint32_t 
     const uint32_t mask = (1u << a.pageShift) - 1u;
     PlanRequest p;
     p.oldLength = before;
-    p.rows = after > before ? after - before : 0u;
+    p.rows = after > before ? min(after - before, kMost) : 0u;
     const uint32_t had = (before >> a.pageShift) + ((before & mask) != 0u), has = (after >> a.pageShift) + ((after & mask) != 0u);
     p.cut = had > a.tableStride || has > a.tableStride;
     p.had = min(had, a.tableStride);
@@ -65,36 +70,38 @@ __global__ void __launch_bounds__(kPlanThreads) k_cache_plan(const PlanArgs a) {
     bool cut = false;
     for (uint32_t r = r0; r < r1; ++r) {
         const PlanRequest p = plan_request(a, r);
-        sum[0] += p.rows;
+        sum[0] = add_counts(sum[0], p.rows);
         sum[1] += p.taken();
         sum[2] += p.given();
         cut |= p.cut;
     }
-    uint32_t scan[3];
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-        scan[i] = sum[i];
+    uint32_t before[3];  // sums over the warp's lanes before this one
+    auto scan = [&](uint32_t own, uint32_t &all) {
+        uint32_t s = own;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
-            const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, scan[i], d);
-            if (lane >= (uint32_t)d) scan[i] += v;
+            const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, s, d);
+            if (lane >= (uint32_t)d) s = add_counts(s, v);
         }
-        if (lane == 31u) warpSum[i][warp] = scan[i];
+        all = s;  // (lane 31's is the warp's)
+        const uint32_t front = __shfl_up_sync(0xFFFFFFFFu, s, 1);
+        return lane ? front : 0u;
+    };
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+        uint32_t all;
+        before[i] = scan(sum[i], all);
+        if (lane == 31u) warpSum[i][warp] = all;
     }
     __syncthreads();
     if (warp < 3u) {
-        uint32_t v = warpSum[warp][lane], s = v;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const uint32_t u = __shfl_up_sync(0xFFFFFFFFu, s, d);
-            if (lane >= (uint32_t)d) s += u;
-        }
-        warpSum[warp][lane] = s - v;
-        if (lane == 31u) first[warp][kPlanThreads] = s;
+        uint32_t all;
+        warpSum[warp][lane] = scan(warpSum[warp][lane], all);
+        if (lane == 31u) first[warp][kPlanThreads] = all;
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 3; ++i) first[i][t] = warpSum[i][warp] + scan[i] - sum[i];
+    for (int i = 0; i < 3; ++i) first[i][t] = add_counts(warpSum[i][warp], before[i]);
     __syncthreads();
     const uint32_t totalRows = first[0][kPlanThreads], totalTaken = first[1][kPlanThreads], totalGiven = first[2][kPlanThreads];
 
@@ -166,7 +173,7 @@ __global__ void __launch_bounds__(kPlanThreads) k_cache_plan(const PlanArgs a) {
         uint32_t row = first[0][t];
         for (uint32_t r = r0; r < r1; ++r) {
             a.rowStart[r] = row;
-            row += plan_request(a, r).rows;
+            row = add_counts(row, plan_request(a, r).rows);
         }
         if (t == 0) a.rowStart[a.requests] = totalRows;
         if (cut) *a.errorFlag = kFlagTableRow;

@@ -92,6 +92,23 @@ def test_plan_without_pages_or_room_says_so_and_stays_inside():
     assert ctx.info().deviceErrorFlag == 15
 
 
+@pytest.mark.parametrize("requests", [4, 1500])
+def test_plan_of_lengths_that_are_none(requests):
+    """Words of -1 in a batch: their requests end with their table rows, and the arrays with themselves."""
+    ctx = context(page=16, requests=requests)
+    new = [5] + [-1] * (requests - 2) + [7]
+    pages = 2 * requests
+    got = run_plan(ctx, [0] * requests, new, np.full((requests, 2), 99999), np.arange(pages), pages, 48)
+    want = np.arange(pages)[::-1]
+    assert got["table"].tolist() == [[want[0], 99999]] + [[want[1 + 2 * r], want[2 + 2 * r]] for r in range(requests - 2)] + [[want[2 * requests - 3], 99999]]
+    assert got["count"][0] == 2
+    assert got["positions"].tolist() == list(range(5)) + list(range(43))
+    slot = lambda r, p: -1 if p >= 32 else got["table"][r, p // 16] * 16 + p % 16  # noqa: E731
+    assert got["slots"].tolist() == [slot(0, p) for p in range(5)] + [slot(1, p) for p in range(43)]
+    assert got["start"][:2].tolist() == [0, 5] and (got["start"][2:] >= 48).all()
+    assert ctx.info().deviceErrorFlag in (14, 15)
+
+
 # ---- rotary positions and append -----------------------------------------------------------------
 
 
@@ -568,6 +585,16 @@ def test_arguments_that_the_library_refuses():
     with pytest.raises(FieldfareError, match="maxRequests"):
         ctx.plan(ints([0] * 3), ints([0] * 3), ints(np.zeros((3, 2))), ints([0]), ints([0]), ints([0]), ints([0] * 4), ints([0]), ints([0]))
     assert ctx.attend(b.q[:0], b.cache, ints(b.table), ints([0, 0, 0]), ints(b.lengths), 1).shape == (0, 4, 64)
+
+
+def test_a_table_that_is_too_large_to_count_is_refused():
+    from ane_fieldfare_b200.attention import FieldfareError
+    from ane_fieldfare_b200.binding import call
+
+    ctx, word = context(requests=4), ints([0] * 8)
+    with pytest.raises(FieldfareError, match="2\\^30"):
+        call("ff_cache_plan", ctx.handle, word.data_ptr(), word.data_ptr(), 4, word.data_ptr(), (1 << 28) + 1, word.data_ptr(), 1, word.data_ptr(),
+             word.data_ptr(), word.data_ptr(), word.data_ptr(), word.data_ptr(), 1, None)
 
 
 def test_kernels_are_counted():
