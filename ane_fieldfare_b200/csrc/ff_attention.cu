@@ -158,7 +158,11 @@ FFAttentionInfo ff_attention_get_info(const FFAttention *att) {
 bool ff_attention_reset_device_error(FFAttention *att, const char **error) {
     if (!begin(att, error)) return false;
     FF_CUDA_OK(cudaDeviceSynchronize(), error);
+    // a call that gave up a wait (flag 17) leaves counts behind; the next one would join parts that are not there yet
+    FF_CUDA_OK(cudaMemset(att->arrived, 0, 3 * att->rowsCtas * sizeof(uint32_t)), error);
+    FF_CUDA_OK(cudaMemset(att->planCount, 0, sizeof(uint32_t)), error);
     FF_CUDA_OK(cudaMemset(att->errorFlag, 0, sizeof(uint32_t)), error);
+    FF_CUDA_OK(cudaDeviceSynchronize(), error);  // (a memset may return before it is done; other streams do not wait for it)
     return true;
 }
 

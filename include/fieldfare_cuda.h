@@ -477,7 +477,8 @@ typedef struct {
 FFAttention *ff_attention_create(int32_t deviceOrdinal, const FFAttentionConfig *config, const char **error);
 void ff_attention_destroy(FFAttention *attention);
 FFAttentionInfo ff_attention_get_info(const FFAttention *attention);
-/* Waits for the device and clears the flag that FFAttentionInfo reports.  It is sticky; a kernel sets it to
+/* Waits for the device and clears the flag that FFAttentionInfo reports, and what a call that gave up a wait leaves in
+ * the handle: after flag 17 results are undefined until this is called.  It is sticky; a kernel sets it to
  * 13: no free page was left, 14: a request is longer than its block table row, 15: more rows than the
  * arrays hold, or a rowStart that goes back (every row is zero then), 16: a page or slot outside the cache, 17: a wait was
  * given up, 18: a position outside the rotary table, 19: more work in a call of ff_attention than 2^32 tiles of 64 keys,

@@ -545,6 +545,33 @@ def test_more_work_than_a_call_counts_is_reported(rows):
     assert ctx.info().deviceErrorFlag == 19
 
 
+@pytest.mark.parametrize("rows", [1, 40])
+def test_a_reset_clears_what_a_call_that_gave_up_leaves(rows):
+    """The counts of parts that have arrived: no call leaves them but one that gave up a wait, so they are set from outside."""
+    import ctypes
+
+    class Handle(ctypes.Structure):  # FFAttention of csrc/ff_attention.cuh, up to the counts
+        _fields_ = [("device", ctypes.c_int), ("smCount", ctypes.c_int), ("config", ctypes.c_uint32 * 6), ("errorFlag", ctypes.c_void_p),
+                    ("planCount", ctypes.c_void_p), ("rowsCtas", ctypes.c_uint32), ("partials", ctypes.c_void_p), ("stats", ctypes.c_void_p),
+                    ("arrived", ctypes.c_void_p)]
+
+    class Words:
+        def __init__(self, pointer, count):
+            self.__cuda_array_interface__ = {"shape": (count,), "typestr": "<i4", "data": (pointer, False), "version": 3}
+
+    b = Batch(4, 2, 64, 16, [3000], [rows])
+    handle = ctypes.cast(b.ctx.handle, ctypes.POINTER(Handle)).contents
+    assert list(handle.config)[:4] == [4, 2, 64, 16] and handle.rowsCtas == 2 * handle.smCount
+    arrived = torch.as_tensor(Words(handle.arrived, 3 * handle.rowsCtas), device="cuda")
+    planned = torch.as_tensor(Words(handle.planCount, 1), device="cuda")
+    assert not arrived.any() and not planned.any()
+    arrived.fill_(1)
+    planned.fill_(1)
+    b.ctx.resetDeviceError()
+    assert not arrived.any() and not planned.any()
+    b.check(b.attend())
+
+
 # ---- refusals --------------------------------------------------------------------------------------
 
 
