@@ -425,8 +425,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
 #pragma unroll
                 for (int G = 0; G < NG; ++G) qSum[G][n][c] = __shfl_sync(0xFFFFFFFFu, mine[G], from) * 0x1p-24f;
                 // q = f16 * 2^(exponent - 140), the codes are 2^-24 of theirs
-                const int e = (int)__shfl_sync(0xFFFFFFFFu, exponent, from) - 116, half = e >> 1;
-                toLog2[n][c] = a.scale * 1.4426950408889634f * power_of_two(half) * power_of_two(e - half);
+                toLog2[n][c] = logit_factor(a.scale, (int)__shfl_sync(0xFFFFFFFFu, exponent, from) - 116);
             }
         }
 

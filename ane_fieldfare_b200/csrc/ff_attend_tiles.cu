@@ -708,7 +708,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                     }
                     if (!meet()) break;
                     auto exponent_of = [&](uint32_t r) { return max(max(largestShared[0][r], largestShared[1][r]), 7u); };
-                    toLog2 = a.scale * 1.4426950408889634f * power_of_two((int)exponent_of(row) - 134);
+                    toLog2 = logit_factor(a.scale, (int)exponent_of(row) - 134);
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         float down[2];
@@ -768,7 +768,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                         most[2] = fmaxf(fmaxf(most[2], u[c]), u[c + 2 < 32 ? c + 2 : c]);
                         most[3] = fmaxf(fmaxf(most[3], u[c + 1]), u[c + 3 < 32 ? c + 3 : c + 1]);
                     }
-                    const float f = toLog2 * about.x, peak = fmaf(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])), f, about.y);
+                    const float f = fmaxf(toLog2 * about.x, 0x1p-126f), peak = fmaf(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])), f, about.y);
                     // the maximum that the tile before settled on
                     float top = kNone;
                     if (i) {

@@ -67,6 +67,12 @@ __device__ __forceinline__ float low16(uint32_t w) { return __uint_as_float(w <<
 __device__ __forceinline__ float high16(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
 // 2^e, 0 below the normal numbers
 __device__ __forceinline__ float power_of_two(int e) { return e < -126 ? 0.0f : __uint_as_float((uint32_t)(min(e, 127) + 127) << 23); }
+// The factor from a product's units to logits: scale, log2 e and 2^e.  Never 0, which times the -infinity of a key that is not seen would be
+// no number: below the smallest number all logits are 0 as far as 32 bits go.
+__device__ __forceinline__ float logit_factor(float scale, int e) {
+    const int half = e >> 1;
+    return fmaxf(scale * 1.4426950408889634f * power_of_two(half) * power_of_two(e - half), 0x1p-149f);
+}
 // a scale word whose scale or bias is no number: its group of values stands for NaN
 __device__ __forceinline__ bool is_broken(uint32_t w) { return (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u; }
 // exponent field of the larger of 16 scale and |bias|

@@ -379,6 +379,30 @@ def test_queries_of_any_size(rows, power):
     b.check(b.attend(scale=128 ** -0.5 / 2.0 ** power), scale=128 ** -0.5 / 2.0 ** power)
 
 
+@pytest.mark.parametrize("rows", [1, 4, 33])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (20, 2)])
+@pytest.mark.parametrize("which", ["all zero", "one zero", "tiny", "zero keys"])
+@pytest.mark.parametrize("power", [0, -80])
+def test_rows_whose_logits_vanish(rows, window, sinks, which, power):
+    """Queries of zero, or so small that no logit differs from zero: the mean of the visible values; their neighbours stay."""
+    b = Batch(4, 2, 128, 16, [150, 70], [rows, max(1, rows - 3)])
+    if which == "all zero":
+        b.q.zero_()
+    elif which == "one zero":
+        b.q[rows // 2, 1] = 0
+        b.q[rows] = 0
+    elif which == "tiny":
+        b.q = (b.q.float() * 2.0 ** -125).bfloat16()
+    else:
+        b.q = (b.q.float() * 2.0 ** -60).bfloat16()
+        many = 220
+        b.k[:130] = 0
+        b.ctx = context(4, 2, 128, 16, tokens=many)
+        b.ctx.append(None, b.k, b.v, None, ints([0] * many), ints([s for mine in b.slots for s in mine]), b.cache)
+    scale = 128 ** -0.5 * 2.0 ** power
+    b.check(b.attend(window, sinks, scale=scale), window, sinks, scale=scale)
+
+
 @pytest.mark.parametrize("rows", [1, 6, 50])
 def test_sharp_logits(rows):
     """One key far above the rest: the running maximum moves, weights vanish."""
