@@ -866,7 +866,7 @@ uint32_t attend_rows_ctas(int smCount) { return 2u * (uint32_t)smCount; }
 
 bool launch_attend_rows(FFAttention *att, const AttendArgs &a, cudaStream_t stream, const char **error) {
     const uint32_t dim = att->cfg.headDim;
-    RowsArgs args{a, att->partials, att->stats, att->arrived, (uint32_t)__builtin_ctz(att->cfg.pageTokens), (uint32_t)__builtin_ctz(std::min(kTileKeys, a.page.pageTokens))};
+    RowsArgs args{a, att->partials, reinterpret_cast<float2 *>(att->stats), att->arrived, (uint32_t)__builtin_ctz(att->cfg.pageTokens), (uint32_t)__builtin_ctz(std::min(kTileKeys, a.page.pageTokens))};
     CUtensorMap codes, words;
     if (!make_pages_maps(&codes, &words, a, dim, 2, error)) return false;
     const uint32_t columns = a.maxRows * (a.heads / a.kvHeads);

@@ -10,7 +10,7 @@
 // warpgroups own a row a thread and take the tiles in turn:
 //   S = Q K^T   A: the rows' queries, in tensor memory for the whole unit (from shared memory an MMA of 64 keys takes 73
 //               cycles, from tensor memory 33); B: the keys, K-major
-//   P = 2^(S f + E - M)   in registers, back into S's columns as f16
+//   P = 2^(S f + E - M)   in registers, back into S's columns as f16; their sum at the largest logit, without E
 //   O += P V    A: P; B: the values, N-major; O stays in tensor memory
 // A tile's warpgroup waits for the maximum M that the one before it settled on, not for its weights; M moves, and O with it, only
 // where a row passes it by 2^8.  (Both warpgroups on each tile, half a row a thread, were slower: what a tile costs besides its
@@ -59,7 +59,7 @@ static_assert(2 * kPacked - 1 >= kSlots, "a free slot says that the ring's place
 struct TilesArgs {
     AttendArgs a;
     float *partials;      // [2 CTAs][rows][DIM]
-    float2 *stats;        // [2 CTAs][rows]
+    float4 *stats;        // [2 CTAs][rows] M, the largest logit L, the weights' sum at 2^L
     uint32_t *arrived;    // [3][CTAs], zero between launches: of a unit, of its first group of parts, of another group
     uint32_t pageShift, pieceShift, tileTokens;  // log2 of a page's tokens and of the keys of a tile on one page; tokens of a row tile
 };
@@ -533,6 +533,9 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
             bool ok = true;
             Walk w;
             for (bool more = first_segment(w); more && ok; more = ok && next_segment(w)) {
+                // Of values far below (2^-64) the largest of the segment so far, or of zeros, the tile's own power would put M so far above its
+                // logits that its weights fell out of 32 bits, and out of the sum.
+                int floorV = -100;
                 const int pLast = w.q.p0 + (int)w.q.tokens - 1;
                 for (uint32_t i = 0; i < w.count; ++i, ++tile) {
                     const uint32_t at = tile % kPacked, info = tile % kInfo;
@@ -586,8 +589,9 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
 #pragma unroll
                     for (int side = 0; side < 2; ++side) {
                         const uint32_t largest = __reduce_max_sync(0xFFFFFFFFu, max(((most[side] & 0xFFFFu) >> 7) + 4u, most[side] >> 23));
-                        exponent[side] = min(max((int)largest - 127 + 6, -100), 120);
+                        exponent[side] = min(max((int)largest - 127 + 6, side ? floorV : -100), 120);
                     }
+                    floorV = max(floorV, exponent[1] - 64);
                     if (!(ok = wait_warp<true>(barInfoFree + 8 * info, tile / kInfo & 1u ^ 1u, &abortFlag))) break;
 #pragma unroll
                     for (int side = 0; side < 2; ++side) {
@@ -599,7 +603,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                     }
                     __syncwarp();
                     if (lane == 0) {
-                        tileInfo[info] = make_float4(power_of_two(exponent[0]), (float)exponent[1], power_of_two(-exponent[1]), unseen ? 1.0f : 0.0f);
+                        tileInfo[info] = make_float4(power_of_two(exponent[0]), (float)exponent[1], unseen ? 1.0f : 0.0f, 0.0f);
                         hidden[info][0] = out[0], hidden[info][1] = out[1];
                         mbar_arrive(barInfo + 8 * info);
                     }
@@ -733,7 +737,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                     __syncwarp();
                     if (lane == 0) mbar_arrive(barQ);
                 }
-                float ref = kNone, sum = 0.0f;  // the warpgroup's part of the weights' sum, at 2^ref
+                float ref = kNone, sum = 0.0f;  // the warpgroup's part of the weights' sum, at 2^ref, its largest logit
                 uint32_t i = (tile ^ wg) & 1u;  // the segment's first tile of this warpgroup
                 for (tile += i; i < w.count; i += 2, tile += 2) {
                     const uint32_t info = tile % kInfo;
@@ -743,10 +747,10 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                     uint32_t lo[32], hi[32];
                     tc_load_32cols(s0, lo);
                     tc_load_32cols(s0 + 32, hi);
-                    const float4 about = tileInfo[info];  // 2^eK, eV, 2^-eV, whether some row does not see some key
+                    const float4 about = tileInfo[info];  // 2^eK, eV, whether some row does not see some key
                     tc_wait_ld();
                     float *s = reinterpret_cast<float *>(lo), *u = reinterpret_cast<float *>(hi);
-                    if (about.w != 0.0f) {
+                    if (about.z != 0.0f) {
                         // the keys that the row sees: up to its own, and above the window's end or below the last sink
                         const uint32_t gone0 = hidden[info][0], gone1 = hidden[info][1];
                         const long long j0 = key_at(w.q, w.t0 + i);
@@ -768,7 +772,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                         most[2] = fmaxf(fmaxf(most[2], u[c]), u[c + 2 < 32 ? c + 2 : c]);
                         most[3] = fmaxf(fmaxf(most[3], u[c + 1]), u[c + 3 < 32 ? c + 3 : c + 1]);
                     }
-                    const float f = fmaxf(toLog2 * about.x, 0x1p-126f), peak = fmaf(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])), f, about.y);
+                    const float f = fmaxf(toLog2 * about.x, 0x1p-126f), product = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+                    const float peak = fmaf(product, f, about.y), level = fmaxf(ref, product * f);
                     // the maximum that the tile before settled on
                     float top = kNone;
                     if (i) {
@@ -796,8 +801,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                     topShared[row] = top;
                     __syncwarp();
                     if (lane == 0) mbar_arrive(barTop + 8 * (wg * 4 + quarter));
-                    sum *= exp2_fast(ref - top);
-                    ref = top;
+                    sum *= exp2_fast(ref - level);
+                    ref = level;
                     const float shift = about.y - top + kWeightScale;
                     const unsigned long long f2 = pair_f32(f, f), shift2 = pair_f32(shift, shift);
                     unsigned long long part = pair_f32(0.0f, 0.0f), part2 = part;
@@ -821,7 +826,9 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                     if (lane == 0) mbar_arrive(barP + 16 * wg);  // (the products of the first 32 keys may begin)
                     weigh(u, s0 + 16);
                     part = add_f32x2(part, part2);
-                    sum = fmaf(first_f32(part) + second_f32(part), about.z, sum);
+                    // (A weight is 2^(S f + eV - M) here.  M is at most 72 above the largest logit plus eV; where it is further above this warpgroup's,
+                    // the other has far larger ones.  M and the logit first: their difference is exact, as P's rounding of M takes it.)
+                    sum = fmaf(first_f32(part) + second_f32(part), exp2_fast(fminf((top - level) - about.y, 120.0f)), sum);
                     tc_wait_st();
                     tc_fence_before();
                     __syncwarp();
@@ -836,10 +843,11 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                 if (!meet() || !(ok = wait_warp<false>(barO + 8 * ((tile - 1) & 1u), (tile - 1) >> 1 & 1u, &abortFlag))) break;
                 tc_fence_after();
                 const float top = topShared[row];
-                sum = sumShared[0][row] * exp2_fast(refShared[0][row] - top) + sumShared[1][row] * exp2_fast(refShared[1][row] - top);
+                const float largest = fmaxf(refShared[0][row], refShared[1][row]);
+                sum = sumShared[0][row] * exp2_fast(refShared[0][row] - largest) + sumShared[1][row] * exp2_fast(refShared[1][row] - largest);
                 const bool whole = w.count == w.q.tiles;
                 const uint32_t part = 2 * cta + (w.t0 == 0 ? 1u : 0u);
-                const float factor = sum == 0.0f ? 0.0f : 1.0f / sum;
+                const float factor = sum == 0.0f ? 0.0f : exp2_fast(top - largest) / sum;  // (-108 .. 120, of the values' powers)
                 if (whole) {
                     // four lanes 64 bytes of a row
                     float factors[4];
@@ -878,7 +886,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                 }
                 tc_fence_before();  // (the next unit's products overwrite O once both warpgroups have brought their queries)
                 if (!whole) {
-                    if (there && wg == 0) args.stats[part * kRows + row] = make_float2(top, sum);
+                    if (there && wg == 0) args.stats[part * kRows + row] = make_float4(top, largest, sum, 0.0f);
                     const uint32_t c0 = cta_of(w.first + kUnitCost), c1 = cta_of(w.first + kUnitCost + w.q.tiles - 1), parts = c1 - c0 + 1;
                     // whether this is the last of `expected` CTAs; then what they wrote is there
                     auto arrive = [&](uint32_t *counter, uint32_t expected) {
@@ -902,14 +910,13 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                         for (uint32_t item = warp - kFirstRowWarp; item < blocks * (DIM / 8 / kValues); item += kRowWarps) {
                             const uint32_t mine = item % blocks * 32 + lane, d = item / blocks * (8 * kValues);
                             if (mine >= used) continue;
-                            float all = kNone, weights = 0.0f, v[8 * kValues];
+                            float all = kNone, level = kNone, weights = 0.0f, v[8 * kValues];
 #pragma unroll
                             for (uint32_t k = 0; k < 8 * kValues; ++k) v[k] = 0.0f;
                             auto place = [&](uint32_t n) { return reinterpret_cast<float4 *>(args.partials) + ((size_t)n * (DIM / 4) + d / 4) * kRows + mine; };
 #pragma unroll 1
                             for (uint32_t k0 = 0; k0 < count; k0 += kAtOnce) {
-                                float2 st[kAtOnce];
-                                float4 t[kAtOnce][2 * kValues];
+                                float4 st[kAtOnce], t[kAtOnce][2 * kValues];
 #pragma unroll
                                 for (uint32_t k = 0; k < kAtOnce; ++k) {
                                     const uint32_t n = part_of(from + min(k0 + k, count - 1) * step);
@@ -917,19 +924,19 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
 #pragma unroll
                                     for (uint32_t h = 0; h < 2 * kValues; ++h) t[k][h] = __ldcg(place(n) + h * kRows);
                                 }
-                                float next = all;
+                                float next = all, nextLevel = level;
 #pragma unroll
-                                for (uint32_t k = 0; k < kAtOnce; ++k) next = fmaxf(next, st[k].x);
+                                for (uint32_t k = 0; k < kAtOnce; ++k) next = fmaxf(next, st[k].x), nextLevel = fmaxf(nextLevel, st[k].y);
                                 const float keep = exp2_fast(all - next);
-                                all = next;
-                                weights *= keep;
+                                weights *= exp2_fast(level - nextLevel);
+                                all = next, level = nextLevel;
 #pragma unroll
                                 for (uint32_t k = 0; k < 8 * kValues; ++k) v[k] *= keep;
 #pragma unroll
                                 for (uint32_t k = 0; k < kAtOnce; ++k) {
                                     if (k0 + k >= count) break;
                                     const float g = exp2_fast(st[k].x - all);
-                                    weights = fmaf(st[k].y, g, weights);
+                                    weights = fmaf(st[k].z, exp2_fast(st[k].y - level), weights);
 #pragma unroll
                                     for (uint32_t h = 0; h < 2 * kValues; ++h) {
                                         v[4 * h] = fmaf(t[k][h].x, g, v[4 * h]), v[4 * h + 1] = fmaf(t[k][h].y, g, v[4 * h + 1]);
@@ -938,7 +945,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                                 }
                             }
                             if (last) {
-                                const float f = weights == 0.0f ? 0.0f : 1.0f / weights;
+                                const float f = weights == 0.0f ? 0.0f : exp2_fast(all - level) / weights;
                                 uint16_t *to = a.out + (size_t)(w.q.firstRow + mine / group) * a.outStride + (w.head * group + mine % group) * DIM + d;
 #pragma unroll
                                 for (uint32_t k = 0; k < 4; ++k)  // value n of run k: column 8 (n % 4) + 2 k + n / 4
@@ -947,11 +954,11 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                             } else {
 #pragma unroll
                                 for (uint32_t h = 0; h < 2 * kValues; ++h) place(part_of(from))[h * kRows] = make_float4(v[4 * h], v[4 * h + 1], v[4 * h + 2], v[4 * h + 3]);
-                                if (d == 0) refShared[0][mine] = all, sumShared[0][mine] = weights;
+                                if (d == 0) topShared[mine] = all, refShared[0][mine] = level, sumShared[0][mine] = weights;
                             }
                         }
                         if (last || !meet()) return;  // (the first one's maxima have been read)
-                        if (wg == 0 && row < used) args.stats[part_of(from) * kRows + row] = make_float2(refShared[0][row], sumShared[0][row]);
+                        if (wg == 0 && row < used) args.stats[part_of(from) * kRows + row] = make_float4(topShared[row], refShared[0][row], sumShared[0][row], 0.0f);
                     };
                     // by groups of 16 first where there are more (a CTA is the first of one unit and inside another at most: a
                     // group's counter goes by which)

@@ -11,7 +11,7 @@ struct FFAttention {
     uint32_t *planCount = nullptr;  // device: CTAs of ff_cache_plan that are done (zero between launches)
     uint32_t rowsCtas = 0;          // CTAs that the scratch below serves
     float *partials = nullptr;      // device: outputs of units that several CTAs share, two parts a CTA
-    float2 *stats = nullptr;        // device: their maxima and sums
+    float4 *stats = nullptr;        // device: their maxima and sums
     uint32_t *arrived = nullptr;    // device: parts of a shared unit that are there (zero between launches)
     uint64_t kernelLaunches = 0;
     uint64_t scratchBytes = 0;

@@ -421,6 +421,22 @@ def test_values_of_very_different_sizes(rows):
     b.check(b.attend())
 
 
+@pytest.mark.parametrize("rows,length", [(1, 300), (6, 300), (50, 300), (1, 4000), (30, 4000)])
+@pytest.mark.parametrize("small", [0.0, 2.0 ** -90])
+@pytest.mark.parametrize("power", [26, 60, 110])
+@pytest.mark.parametrize("where", ["first", "last", "between"])
+def test_weights_of_small_values_count_beside_large_ones(rows, length, small, power, where):
+    """Tiles of values that are zero or tiny among large ones: their weights are in the sum all the same."""
+    b = Batch(4, 2, 64, 16, [length], [rows])
+    v = b.v.float() * 2.0 ** power
+    third = length // 3
+    v[{"first": slice(0, third), "last": slice(2 * third, length), "between": slice(third, 2 * third)}[where]] *= small / 2.0 ** power
+    for a in range(0, length, 1024):
+        c = min(length, a + 1024)
+        context(4, 2, 64, 16, tokens=1024).append(None, b.k[a:c], v[a:c].bfloat16(), None, ints([0] * (c - a)), ints(b.slots[0][a:c]), b.cache)
+    b.check(b.attend())
+
+
 @pytest.mark.parametrize("rows", [1, 12, 70])
 def test_strides_streams_and_repeats(rows):
     b = Batch(8, 2, 128, 32, [500, 77, 1200], [rows] * 3)
