@@ -13,7 +13,10 @@ namespace ff {
 // pages and the table entries.  The k-th page taken is the k-th from the top of the stack as it stands with the
 // returned pages on it; where that is a returned page its id is read from the table entry it came from, which
 // nothing writes: a request either grows or shrinks.  So no value passes through memory that this launch writes.
-// Bound by latency: two rounds of loads, a scan, a search of ten steps; 4.0 us for 16 requests of a decode step, 6.3 us for 1000
+// Entries that are no page (of requests for which none was left) do not go back.  A CTA that meets one among its share of those
+// given back says so at the end, and the last CTA does all again with the pages alone counted.  (Looked for beforehand by every CTA
+// they cost 1000 mixed requests 2.1 us, this way 0.8.)
+// Bound by latency: two rounds of loads, a scan, a search of ten steps; 3.9 us for 16 requests of a decode step, 7.3 us for 1000
 // requests that grow, shrink and end (in a graph; a call from Python is 8.5 us of the host's time).
 constexpr int kPlanThreads = 1024;
 
@@ -55,88 +58,69 @@ __device__ __forceinline__ PlanRequest plan_request(const PlanArgs &a, uint32_t 
     return p;
 }
 
-__global__ void __launch_bounds__(kPlanThreads) k_cache_plan(const PlanArgs a) {
-    // first row, page taken and page given back of every thread's run of requests, and behind the last
-    __shared__ uint32_t first[3][kPlanThreads + 1];
-    __shared__ uint32_t warpSum[3][32];
-    __shared__ bool last;
-    const uint32_t t = threadIdx.x, lane = t & 31u, warp = t >> 5;
-    const uint32_t run = (a.requests + kPlanThreads - 1) / kPlanThreads;
-    const uint32_t r0 = min(t * run, a.requests), r1 = min(r0 + run, a.requests);
-    pdl_enter();
-    const uint32_t free = min(__ldg(a.freeCountIn), a.pageCount);
-
-    uint32_t sum[3] = {0u, 0u, 0u};
-    bool cut = false;
-    for (uint32_t r = r0; r < r1; ++r) {
-        const PlanRequest p = plan_request(a, r);
-        sum[0] = add_counts(sum[0], p.rows);
-        sum[1] += p.taken();
-        sum[2] += p.given();
-        cut |= p.cut;
+// What every CTA knows: first row, page taken and page given back of every thread's run of requests, and behind the last.
+struct PlanSums {
+    uint32_t first[3][kPlanThreads + 1];
+    uint32_t warpSum[3][32];
+};
+// The kind's sum over the CTA's threads before each of them; `own` the thread's.
+__device__ __forceinline__ uint32_t warp_scan(uint32_t own, uint32_t *all) {
+    const uint32_t lane = threadIdx.x & 31u;
+    uint32_t s = own;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, s, d);
+        if (lane >= (uint32_t)d) s = add_counts(s, v);
     }
-    uint32_t before[3];  // sums over the warp's lanes before this one
-    auto scan = [&](uint32_t own, uint32_t &all) {
-        uint32_t s = own;
+    if (lane == 31u) *all = s;
+    const uint32_t front = __shfl_up_sync(0xFFFFFFFFu, s, 1);
+    return lane ? front : 0u;
+}
+// the run that holds the n-th of a kind, n below its total
+__device__ __forceinline__ uint32_t run_of(const uint32_t *first, uint32_t n) {
+    uint32_t low = 0, high = kPlanThreads;  // first[low] <= n < first[high]
 #pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, s, d);
-            if (lane >= (uint32_t)d) s = add_counts(s, v);
-        }
-        all = s;  // (lane 31's is the warp's)
-        const uint32_t front = __shfl_up_sync(0xFFFFFFFFu, s, 1);
-        return lane ? front : 0u;
-    };
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-        uint32_t all;
-        before[i] = scan(sum[i], all);
-        if (lane == 31u) warpSum[i][warp] = all;
+    for (int i = 0; i < 10; ++i) {
+        const uint32_t mid = (low + high) >> 1;
+        if (first[mid] <= n) low = mid;
+        else high = mid;
     }
-    __syncthreads();
-    if (warp < 3u) {
-        uint32_t all;
-        warpSum[warp][lane] = scan(warpSum[warp][lane], all);
-        if (lane == 31u) first[warp][kPlanThreads] = all;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < 3; ++i) first[i][t] = add_counts(warpSum[i][warp], before[i]);
-    __syncthreads();
-    const uint32_t totalRows = first[0][kPlanThreads], totalTaken = first[1][kPlanThreads], totalGiven = first[2][kPlanThreads];
-
-    // the run that holds the n-th of a kind, n below its total
-    auto run_of = [&](int kind, uint32_t n) {
-        uint32_t low = 0, high = kPlanThreads;  // first[low] <= n < first[high]
-#pragma unroll
-        for (int i = 0; i < 10; ++i) {
-            const uint32_t mid = (low + high) >> 1;
-            if (first[kind][mid] <= n) low = mid;
-            else high = mid;
-        }
-        return low;
-    };
-    // the page on place `at` of the stack with the returned pages on it
-    auto stack_page = [&](uint32_t at) {
-        if (at < free) return __ldg(a.freePages + at);
-        uint32_t n = at - free;
-        const uint32_t g = run_of(2, n);
-        n -= first[2][g];
+    return low;
+}
+// Rows, table entries and returned pages, shared among `step` threads.  kHoles: of the entries given back those alone count (in
+// `first` too) that are pages.  Whether one that is none was met.
+template <bool kHoles>
+__device__ __forceinline__ bool plan_write(const PlanArgs &a, const PlanSums &s, uint32_t free, uint32_t run, uint32_t at, uint32_t step) {
+    const uint32_t totalRows = s.first[0][kPlanThreads], totalTaken = s.first[1][kPlanThreads], totalGiven = s.first[2][kPlanThreads], height = free + totalGiven;
+    // the page on place `place` of the stack with the returned pages on it
+    auto stack_page = [&](uint32_t place) {
+        if (place < free) return __ldg(a.freePages + place);
+        uint32_t n = place - free;
+        const uint32_t g = run_of(s.first[2], n);
+        n -= s.first[2][g];
         for (uint32_t r = g * run;; ++r) {
             const PlanRequest p = plan_request(a, r);
-            if (n < p.given()) return a.blockTable[(size_t)r * a.tableStride + p.has + n];
-            n -= p.given();
+            const uint32_t *entries = a.blockTable + (size_t)r * a.tableStride + p.has;
+            if (!kHoles) {
+                if (n < p.given()) return entries[n];
+                n -= p.given();
+            } else {
+                for (uint32_t i = 0; i < p.given(); ++i)
+                    if (entries[i] < a.pageCount && n-- == 0u) return entries[i];
+            }
         }
     };
-    const uint32_t height = free + totalGiven;
-    auto taken_page = [&](uint32_t k) { return k < height ? stack_page(height - 1u - k) : FF_NO_PAGE; };
-
-    const uint32_t at = blockIdx.x * kPlanThreads + t, step = gridDim.x * kPlanThreads;
+    auto taken_page = [&](uint32_t k) {
+        const uint32_t place = height - 1u - k, page = k < height ? stack_page(place) : FF_NO_PAGE;
+        if (page < a.pageCount) return page;
+        if (k >= height || place < free) *a.errorFlag = kFlagNoPage;
+        return FF_NO_PAGE;
+    };
     for (uint32_t i = at; i < a.rows; i += step) {
         uint32_t position = 0, slot = FF_NO_SLOT;
         if (i < totalRows) {
-            const uint32_t g = run_of(0, i);
-            uint32_t n = i - first[0][g], taken = first[1][g];
+            const uint32_t g = run_of(s.first[0], i);
+            uint32_t n = i - s.first[0][g], taken = s.first[1][g];
             for (uint32_t r = g * run;; ++r) {
                 const PlanRequest p = plan_request(a, r);
                 if (n < p.rows) {
@@ -156,8 +140,8 @@ __global__ void __launch_bounds__(kPlanThreads) k_cache_plan(const PlanArgs a) {
         a.slots[i] = slot;
     }
     for (uint32_t k = at; k < totalTaken; k += step) {
-        const uint32_t g = run_of(1, k);
-        uint32_t n = k - first[1][g];
+        const uint32_t g = run_of(s.first[1], k);
+        uint32_t n = k - s.first[1][g];
         for (uint32_t r = g * run;; ++r) {
             const PlanRequest p = plan_request(a, r);
             if (n < p.taken()) {
@@ -167,26 +151,91 @@ __global__ void __launch_bounds__(kPlanThreads) k_cache_plan(const PlanArgs a) {
             n -= p.taken();
         }
     }
-    for (uint32_t k = at; k < totalGiven; k += step)
-        if (free + k < a.pageCount) a.freePages[free + k] = stack_page(free + k);
+    bool met = false;
+    for (uint32_t k = at; k < totalGiven; k += step) {
+        const uint32_t page = stack_page(free + k);
+        met |= page >= a.pageCount;
+        if (free + k < a.pageCount) a.freePages[free + k] = page;
+    }
+    return met;
+}
+// All of it by the last CTA, where entries that are no page were given back.
+__device__ __noinline__ void plan_again(const PlanArgs &a, PlanSums &s, uint32_t free, uint32_t run) {
+    const uint32_t t = threadIdx.x, warp = t >> 5;
+    const uint32_t r0 = min(t * run, a.requests), r1 = min(r0 + run, a.requests);
+    uint32_t own = 0;
+    for (uint32_t r = r0; r < r1; ++r) {
+        const PlanRequest p = plan_request(a, r);
+        for (uint32_t i = 0; i < p.given(); ++i) own += a.blockTable[(size_t)r * a.tableStride + p.has + i] < a.pageCount;
+    }
+    const uint32_t front = warp_scan(own, &s.warpSum[2][warp]);
+    __syncthreads();
+    uint32_t before = 0, total = 0;
+    for (uint32_t w = 0; w < 32u; ++w) {
+        if (w == warp) before = total;
+        total += s.warpSum[2][w];
+    }
+    s.first[2][t] = before + front;
+    if (t == 0) s.first[2][kPlanThreads] = total;
+    __syncthreads();
+    plan_write<true>(a, s, free, run, t, kPlanThreads);
+}
+
+__global__ void __launch_bounds__(kPlanThreads) k_cache_plan(const __grid_constant__ PlanArgs a) {
+    __shared__ PlanSums s;
+    __shared__ uint32_t last, again;
+    const uint32_t t = threadIdx.x, lane = t & 31u, warp = t >> 5;
+    const uint32_t run = (a.requests + kPlanThreads - 1) / kPlanThreads;
+    const uint32_t r0 = min(t * run, a.requests), r1 = min(r0 + run, a.requests);
+    pdl_enter();
+    const uint32_t free = min(__ldg(a.freeCountIn), a.pageCount);
+
+    uint32_t sum[3] = {0u, 0u, 0u};
+    bool cut = false;
+    for (uint32_t r = r0; r < r1; ++r) {
+        const PlanRequest p = plan_request(a, r);
+        sum[0] = add_counts(sum[0], p.rows);
+        sum[1] += p.taken();
+        sum[2] += p.given();
+        cut |= p.cut;
+    }
+    uint32_t before[3];  // sums over the warp's lanes before this one
+#pragma unroll
+    for (int i = 0; i < 3; ++i) before[i] = warp_scan(sum[i], &s.warpSum[i][warp]);
+    __syncthreads();
+    if (warp < 3u) s.warpSum[warp][lane] = warp_scan(s.warpSum[warp][lane], &s.first[warp][kPlanThreads]);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 3; ++i) s.first[i][t] = add_counts(s.warpSum[i][warp], before[i]);
+    __syncthreads();
+
+    const bool met = plan_write<false>(a, s, free, run, blockIdx.x * kPlanThreads + t, gridDim.x * kPlanThreads);
     if (blockIdx.x == 0) {
-        uint32_t row = first[0][t];
+        uint32_t row = s.first[0][t];
         for (uint32_t r = r0; r < r1; ++r) {
             a.rowStart[r] = row;
             row = add_counts(row, plan_request(a, r).rows);
         }
-        if (t == 0) a.rowStart[a.requests] = totalRows;
+        if (t == 0) a.rowStart[a.requests] = s.first[0][kPlanThreads];
         if (cut) *a.errorFlag = kFlagTableRow;
-        if (t == 0 && totalTaken > height) *a.errorFlag = kFlagNoPage;
-        if (t == 0 && totalRows > a.rows) *a.errorFlag = kFlagRows;
+        if (t == 0 && s.first[0][kPlanThreads] > a.rows) *a.errorFlag = kFlagRows;
     }
     // the stack's height may go back to the word it came from: written when every CTA has read that
+    const bool some = __syncthreads_or(met);
+    if (t == 0) {
+        if (s.first[2][kPlanThreads]) __threadfence();  // (what this CTA wrote comes before what the last one may write over it)
+        const uint32_t n = atomicAdd(a.done, some ? 0x10001u : 1u);
+        last = (n & 0xFFFFu) == gridDim.x - 1u;
+        again = some || n >> 16;
+        if (again) __threadfence();
+    }
     __syncthreads();
-    if (t == 0) last = atomicAdd(a.done, 1u) == gridDim.x - 1u;
-    __syncthreads();
-    if (last && t == 0) {
+    if (!last) return;
+    if (again) plan_again(a, s, free, run);
+    if (t == 0) {
+        const uint32_t height = free + s.first[2][kPlanThreads], taken = s.first[1][kPlanThreads];
         *a.done = 0u;
-        *a.freeCountOut = height > totalTaken ? min(height - totalTaken, a.pageCount) : 0u;
+        *a.freeCountOut = height > taken ? min(height - taken, a.pageCount) : 0u;
     }
 }
 

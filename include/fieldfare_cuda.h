@@ -498,7 +498,8 @@ uint64_t ff_cache_page_bytes(const FFAttentionConfig *config);
  *   rowStart   [requests + 1], positions and slots [rows]: rows behind the last request's get position 0 and
  *              FF_NO_SLOT
  * A request that finds no page, or no room in its table row, gets FF_NO_PAGE entries and FF_NO_SLOT rows (flags 13
- * and 14). */
+ * and 14).  Such entries are not given back: a stack that holds every page once goes on doing so.  A block table has at
+ * most 2^30 entries. */
 bool ff_cache_plan(FFAttention *attention, const uint32_t *oldLengths, const uint32_t *newLengths, uint32_t requests,
                    uint32_t *blockTable, uint32_t tableStride, uint32_t *freePages, uint32_t pageCount,
                    const uint32_t *freeCountIn, uint32_t *freeCountOut, uint32_t *rowStart, uint32_t *positions,

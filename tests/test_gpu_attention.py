@@ -92,6 +92,54 @@ def test_plan_without_pages_or_room_says_so_and_stays_inside():
     assert ctx.info().deviceErrorFlag == 15
 
 
+@pytest.mark.parametrize("requests,pages,most,steps", [(2, 4, 64, 12), (5, 9, 100, 30), (40, 70, 90, 12), (1500, 900, 40, 6)])
+def test_plan_after_the_pages_ran_out(requests, pages, most, steps):
+    """Requests that found no page shrink, end and grow again: every page is in one place all the time, and none is lost."""
+    page, width, rng = 16, -(-most // 16), np.random.RandomState(requests)
+    ctx = context(page=page, requests=requests, tokens=requests * most)
+    table, free, count, old = np.full((requests, width), -1), np.full(pages, -1), pages, np.zeros(requests, dtype=int)
+    free[:] = rng.permutation(pages)
+    ranOut = 0
+    for step in range(steps):
+        new = np.where(rng.rand(requests) < 0.7, rng.randint(0, most + 1, requests), old)
+        if step % 3 == 2:
+            new = np.where(rng.rand(requests) < 0.5, 0, np.minimum(new, old))
+        if step == steps - 1:
+            new[:] = 0
+        got = run_plan(ctx, old, new, table, free, count, requests * most)
+        has = [list(table[r, :-(-old[r] // page)]) for r in range(requests)]
+        stack = list(free[:count])
+        for r in range(requests):
+            while len(has[r]) > -(-new[r] // page):
+                has[r].pop()
+        for r in range(requests):  # given back in order of their places
+            stack += [p for p in table[r, len(has[r]):-(-old[r] // page)] if p >= 0]
+        short = False
+        for r in range(requests):
+            while len(has[r]) < -(-new[r] // page):
+                has[r].append(stack.pop() if stack else -1)
+                short |= has[r][-1] < 0
+        assert [list(got["table"][r, :len(has[r])]) for r in range(requests)] == has
+        assert got["count"][0] == len(stack) and list(got["free"][:len(stack)]) == stack
+        held = [p for mine in has for p in mine if p >= 0]
+        assert sorted(held + stack) == list(range(pages))
+        slots = [has[r][p // page] * page + p % page if has[r][p // page] >= 0 else -1 for r in range(requests) for p in range(old[r], new[r])]
+        assert list(got["slots"][:len(slots)]) == slots
+        assert ctx.info().deviceErrorFlag == (13 if short else 0)
+        ctx.resetDeviceError()
+        ranOut += short
+        table, free, count, old = got["table"], got["free"], len(stack), new
+    assert ranOut and sorted(free) == list(range(pages))
+
+
+def test_plan_does_not_hand_out_what_is_no_page():
+    ctx = context(page=16)
+    got = run_plan(ctx, [0], [40], [[7, 7, 7]], [2, 99, 0, -1], 3, 40)
+    assert got["table"].tolist() == [[0, -1, 2]]
+    assert got["slots"].tolist() == list(range(16)) + [-1] * 16 + list(range(32, 40))
+    assert ctx.info().deviceErrorFlag == 13
+
+
 @pytest.mark.parametrize("requests", [4, 1500])
 def test_plan_of_lengths_that_are_none(requests):
     """Words of -1 in a batch: their requests end with their table rows, and the arrays with themselves."""
