@@ -8,7 +8,8 @@ keys and values into the cache (once per layer); `attend` is the attention over 
 The cache's memory is the caller's: `newCache(pages)` per layer, uint8 [pages][kvHeads][bytes of a block]; its layout
 stands in include/fieldfare_cuda.h.  Lengths, tables, positions and slots are int32 CUDA tensors.  Wrong shapes, types or
 devices raise `ValueError`, what the library refuses raises `FieldfareError`; what a kernel finds in its data (no free
-page, a page outside the cache) stands in `info().deviceErrorFlag`.
+page, a page outside the cache) stands in `info().deviceErrorFlag`.  A result that a call with `stream` allocates belongs to that
+stream, as torch counts it: to use it on another, wait for the stream, and `record_stream` it there.
 """
 from __future__ import annotations
 
@@ -68,6 +69,13 @@ class AttentionContext:
         call("ff_attention_reset_device_error", self.handle)
 
     # -- arguments ---------------------------------------------------------------------------------
+
+    def _new(self, shape: tuple, dtype: torch.dtype, stream) -> torch.Tensor:
+        """Memory for a result, of the stream that writes it: the current stream may still use what it has freed."""
+        if stream is None:
+            return torch.empty(shape, dtype=dtype, device=self.device)
+        with torch.cuda.stream(stream):
+            return torch.empty(shape, dtype=dtype, device=self.device)
 
     # (A step of small calls is bound by the host: `get_device` and `is` cost a fifth of comparing torch.device objects, one
     # look at shape and strides a third of four.)
@@ -139,7 +147,7 @@ class AttentionContext:
             raise ValueError(f"scaling must be one of {sorted(_SCALING)}")
         rotary = self.headDim if rotaryDim is None else rotaryDim
         config = FFRopeConfig(base, rotary, _SCALING[scaling], factor, lowTurns, highTurns, originalContext, amplitude)
-        table = torch.empty((positions, max(0, rotary) // 2, 2), dtype=torch.float32, device=self.device)
+        table = self._new((positions, max(0, rotary) // 2, 2), torch.float32, stream)
         call("ff_rope_table", self.handle, ctypes.byref(config), table.data_ptr(), positions, _stream(stream))
         return table
 
@@ -150,7 +158,7 @@ class AttentionContext:
             raise ValueError("x must be [tokens][heads][headDim], with one position per row")
         tokens, heads = x.shape[:2]
         if y is None:
-            y = torch.empty((tokens, heads, self.headDim), dtype=torch.bfloat16, device=self.device)
+            y = self._new((tokens, heads, self.headDim), torch.bfloat16, stream)
         rope = self._rope(table, interleaved)
         self._ints("positions", positions)
         call("ff_rope", self.handle, *self._heads(x, heads, tokens, "x"), ctypes.byref(rope), positions.data_ptr(), heads, tokens,
@@ -168,7 +176,7 @@ class AttentionContext:
         query, out = (None, 0), (None, 0)
         if q is not None:
             if qOut is None:
-                qOut = torch.empty((tokens, self.heads, self.headDim), dtype=torch.bfloat16, device=self.device)
+                qOut = self._new((tokens, self.heads, self.headDim), torch.bfloat16, stream)
             query, out = self._heads(q, self.heads, tokens, "q"), self._heads(qOut, self.heads, tokens, "qOut")
         rope = self._rope(table, interleaved)
         self._ints("positions slots", positions, slots)
@@ -183,9 +191,9 @@ class AttentionContext:
         tokens = slots.numel()
         shape = (tokens, self.kvHeads, self.headDim)
         if k is None:
-            k = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
+            k = self._new(shape, torch.bfloat16, stream)
         if v is None:
-            v = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
+            v = self._new(shape, torch.bfloat16, stream)
         if not (k.is_contiguous() and v.is_contiguous()):
             raise ValueError("k and v must be contiguous")
         self._ints("slots", slots)
@@ -207,7 +215,7 @@ class AttentionContext:
         if window < 0 or sinks < 0 or maxRows < 0:
             raise ValueError("window, sinks and maxRows must not be negative")
         if out is None:
-            out = torch.empty((tokens, self.heads, self.headDim), dtype=torch.bfloat16, device=self.device)
+            out = self._new((tokens, self.heads, self.headDim), torch.bfloat16, stream)
         self._ints("blockTable rowStart lengths", blockTable, rowStart, lengths)
         call("ff_attention", self.handle, *self._heads(q, self.heads, tokens, "q"), tokens, *self._cache(pages), blockTable.data_ptr(), shape[1],
              rowStart.data_ptr(), lengths.data_ptr(), requests, maxRows, self.headDim ** -0.5 if scale is None else scale, window, sinks,

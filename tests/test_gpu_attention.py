@@ -503,6 +503,26 @@ def test_strides_streams_and_repeats(rows):
         assert torch.equal(b.attend(), want)
 
 
+def test_outputs_are_memory_of_the_stream_that_writes_them():
+    """What a call allocates for a stream is not what the current stream may still be using."""
+    b = Batch(4, 2, 64, 16, [5000], [1000], seed=5)
+    table, at, slots = b.ctx.ropeTable(64), ints([5] * 1000), ints(b.slots[0][:1000])
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    calls = [((1000, 4, 64), lambda: [b.attend(stream=side)]), ((1000, 4, 64), lambda: [b.ctx.rope(b.q, table, at, stream=side)]),
+             ((1000, 4, 64), lambda: [b.ctx.append(b.q, b.k[:1000], b.v[:1000], table, at, slots, b.cache, stream=side)]),
+             ((1000, 2, 64), lambda: b.ctx.read(b.cache, slots, stream=side)), ((4000, 2, 64), lambda: [b.ctx.ropeTable(4000, rotaryDim=64, stream=side)])]
+    for shape, run in calls:
+        torch.cuda.synchronize()
+        used = [torch.empty(shape, dtype=torch.bfloat16, device="cuda") for _ in range(3)]
+        held = {t.data_ptr() for t in used}
+        del used  # (the current stream's work on them may be in flight)
+        out = run()
+        torch.cuda.synchronize()
+        assert not held & {t.data_ptr() for t in out}
+
+
 @pytest.mark.parametrize("rows,bound", [(1, 16), (1, 400), (9, 16), (9, 100), (100, 4096)])
 def test_the_bound_on_a_requests_rows_may_be_loose(rows, bound):
     b = Batch(4, 2, 128, 16, [400, 111], [rows, 1])
