@@ -18,6 +18,7 @@ store and per-call blob binding.
 from __future__ import annotations
 
 import ctypes
+from contextlib import nullcontext
 from dataclasses import dataclass
 from typing import List, Optional, Sequence
 
@@ -50,6 +51,12 @@ def _stream(stream: Optional[torch.cuda.Stream]) -> Optional[int]:
     # torch.cuda.current_stream() without the stream object it makes (several microseconds a call,
     # more than a decode operator's own launch)
     return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice()) or None
+
+
+def _owner(stream: Optional[torch.cuda.Stream]):
+    """Within it, memory for results is that of the stream that writes them: the current one may still use what it has
+    freed."""
+    return nullcontext() if stream is None else torch.cuda.stream(stream)
 
 
 def validateGTurboLayout(path: str, d: int, f: int) -> binding.FFGTurboLayoutInfo:
@@ -221,7 +228,8 @@ class HotpathContext:
                  stream=None) -> torch.Tensor:
         tokens = x.shape[0]
         if y is None:
-            y = torch.empty((tokens, self.d), dtype=torch.bfloat16, device=x.device)
+            with _owner(stream):
+                y = torch.empty((tokens, self.d), dtype=torch.bfloat16, device=x.device)
         call("ff_moe_layer", self.handle, layer, _ptr(x), tokens, _ptr(y), _ptr(ids), _ptr(weights),
              _stream(stream))
         return y
@@ -233,7 +241,8 @@ class HotpathContext:
         4's stack); `ids` int32 [layerCount, tokens, K] receives every layer's routes."""
         tokens = x.shape[0]
         if y is None:
-            y = torch.empty((tokens, self.d), dtype=torch.bfloat16, device=x.device)
+            with _owner(stream):
+                y = torch.empty((tokens, self.d), dtype=torch.bfloat16, device=x.device)
         call("ff_moe_stack", self.handle, firstLayer, layerCount, _ptr(x), tokens, eps, _ptr(y),
              _ptr(ids), _stream(stream))
         return y
@@ -251,7 +260,8 @@ class HotpathContext:
     def rmsnorm(self, x: torch.Tensor, w: Optional[torch.Tensor], eps: float,
                 y: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
         if y is None:
-            y = torch.empty_like(x)
+            with _owner(stream):
+                y = torch.empty_like(x)
         call("ff_rmsnorm", self.handle, _ptr(x), _ptr(w), eps, x.shape[0], _ptr(y), _stream(stream))
         return y
 
@@ -461,8 +471,9 @@ class PrefillGroupedRoutedMoE:
         token, group, rank, 0 — rows past the kept routes are unwritten —, offsets int32 [groups+1]),
         both on the device; asynchronous on the stream."""
         tokens = groupIds.shape[0]
-        pairs = torch.empty((tokens * self.context.topK, 4), dtype=torch.int32, device=groupIds.device)
-        offsets = torch.empty(groups + 1, dtype=torch.int32, device=groupIds.device)
+        with _owner(stream):
+            pairs = torch.empty((tokens * self.context.topK, 4), dtype=torch.int32, device=groupIds.device)
+            offsets = torch.empty(groups + 1, dtype=torch.int32, device=groupIds.device)
         call("ff_sort_routes", self.context.handle, _ptr(groupIds), tokens, groups, _ptr(pairs), _ptr(offsets),
              _stream(stream))
         return pairs, offsets
