@@ -26,6 +26,8 @@ __all__ = ["AttentionContext", "FieldfareError", "NO_SLOT"]
 
 NO_SLOT = -1  # as int32; also a table entry without a page
 
+_WORD = 0xFFFFFFFF  # (ctypes would cut what is more without a word)
+
 _SCALING = {"none": 0, "linear": 1, "byParts": 2}
 
 
@@ -98,7 +100,11 @@ class AttentionContext:
         row, head, value = t.stride()
         if tokens and (value != 1 or (head != dim and heads > 1)):
             raise ValueError(f"{what} must have the heads of a row side by side")
-        return t.data_ptr(), row if tokens > 1 else heads * dim
+        if tokens < 2:
+            return t.data_ptr(), heads * dim
+        if row > _WORD:
+            raise ValueError(f"rows of {what} must be less than 2^32 elements apart")
+        return t.data_ptr(), row
 
     def _cache(self, pages: torch.Tensor) -> tuple:
         count = pages.shape[0] if pages.dim() else 0
@@ -214,6 +220,8 @@ class AttentionContext:
             raise ValueError("lengths, blockTable and rowStart must agree on the number of requests")
         if window < 0 or sinks < 0 or maxRows < 0:
             raise ValueError("window, sinks and maxRows must not be negative")
+        if window > _WORD or sinks > _WORD or maxRows > _WORD:  # (more than any request has)
+            window, sinks, maxRows = min(window, _WORD), min(sinks, _WORD), min(maxRows, _WORD)
         if out is None:
             out = self._new((tokens, self.heads, self.headDim), torch.bfloat16, stream)
         self._ints("blockTable rowStart lengths", blockTable, rowStart, lengths)

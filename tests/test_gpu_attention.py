@@ -722,6 +722,29 @@ def test_arguments_that_the_library_refuses():
     assert ctx.attend(b.q[:0], b.cache, ints(b.table), ints([0, 0, 0]), ints(b.lengths), 1).shape == (0, 4, 64)
 
 
+def test_numbers_past_32_bits_are_not_cut():
+    """Rows further apart than 2^32 elements are refused; windows, sinks and bounds on rows past 2^32 are what they say."""
+    b = Batch(4, 2, 64, 16, [300, 200], [2, 2])
+    far = torch.empty((1 << 32) + 4096, dtype=torch.bfloat16, device="cuda")
+    q = far.as_strided((4, 4, 64), ((1 << 32) // 3 // 8 * 8, 64, 1))  # below 2^32, the last row past it
+    q.copy_(b.q)
+    b.check(b.ctx.attend(q, b.cache, ints(b.table), ints([0, 2, 4]), ints(b.lengths), 2))
+    q = far.as_strided((2, 4, 64), ((1 << 32) + 256, 64, 1))
+    q.copy_(b.q[:2])
+    one = ints(b.table[:1]), ints([0, 2]), ints(b.lengths[:1])
+    with pytest.raises(ValueError, match="apart"):
+        b.ctx.attend(q, b.cache, *one, 2)
+    with pytest.raises(ValueError, match="apart"):
+        b.ctx.attend(b.q[:2], b.cache, *one, 2, out=q)
+    del far, q
+    want = b.attend()
+    assert torch.equal(b.attend(window=(1 << 32) + 5), want)
+    assert torch.equal(b.attend(window=1 << 32, sinks=(1 << 32) + 3), want)
+    assert torch.equal(b.attend(window=7, sinks=(1 << 32) + 3), want)
+    assert torch.equal(b.ctx.attend(b.q, b.cache, ints(b.table), ints([0, 2, 4]), ints(b.lengths), (1 << 32) + 2),
+                       b.ctx.attend(b.q, b.cache, ints(b.table), ints([0, 2, 4]), ints(b.lengths), 4))
+
+
 def test_a_table_that_is_too_large_to_count_is_refused():
     from ane_fieldfare_b200.attention import FieldfareError
     from ane_fieldfare_b200.binding import call
