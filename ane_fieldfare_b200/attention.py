@@ -157,9 +157,9 @@ class AttentionContext:
         call("ff_rope_table", self.handle, ctypes.byref(config), table.data_ptr(), positions, _stream(stream))
         return table
 
-    def rope(self, x: torch.Tensor, table: torch.Tensor, positions: torch.Tensor, y: Optional[torch.Tensor] = None,
+    def rope(self, x: torch.Tensor, table: Optional[torch.Tensor], positions: torch.Tensor, y: Optional[torch.Tensor] = None,
              *, interleaved: bool = False, stream=None) -> torch.Tensor:
-        """Rotated heads of x [tokens][any heads][headDim]; y may be x."""
+        """Rotated heads of x [tokens][any heads][headDim] (table None: as they are); y may be x."""
         if x.dim() != 3 or positions.numel() != x.shape[0]:
             raise ValueError("x must be [tokens][heads][headDim], with one position per row")
         tokens, heads = x.shape[:2]

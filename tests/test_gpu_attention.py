@@ -204,6 +204,19 @@ def test_rope_turns_pairs_and_rounds_once(dim, rotary, interleaved):
         assert torch.equal(x, y)
 
 
+@pytest.mark.parametrize("dim,heads", [(64, 5), (256, 3)])
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_heads_that_do_not_rotate_pass_through_the_kernel(dim, heads, interleaved):
+    """No rotary table: bit for bit what came in, NaN and all, at other strides."""
+    ctx = context(dim=dim)
+    x = torch.randint(-32768, 32768, (9, heads, dim), device="cuda", generator=generator()).to(torch.int16).view(torch.bfloat16)
+    y = torch.zeros((9, heads + 2, dim), dtype=torch.bfloat16, device="cuda")
+    before = ctx.info().kernelLaunches
+    ctx.rope(x, None, ints([4_000_000_000 - (1 << 32)] * 9), y[:, 1:-1], interleaved=interleaved)
+    assert torch.equal(y[:, 1:-1].contiguous().view(torch.int16), x.view(torch.int16)) and not y[:, 0].any() and not y[:, -1].any()
+    assert ctx.info().kernelLaunches == before + 1 and ctx.info().deviceErrorFlag == 0
+
+
 def test_a_position_outside_the_table_is_reported():
     ctx = context()
     x = rows_of(generator(), 2, 4, 64)
