@@ -18,13 +18,16 @@
 // Logits are then exact but for 32-bit sums.  A weight is rounded to 11 bits once, for sum and output alike; times the value scale it
 // would be rounded again, so that the codes' and the biases' part of a value that is near zero would not cancel: what that
 // rounding leaves goes through a second product (up to four columns: through the four columns that a tile of eight has to spare).
-// A weight below 2^-24 of the largest of its warp's keys so far is lost.
+// A weight below 2^-24 of the largest of its warp's keys so far is lost, and what of a value is below 2^-31 of the largest value so far.
 //
-// Bound by the cache's bytes and by latency.  131072 keys of 8 heads of 128 (151 MB) take 45 us, 3.3 TB/s or 51 % of a copy's
-// rate; with the arithmetic left out 33 us.  A warp executes 611 instructions for 32 keys of 128, all of the kernel's counted.  64
-// ragged requests (261 MB) take 75 us, 3.5 TB/s, at 46 % of the issue slots, and 53 us with the arithmetic left out.  Three CTAs an SM
-// with fewer registers a thread: 131072 keys 48.4 us where two take 44.3, ragged 73.4 and 73.1.  2000 keys of 8 heads of 256 are 13.5 us of
-// waits one after another: look-up of the requests 1.0, queries 1.7, tiles 3.4, joins in the CTA 1 and of the parts 2.
+// Bound by the cache's bytes and by latency.  131072 keys of 8 heads of 128 (151 MB) take 46.8 us, 3.2 TB/s or 49 % of a copy's
+// rate; with the arithmetic left out 33 us.  A warp executes about 610 instructions for 32 keys of 128, all of the kernel's counted.  64
+// ragged requests (261 MB) take 76.5 us, 3.4 TB/s, at 46 % of the issue slots, and 53 us with the arithmetic left out.  Three CTAs an SM
+// with fewer registers a thread: 131072 keys 48.4 us where two took 44.3, ragged 73.4 and 73.1.  2000 keys of 8 heads of 256 are 14.1 us of
+// waits one after another (in a timeline of 13.5: look-up of the requests 1.0, queries 1.7, tiles 3.4, joins in the CTA 1 and of the
+// parts 2; the checks of lengths and row starts came behind it).
+// Registers: none spill at 64 values a head; at 128, 240 bytes with more than 8 columns; at 256, 144 bytes with up to 4 columns, 128
+// with up to 8 and 532 with more, which also leave room for one CTA an SM alone.
 #include <algorithm>
 #include <string>
 

@@ -19,16 +19,17 @@
 //
 // f16 holds 11 bits of keys, values and weights where bf16 would hold 8; its range is kept by powers of two: a row's
 // own for the queries, a tile's own for keys (taken back with the logits) and for values (E, part of the exponent of P and
-// of the maximum M that P stays below 2^14 of; keys and values of 2^116 and more are out of its reach).  A weight below 2^-30 of the largest of
-// its part of the keys is lost.  A code masked in place is the f16 code * 2^-24 or * 2^-20, and one FMA with scale times 2^24 or
+// of the maximum M that P stays below 2^14 of; keys and values of 2^116 and more are out of its reach).  Lost is what of a key or value is
+// below 2^-20 of the largest of its tile, and a weight whose product with its tile's largest value is below 2^-30 of the largest such of its
+// part of the keys; it is in the sum of the weights all the same, which does not know E.  A code masked in place is the f16 code * 2^-24 or * 2^-20, and one FMA with scale times 2^24 or
 // 2^20 and the bias rounds once: nine instructions a word of eight codes.
 //
-// 4096 rows of 16 heads of 256 over 36864 keys take 2.19 ms, 1.07 PFLOP/s: 66 % of the burst bf16 rate, 78 % of the sustained one
-// (at 36864 keys the power limit holds the clock below its maximum).  A tile takes 1.16 us.  Its MMAs alone are 1077 cycles: 16 of
+// 4096 rows of 16 heads of 256 over 36864 keys take 2.28 ms, 1.03 PFLOP/s: 63 % of the burst bf16 rate, 75 % of the sustained one
+// (at 36864 keys the power limit holds the clock below its maximum).  A tile takes 1.2 us.  Its MMAs alone are 1077 cycles: 16 of
 // 32.8 and 4 of 138, each form timed by itself.  The tensor pipe is active 45 % of the time at 8192 keys: S of a tile waits in one of
 // two buffers until its weights are formed, and tensor memory has no third at 256 values a head.  4096 rows in a window of 1024 take
-// 143 us: 19 tiles a unit, beside which queries, first logits, output and parts of units count; five ragged requests of up to
-// 613 rows with 14 heads of 64 27.5 us.
+// 148 us: 19 tiles a unit, beside which queries, first logits, output and parts of units count; five ragged requests of up to
+// 613 rows with 14 heads of 64 28.5 us.
 #include <algorithm>
 #include <string>
 
@@ -42,8 +43,8 @@ namespace {
 constexpr int kKeyCopyWarp = 0, kMmaWarp = 1, kScaleWarp = 2, kValueCopyWarp = 3, kDequantWarps = 16, kRowGroups = 2;
 constexpr int kFirstDequant = 4, kFirstRowWarp = kFirstDequant + kDequantWarps, kRowWarps = 4 * kRowGroups;
 constexpr int kTilesThreads = 32 * (kFirstRowWarp + kRowWarps);
-// registers a thread by role: together no more than the launch's 72 each (4096 rows over 36864 keys, in one run: eight
-// expanding warps 2.34 ms, twelve 2.12 to 2.14, sixteen 2.01; a later run at another clock took 2.19)
+// registers a thread by role: together no more than the launch's 72 each (4096 rows over 36864 keys, one after the other on one
+// card: eight expanding warps 2.34 ms, twelve 2.12 to 2.14, sixteen 2.01)
 constexpr int kRegsOthers = 48, kRegsRows = 128;
 static_assert(128 * kRegsOthers + 32 * kDequantWarps * kRegsOthers + 32 * kRowWarps * kRegsRows <= kTilesThreads * 72, "register split");
 constexpr uint32_t kRows = kTileRows;

@@ -8,8 +8,10 @@ namespace ff {
 
 bool launch_attend(FFAttention *att, const AttendArgs &a, cudaStream_t stream, const char **error) {
     // Columns of a key/value head: up to 16 as columns of mma.sync, which then take as long as the cache's bytes; more as rows of
-    // tcgen05.mma.  us as columns / as rows: 16 columns of 128, 64 requests of up to 16384 keys 43 / 67; 10 of 256, 8 x 4000 keys
-    // 57 / 53; 32 of 256, 20000 keys 66 / 41; 32 of 128, 16 requests of up to 3000 keys 44 / 30.
+    // tcgen05.mma.  us as columns / as rows: 16 columns of 128, 64 requests of up to 16384 keys 72 / 98; 32 of 128, 16 requests of
+    // up to 3000 keys 28 / 28; 2 of 256 in a window of 1024 13 / 20; 4 of 256, 8000 keys 20 / 33; 32 of 256, 20000 keys 68 / 45.  At
+    // 256 values a head, where more than 8 columns spill registers, 9 to 16 go the slower way (10, 8 x 4000 keys 59 / 54; 16, 8000 keys
+    // 42 / 34, in a window of 1024 24 / 21): the boundary is one for all head sizes.
     if (a.maxRows * (a.heads / a.kvHeads) <= 16) return launch_attend_rows(att, a, stream, error);
     return launch_attend_tiles(att, a, stream, error);
 }

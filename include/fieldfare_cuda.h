@@ -481,9 +481,9 @@ FFAttentionInfo ff_attention_get_info(const FFAttention *attention);
  * the handle: after flag 17 results are undefined until this is called.  It is sticky; a kernel sets it to
  * 13: no free page was left, 14: a request is longer than its block table row, 15: more rows than the
  * arrays hold, or a rowStart that goes back (every row is zero then), 16: a page or slot outside the cache, 17: a wait was
- * given up, 18: a position outside the rotary table, 19: more work in a call of ff_attention than 2^32 tiles of 64 keys,
- * counted for every head and tile of rows (every row is zero then).  What such an entry names is left out; nothing outside
- * the arrays is touched. */
+ * given up, 18: a position outside the rotary table (its row is turned as position 0), 19: more work in a call of ff_attention than 2^32 tiles of 64 keys,
+ * counted for every head and tile of rows (every row is zero then).  What else such an entry names is left out; nothing
+ * outside the arrays is touched. */
 bool ff_attention_reset_device_error(FFAttention *attention, const char **error);
 /* Bytes of one page of one layer; 0 for a configuration that ff_attention_create refuses. */
 uint64_t ff_cache_page_bytes(const FFAttentionConfig *config);
@@ -563,8 +563,11 @@ bool ff_cache_read(FFAttention *attention, const void *pages, uint32_t pageCount
  * maxRows: no request has more rows (it chooses the kernel; rows past it are zero, flag 15).  Up to 16 columns (rows times
  * heads/kvHeads) run on mma.sync on the codes as they lie, more on the 5th-generation tensor cores; either way the keys are
  * split over the CTAs, so that one request fills the GPU.  Keys on a page outside the cache are not seen (flag 16).
- * Sums are fp32, factors f16 at powers of two of their own: weights below 2^-24 of the largest of their part of the keys may count
- * as zero; keys and values from 2^116 on and queries from 2^110 on may give results that are not finite. */
+ * Sums are fp32, factors f16 at powers of two of their own.  So these may count as zero: up to 16 columns, weights below 2^-24 of
+ * the largest of their part of the keys, and values below 2^-31 of the largest that came before; more columns, keys and values
+ * below 2^-20 of the largest of their 64 keys, and weights that, times the largest value of their 64 keys, are below 2^-30 of the
+ * largest such product.  Keys and values from 2^116 on, queries from 2^110 on, and logits (scale q.k) from 2^24 on may give results
+ * that are not finite. */
 bool ff_attention(FFAttention *attention, const uint16_t *q, uint32_t qStride, uint32_t tokens, const void *pages,
                   uint32_t pageCount, const uint32_t *blockTable, uint32_t tableStride, const uint32_t *rowStart,
                   const uint32_t *lengths, uint32_t requests, uint32_t maxRows, float scale, uint32_t window,
