@@ -22,9 +22,11 @@ from . import binding
 from .binding import FFAttentionConfig, FFRope, FFRopeConfig, FieldfareError, call
 from .hotpath import _stream
 
-__all__ = ["AttentionContext", "FieldfareError", "NO_SLOT"]
+__all__ = ["AttentionContext", "BLOCK_KEYS", "FieldfareError", "NO_SLOT"]
 
 NO_SLOT = -1  # as int32; also a table entry without a page
+
+BLOCK_KEYS = 64  # of a block that selectBlocks names
 
 _WORD = 0xFFFFFFFF  # (ctypes would cut what is more without a word)
 
@@ -129,10 +131,11 @@ class AttentionContext:
 
     def plan(self, oldLengths: torch.Tensor, newLengths: torch.Tensor, blockTable: torch.Tensor, freePages: torch.Tensor,
              freeCount: torch.Tensor, freeCountOut: torch.Tensor, rowStart: torch.Tensor, positions: torch.Tensor,
-             slots: torch.Tensor, stream=None):
+             slots: torch.Tensor, stream=None, *, heldPages: Optional[torch.Tensor] = None):
         """Request r goes from oldLengths[r] to newLengths[r] tokens: pages given back and taken (blockTable [requests]
         [pages], the stack freePages with freeCount [1] entries; freeCountOut may be freeCount), and a row for every new
-        token: rowStart [requests + 1], positions and slots [rows]."""
+        token: rowStart [requests + 1], positions and slots [rows].  heldPages [requests]: of a request's pages the first that
+        are another's (a shared prefix), neither taken nor given back."""
         requests, rows = oldLengths.numel(), slots.numel()
         shape = blockTable.shape
         if newLengths.numel() != requests or len(shape) != 2 or shape[0] != requests or rowStart.numel() != requests + 1:
@@ -141,6 +144,14 @@ class AttentionContext:
             raise ValueError("one position and one slot per row; one word for the stack's height")
         self._ints("oldLengths newLengths blockTable freePages freeCount freeCountOut rowStart positions slots", oldLengths, newLengths,
                    blockTable, freePages, freeCount, freeCountOut, rowStart, positions, slots)
+        if heldPages is not None:
+            if heldPages.numel() != requests:
+                raise ValueError("heldPages must have an entry per request")
+            self._ints("heldPages", heldPages)
+            call("ff_cache_plan_shared", self.handle, oldLengths.data_ptr(), newLengths.data_ptr(), requests, blockTable.data_ptr(), shape[1],
+                 freePages.data_ptr(), freePages.numel(), freeCount.data_ptr(), freeCountOut.data_ptr(), rowStart.data_ptr(),
+                 positions.data_ptr(), slots.data_ptr(), rows, heldPages.data_ptr(), _stream(stream))
+            return
         call("ff_cache_plan", self.handle, oldLengths.data_ptr(), newLengths.data_ptr(), requests, blockTable.data_ptr(), shape[1],
              freePages.data_ptr(), freePages.numel(), freeCount.data_ptr(), freeCountOut.data_ptr(), rowStart.data_ptr(),
              positions.data_ptr(), slots.data_ptr(), rows, _stream(stream))
@@ -229,3 +240,49 @@ class AttentionContext:
              rowStart.data_ptr(), lengths.data_ptr(), requests, maxRows, self.headDim ** -0.5 if scale is None else scale, window, sinks,
              *self._heads(out, self.heads, tokens, "out"), _stream(stream))
         return out
+
+    # -- a part of a long context ------------------------------------------------------------------
+
+    def newMeans(self, pages: int) -> torch.Tensor:
+        """Memory for the mean keys of one layer's cache, bf16 [pages][kvHeads][blocks of a page][headDim]."""
+        return torch.zeros((pages, self.kvHeads, max(1, self.pageTokens // BLOCK_KEYS), self.headDim), dtype=torch.bfloat16, device=self.device)
+
+    def _means(self, means: torch.Tensor) -> tuple:
+        count = means.shape[0] if means.dim() else 0
+        if (means.dtype is not torch.bfloat16 or means.get_device() != self._ordinal or not means.is_contiguous()
+                or means.numel() != count * self.kvHeads * max(1, self.pageTokens // BLOCK_KEYS) * self.headDim):
+            raise ValueError(f"mean keys are contiguous bf16 [pages][{self.kvHeads}][{max(1, self.pageTokens // BLOCK_KEYS)}][{self.headDim}] on {self.device}")
+        return means.data_ptr(), count
+
+    def blockMeans(self, pages: torch.Tensor, blockTable: torch.Tensor, oldLengths: torch.Tensor, newLengths: torch.Tensor,
+                   means: torch.Tensor, stream=None):
+        """The mean keys of the blocks of 64 keys that requests complete by going from oldLengths to newLengths tokens, of
+        which `pages` holds the keys (append first)."""
+        requests, shape = newLengths.numel(), blockTable.shape
+        if oldLengths.numel() != requests or len(shape) != 2 or shape[0] != requests:
+            raise ValueError("lengths and blockTable must agree on the number of requests")
+        self._ints("blockTable oldLengths newLengths", blockTable, oldLengths, newLengths)
+        (cache, count), (to, places) = self._cache(pages), self._means(means)
+        if places != count:
+            raise ValueError("pages and means must agree on the number of pages")
+        call("ff_block_means", self.handle, cache, count, blockTable.data_ptr(), shape[1], oldLengths.data_ptr(), newLengths.data_ptr(),
+             requests, to, _stream(stream))
+
+    def selectBlocks(self, q: torch.Tensor, means: torch.Tensor, blockTable: torch.Tensor, rowStart: torch.Tensor,
+                     lengths: torch.Tensor, blocks: int, *, first: int = 1, last: int = 1, ids: Optional[torch.Tensor] = None,
+                     stream=None) -> torch.Tensor:
+        """The blocks that every row attends to, int32 [tokens][kvHeads][blocks] in ascending order, -1 behind: the first
+        `first`, the last `last`, and of those between them the ones whose mean keys the row's queries score highest."""
+        tokens, requests, shape = q.shape[0], lengths.numel(), blockTable.shape
+        if rowStart.numel() != requests + 1 or len(shape) != 2 or shape[0] != requests:
+            raise ValueError("lengths, blockTable and rowStart must agree on the number of requests")
+        if not 0 <= first <= _WORD or not 0 <= last <= _WORD or not 0 <= blocks <= _WORD:
+            raise ValueError("blocks, first and last must not be negative, or 2^32 and more")
+        if ids is None:
+            ids = self._new((tokens, self.kvHeads, blocks), torch.int32, stream)
+        elif ids.shape != (tokens, self.kvHeads, blocks):
+            raise ValueError(f"ids must be [{tokens}][{self.kvHeads}][{blocks}]")
+        self._ints("blockTable rowStart lengths ids", blockTable, rowStart, lengths, ids)
+        call("ff_select_blocks", self.handle, *self._heads(q, self.heads, tokens, "q"), tokens, *self._means(means), blockTable.data_ptr(), shape[1],
+             rowStart.data_ptr(), lengths.data_ptr(), requests, blocks, first, last, ids.data_ptr(), _stream(stream))
+        return ids

@@ -63,6 +63,23 @@ bool check_cache(const FFAttention *att, const void *pages, uint32_t pageCount, 
     return true;
 }
 
+bool check_requests(const FFAttention *att, uint32_t requests, const char **error) {
+    if (requests > att->cfg.maxRequests)
+        return fail(error, std::to_string(requests) + " requests exceed the handle's maxRequests " + std::to_string(att->cfg.maxRequests));
+    return true;
+}
+
+bool check_table(const uint32_t *blockTable, uint32_t tableStride, const char **error) {
+    if (!blockTable || !aligned(blockTable, 4)) return fail(error, "blockTable must be non-null and 4-byte aligned");
+    if (tableStride == 0) return fail(error, "tableStride must be positive");
+    return true;
+}
+
+constexpr uint32_t kSelectBlock = 64;  // keys
+
+// keys that a row of the block table has room for
+uint32_t table_keys(const FFAttentionConfig &c, uint32_t tableStride) { return (uint32_t)std::min<uint64_t>((uint64_t)tableStride * c.pageTokens, UINT32_MAX); }
+
 bool check_rope(const FFAttention *att, const FFRope *rope, const uint32_t *positions, const char **error) {
     if (!rope) return fail(error, "rope is null");
     if (rope->rotaryDim % 16 || rope->rotaryDim > att->cfg.headDim) return fail(error, "rotaryDim must be a multiple of 16 up to headDim");
@@ -168,9 +185,9 @@ bool ff_attention_reset_device_error(FFAttention *att, const char **error) {
     return true;
 }
 
-bool ff_cache_plan(FFAttention *att, const uint32_t *oldLengths, const uint32_t *newLengths, uint32_t requests, uint32_t *blockTable,
-                   uint32_t tableStride, uint32_t *freePages, uint32_t pageCount, const uint32_t *freeCountIn, uint32_t *freeCountOut,
-                   uint32_t *rowStart, uint32_t *positions, uint32_t *slots, uint32_t rows, void *stream, const char **error) {
+bool ff_cache_plan_shared(FFAttention *att, const uint32_t *oldLengths, const uint32_t *newLengths, uint32_t requests, uint32_t *blockTable,
+                          uint32_t tableStride, uint32_t *freePages, uint32_t pageCount, const uint32_t *freeCountIn, uint32_t *freeCountOut,
+                          uint32_t *rowStart, uint32_t *positions, uint32_t *slots, uint32_t rows, const uint32_t *heldPages, void *stream, const char **error) {
     if (!begin(att, error)) return false;
     if (requests > att->cfg.maxRequests)
         return fail(error, std::to_string(requests) + " requests exceed the handle's maxRequests " + std::to_string(att->cfg.maxRequests));
@@ -179,13 +196,21 @@ bool ff_cache_plan(FFAttention *att, const uint32_t *oldLengths, const uint32_t 
         return fail(error, "null argument");
     const uintptr_t all = reinterpret_cast<uintptr_t>(oldLengths) | reinterpret_cast<uintptr_t>(newLengths) | reinterpret_cast<uintptr_t>(blockTable) |
                           reinterpret_cast<uintptr_t>(freePages) | reinterpret_cast<uintptr_t>(freeCountIn) | reinterpret_cast<uintptr_t>(freeCountOut) |
-                          reinterpret_cast<uintptr_t>(rowStart) | reinterpret_cast<uintptr_t>(positions) | reinterpret_cast<uintptr_t>(slots);
+                          reinterpret_cast<uintptr_t>(rowStart) | reinterpret_cast<uintptr_t>(positions) | reinterpret_cast<uintptr_t>(slots) |
+                          reinterpret_cast<uintptr_t>(heldPages);
     if (all & 3u) return fail(error, "arrays must be 4-byte aligned");
     if (tableStride == 0) return fail(error, "tableStride must be positive");
     if ((uint64_t)requests * tableStride > 1u << 30) return fail(error, "the block table has more than 2^30 entries");
     if ((uint64_t)pageCount * att->cfg.pageTokens >= FF_NO_SLOT) return fail(error, "the cache has more slots than 32 bits name");
     return launch_cache_plan(att, oldLengths, newLengths, requests, blockTable, tableStride, freePages, pageCount, freeCountIn, freeCountOut,
-                             rowStart, positions, slots, rows, static_cast<cudaStream_t>(stream), error);
+                             rowStart, positions, slots, rows, heldPages, static_cast<cudaStream_t>(stream), error);
+}
+
+bool ff_cache_plan(FFAttention *att, const uint32_t *oldLengths, const uint32_t *newLengths, uint32_t requests, uint32_t *blockTable,
+                   uint32_t tableStride, uint32_t *freePages, uint32_t pageCount, const uint32_t *freeCountIn, uint32_t *freeCountOut,
+                   uint32_t *rowStart, uint32_t *positions, uint32_t *slots, uint32_t rows, void *stream, const char **error) {
+    return ff_cache_plan_shared(att, oldLengths, newLengths, requests, blockTable, tableStride, freePages, pageCount, freeCountIn, freeCountOut, rowStart,
+                                positions, slots, rows, nullptr, stream, error);
 }
 
 bool ff_rope_table(FFAttention *att, const FFRopeConfig *config, float *table, uint32_t positions, void *stream, const char **error) {
@@ -266,6 +291,42 @@ bool ff_attention(FFAttention *att, const uint16_t *q, uint32_t qStride, uint32_
                  (uint32_t)std::min<uint64_t>((uint64_t)tableStride * c.pageTokens, UINT32_MAX), blockTable, rowStart, lengths, requests,
                  std::min(maxRows, std::max(1u, tokens)), scale, window, sinks, c.heads, c.kvHeads, page_layout(c), att->errorFlag};
     return launch_attend(att, a, static_cast<cudaStream_t>(stream), error);
+}
+
+bool ff_block_means(FFAttention *att, const void *pages, uint32_t pageCount, const uint32_t *blockTable, uint32_t tableStride, const uint32_t *oldLengths,
+                    const uint32_t *newLengths, uint32_t requests, uint16_t *means, void *stream, const char **error) {
+    if (!begin(att, error)) return false;
+    const FFAttentionConfig &c = att->cfg;
+    if (!check_requests(att, requests, error)) return false;
+    if (requests == 0) return true;
+    if (!check_cache(att, pages, pageCount, error) || !check_table(blockTable, tableStride, error)) return false;
+    if (!oldLengths || !newLengths || !means) return fail(error, "null argument");
+    if (!aligned(oldLengths, 4) || !aligned(newLengths, 4)) return fail(error, "arrays must be 4-byte aligned");
+    if (!aligned(means, 16)) return fail(error, "means must be 16-byte aligned");
+    return launch_block_means(att, static_cast<const uint8_t *>(pages), pageCount, blockTable, tableStride, table_keys(c, tableStride), oldLengths, newLengths,
+                              requests, means, static_cast<cudaStream_t>(stream), error);
+}
+
+bool ff_select_blocks(FFAttention *att, const uint16_t *q, uint32_t qStride, uint32_t tokens, const uint16_t *means, uint32_t pageCount,
+                      const uint32_t *blockTable, uint32_t tableStride, const uint32_t *rowStart, const uint32_t *lengths, uint32_t requests,
+                      uint32_t blocks, uint32_t first, uint32_t last, uint32_t *ids, void *stream, const char **error) {
+    if (!begin(att, error)) return false;
+    const FFAttentionConfig &c = att->cfg;
+    if (blocks == 0 || blocks > (1u << 20)) return fail(error, "need 1..2^20 blocks a list");
+    if (last == 0) return fail(error, "a row's own block is always in its list: last must be positive");
+    if (first > blocks || last > blocks - first) return fail(error, "the first and the last blocks are more than a list holds");
+    if (tokens == 0) return true;
+    if (!check_tokens(att, tokens, error) || !check_heads(att, q, qStride, c.heads, "query", error) || !check_requests(att, requests, error) ||
+        !check_table(blockTable, tableStride, error))
+        return false;
+    if (!means || !rowStart || !lengths || !ids) return fail(error, "null argument");
+    if (!aligned(means, 16)) return fail(error, "means must be 16-byte aligned");
+    if (!aligned(rowStart, 4) || !aligned(lengths, 4) || !aligned(ids, 4)) return fail(error, "arrays must be 4-byte aligned");
+    if ((uint64_t)pageCount * c.pageTokens >= FF_NO_SLOT) return fail(error, "the cache has more slots than 32 bits name");
+    const uint64_t keys = (uint64_t)tableStride * c.pageTokens;
+    if (keys > 1u << 21) return fail(error, "block table rows of more than 2^21 keys: their scores do not fit a CTA");
+    return launch_select_blocks(att, q, qStride, tokens, means, pageCount, blockTable, tableStride, (uint32_t)((keys + kSelectBlock - 1) / kSelectBlock), rowStart,
+                                lengths, requests, blocks, first, last, ids, static_cast<cudaStream_t>(stream), error);
 }
 
 }  // extern "C"

@@ -27,6 +27,7 @@ enum AttentionFlag : uint32_t {
     kFlagWait = 17,
     kFlagPosition = 18,
     kFlagWork = 19,
+    kFlagHeld = 20,
 };
 
 // A block: one key/value head of one page.  Offsets in bytes from its start.
@@ -79,7 +80,8 @@ struct AttendArgs {
 // ff_cache.cu
 bool launch_cache_plan(FFAttention *att, const uint32_t *oldLengths, const uint32_t *newLengths, uint32_t requests, uint32_t *blockTable,
                        uint32_t tableStride, uint32_t *freePages, uint32_t pageCount, const uint32_t *freeCountIn, uint32_t *freeCountOut,
-                       uint32_t *rowStart, uint32_t *positions, uint32_t *slots, uint32_t rows, cudaStream_t stream, const char **error);
+                       uint32_t *rowStart, uint32_t *positions, uint32_t *slots, uint32_t rows, const uint32_t *heldPages, cudaStream_t stream,
+                       const char **error);
 bool launch_rope_table(FFAttention *att, const FFRopeConfig &config, float *table, uint32_t positions, cudaStream_t stream, const char **error);
 // Rows of heads that a launch rotates (keys: also quantizes); null pointers: none.
 struct RopeRows {
@@ -92,6 +94,13 @@ bool launch_rope_rows(FFAttention *att, const RopeRows &rows, const FFRope &rope
                       uint32_t tokens, uint8_t *pages, uint32_t pageCount, cudaStream_t stream, const char **error);
 bool launch_cache_read(FFAttention *att, const uint8_t *pages, uint32_t pageCount, const uint32_t *slots, uint32_t tokens, uint16_t *k,
                        uint16_t *v, cudaStream_t stream, const char **error);
+
+// ff_blocks.cu
+bool launch_block_means(FFAttention *att, const uint8_t *pages, uint32_t pageCount, const uint32_t *blockTable, uint32_t tableStride, uint32_t tableKeys,
+                        const uint32_t *oldLengths, const uint32_t *newLengths, uint32_t requests, uint16_t *means, cudaStream_t stream, const char **error);
+bool launch_select_blocks(FFAttention *att, const uint16_t *q, uint32_t qStride, uint32_t tokens, const uint16_t *means, uint32_t pageCount,
+                          const uint32_t *blockTable, uint32_t tableStride, uint32_t tableBlocks, const uint32_t *rowStart, const uint32_t *lengths,
+                          uint32_t requests, uint32_t blocks, uint32_t first, uint32_t last, uint32_t *ids, cudaStream_t stream, const char **error);
 
 // ff_attend_rows.cu
 uint32_t attend_rows_ctas(int smCount);

@@ -31,6 +31,7 @@ struct PlanArgs {
     uint32_t *freeCountOut, *rowStart, *positions, *slots;
     uint32_t rows, pageShift;
     uint32_t *done, *errorFlag;
+    const uint32_t *heldPages;  // null: none
 };
 
 // Rows are counted up to here, what is more stays there: more than the arrays hold by far (2^24), and two counts add up in 32
@@ -39,8 +40,8 @@ constexpr uint32_t kMost = 1u << 30;
 __device__ __forceinline__ uint32_t add_counts(uint32_t a, uint32_t b) { return min(a + b, kMost); }
 
 struct PlanRequest {
-    uint32_t rows, had, has;  // new rows; pages before and after, as far as the table row goes
-    uint32_t oldLength;
+    uint32_t rows, had, has;  // new rows; pages before and after, as far as the table row goes; not below `held`
+    uint32_t oldLength, held;  // held: its first pages that are another's, which it neither takes nor gives back
     bool cut;
     __device__ uint32_t taken() const { return has > had ? has - had : 0u; }
     __device__ uint32_t given() const { return had > has ? had - has : 0u; }
@@ -53,8 +54,9 @@ __device__ __forceinline__ PlanRequest plan_request(const PlanArgs &a, uint32_t 
     p.rows = after > before ? min(after - before, kMost) : 0u;
     const uint32_t had = (before >> a.pageShift) + ((before & mask) != 0u), has = (after >> a.pageShift) + ((after & mask) != 0u);
     p.cut = had > a.tableStride || has > a.tableStride;
-    p.had = min(had, a.tableStride);
-    p.has = min(has, a.tableStride);
+    p.held = a.heldPages ? min(__ldg(a.heldPages + r), a.tableStride) : 0u;
+    p.had = max(min(had, a.tableStride), p.held);
+    p.has = max(min(has, a.tableStride), p.held);
     return p;
 }
 
@@ -127,7 +129,8 @@ __device__ __forceinline__ bool plan_write(const PlanArgs &a, const PlanSums &s,
                     position = p.oldLength + n;
                     const uint32_t index = position >> a.pageShift;
                     uint32_t page = FF_NO_PAGE;
-                    if (index < p.had) page = a.blockTable[(size_t)r * a.tableStride + index];
+                    if (index < p.held) *a.errorFlag = kFlagHeld;
+                    else if (index < p.had) page = a.blockTable[(size_t)r * a.tableStride + index];
                     else if (index < p.has) page = taken_page(taken + index - p.had);
                     if (page < a.pageCount) slot = (page << a.pageShift) | (position & ((1u << a.pageShift) - 1u));
                     break;
@@ -243,9 +246,10 @@ static uint32_t shift_of(uint32_t pageTokens) { return (uint32_t)__builtin_ctz(p
 
 bool launch_cache_plan(FFAttention *att, const uint32_t *oldLengths, const uint32_t *newLengths, uint32_t requests, uint32_t *blockTable,
                        uint32_t tableStride, uint32_t *freePages, uint32_t pageCount, const uint32_t *freeCountIn, uint32_t *freeCountOut,
-                       uint32_t *rowStart, uint32_t *positions, uint32_t *slots, uint32_t rows, cudaStream_t stream, const char **error) {
+                       uint32_t *rowStart, uint32_t *positions, uint32_t *slots, uint32_t rows, const uint32_t *heldPages, cudaStream_t stream,
+                       const char **error) {
     PlanArgs a{oldLengths, newLengths, requests, blockTable, tableStride, freePages, pageCount, freeCountIn, freeCountOut,
-               rowStart, positions, slots, rows, shift_of(att->cfg.pageTokens), att->planCount, att->errorFlag};
+               rowStart, positions, slots, rows, shift_of(att->cfg.pageTokens), att->planCount, att->errorFlag, heldPages};
     const uint32_t grid = std::max(1u, std::min((rows + kPlanThreads - 1) / kPlanThreads, (uint32_t)att->smCount));
     return launched(att, launch_pdl(k_cache_plan, dim3(grid), dim3(kPlanThreads), 0, stream, a), "k_cache_plan", error);
 }

@@ -482,7 +482,8 @@ FFAttentionInfo ff_attention_get_info(const FFAttention *attention);
  * 13: no free page was left, 14: a request is longer than its block table row, 15: more rows than the
  * arrays hold, or a rowStart that goes back (every row is zero then), 16: a page or slot outside the cache, 17: a wait was
  * given up, 18: a position outside the rotary table (its row is turned as position 0), 19: more work in a call of ff_attention than 2^32 tiles of 64 keys,
- * counted for every head and tile of rows (every row is zero then).  What else such an entry names is left out; nothing
+ * counted for every head and tile of rows (every row is zero then), 20: a new token on a page that its request only
+ * shares.  What else such an entry names is left out; nothing
  * outside the arrays is touched. */
 bool ff_attention_reset_device_error(FFAttention *attention, const char **error);
 /* Bytes of one page of one layer; 0 for a configuration that ff_attention_create refuses. */
@@ -504,6 +505,15 @@ bool ff_cache_plan(FFAttention *attention, const uint32_t *oldLengths, const uin
                    uint32_t *blockTable, uint32_t tableStride, uint32_t *freePages, uint32_t pageCount,
                    const uint32_t *freeCountIn, uint32_t *freeCountOut, uint32_t *rowStart, uint32_t *positions,
                    uint32_t *slots, uint32_t rows, void *stream, const char **error);
+
+/* The same where requests share pages, as those of a long prefix that one of them holds: heldPages[r] of request r's first
+ * table entries are another request's pages (null: none are).  The caller writes these entries, counts the request's old length from behind
+ * them, and sees to it that their owner keeps them as long.  They are neither taken nor given back, whatever the lengths; a
+ * new token on one of them gets FF_NO_SLOT (flag 20). */
+bool ff_cache_plan_shared(FFAttention *attention, const uint32_t *oldLengths, const uint32_t *newLengths, uint32_t requests,
+                          uint32_t *blockTable, uint32_t tableStride, uint32_t *freePages, uint32_t pageCount,
+                          const uint32_t *freeCountIn, uint32_t *freeCountOut, uint32_t *rowStart, uint32_t *positions,
+                          uint32_t *slots, uint32_t rows, const uint32_t *heldPages, void *stream, const char **error);
 
 /* How a model's rotary frequencies base^(-2i/rotaryDim) are scaled for contexts longer than it was trained on. */
 typedef enum {
@@ -572,6 +582,31 @@ bool ff_attention(FFAttention *attention, const uint16_t *q, uint32_t qStride, u
                   uint32_t pageCount, const uint32_t *blockTable, uint32_t tableStride, const uint32_t *rowStart,
                   const uint32_t *lengths, uint32_t requests, uint32_t maxRows, float scale, uint32_t window,
                   uint32_t sinks, uint16_t *out, uint32_t outStride, void *stream, const char **error);
+
+/* Attention over a part of a long context: blocks of 64 keys (positions 64 b .. 64 b + 63) chosen for every row and key/value
+ * head by the scores of their mean keys.
+ *
+ * Mean keys of the blocks that requests complete by going from oldLengths[r] to newLengths[r] tokens (call it behind the step's
+ * appends; a block that is completed again after rows were taken back is formed again).  means: bf16 [pageCount][kvHeads]
+ * [max(1, pageTokens / 64)][headDim], a block on several pages at the last of them.  With m the mean of what the cache holds,
+ * in 64 bits, and e the exponent of its largest value (2^e <= |m| < 2^(e+1), within -60 .. 60): m in whole numbers of 2^(e-6), to the nearest,
+ * at most 127 of them.  A block with a key that stands for NaN is NaN throughout; one with a page outside the cache is zeros (flag 16). */
+bool ff_block_means(FFAttention *attention, const void *pages, uint32_t pageCount, const uint32_t *blockTable,
+                    uint32_t tableStride, const uint32_t *oldLengths, const uint32_t *newLengths, uint32_t requests,
+                    uint16_t *means, void *stream, const char **error);
+
+/* For every row and key/value head the ids of `blocks` blocks, ascending, ids uint32 [tokens][kvHeads][blocks]: the first
+ * `first`, the last `last` up to the row's own (at least its own, which may not be complete), and of those between them the ones that score
+ * highest, of equal ones the first.  A row with no more blocks than that gets all of them, and FF_NO_SLOT behind; a row that
+ * sees no key, and rows of no request, FF_NO_SLOT alone.  Score of a block: the largest q'.m over the head's query heads, m its mean as held,
+ * q' the query in whole numbers of 2^(e-6), to the nearest, at most 127 (e the exponent of its largest value, at least -100 and
+ * 60 below the largest e of the group; a query with a value that is not finite counts as zeros).  Such sums are exact: the lists do not
+ * depend on how they are formed.  NaN scores come first; blocks whose mean lies on a page outside the cache (flag 16) last.  q, rowStart
+ * and lengths as for ff_attention.  A row of the block table has room for at most 2^21 keys. */
+bool ff_select_blocks(FFAttention *attention, const uint16_t *q, uint32_t qStride, uint32_t tokens, const uint16_t *means,
+                      uint32_t pageCount, const uint32_t *blockTable, uint32_t tableStride, const uint32_t *rowStart,
+                      const uint32_t *lengths, uint32_t requests, uint32_t blocks, uint32_t first, uint32_t last,
+                      uint32_t *ids, void *stream, const char **error);
 
 /* Device-side result of the last ff_moe_prefill permute, copied to the host after a sync:
  * the expert-sorted pairs and per-expert row offsets [experts+1].  For parity tests. */
