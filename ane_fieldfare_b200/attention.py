@@ -286,3 +286,20 @@ class AttentionContext:
         call("ff_select_blocks", self.handle, *self._heads(q, self.heads, tokens, "q"), tokens, *self._means(means), blockTable.data_ptr(), shape[1],
              rowStart.data_ptr(), lengths.data_ptr(), requests, blocks, first, last, ids.data_ptr(), _stream(stream))
         return ids
+
+    def attendSelected(self, q: torch.Tensor, pages: torch.Tensor, blockTable: torch.Tensor, rowStart: torch.Tensor,
+                       lengths: torch.Tensor, ids: torch.Tensor, *, scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                       stream=None) -> torch.Tensor:
+        """`attend` over the blocks that ids [tokens][kvHeads][blocks] lists for every row and key/value head, up to the row's own key."""
+        tokens, requests, shape = q.shape[0], lengths.numel(), blockTable.shape
+        if rowStart.numel() != requests + 1 or len(shape) != 2 or shape[0] != requests:
+            raise ValueError("lengths, blockTable and rowStart must agree on the number of requests")
+        if ids.dim() != 3 or ids.shape[:2] != (tokens, self.kvHeads):
+            raise ValueError(f"ids must be [{tokens}][{self.kvHeads}][blocks]")
+        if out is None:
+            out = self._new((tokens, self.heads, self.headDim), torch.bfloat16, stream)
+        self._ints("blockTable rowStart lengths ids", blockTable, rowStart, lengths, ids)
+        call("ff_attention_selected", self.handle, *self._heads(q, self.heads, tokens, "q"), tokens, *self._cache(pages), blockTable.data_ptr(),
+             shape[1], rowStart.data_ptr(), lengths.data_ptr(), requests, ids.data_ptr(), ids.shape[2],
+             self.headDim ** -0.5 if scale is None else scale, *self._heads(out, self.heads, tokens, "out"), _stream(stream))
+        return out

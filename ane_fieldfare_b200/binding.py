@@ -152,6 +152,8 @@ SIGNATURES = {
     "ff_block_means": (c_bool, [c_void_p, _P, c_uint32, _P, c_uint32, _P, _P, c_uint32, _P, _P, _ERR]),
     "ff_select_blocks": (c_bool, [c_void_p, _P, c_uint32, c_uint32, _P, c_uint32, _P, c_uint32, _P, _P, c_uint32, c_uint32,
                                   c_uint32, c_uint32, _P, _P, _ERR]),
+    "ff_attention_selected": (c_bool, [c_void_p, _P, c_uint32, c_uint32, _P, c_uint32, _P, c_uint32, _P, _P, c_uint32, _P,
+                                       c_uint32, c_float, _P, c_uint32, _P, _ERR]),
     "ff_rope_table": (c_bool, [c_void_p, POINTER(FFRopeConfig), _P, c_uint32, _P, _ERR]),
     "ff_rope": (c_bool, [c_void_p, _P, c_uint32, POINTER(FFRope), _P, c_uint32, c_uint32, _P, c_uint32, _P, _ERR]),
     "ff_cache_append": (c_bool, [c_void_p, _P, c_uint32, _P, c_uint32, _P, c_uint32, POINTER(FFRope), _P, _P, c_uint32,

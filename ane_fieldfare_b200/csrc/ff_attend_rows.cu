@@ -40,6 +40,7 @@ namespace {
 constexpr int kConsumers = 4;                      // warps that compute: two a tile, 32 keys each
 constexpr int kRowsThreads = 32 * (kConsumers + 1);
 constexpr uint32_t kWaitLimit = 1u << 20;
+constexpr uint32_t kListedStarts = 512;           // requests whose first rows are kept, where rows look for theirs
 constexpr uint32_t kUnitCost = 8;                 // tiles' time that a unit takes besides its tiles
 static_assert(kTileKeys == 64 && kConsumers == 4, "two warps a tile, 32 keys each");
 
@@ -100,10 +101,18 @@ __device__ __noinline__ void wait_rows(uint32_t bar, uint32_t parity, volatile u
     *abortFlag = 1u;
 }
 
+// What a launch's "requests" are.  Listed: every row is one, its key tiles are the blocks of its list, for each key/value head another.
+enum class RowsOf { kRequest, kListed };
+
+constexpr uint32_t kNoKey = 0x7FFFFF80u;  // the first key of a tile that an entry of a list does not name; 64 more are still an int
+
 // One request as the kernel sees it.
 struct RowsRequest {
     uint32_t firstRow, rows, tilesSink, lowTile, tiles, columnTiles;
     int length, p0;  // p0: position of its first row
+};
+struct ListedRequest : RowsRequest {
+    uint32_t table;  // its row of the block table
 };
 
 // MMA row r (0..7) of eight keys: the key it stands for.  A permutation with which the eight lanes a quarter reads codes
@@ -114,8 +123,10 @@ __device__ __forceinline__ uint32_t key_of_row(uint32_t r) {
     const uint32_t t = r >> 1, odd = r & 1u;
     return DIM == 128 ? (t & 1u) | (odd << 1) | ((t & 2u) << 1) : t | (odd << 2);
 }
-template <int DIM, int NT, bool SPLIT>
+template <int DIM, int NT, bool SPLIT, RowsOf OF>
 __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_attend_rows(const __grid_constant__ CUtensorMap mapCodes, const __grid_constant__ CUtensorMap mapWords, const RowsArgs args) {
+    constexpr bool kListed = OF == RowsOf::kListed;
+    using Request = std::conditional_t<kListed, ListedRequest, RowsRequest>;
     constexpr int NG = DIM / 64, CB = DIM / 2, WB = NG * 4;
     constexpr uint32_t kStage = rows_stage_bytes(DIM), kStages = rows_stages(DIM), kColumns = SPLIT ? 4 : 8 * NT;
     static_assert(!SPLIT || NT == 1, "four columns, each twice");
@@ -127,7 +138,8 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
     __shared__ float joinBias[kConsumers][NG][kColumns];
     __shared__ uint32_t lastPart;
     __shared__ volatile uint32_t abortFlag;  // a wait was given up: nothing more is copied, what there is to multiply and join goes on
-    __shared__ RowsRequest known[kRowsThreads];
+    __shared__ Request known[kRowsThreads];
+    __shared__ uint32_t listedKey[kListed ? kStages : 1], listedStart[kListed ? kListedStarts + 1 : 1];
     const AttendArgs &a = args.a;
     const uint32_t tid = threadIdx.x, warp = (uint32_t)warp_index(), lane = tid & 31u;
     const uint32_t ring = (sm_addr(rowsSmem) + 1023u) & ~1023u;
@@ -145,8 +157,32 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
     pdl_enter();
 
     // ---- the plan: how many tiles each request is, and this CTA's run of them ----
+    const uint32_t requests = kListed ? a.tokens : a.requests;
+    auto start_of_row = [&](uint32_t r) { return kListed && a.requests <= kListedStarts ? listedStart[r] : __ldg(a.rowStart + r); };
+    if (kListed && a.requests <= kListedStarts) {
+        for (uint32_t r = tid; r <= a.requests; r += kRowsThreads) listedStart[r] = __ldg(a.rowStart + r);
+        __syncthreads();
+    }
     auto look_up = [&](uint32_t r) {
-        RowsRequest q{};
+        Request q{};
+        if constexpr (kListed) {
+            // the row's request: the last that begins at it or before
+            uint32_t low = 0, high = a.requests;
+            while (high - low > 1) {
+                const uint32_t mid = (low + high) >> 1;
+                if (start_of_row(mid) <= r) low = mid;
+                else high = mid;
+            }
+            if (a.requests == 0 || r < start_of_row(low) || r >= start_of_row(low + 1)) return q;
+            q.firstRow = r;
+            q.rows = 1;
+            q.table = low;
+            q.length = (int)min(__ldg(a.lengths + low), 0x7FFFFFFFu);
+            q.p0 = (int)max((long long)q.length - (long long)(start_of_row(low + 1) - r), -1ll);
+            q.columnTiles = (group + kColumns - 1) / kColumns;
+            q.tiles = max(1u, min(a.listed, ((uint32_t)q.p0 + kTileKeys) / kTileKeys));
+            return q;
+        }
         const uint32_t begin = min(__ldg(a.rowStart + r), a.tokens), end = min(__ldg(a.rowStart + r + 1), a.tokens);
         const uint32_t rows = end > begin ? end - begin : 0u;
         q.firstRow = begin;
@@ -167,20 +203,23 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
     // A unit costs its tiles and kUnitCost more: its queries, joins and output take as long.  (Cut by tiles alone, the CTAs with the
     // short requests of a ragged batch took 94 us where the others took 62.  kUnitCost 1, 3, 6, 8, 10, 14: ragged 90, 81, 72, 73,
     // 74, 78 us, 4 x 16 rows in a window 42, 39, 36, 35, 37, 37; 1 and 3 with CTAs of two tiles or more, the others of three.)
-    auto unit_cost = [](const RowsRequest &q) { return q.rows ? q.tiles + kUnitCost : 0u; };
-    const uint32_t run = (a.requests + kRowsThreads - 1) / kRowsThreads;
+    auto unit_cost = [](const Request &q) { return q.rows ? q.tiles + kUnitCost : 0u; };
+    const uint32_t run = (requests + kRowsThreads - 1) / kRowsThreads;
     auto request_of = [&](uint32_t r) { return run == 1 ? known[r] : look_up(r); };  // (a batch of up to 160 is looked up once)
-    const uint32_t r0 = min(tid * run, a.requests), r1 = min(r0 + run, a.requests);
+    const uint32_t r0 = min(tid * run, requests), r1 = min(r0 + run, requests);
     // rowStart goes back, to rows that several requests would write: such a call is refused like one with too much work
     auto goes_back = [&](uint32_t r) { return __ldg(a.rowStart + r + 1) < __ldg(a.rowStart + r); };
     uint32_t sum = 0;
     for (uint32_t r = r0; r < r1; ++r) {
-        const RowsRequest q = look_up(r);
+        const Request q = look_up(r);
         if (run == 1) known[r] = q;
-        if (q.rows && q.p0 + (int)q.rows > 0 && (uint32_t)(q.p0 + (int)q.rows) > a.tableKeys) *a.errorFlag = kFlagTableRow;  // (what the row has no room for is not walked)
+        if (!kListed && q.rows && q.p0 + (int)q.rows > 0 && (uint32_t)(q.p0 + (int)q.rows) > a.tableKeys) *a.errorFlag = kFlagTableRow;  // (what the row has no room for is not walked)
         sum = add_work(sum, work_of(unit_cost(q), q.columnTiles * a.kvHeads));
-        if (goes_back(r)) sum = kTooMuch;
+        if (!kListed && goes_back(r)) sum = kTooMuch;
     }
+    if (kListed)
+        for (uint32_t r = tid; r < a.requests; r += kRowsThreads)
+            if (goes_back(r)) sum = kTooMuch;
     uint32_t scan = sum;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -204,13 +243,19 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
     {
         const uint32_t covered = a.requests && !refused ? min(__ldg(a.rowStart + a.requests), a.tokens) : 0u;
         const uint32_t perRow = a.heads * DIM / 8;
+        if (kListed && covered)
+            for (uint32_t row = blockIdx.x; row < min(__ldg(a.rowStart), covered); row += gridDim.x)
+                for (uint32_t i = tid; i < perRow; i += kRowsThreads) *reinterpret_cast<uint4 *>(a.out + (size_t)row * a.outStride + i * 8) = make_uint4(0u, 0u, 0u, 0u);
         for (uint32_t row = covered + blockIdx.x; row < a.tokens; row += gridDim.x)
             for (uint32_t i = tid; i < perRow; i += kRowsThreads) *reinterpret_cast<uint4 *>(a.out + (size_t)row * a.outStride + i * 8) = make_uint4(0u, 0u, 0u, 0u);
         if (blockIdx.x == 0) {
             if (tid == 0 && refused) *a.errorFlag = kFlagWork;
             __syncthreads();
             if (tid == 0 && a.requests && __ldg(a.rowStart + a.requests) > a.tokens) *a.errorFlag = kFlagRows;
-            for (uint32_t r = r0; r < r1; ++r) {
+            if (kListed)
+                for (uint32_t r = tid; r < a.requests; r += kRowsThreads)
+                    if (goes_back(r)) *a.errorFlag = kFlagRows;
+            for (uint32_t r = r0; r < r1 && !kListed; ++r) {
                 if (goes_back(r)) *a.errorFlag = kFlagRows;
                 if (refused) continue;
                 const uint32_t begin = min(__ldg(a.rowStart + r), a.tokens), end = min(__ldg(a.rowStart + r + 1), a.tokens);
@@ -232,7 +277,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
     // this CTA's.
     struct Walk {
         uint32_t r, unit, first;
-        RowsRequest q;
+        Request q;
         uint32_t t0, count, head, column0;
     };
     auto take = [&](Walk &w) {
@@ -292,14 +337,26 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
             if (count == 0) continue;
             const int keysEnd = w.q.p0 + (int)w.q.rows;
             auto key_at = [&](uint32_t t) { return (t < w.q.tilesSink ? t : w.q.lowTile + t - w.q.tilesSink) * kTileKeys; };
+            uint32_t keyNext = kNoKey;  // listed: the first key of the lane's tile
             auto page_of = [&](uint32_t base) {
                 const uint32_t t = base + (lane >> perTileShift);
                 uint32_t page = FF_NO_PAGE;
+                if (kListed) keyNext = kNoKey;
                 if (t < t0 + count) {
-                    const uint32_t key = key_at(t) + ((lane & (pieces - 1u)) << args.pieceShift);
-                    if ((int)key < keysEnd) {
+                    uint32_t tileKey;
+                    size_t table;
+                    if constexpr (kListed) {
+                        const uint32_t id = __ldg(a.ids + ((size_t)w.r * a.kvHeads + head) * a.listed + t);
+                        tileKey = keyNext = id < kNoKey / kTileKeys ? id * kTileKeys : kNoKey;
+                        table = w.q.table;
+                    } else {
+                        tileKey = key_at(t);
+                        table = w.r;
+                    }
+                    const uint32_t key = tileKey + ((lane & (pieces - 1u)) << args.pieceShift);
+                    if ((!kListed || tileKey != kNoKey) && (int)key < keysEnd) {
                         const uint32_t index = key >> args.pageShift;
-                        if (index < a.tableStride) page = __ldg(a.blockTable + (size_t)w.r * a.tableStride + index);
+                        if (index < a.tableStride) page = __ldg(a.blockTable + table * a.tableStride + index);
                         else *a.errorFlag = kFlagTableRow;
                         if (page >= a.pageCount && index < a.tableStride) *a.errorFlag = kFlagPage;
                     }
@@ -308,7 +365,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
             };
             uint32_t pagesNext = page_of(t0);
             for (uint32_t t = t0; t < t0 + count && ok; t += tilesPer) {
-                const uint32_t pagesNow = pagesNext;
+                const uint32_t pagesNow = pagesNext, keyNow = keyNext;
                 pagesNext = page_of(t + tilesPer);
                 const uint32_t many = min(tilesPer, t0 + count - t);
                 for (uint32_t i = 0; i < many; ++i) {
@@ -316,8 +373,10 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
                     const uint32_t lives = __ballot_sync(0xFFFFFFFFu, lane < pieces && mine < a.pageCount);
                     if (!mbar_try_wait(barEmpty + 8 * stage, phase ^ 1u)) wait_rows(barEmpty + 8 * stage, phase ^ 1u, &abortFlag);
                     if (!(ok = __all_sync(0xFFFFFFFFu, abortFlag == 0u))) break;  // (a stage may still wait for its copies)
-                    const uint32_t bar = barFull + 8 * stage, base = ring + stage * kStage, inTile = key_at(t + i) & (a.page.pageTokens - 1u);
+                    const uint32_t tileKey = kListed ? __shfl_sync(0xFFFFFFFFu, keyNow, i << perTileShift) : key_at(t + i);
+                    const uint32_t bar = barFull + 8 * stage, base = ring + stage * kStage, inTile = tileKey & (a.page.pageTokens - 1u);
                     if (elect_one()) {
+                        if (kListed) listedKey[stage] = tileKey;
                         holes[stage] = ~lives;
                         bar_expect(bar, (uint32_t)__popc(lives) * (pieceCodes + pieceWords));
                     }
@@ -451,11 +510,11 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
 
         for (uint32_t i = t0 + ((n0 ^ (warp >> 1)) & 1u); i < t0 + count; i += 2) {
             const uint32_t number = n0 + i - t0, stage = number % kStages, phase = number / kStages & 1u;
-            const uint32_t tileKey = (i < w.q.tilesSink ? i : w.q.lowTile + i - w.q.tilesSink) * kTileKeys;
-            const int j0 = (int)(tileKey + warpKey);
             const uint32_t base = ring + stage * kStage;
             if (!mbar_try_wait(barFull + 8 * stage, phase)) wait_rows(barFull + 8 * stage, phase, &abortFlag);
             __syncwarp();
+            const uint32_t tileKey = kListed ? listedKey[stage] : (i < w.q.tilesSink ? i : w.q.lowTile + i - w.q.tilesSink) * kTileKeys;
+            const int j0 = (int)(tileKey + warpKey);
             const uint32_t gone = holes[stage], hole0 = gone >> (warpKey >> args.pieceShift) & 1u, hole1 = gone >> ((warpKey + 16) >> args.pieceShift) & 1u;
             // keys that not every row of the tile sees
             const bool careful = (hole0 | hole1) || j0 + 31 > pFirst || (a.window && (long long)j0 <= (long long)pLast - a.window && (uint32_t)j0 + 32u > a.sinks);
@@ -832,15 +891,15 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
     if (lane == 0 && abortFlag) *a.errorFlag = kFlagWait;
 }
 
-KernelSmemMemo rowsMemo[3][3];
+KernelSmemMemo rowsMemo[2][3][3];
 
-template <int DIM, int NT, bool SPLIT = false>
+template <RowsOf OF, int DIM, int NT, bool SPLIT = false>
 bool launch_rows(FFAttention *att, KernelSmemMemo &memo, const CUtensorMap &codes, const CUtensorMap &words, const RowsArgs &args, cudaStream_t stream, const char **error) {
     const size_t smem = rows_smem(DIM, NT);
     int perSm = 0;
-    if (!memo.prepare(k_attend_rows<DIM, NT, SPLIT>, att->device, smem, kRowsThreads, &perSm, error)) return false;
+    if (!memo.prepare(k_attend_rows<DIM, NT, SPLIT, OF>, att->device, smem, kRowsThreads, &perSm, error)) return false;
     const uint32_t grid = std::min((uint32_t)(att->smCount * std::max(1, perSm)), att->rowsCtas);
-    return launched(att, launch_pdl(k_attend_rows<DIM, NT, SPLIT>, dim3(grid), dim3(kRowsThreads), smem, stream, codes, words, args), "k_attend_rows", error);
+    return launched(att, launch_pdl(k_attend_rows<DIM, NT, SPLIT, OF>, dim3(grid), dim3(kRowsThreads), smem, stream, codes, words, args), "k_attend_rows", error);
 }
 
 }  // namespace
@@ -867,25 +926,34 @@ bool make_pages_maps(CUtensorMap *codes, CUtensorMap *words, const AttendArgs &a
 
 uint32_t attend_rows_ctas(int smCount) { return 2u * (uint32_t)smCount; }
 
-bool launch_attend_rows(FFAttention *att, const AttendArgs &a, cudaStream_t stream, const char **error) {
+template <RowsOf OF>
+static bool launch_columns(FFAttention *att, const AttendArgs &a, uint32_t columns, cudaStream_t stream, const char **error) {
     const uint32_t dim = att->cfg.headDim;
     RowsArgs args{a, att->partials, reinterpret_cast<float2 *>(att->stats), att->arrived, (uint32_t)__builtin_ctz(att->cfg.pageTokens), (uint32_t)__builtin_ctz(std::min(kTileKeys, a.page.pageTokens))};
     CUtensorMap codes, words;
     if (!make_pages_maps(&codes, &words, a, dim, 2, error)) return false;
-    const uint32_t columns = a.maxRows * (a.heads / a.kvHeads);
+    auto &memo = rowsMemo[(int)OF];
     if (dim == 256) {
-        if (columns <= 4) return launch_rows<256, 1, true>(att, rowsMemo[0][0], codes, words, args, stream, error);
-        if (columns <= 8) return launch_rows<256, 1>(att, rowsMemo[0][1], codes, words, args, stream, error);
-        return launch_rows<256, 2>(att, rowsMemo[0][2], codes, words, args, stream, error);
+        if (columns <= 4) return launch_rows<OF, 256, 1, true>(att, memo[0][0], codes, words, args, stream, error);
+        if (columns <= 8) return launch_rows<OF, 256, 1>(att, memo[0][1], codes, words, args, stream, error);
+        return launch_rows<OF, 256, 2>(att, memo[0][2], codes, words, args, stream, error);
     }
     if (dim == 128) {
-        if (columns <= 4) return launch_rows<128, 1, true>(att, rowsMemo[1][0], codes, words, args, stream, error);
-        if (columns <= 8) return launch_rows<128, 1>(att, rowsMemo[1][1], codes, words, args, stream, error);
-        return launch_rows<128, 2>(att, rowsMemo[1][2], codes, words, args, stream, error);
+        if (columns <= 4) return launch_rows<OF, 128, 1, true>(att, memo[1][0], codes, words, args, stream, error);
+        if (columns <= 8) return launch_rows<OF, 128, 1>(att, memo[1][1], codes, words, args, stream, error);
+        return launch_rows<OF, 128, 2>(att, memo[1][2], codes, words, args, stream, error);
     }
-    if (columns <= 4) return launch_rows<64, 1, true>(att, rowsMemo[2][0], codes, words, args, stream, error);
-    if (columns <= 8) return launch_rows<64, 1>(att, rowsMemo[2][1], codes, words, args, stream, error);
-    return launch_rows<64, 2>(att, rowsMemo[2][2], codes, words, args, stream, error);
+    if (columns <= 4) return launch_rows<OF, 64, 1, true>(att, memo[2][0], codes, words, args, stream, error);
+    if (columns <= 8) return launch_rows<OF, 64, 1>(att, memo[2][1], codes, words, args, stream, error);
+    return launch_rows<OF, 64, 2>(att, memo[2][2], codes, words, args, stream, error);
+}
+
+bool launch_attend_rows(FFAttention *att, const AttendArgs &a, cudaStream_t stream, const char **error) {
+    return launch_columns<RowsOf::kRequest>(att, a, a.maxRows * (a.heads / a.kvHeads), stream, error);
+}
+
+bool launch_attend_listed(FFAttention *att, const AttendArgs &a, cudaStream_t stream, const char **error) {
+    return launch_columns<RowsOf::kListed>(att, a, a.heads / a.kvHeads, stream, error);
 }
 
 }  // namespace ff

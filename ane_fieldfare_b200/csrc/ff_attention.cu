@@ -69,13 +69,17 @@ bool check_requests(const FFAttention *att, uint32_t requests, const char **erro
     return true;
 }
 
-bool check_table(const uint32_t *blockTable, uint32_t tableStride, const char **error) {
+bool check_table(const uint32_t *blockTable, uint32_t tableStride, const uint32_t *rowStart, const uint32_t *lengths, uint32_t requests, const char **error) {
+    if (!rowStart || !aligned(rowStart, 4)) return fail(error, "rows' starts (or old lengths) must be non-null and 4-byte aligned");
+    if (requests == 0) return true;
+    if (!lengths || !aligned(lengths, 4)) return fail(error, "lengths must be non-null and 4-byte aligned");
     if (!blockTable || !aligned(blockTable, 4)) return fail(error, "blockTable must be non-null and 4-byte aligned");
     if (tableStride == 0) return fail(error, "tableStride must be positive");
     return true;
 }
 
 constexpr uint32_t kSelectBlock = 64;  // keys
+constexpr uint32_t kMostListed = 1u << 20;
 
 // keys that a row of the block table has room for
 uint32_t table_keys(const FFAttentionConfig &c, uint32_t tableStride) { return (uint32_t)std::min<uint64_t>((uint64_t)tableStride * c.pageTokens, UINT32_MAX); }
@@ -287,9 +291,8 @@ bool ff_attention(FFAttention *att, const uint16_t *q, uint32_t qStride, uint32_
     if (tableStride == 0 || maxRows == 0) return fail(error, "tableStride and maxRows must be positive");
     if (!(scale > 0.0f && scale < INFINITY)) return fail(error, "scale must be positive and finite");
     if (sinks && !window) return fail(error, "sinks need a window");
-    AttendArgs a{q, out, qStride, outStride, tokens, static_cast<const uint8_t *>(pages), pageCount, tableStride,
-                 (uint32_t)std::min<uint64_t>((uint64_t)tableStride * c.pageTokens, UINT32_MAX), blockTable, rowStart, lengths, requests,
-                 std::min(maxRows, std::max(1u, tokens)), scale, window, sinks, c.heads, c.kvHeads, page_layout(c), att->errorFlag};
+    AttendArgs a{q, out, qStride, outStride, tokens, static_cast<const uint8_t *>(pages), pageCount, tableStride, table_keys(c, tableStride), blockTable, rowStart, lengths, requests,
+                 std::min(maxRows, std::max(1u, tokens)), scale, window, sinks, c.heads, c.kvHeads, page_layout(c), att->errorFlag, nullptr, 0};
     return launch_attend(att, a, static_cast<cudaStream_t>(stream), error);
 }
 
@@ -299,10 +302,8 @@ bool ff_block_means(FFAttention *att, const void *pages, uint32_t pageCount, con
     const FFAttentionConfig &c = att->cfg;
     if (!check_requests(att, requests, error)) return false;
     if (requests == 0) return true;
-    if (!check_cache(att, pages, pageCount, error) || !check_table(blockTable, tableStride, error)) return false;
-    if (!oldLengths || !newLengths || !means) return fail(error, "null argument");
-    if (!aligned(oldLengths, 4) || !aligned(newLengths, 4)) return fail(error, "arrays must be 4-byte aligned");
-    if (!aligned(means, 16)) return fail(error, "means must be 16-byte aligned");
+    if (!check_cache(att, pages, pageCount, error) || !check_table(blockTable, tableStride, oldLengths, newLengths, requests, error)) return false;
+    if (!means || !aligned(means, 16)) return fail(error, "means must be non-null and 16-byte aligned");
     return launch_block_means(att, static_cast<const uint8_t *>(pages), pageCount, blockTable, tableStride, table_keys(c, tableStride), oldLengths, newLengths,
                               requests, means, static_cast<cudaStream_t>(stream), error);
 }
@@ -312,21 +313,38 @@ bool ff_select_blocks(FFAttention *att, const uint16_t *q, uint32_t qStride, uin
                       uint32_t blocks, uint32_t first, uint32_t last, uint32_t *ids, void *stream, const char **error) {
     if (!begin(att, error)) return false;
     const FFAttentionConfig &c = att->cfg;
-    if (blocks == 0 || blocks > (1u << 20)) return fail(error, "need 1..2^20 blocks a list");
+    if (blocks == 0 || blocks > kMostListed) return fail(error, "need 1..2^20 blocks a list");
     if (last == 0) return fail(error, "a row's own block is always in its list: last must be positive");
     if (first > blocks || last > blocks - first) return fail(error, "the first and the last blocks are more than a list holds");
     if (tokens == 0) return true;
     if (!check_tokens(att, tokens, error) || !check_heads(att, q, qStride, c.heads, "query", error) || !check_requests(att, requests, error) ||
-        !check_table(blockTable, tableStride, error))
+        !check_table(blockTable, tableStride, rowStart, lengths, requests, error))
         return false;
-    if (!means || !rowStart || !lengths || !ids) return fail(error, "null argument");
-    if (!aligned(means, 16)) return fail(error, "means must be 16-byte aligned");
-    if (!aligned(rowStart, 4) || !aligned(lengths, 4) || !aligned(ids, 4)) return fail(error, "arrays must be 4-byte aligned");
+    if (!means || !aligned(means, 16)) return fail(error, "means must be non-null and 16-byte aligned");
+    if (!ids || !aligned(ids, 4)) return fail(error, "ids must be non-null and 4-byte aligned");
     if ((uint64_t)pageCount * c.pageTokens >= FF_NO_SLOT) return fail(error, "the cache has more slots than 32 bits name");
     const uint64_t keys = (uint64_t)tableStride * c.pageTokens;
     if (keys > 1u << 21) return fail(error, "block table rows of more than 2^21 keys: their scores do not fit a CTA");
     return launch_select_blocks(att, q, qStride, tokens, means, pageCount, blockTable, tableStride, (uint32_t)((keys + kSelectBlock - 1) / kSelectBlock), rowStart,
                                 lengths, requests, blocks, first, last, ids, static_cast<cudaStream_t>(stream), error);
+}
+
+bool ff_attention_selected(FFAttention *att, const uint16_t *q, uint32_t qStride, uint32_t tokens, const void *pages, uint32_t pageCount,
+                           const uint32_t *blockTable, uint32_t tableStride, const uint32_t *rowStart, const uint32_t *lengths, uint32_t requests,
+                           const uint32_t *ids, uint32_t blocks, float scale, uint16_t *out, uint32_t outStride, void *stream, const char **error) {
+    if (!begin(att, error)) return false;
+    const FFAttentionConfig &c = att->cfg;
+    if (blocks == 0 || blocks > kMostListed) return fail(error, "need 1..2^20 blocks a list");
+    if (!(scale > 0.0f && scale < INFINITY)) return fail(error, "scale must be positive and finite");
+    if (tokens == 0) return true;
+    if (!check_tokens(att, tokens, error) || !check_heads(att, q, qStride, c.heads, "query", error) ||
+        !check_heads(att, out, outStride, c.heads, "output", error) || !check_cache(att, pages, pageCount, error) ||
+        !check_requests(att, requests, error) || !check_table(blockTable, tableStride, rowStart, lengths, requests, error))
+        return false;
+    if (!ids || !aligned(ids, 4)) return fail(error, "ids must be non-null and 4-byte aligned");
+    AttendArgs a{q, out, qStride, outStride, tokens, static_cast<const uint8_t *>(pages), pageCount, tableStride, table_keys(c, tableStride), blockTable,
+                 rowStart, lengths, requests, 1, scale, 0, 0, c.heads, c.kvHeads, page_layout(c), att->errorFlag, ids, blocks};
+    return launch_attend_listed(att, a, static_cast<cudaStream_t>(stream), error);
 }
 
 }  // extern "C"

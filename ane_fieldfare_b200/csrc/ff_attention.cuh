@@ -75,6 +75,8 @@ struct AttendArgs {
     uint32_t heads, kvHeads;
     PageLayout page;
     uint32_t *errorFlag;
+    const uint32_t *ids;  // lists of blocks [tokens][kvHeads][listed], or null
+    uint32_t listed;
 };
 
 // ff_cache.cu
@@ -105,6 +107,7 @@ bool launch_select_blocks(FFAttention *att, const uint16_t *q, uint32_t qStride,
 // ff_attend_rows.cu
 uint32_t attend_rows_ctas(int smCount);
 bool launch_attend_rows(FFAttention *att, const AttendArgs &args, cudaStream_t stream, const char **error);
+bool launch_attend_listed(FFAttention *att, const AttendArgs &args, cudaStream_t stream, const char **error);
 
 // ff_attend_tiles.cu
 bool launch_attend_tiles(FFAttention *att, const AttendArgs &args, cudaStream_t stream, const char **error);

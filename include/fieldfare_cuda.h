@@ -608,6 +608,16 @@ bool ff_select_blocks(FFAttention *attention, const uint16_t *q, uint32_t qStrid
                       const uint32_t *lengths, uint32_t requests, uint32_t blocks, uint32_t first, uint32_t last,
                       uint32_t *ids, void *stream, const char **error);
 
+/* ff_attention over listed blocks: a row at position p, for key/value head g, sees the keys j <= p of the blocks that its list names, ids uint32
+ * [tokens][kvHeads][blocks].  Of a list the first p / 64 + 1 entries count (the row sees no more blocks), in any order; a block that is
+ * named twice counts twice, an entry that is no block with a key of the row's (FF_NO_SLOT) not at all.  A row that sees no key, and rows of
+ * no request, are zero.  The keys of a row are its own, so that many rows of one request read a block as often as they name it: from some hundred
+ * rows on ff_attention over all keys is the shorter way.  Otherwise as ff_attention with up to 16 columns. */
+bool ff_attention_selected(FFAttention *attention, const uint16_t *q, uint32_t qStride, uint32_t tokens, const void *pages,
+                           uint32_t pageCount, const uint32_t *blockTable, uint32_t tableStride, const uint32_t *rowStart,
+                           const uint32_t *lengths, uint32_t requests, const uint32_t *ids, uint32_t blocks, float scale,
+                           uint16_t *out, uint32_t outStride, void *stream, const char **error);
+
 /* Device-side result of the last ff_moe_prefill permute, copied to the host after a sync:
  * the expert-sorted pairs and per-expert row offsets [experts+1].  For parity tests. */
 bool ff_last_prefill_routes(FFContext *ctx, FFTokenExpertPair *sortedPairs, uint32_t *offsets,
