@@ -241,6 +241,28 @@ class AttentionContext:
              *self._heads(out, self.heads, tokens, "out"), _stream(stream))
         return out
 
+    def attendShared(self, q: torch.Tensor, pages: torch.Tensor, blockTable: torch.Tensor, rowStart: torch.Tensor,
+                     lengths: torch.Tensor, maxRows: int, groupStart: torch.Tensor, prefixLengths: torch.Tensor, *,
+                     scale: Optional[float] = None, out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+        """`attend` without a window, where requests groupStart[g] .. groupStart[g + 1] - 1 hold the same first prefixLengths[g]
+        keys on the same pages: these are read once for all rows of the group."""
+        tokens, requests, groups, shape = q.shape[0], lengths.numel(), prefixLengths.numel(), blockTable.shape
+        if rowStart.numel() != requests + 1 or len(shape) != 2 or shape[0] != requests:
+            raise ValueError("lengths, blockTable and rowStart must agree on the number of requests")
+        if groupStart.numel() != groups + 1:
+            raise ValueError("groupStart must have one entry more than prefixLengths")
+        if maxRows < 0:
+            raise ValueError("maxRows must not be negative")
+        if out is None:
+            out = self._new((tokens, self.heads, self.headDim), torch.bfloat16, stream)
+        self._ints("blockTable rowStart lengths groupStart prefixLengths", blockTable, rowStart, lengths, groupStart, prefixLengths)
+        workspace = self._new((16 + 4 * tokens * self.heads * (self.headDim + 2) + 8,), torch.uint8, stream)
+        call("ff_attention_shared", self.handle, *self._heads(q, self.heads, tokens, "q"), tokens, *self._cache(pages), blockTable.data_ptr(), shape[1],
+             rowStart.data_ptr(), lengths.data_ptr(), requests, min(maxRows, _WORD), groupStart.data_ptr(), prefixLengths.data_ptr(), groups,
+             self.headDim ** -0.5 if scale is None else scale, workspace.data_ptr(), *self._heads(out, self.heads, tokens, "out"),
+             _stream(stream))
+        return out
+
     # -- a part of a long context ------------------------------------------------------------------
 
     def newMeans(self, pages: int) -> torch.Tensor:

@@ -102,7 +102,9 @@ __device__ __noinline__ void wait_rows(uint32_t bar, uint32_t parity, volatile u
 }
 
 // What a launch's "requests" are.  Listed: every row is one, its key tiles are the blocks of its list, for each key/value head another.
-enum class RowsOf { kRequest, kListed };
+// Prefix: the groups of requests that share a prefix, whose rows all see its keys; results go to args.a.shared, not yet out.  Suffix: requests
+// from behind their group's prefix on, what the prefix gave joined to it.
+enum class RowsOf { kRequest, kListed, kPrefix, kSuffix };
 
 constexpr uint32_t kNoKey = 0x7FFFFF80u;  // the first key of a tile that an entry of a list does not name; 64 more are still an int
 
@@ -112,7 +114,7 @@ struct RowsRequest {
     int length, p0;  // p0: position of its first row
 };
 struct ListedRequest : RowsRequest {
-    uint32_t table;  // its row of the block table
+    uint32_t table;  // its row of the block table; suffix: whether the rows have a prefix
 };
 
 // MMA row r (0..7) of eight keys: the key it stands for.  A permutation with which the eight lanes a quarter reads codes
@@ -125,8 +127,8 @@ __device__ __forceinline__ uint32_t key_of_row(uint32_t r) {
 }
 template <int DIM, int NT, bool SPLIT, RowsOf OF>
 __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_attend_rows(const __grid_constant__ CUtensorMap mapCodes, const __grid_constant__ CUtensorMap mapWords, const RowsArgs args) {
-    constexpr bool kListed = OF == RowsOf::kListed;
-    using Request = std::conditional_t<kListed, ListedRequest, RowsRequest>;
+    constexpr bool kListed = OF == RowsOf::kListed, kPrefix = OF == RowsOf::kPrefix, kSuffix = OF == RowsOf::kSuffix;
+    using Request = std::conditional_t<OF == RowsOf::kRequest, RowsRequest, ListedRequest>;
     constexpr int NG = DIM / 64, CB = DIM / 2, WB = NG * 4;
     constexpr uint32_t kStage = rows_stage_bytes(DIM), kStages = rows_stages(DIM), kColumns = SPLIT ? 4 : 8 * NT;
     static_assert(!SPLIT || NT == 1, "four columns, each twice");
@@ -157,7 +159,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
     pdl_enter();
 
     // ---- the plan: how many tiles each request is, and this CTA's run of them ----
-    const uint32_t requests = kListed ? a.tokens : a.requests;
+    const uint32_t requests = kListed ? a.tokens : kPrefix ? a.shared.groups : a.requests;
     auto start_of_row = [&](uint32_t r) { return kListed && a.requests <= kListedStarts ? listedStart[r] : __ldg(a.rowStart + r); };
     if (kListed && a.requests <= kListedStarts) {
         for (uint32_t r = tid; r <= a.requests; r += kRowsThreads) listedStart[r] = __ldg(a.rowStart + r);
@@ -183,6 +185,17 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
             q.tiles = max(1u, min(a.listed, ((uint32_t)q.p0 + kTileKeys) / kTileKeys));
             return q;
         }
+        if constexpr (kPrefix) {
+            const SharedGroup g = shared_group(a, r);
+            q.firstRow = g.firstRow;
+            q.rows = g.keys ? g.rows : 0u;
+            q.table = g.request;
+            q.length = (int)g.keys;
+            q.p0 = q.length - 1;  // (every row sees every key)
+            q.columnTiles = (q.rows * group + kColumns - 1) / kColumns;
+            q.tiles = g.keys / kTileKeys;
+            return q;
+        }
         const uint32_t begin = min(__ldg(a.rowStart + r), a.tokens), end = min(__ldg(a.rowStart + r + 1), a.tokens);
         const uint32_t rows = end > begin ? end - begin : 0u;
         q.firstRow = begin;
@@ -190,12 +203,17 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
         q.p0 = q.length - (int)rows;
         q.rows = min(rows, a.maxRows);
         if (q.rows == 0) return q;
+        const uint32_t prefix = kSuffix ? shared_keys(a, r, q.p0) : 0u;
         q.columnTiles = (q.rows * group + kColumns - 1) / kColumns;
         const uint32_t last = (uint32_t)max(0, q.p0 + (int)q.rows), ends = (min(last, a.tableKeys) + kTileKeys - 1) / kTileKeys;
         if (a.window) {
             const uint32_t low = (uint32_t)max((long long)0, (long long)q.p0 - (long long)a.window + 1);
             q.lowTile = min(low / kTileKeys, ends);
             q.tilesSink = min((uint32_t)(((unsigned long long)a.sinks + kTileKeys - 1) / kTileKeys), q.lowTile);
+        }
+        if constexpr (kSuffix) {
+            q.table = prefix != 0u;
+            q.lowTile = prefix / kTileKeys;
         }
         q.tiles = max(1u, q.tilesSink + ends - q.lowTile);  // (a request without keys: one tile that nobody sees)
         return q;
@@ -208,18 +226,22 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
     auto request_of = [&](uint32_t r) { return run == 1 ? known[r] : look_up(r); };  // (a batch of up to 160 is looked up once)
     const uint32_t r0 = min(tid * run, requests), r1 = min(r0 + run, requests);
     // rowStart goes back, to rows that several requests would write: such a call is refused like one with too much work
-    auto goes_back = [&](uint32_t r) { return __ldg(a.rowStart + r + 1) < __ldg(a.rowStart + r); };
+    auto goes_back = [&](uint32_t r) {
+        if constexpr (kPrefix) return __ldg(a.shared.groupStart + r + 1) < __ldg(a.shared.groupStart + r);
+        return __ldg(a.rowStart + r + 1) < __ldg(a.rowStart + r);
+    };
     uint32_t sum = 0;
     for (uint32_t r = r0; r < r1; ++r) {
         const Request q = look_up(r);
         if (run == 1) known[r] = q;
-        if (!kListed && q.rows && q.p0 + (int)q.rows > 0 && (uint32_t)(q.p0 + (int)q.rows) > a.tableKeys) *a.errorFlag = kFlagTableRow;  // (what the row has no room for is not walked)
+        if (!kListed && !kPrefix && q.rows && q.p0 + (int)q.rows > 0 && (uint32_t)(q.p0 + (int)q.rows) > a.tableKeys) *a.errorFlag = kFlagTableRow;  // (what the row has no room for is not walked)
         sum = add_work(sum, work_of(unit_cost(q), q.columnTiles * a.kvHeads));
         if (!kListed && goes_back(r)) sum = kTooMuch;
     }
     if (kListed)
         for (uint32_t r = tid; r < a.requests; r += kRowsThreads)
             if (goes_back(r)) sum = kTooMuch;
+    if ((kPrefix || kSuffix) && shared_refused<kSuffix>(a, tid, kRowsThreads)) sum = kTooMuch;
     uint32_t scan = sum;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -239,11 +261,14 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
     if (tid == 0) first[kRowsThreads] = total;
     __syncthreads();
 
+    if constexpr (kPrefix) {
+        if (blockIdx.x == 0 && tid == 0) *a.shared.refused = refused;
+    }
     // rows that no unit writes: behind the last request's, and past maxRows
-    {
+    if constexpr (!kPrefix) {
         const uint32_t covered = a.requests && !refused ? min(__ldg(a.rowStart + a.requests), a.tokens) : 0u;
         const uint32_t perRow = a.heads * DIM / 8;
-        if (kListed && covered)
+        if (OF != RowsOf::kRequest && covered)
             for (uint32_t row = blockIdx.x; row < min(__ldg(a.rowStart), covered); row += gridDim.x)
                 for (uint32_t i = tid; i < perRow; i += kRowsThreads) *reinterpret_cast<uint4 *>(a.out + (size_t)row * a.outStride + i * 8) = make_uint4(0u, 0u, 0u, 0u);
         for (uint32_t row = covered + blockIdx.x; row < a.tokens; row += gridDim.x)
@@ -252,6 +277,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
             if (tid == 0 && refused) *a.errorFlag = kFlagWork;
             __syncthreads();
             if (tid == 0 && a.requests && __ldg(a.rowStart + a.requests) > a.tokens) *a.errorFlag = kFlagRows;
+            if (kSuffix && shared_refused<false>(a, tid, kRowsThreads)) *a.errorFlag = kFlagRows;
             if (kListed)
                 for (uint32_t r = tid; r < a.requests; r += kRowsThreads)
                     if (goes_back(r)) *a.errorFlag = kFlagRows;
@@ -352,6 +378,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
                     } else {
                         tileKey = key_at(t);
                         table = w.r;
+                        if constexpr (kPrefix) table = w.q.table;
                     }
                     const uint32_t key = tileKey + ((lane & (pieces - 1u)) << args.pieceShift);
                     if ((!kListed || tileKey != kNoKey) && (int)key < keysEnd) {
@@ -783,9 +810,25 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
         const uint32_t used = min(kColumns, columns - column0);
         const bool whole = count == unitTiles;
         const uint32_t slot = 2 * cta + (t0 == 0 ? 1u : 0u);
-        auto write = [&](uint32_t column, uint32_t at, const float4 &v, float weights) {
-            const float f = weights == 0.0f ? 0.0f : 1.0f / weights;
+        auto write = [&](uint32_t column, uint32_t at, float4 v, float weights, float level) {
+            float f = weights == 0.0f ? 0.0f : 1.0f / weights;
             const uint32_t global = column0 + column;
+            if constexpr (kPrefix || kSuffix) {
+                const size_t place = (size_t)(w.q.firstRow + global / group) * a.heads + head * group + global % group;
+                float4 *part = reinterpret_cast<float4 *>(a.shared.values + place * DIM + at);
+                if constexpr (kPrefix) {
+                    *part = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+                    if (at == 0) a.shared.stats[place] = make_float2(level, weights);
+                    return;
+                } else if (w.q.table) {
+                    const float2 st = __ldcg(a.shared.stats + place);
+                    const float4 u = __ldcg(part);
+                    const float most = fmaxf(level, st.x), mine = exp2_fast(level - most), other = st.y * exp2_fast(st.x - most);
+                    const float all = fmaf(weights, mine, other);
+                    f = all == 0.0f ? 0.0f : 1.0f / all;
+                    v = make_float4(fmaf(v.x, mine, u.x * other), fmaf(v.y, mine, u.y * other), fmaf(v.z, mine, u.z * other), fmaf(v.w, mine, u.w * other));
+                }
+            }
             uint16_t *to = a.out + (size_t)(w.q.firstRow + global / group) * a.outStride + (head * group + global % group) * DIM + at;
             *reinterpret_cast<uint2 *>(to) = make_uint2(pack_bf16x2(v.x * f, v.y * f), pack_bf16x2(v.z * f, v.w * f));
         };
@@ -800,7 +843,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
             for (int k = 0; k < kConsumers; ++k) weights += joinStats[k][column].y * exp2_fast(joinStats[k][column].x - all);
             const float4 sum4 = make_float4(u.x + v.x, u.y + v.y, u.z + v.z, u.w + v.w);
             if (whole) {
-                write(column, at, sum4, weights);
+                write(column, at, sum4, weights, all);
             } else {
                 *reinterpret_cast<float4 *>(args.partials + ((size_t)slot * kColumns + column) * DIM + at) = sum4;
                 if (at == 0) args.stats[slot * kColumns + column] = make_float2(all, weights);
@@ -858,7 +901,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
                         }
                     }
                     if (last) {
-                        write(column, at, sum4, weights);
+                        write(column, at, sum4, weights, all);
                     } else {
                         *reinterpret_cast<float4 *>(args.partials + ((size_t)slot_of(from) * kColumns + column) * DIM + at) = sum4;
                         if (at == 0) joinStats[0][column] = make_float2(all, weights);
@@ -891,7 +934,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
     if (lane == 0 && abortFlag) *a.errorFlag = kFlagWait;
 }
 
-KernelSmemMemo rowsMemo[2][3][3];
+KernelSmemMemo rowsMemo[4][3][3];
 
 template <RowsOf OF, int DIM, int NT, bool SPLIT = false>
 bool launch_rows(FFAttention *att, KernelSmemMemo &memo, const CUtensorMap &codes, const CUtensorMap &words, const RowsArgs &args, cudaStream_t stream, const char **error) {
@@ -954,6 +997,14 @@ bool launch_attend_rows(FFAttention *att, const AttendArgs &a, cudaStream_t stre
 
 bool launch_attend_listed(FFAttention *att, const AttendArgs &a, cudaStream_t stream, const char **error) {
     return launch_columns<RowsOf::kListed>(att, a, a.heads / a.kvHeads, stream, error);
+}
+
+bool launch_attend_prefix_rows(FFAttention *att, const AttendArgs &a, cudaStream_t stream, const char **error) {
+    return launch_columns<RowsOf::kPrefix>(att, a, a.tokens * (a.heads / a.kvHeads), stream, error);
+}
+
+bool launch_attend_suffix_rows(FFAttention *att, const AttendArgs &a, cudaStream_t stream, const char **error) {
+    return launch_columns<RowsOf::kSuffix>(att, a, a.maxRows * (a.heads / a.kvHeads), stream, error);
 }
 
 }  // namespace ff

@@ -155,15 +155,25 @@ __device__ __forceinline__ unsigned long long spread_bits(uint32_t v) {
     return (x | x << 1) & 0x5555555555555555ull;
 }
 
+// What a launch's "requests" are.  Prefix: the groups of requests that share a prefix, whose rows all see its keys; results go to
+// args.a.shared, not yet out.  Suffix: requests from behind their group's prefix on, what the prefix gave joined to it.
+enum class TilesOf { kRequest, kPrefix, kSuffix };
+
 // A row tile of a request as the kernel sees it.
 struct RowTileOf {
     uint32_t r, firstRow, tokens;          // its request, first row of q, tokens
     int p0;                                // position of its first token
     uint32_t tilesSink, lowTile, tiles;    // key tiles: the first tilesSink, then from lowTile on
 };
+struct SharedTileOf : RowTileOf {
+    bool joins;  // suffix: whether the rows have a prefix
+};
 
-template <int DIM>
+template <int DIM, TilesOf OF>
 __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_constant__ CUtensorMap mapCodes, const __grid_constant__ CUtensorMap mapWords, const TilesArgs args) {
+    constexpr bool kPrefix = OF == TilesOf::kPrefix, kSuffix = OF == TilesOf::kSuffix;
+    using RowTile = std::conditional_t<OF == TilesOf::kRequest, RowTileOf, SharedTileOf>;
+    using Known = std::conditional_t<OF == TilesOf::kRequest, uint3, uint4>;  // first row, rows, length; prefix: its request; suffix: its prefix's keys
     constexpr int NG = DIM / 64, CB = DIM / 2, WB = NG * 4;
     constexpr uint32_t kSlot = slot_bytes(DIM), kPack = packed_bytes(DIM);
     constexpr uint32_t kWordSide = words_bytes(DIM) / 2, kUnits = kTileKeys * NG;  // of a slot: a key's group of 64 values
@@ -177,7 +187,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
     __shared__ uint32_t firstTile[kTilesThreads + 1], firstWork[kTilesThreads + 1], warpSums[32];
     __shared__ uint32_t holes[kPacked], hidden[kInfo][2];
     __shared__ float4 tileInfo[kInfo];
-    __shared__ uint3 known[kTilesThreads];
+    __shared__ Known known[kTilesThreads];
     __shared__ float topShared[kRows], sumShared[kRowGroups][kRows], refShared[kRowGroups][kRows];
     __shared__ uint32_t largestShared[kRowGroups][kRows];
     const AttendArgs &a = args.a;
@@ -226,27 +236,45 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
 
     // ---- the plan: row tiles of the requests, key tiles of those, this CTA's run ----
     // A request: its first row, rows, length; looked up once where there is a thread for each.
-    const uint32_t run = (a.requests + kTilesThreads - 1) / kTilesThreads;
+    const uint32_t requests = kPrefix ? a.shared.groups : a.requests, run = (requests + kTilesThreads - 1) / kTilesThreads;
     auto look_up = [&](uint32_t r) {
-        const uint32_t begin = min(__ldg(a.rowStart + r), a.tokens), end = min(__ldg(a.rowStart + r + 1), a.tokens);
-        return make_uint3(begin, end > begin ? end - begin : 0u, min(__ldg(a.lengths + r), 0x7FFFFFFFu));
+        if constexpr (kPrefix) {
+            const SharedGroup g = shared_group(a, r);
+            return make_uint4(g.firstRow, g.keys ? g.rows : 0u, g.keys, g.request);
+        } else {
+            const uint32_t begin = min(__ldg(a.rowStart + r), a.tokens), end = min(__ldg(a.rowStart + r + 1), a.tokens);
+            const uint32_t rows = end > begin ? end - begin : 0u, length = min(__ldg(a.lengths + r), 0x7FFFFFFFu);
+            if constexpr (kSuffix) return make_uint4(begin, rows, length, rows ? shared_keys(a, r, (int)length - (int)rows) : 0u);
+            else return make_uint3(begin, rows, length);
+        }
     };
     auto request = [&](uint32_t r) { return run == 1 ? known[r] : look_up(r); };
     auto row_tiles_of = [&](uint32_t r) { return (min(request(r).y, a.maxRows) + args.tileTokens - 1) / args.tileTokens; };
     auto row_tile = [&](uint32_t r, uint32_t i) {
-        RowTileOf q;
-        const uint3 of = request(r);
+        RowTile q;
+        const Known of = request(r);
         const uint32_t used = min(of.y, a.maxRows);
         q.r = r;
         q.firstRow = of.x + i * args.tileTokens;
         q.tokens = min(args.tileTokens, used - i * args.tileTokens);
         q.p0 = (int)of.z - (int)of.y + (int)(i * args.tileTokens);
+        if constexpr (kPrefix) {
+            q.r = of.w;
+            q.p0 = (int)of.z - 1;  // (every row sees every key)
+            q.lowTile = q.tilesSink = 0;
+            q.tiles = of.z / kTileKeys;
+            return q;
+        }
         const uint32_t last = (uint32_t)max(0, q.p0 + (int)q.tokens), ends = (min(last, a.tableKeys) + kTileKeys - 1) / kTileKeys;
         q.lowTile = q.tilesSink = 0;
         if (a.window) {
             const uint32_t low = (uint32_t)max((long long)0, (long long)q.p0 - (long long)a.window + 1);
             q.lowTile = min(low / kTileKeys, ends);
             q.tilesSink = min((uint32_t)(((unsigned long long)a.sinks + kTileKeys - 1) / kTileKeys), q.lowTile);
+        }
+        if constexpr (kSuffix) {
+            q.joins = of.w != 0u;
+            q.lowTile = of.w / kTileKeys;
         }
         q.tiles = max(1u, q.tilesSink + ends - q.lowTile);  // (rows without keys: one tile that nobody sees)
         return q;
@@ -282,16 +310,20 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
         }
         return low;
     };
-    const uint32_t r0 = min(tid * run, a.requests), r1 = min(r0 + run, a.requests);
+    const uint32_t r0 = min(tid * run, requests), r1 = min(r0 + run, requests);
     // rowStart goes back, to rows that several requests would write: such a call is refused like one with too much work
-    auto goes_back = [&](uint32_t r) { return __ldg(a.rowStart + r + 1) < __ldg(a.rowStart + r); };
+    auto goes_back = [&](uint32_t r) {
+        if constexpr (kPrefix) return false;  // (shared_refused looks)
+        else return __ldg(a.rowStart + r + 1) < __ldg(a.rowStart + r);
+    };
     uint32_t mineTiles = 0;
     for (uint32_t r = r0; r < r1; ++r) {
-        const uint3 of = look_up(r);
+        const Known of = look_up(r);
         if (run == 1) known[r] = of;
         mineTiles = goes_back(r) ? kTooMuch : add_work(mineTiles, (min(of.y, a.maxRows) + args.tileTokens - 1) / args.tileTokens);
-        if (of.y && (int)of.z - (int)of.y + (int)min(of.y, a.maxRows) > 0 && of.z - of.y + min(of.y, a.maxRows) > a.tableKeys) *a.errorFlag = kFlagTableRow;  // (what the row has no room for is not walked)
+        if (!kPrefix && of.y && (int)of.z - (int)of.y + (int)min(of.y, a.maxRows) > 0 && of.z - of.y + min(of.y, a.maxRows) > a.tableKeys) *a.errorFlag = kFlagTableRow;  // (what the row has no room for is not walked)
     }
+    if ((kPrefix || kSuffix) && shared_refused<kSuffix>(a, tid, kTilesThreads)) mineTiles = kTooMuch;
     const uint32_t allTiles = block_scan(mineTiles, firstTile);
     const uint32_t rowTiles = allTiles == kTooMuch ? 0u : allTiles;
     // the n-th row tile
@@ -332,15 +364,22 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
     const bool refused = allTiles == kTooMuch || allWork == kTooMuch;  // (the places of units are nothing then)
     const uint32_t total = refused ? 0u : allWork;
 
+    if constexpr (kPrefix) {
+        if (blockIdx.x == 0 && tid == 0) *a.shared.refused = refused;
+    }
     // rows that no unit writes: behind the last request's, and past maxRows
-    {
+    if constexpr (!kPrefix) {
         const uint32_t covered = a.requests && !refused ? min(__ldg(a.rowStart + a.requests), a.tokens) : 0u;
         const uint32_t perRow = a.heads * DIM / 8;
+        if (kSuffix && covered)
+            for (uint32_t row = blockIdx.x; row < min(__ldg(a.rowStart), covered); row += gridDim.x)
+                for (uint32_t i = tid; i < perRow; i += kTilesThreads) *reinterpret_cast<uint4 *>(a.out + (size_t)row * a.outStride + i * 8) = make_uint4(0u, 0u, 0u, 0u);
         for (uint32_t row = covered + blockIdx.x; row < a.tokens; row += gridDim.x)
             for (uint32_t i = tid; i < perRow; i += kTilesThreads) *reinterpret_cast<uint4 *>(a.out + (size_t)row * a.outStride + i * 8) = make_uint4(0u, 0u, 0u, 0u);
         if (blockIdx.x == 0) {
             if (tid == 0 && refused) *a.errorFlag = kFlagWork;
             __syncthreads();
+            if (kSuffix && shared_refused<false>(a, tid, kTilesThreads)) *a.errorFlag = kFlagRows;
             if (tid == 0 && a.requests && __ldg(a.rowStart + a.requests) > a.tokens) *a.errorFlag = kFlagRows;
             for (uint32_t r = r0; r < r1; ++r) {
                 if (goes_back(r)) *a.errorFlag = kFlagRows;
@@ -362,7 +401,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
     // tiles and kUnitCost more: its queries, first logits and output take as long.
     struct Walk {
         Place place;
-        RowTileOf q;
+        RowTile q;
         uint32_t first, head, t0, count;  // segment [t0, t0 + count)
     };
     auto take = [&](Walk &w) {
@@ -402,7 +441,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
         take(w);
         return w.count != 0 || next_segment(w);
     };
-    auto key_at = [&](const RowTileOf &q, uint32_t t) { return (t < q.tilesSink ? t : q.lowTile + t - q.tilesSink) * kTileKeys; };
+    auto key_at = [&](const RowTile &q, uint32_t t) { return (t < q.tilesSink ? t : q.lowTile + t - q.tilesSink) * kTileKeys; };
     const uint32_t pieceKeys = 1u << args.pieceShift, pieces = kTileKeys >> args.pieceShift;
 
     if (warp < (uint32_t)kFirstRowWarp) {
@@ -848,11 +887,42 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                 sum = sumShared[0][row] * exp2_fast(refShared[0][row] - largest) + sumShared[1][row] * exp2_fast(refShared[1][row] - largest);
                 const bool whole = w.count == w.q.tiles;
                 const uint32_t part = 2 * cta + (w.t0 == 0 ? 1u : 0u);
-                const float factor = sum == 0.0f ? 0.0f : exp2_fast(top - largest) / sum;  // (-108 .. 120, of the values' powers)
+                float factor = sum == 0.0f ? 0.0f : exp2_fast(top - largest) / sum;  // (-108 .. 120, of the values' powers)
+                // a row's place among those of the prefix, and the first of its values there
+                auto shared_place = [&](uint32_t token, uint32_t h) { return (size_t)(w.q.firstRow + token) * a.heads + w.head * group + h; };
+                // what the prefix gives the row's result, and what the row's own part keeps; the sums there are of the weights themselves
+                constexpr float kUnweight = 1.0f / (1u << (int)kWeightScale);
+                auto join_prefix = [&](size_t place, float level, float weights, float &keep) {
+                    weights *= kUnweight;
+                    const float2 st = __ldcg(a.shared.stats + place);
+                    const float most = fmaxf(level, st.x), mine = exp2_fast(level - most), other = st.y * exp2_fast(st.x - most), all = fmaf(weights, mine, other);
+                    keep = weights == 0.0f || all == 0.0f ? 0.0f : weights * mine / all;
+                    return all == 0.0f ? 0.0f : other / all;
+                };
+                float given = 0.0f;
+                if constexpr (kPrefix) {
+                    if (whole && there && wg == 0) a.shared.stats[shared_place(token, row % group)] = make_float2(largest, sum * kUnweight);
+                }
+                if constexpr (kSuffix) {
+                    if (whole && there && w.q.joins) {
+                        float keep;
+                        given = join_prefix(shared_place(token, row % group), largest, sum, keep);
+                        factor *= keep;
+                    }
+                }
                 if (whole) {
                     // four lanes 64 bytes of a row
                     float factors[4];
                     uint16_t *to[4];
+                    [[maybe_unused]] float gives[4];
+                    [[maybe_unused]] float *shared[4];
+                    if constexpr (kPrefix || kSuffix) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            gives[k] = __shfl_sync(0xFFFFFFFFu, given, 8 * k + (lane >> 2));
+                            shared[k] = a.shared.values + shared_place(mineRows[k] >> 16, mineRows[k] & 0xFFFFu) * DIM + 8 * (lane & 3u);
+                        }
+                    }
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         factors[k] = __shfl_sync(0xFFFFFFFFu, factor, 8 * k + (lane >> 2));
@@ -868,8 +938,22 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                         for (int k = 0; k < 4; ++k) {
                             const uint32_t *u = o[k >> 1] + 2 * (k & 1);  // u[4 j], u[4 j + 1]: values j and j + 4 of the lane's run
                             auto at = [&](int n) { return __uint_as_float(u[4 * (n & 3) + (n >> 2)]) * factors[k]; };
-                            if ((mineRows[k] >> 16) < w.q.tokens)
+                            if ((mineRows[k] >> 16) < w.q.tokens) {
+                                if constexpr (kPrefix) {
+                                    *reinterpret_cast<float4 *>(shared[k] + c) = make_float4(at(0), at(1), at(2), at(3));
+                                    *reinterpret_cast<float4 *>(shared[k] + c + 4) = make_float4(at(4), at(5), at(6), at(7));
+                                    continue;
+                                } else if constexpr (kSuffix) {
+                                    if (w.q.joins) {
+                                        const float4 x = __ldcg(reinterpret_cast<const float4 *>(shared[k] + c)), y = __ldcg(reinterpret_cast<const float4 *>(shared[k] + c + 4));
+                                        const float g = gives[k];
+                                        *reinterpret_cast<uint4 *>(to[k] + c) = make_uint4(pack_bf16x2(fmaf(x.x, g, at(0)), fmaf(x.y, g, at(1))), pack_bf16x2(fmaf(x.z, g, at(2)), fmaf(x.w, g, at(3))),
+                                                                                           pack_bf16x2(fmaf(y.x, g, at(4)), fmaf(y.y, g, at(5))), pack_bf16x2(fmaf(y.z, g, at(6)), fmaf(y.w, g, at(7))));
+                                        continue;
+                                    }
+                                }
                                 *reinterpret_cast<uint4 *>(to[k] + c) = make_uint4(pack_bf16x2(at(0), at(1)), pack_bf16x2(at(2), at(3)), pack_bf16x2(at(4), at(5)), pack_bf16x2(at(6), at(7)));
+                            }
                         }
                     }
                 } else {
@@ -946,7 +1030,33 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                                 }
                             }
                             if (last) {
-                                const float f = weights == 0.0f ? 0.0f : exp2_fast(all - level) / weights;
+                                float f = weights == 0.0f ? 0.0f : exp2_fast(all - level) / weights;
+                                if constexpr (kPrefix || kSuffix) {
+                                    const size_t place = shared_place(mine / group, mine % group);
+                                    float *values = a.shared.values + place * DIM + d;
+                                    if constexpr (kPrefix) {
+                                        if (d == 0) a.shared.stats[place] = make_float2(level, weights * kUnweight);
+#pragma unroll
+                                        for (uint32_t k = 0; k < 4; ++k) {
+                                            *reinterpret_cast<float4 *>(values + 8 * k) = make_float4(v[2 * k] * f, v[8 + 2 * k] * f, v[16 + 2 * k] * f, v[24 + 2 * k] * f);
+                                            *reinterpret_cast<float4 *>(values + 8 * k + 4) = make_float4(v[2 * k + 1] * f, v[9 + 2 * k] * f, v[17 + 2 * k] * f, v[25 + 2 * k] * f);
+                                        }
+                                        continue;
+                                    } else if (w.q.joins) {
+                                        float keep;
+                                        const float g = join_prefix(place, level, weights, keep);
+                                        f *= keep;
+#pragma unroll
+                                        for (uint32_t k = 0; k < 4; ++k) {
+                                            const float4 x = __ldcg(reinterpret_cast<const float4 *>(values + 8 * k)), y = __ldcg(reinterpret_cast<const float4 *>(values + 8 * k + 4));
+                                            v[2 * k] = fmaf(v[2 * k], f, x.x * g), v[8 + 2 * k] = fmaf(v[8 + 2 * k], f, x.y * g);
+                                            v[16 + 2 * k] = fmaf(v[16 + 2 * k], f, x.z * g), v[24 + 2 * k] = fmaf(v[24 + 2 * k], f, x.w * g);
+                                            v[2 * k + 1] = fmaf(v[2 * k + 1], f, y.x * g), v[9 + 2 * k] = fmaf(v[9 + 2 * k], f, y.y * g);
+                                            v[17 + 2 * k] = fmaf(v[17 + 2 * k], f, y.z * g), v[25 + 2 * k] = fmaf(v[25 + 2 * k], f, y.w * g);
+                                        }
+                                        f = 1.0f;
+                                    }
+                                }
                                 uint16_t *to = a.out + (size_t)(w.q.firstRow + mine / group) * a.outStride + (w.head * group + mine % group) * DIM + d;
 #pragma unroll
                                 for (uint32_t k = 0; k < 4; ++k)  // value n of run k: column 8 (n % 4) + 2 k + n / 4
@@ -990,24 +1100,30 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
     if (warp == (uint32_t)kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
-KernelSmemMemo tilesMemo[3];
+KernelSmemMemo tilesMemo[3][3];
 
-template <int DIM>
+template <TilesOf OF, int DIM>
 bool launch_tiles(FFAttention *att, KernelSmemMemo &memo, const CUtensorMap &codes, const CUtensorMap &words, const TilesArgs &args, cudaStream_t stream, const char **error) {
-    if (!memo.prepare(k_attend_tiles<DIM>, att->device, tiles_smem(DIM), kTilesThreads, nullptr, error)) return false;
-    return launched(att, launch_pdl(k_attend_tiles<DIM>, dim3(att->smCount), dim3(kTilesThreads), tiles_smem(DIM), stream, codes, words, args), "k_attend_tiles", error);
+    if (!memo.prepare(k_attend_tiles<DIM, OF>, att->device, tiles_smem(DIM), kTilesThreads, nullptr, error)) return false;
+    return launched(att, launch_pdl(k_attend_tiles<DIM, OF>, dim3(att->smCount), dim3(kTilesThreads), tiles_smem(DIM), stream, codes, words, args), "k_attend_tiles", error);
 }
 
 }  // namespace
 
-bool launch_attend_tiles(FFAttention *att, const AttendArgs &a, cudaStream_t stream, const char **error) {
+template <TilesOf OF>
+static bool launch_tiles_of(FFAttention *att, const AttendArgs &a, cudaStream_t stream, const char **error) {
     const uint32_t dim = att->cfg.headDim;
     TilesArgs args{a, att->partials, att->stats, att->arrived, (uint32_t)__builtin_ctz(att->cfg.pageTokens), (uint32_t)__builtin_ctz(std::min(kTileKeys, a.page.pageTokens)), kRows / (a.heads / a.kvHeads)};
     CUtensorMap codes, words;
     if (!make_pages_maps(&codes, &words, a, dim, 1, error)) return false;
-    if (dim == 256) return launch_tiles<256>(att, tilesMemo[2], codes, words, args, stream, error);
-    if (dim == 128) return launch_tiles<128>(att, tilesMemo[1], codes, words, args, stream, error);
-    return launch_tiles<64>(att, tilesMemo[0], codes, words, args, stream, error);
+    auto &memo = tilesMemo[(int)OF];
+    if (dim == 256) return launch_tiles<OF, 256>(att, memo[2], codes, words, args, stream, error);
+    if (dim == 128) return launch_tiles<OF, 128>(att, memo[1], codes, words, args, stream, error);
+    return launch_tiles<OF, 64>(att, memo[0], codes, words, args, stream, error);
 }
+
+bool launch_attend_tiles(FFAttention *att, const AttendArgs &a, cudaStream_t stream, const char **error) { return launch_tiles_of<TilesOf::kRequest>(att, a, stream, error); }
+bool launch_attend_prefix_tiles(FFAttention *att, const AttendArgs &a, cudaStream_t stream, const char **error) { return launch_tiles_of<TilesOf::kPrefix>(att, a, stream, error); }
+bool launch_attend_suffix_tiles(FFAttention *att, const AttendArgs &a, cudaStream_t stream, const char **error) { return launch_tiles_of<TilesOf::kSuffix>(att, a, stream, error); }
 
 }  // namespace ff

@@ -16,6 +16,17 @@ bool launch_attend(FFAttention *att, const AttendArgs &a, cudaStream_t stream, c
     return launch_attend_tiles(att, a, stream, error);
 }
 
+// Two launches: the groups' rows over their prefixes, then the requests' rows from behind them.  Each goes to the kernel that its columns
+// ask for, as above; those of a group are all its rows' (bounded by the rows of the call).
+bool launch_attend_shared(FFAttention *att, AttendArgs a, cudaStream_t stream, const char **error) {
+    const uint64_t group = a.heads / a.kvHeads;
+    const uint32_t maxRows = a.maxRows;
+    a.maxRows = a.tokens;
+    if (!(a.tokens * group <= 16 ? launch_attend_prefix_rows(att, a, stream, error) : launch_attend_prefix_tiles(att, a, stream, error))) return false;
+    a.maxRows = maxRows;
+    return maxRows * group <= 16 ? launch_attend_suffix_rows(att, a, stream, error) : launch_attend_suffix_tiles(att, a, stream, error);
+}
+
 }  // namespace ff
 
 using namespace ff;
@@ -80,6 +91,18 @@ bool check_table(const uint32_t *blockTable, uint32_t tableStride, const uint32_
 
 constexpr uint32_t kSelectBlock = 64;  // keys
 constexpr uint32_t kMostListed = 1u << 20;
+
+// The workspace of ff_attention_shared: a word, the rows' maxima and sums, their values.
+struct SharedLayout {
+    uint64_t stats, values, bytes;
+};
+SharedLayout shared_layout(const FFAttentionConfig &c, uint32_t tokens) {
+    const uint64_t rows = (uint64_t)tokens * c.heads;
+    SharedLayout l{16, 0, 0};
+    l.values = (l.stats + rows * sizeof(float2) + 15) / 16 * 16;
+    l.bytes = l.values + rows * c.headDim * sizeof(float);
+    return l;
+}
 
 // keys that a row of the block table has room for
 uint32_t table_keys(const FFAttentionConfig &c, uint32_t tableStride) { return (uint32_t)std::min<uint64_t>((uint64_t)tableStride * c.pageTokens, UINT32_MAX); }
@@ -292,7 +315,7 @@ bool ff_attention(FFAttention *att, const uint16_t *q, uint32_t qStride, uint32_
     if (!(scale > 0.0f && scale < INFINITY)) return fail(error, "scale must be positive and finite");
     if (sinks && !window) return fail(error, "sinks need a window");
     AttendArgs a{q, out, qStride, outStride, tokens, static_cast<const uint8_t *>(pages), pageCount, tableStride, table_keys(c, tableStride), blockTable, rowStart, lengths, requests,
-                 std::min(maxRows, std::max(1u, tokens)), scale, window, sinks, c.heads, c.kvHeads, page_layout(c), att->errorFlag, nullptr, 0};
+                 std::min(maxRows, std::max(1u, tokens)), scale, window, sinks, c.heads, c.kvHeads, page_layout(c), att->errorFlag, nullptr, 0, {}};
     return launch_attend(att, a, static_cast<cudaStream_t>(stream), error);
 }
 
@@ -343,8 +366,37 @@ bool ff_attention_selected(FFAttention *att, const uint16_t *q, uint32_t qStride
         return false;
     if (!ids || !aligned(ids, 4)) return fail(error, "ids must be non-null and 4-byte aligned");
     AttendArgs a{q, out, qStride, outStride, tokens, static_cast<const uint8_t *>(pages), pageCount, tableStride, table_keys(c, tableStride), blockTable,
-                 rowStart, lengths, requests, 1, scale, 0, 0, c.heads, c.kvHeads, page_layout(c), att->errorFlag, ids, blocks};
+                 rowStart, lengths, requests, 1, scale, 0, 0, c.heads, c.kvHeads, page_layout(c), att->errorFlag, ids, blocks, {}};
     return launch_attend_listed(att, a, static_cast<cudaStream_t>(stream), error);
+}
+
+uint64_t ff_attention_shared_bytes(const FFAttentionConfig *config, uint32_t tokens) {
+    return config && supported(*config, nullptr) ? shared_layout(*config, tokens).bytes : 0;
+}
+
+bool ff_attention_shared(FFAttention *att, const uint16_t *q, uint32_t qStride, uint32_t tokens, const void *pages, uint32_t pageCount,
+                         const uint32_t *blockTable, uint32_t tableStride, const uint32_t *rowStart, const uint32_t *lengths, uint32_t requests,
+                         uint32_t maxRows, const uint32_t *groupStart, const uint32_t *prefixLengths, uint32_t groups, float scale, void *workspace,
+                         uint16_t *out, uint32_t outStride, void *stream, const char **error) {
+    if (!begin(att, error)) return false;
+    const FFAttentionConfig &c = att->cfg;
+    if (!(scale > 0.0f && scale < INFINITY)) return fail(error, "scale must be positive and finite");
+    if (maxRows == 0) return fail(error, "maxRows must be positive");
+    if (tokens == 0) return true;
+    if (!check_tokens(att, tokens, error) || !check_heads(att, q, qStride, c.heads, "query", error) ||
+        !check_heads(att, out, outStride, c.heads, "output", error) || !check_cache(att, pages, pageCount, error) ||
+        !check_requests(att, requests, error) || !check_table(blockTable, tableStride, rowStart, lengths, requests, error))
+        return false;
+    if (groups > requests) return fail(error, "more groups than requests");
+    if (groups && (!groupStart || !prefixLengths || !aligned(groupStart, 4) || !aligned(prefixLengths, 4)))
+        return fail(error, "groupStart and prefixLengths must be non-null and 4-byte aligned");
+    if (!workspace || !aligned(workspace, 16)) return fail(error, "workspace must be non-null and 16-byte aligned");
+    const SharedLayout l = shared_layout(c, tokens);
+    uint8_t *w = static_cast<uint8_t *>(workspace);
+    AttendArgs a{q, out, qStride, outStride, tokens, static_cast<const uint8_t *>(pages), pageCount, tableStride, table_keys(c, tableStride), blockTable,
+                 rowStart, lengths, requests, std::min(maxRows, tokens), scale, 0, 0, c.heads, c.kvHeads, page_layout(c), att->errorFlag, nullptr, 0,
+                 {groupStart, prefixLengths, groups, reinterpret_cast<uint32_t *>(w), reinterpret_cast<float2 *>(w + l.stats), reinterpret_cast<float *>(w + l.values)}};
+    return launch_attend_shared(att, a, static_cast<cudaStream_t>(stream), error);
 }
 
 }  // extern "C"

@@ -62,6 +62,15 @@ inline bool launched(FFAttention *att, cudaError_t status, const char *what, con
     return true;
 }
 
+// Requests that share a prefix, and what the rows' attention over it gives the launch behind (device memory of the caller's).
+struct SharedPrefix {
+    const uint32_t *groupStart, *prefixLengths;
+    uint32_t groups;
+    uint32_t *refused;  // whether the prefix launch wrote nothing
+    float2 *stats;      // [tokens][heads] largest logit (log2), the weights' sum at it
+    float *values;      // [tokens][heads][headDim] their mean of the values
+};
+
 struct AttendArgs {
     const uint16_t *q;
     uint16_t *out;
@@ -77,6 +86,7 @@ struct AttendArgs {
     uint32_t *errorFlag;
     const uint32_t *ids;  // lists of blocks [tokens][kvHeads][listed], or null
     uint32_t listed;
+    SharedPrefix shared;
 };
 
 // ff_cache.cu
@@ -108,11 +118,16 @@ bool launch_select_blocks(FFAttention *att, const uint16_t *q, uint32_t qStride,
 uint32_t attend_rows_ctas(int smCount);
 bool launch_attend_rows(FFAttention *att, const AttendArgs &args, cudaStream_t stream, const char **error);
 bool launch_attend_listed(FFAttention *att, const AttendArgs &args, cudaStream_t stream, const char **error);
+bool launch_attend_prefix_rows(FFAttention *att, const AttendArgs &args, cudaStream_t stream, const char **error);
+bool launch_attend_suffix_rows(FFAttention *att, const AttendArgs &args, cudaStream_t stream, const char **error);
 
 // ff_attend_tiles.cu
 bool launch_attend_tiles(FFAttention *att, const AttendArgs &args, cudaStream_t stream, const char **error);
+bool launch_attend_prefix_tiles(FFAttention *att, const AttendArgs &args, cudaStream_t stream, const char **error);
+bool launch_attend_suffix_tiles(FFAttention *att, const AttendArgs &args, cudaStream_t stream, const char **error);
 
 // ff_attention.cu
 bool launch_attend(FFAttention *att, const AttendArgs &args, cudaStream_t stream, const char **error);
+bool launch_attend_shared(FFAttention *att, AttendArgs args, cudaStream_t stream, const char **error);
 
 }  // namespace ff

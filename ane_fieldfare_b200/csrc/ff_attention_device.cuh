@@ -89,6 +89,48 @@ constexpr uint32_t kTooMuch = 0xFFFFFFFFu;
 __device__ __forceinline__ uint32_t add_work(uint32_t a, uint32_t b) { return a + b < a ? kTooMuch : a + b; }
 __device__ __forceinline__ uint32_t work_of(uint32_t tiles, uint32_t units) { return __umulhi(tiles, units) ? kTooMuch : tiles * units; }
 
+// A group of requests that share a prefix: its rows, its first request, and the keys of the prefix in whole tiles (the others are
+// walked with the requests' own).
+struct SharedGroup {
+    uint32_t firstRow, rows, request, keys;
+};
+__device__ __forceinline__ uint32_t prefix_keys(const AttendArgs &a, uint32_t g, uint32_t first) {  // no longer than its first request
+    return min(min(__ldg(a.shared.prefixLengths + g), a.tableKeys), min(__ldg(a.lengths + first), 0x7FFFFFFFu)) / kTileKeys * kTileKeys;
+}
+__device__ __forceinline__ SharedGroup shared_group(const AttendArgs &a, uint32_t g) {
+    const uint32_t first = min(__ldg(a.shared.groupStart + g), a.requests), last = min(__ldg(a.shared.groupStart + g + 1), a.requests);
+    SharedGroup s{0u, 0u, first, 0u};
+    if (first >= last) return s;
+    const uint32_t begin = min(__ldg(a.rowStart + first), a.tokens), end = min(__ldg(a.rowStart + last), a.tokens);
+    s.firstRow = begin;
+    s.rows = end > begin ? end - begin : 0u;
+    s.keys = prefix_keys(a, g, first);
+    return s;
+}
+// The keys of request r's prefix, as its rows from position p0 on take them from the group's launch: none where the first of them does not
+// see them all (the request then walks all of its keys by itself), or where r is in no group.
+__device__ __forceinline__ uint32_t shared_keys(const AttendArgs &a, uint32_t r, int p0) {
+    uint32_t low = 0, high = a.shared.groups;
+    while (high - low > 1) {
+        const uint32_t mid = (low + high) >> 1;
+        if (__ldg(a.shared.groupStart + mid) <= r) low = mid;
+        else high = mid;
+    }
+    if (a.shared.groups == 0) return 0u;
+    const uint32_t first = __ldg(a.shared.groupStart + low);
+    if (r < first || r >= __ldg(a.shared.groupStart + low + 1)) return 0u;
+    const uint32_t keys = prefix_keys(a, low, first);
+    return p0 >= 0 && (uint32_t)p0 + 1u >= keys ? keys : 0u;
+}
+// Whether the thread's share of the groups goes back, or of the row starts (groups' rows could overlap then); behind the prefix launch (kSaid): or that wrote nothing.
+template <bool kSaid>
+__device__ __forceinline__ bool shared_refused(const AttendArgs &a, uint32_t thread, uint32_t threads) {
+    bool back = kSaid && __ldcg(a.shared.refused) != 0u;
+    for (uint32_t g = thread; g < a.shared.groups; g += threads) back |= __ldg(a.shared.groupStart + g + 1) < __ldg(a.shared.groupStart + g);
+    for (uint32_t r = thread; r < a.requests; r += threads) back |= __ldg(a.rowStart + r + 1) < __ldg(a.rowStart + r);
+    return back;
+}
+
 // The cache's pages as tensors: codes [blocks][keys, values][tokens][bytes], a box the part of a tile that lies on one page, of
 // `sides` of the two; scale words [blocks][keys, values][words], a box both sides of such a part.
 bool make_pages_maps(CUtensorMap *codes, CUtensorMap *words, const AttendArgs &a, uint32_t dim, uint32_t sides, const char **error);
