@@ -164,13 +164,17 @@ __global__ void __launch_bounds__(kMeansThreads) k_block_means(const __grid_cons
 
 // ---- selection -----------------------------------------------------------------------------------
 
-// A CTA takes `rows` neighbouring rows of one key/value head.  Scores: the blocks' means times the rows' queries, 16 blocks a
-// warp at a time on mma.sync.  Both factors are whole numbers of at most 7 bits times a power of two of their own (the means as they are
-// held, the queries as they are staged), so that every sum is below 2^23 of its unit and exact in whatever order; the largest of a
-// row's heads is the score.  Then the bound that as many scores reach as are wanted, by halving the range of scores as whole
-// numbers, until the number that reaches it is the number wanted or the range is one score, of which the first blocks are taken.
-constexpr int kSelectThreads = 512, kSelectWarps = kSelectThreads / 32;
-constexpr uint32_t kSelectRows = 8;  // rows of a CTA, at most: the columns of a product
+// Scores: the blocks' means times the rows' queries, 16 blocks a warp at a time on mma.sync.  Both factors are whole numbers of at
+// most 7 bits times a power of two of their own (the means as they are held, the queries as they are staged), so that every sum is below 2^23 of
+// its unit and exact in whatever order; the largest of a row's heads is the score.  Then the bound that as many scores reach as are
+// wanted, two bits of it at a time, until the number that reaches it is the number wanted or all bits are known: of the scores at the
+// bound the first are taken.
+//
+// Two forms.  k_select_split: a cluster of CTAs for each row and head, which share the blocks; the first of them gets the others' scores and
+// makes the list.  k_select_rows: some neighbouring rows a CTA, which read the means of their request once; a warp makes a list.
+constexpr int kSelectThreads = 256, kSelectWarps = kSelectThreads / 32;
+constexpr uint32_t kSelectColumns = 64;  // of a CTA's product, at most
+constexpr uint32_t kMostSplit = 8;       // CTAs of a cluster, at most
 
 struct SelectArgs {
     const uint16_t *q;
@@ -183,7 +187,7 @@ struct SelectArgs {
     uint32_t requests, heads, kvHeads, pageShift;
     uint32_t blocks, first, last;
     uint32_t *ids;
-    uint32_t rows, rowColumns;  // of a CTA; columns of a row: the heads of its group, to a power of two or a multiple of 8
+    uint32_t rows, rowColumns, columns;  // of a CTA; columns of a row: the heads of its group, to a power of two or a multiple of 8
     uint32_t *errorFlag;
 };
 
@@ -201,26 +205,35 @@ __device__ __forceinline__ uint32_t order_of(float score) {
 __host__ __device__ constexpr uint32_t select_query_stride(uint32_t dim) { return 2u * dim + 64u; }  // bytes; 64 modulo 128: no conflicts
 inline uint32_t select_smem(uint32_t dim, uint32_t columns, uint32_t rows, uint32_t tableBlocks) { return columns * select_query_stride(dim) + rows * tableBlocks * 4u; }
 
+// What a CTA knows of its rows.
+struct SelectRows {
+    uint32_t request[kSelectWarps], seen[kSelectWarps];  // of each row; blocks that it sees
+    int exponents[kSelectColumns];                       // of a column's largest value; kNoNumber: it has a value that is not finite
+    static constexpr int kNoNumber = -1000;
+};
+// the query of column c, or null: a row's columns are its heads, the last of them again in what is left
 template <int DIM>
-__global__ void __launch_bounds__(kSelectThreads) k_select_blocks(const __grid_constant__ SelectArgs a) {
-    constexpr uint32_t kStride = select_query_stride(DIM), kChunks = DIM / 32;
-    extern __shared__ __align__(16) uint8_t selectSmem[];
-    __shared__ int exponents[64];
-    __shared__ uint32_t requestOf[kSelectRows], seenBlocks[kSelectRows], counts[2][kSelectWarps], greater[kSelectWarps], equal[kSelectWarps];
-    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5, g = lane >> 2, t = lane & 3u;
-    const uint32_t head = blockIdx.y, row0 = blockIdx.x * a.rows, rows = min(a.rows, a.tokens - row0), group = a.heads / a.kvHeads;
-    const uint32_t columns = (a.rows * a.rowColumns + 7u) & ~7u;
-    uint32_t *scores = reinterpret_cast<uint32_t *>(selectSmem + columns * kStride);  // [rows][tableBlocks]
-    if (tid < kSelectRows) requestOf[tid] = FF_NO_SLOT, seenBlocks[tid] = 0u;
-    pdl_enter();
-    __syncthreads();
-
-    // ---- the rows' requests and the blocks that they see ----
+__device__ __forceinline__ const uint16_t *select_column(const SelectArgs &a, uint32_t row0, uint32_t rows, uint32_t head, uint32_t c) {
+    const uint32_t i = c / a.rowColumns, group = a.heads / a.kvHeads;
+    return i < rows ? a.q + (size_t)(row0 + i) * a.qStride + (size_t)(head * group + min(c % a.rowColumns, group - 1u)) * DIM : nullptr;
+}
+// Requests and blocks of the rows, and the columns' exponents; a barrier in front, which s.request and s.seen are cleared before, and one behind.
+template <int DIM>
+__device__ __forceinline__ void select_look_up(const SelectArgs &a, SelectRows &s, uint32_t row0, uint32_t rows, uint32_t head) {
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+    for (uint32_t c = warp; c < a.columns; c += kSelectWarps) {
+        const uint16_t *src = select_column<DIM>(a, row0, rows, head, c);
+        uint32_t most = 0;
+#pragma unroll
+        for (uint32_t d = 2 * lane; d < DIM; d += 64)
+            if (src) most = __vmaxu2(most, __ldg(reinterpret_cast<const uint32_t *>(src + d)) & 0x7FFF7FFFu);
+        most = __reduce_max_sync(0xFFFFFFFFu, max(most & 0xFFFFu, most >> 16)) >> 7;
+        if (lane == 0) s.exponents[c] = most == 255u ? SelectRows::kNoNumber : max((int)most - 127, -100);
+    }
     for (uint32_t r = tid; r < a.requests; r += kSelectThreads) {
-        const uint32_t begin = __ldg(a.rowStart + r), end = __ldg(a.rowStart + r + 1);
-        if (end < begin && blockIdx.x == 0) *a.errorFlag = kFlagRows;
+        const uint32_t begin = __ldg(a.rowStart + r), end = __ldg(a.rowStart + r + 1), length = min(__ldg(a.lengths + r), 0x7FFFFFFFu);
+        if (end < begin) *a.errorFlag = kFlagRows;
         if (end <= row0 || begin >= row0 + rows || end <= begin) continue;
-        const uint32_t length = min(__ldg(a.lengths + r), 0x7FFFFFFFu);
         for (uint32_t i = 0; i < rows; ++i) {
             const uint32_t row = row0 + i;
             if (row < begin || row >= end) continue;
@@ -230,175 +243,250 @@ __global__ void __launch_bounds__(kSelectThreads) k_select_blocks(const __grid_c
                 seen = a.tableBlocks;
                 *a.errorFlag = kFlagTableRow;
             }
-            requestOf[i] = r;
-            seenBlocks[i] = seen;
+            s.request[i] = r;
+            s.seen[i] = seen;
         }
     }
-    __syncthreads();
-    const uint32_t wanted = a.blocks - a.first - a.last;
-    bool any = false;  // whether some row has more blocks than it takes
-#pragma unroll 1
-    for (uint32_t i = 0; i < rows; ++i) any |= seenBlocks[i] > a.blocks;
-
-    if (any && wanted) {
-        // ---- queries: whole numbers of at most 7 bits, at a power of two of the head's largest value ----
-        // (exponent of a column's largest value, then of its row's largest)
-        for (uint32_t c = warp; c < columns; c += kSelectWarps) {
-            const uint32_t i = c / a.rowColumns, h = min(c % a.rowColumns, group - 1u);
-            uint32_t most = 0;
-            if (i < rows) {
-                const uint16_t *src = a.q + (size_t)(row0 + i) * a.qStride + (head * group + h) * DIM;
+}
+// The columns as they are multiplied: whole numbers of at most 7 bits at the exponents, times a power of two that a row's columns share.
+template <int DIM>
+__device__ __forceinline__ void select_stage(const SelectArgs &a, const SelectRows &s, uint32_t row0, uint32_t rows, uint32_t head, uint8_t *to) {
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
+    for (uint32_t c = warp; c < a.columns; c += kSelectWarps) {
+        const uint16_t *src = select_column<DIM>(a, row0, rows, head, c);
+        const uint32_t c0 = c / a.rowColumns * a.rowColumns;
+        int top = -100;
+        for (uint32_t k = lane; k < a.rowColumns; k += 32)
+            if (c0 + k < a.columns) top = max(top, s.exponents[c0 + k]);
+        top = __reduce_max_sync(0xFFFFFFFFu, top);
+        const int mine = s.exponents[c], e = max(mine, top - 60);
+        if (mine == SelectRows::kNoNumber) src = nullptr;  // (counts as zeros)
+        const float down = power_of_two(6 - e), up = power_of_two(e - top);
 #pragma unroll
-                for (uint32_t d = 2 * lane; d < DIM; d += 64) most = __vmaxu2(most, __ldg(reinterpret_cast<const uint32_t *>(src + d)) & 0x7FFF7FFFu);
-            }
-            most = __reduce_max_sync(0xFFFFFFFFu, max(most & 0xFFFFu, most >> 16)) >> 7;
-            if (lane == 0 && c % a.rowColumns < 64u) exponents[c % 64u] = most == 255u ? -1000 : max((int)most - 127, -100);
+        for (uint32_t d = 2 * lane; d < DIM; d += 64) {
+            const uint32_t v = src ? __ldg(reinterpret_cast<const uint32_t *>(src + d)) : 0u;
+            const float x = fminf(fmaxf(rintf(low16(v) * down), -127.0f), 127.0f) * up, y = fminf(fmaxf(rintf(high16(v) * down), -127.0f), 127.0f) * up;
+            *reinterpret_cast<uint32_t *>(to + c * select_query_stride(DIM) + 2 * d) = pack_bf16x2(x, y);
         }
-        __syncthreads();
-        for (uint32_t c = warp; c < columns; c += kSelectWarps) {
-            const uint32_t i = c / a.rowColumns, h = min(c % a.rowColumns, group - 1u);
-            int top = -100;
-            for (uint32_t k = 0; k < a.rowColumns; ++k) top = max(top, exponents[(i * a.rowColumns + k) % 64u]);
-            const int mine = exponents[c % 64u];
-            const bool none = i >= rows || mine == -1000;  // (a head with a value that is no number counts as zeros)
-            const int e = max(mine, top - 60);
-            const float down = power_of_two(6 - e), up = power_of_two(e - top);
-            const uint16_t *src = a.q + (size_t)(row0 + (none ? 0u : i)) * a.qStride + (head * group + h) * DIM;
+    }
+}
+// Scores of request r's blocks below `end`, in whole numbers of their order, to store(row of the CTA, block, score): sixteen at a time from
+// 16 tile on, 16 step apart.
+template <int DIM, typename Store>
+__device__ __forceinline__ void select_score(const SelectArgs &a, const uint8_t *queries, uint32_t head, uint32_t r, uint32_t end, uint32_t tile, uint32_t step, Store store) {
+    constexpr uint32_t kChunks = DIM / 32;
+    const uint32_t lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u, perPage = max(1u, (1u << a.pageShift) >> kBlockShift);
+    auto page_of = [&](uint32_t base) {  // of the mean of block base + lane % 16
+        const uint32_t b = base + (lane & 15u);
+        return b < end ? __ldg(a.blockTable + (size_t)r * a.tableStride + (((b << kBlockShift) + kTileKeys - 1u) >> a.pageShift)) : 0u;
+    };
+    uint32_t pageNext = page_of(16 * tile);
+    for (uint32_t base = 16 * tile; base < end; base += 16 * step) {
+        const uint32_t page = pageNext;
+        const bool outside = page >= a.pageCount;
+        uint4 v[2][kChunks];
 #pragma unroll
-            for (uint32_t d = 2 * lane; d < DIM; d += 64) {
-                const uint32_t v = none ? 0u : __ldg(reinterpret_cast<const uint32_t *>(src + d));
-                const float x = fminf(fmaxf(rintf(low16(v) * down), -127.0f), 127.0f) * up, y = fminf(fmaxf(rintf(high16(v) * down), -127.0f), 127.0f) * up;
-                *reinterpret_cast<uint32_t *>(selectSmem + c * kStride + 2 * d) = pack_bf16x2(x, y);
-            }
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t b = base + g + 8 * h, mine = __shfl_sync(0xFFFFFFFFu, outside ? 0u : page, g + 8 * h);
+            const uint4 *src = reinterpret_cast<const uint4 *>(a.means + (((size_t)mine * a.kvHeads + head) * perPage + (b & (perPage - 1u))) * DIM) + t;
+#pragma unroll
+            for (uint32_t c = 0; c < kChunks; ++c) v[h][c] = a.pageCount ? __ldg(src + 4 * c) : make_uint4(0u, 0u, 0u, 0u);
         }
-        __syncthreads();
-
-        // ---- scores, request by request ----
-        const uint32_t perPage = max(1u, (1u << a.pageShift) >> kBlockShift);
-        for (uint32_t i0 = 0, i1; i0 < rows; i0 = i1) {
-            uint32_t end = 0;  // blocks that a row of the request may choose
-            for (i1 = i0; i1 < rows && requestOf[i1] == requestOf[i0]; ++i1)
-                if (seenBlocks[i1] > a.blocks) end = max(end, seenBlocks[i1] - a.last);
-            const uint32_t r = requestOf[i0];
-            if (r == FF_NO_SLOT || end == 0) continue;
-            auto page_of = [&](uint32_t base) {  // of the mean of block base + lane, lane < 16
-                const uint32_t b = base + (lane & 15u);
-                return b < end ? __ldg(a.blockTable + (size_t)r * a.tableStride + (((b << kBlockShift) + kTileKeys - 1u) >> a.pageShift)) : FF_NO_PAGE;
-            };
-            uint32_t pageNext = page_of(16 * warp);
-            for (uint32_t base = 16 * warp; base < end; base += 16 * kSelectWarps) {
-                const uint32_t page = pageNext;
-                uint4 v[2][kChunks];
+        pageNext = page_of(base + 16 * step);
+        const uint32_t gone = __ballot_sync(0xFFFFFFFFu, outside);
+        if (gone && lane == 0) *a.errorFlag = kFlagPage;
+        float best[4];  // [block g: column 2 t, 2 t + 1; block g + 8: likewise] of the columns so far that are the row's
+        for (uint32_t n = 0; n < a.columns; n += 8) {
+            float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const uint32_t b = base + g + 8 * h, mine = __shfl_sync(0xFFFFFFFFu, page, g + 8 * h);
-                    const uint16_t *src = a.means + (((size_t)mine * a.kvHeads + head) * perPage + (b & (perPage - 1u))) * DIM + 8 * t;
+            for (uint32_t c = 0; c < kChunks; ++c) {
+                const uint4 b = *reinterpret_cast<const uint4 *>(queries + (n + g) * select_query_stride(DIM) + 64 * c + 16 * t);
+                mma_bf16(acc, v[0][c].x, v[1][c].x, v[0][c].y, v[1][c].y, b.x, b.y);
+                mma_bf16(acc, v[0][c].z, v[1][c].z, v[0][c].w, v[1][c].w, b.z, b.w);
+            }
+            const bool begins = a.rowColumns <= 8 || n % a.rowColumns == 0;
 #pragma unroll
-                    for (uint32_t c = 0; c < kChunks; ++c) v[h][c] = mine < a.pageCount ? __ldg(reinterpret_cast<const uint4 *>(src + 32 * c)) : make_uint4(0u, 0u, 0u, 0u);
+            for (int k = 0; k < 4; ++k) best[k] = begins || acc[k] != acc[k] ? acc[k] : fmaxf(best[k], acc[k]);  // (a NaN mean makes all columns NaN)
+            if (a.rowColumns > 8 && (n + 8) % a.rowColumns) continue;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t b = base + g + 8 * h, width = min(a.rowColumns, 8u);
+                uint32_t k0 = order_of(best[2 * h]), k1 = order_of(best[2 * h + 1]);
+                if (gone >> (g + 8 * h) & 1u) k0 = k1 = 0u;
+                if (width > 1) k0 = max(k0, k1);
+                if (width > 2) k0 = max(k0, __shfl_xor_sync(0xFFFFFFFFu, k0, 1));
+                if (width > 4) k0 = max(k0, __shfl_xor_sync(0xFFFFFFFFu, k0, 2));
+                if (b < end && (2 * t) % width == 0u) {
+                    store((n + 2 * t) / a.rowColumns, b, k0);
+                    if (width == 1) store(n + 2 * t + 1, b, k1);
                 }
-                pageNext = page_of(base + 16 * kSelectWarps);
-                float best[2][2] = {{-INFINITY, -INFINITY}, {-INFINITY, -INFINITY}};  // [block g, g + 8][column 2 t, 2 t + 1]
-                for (uint32_t n = 0; n < columns; n += 8) {
-                    float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                    for (uint32_t c = 0; c < kChunks; ++c) {
-                        const uint4 b = *reinterpret_cast<const uint4 *>(selectSmem + (n + g) * kStride + 64 * c + 16 * t);
-                        mma_bf16(acc, v[0][c].x, v[1][c].x, v[0][c].y, v[1][c].y, b.x, b.y);
-                        mma_bf16(acc, v[0][c].z, v[1][c].z, v[0][c].w, v[1][c].w, b.z, b.w);
-                    }
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        // (a NaN mean makes all columns NaN: it stays)
-                        best[k >> 1][k & 1] = acc[k] != acc[k] ? acc[k] : fmaxf(best[k >> 1][k & 1], acc[k]);
-                    }
-                }
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    uint32_t k0 = order_of(best[h][0]), k1 = order_of(best[h][1]);
-                    if (__shfl_sync(0xFFFFFFFFu, page, g + 8 * h) >= a.pageCount) k0 = k1 = 0u;
-                    const uint32_t b = base + g + 8 * h;
-                    if (a.rowColumns > 1) k0 = k1 = max(k0, k1);
-                    if (a.rowColumns > 2) k0 = max(k0, __shfl_xor_sync(0xFFFFFFFFu, k0, 1));
-                    if (a.rowColumns > 4) k0 = max(k0, __shfl_xor_sync(0xFFFFFFFFu, k0, 2));
-                    if (b >= end) continue;
-                    if (a.rowColumns == 1) {
-                        if (2 * t >= i0 && 2 * t < i1) scores[2 * t * a.tableBlocks + b] = k0;
-                        if (2 * t + 1 >= i0 && 2 * t + 1 < i1) scores[(2 * t + 1) * a.tableBlocks + b] = k1;
-                    } else if ((2 * t) % min(a.rowColumns, 8u) == 0u) {
-                        const uint32_t i = 2 * t / min(a.rowColumns, 8u);
-                        if (i >= i0 && i < i1) scores[i * a.tableBlocks + b] = k0;
-                    }
-                }
-                if (__any_sync(0xFFFFFFFFu, lane < 16u && base + lane < end && page >= a.pageCount)) *a.errorFlag = kFlagPage;
             }
         }
     }
-    __syncthreads();
+}
+// The bound: the largest number that at least `wanted` of n scores reach, or any that `wanted` of them do.  count(t, step): how many reach t + step,
+// t + 2 step, t + 3 step.
+template <typename Count>
+__device__ __forceinline__ uint32_t select_bound(uint32_t n, uint32_t wanted, Count count) {
+    uint32_t low = 0, reached = n;
+    for (int shift = 30; shift >= 0 && reached != wanted; shift -= 2) {
+        const uint3 c = count(low, 1u << shift);
+        const uint32_t up = (c.x >= wanted) + (c.y >= wanted) + (c.z >= wanted);
+        reached = up == 0 ? reached : up == 1 ? c.x : up == 2 ? c.y : c.z;
+        low += up << shift;
+    }
+    return low;
+}
 
-    // ---- the lists, a row after the other ----
-    for (uint32_t i = 0; i < rows; ++i) {
-        const uint32_t seen = seenBlocks[i];
-        uint32_t *out = a.ids + ((size_t)(row0 + i) * a.kvHeads + head) * a.blocks;
-        if (seen <= a.blocks) {
-            for (uint32_t k = tid; k < a.blocks; k += kSelectThreads) out[k] = k < seen ? k : FF_NO_SLOT;
-            continue;
-        }
-        for (uint32_t k = tid; k < a.first; k += kSelectThreads) out[k] = k;
-        for (uint32_t k = tid; k < a.last; k += kSelectThreads) out[a.blocks - a.last + k] = seen - a.last + k;
-        if (!wanted) continue;
-        const uint32_t *mine = scores + i * a.tableBlocks + a.first, n = seen - a.last - a.first;  // (more than wanted)
-        // the largest bound that `wanted` scores reach: low is reached by that many, high is not
-        uint32_t low = 0, high = 0, reached = n;
-        uint32_t turn = 0;
-        auto count = [&](uint32_t bound) {
-            uint32_t c = 0;
-            for (uint32_t k = tid; k < n; k += kSelectThreads) c += mine[k] >= bound;
-            c = __reduce_add_sync(0xFFFFFFFFu, c);
-            if (lane == 0) counts[turn][warp] = c;
-            __syncthreads();
-            c = __reduce_add_sync(0xFFFFFFFFu, lane < kSelectWarps ? counts[turn][lane] : 0u);
-            turn ^= 1u;
-            return c;
-        };
-        // (high = 0 stands for 2^32)
-        while (reached != wanted && high - low != 1u) {
-            const uint32_t mid = low + (uint32_t)(((high ? (unsigned long long)high : 1ull << 32) - low) >> 1);
-            const uint32_t c = count(mid);
-            if (c >= wanted) low = mid, reached = c;
-            else high = mid;
-        }
-        // those above the bound, and the first of those at it
-        const uint32_t each = (n + kSelectThreads - 1) / kSelectThreads * 32u, k0 = min(warp * each, n), k1 = min(k0 + each, n);
-        uint32_t above = 0, at = 0;
-        for (uint32_t k = k0; k < k1; k += 32) {
-            const uint32_t v = k + lane < k1 ? mine[k + lane] : 0u;
-            const bool there = k + lane < k1;
-            above += __popc(__ballot_sync(0xFFFFFFFFu, there && v > low));
-            at += __popc(__ballot_sync(0xFFFFFFFFu, there && v == low));
-        }
-        if (lane == 0) greater[warp] = above, equal[warp] = at;
+template <int DIM>
+__global__ void __launch_bounds__(kSelectThreads) k_select_split(const __grid_constant__ SelectArgs a) {
+    extern __shared__ __align__(16) uint8_t selectSmem[];
+    __shared__ SelectRows s;
+    __shared__ uint4 counts[2][kSelectWarps];
+    __shared__ uint32_t greater[kSelectWarps], equal[kSelectWarps];
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+    const uint32_t head = blockIdx.z, row = blockIdx.y, cta = blockIdx.x, ctas = gridDim.x;
+    uint32_t *scores = reinterpret_cast<uint32_t *>(selectSmem + a.columns * select_query_stride(DIM));  // those of the cluster's first CTA count
+    if (tid == 0) s.request[0] = FF_NO_SLOT, s.seen[0] = 0u;
+    pdl_enter();
+    if (ctas > 1) cluster_sync_all();  // (the first CTA is there to be written to)
+    else __syncthreads();
+    select_look_up<DIM>(a, s, row, 1, head);
+    __syncthreads();
+    const uint32_t seen = s.seen[0], wanted = a.blocks - a.first - a.last;
+    uint32_t *out = a.ids + ((size_t)row * a.kvHeads + head) * a.blocks;
+    if (seen > a.blocks && wanted) {
+        select_stage<DIM>(a, s, row, 1, head, selectSmem);
         __syncthreads();
-        uint32_t aboveBefore = 0, atBefore = 0, aboveAll = 0;
+        const uint32_t to = ctas > 1 ? map_to_cta(sm_addr(scores), 0) : 0u;
+        select_score<DIM>(a, selectSmem, head, s.request[0], seen - a.last, cta * kSelectWarps + warp, ctas * kSelectWarps, [&](uint32_t i, uint32_t b, uint32_t score) {
+            if (i) return;  // (a column of no row)
+            if (ctas > 1) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to + 4 * b), "r"(score) : "memory");
+            else scores[b] = score;
+        });
+    }
+    if (ctas > 1) cluster_sync_all();
+    else __syncthreads();
+    if (cta) return;
+
+    if (seen <= a.blocks) {
+        for (uint32_t k = tid; k < a.blocks; k += kSelectThreads) out[k] = k < seen ? k : FF_NO_SLOT;
+        return;
+    }
+    for (uint32_t k = tid; k < a.first; k += kSelectThreads) out[k] = k;
+    for (uint32_t k = tid; k < a.last; k += kSelectThreads) out[a.blocks - a.last + k] = seen - a.last + k;
+    if (!wanted) return;
+    const uint32_t *mine = scores + a.first, n = seen - a.last - a.first;  // (more than wanted)
+    uint32_t turn = 0;
+    const uint32_t low = select_bound(n, wanted, [&](uint32_t t, uint32_t step) {
+        uint3 c = make_uint3(0u, 0u, 0u);
+#pragma unroll 4
+        for (uint32_t k = tid; k < n; k += kSelectThreads) {
+            const uint32_t v = mine[k];
+            c.x += v >= t + step, c.y += v >= t + 2 * step, c.z += v >= t + 3 * step;
+        }
+        c.x = __reduce_add_sync(0xFFFFFFFFu, c.x), c.y = __reduce_add_sync(0xFFFFFFFFu, c.y), c.z = __reduce_add_sync(0xFFFFFFFFu, c.z);
+        if (lane == 0) counts[turn][warp] = make_uint4(c.x, c.y, c.z, 0u);
+        __syncthreads();
+        c = make_uint3(0u, 0u, 0u);
 #pragma unroll
-        for (uint32_t w = 0; w < kSelectWarps; ++w) {
-            if (w < warp) aboveBefore += greater[w], atBefore += equal[w];
-            aboveAll += greater[w];
+        for (int w = 0; w < kSelectWarps; ++w) {
+            const uint4 of = counts[turn][w];
+            c.x += of.x, c.y += of.y, c.z += of.z;
         }
-        const uint32_t ties = wanted - aboveAll;
-        for (uint32_t k = k0; k < k1; k += 32) {
-            const bool there = k + lane < k1;
-            const uint32_t v = there ? mine[k + lane] : 0u;
-            const uint32_t up = __ballot_sync(0xFFFFFFFFu, there && v > low), same = __ballot_sync(0xFFFFFFFFu, there && v == low), under = (1u << lane) - 1u;
-            const uint32_t sameBefore = atBefore + __popc(same & under);
-            if (there && (v > low || (v == low && sameBefore < ties))) out[a.first + aboveBefore + __popc(up & under) + min(sameBefore, ties)] = a.first + k + lane;
-            aboveBefore += __popc(up);
-            atBefore += __popc(same);
-        }
-        __syncthreads();  // (the counts are free for the next row)
+        turn ^= 1u;
+        return c;
+    });
+    // those above the bound, and the first of those at it: a warp a run of the blocks
+    const uint32_t each = (n + kSelectThreads - 1) / kSelectThreads * 32u, k0 = min(warp * each, n), k1 = min(k0 + each, n);
+    uint32_t above = 0, at = 0;
+    for (uint32_t k = k0 + lane; k < k1; k += 32) {
+        above += mine[k] > low;
+        at += mine[k] == low;
+    }
+    above = __reduce_add_sync(0xFFFFFFFFu, above), at = __reduce_add_sync(0xFFFFFFFFu, at);
+    if (lane == 0) greater[warp] = above, equal[warp] = at;
+    __syncthreads();
+    uint32_t aboveBefore = 0, atBefore = 0, aboveAll = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kSelectWarps; ++w) {
+        if (w < warp) aboveBefore += greater[w], atBefore += equal[w];
+        aboveAll += greater[w];
+    }
+    const uint32_t ties = wanted - aboveAll, under = (1u << lane) - 1u;
+    for (uint32_t k = k0; k < k1; k += 32) {
+        const bool there = k + lane < k1;
+        const uint32_t v = there ? mine[k + lane] : 0u;
+        const uint32_t up = __ballot_sync(0xFFFFFFFFu, there && v > low), same = __ballot_sync(0xFFFFFFFFu, there && v == low);
+        const uint32_t sameBefore = atBefore + __popc(same & under);
+        if (there && (v > low || (v == low && sameBefore < ties))) out[a.first + aboveBefore + __popc(up & under) + min(sameBefore, ties)] = a.first + k + lane;
+        aboveBefore += __popc(up);
+        atBefore += __popc(same);
     }
 }
 
-KernelSmemMemo selectMemo[3];
+template <int DIM>
+__global__ void __launch_bounds__(kSelectThreads) k_select_rows(const __grid_constant__ SelectArgs a) {
+    extern __shared__ __align__(16) uint8_t selectSmem[];
+    __shared__ SelectRows s;
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+    const uint32_t head = blockIdx.y, row0 = blockIdx.x * a.rows, rows = min(a.rows, a.tokens - row0);
+    uint32_t *scores = reinterpret_cast<uint32_t *>(selectSmem + a.columns * select_query_stride(DIM));  // [rows][tableBlocks]
+    if (tid < kSelectWarps) s.request[tid] = FF_NO_SLOT, s.seen[tid] = 0u;
+    pdl_enter();
+    __syncthreads();
+    select_look_up<DIM>(a, s, row0, rows, head);
+    __syncthreads();
+    const uint32_t wanted = a.blocks - a.first - a.last;
+    select_stage<DIM>(a, s, row0, rows, head, selectSmem);
+    __syncthreads();
+    for (uint32_t i0 = 0, i1; i0 < rows; i0 = i1) {  // request by request
+        uint32_t end = 0;  // blocks that a row of the request may choose
+        for (i1 = i0; i1 < rows && s.request[i1] == s.request[i0]; ++i1)
+            if (s.seen[i1] > a.blocks) end = max(end, s.seen[i1] - a.last);
+        if (s.request[i0] == FF_NO_SLOT || !wanted) continue;
+        select_score<DIM>(a, selectSmem, head, s.request[i0], end, warp, kSelectWarps, [&](uint32_t i, uint32_t b, uint32_t score) {
+            if (i >= i0 && i < i1) scores[i * a.tableBlocks + b] = score;
+        });
+    }
+    __syncthreads();
+
+    if (warp >= rows) return;
+    const uint32_t seen = s.seen[warp];
+    uint32_t *out = a.ids + ((size_t)(row0 + warp) * a.kvHeads + head) * a.blocks;
+    if (seen <= a.blocks) {
+        for (uint32_t k = lane; k < a.blocks; k += 32) out[k] = k < seen ? k : FF_NO_SLOT;
+        return;
+    }
+    for (uint32_t k = lane; k < a.first; k += 32) out[k] = k;
+    for (uint32_t k = lane; k < a.last; k += 32) out[a.blocks - a.last + k] = seen - a.last + k;
+    if (!wanted) return;
+    const uint32_t *mine = scores + warp * a.tableBlocks + a.first, n = seen - a.last - a.first;  // (more than wanted)
+    const uint32_t low = select_bound(n, wanted, [&](uint32_t t, uint32_t step) {
+        uint3 c = make_uint3(0u, 0u, 0u);
+#pragma unroll 4
+        for (uint32_t k = lane; k < n; k += 32) {
+            const uint32_t v = mine[k];
+            c.x += v >= t + step, c.y += v >= t + 2 * step, c.z += v >= t + 3 * step;
+        }
+        return make_uint3(__reduce_add_sync(0xFFFFFFFFu, c.x), __reduce_add_sync(0xFFFFFFFFu, c.y), __reduce_add_sync(0xFFFFFFFFu, c.z));
+    });
+    uint32_t above = 0;
+    for (uint32_t k = lane; k < n; k += 32) above += mine[k] > low;
+    const uint32_t ties = wanted - __reduce_add_sync(0xFFFFFFFFu, above), under = (1u << lane) - 1u;
+    uint32_t aboveBefore = 0, atBefore = 0;
+    for (uint32_t k = 0; k < n; k += 32) {
+        const bool there = k + lane < n;
+        const uint32_t v = there ? mine[k + lane] : 0u;
+        const uint32_t up = __ballot_sync(0xFFFFFFFFu, there && v > low), same = __ballot_sync(0xFFFFFFFFu, there && v == low);
+        const uint32_t sameBefore = atBefore + __popc(same & under);
+        if (there && (v > low || (v == low && sameBefore < ties))) out[a.first + aboveBefore + __popc(up & under) + min(sameBefore, ties)] = a.first + k + lane;
+        aboveBefore += __popc(up);
+        atBefore += __popc(same);
+    }
+}
+
+KernelSmemMemo selectMemo[2][3];
 
 }  // namespace
 
@@ -417,25 +505,48 @@ bool launch_select_blocks(FFAttention *att, const uint16_t *q, uint32_t qStride,
                           const uint32_t *blockTable, uint32_t tableStride, uint32_t tableBlocks, const uint32_t *rowStart, const uint32_t *lengths,
                           uint32_t requests, uint32_t blocks, uint32_t first, uint32_t last, uint32_t *ids, cudaStream_t stream, const char **error) {
     const FFAttentionConfig &c = att->cfg;
-    const uint32_t group = c.heads / c.kvHeads;
+    const uint32_t group = c.heads / c.kvHeads, sms = (uint32_t)att->smCount;
     uint32_t rowColumns = group > 8 ? (group + 7u) & ~7u : 1u;
     while (rowColumns < group) rowColumns *= 2;
-    // As many rows as a product has columns for, which then read the means once; one where the CTAs would not fill the GPU, and where
-    // the scores would not leave room for two CTAs an SM.
-    uint32_t rows = rowColumns < 8 ? kSelectRows / rowColumns : 1u;
-    if ((uint64_t)tokens * c.kvHeads <= 2ull * att->smCount) rows = 1;
-    while (rows > 1 && select_smem(c.headDim, 8, rows, tableBlocks) > 100u * 1024u) rows /= 2;
-    const uint32_t columns = (rows * rowColumns + 7u) & ~7u, smem = select_smem(c.headDim, columns, rows, tableBlocks);
-    const SelectArgs args{q, qStride, tokens, means, pageCount, blockTable, tableStride, tableBlocks, rowStart, lengths, requests, c.heads, c.kvHeads,
-                          (uint32_t)__builtin_ctz(c.pageTokens), blocks, first, last, ids, rows, rowColumns, att->errorFlag};
-    const dim3 grid((tokens + rows - 1) / rows, c.kvHeads);
-    auto launch = [&](auto kernel, KernelSmemMemo &memo) {
-        if (!memo.prepare(kernel, att->device, smem, kSelectThreads, nullptr, error)) return false;
-        return launched(att, launch_pdl(kernel, grid, dim3(kSelectThreads), smem, stream, args), "k_select_blocks", error);
+    SelectArgs args{q, qStride, tokens, means, pageCount, blockTable, tableStride, tableBlocks, rowStart, lengths, requests, c.heads, c.kvHeads,
+                    (uint32_t)__builtin_ctz(c.pageTokens), blocks, first, last, ids, 1, rowColumns, 0, att->errorFlag};
+    const uint64_t lists = (uint64_t)tokens * c.kvHeads;
+    const int dim = c.headDim == 256 ? 2 : c.headDim == 128 ? 1 : 0;
+    if (lists <= 4ull * sms) {
+        // CTAs to fill the GPU, as long as each of them has eight warps' blocks
+        uint32_t ctas = 1;
+        while (ctas < kMostSplit && 2 * ctas * lists <= 2 * sms && 2 * ctas * kSelectWarps * 16 <= tableBlocks) ctas *= 2;
+        args.columns = std::max(8u, rowColumns);
+        const uint32_t smem = select_smem(c.headDim, args.columns, 1, tableBlocks);
+        auto launch = [&](auto kernel) {
+            if (!selectMemo[0][dim].prepare(kernel, att->device, smem, kSelectThreads, nullptr, error)) return false;
+            cudaLaunchConfig_t config{};
+            config.gridDim = dim3(ctas, tokens, c.kvHeads);
+            config.blockDim = dim3(kSelectThreads);
+            config.dynamicSmemBytes = smem;
+            config.stream = stream;
+            cudaLaunchAttribute attributes[2]{};
+            attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+            attributes[0].val.programmaticStreamSerializationAllowed = 1;
+            attributes[1].id = cudaLaunchAttributeClusterDimension;
+            attributes[1].val.clusterDim.x = ctas;
+            attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
+            config.attrs = attributes;
+            config.numAttrs = 2;
+            return launched(att, cudaLaunchKernelEx(&config, kernel, args), "k_select_split", error);
+        };
+        return dim == 2 ? launch(k_select_split<256>) : dim == 1 ? launch(k_select_split<128>) : launch(k_select_split<64>);
+    }
+    // A warp's list each, as far as the columns and the shared memory for their scores go.
+    args.rows = std::min((uint32_t)kSelectWarps, kSelectColumns / rowColumns);
+    while (args.rows > 1 && select_smem(c.headDim, std::max(8u, args.rows * rowColumns), args.rows, tableBlocks) > 100u * 1024u) args.rows /= 2;
+    args.columns = (args.rows * rowColumns + 7u) & ~7u;
+    const uint32_t smem = select_smem(c.headDim, args.columns, args.rows, tableBlocks);
+    auto launch = [&](auto kernel) {
+        if (!selectMemo[1][dim].prepare(kernel, att->device, smem, kSelectThreads, nullptr, error)) return false;
+        return launched(att, launch_pdl(kernel, dim3((tokens + args.rows - 1) / args.rows, c.kvHeads), dim3(kSelectThreads), smem, stream, args), "k_select_rows", error);
     };
-    if (c.headDim == 256) return launch(k_select_blocks<256>, selectMemo[2]);
-    if (c.headDim == 128) return launch(k_select_blocks<128>, selectMemo[1]);
-    return launch(k_select_blocks<64>, selectMemo[0]);
+    return dim == 2 ? launch(k_select_rows<256>) : dim == 1 ? launch(k_select_rows<128>) : launch(k_select_rows<64>);
 }
 
 }  // namespace ff
