@@ -166,15 +166,16 @@ __global__ void __launch_bounds__(kMeansThreads) k_block_means(const __grid_cons
 
 // Scores: the blocks' means times the rows' queries, 16 blocks a warp at a time on mma.sync.  Both factors are whole numbers of at
 // most 7 bits times a power of two of their own (the means as they are held, the queries as they are staged), so that every sum is below 2^23 of
-// its unit and exact in whatever order; the largest of a row's heads is the score.  Then the bound that as many scores reach as are
-// wanted, two bits of it at a time, until the number that reaches it is the number wanted or all bits are known: of the scores at the
-// bound the first are taken.
+// its unit and exact in whatever order; the largest of a row's heads is the score.  The scores wanted are found by counting them in 256 ranges
+// of equal width, those of the range that holds the last one wanted in 256 ranges again, and so on until a few are left, which are compared with
+// one another, or equal ones, of which the first are taken.
 //
 // Two forms.  k_select_split: a cluster of CTAs for each row and head, which share the blocks; the first of them gets the others' scores and
 // makes the list.  k_select_rows: some neighbouring rows a CTA, which read the means of their request once; a warp makes a list.
-constexpr int kSelectThreads = 256, kSelectWarps = kSelectThreads / 32;
-constexpr uint32_t kSelectColumns = 64;  // of a CTA's product, at most
-constexpr uint32_t kMostSplit = 8;       // CTAs of a cluster, at most
+constexpr uint32_t kRowsWarps = 8;        // of k_select_rows
+constexpr uint32_t kSelectColumns = 64;   // of a CTA's product, at most
+constexpr uint32_t kMostSplit = 8;        // CTAs of a cluster, at most
+constexpr uint32_t kBins = 256, kFew = 32;
 
 struct SelectArgs {
     const uint16_t *q;
@@ -207,30 +208,19 @@ inline uint32_t select_smem(uint32_t dim, uint32_t columns, uint32_t rows, uint3
 
 // What a CTA knows of its rows.
 struct SelectRows {
-    uint32_t request[kSelectWarps], seen[kSelectWarps];  // of each row; blocks that it sees
-    int exponents[kSelectColumns];                       // of a column's largest value; kNoNumber: it has a value that is not finite
-    static constexpr int kNoNumber = -1000;
+    uint32_t request[kRowsWarps], seen[kRowsWarps];  // of each row; blocks that it sees
+    int exponents[kSelectColumns];                   // of a column's largest value, where a row has more than eight
 };
-// the query of column c, or null: a row's columns are its heads, the last of them again in what is left
-template <int DIM>
-__device__ __forceinline__ const uint16_t *select_column(const SelectArgs &a, uint32_t row0, uint32_t rows, uint32_t head, uint32_t c) {
-    const uint32_t i = c / a.rowColumns, group = a.heads / a.kvHeads;
-    return i < rows ? a.q + (size_t)(row0 + i) * a.qStride + (size_t)(head * group + min(c % a.rowColumns, group - 1u)) * DIM : nullptr;
+constexpr int kNoNumber = -1000;  // the exponent of a query with a value that is not finite
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
 }
-// Requests and blocks of the rows, and the columns' exponents; a barrier in front, which s.request and s.seen are cleared before, and one behind.
-template <int DIM>
-__device__ __forceinline__ void select_look_up(const SelectArgs &a, SelectRows &s, uint32_t row0, uint32_t rows, uint32_t head) {
-    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
-    for (uint32_t c = warp; c < a.columns; c += kSelectWarps) {
-        const uint16_t *src = select_column<DIM>(a, row0, rows, head, c);
-        uint32_t most = 0;
-#pragma unroll
-        for (uint32_t d = 2 * lane; d < DIM; d += 64)
-            if (src) most = __vmaxu2(most, __ldg(reinterpret_cast<const uint32_t *>(src + d)) & 0x7FFF7FFFu);
-        most = __reduce_max_sync(0xFFFFFFFFu, max(most & 0xFFFFu, most >> 16)) >> 7;
-        if (lane == 0) s.exponents[c] = most == 255u ? SelectRows::kNoNumber : max((int)most - 127, -100);
-    }
-    for (uint32_t r = tid; r < a.requests; r += kSelectThreads) {
+
+// The rows' requests and the blocks that they see (s.request and s.seen are cleared, a barrier in front and behind).
+__device__ __forceinline__ void select_look_up(const SelectArgs &a, SelectRows &s, uint32_t row0, uint32_t rows, uint32_t thread, uint32_t threads) {
+    for (uint32_t r = thread; r < a.requests; r += threads) {
         const uint32_t begin = __ldg(a.rowStart + r), end = __ldg(a.rowStart + r + 1), length = min(__ldg(a.lengths + r), 0x7FFFFFFFu);
         if (end < begin) *a.errorFlag = kFlagRows;
         if (end <= row0 || begin >= row0 + rows || end <= begin) continue;
@@ -248,34 +238,73 @@ __device__ __forceinline__ void select_look_up(const SelectArgs &a, SelectRows &
         }
     }
 }
-// The columns as they are multiplied: whole numbers of at most 7 bits at the exponents, times a power of two that a row's columns share.
+// A row's queries as they are multiplied: whole numbers of at most 7 bits at a power of two of the query's largest value, times one that the row's
+// columns share; the last head again in what is left of the row's columns.
 template <int DIM>
-__device__ __forceinline__ void select_stage(const SelectArgs &a, const SelectRows &s, uint32_t row0, uint32_t rows, uint32_t head, uint8_t *to) {
-    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5;
-    for (uint32_t c = warp; c < a.columns; c += kSelectWarps) {
-        const uint16_t *src = select_column<DIM>(a, row0, rows, head, c);
-        const uint32_t c0 = c / a.rowColumns * a.rowColumns;
-        int top = -100;
-        for (uint32_t k = lane; k < a.rowColumns; k += 32)
-            if (c0 + k < a.columns) top = max(top, s.exponents[c0 + k]);
-        top = __reduce_max_sync(0xFFFFFFFFu, top);
-        const int mine = s.exponents[c], e = max(mine, top - 60);
-        if (mine == SelectRows::kNoNumber) src = nullptr;  // (counts as zeros)
+struct Query {
+    uint32_t v[DIM / 64];
+    __device__ __forceinline__ void load(const uint16_t *src) {
+#pragma unroll
+        for (int i = 0; i < DIM / 64; ++i) v[i] = __ldg(reinterpret_cast<const uint32_t *>(src) + (threadIdx.x & 31u) + 32 * i);
+    }
+    __device__ __forceinline__ int exponent() const {  // of the largest value
+        uint32_t most = 0;
+#pragma unroll
+        for (int i = 0; i < DIM / 64; ++i) most = __vmaxu2(most, v[i] & 0x7FFF7FFFu);
+        most = __reduce_max_sync(0xFFFFFFFFu, max(most & 0xFFFFu, most >> 16)) >> 7;
+        return most == 255u ? kNoNumber : max((int)most - 127, -100);
+    }
+    __device__ __forceinline__ void store(uint8_t *to, int mine, int top) const {
+        const int e = max(mine, top - 60);
         const float down = power_of_two(6 - e), up = power_of_two(e - top);
 #pragma unroll
-        for (uint32_t d = 2 * lane; d < DIM; d += 64) {
-            const uint32_t v = src ? __ldg(reinterpret_cast<const uint32_t *>(src + d)) : 0u;
-            const float x = fminf(fmaxf(rintf(low16(v) * down), -127.0f), 127.0f) * up, y = fminf(fmaxf(rintf(high16(v) * down), -127.0f), 127.0f) * up;
-            *reinterpret_cast<uint32_t *>(to + c * select_query_stride(DIM) + 2 * d) = pack_bf16x2(x, y);
+        for (int i = 0; i < DIM / 64; ++i) {
+            const uint32_t w = mine == kNoNumber ? 0u : v[i];  // (counts as zeros)
+            const float x = fminf(fmaxf(rintf(low16(w) * down), -127.0f), 127.0f) * up, y = fminf(fmaxf(rintf(high16(w) * down), -127.0f), 127.0f) * up;
+            reinterpret_cast<uint32_t *>(to)[(threadIdx.x & 31u) + 32 * i] = pack_bf16x2(x, y);
         }
     }
+};
+// up to eight columns a row: by one warp
+template <int DIM, int LOG>
+__device__ __forceinline__ void select_stage(const SelectArgs &a, uint32_t row, uint32_t head, uint8_t *to) {
+    const uint32_t group = a.heads / a.kvHeads;
+    const uint16_t *src = a.q + (size_t)row * a.qStride + (size_t)head * group * DIM;
+    Query<DIM> q[1 << LOG];
+    int exponent[1 << LOG], top = -100;
+#pragma unroll
+    for (int c = 0; c < 1 << LOG; ++c) q[c].load(src + min((uint32_t)c, group - 1u) * DIM);
+#pragma unroll
+    for (int c = 0; c < 1 << LOG; ++c) top = max(top, exponent[c] = q[c].exponent());
+#pragma unroll
+    for (int c = 0; c < 1 << LOG; ++c) q[c].store(to + c * select_query_stride(DIM), exponent[c], top);
 }
-// Scores of request r's blocks below `end`, in whole numbers of their order, to store(row of the CTA, block, score): sixteen at a time from
-// 16 tile on, 16 step apart.
-template <int DIM, typename Store>
-__device__ __forceinline__ void select_score(const SelectArgs &a, const uint8_t *queries, uint32_t head, uint32_t r, uint32_t end, uint32_t tile, uint32_t step, Store store) {
-    constexpr uint32_t kChunks = DIM / 32;
-    const uint32_t lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u, perPage = max(1u, (1u << a.pageShift) >> kBlockShift);
+// more: by all warps, with a barrier between
+template <int DIM>
+__device__ __forceinline__ void select_stage_wide(const SelectArgs &a, SelectRows &s, uint32_t row0, uint32_t rows, uint32_t head, uint8_t *to, uint32_t warps) {
+    const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, group = a.heads / a.kvHeads, columns = rows * a.rowColumns;
+    auto column = [&](uint32_t c) { return a.q + (size_t)(row0 + c / a.rowColumns) * a.qStride + (size_t)(head * group + min(c % a.rowColumns, group - 1u)) * DIM; };
+    Query<DIM> q;
+    for (uint32_t c = warp; c < columns; c += warps) {
+        q.load(column(c));
+        const int e = q.exponent();
+        if (lane == 0) s.exponents[c] = e;
+    }
+    __syncthreads();
+    for (uint32_t c = warp; c < columns; c += warps) {
+        q.load(column(c));
+        int top = -100;
+        for (uint32_t k = lane; k < a.rowColumns; k += 32) top = max(top, s.exponents[c / a.rowColumns * a.rowColumns + k]);
+        q.store(to + c * select_query_stride(DIM), s.exponents[c], __reduce_max_sync(0xFFFFFFFFu, top));
+    }
+}
+// Scores of request r's blocks below `end`, in whole numbers of their order, to scores[row of the CTA * stride + block] for rows i0 .. i1 - 1
+// (REMOTE: in another CTA's shared memory): sixteen at a time from 16 tile on, 16 step apart.
+template <int DIM, int LOG, bool REMOTE>
+__device__ __forceinline__ void select_score(const SelectArgs &a, const uint8_t *queries, uint32_t head, uint32_t r, uint32_t end, uint32_t tile, uint32_t step, uint32_t i0, uint32_t i1,
+                                             uint32_t scores, uint32_t stride) {
+    constexpr uint32_t kChunks = DIM / 32, kRowsOfTile = 8 >> LOG;
+    const uint32_t lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u, perPage = max(1u, (1u << a.pageShift) >> kBlockShift), tilesOfRow = LOG == 3 ? a.rowColumns / 8 : 1u;
     auto page_of = [&](uint32_t base) {  // of the mean of block base + lane % 16
         const uint32_t b = base + (lane & 15u);
         return b < end ? __ldg(a.blockTable + (size_t)r * a.tableStride + (((b << kBlockShift) + kTileKeys - 1u) >> a.pageShift)) : 0u;
@@ -295,198 +324,244 @@ __device__ __forceinline__ void select_score(const SelectArgs &a, const uint8_t 
         pageNext = page_of(base + 16 * step);
         const uint32_t gone = __ballot_sync(0xFFFFFFFFu, outside);
         if (gone && lane == 0) *a.errorFlag = kFlagPage;
-        float best[4];  // [block g: column 2 t, 2 t + 1; block g + 8: likewise] of the columns so far that are the row's
-        for (uint32_t n = 0; n < a.columns; n += 8) {
-            float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (uint32_t i = i0 / kRowsOfTile * kRowsOfTile; i < i1; i += kRowsOfTile) {
+            const uint8_t *from = queries + (i / kRowsOfTile * tilesOfRow * 8 + g) * select_query_stride(DIM) + 16 * t;
+            float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // [block g: column 2 t, 2 t + 1; block g + 8: likewise]
+            for (uint32_t n = 0; n < tilesOfRow; ++n) {
+                float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (uint32_t c = 0; c < kChunks; ++c) {
-                const uint4 b = *reinterpret_cast<const uint4 *>(queries + (n + g) * select_query_stride(DIM) + 64 * c + 16 * t);
-                mma_bf16(acc, v[0][c].x, v[1][c].x, v[0][c].y, v[1][c].y, b.x, b.y);
-                mma_bf16(acc, v[0][c].z, v[1][c].z, v[0][c].w, v[1][c].w, b.z, b.w);
+                for (uint32_t c = 0; c < kChunks; ++c) {
+                    const uint4 b = *reinterpret_cast<const uint4 *>(from + n * 8 * select_query_stride(DIM) + 64 * c);
+                    mma_bf16(acc, v[0][c].x, v[1][c].x, v[0][c].y, v[1][c].y, b.x, b.y);
+                    mma_bf16(acc, v[0][c].z, v[1][c].z, v[0][c].w, v[1][c].w, b.z, b.w);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) best[k] = LOG == 3 ? max_nan(best[k], acc[k]) : acc[k];
             }
-            const bool begins = a.rowColumns <= 8 || n % a.rowColumns == 0;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) best[k] = begins || acc[k] != acc[k] ? acc[k] : fmaxf(best[k], acc[k]);  // (a NaN mean makes all columns NaN)
-            if (a.rowColumns > 8 && (n + 8) % a.rowColumns) continue;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const uint32_t b = base + g + 8 * h, width = min(a.rowColumns, 8u);
-                uint32_t k0 = order_of(best[2 * h]), k1 = order_of(best[2 * h + 1]);
-                if (gone >> (g + 8 * h) & 1u) k0 = k1 = 0u;
-                if (width > 1) k0 = max(k0, k1);
-                if (width > 2) k0 = max(k0, __shfl_xor_sync(0xFFFFFFFFu, k0, 1));
-                if (width > 4) k0 = max(k0, __shfl_xor_sync(0xFFFFFFFFu, k0, 2));
-                if (b < end && (2 * t) % width == 0u) {
-                    store((n + 2 * t) / a.rowColumns, b, k0);
-                    if (width == 1) store(n + 2 * t + 1, b, k1);
+                float x = best[2 * h];
+                if (LOG > 0) x = max_nan(x, best[2 * h + 1]);
+                if (LOG > 1) x = max_nan(x, __shfl_xor_sync(0xFFFFFFFFu, x, 1));
+                if (LOG > 2) x = max_nan(x, __shfl_xor_sync(0xFFFFFFFFu, x, 2));
+                const uint32_t b = base + g + 8 * h;
+                const bool none = gone >> (g + 8 * h) & 1u;
+                if (b >= end || (LOG > 0 && (2 * t) & ((1 << LOG) - 1))) continue;
+#pragma unroll
+                for (int k = 0; k < (LOG == 0 ? 2 : 1); ++k) {
+                    const uint32_t row = i + (2 * t >> LOG) + k, order = none ? 0u : order_of(LOG == 0 ? best[2 * h + k] : x);
+                    if (row < i0 || row >= i1) continue;
+                    if (REMOTE) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(scores + 4 * (row * stride + b)), "r"(order) : "memory");
+                    else asm volatile("st.shared.u32 [%0], %1;" ::"r"(scores + 4 * (row * stride + b)), "r"(order) : "memory");
                 }
             }
         }
     }
 }
-// The bound: the largest number that at least `wanted` of n scores reach, or any that `wanted` of them do.  count(t, step): how many reach t + step,
-// t + 2 step, t + 3 step.
-template <typename Count>
-__device__ __forceinline__ uint32_t select_bound(uint32_t n, uint32_t wanted, Count count) {
-    uint32_t low = 0, reached = n;
-    for (int shift = 30; shift >= 0 && reached != wanted; shift -= 2) {
-        const uint3 c = count(low, 1u << shift);
-        const uint32_t up = (c.x >= wanted) + (c.y >= wanted) + (c.z >= wanted);
-        reached = up == 0 ? reached : up == 1 ? c.x : up == 2 ? c.y : c.z;
-        low += up << shift;
+
+// The `wanted` largest of n scores (more than wanted), of equal ones the first, by WARPS warps: ids first + place, ascending, to out.
+struct SelectCounts {
+    uint32_t bins[2][kBins];  // of this level, of the next
+    uint2 few[kFew];          // score, place
+    uint32_t least[2][16], most[2][16], above[16], same[16], held;  // of each warp
+};
+template <int WARPS>
+__device__ __forceinline__ void select_meet() {
+    if (WARPS == 1) __syncwarp();
+    else __syncthreads();
+}
+__device__ __forceinline__ float score_of(uint32_t order) { return __uint_as_float(order ^ ((order >> 31) ? 0x80000000u : 0xFFFFFFFFu)); }
+template <int WARPS>
+__device__ __forceinline__ void select_largest(const uint32_t *scores, uint32_t n, uint32_t wanted, uint32_t first, uint32_t *out, SelectCounts &s) {
+    const uint32_t lane = threadIdx.x & 31u, warp = WARPS == 1 ? 0u : threadIdx.x >> 5, thread = WARPS == 1 ? lane : threadIdx.x;
+    const uint32_t each = (n + 32 * WARPS - 1) / (32 * WARPS) * 32u, k0 = min(warp * each, n), k1 = min(k0 + each, n);  // a warp's run of them
+    // Of the scores from `low` to `high`, which are the least and the greatest of them, `left` are wanted; those above are, those below are not.
+    uint32_t low = 0xFFFFFFFFu, high = 0u, left = wanted, few = n;
+    auto all_warps = [&](uint32_t *lows, uint32_t *highs) {
+        low = __reduce_min_sync(0xFFFFFFFFu, low), high = __reduce_max_sync(0xFFFFFFFFu, high);
+        if (WARPS > 1 && lane == 0) lows[warp] = low, highs[warp] = high;
+        select_meet<WARPS>();
+        if (WARPS > 1) low = __reduce_min_sync(0xFFFFFFFFu, lows[lane % WARPS]), high = __reduce_max_sync(0xFFFFFFFFu, highs[lane % WARPS]);
+    };
+    for (uint32_t k = thread; k < kBins; k += 32 * WARPS) s.bins[0][k] = 0u;
+    if (thread == 0) s.held = 0u;
+#pragma unroll 4
+    for (uint32_t k = k0 + lane; k < k1; k += 32) low = min(low, scores[k]), high = max(high, scores[k]);
+    all_warps(s.least[1], s.most[1]);
+    for (uint32_t level = 0; low != high && few > kFew; ++level) {
+        // Ranges of equal width, twice of the scores' values (which lie evenly), then of the whole numbers that stand for them (which ends).
+        // Scores that are no number, or of no mean, are the last and the first of these.
+        const uint32_t least = low, most = high, *bins = s.bins[level & 1u];
+        const bool values = level < 2 && least > 0x00800000u && most < 0xFF800000u;
+        const float from = score_of(least), widthInverse = (kBins - 1) / (score_of(most) - from);
+        const uint32_t shift = max(0, 24 - __clz(most - least));
+        auto bin_of = [&](uint32_t v) { return values ? min((uint32_t)((score_of(v) - from) * widthInverse), kBins - 1u) : (v - least) >> shift; };
+#pragma unroll 4
+        for (uint32_t k = k0 + lane; k < k1; k += 32) {
+            const uint32_t v = scores[k];
+            if (v >= least && v <= most) atomicAdd(&s.bins[level & 1u][bin_of(v)], 1u);
+        }
+        select_meet<WARPS>();
+        // the range that holds the last one wanted: a lane has eight, the uppermost lane the last
+        uint32_t counts[kBins / 32], sum = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < kBins / 32; ++i) sum += counts[i] = bins[lane * (kBins / 32) + i];
+        for (uint32_t k = thread; k < kBins; k += 32 * WARPS) s.bins[~level & 1u][k] = 0u;
+        uint32_t above = sum;  // in this lane's ranges and above
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const uint32_t v = __shfl_down_sync(0xFFFFFFFFu, above, d);
+            if (lane + d < 32) above += v;
+        }
+        above -= sum;
+        const bool here = above < left && above + sum >= left;
+        uint32_t bin = 0, over = above, inside = 0;
+        bool found = false;
+#pragma unroll
+        for (int i = kBins / 32 - 1; i >= 0; --i)
+            if (!found) {
+                if (over + counts[i] >= left) bin = lane * (kBins / 32) + i, inside = counts[i], found = true;
+                else over += counts[i];
+            }
+        const uint32_t source = 31u - __clz(__ballot_sync(0xFFFFFFFFu, here));
+        bin = __shfl_sync(0xFFFFFFFFu, bin, source), few = __shfl_sync(0xFFFFFFFFu, inside, source), left -= __shfl_sync(0xFFFFFFFFu, over, source);
+        low = 0xFFFFFFFFu, high = 0u;
+#pragma unroll 4
+        for (uint32_t k = k0 + lane; k < k1; k += 32) {
+            const uint32_t v = scores[k];
+            if (v >= least && v <= most && bin_of(v) == bin) low = min(low, v), high = max(high, v);
+        }
+        all_warps(s.least[level & 1u], s.most[level & 1u]);
     }
-    return low;
+    const bool equal = low == high;
+    // a few scores: the last one wanted is the `left`-th largest of them, with its place
+    uint32_t bound = low, place = 0xFFFFFFFFu;
+    if (!equal) {
+        for (uint32_t k = k0 + lane; k < k1; k += 32) {
+            const uint32_t v = scores[k];
+            if (v >= low && v <= high) s.few[atomicAdd(&s.held, 1u)] = make_uint2(v, k);
+        }
+        select_meet<WARPS>();
+        const uint2 mine = s.few[min(lane, few - 1u)];
+        uint32_t before = 0;
+        for (uint32_t i = 0; i < few; ++i) {
+            const uint2 other = s.few[i];
+            before += other.x > mine.x || (other.x == mine.x && other.y < mine.y);
+        }
+        const uint32_t who = __ballot_sync(0xFFFFFFFFu, lane < few && before == left - 1u);
+        bound = __shfl_sync(0xFFFFFFFFu, mine.x, __ffs(who) - 1), place = __shfl_sync(0xFFFFFFFFu, mine.y, __ffs(who) - 1);
+    }
+    // those above the bound, and of those at it the first (equal: `left` of them; otherwise up to the place)
+    uint32_t aboveBefore = 0, sameBefore = 0;
+    auto above_it = [&](uint32_t v, uint32_t k) { return v > bound || (!equal && v == bound && k <= place); };
+    auto at_it = [&](uint32_t v) { return equal && v == bound; };
+    if (WARPS > 1) {
+        uint32_t above = 0, same = 0;
+        for (uint32_t k = k0 + lane; k < k1; k += 32) {
+            const uint32_t v = scores[k];
+            above += above_it(v, k), same += at_it(v);
+        }
+        above = __reduce_add_sync(0xFFFFFFFFu, above), same = __reduce_add_sync(0xFFFFFFFFu, same);
+        if (lane == 0) s.above[warp] = above, s.same[warp] = same;
+        select_meet<WARPS>();
+        const bool front = lane < warp;
+        aboveBefore = __reduce_add_sync(0xFFFFFFFFu, front ? s.above[lane % WARPS] : 0u), sameBefore = __reduce_add_sync(0xFFFFFFFFu, front ? s.same[lane % WARPS] : 0u);
+    }
+    const uint32_t under = (1u << lane) - 1u;
+    for (uint32_t k = k0; k < k1; k += 32) {
+        const bool there = k + lane < k1;
+        const uint32_t v = there ? scores[k + lane] : 0u;
+        const bool up = there && above_it(v, k + lane), same = there && at_it(v);
+        const uint32_t ups = __ballot_sync(0xFFFFFFFFu, up), sames = __ballot_sync(0xFFFFFFFFu, same);
+        const uint32_t at = sameBefore + __popc(sames & under);
+        if (up || (same && at < left)) out[aboveBefore + __popc(ups & under) + min(at, left)] = first + k + lane;
+        aboveBefore += __popc(ups);
+        sameBefore += __popc(sames);
+    }
+}
+// What of a list needs no scores, by `threads` threads; whether that is all of it.
+__device__ __forceinline__ bool select_always(const SelectArgs &a, uint32_t *out, uint32_t seen, uint32_t thread, uint32_t threads) {
+    if (seen <= a.blocks) {
+        for (uint32_t k = thread; k < a.blocks; k += threads) out[k] = k < seen ? k : FF_NO_SLOT;
+        return true;
+    }
+    for (uint32_t k = thread; k < a.first; k += threads) out[k] = k;
+    for (uint32_t k = thread; k < a.last; k += threads) out[a.blocks - a.last + k] = seen - a.last + k;
+    return a.blocks == a.first + a.last;
 }
 
-template <int DIM>
-__global__ void __launch_bounds__(kSelectThreads) k_select_split(const __grid_constant__ SelectArgs a) {
+// warps of k_select_split: at 256 values a head a warp's registers leave room for eight
+__host__ __device__ constexpr uint32_t split_warps(int dim) { return dim == 256 ? 8u : 16u; }
+
+template <int DIM, int LOG>
+__global__ void __launch_bounds__(32 * split_warps(DIM)) k_select_split(const __grid_constant__ SelectArgs a) {
+    constexpr uint32_t kWarps = split_warps(DIM);
     extern __shared__ __align__(16) uint8_t selectSmem[];
     __shared__ SelectRows s;
-    __shared__ uint4 counts[2][kSelectWarps];
-    __shared__ uint32_t greater[kSelectWarps], equal[kSelectWarps];
-    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+    __shared__ SelectCounts counts;
+    const uint32_t tid = threadIdx.x, warp = tid >> 5;
     const uint32_t head = blockIdx.z, row = blockIdx.y, cta = blockIdx.x, ctas = gridDim.x;
     uint32_t *scores = reinterpret_cast<uint32_t *>(selectSmem + a.columns * select_query_stride(DIM));  // those of the cluster's first CTA count
     if (tid == 0) s.request[0] = FF_NO_SLOT, s.seen[0] = 0u;
     pdl_enter();
-    if (ctas > 1) cluster_sync_all();  // (the first CTA is there to be written to)
-    else __syncthreads();
-    select_look_up<DIM>(a, s, row, 1, head);
+    if (ctas > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // (the first CTA is there to be written to: waited for below)
     __syncthreads();
+    const bool wide = LOG == 3 && a.rowColumns > 8;
+    if (!wide && warp == 0) select_stage<DIM, LOG>(a, row, head, selectSmem);
+    if (!wide && warp == 1 && LOG < 3)  // (columns of no row)
+        for (uint32_t k = tid & 31u; k < (8 - (1 << LOG)) * select_query_stride(DIM) / 4; k += 32) reinterpret_cast<uint32_t *>(selectSmem + (1 << LOG) * select_query_stride(DIM))[k] = 0u;
+    if (wide) select_stage_wide<DIM>(a, s, row, 1, head, selectSmem, kWarps);
+    select_look_up(a, s, row, 1, (tid + 32 * (kWarps - 2)) % (32 * kWarps), 32 * kWarps);  // (from the third warp on: the first has something to do)
+    __syncthreads();
+    if (ctas > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     const uint32_t seen = s.seen[0], wanted = a.blocks - a.first - a.last;
-    uint32_t *out = a.ids + ((size_t)row * a.kvHeads + head) * a.blocks;
     if (seen > a.blocks && wanted) {
-        select_stage<DIM>(a, s, row, 1, head, selectSmem);
-        __syncthreads();
-        const uint32_t to = ctas > 1 ? map_to_cta(sm_addr(scores), 0) : 0u;
-        select_score<DIM>(a, selectSmem, head, s.request[0], seen - a.last, cta * kSelectWarps + warp, ctas * kSelectWarps, [&](uint32_t i, uint32_t b, uint32_t score) {
-            if (i) return;  // (a column of no row)
-            if (ctas > 1) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to + 4 * b), "r"(score) : "memory");
-            else scores[b] = score;
-        });
+        const uint32_t tile = cta * kWarps + warp, step = ctas * kWarps;
+        if (cta) select_score<DIM, LOG, true>(a, selectSmem, head, s.request[0], seen - a.last, tile, step, 0, 1, map_to_cta(sm_addr(scores), 0), 0);
+        else select_score<DIM, LOG, false>(a, selectSmem, head, s.request[0], seen - a.last, tile, step, 0, 1, sm_addr(scores), 0);
     }
     if (ctas > 1) cluster_sync_all();
     else __syncthreads();
     if (cta) return;
-
-    if (seen <= a.blocks) {
-        for (uint32_t k = tid; k < a.blocks; k += kSelectThreads) out[k] = k < seen ? k : FF_NO_SLOT;
-        return;
-    }
-    for (uint32_t k = tid; k < a.first; k += kSelectThreads) out[k] = k;
-    for (uint32_t k = tid; k < a.last; k += kSelectThreads) out[a.blocks - a.last + k] = seen - a.last + k;
-    if (!wanted) return;
-    const uint32_t *mine = scores + a.first, n = seen - a.last - a.first;  // (more than wanted)
-    uint32_t turn = 0;
-    const uint32_t low = select_bound(n, wanted, [&](uint32_t t, uint32_t step) {
-        uint3 c = make_uint3(0u, 0u, 0u);
-#pragma unroll 4
-        for (uint32_t k = tid; k < n; k += kSelectThreads) {
-            const uint32_t v = mine[k];
-            c.x += v >= t + step, c.y += v >= t + 2 * step, c.z += v >= t + 3 * step;
-        }
-        c.x = __reduce_add_sync(0xFFFFFFFFu, c.x), c.y = __reduce_add_sync(0xFFFFFFFFu, c.y), c.z = __reduce_add_sync(0xFFFFFFFFu, c.z);
-        if (lane == 0) counts[turn][warp] = make_uint4(c.x, c.y, c.z, 0u);
-        __syncthreads();
-        c = make_uint3(0u, 0u, 0u);
-#pragma unroll
-        for (int w = 0; w < kSelectWarps; ++w) {
-            const uint4 of = counts[turn][w];
-            c.x += of.x, c.y += of.y, c.z += of.z;
-        }
-        turn ^= 1u;
-        return c;
-    });
-    // those above the bound, and the first of those at it: a warp a run of the blocks
-    const uint32_t each = (n + kSelectThreads - 1) / kSelectThreads * 32u, k0 = min(warp * each, n), k1 = min(k0 + each, n);
-    uint32_t above = 0, at = 0;
-    for (uint32_t k = k0 + lane; k < k1; k += 32) {
-        above += mine[k] > low;
-        at += mine[k] == low;
-    }
-    above = __reduce_add_sync(0xFFFFFFFFu, above), at = __reduce_add_sync(0xFFFFFFFFu, at);
-    if (lane == 0) greater[warp] = above, equal[warp] = at;
-    __syncthreads();
-    uint32_t aboveBefore = 0, atBefore = 0, aboveAll = 0;
-#pragma unroll
-    for (uint32_t w = 0; w < kSelectWarps; ++w) {
-        if (w < warp) aboveBefore += greater[w], atBefore += equal[w];
-        aboveAll += greater[w];
-    }
-    const uint32_t ties = wanted - aboveAll, under = (1u << lane) - 1u;
-    for (uint32_t k = k0; k < k1; k += 32) {
-        const bool there = k + lane < k1;
-        const uint32_t v = there ? mine[k + lane] : 0u;
-        const uint32_t up = __ballot_sync(0xFFFFFFFFu, there && v > low), same = __ballot_sync(0xFFFFFFFFu, there && v == low);
-        const uint32_t sameBefore = atBefore + __popc(same & under);
-        if (there && (v > low || (v == low && sameBefore < ties))) out[a.first + aboveBefore + __popc(up & under) + min(sameBefore, ties)] = a.first + k + lane;
-        aboveBefore += __popc(up);
-        atBefore += __popc(same);
-    }
+    uint32_t *out = a.ids + ((size_t)row * a.kvHeads + head) * a.blocks;
+    if (select_always(a, out, seen, tid, 32 * kWarps)) return;
+    select_largest<kWarps>(scores + a.first, seen - a.last - a.first, wanted, a.first, out + a.first, counts);
 }
 
-template <int DIM>
-__global__ void __launch_bounds__(kSelectThreads) k_select_rows(const __grid_constant__ SelectArgs a) {
+template <int DIM, int LOG>
+__global__ void __launch_bounds__(32 * kRowsWarps) k_select_rows(const __grid_constant__ SelectArgs a) {
     extern __shared__ __align__(16) uint8_t selectSmem[];
     __shared__ SelectRows s;
+    __shared__ SelectCounts counts[kRowsWarps];
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
     const uint32_t head = blockIdx.y, row0 = blockIdx.x * a.rows, rows = min(a.rows, a.tokens - row0);
     uint32_t *scores = reinterpret_cast<uint32_t *>(selectSmem + a.columns * select_query_stride(DIM));  // [rows][tableBlocks]
-    if (tid < kSelectWarps) s.request[tid] = FF_NO_SLOT, s.seen[tid] = 0u;
+    if (tid < kRowsWarps) s.request[tid] = FF_NO_SLOT, s.seen[tid] = 0u;
     pdl_enter();
     __syncthreads();
-    select_look_up<DIM>(a, s, row0, rows, head);
-    __syncthreads();
     const uint32_t wanted = a.blocks - a.first - a.last;
-    select_stage<DIM>(a, s, row0, rows, head, selectSmem);
+    if (LOG == 3 && a.rowColumns > 8) select_stage_wide<DIM>(a, s, row0, rows, head, selectSmem, kRowsWarps);
+    else if (warp < rows) select_stage<DIM, LOG>(a, row0 + warp, head, selectSmem + (warp << LOG) * select_query_stride(DIM));
+    else if ((warp << LOG) < a.columns)  // (columns of no row)
+        for (uint32_t k = lane; k < (select_query_stride(DIM) << LOG) / 4; k += 32) reinterpret_cast<uint32_t *>(selectSmem + (warp << LOG) * select_query_stride(DIM))[k] = 0u;
+    select_look_up(a, s, row0, rows, tid, 32 * kRowsWarps);
     __syncthreads();
     for (uint32_t i0 = 0, i1; i0 < rows; i0 = i1) {  // request by request
         uint32_t end = 0;  // blocks that a row of the request may choose
         for (i1 = i0; i1 < rows && s.request[i1] == s.request[i0]; ++i1)
             if (s.seen[i1] > a.blocks) end = max(end, s.seen[i1] - a.last);
         if (s.request[i0] == FF_NO_SLOT || !wanted) continue;
-        select_score<DIM>(a, selectSmem, head, s.request[i0], end, warp, kSelectWarps, [&](uint32_t i, uint32_t b, uint32_t score) {
-            if (i >= i0 && i < i1) scores[i * a.tableBlocks + b] = score;
-        });
+        select_score<DIM, LOG, false>(a, selectSmem, head, s.request[i0], end, warp, kRowsWarps, i0, i1, sm_addr(scores), a.tableBlocks);
     }
     __syncthreads();
-
     if (warp >= rows) return;
     const uint32_t seen = s.seen[warp];
     uint32_t *out = a.ids + ((size_t)(row0 + warp) * a.kvHeads + head) * a.blocks;
-    if (seen <= a.blocks) {
-        for (uint32_t k = lane; k < a.blocks; k += 32) out[k] = k < seen ? k : FF_NO_SLOT;
-        return;
-    }
-    for (uint32_t k = lane; k < a.first; k += 32) out[k] = k;
-    for (uint32_t k = lane; k < a.last; k += 32) out[a.blocks - a.last + k] = seen - a.last + k;
-    if (!wanted) return;
-    const uint32_t *mine = scores + warp * a.tableBlocks + a.first, n = seen - a.last - a.first;  // (more than wanted)
-    const uint32_t low = select_bound(n, wanted, [&](uint32_t t, uint32_t step) {
-        uint3 c = make_uint3(0u, 0u, 0u);
-#pragma unroll 4
-        for (uint32_t k = lane; k < n; k += 32) {
-            const uint32_t v = mine[k];
-            c.x += v >= t + step, c.y += v >= t + 2 * step, c.z += v >= t + 3 * step;
-        }
-        return make_uint3(__reduce_add_sync(0xFFFFFFFFu, c.x), __reduce_add_sync(0xFFFFFFFFu, c.y), __reduce_add_sync(0xFFFFFFFFu, c.z));
-    });
-    uint32_t above = 0;
-    for (uint32_t k = lane; k < n; k += 32) above += mine[k] > low;
-    const uint32_t ties = wanted - __reduce_add_sync(0xFFFFFFFFu, above), under = (1u << lane) - 1u;
-    uint32_t aboveBefore = 0, atBefore = 0;
-    for (uint32_t k = 0; k < n; k += 32) {
-        const bool there = k + lane < n;
-        const uint32_t v = there ? mine[k + lane] : 0u;
-        const uint32_t up = __ballot_sync(0xFFFFFFFFu, there && v > low), same = __ballot_sync(0xFFFFFFFFu, there && v == low);
-        const uint32_t sameBefore = atBefore + __popc(same & under);
-        if (there && (v > low || (v == low && sameBefore < ties))) out[a.first + aboveBefore + __popc(up & under) + min(sameBefore, ties)] = a.first + k + lane;
-        aboveBefore += __popc(up);
-        atBefore += __popc(same);
-    }
+    if (select_always(a, out, seen, lane, 32)) return;
+    select_largest<1>(scores + warp * a.tableBlocks + a.first, seen - a.last - a.first, wanted, a.first, out + a.first, counts[warp]);
 }
 
-KernelSmemMemo selectMemo[2][3];
+KernelSmemMemo selectMemo[2][3][4];
 
 }  // namespace
 
@@ -511,18 +586,27 @@ bool launch_select_blocks(FFAttention *att, const uint16_t *q, uint32_t qStride,
     SelectArgs args{q, qStride, tokens, means, pageCount, blockTable, tableStride, tableBlocks, rowStart, lengths, requests, c.heads, c.kvHeads,
                     (uint32_t)__builtin_ctz(c.pageTokens), blocks, first, last, ids, 1, rowColumns, 0, att->errorFlag};
     const uint64_t lists = (uint64_t)tokens * c.kvHeads;
-    const int dim = c.headDim == 256 ? 2 : c.headDim == 128 ? 1 : 0;
+    const int dim = c.headDim == 256 ? 2 : c.headDim == 128 ? 1 : 0, log = rowColumns >= 8 ? 3 : __builtin_ctz(rowColumns);
+    auto of_shape = [&](auto launch) {  // launch(values of a head, columns of a row as a power of two), as constants
+        auto of_dim = [&](auto d) {
+            return log == 3 ? launch(d, std::integral_constant<int, 3>()) : log == 2 ? launch(d, std::integral_constant<int, 2>())
+                 : log == 1 ? launch(d, std::integral_constant<int, 1>()) : launch(d, std::integral_constant<int, 0>());
+        };
+        return dim == 2 ? of_dim(std::integral_constant<int, 256>()) : dim == 1 ? of_dim(std::integral_constant<int, 128>()) : of_dim(std::integral_constant<int, 64>());
+    };
     if (lists <= 4ull * sms) {
-        // CTAs to fill the GPU, as long as each of them has eight warps' blocks
+        // CTAs to fill the GPU, as long as each of them has its warps' blocks
+        const uint32_t warps = split_warps((int)c.headDim);
         uint32_t ctas = 1;
-        while (ctas < kMostSplit && 2 * ctas * lists <= 2 * sms && 2 * ctas * kSelectWarps * 16 <= tableBlocks) ctas *= 2;
+        while (ctas < kMostSplit && 2 * ctas * lists <= 2 * sms && 2 * ctas * warps * 16 <= tableBlocks) ctas *= 2;
         args.columns = std::max(8u, rowColumns);
         const uint32_t smem = select_smem(c.headDim, args.columns, 1, tableBlocks);
-        auto launch = [&](auto kernel) {
-            if (!selectMemo[0][dim].prepare(kernel, att->device, smem, kSelectThreads, nullptr, error)) return false;
+        return of_shape([&](auto d, auto l) {
+            const auto kernel = k_select_split<d.value, l.value>;
+            if (!selectMemo[0][dim][log].prepare(kernel, att->device, smem, 32 * warps, nullptr, error)) return false;
             cudaLaunchConfig_t config{};
             config.gridDim = dim3(ctas, tokens, c.kvHeads);
-            config.blockDim = dim3(kSelectThreads);
+            config.blockDim = dim3(32 * warps);
             config.dynamicSmemBytes = smem;
             config.stream = stream;
             cudaLaunchAttribute attributes[2]{};
@@ -534,19 +618,18 @@ bool launch_select_blocks(FFAttention *att, const uint16_t *q, uint32_t qStride,
             config.attrs = attributes;
             config.numAttrs = 2;
             return launched(att, cudaLaunchKernelEx(&config, kernel, args), "k_select_split", error);
-        };
-        return dim == 2 ? launch(k_select_split<256>) : dim == 1 ? launch(k_select_split<128>) : launch(k_select_split<64>);
+        });
     }
     // A warp's list each, as far as the columns and the shared memory for their scores go.
-    args.rows = std::min((uint32_t)kSelectWarps, kSelectColumns / rowColumns);
+    args.rows = std::min(kRowsWarps, kSelectColumns / rowColumns);
     while (args.rows > 1 && select_smem(c.headDim, std::max(8u, args.rows * rowColumns), args.rows, tableBlocks) > 100u * 1024u) args.rows /= 2;
-    args.columns = (args.rows * rowColumns + 7u) & ~7u;
+    args.columns = std::max(8u, args.rows * rowColumns);
     const uint32_t smem = select_smem(c.headDim, args.columns, args.rows, tableBlocks);
-    auto launch = [&](auto kernel) {
-        if (!selectMemo[1][dim].prepare(kernel, att->device, smem, kSelectThreads, nullptr, error)) return false;
-        return launched(att, launch_pdl(kernel, dim3((tokens + args.rows - 1) / args.rows, c.kvHeads), dim3(kSelectThreads), smem, stream, args), "k_select_rows", error);
-    };
-    return dim == 2 ? launch(k_select_rows<256>) : dim == 1 ? launch(k_select_rows<128>) : launch(k_select_rows<64>);
+    return of_shape([&](auto d, auto l) {
+        const auto kernel = k_select_rows<d.value, l.value>;
+        if (!selectMemo[1][dim][log].prepare(kernel, att->device, smem, 32 * kRowsWarps, nullptr, error)) return false;
+        return launched(att, launch_pdl(kernel, dim3((tokens + args.rows - 1) / args.rows, c.kvHeads), dim3(32 * kRowsWarps), smem, stream, args), "k_select_rows", error);
+    });
 }
 
 }  // namespace ff
