@@ -188,12 +188,12 @@ struct SelectArgs {
     uint32_t requests, heads, kvHeads, pageShift;
     uint32_t blocks, first, last;
     uint32_t *ids;
-    uint32_t rows, rowColumns, columns;  // of a CTA; columns of a row: the heads of its group, to a power of two or a multiple of 8
+    uint32_t rows, rowColumns, columns;  // of a CTA; columns of a row: the heads of its group, to a power of two or a multiple of 8 (the last head again)
     uint32_t *errorFlag;
 };
 
 __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -238,8 +238,7 @@ __device__ __forceinline__ void select_look_up(const SelectArgs &a, SelectRows &
         }
     }
 }
-// A row's queries as they are multiplied: whole numbers of at most 7 bits at a power of two of the query's largest value, times one that the row's
-// columns share; the last head again in what is left of the row's columns.
+// A query as it is multiplied: whole numbers of at most 7 bits at a power of two of its largest value, times one that the row's queries share.
 template <int DIM>
 struct Query {
     uint32_t v[DIM / 64];
@@ -265,22 +264,29 @@ struct Query {
         }
     }
 };
-// up to eight columns a row: by one warp
-template <int DIM, int LOG>
-__device__ __forceinline__ void select_stage(const SelectArgs &a, uint32_t row, uint32_t head, uint8_t *to) {
-    const uint32_t group = a.heads / a.kvHeads;
-    const uint16_t *src = a.q + (size_t)row * a.qStride + (size_t)head * group * DIM;
-    Query<DIM> q[1 << LOG];
-    int exponent[1 << LOG], top = -100;
-#pragma unroll
-    for (int c = 0; c < 1 << LOG; ++c) q[c].load(src + min((uint32_t)c, group - 1u) * DIM);
-#pragma unroll
-    for (int c = 0; c < 1 << LOG; ++c) top = max(top, exponent[c] = q[c].exponent());
-#pragma unroll
-    for (int c = 0; c < 1 << LOG; ++c) q[c].store(to + c * select_query_stride(DIM), exponent[c], top);
+// Where column c of a row stands among the CTA's: a tile of eight holds 8 / RT columns of each of RT rows, so that what a lane gets of a row's
+// tiles are columns of one row (RT 4; RT 8: of two) and the largest of them is found without a look at other lanes.
+template <int RT>
+__device__ __forceinline__ uint32_t column_place(uint32_t row, uint32_t c, uint32_t rowColumns) {
+    constexpr uint32_t kEach = 8 / RT;
+    return (row / RT * (rowColumns / kEach) + c / kEach) * 8 + row % RT * kEach + c % kEach;
 }
-// more: by all warps, with a barrier between
-template <int DIM>
+// a row's columns, up to eight, by one warp
+template <int DIM, int RT, int COLUMNS>
+__device__ __forceinline__ void select_stage(const SelectArgs &a, uint32_t row0, uint32_t row, uint32_t head, uint8_t *to) {
+    const uint32_t group = a.heads / a.kvHeads;
+    const uint16_t *src = a.q + (size_t)(row0 + row) * a.qStride + (size_t)head * group * DIM;
+    Query<DIM> q[COLUMNS];
+    int exponent[COLUMNS], top = -100;
+#pragma unroll
+    for (int c = 0; c < COLUMNS; ++c) q[c].load(src + min((uint32_t)c, group - 1u) * DIM);
+#pragma unroll
+    for (int c = 0; c < COLUMNS; ++c) top = max(top, exponent[c] = q[c].exponent());
+#pragma unroll
+    for (int c = 0; c < COLUMNS; ++c) q[c].store(to + column_place<RT>(row, c, COLUMNS) * select_query_stride(DIM), exponent[c], top);
+}
+// any number, by all warps, with a barrier between
+template <int DIM, int RT>
 __device__ __forceinline__ void select_stage_wide(const SelectArgs &a, SelectRows &s, uint32_t row0, uint32_t rows, uint32_t head, uint8_t *to, uint32_t warps) {
     const uint32_t lane = threadIdx.x & 31u, warp = threadIdx.x >> 5, group = a.heads / a.kvHeads, columns = rows * a.rowColumns;
     auto column = [&](uint32_t c) { return a.q + (size_t)(row0 + c / a.rowColumns) * a.qStride + (size_t)(head * group + min(c % a.rowColumns, group - 1u)) * DIM; };
@@ -295,16 +301,16 @@ __device__ __forceinline__ void select_stage_wide(const SelectArgs &a, SelectRow
         q.load(column(c));
         int top = -100;
         for (uint32_t k = lane; k < a.rowColumns; k += 32) top = max(top, s.exponents[c / a.rowColumns * a.rowColumns + k]);
-        q.store(to + c * select_query_stride(DIM), s.exponents[c], __reduce_max_sync(0xFFFFFFFFu, top));
+        q.store(to + column_place<RT>(c / a.rowColumns, c % a.rowColumns, a.rowColumns) * select_query_stride(DIM), s.exponents[c], __reduce_max_sync(0xFFFFFFFFu, top));
     }
 }
 // Scores of request r's blocks below `end`, in whole numbers of their order, to scores[row of the CTA * stride + block] for rows i0 .. i1 - 1
-// (REMOTE: in another CTA's shared memory): sixteen at a time from 16 tile on, 16 step apart.
-template <int DIM, int LOG, bool REMOTE>
+// (REMOTE: in another CTA's shared memory): sixteen at a time from 16 tile on, 16 step apart.  TILES: of eight columns for RT rows, 0 for any number.
+template <int DIM, int RT, int TILES, bool REMOTE>
 __device__ __forceinline__ void select_score(const SelectArgs &a, const uint8_t *queries, uint32_t head, uint32_t r, uint32_t end, uint32_t tile, uint32_t step, uint32_t i0, uint32_t i1,
                                              uint32_t scores, uint32_t stride) {
-    constexpr uint32_t kChunks = DIM / 32, kRowsOfTile = 8 >> LOG;
-    const uint32_t lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u, perPage = max(1u, (1u << a.pageShift) >> kBlockShift), tilesOfRow = LOG == 3 ? a.rowColumns / 8 : 1u;
+    constexpr uint32_t kChunks = DIM / 32;
+    const uint32_t lane = threadIdx.x & 31u, g = lane >> 2, t = lane & 3u, perPage = max(1u, (1u << a.pageShift) >> kBlockShift), tiles = TILES ? TILES : a.rowColumns * RT / 8;
     auto page_of = [&](uint32_t base) {  // of the mean of block base + lane % 16
         const uint32_t b = base + (lane & 15u);
         return b < end ? __ldg(a.blockTable + (size_t)r * a.tableStride + (((b << kBlockShift) + kTileKeys - 1u) >> a.pageShift)) : 0u;
@@ -324,10 +330,11 @@ __device__ __forceinline__ void select_score(const SelectArgs &a, const uint8_t 
         pageNext = page_of(base + 16 * step);
         const uint32_t gone = __ballot_sync(0xFFFFFFFFu, outside);
         if (gone && lane == 0) *a.errorFlag = kFlagPage;
-        for (uint32_t i = i0 / kRowsOfTile * kRowsOfTile; i < i1; i += kRowsOfTile) {
-            const uint8_t *from = queries + (i / kRowsOfTile * tilesOfRow * 8 + g) * select_query_stride(DIM) + 16 * t;
+        for (uint32_t i = i0 / RT * RT; i < i1; i += RT) {
+            const uint8_t *from = queries + (i / RT * tiles * 8 + g) * select_query_stride(DIM) + 16 * t;
             float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};  // [block g: column 2 t, 2 t + 1; block g + 8: likewise]
-            for (uint32_t n = 0; n < tilesOfRow; ++n) {
+#pragma unroll
+            for (uint32_t n = 0; n < tiles; ++n) {
                 float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (uint32_t c = 0; c < kChunks; ++c) {
@@ -336,23 +343,28 @@ __device__ __forceinline__ void select_score(const SelectArgs &a, const uint8_t 
                     mma_bf16(acc, v[0][c].z, v[1][c].z, v[0][c].w, v[1][c].w, b.z, b.w);
                 }
 #pragma unroll
-                for (int k = 0; k < 4; ++k) best[k] = LOG == 3 ? max_nan(best[k], acc[k]) : acc[k];
+                for (int k = 0; k < 4; ++k) best[k] = max_nan(best[k], acc[k]);
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                float x = best[2 * h];
-                if (LOG > 0) x = max_nan(x, best[2 * h + 1]);
-                if (LOG > 1) x = max_nan(x, __shfl_xor_sync(0xFFFFFFFFu, x, 1));
-                if (LOG > 2) x = max_nan(x, __shfl_xor_sync(0xFFFFFFFFu, x, 2));
                 const uint32_t b = base + g + 8 * h;
                 const bool none = gone >> (g + 8 * h) & 1u;
-                if (b >= end || (LOG > 0 && (2 * t) & ((1 << LOG) - 1))) continue;
-#pragma unroll
-                for (int k = 0; k < (LOG == 0 ? 2 : 1); ++k) {
-                    const uint32_t row = i + (2 * t >> LOG) + k, order = none ? 0u : order_of(LOG == 0 ? best[2 * h + k] : x);
-                    if (row < i0 || row >= i1) continue;
+                auto put = [&](uint32_t row, float x) {
+                    const uint32_t order = none ? 0u : order_of(x);
+                    if (b >= end || row < i0 || row >= i1) return;
                     if (REMOTE) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(scores + 4 * (row * stride + b)), "r"(order) : "memory");
                     else asm volatile("st.shared.u32 [%0], %1;" ::"r"(scores + 4 * (row * stride + b)), "r"(order) : "memory");
+                };
+                if (RT == 8) {
+                    put(i + 2 * t, best[2 * h]);
+                    put(i + 2 * t + 1, best[2 * h + 1]);
+                } else {
+                    float x = max_nan(best[2 * h], best[2 * h + 1]);
+                    if (RT == 1) {
+                        x = max_nan(x, __shfl_xor_sync(0xFFFFFFFFu, x, 1));
+                        x = max_nan(x, __shfl_xor_sync(0xFFFFFFFFu, x, 2));
+                    }
+                    if (RT == 4 || t == 0) put(i + (RT == 4 ? t : 0u), x);
                 }
             }
         }
@@ -361,7 +373,7 @@ __device__ __forceinline__ void select_score(const SelectArgs &a, const uint8_t 
 
 // The `wanted` largest of n scores (more than wanted), of equal ones the first, by WARPS warps: ids first + place, ascending, to out.
 struct SelectCounts {
-    uint32_t bins[2][kBins];  // of this level, of the next
+    __align__(16) uint32_t bins[2][kBins];  // of this level, of the next
     uint2 few[kFew];          // score, place
     uint32_t least[2][16], most[2][16], above[16], same[16], held;  // of each warp
 };
@@ -405,7 +417,11 @@ __device__ __forceinline__ void select_largest(const uint32_t *scores, uint32_t 
         // the range that holds the last one wanted: a lane has eight, the uppermost lane the last
         uint32_t counts[kBins / 32], sum = 0;
 #pragma unroll
-        for (uint32_t i = 0; i < kBins / 32; ++i) sum += counts[i] = bins[lane * (kBins / 32) + i];
+        for (uint32_t i = 0; i < kBins / 32; i += 4) {
+            const uint4 four = *reinterpret_cast<const uint4 *>(bins + lane * (kBins / 32) + i);
+            counts[i] = four.x, counts[i + 1] = four.y, counts[i + 2] = four.z, counts[i + 3] = four.w;
+            sum += four.x + four.y + four.z + four.w;
+        }
         for (uint32_t k = thread; k < kBins; k += 32 * WARPS) s.bins[~level & 1u][k] = 0u;
         uint32_t above = sum;  // in this lane's ranges and above
 #pragma unroll
@@ -464,7 +480,7 @@ __device__ __forceinline__ void select_largest(const uint32_t *scores, uint32_t 
         above = __reduce_add_sync(0xFFFFFFFFu, above), same = __reduce_add_sync(0xFFFFFFFFu, same);
         if (lane == 0) s.above[warp] = above, s.same[warp] = same;
         select_meet<WARPS>();
-        const bool front = lane < warp;
+        const bool front = (int)lane < (int)warp;
         aboveBefore = __reduce_add_sync(0xFFFFFFFFu, front ? s.above[lane % WARPS] : 0u), sameBefore = __reduce_add_sync(0xFFFFFFFFu, front ? s.same[lane % WARPS] : 0u);
     }
     const uint32_t under = (1u << lane) - 1u;
@@ -490,12 +506,9 @@ __device__ __forceinline__ bool select_always(const SelectArgs &a, uint32_t *out
     return a.blocks == a.first + a.last;
 }
 
-// warps of k_select_split: at 256 values a head a warp's registers leave room for eight
-__host__ __device__ constexpr uint32_t split_warps(int dim) { return dim == 256 ? 8u : 16u; }
-
-template <int DIM, int LOG>
-__global__ void __launch_bounds__(32 * split_warps(DIM)) k_select_split(const __grid_constant__ SelectArgs a) {
-    constexpr uint32_t kWarps = split_warps(DIM);
+template <int DIM, int TILES, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) k_select_split(const __grid_constant__ SelectArgs a) {
+    constexpr uint32_t kWarps = WARPS;
     extern __shared__ __align__(16) uint8_t selectSmem[];
     __shared__ SelectRows s;
     __shared__ SelectCounts counts;
@@ -506,19 +519,32 @@ __global__ void __launch_bounds__(32 * split_warps(DIM)) k_select_split(const __
     pdl_enter();
     if (ctas > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");  // (the first CTA is there to be written to: waited for below)
     __syncthreads();
-    const bool wide = LOG == 3 && a.rowColumns > 8;
-    if (!wide && warp == 0) select_stage<DIM, LOG>(a, row, head, selectSmem);
-    if (!wide && warp == 1 && LOG < 3)  // (columns of no row)
-        for (uint32_t k = tid & 31u; k < (8 - (1 << LOG)) * select_query_stride(DIM) / 4; k += 32) reinterpret_cast<uint32_t *>(selectSmem + (1 << LOG) * select_query_stride(DIM))[k] = 0u;
-    if (wide) select_stage_wide<DIM>(a, s, row, 1, head, selectSmem, kWarps);
-    select_look_up(a, s, row, 1, (tid + 32 * (kWarps - 2)) % (32 * kWarps), 32 * kWarps);  // (from the third warp on: the first has something to do)
+    // a warp a column, where there are no more: its exponent in front of the look at the requests, the numbers behind
+    [[maybe_unused]] Query<DIM> q;
+    [[maybe_unused]] int exponent = kNoNumber;
+    if (TILES == 1 && warp < 8) {
+        q.load(a.q + (size_t)row * a.qStride + (size_t)(head * (a.heads / a.kvHeads) + min(warp, a.heads / a.kvHeads - 1u)) * DIM);
+        exponent = q.exponent();
+        if ((tid & 31u) == 0) s.exponents[warp] = exponent;
+    }
+    if (TILES != 1) select_stage_wide<DIM, 1>(a, s, row, 1, head, selectSmem, kWarps);
+    select_look_up(a, s, row, 1, (tid + 32 * (kWarps - 8)) % (32 * kWarps), 32 * kWarps);  // (from the ninth warp on, where there is one)
     __syncthreads();
+    if (TILES == 1) {
+        if (warp < 8) {
+            int top = -100;
+#pragma unroll
+            for (int c = 0; c < 8; ++c) top = max(top, s.exponents[c]);
+            q.store(selectSmem + warp * select_query_stride(DIM), exponent, top);
+        }
+        __syncthreads();
+    }
     if (ctas > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     const uint32_t seen = s.seen[0], wanted = a.blocks - a.first - a.last;
     if (seen > a.blocks && wanted) {
         const uint32_t tile = cta * kWarps + warp, step = ctas * kWarps;
-        if (cta) select_score<DIM, LOG, true>(a, selectSmem, head, s.request[0], seen - a.last, tile, step, 0, 1, map_to_cta(sm_addr(scores), 0), 0);
-        else select_score<DIM, LOG, false>(a, selectSmem, head, s.request[0], seen - a.last, tile, step, 0, 1, sm_addr(scores), 0);
+        if (cta) select_score<DIM, 1, TILES, true>(a, selectSmem, head, s.request[0], seen - a.last, tile, step, 0, 1, map_to_cta(sm_addr(scores), 0), 0);
+        else select_score<DIM, 1, TILES, false>(a, selectSmem, head, s.request[0], seen - a.last, tile, step, 0, 1, sm_addr(scores), 0);
     }
     if (ctas > 1) cluster_sync_all();
     else __syncthreads();
@@ -528,8 +554,8 @@ __global__ void __launch_bounds__(32 * split_warps(DIM)) k_select_split(const __
     select_largest<kWarps>(scores + a.first, seen - a.last - a.first, wanted, a.first, out + a.first, counts);
 }
 
-template <int DIM, int LOG>
-__global__ void __launch_bounds__(32 * kRowsWarps) k_select_rows(const __grid_constant__ SelectArgs a) {
+template <int DIM, int RT, int TILES>
+__global__ void __launch_bounds__(32 * kRowsWarps, DIM == 256 ? 2 : DIM == 128 ? 3 : 4) k_select_rows(const __grid_constant__ SelectArgs a) {
     extern __shared__ __align__(16) uint8_t selectSmem[];
     __shared__ SelectRows s;
     __shared__ SelectCounts counts[kRowsWarps];
@@ -540,10 +566,8 @@ __global__ void __launch_bounds__(32 * kRowsWarps) k_select_rows(const __grid_co
     pdl_enter();
     __syncthreads();
     const uint32_t wanted = a.blocks - a.first - a.last;
-    if (LOG == 3 && a.rowColumns > 8) select_stage_wide<DIM>(a, s, row0, rows, head, selectSmem, kRowsWarps);
-    else if (warp < rows) select_stage<DIM, LOG>(a, row0 + warp, head, selectSmem + (warp << LOG) * select_query_stride(DIM));
-    else if ((warp << LOG) < a.columns)  // (columns of no row)
-        for (uint32_t k = lane; k < (select_query_stride(DIM) << LOG) / 4; k += 32) reinterpret_cast<uint32_t *>(selectSmem + (warp << LOG) * select_query_stride(DIM))[k] = 0u;
+    if (TILES == 0) select_stage_wide<DIM, RT>(a, s, row0, rows, head, selectSmem, kRowsWarps);
+    else if (warp < rows) select_stage<DIM, RT, (TILES ? TILES : 1) * 8 / RT>(a, row0, warp, head, selectSmem);
     select_look_up(a, s, row0, rows, tid, 32 * kRowsWarps);
     __syncthreads();
     for (uint32_t i0 = 0, i1; i0 < rows; i0 = i1) {  // request by request
@@ -551,7 +575,7 @@ __global__ void __launch_bounds__(32 * kRowsWarps) k_select_rows(const __grid_co
         for (i1 = i0; i1 < rows && s.request[i1] == s.request[i0]; ++i1)
             if (s.seen[i1] > a.blocks) end = max(end, s.seen[i1] - a.last);
         if (s.request[i0] == FF_NO_SLOT || !wanted) continue;
-        select_score<DIM, LOG, false>(a, selectSmem, head, s.request[i0], end, warp, kRowsWarps, i0, i1, sm_addr(scores), a.tableBlocks);
+        select_score<DIM, RT, TILES, false>(a, selectSmem, head, s.request[i0], end, warp, kRowsWarps, i0, i1, sm_addr(scores), a.tableBlocks);
     }
     __syncthreads();
     if (warp >= rows) return;
@@ -561,7 +585,7 @@ __global__ void __launch_bounds__(32 * kRowsWarps) k_select_rows(const __grid_co
     select_largest<1>(scores + warp * a.tableBlocks + a.first, seen - a.last - a.first, wanted, a.first, out + a.first, counts[warp]);
 }
 
-KernelSmemMemo selectMemo[2][3][4];
+KernelSmemMemo splitMemo[3][4], rowsMemo[3][6];
 
 }  // namespace
 
@@ -581,29 +605,24 @@ bool launch_select_blocks(FFAttention *att, const uint16_t *q, uint32_t qStride,
                           uint32_t requests, uint32_t blocks, uint32_t first, uint32_t last, uint32_t *ids, cudaStream_t stream, const char **error) {
     const FFAttentionConfig &c = att->cfg;
     const uint32_t group = c.heads / c.kvHeads, sms = (uint32_t)att->smCount;
-    uint32_t rowColumns = group > 8 ? (group + 7u) & ~7u : 1u;
-    while (rowColumns < group) rowColumns *= 2;
     SelectArgs args{q, qStride, tokens, means, pageCount, blockTable, tableStride, tableBlocks, rowStart, lengths, requests, c.heads, c.kvHeads,
-                    (uint32_t)__builtin_ctz(c.pageTokens), blocks, first, last, ids, 1, rowColumns, 0, att->errorFlag};
+                    (uint32_t)__builtin_ctz(c.pageTokens), blocks, first, last, ids, 1, (group + 7u) & ~7u, 0, att->errorFlag};
     const uint64_t lists = (uint64_t)tokens * c.kvHeads;
-    const int dim = c.headDim == 256 ? 2 : c.headDim == 128 ? 1 : 0, log = rowColumns >= 8 ? 3 : __builtin_ctz(rowColumns);
-    auto of_shape = [&](auto launch) {  // launch(values of a head, columns of a row as a power of two), as constants
-        auto of_dim = [&](auto d) {
-            return log == 3 ? launch(d, std::integral_constant<int, 3>()) : log == 2 ? launch(d, std::integral_constant<int, 2>())
-                 : log == 1 ? launch(d, std::integral_constant<int, 1>()) : launch(d, std::integral_constant<int, 0>());
-        };
-        return dim == 2 ? of_dim(std::integral_constant<int, 256>()) : dim == 1 ? of_dim(std::integral_constant<int, 128>()) : of_dim(std::integral_constant<int, 64>());
+    const int dim = c.headDim == 256 ? 2 : c.headDim == 128 ? 1 : 0;
+    auto of_dim = [&](auto launch) {  // launch(values of a head, as a constant)
+        return dim == 2 ? launch(std::integral_constant<int, 256>()) : dim == 1 ? launch(std::integral_constant<int, 128>()) : launch(std::integral_constant<int, 64>());
     };
-    if (lists <= 4ull * sms) {
-        // CTAs to fill the GPU, as long as each of them has its warps' blocks
-        const uint32_t warps = split_warps((int)c.headDim);
+    // A cluster a list where lists are few, or most rows another request's: these have no means in common.
+    if (lists <= 4ull * sms || ((uint64_t)tokens < 4ull * requests && tokens <= 65535)) {
+        // Sixteen warps where a CTA has an SM for itself (at 256 values a head their registers leave room for eight); CTAs to fill
+        // the GPU, as long as each of them has its warps' blocks.
+        const uint32_t warps = lists <= sms && dim < 2 ? 16u : 8u;
         uint32_t ctas = 1;
-        while (ctas < kMostSplit && 2 * ctas * lists <= 2 * sms && 2 * ctas * warps * 16 <= tableBlocks) ctas *= 2;
-        args.columns = std::max(8u, rowColumns);
+        while (ctas < kMostSplit && 2 * ctas * lists <= (warps == 16 ? sms : 2 * sms) && 2 * ctas * warps * 16 <= tableBlocks) ctas *= 2;
+        args.columns = args.rowColumns;
         const uint32_t smem = select_smem(c.headDim, args.columns, 1, tableBlocks);
-        return of_shape([&](auto d, auto l) {
-            const auto kernel = k_select_split<d.value, l.value>;
-            if (!selectMemo[0][dim][log].prepare(kernel, att->device, smem, 32 * warps, nullptr, error)) return false;
+        auto launch = [&](auto kernel, KernelSmemMemo &memo) {
+            if (!memo.prepare(kernel, att->device, smem, 32 * warps, nullptr, error)) return false;
             cudaLaunchConfig_t config{};
             config.gridDim = dim3(ctas, tokens, c.kvHeads);
             config.blockDim = dim3(32 * warps);
@@ -618,17 +637,33 @@ bool launch_select_blocks(FFAttention *att, const uint16_t *q, uint32_t qStride,
             config.attrs = attributes;
             config.numAttrs = 2;
             return launched(att, cudaLaunchKernelEx(&config, kernel, args), "k_select_split", error);
+        };
+        return of_dim([&](auto d) {
+            constexpr int kMost = d.value == 256 ? 8 : 16;
+            const bool one = args.rowColumns == 8;
+            if (warps == 16) return one ? launch(k_select_split<d.value, 1, kMost>, splitMemo[dim][0]) : launch(k_select_split<d.value, 0, kMost>, splitMemo[dim][1]);
+            return one ? launch(k_select_split<d.value, 1, 8>, splitMemo[dim][2]) : launch(k_select_split<d.value, 0, 8>, splitMemo[dim][3]);
         });
     }
     // A warp's list each, as far as the columns and the shared memory for their scores go.
-    args.rows = std::min(kRowsWarps, kSelectColumns / rowColumns);
-    while (args.rows > 1 && select_smem(c.headDim, std::max(8u, args.rows * rowColumns), args.rows, tableBlocks) > 100u * 1024u) args.rows /= 2;
-    args.columns = std::max(8u, args.rows * rowColumns);
-    const uint32_t smem = select_smem(c.headDim, args.columns, args.rows, tableBlocks);
-    return of_shape([&](auto d, auto l) {
-        const auto kernel = k_select_rows<d.value, l.value>;
-        if (!selectMemo[1][dim][log].prepare(kernel, att->device, smem, 32 * kRowsWarps, nullptr, error)) return false;
+    uint32_t narrow = group > 8 ? args.rowColumns : 1u;
+    while (narrow < group) narrow *= 2;
+    args.rows = std::min(kRowsWarps, kSelectColumns / narrow);
+    while (args.rows > 1 && select_smem(c.headDim, std::max(8u, args.rows * narrow), args.rows, tableBlocks) > 100u * 1024u) args.rows /= 2;
+    const uint32_t together = args.rows < 4 ? 1u : narrow == 1 && args.rows == 8 ? 8u : 4u;  // rows of a tile of columns
+    if (together > 1) args.rowColumns = std::max(narrow, 8u / together);
+    args.rows = args.rows / together * together;
+    args.columns = args.rows * args.rowColumns;
+    const uint32_t smem = select_smem(c.headDim, args.columns, args.rows, tableBlocks), tiles = args.rowColumns * together / 8;
+    auto launch = [&](auto kernel, KernelSmemMemo &memo) {
+        if (!memo.prepare(kernel, att->device, smem, 32 * kRowsWarps, nullptr, error)) return false;
         return launched(att, launch_pdl(kernel, dim3((tokens + args.rows - 1) / args.rows, c.kvHeads), dim3(32 * kRowsWarps), smem, stream, args), "k_select_rows", error);
+    };
+    return of_dim([&](auto d) {
+        if (together == 8) return launch(k_select_rows<d.value, 8, 1>, rowsMemo[dim][0]);
+        if (together == 1) return launch(k_select_rows<d.value, 1, 0>, rowsMemo[dim][1]);
+        return tiles == 1 ? launch(k_select_rows<d.value, 4, 1>, rowsMemo[dim][2]) : tiles == 2 ? launch(k_select_rows<d.value, 4, 2>, rowsMemo[dim][3])
+             : tiles == 4 ? launch(k_select_rows<d.value, 4, 4>, rowsMemo[dim][4]) : launch(k_select_rows<d.value, 4, 0>, rowsMemo[dim][5]);
     });
 }
 
