@@ -14,9 +14,10 @@ constexpr int kLeastExponent = -60, kMostExponent = 60;  // of a mean's largest 
 
 // ---- mean keys -----------------------------------------------------------------------------------
 
-// A warp takes a block of a key/value head: 64 keys of code * scale + bias summed in 64 bits, where the sum is exact unless the
-// scales of a block are 2^35 apart; then whole numbers of 2^(e - 6), e the exponent of the largest value: 7 bits and a sign, which
-// bf16 holds.  So nothing about a mean depends on the order of sums.
+// A warp takes a block of a key/value head, 64 keys of code * scale + bias, 32 codes a lane and load.  Where the scales are no more than 2^6
+// apart the products' sum is exact in 32 bits (a code times a scale has 12 bits, 64 of them 18); other blocks are summed in 64 bits, as the
+// biases are, exact unless the scales are 2^35 apart.  Then whole numbers of 2^(e - 6), e the exponent of the largest value: 7 bits and a sign,
+// which bf16 holds.  So nothing about a mean depends on the order of sums.
 constexpr int kMeansThreads = 256;
 
 struct MeansArgs {
@@ -31,10 +32,49 @@ struct MeansArgs {
     uint32_t *errorFlag;
 };
 
+__device__ __forceinline__ unsigned long long pair_f32(float a, float b) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ unsigned long long pair_u32(uint32_t a, uint32_t b) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(a), "r"(b));
+    return r;
+}
+__device__ __forceinline__ unsigned long long fma_f32x2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ unsigned long long add_f32x2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// 32 values a lane, of lanes `lanes` apart up to 32, added up: each round a lane gives half of what it has and takes the other half of its
+// partner's; the first values are then the lane's, `at` of those 32 where they begin.
+template <int LANES, typename T>
+__device__ __forceinline__ uint32_t join_lanes(T (&value)[32]) {
+    uint32_t at = 0;
+    int half = 16;
+#pragma unroll
+    for (uint32_t mask = LANES; mask < 32; mask *= 2, half /= 2) {
+        const bool upper = threadIdx.x & mask;
+        if (upper) at += half;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            if (i >= half) break;
+            const T give = upper ? value[i] : value[i + half], keep = upper ? value[i + half] : value[i];
+            value[i] = keep + __shfl_xor_sync(0xFFFFFFFFu, give, mask);
+        }
+    }
+    return at;
+}
 template <int DIM>
-__global__ void __launch_bounds__(kMeansThreads) k_block_means(const __grid_constant__ MeansArgs a) {
-    constexpr uint32_t CB = DIM / 2, NG = DIM / 64, kLanes = CB / 8, kKeys = 32 / kLanes;  // lanes a key, keys at once
-    constexpr int kRounds = kKeys == 8 ? 3 : kKeys == 4 ? 2 : 1, kMine = 16 >> kRounds;
+__global__ void __launch_bounds__(kMeansThreads, 2) k_block_means(const __grid_constant__ MeansArgs a) {
+    constexpr uint32_t CB = DIM / 2, NG = DIM / 64, kLanes = CB / 16, kKeys = 32 / kLanes;  // lanes a key, keys at once
+    constexpr int kSteps = kTileKeys / kKeys, kAtOnce = kSteps < 8 ? kSteps : 8, kMine = 32 / kKeys;  // loads of a block, in flight; values of a mean that are a lane's
     __shared__ uint32_t first[kMeansThreads + 1], warpSums[kMeansThreads / 32];
     const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
     pdl_enter();
@@ -104,60 +144,101 @@ __global__ void __launch_bounds__(kMeansThreads) k_block_means(const __grid_cons
         const uint32_t lastPage = __shfl_sync(0xFFFFFFFFu, page, pieces - 1u);
         if (hole && lane == 0) *a.errorFlag = kFlagPage;
         if (lastPage >= a.pageCount) continue;
-        double value[16], bias = 0.0;
+        // key k * kKeys + keyLane of the block: its codes, its word
+        auto block_of = [&](int k) {
+            const uint32_t key = k * kKeys + keyLane;
+            return a.pages + ((size_t)__shfl_sync(0xFFFFFFFFu, page, key >> pieceShift) * a.kvHeads + head) * a.page.blockBytes;
+        };
+        auto at_of = [&](int k) { return (key0 + k * kKeys + keyLane) & (pageTokens - 1u); };
+        uint32_t words[kSteps], most = 0, least = 0xFFu, at;  // exponents of the scales
+        double bias = 0.0, mean[kMine];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) value[i] = 0.0;
-        if (!hole) {
-#pragma unroll 4
-            for (uint32_t k = 0; k < kTileKeys / kKeys; ++k) {
-                const uint32_t key = k * kKeys + keyLane;
-                const uint32_t at = (key0 + key) & (pageTokens - 1u);
-                const uint8_t *block = a.pages + ((size_t)__shfl_sync(0xFFFFFFFFu, page, key >> pieceShift) * a.kvHeads + head) * a.page.blockBytes;
-                const uint2 codes = __ldg(reinterpret_cast<const uint2 *>(block + (size_t)at * CB + inKey * 8));
-                const uint32_t word = __ldg(reinterpret_cast<const uint32_t *>(block + a.page.keyWords + (size_t)at * (NG * 4)) + inKey / (kLanes / NG));
-                const double scale = (double)low16(word);
-                bias += (double)high16(word);
+        for (int k = 0; k < kSteps; ++k) words[k] = hole ? 0u : __ldg(reinterpret_cast<const uint32_t *>(block_of(k) + a.page.keyWords + (size_t)at_of(k) * (NG * 4)) + inKey / (kLanes / NG));
+        auto codes_of = [&](int k) { return hole ? make_uint4(0u, 0u, 0u, 0u) : __ldg(reinterpret_cast<const uint4 *>(block_of(k) + (size_t)at_of(k) * CB) + inKey); };
+        uint4 codes[kAtOnce];
 #pragma unroll
-                for (int i = 0; i < 16; ++i)  // (2^52 + code less 2^52: a conversion takes longer)
-                    value[i] = fma(scale, __hiloint2double(0x43300000, (int)((i < 8 ? codes.x : codes.y) >> (4 * (i & 7)) & 15u)) - 0x1p52, value[i]);
+        for (int k = 0; k < kAtOnce; ++k) codes[k] = codes_of(k);
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+            const uint32_t e = words[k] >> 7 & 0xFFu;
+            most = max(most, e);
+            if (words[k] & 0x7FFFu) least = min(least, max(e, 1u));
+            bias += (double)high16(words[k]);
+        }
+        most = __reduce_max_sync(0xFFFFFFFFu, most), least = __reduce_min_sync(0xFFFFFFFFu, least);
+        if (most < 0xFFu && most <= least + 6u) {
+            // Nibbles i and i + 4 of a word, masked in place: 2^23 + 16^i code, less 2^23, times the scale / 16^i; two codes an instruction.
+            unsigned long long sums[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sums[i] = pair_f32(0.0f, 0.0f);
+            const unsigned long long less = pair_f32(-8388608.0f, -8388608.0f);
+#pragma unroll
+            for (int k0 = 0; k0 < kSteps; k0 += kAtOnce) {
+#pragma unroll
+                for (int k = 0; k < kAtOnce; ++k) {
+                    const float scale = low16(words[k0 + k]);
+                    const uint32_t word[4] = {codes[k].x, codes[k].y, codes[k].z, codes[k].w};
+                    if (k0 + kAtOnce < kSteps) codes[k] = codes_of(k0 + kAtOnce + k);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float down = scale * (i == 0 ? 1.0f : i == 1 ? 0x1p-4f : i == 2 ? 0x1p-8f : 0x1p-12f);
+                        const unsigned long long factor = pair_f32(down, down);
+                        const uint32_t mask = 15u << (4 * i);
+#pragma unroll
+                        for (int w = 0; w < 4; ++w)
+                            sums[4 * w + i] = fma_f32x2(add_f32x2(pair_u32((word[w] & mask) | 0x4B000000u, (word[w] >> 16 & mask) | 0x4B000000u), less), factor, sums[4 * w + i]);
+                    }
+                }
             }
+            float value[32];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) value[8 * (i / 4) + i % 4] = __uint_as_float((uint32_t)sums[i]), value[8 * (i / 4) + i % 4 + 4] = __uint_as_float((uint32_t)(sums[i] >> 32));
+            at = join_lanes<kLanes>(value);
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) mean[i] = value[i];
+        } else {
+            double value[32];
+#pragma unroll
+            for (int i = 0; i < 32; ++i) value[i] = 0.0;
+#pragma unroll 1
+            for (int k = 0; k < kSteps; ++k) {
+                const uint4 four = codes_of(k);
+                const uint32_t word[4] = {four.x, four.y, four.z, four.w};
+                const double scale = (double)low16(__ldg(reinterpret_cast<const uint32_t *>(block_of(k) + a.page.keyWords + (size_t)at_of(k) * (NG * 4)) + inKey / (kLanes / NG)));
+#pragma unroll
+                for (int i = 0; i < 32; ++i)  // (2^52 + code less 2^52: a conversion takes longer)
+                    value[i] = fma(scale, __hiloint2double(0x43300000, (int)(word[i / 8] >> (4 * (i & 7)) & 15u)) - 0x1p52, value[i]);
+            }
+            at = join_lanes<kLanes>(value);
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) mean[i] = value[i];
         }
 #pragma unroll
-        for (int i = 0; i < 16; ++i) value[i] += bias;
-        // the keys' lanes joined: each round a lane gives half of its values and takes the other half's of its partner
-        uint32_t at = 16 * inKey;
+        for (uint32_t mask = kLanes; mask < 32; mask *= 2) bias += __shfl_xor_sync(0xFFFFFFFFu, bias, mask);
+        at += 32 * inKey;
+        most = 0;
 #pragma unroll
-        for (int round = 0; round < kRounds; ++round) {
-            const int half = 8 >> round;
-            const uint32_t mask = kLanes << round;
-            const bool upper = lane & mask;
-            if (upper) at += half;
-#pragma unroll
-            for (int i = 0; i < half; ++i) {
-                const double give = upper ? value[i] : value[i + half], keep = upper ? value[i + half] : value[i];
-                value[i] = keep + __shfl_xor_sync(0xFFFFFFFFu, give, mask);
-            }
+        for (int i = 0; i < kMine; ++i) {
+            mean[i] += bias;
+            most = max(most, (uint32_t)__double2hiint(mean[i]) & 0x7FF00000u);
         }
-        uint32_t most = 0;
-#pragma unroll
-        for (int i = 0; i < kMine; ++i) most = max(most, (uint32_t)__double2hiint(value[i]) & 0x7FF00000u);
         most = __reduce_max_sync(0xFFFFFFFFu, most) >> 20;
         const bool broken = most == 0x7FFu;
         const int e = min(max((int)most - 1023 - 6, kLeastExponent), kMostExponent);  // (the mean is the sum / 64)
         const double down = __hiloint2double((1023 - e) << 20, 0);
         const float up = power_of_two(e - 6);
-        uint32_t out[(kMine + 1) / 2];
+        uint32_t out[kMine / 2];
 #pragma unroll
         for (int i = 0; i < kMine; i += 2) {
             float v[2];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) v[k] = broken ? NAN : (float)fmin(fmax(rint(value[i + k] * down), -127.0), 127.0) * up;
+            for (int k = 0; k < 2; ++k) v[k] = broken ? NAN : (float)fmin(fmax(rint(mean[i + k] * down), -127.0), 127.0) * up;
             out[i / 2] = pack_bf16x2(v[0], v[1]);
         }
         const uint32_t perPage = max(1u, pageTokens >> kBlockShift), place = (key0 & (pageTokens - 1u)) >> kBlockShift;
         uint16_t *to = a.means + (((size_t)lastPage * a.kvHeads + head) * perPage + (pageTokens > kTileKeys ? place : 0u)) * DIM + at;
-        if (kMine == 8) *reinterpret_cast<uint4 *>(to) = make_uint4(out[0], out[1 % ((kMine + 1) / 2)], out[2 % ((kMine + 1) / 2)], out[3 % ((kMine + 1) / 2)]);
-        else if (kMine == 4) *reinterpret_cast<uint2 *>(to) = make_uint2(out[0], out[1 % ((kMine + 1) / 2)]);
+        if (kMine == 8) *reinterpret_cast<uint4 *>(to) = make_uint4(out[0], out[1 % (kMine / 2)], out[2 % (kMine / 2)], out[3 % (kMine / 2)]);
+        else if (kMine == 4) *reinterpret_cast<uint2 *>(to) = make_uint2(out[0], out[1 % (kMine / 2)]);
         else *reinterpret_cast<uint32_t *>(to) = out[0];
     }
 }
@@ -595,7 +676,7 @@ bool launch_block_means(FFAttention *att, const uint8_t *pages, uint32_t pageCou
     const MeansArgs args{pages, pageCount, blockTable, tableStride, tableKeys, oldLengths, newLengths, requests, c.kvHeads, (uint32_t)__builtin_ctz(c.pageTokens),
                          page_layout(c), means, att->errorFlag};
     const uint64_t most = ((uint64_t)requests * (tableKeys / kTileKeys) * c.kvHeads + kMeansThreads / 32 - 1) / (kMeansThreads / 32);
-    const uint32_t grid = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(most, 4u * (uint32_t)att->smCount));
+    const uint32_t grid = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(most, 2u * (uint32_t)att->smCount));
     auto launch = [&](auto kernel) { return launched(att, launch_pdl(kernel, dim3(grid), dim3(kMeansThreads), 0, stream, args), "k_block_means", error); };
     return c.headDim == 256 ? launch(k_block_means<256>) : c.headDim == 128 ? launch(k_block_means<128>) : launch(k_block_means<64>);
 }
