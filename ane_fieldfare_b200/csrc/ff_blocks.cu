@@ -18,7 +18,8 @@ constexpr int kLeastExponent = -60, kMostExponent = 60;  // of a mean's largest 
 // apart the products' sum is exact in 32 bits (a code times a scale has 12 bits, 64 of them 18); other blocks are summed in 64 bits, as the
 // biases are, exact unless the scales are 2^35 apart.  Then whole numbers of 2^(e - 6), e the exponent of the largest value: 7 bits and a sign,
 // which bf16 holds.  So nothing about a mean depends on the order of sums.
-constexpr int kMeansThreads = 256;
+constexpr int kMeansThreads = 512;
+constexpr uint32_t kMeansWaitLimit = 1u << 20;
 
 struct MeansArgs {
     const uint8_t *pages;
@@ -71,12 +72,22 @@ __device__ __forceinline__ uint32_t join_lanes(T (&value)[32]) {
     }
     return at;
 }
+__host__ __device__ constexpr uint32_t means_bytes(uint32_t dim) { return kTileKeys * (dim / 2 + dim / 16); }  // of a block's keys
+
 template <int DIM>
-__global__ void __launch_bounds__(kMeansThreads, 2) k_block_means(const __grid_constant__ MeansArgs a) {
+__global__ void __launch_bounds__(kMeansThreads) k_block_means(const __grid_constant__ MeansArgs a) {
     constexpr uint32_t CB = DIM / 2, NG = DIM / 64, kLanes = CB / 16, kKeys = 32 / kLanes;  // lanes a key, keys at once
-    constexpr int kSteps = kTileKeys / kKeys, kAtOnce = kSteps < 8 ? kSteps : 8, kMine = 32 / kKeys;  // loads of a block, in flight; values of a mean that are a lane's
+    constexpr int kSteps = kTileKeys / kKeys, kMine = 32 / kKeys;  // turns of a block; values of a mean that are a lane's
+    extern __shared__ __align__(16) uint8_t meansSmem[];
+    __shared__ __align__(8) uint64_t barriers[kMeansThreads / 32];
     __shared__ uint32_t first[kMeansThreads + 1], warpSums[kMeansThreads / 32];
-    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = tid >> 5;
+    const uint32_t tid = threadIdx.x, lane = tid & 31u, warp = (uint32_t)warp_index();
+    const uint32_t bar = sm_addr(barriers) + 8 * warp, held = sm_addr(meansSmem) + warp * means_bytes(DIM), heldWords = held + kTileKeys * CB;  // the warp's block
+    uint32_t parity = 0;
+    if (lane == 0) {
+        bar_init(bar, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
     pdl_enter();
 
     // blocks that the requests complete, and where each thread's run of requests begins among them
@@ -118,11 +129,16 @@ __global__ void __launch_bounds__(kMeansThreads, 2) k_block_means(const __grid_c
     __syncthreads();
 
     const uint32_t inKey = lane % kLanes, keyLane = lane / kLanes, pieceShift = min(a.pageShift, kBlockShift), pageTokens = 1u << a.pageShift;
-    const unsigned long long items = (unsigned long long)total * a.kvHeads;
-    for (unsigned long long item = (unsigned long long)blockIdx.x * (kMeansThreads / 32) + warp; item < items; item += (unsigned long long)gridDim.x * (kMeansThreads / 32)) {
-        uint32_t n = (uint32_t)(item / a.kvHeads);
-        const uint32_t head = (uint32_t)(item % a.kvHeads);
-        uint32_t low = 0, high = kMeansThreads;
+    const unsigned long long items = (unsigned long long)total * a.kvHeads, step = (unsigned long long)gridDim.x * (kMeansThreads / 32);
+    const uint32_t pieces = kTileKeys >> pieceShift;
+    struct Block {
+        uint32_t head, key0, page;  // a lane holds the page of one piece
+    };
+    auto locate = [&](unsigned long long item) {
+        Block b{0u, 0u, 0u};
+        if (item >= items) return b;
+        uint32_t n = (uint32_t)(item / a.kvHeads), low = 0, high = kMeansThreads;
+        b.head = (uint32_t)(item % a.kvHeads);
         while (high - low > 1) {
             const uint32_t mid = (low + high) >> 1;
             if (first[mid] <= n) low = mid;
@@ -135,65 +151,83 @@ __global__ void __launch_bounds__(kMeansThreads, 2) k_block_means(const __grid_c
             n -= s.count;
             s = span_of(++r);
         }
-        const uint32_t key0 = (s.begin + n) << kBlockShift;
-        // a lane holds the page of one piece of the block
-        const uint32_t pieces = kTileKeys >> pieceShift;
-        uint32_t page = 0;
-        if (lane < pieces) page = __ldg(a.blockTable + (size_t)r * a.tableStride + ((key0 + (lane << pieceShift)) >> a.pageShift));
+        b.key0 = (s.begin + n) << kBlockShift;
+        if (lane < pieces) b.page = __ldg(a.blockTable + (size_t)r * a.tableStride + ((b.key0 + (lane << pieceShift)) >> a.pageShift));
+        return b;
+    };
+    Block next = locate((unsigned long long)blockIdx.x * (kMeansThreads / 32) + warp);
+    for (unsigned long long item = (unsigned long long)blockIdx.x * (kMeansThreads / 32) + warp; item < items; item += step) {
+        const uint32_t head = next.head, key0 = next.key0, page = next.page;
         const bool hole = __any_sync(0xFFFFFFFFu, page >= a.pageCount);
         const uint32_t lastPage = __shfl_sync(0xFFFFFFFFu, page, pieces - 1u);
         if (hole && lane == 0) *a.errorFlag = kFlagPage;
-        if (lastPage >= a.pageCount) continue;
-        // key k * kKeys + keyLane of the block: its codes, its word
-        auto block_of = [&](int k) {
-            const uint32_t key = k * kKeys + keyLane;
-            return a.pages + ((size_t)__shfl_sync(0xFFFFFFFFu, page, key >> pieceShift) * a.kvHeads + head) * a.page.blockBytes;
-        };
-        auto at_of = [&](int k) { return (key0 + k * kKeys + keyLane) & (pageTokens - 1u); };
-        uint32_t words[kSteps], most = 0, least = 0xFFu, at;  // exponents of the scales
-        double bias = 0.0, mean[kMine];
-#pragma unroll
-        for (int k = 0; k < kSteps; ++k) words[k] = hole ? 0u : __ldg(reinterpret_cast<const uint32_t *>(block_of(k) + a.page.keyWords + (size_t)at_of(k) * (NG * 4)) + inKey / (kLanes / NG));
-        auto codes_of = [&](int k) { return hole ? make_uint4(0u, 0u, 0u, 0u) : __ldg(reinterpret_cast<const uint4 *>(block_of(k) + (size_t)at_of(k) * CB) + inKey); };
-        uint4 codes[kAtOnce];
-#pragma unroll
-        for (int k = 0; k < kAtOnce; ++k) codes[k] = codes_of(k);
+        // the block as it lies, piece by piece, into the warp's shared memory
+        __syncwarp();  // (the one before has been read)
+        const uint32_t at0 = key0 & (pageTokens - 1u);
+        if (lane == 0 && !hole) bar_expect(bar, means_bytes(DIM));
+        __syncwarp();
+        if (lane < pieces && !hole) {
+            const uint8_t *block = a.pages + ((size_t)page * a.kvHeads + head) * a.page.blockBytes;
+            bulk_copy(held + lane * (CB << pieceShift), block + (size_t)at0 * CB, CB << pieceShift, bar);
+            bulk_copy(heldWords + lane * ((NG * 4) << pieceShift), block + a.page.keyWords + (size_t)at0 * (NG * 4), (NG * 4) << pieceShift, bar);
+        }
+        __syncwarp();
+        next = locate(item + step);  // (while the block comes)
+        if (!hole) {
+            bool there = mbar_try_wait(bar, parity);
+#pragma unroll 1
+            for (uint32_t i = 0; i < kMeansWaitLimit && !there; ++i) there = mbar_try_wait(bar, parity);
+            parity ^= 1u;
+            if (!__all_sync(0xFFFFFFFFu, there)) {
+                if (lane == 0) *a.errorFlag = kFlagWait;
+                break;  // (a later copy would take this one's bytes for its own)
+            }
+        }
+        // key k * kKeys + keyLane of the block: its word, its codes
+        const uint32_t myCodes = held + keyLane * CB + inKey * 16, myWords = heldWords + (keyLane * NG + inKey / (kLanes / NG)) * 4;
+        auto word_of = [&](int k) { return hole ? 0u : lds32(myWords + k * (kKeys * NG * 4)); };
+        auto codes_of = [&](int k) { return hole ? make_uint4(0u, 0u, 0u, 0u) : lds128(myCodes + k * (kKeys * CB)); };
+        uint32_t most = 0, least = 0xFFu, biasMost = 0, biasLeast = 0xFFu, at;  // exponents of the scales, of the biases
 #pragma unroll
         for (int k = 0; k < kSteps; ++k) {
-            const uint32_t e = words[k] >> 7 & 0xFFu;
-            most = max(most, e);
-            if (words[k] & 0x7FFFu) least = min(least, max(e, 1u));
-            bias += (double)high16(words[k]);
+            const uint32_t w = word_of(k), e = w >> 7 & 0xFFu, f = w >> 23 & 0xFFu;
+            most = max(most, e), biasMost = max(biasMost, f);
+            if (w & 0x7FFFu) least = min(least, max(e, 1u));
+            if (w & 0x7FFF0000u) biasLeast = min(biasLeast, max(f, 1u));
         }
         most = __reduce_max_sync(0xFFFFFFFFu, most), least = __reduce_min_sync(0xFFFFFFFFu, least);
-        if (most < 0xFFu && most <= least + 6u) {
+        biasMost = __reduce_max_sync(0xFFFFFFFFu, biasMost), biasLeast = __reduce_min_sync(0xFFFFFFFFu, biasLeast);
+        double mean[kMine], bias = 0.0;
+        if (max(most, biasMost) < 0xFFu && most <= least + 6u && biasMost <= biasLeast + 9u) {
             // Nibbles i and i + 4 of a word, masked in place: 2^23 + 16^i code, less 2^23, times the scale / 16^i; two codes an instruction.
             unsigned long long sums[16];
+            float biases = 0.0f;
 #pragma unroll
             for (int i = 0; i < 16; ++i) sums[i] = pair_f32(0.0f, 0.0f);
             const unsigned long long less = pair_f32(-8388608.0f, -8388608.0f);
+#pragma unroll 4
+            for (int k = 0; k < kSteps; ++k) {
+                const uint32_t w = word_of(k);
+                const uint4 four = codes_of(k);
+                const uint32_t word[4] = {four.x, four.y, four.z, four.w};
+                biases += high16(w);
 #pragma unroll
-            for (int k0 = 0; k0 < kSteps; k0 += kAtOnce) {
+                for (int i = 0; i < 4; ++i) {
+                    const float down = low16(w) * (i == 0 ? 1.0f : i == 1 ? 0x1p-4f : i == 2 ? 0x1p-8f : 0x1p-12f);
+                    const unsigned long long factor = pair_f32(down, down);
+                    const uint32_t mask = 15u << (4 * i);
 #pragma unroll
-                for (int k = 0; k < kAtOnce; ++k) {
-                    const float scale = low16(words[k0 + k]);
-                    const uint32_t word[4] = {codes[k].x, codes[k].y, codes[k].z, codes[k].w};
-                    if (k0 + kAtOnce < kSteps) codes[k] = codes_of(k0 + kAtOnce + k);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float down = scale * (i == 0 ? 1.0f : i == 1 ? 0x1p-4f : i == 2 ? 0x1p-8f : 0x1p-12f);
-                        const unsigned long long factor = pair_f32(down, down);
-                        const uint32_t mask = 15u << (4 * i);
-#pragma unroll
-                        for (int w = 0; w < 4; ++w)
-                            sums[4 * w + i] = fma_f32x2(add_f32x2(pair_u32((word[w] & mask) | 0x4B000000u, (word[w] >> 16 & mask) | 0x4B000000u), less), factor, sums[4 * w + i]);
-                    }
+                    for (int n = 0; n < 4; ++n)
+                        sums[4 * n + i] = fma_f32x2(add_f32x2(pair_u32((word[n] & mask) | 0x4B000000u, (word[n] >> 16 & mask) | 0x4B000000u), less), factor, sums[4 * n + i]);
                 }
             }
             float value[32];
 #pragma unroll
             for (int i = 0; i < 16; ++i) value[8 * (i / 4) + i % 4] = __uint_as_float((uint32_t)sums[i]), value[8 * (i / 4) + i % 4 + 4] = __uint_as_float((uint32_t)(sums[i] >> 32));
             at = join_lanes<kLanes>(value);
+#pragma unroll
+            for (uint32_t mask = kLanes; mask < 32; mask *= 2) biases += __shfl_xor_sync(0xFFFFFFFFu, biases, mask);
+            bias = biases;
 #pragma unroll
             for (int i = 0; i < kMine; ++i) mean[i] = value[i];
         } else {
@@ -202,19 +236,21 @@ __global__ void __launch_bounds__(kMeansThreads, 2) k_block_means(const __grid_c
             for (int i = 0; i < 32; ++i) value[i] = 0.0;
 #pragma unroll 1
             for (int k = 0; k < kSteps; ++k) {
+                const uint32_t w = word_of(k);
                 const uint4 four = codes_of(k);
                 const uint32_t word[4] = {four.x, four.y, four.z, four.w};
-                const double scale = (double)low16(__ldg(reinterpret_cast<const uint32_t *>(block_of(k) + a.page.keyWords + (size_t)at_of(k) * (NG * 4)) + inKey / (kLanes / NG)));
+                const double scale = (double)low16(w);
+                bias += (double)high16(w);
 #pragma unroll
                 for (int i = 0; i < 32; ++i)  // (2^52 + code less 2^52: a conversion takes longer)
                     value[i] = fma(scale, __hiloint2double(0x43300000, (int)(word[i / 8] >> (4 * (i & 7)) & 15u)) - 0x1p52, value[i]);
             }
             at = join_lanes<kLanes>(value);
 #pragma unroll
+            for (uint32_t mask = kLanes; mask < 32; mask *= 2) bias += __shfl_xor_sync(0xFFFFFFFFu, bias, mask);
+#pragma unroll
             for (int i = 0; i < kMine; ++i) mean[i] = value[i];
         }
-#pragma unroll
-        for (uint32_t mask = kLanes; mask < 32; mask *= 2) bias += __shfl_xor_sync(0xFFFFFFFFu, bias, mask);
         at += 32 * inKey;
         most = 0;
 #pragma unroll
@@ -236,6 +272,7 @@ __global__ void __launch_bounds__(kMeansThreads, 2) k_block_means(const __grid_c
             out[i / 2] = pack_bf16x2(v[0], v[1]);
         }
         const uint32_t perPage = max(1u, pageTokens >> kBlockShift), place = (key0 & (pageTokens - 1u)) >> kBlockShift;
+        if (lastPage >= a.pageCount) continue;  // (nowhere to keep it)
         uint16_t *to = a.means + (((size_t)lastPage * a.kvHeads + head) * perPage + (pageTokens > kTileKeys ? place : 0u)) * DIM + at;
         if (kMine == 8) *reinterpret_cast<uint4 *>(to) = make_uint4(out[0], out[1 % (kMine / 2)], out[2 % (kMine / 2)], out[3 % (kMine / 2)]);
         else if (kMine == 4) *reinterpret_cast<uint2 *>(to) = make_uint2(out[0], out[1 % (kMine / 2)]);
@@ -666,7 +703,7 @@ __global__ void __launch_bounds__(32 * kRowsWarps, DIM == 256 ? 2 : DIM == 128 ?
     select_largest<1>(scores + warp * a.tableBlocks + a.first, seen - a.last - a.first, wanted, a.first, out + a.first, counts[warp]);
 }
 
-KernelSmemMemo splitMemo[3][4], rowsMemo[3][6];
+KernelSmemMemo meansMemo[3], splitMemo[3][4], rowsMemo[3][6];
 
 }  // namespace
 
@@ -676,9 +713,12 @@ bool launch_block_means(FFAttention *att, const uint8_t *pages, uint32_t pageCou
     const MeansArgs args{pages, pageCount, blockTable, tableStride, tableKeys, oldLengths, newLengths, requests, c.kvHeads, (uint32_t)__builtin_ctz(c.pageTokens),
                          page_layout(c), means, att->errorFlag};
     const uint64_t most = ((uint64_t)requests * (tableKeys / kTileKeys) * c.kvHeads + kMeansThreads / 32 - 1) / (kMeansThreads / 32);
-    const uint32_t grid = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(most, 2u * (uint32_t)att->smCount));
-    auto launch = [&](auto kernel) { return launched(att, launch_pdl(kernel, dim3(grid), dim3(kMeansThreads), 0, stream, args), "k_block_means", error); };
-    return c.headDim == 256 ? launch(k_block_means<256>) : c.headDim == 128 ? launch(k_block_means<128>) : launch(k_block_means<64>);
+    const uint32_t grid = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>(most, (uint32_t)att->smCount)), smem = kMeansThreads / 32 * means_bytes(c.headDim);
+    auto launch = [&](auto kernel, KernelSmemMemo &memo) {
+        if (!memo.prepare(kernel, att->device, smem, kMeansThreads, nullptr, error)) return false;
+        return launched(att, launch_pdl(kernel, dim3(grid), dim3(kMeansThreads), smem, stream, args), "k_block_means", error);
+    };
+    return c.headDim == 256 ? launch(k_block_means<256>, meansMemo[2]) : c.headDim == 128 ? launch(k_block_means<128>, meansMemo[1]) : launch(k_block_means<64>, meansMemo[0]);
 }
 
 bool launch_select_blocks(FFAttention *att, const uint16_t *q, uint32_t qStride, uint32_t tokens, const uint16_t *means, uint32_t pageCount,
