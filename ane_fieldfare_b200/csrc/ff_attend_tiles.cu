@@ -441,6 +441,15 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
         take(w);
         return w.count != 0 || next_segment(w);
     };
+    // (by one warp for all: by each for itself it took 5000 cycles, most of them waiting for issue slots)
+    __shared__ Walk firstWalk;
+    __shared__ bool firstMore;
+    if (warp == 0 && begin < end) {
+        Walk w;
+        const bool more = first_segment(w);
+        if (lane == 0) firstWalk = w, firstMore = more;
+    }
+    __syncthreads();
     auto key_at = [&](const RowTile &q, uint32_t t) { return (t < q.tilesSink ? t : q.lowTile + t - q.tilesSink) * kTileKeys; };
     const uint32_t pieceKeys = 1u << args.pieceShift, pieces = kTileKeys >> args.pieceShift;
 
@@ -459,8 +468,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
             const uint32_t perTileShift = 6u - args.pieceShift, tilesPer = 32u >> perTileShift;  // pieces of a tile, as a shift; tiles whose pages a warp holds
             uint32_t stage = 0, phase = 0;
             bool ok = true;
-            Walk w;
-            for (bool more = first_segment(w); more && ok; more = ok && next_segment(w)) {
+            Walk w = firstWalk;
+            for (bool more = firstMore; more && ok; more = ok && next_segment(w)) {
                 const int keysEnd = w.q.p0 + (int)w.q.tokens;
                 // a lane holds the page of one piece of `tilesPer` tiles from `base` on
                 auto page_of = [&](uint32_t base) {
@@ -512,7 +521,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
             // ---------------- MMAs ----------------
             uint32_t slot = 0, phase = 0, tile = 0, unitNo = 0;  // tile: key tiles so far (its S buffer, the barriers' parities)
             bool ok = true;
-            Walk w;
+            Walk w = firstWalk;
             const uint32_t idescS = idesc_f16(kTileKeys, false), idescO = idesc_f16(DIM, true);
             auto scores = [&](uint32_t n) {  // S of the n-th tile, from the slot that is next
                 if (!wait_warp<false>(barTile + 8 * slot, phase, &abortFlag)) return false;
@@ -530,7 +539,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                 if (++slot == kSlots) slot = 0, phase ^= 1u;
                 return true;
             };
-            for (bool more = first_segment(w); more && ok; more = ok && next_segment(w)) {
+            for (bool more = firstMore; more && ok; more = ok && next_segment(w)) {
                 ok = wait_warp<false>(barQ, unitNo & 1u, &abortFlag);
                 tc_fence_after();
                 ok = ok && scores(tile);
@@ -571,8 +580,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
             // 16 scale and |bias| of the tile 2^-6 .. 2^-5.
             uint32_t tile = 0;
             bool ok = true;
-            Walk w;
-            for (bool more = first_segment(w); more && ok; more = ok && next_segment(w)) {
+            Walk w = firstWalk;
+            for (bool more = firstMore; more && ok; more = ok && next_segment(w)) {
                 // Of values far below (2^-64) the largest of the segment so far, or of zeros, the tile's own power would put M so far above its
                 // logits that its weights fell out of 32 bits, and out of the sum.
                 int floorV = -100;
@@ -691,8 +700,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                     mbar_arrive(barTile + 8 * slot);
                 }
             };
-            Walk w;
-            for (bool more = first_segment(w); more && ok; more = ok && next_segment(w)) {
+            Walk w = firstWalk;
+            for (bool more = firstMore; more && ok; more = ok && next_segment(w)) {
                 // a segment of n tiles is 2 n slots: K0, then for every tile i the keys of i + 1 (all but the last) and the values of i
                 for (uint32_t k = 0; k < 2 * w.count && ok; ++k, ++item) {
                     if (item % kGroups != grp) continue;
@@ -716,8 +725,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                 const uint32_t r = quarter * 32 + 8 * k + (lane >> 2);
                 mineRows[k] = (r / group) << 16 | r % group;
             }
-            Walk w;
-            for (bool more = first_segment(w); more && ok; more = ok && next_segment(w)) {
+            Walk w = firstWalk;
+            for (bool more = firstMore; more && ok; more = ok && next_segment(w)) {
                 const uint32_t token = row / group;
                 const bool there = token < w.q.tokens;
                 const int p = w.q.p0 + (int)token;
