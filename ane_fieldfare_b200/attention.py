@@ -48,6 +48,7 @@ class AttentionContext:
         self.heads, self.kvHeads, self.headDim, self.pageTokens = heads, kvHeads, headDim, pageTokens
         self.maxRequests, self.maxTokens = maxRequests, maxTokens
         self.pageBytes = lib.ff_cache_page_bytes(ctypes.byref(self.config))
+        self._sharedBytes = {}  # of attendShared's workspace, by rows
 
     @property
     def handle(self):
@@ -242,10 +243,10 @@ class AttentionContext:
         return out
 
     def attendShared(self, q: torch.Tensor, pages: torch.Tensor, blockTable: torch.Tensor, rowStart: torch.Tensor,
-                     lengths: torch.Tensor, maxRows: int, groupStart: torch.Tensor, prefixLengths: torch.Tensor, *,
+                     lengths: torch.Tensor, maxRows: int, groupStart: torch.Tensor, prefixLengths: torch.Tensor, *, always: bool = False,
                      scale: Optional[float] = None, out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
         """`attend` without a window, where requests groupStart[g] .. groupStart[g + 1] - 1 hold the same first prefixLengths[g]
-        keys on the same pages: these are read once for all rows of the group."""
+        keys on the same pages: these are read once for all rows of the group, where that is shorter (always: in any case)."""
         tokens, requests, groups, shape = q.shape[0], lengths.numel(), prefixLengths.numel(), blockTable.shape
         if rowStart.numel() != requests + 1 or len(shape) != 2 or shape[0] != requests:
             raise ValueError("lengths, blockTable and rowStart must agree on the number of requests")
@@ -256,9 +257,12 @@ class AttentionContext:
         if out is None:
             out = self._new((tokens, self.heads, self.headDim), torch.bfloat16, stream)
         self._ints("blockTable rowStart lengths groupStart prefixLengths", blockTable, rowStart, lengths, groupStart, prefixLengths)
-        workspace = self._new((16 + 4 * tokens * self.heads * (self.headDim + 2) + 8,), torch.uint8, stream)
+        bytes_ = self._sharedBytes.get(tokens)
+        if bytes_ is None:
+            bytes_ = self._sharedBytes.setdefault(tokens, binding.load().ff_attention_shared_bytes(ctypes.byref(self.config), tokens))
+        workspace = self._new((bytes_,), torch.uint8, stream)
         call("ff_attention_shared", self.handle, *self._heads(q, self.heads, tokens, "q"), tokens, *self._cache(pages), blockTable.data_ptr(), shape[1],
-             rowStart.data_ptr(), lengths.data_ptr(), requests, min(maxRows, _WORD), groupStart.data_ptr(), prefixLengths.data_ptr(), groups,
+             rowStart.data_ptr(), lengths.data_ptr(), requests, min(maxRows, _WORD), groupStart.data_ptr(), prefixLengths.data_ptr(), groups, always,
              self.headDim ** -0.5 if scale is None else scale, workspace.data_ptr(), *self._heads(out, self.heads, tokens, "out"),
              _stream(stream))
         return out

@@ -156,7 +156,8 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    pdl_enter();
+    // (Behind a launch over the prefixes this one begins while that ends: what it reads of the caller's is from before both.)
+    if (!kSuffix || !a.shared.launched) pdl_enter();
 
     // ---- the plan: how many tiles each request is, and this CTA's run of them ----
     const uint32_t requests = kListed ? a.tokens : kPrefix ? a.shared.groups : a.requests;
@@ -241,7 +242,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
     if (kListed)
         for (uint32_t r = tid; r < a.requests; r += kRowsThreads)
             if (goes_back(r)) sum = kTooMuch;
-    if ((kPrefix || kSuffix) && shared_refused<kSuffix>(a, tid, kRowsThreads)) sum = kTooMuch;
+    if ((kPrefix || kSuffix) && shared_refused(a, tid, kRowsThreads)) sum = kTooMuch;
     uint32_t scan = sum;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -261,9 +262,6 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
     if (tid == 0) first[kRowsThreads] = total;
     __syncthreads();
 
-    if constexpr (kPrefix) {
-        if (blockIdx.x == 0 && tid == 0) *a.shared.refused = refused;
-    }
     // rows that no unit writes: behind the last request's, and past maxRows
     if constexpr (!kPrefix) {
         const uint32_t covered = a.requests && !refused ? min(__ldg(a.rowStart + a.requests), a.tokens) : 0u;
@@ -277,7 +275,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
             if (tid == 0 && refused) *a.errorFlag = kFlagWork;
             __syncthreads();
             if (tid == 0 && a.requests && __ldg(a.rowStart + a.requests) > a.tokens) *a.errorFlag = kFlagRows;
-            if (kSuffix && shared_refused<false>(a, tid, kRowsThreads)) *a.errorFlag = kFlagRows;
+            if (kSuffix && shared_refused(a, tid, kRowsThreads)) *a.errorFlag = kFlagRows;
             if (kListed)
                 for (uint32_t r = tid; r < a.requests; r += kRowsThreads)
                     if (goes_back(r)) *a.errorFlag = kFlagRows;
@@ -292,9 +290,12 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
             }
         }
     }
-    if (total == 0 || refused) return;
+    auto leave = [&] {  // (this launch is not over before the one in front)
+        if constexpr (kSuffix) pdl_wait();
+    };
+    if (total == 0 || refused) return leave();
     const uint32_t ctas = min(gridDim.x, max(1u, total / 3u)), cta = blockIdx.x;
-    if (cta >= ctas) return;
+    if (cta >= ctas) return leave();
     auto start_of = [&](uint32_t c) { return (uint32_t)((unsigned long long)c * total / ctas); };
     auto cta_of = [&](uint32_t x) { return (uint32_t)((((unsigned long long)x + 1) * ctas - 1) / total); };
     const uint32_t begin = start_of(cta), end = start_of(cta + 1);
@@ -425,7 +426,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
             for (uint32_t i = 0; i < kWaitLimit && !mbar_try_wait(barFull + 8 * s, parity); ++i) __nanosleep(40);
         }
         if (lane == 0 && abortFlag) *a.errorFlag = kFlagWait;
-        return;
+        return leave();
     }
 
     // ---------------- 32 keys of every second tile ----------------
@@ -756,6 +757,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
             if (lane == 0) mbar_arrive(barEmpty + 8 * stage);
         }
 
+        if constexpr (kSuffix) pdl_wait();  // (for what the prefixes gave, and the parts' memory)
         // ---- the warps' outputs joined ----
         const float unscale = power_of_two(E);
         const bool mineToo = !SPLIT || t < 2;  // columns 4 .. 7 are the rests of columns 0 .. 3
@@ -932,6 +934,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
         named_barrier(1, 32 * kConsumers);  // the joining buffers are free
     } while (next_unit(w));
     if (lane == 0 && abortFlag) *a.errorFlag = kFlagWait;
+    leave();
 }
 
 KernelSmemMemo rowsMemo[4][3][3];

@@ -52,10 +52,16 @@ constexpr uint32_t kRows = kTileRows;
 // is 2^-30 of the largest is still something.
 constexpr float kWeightScale = 6.0f;
 constexpr uint32_t kUnitCost = 8;  // tiles' time that a unit takes besides its tiles
-constexpr uint32_t kInfo = 4;   // tiles whose scales and exponents are kept
 constexpr uint32_t kSlots = 4, kPacked = 3;  // expanded tiles; packed ones, of keys and of values each
-// The values of tile m are item 2 m + 1 or 2 m + 2 of the expansion: those kPacked tiles before them are at least kSlots items before.
-static_assert(2 * kPacked - 1 >= kSlots, "a free slot says that the ring's place was read");
+// S has as many buffers as tensor memory has room for beside queries and outputs; its products run as far ahead of those of the weights as
+// the rings allow; scales and exponents are kept for that many tiles and as many more.
+__host__ __device__ constexpr uint32_t score_buffers(int dim) { return dim == 256 ? 2u : 4u; }
+__host__ __device__ constexpr uint32_t tiles_ahead(int dim) { return dim == 256 ? 2u : 3u; }
+__host__ __device__ constexpr uint32_t info_tiles(int dim) { return dim == 256 ? 4u : 8u; }
+// The expansion's items are the keys of as many tiles, then values and keys in turn, at the end of a unit the values that are left: no more
+// values than that one behind the other.  So the values kPacked tiles before a tile's are at least kPacked + 1 items before.
+static_assert(kPacked + 1 >= kSlots && tiles_ahead(64) <= kPacked && tiles_ahead(256) <= kPacked, "a free slot says that the ring's place was read");
+static_assert(tiles_ahead(64) <= score_buffers(64) && tiles_ahead(256) <= score_buffers(256), "a buffer each");
 
 struct TilesArgs {
     AttendArgs a;
@@ -68,7 +74,7 @@ struct TilesArgs {
 __host__ __device__ constexpr uint32_t slot_bytes(int dim) { return kTileKeys * dim * 2; }
 __host__ __device__ constexpr uint32_t packed_bytes(int dim) { return (kTileKeys * dim / 2 + 1023u) & ~1023u; }
 __host__ __device__ constexpr uint32_t words_bytes(int dim) { return 2u * kTileKeys * (dim / 64) * 4u; }  // of a tile, keys' and values'
-__host__ __device__ constexpr uint32_t tiles_smem(int dim) { return 1024u + kSlots * slot_bytes(dim) + 2 * kPacked * packed_bytes(dim) + (kInfo + kPacked) * words_bytes(dim); }
+__host__ __device__ constexpr uint32_t tiles_smem(int dim) { return 1024u + kSlots * slot_bytes(dim) + 2 * kPacked * packed_bytes(dim) + (info_tiles(dim) + kPacked) * words_bytes(dim); }
 
 // K-major or N-major tile of f16 with the 128-byte swizzle: rows of 128 bytes, groups of eight 1024 bytes apart; N-major:
 // the next 64 values `lead` bytes further.
@@ -179,9 +185,10 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
     constexpr uint32_t kWordSide = words_bytes(DIM) / 2, kUnits = kTileKeys * NG;  // of a slot: a key's group of 64 values
     // (no more groups than slots: one that waited for a slot two rounds ahead would take one round's parity for the other's)
     constexpr uint32_t kGroupWarps = DIM == 64 ? 2 : 4, kGroups = kDequantWarps / kGroupWarps < kSlots ? kDequantWarps / kGroupWarps : kSlots, kUnitsEach = kUnits / (32 * kGroupWarps);
+    constexpr uint32_t kInfo = info_tiles(DIM), kBuffers = score_buffers(DIM), kAhead = tiles_ahead(DIM);
     constexpr uint32_t kColQ = 0, kColO = DIM / 2, kColS = kColO + DIM;
     extern __shared__ uint8_t tilesSmem[];
-    __shared__ __align__(8) uint64_t barriers[2 * kSlots + 4 * kPacked + 2 * kInfo + 2 + 4 + 2 + 1 + 1 + 8 + 1];
+    __shared__ __align__(8) uint64_t barriers[2 * kSlots + 4 * kPacked + 2 * kInfo + kBuffers + 2 * kBuffers + 2 + 1 + 1 + 8 + 1];
     __shared__ uint32_t tmemSlot, lastPart;
     __shared__ volatile uint32_t abortFlag;
     __shared__ uint32_t firstTile[kTilesThreads + 1], firstWork[kTilesThreads + 1], warpSums[32];
@@ -197,7 +204,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
     const uint32_t bar0 = sm_addr(barriers);
     const uint32_t barTile = bar0, barTileFree = barTile + 8 * kSlots, barPack = barTileFree + 8 * kSlots, barPackFree = barPack + 16 * kPacked;  // keys', then values'
     const uint32_t barInfo = barPackFree + 16 * kPacked, barInfoFree = barInfo + 8 * kInfo;
-    const uint32_t barS = barInfoFree + 8 * kInfo, barP = barS + 16, barO = barP + 32, barQ = barO + 16, barJoin = barQ + 8, barTop = barJoin + 8, barDone = barTop + 64;
+    const uint32_t barS = barInfoFree + 8 * kInfo, barP = barS + 8 * kBuffers, barO = barP + 16 * kBuffers, barQ = barO + 16, barJoin = barQ + 8, barTop = barJoin + 8, barDone = barTop + 64;
     if (tid == 0) {
         abortFlag = 0;
         for (uint32_t s = 0; s < kSlots; ++s) {
@@ -212,12 +219,12 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
             mbar_init(barInfo + 8 * s, 1);
             mbar_init(barInfoFree + 8 * s, 1);
         }
-        for (uint32_t s = 0; s < 2; ++s) {
+        for (uint32_t s = 0; s < kBuffers; ++s) {
             mbar_init(barS + 8 * s, 1);
             mbar_init(barP + 16 * s, 4);  // the first 32 keys' weights
             mbar_init(barP + 16 * s + 8, 4);
-            mbar_init(barO + 8 * s, 1);
         }
+        for (uint32_t s = 0; s < 2; ++s) mbar_init(barO + 8 * s, 1);
         mbar_init(barQ, kRowWarps);
         mbar_init(barJoin, kRowWarps);
         for (uint32_t s = 0; s < 8; ++s) mbar_init(barTop + 8 * s, 1);
@@ -232,7 +239,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, tmemSlot, 0);
-    pdl_enter();
+    // (Behind a launch over the prefixes this one begins while that ends: what it reads of the caller's is from before both.)
+    if (!kSuffix || !a.shared.launched) pdl_enter();
 
     // ---- the plan: row tiles of the requests, key tiles of those, this CTA's run ----
     // A request: its first row, rows, length; looked up once where there is a thread for each.
@@ -323,7 +331,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
         mineTiles = goes_back(r) ? kTooMuch : add_work(mineTiles, (min(of.y, a.maxRows) + args.tileTokens - 1) / args.tileTokens);
         if (!kPrefix && of.y && (int)of.z - (int)of.y + (int)min(of.y, a.maxRows) > 0 && of.z - of.y + min(of.y, a.maxRows) > a.tableKeys) *a.errorFlag = kFlagTableRow;  // (what the row has no room for is not walked)
     }
-    if ((kPrefix || kSuffix) && shared_refused<kSuffix>(a, tid, kTilesThreads)) mineTiles = kTooMuch;
+    if ((kPrefix || kSuffix) && shared_refused(a, tid, kTilesThreads)) mineTiles = kTooMuch;
     const uint32_t allTiles = block_scan(mineTiles, firstTile);
     const uint32_t rowTiles = allTiles == kTooMuch ? 0u : allTiles;
     // the n-th row tile
@@ -364,9 +372,6 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
     const bool refused = allTiles == kTooMuch || allWork == kTooMuch;  // (the places of units are nothing then)
     const uint32_t total = refused ? 0u : allWork;
 
-    if constexpr (kPrefix) {
-        if (blockIdx.x == 0 && tid == 0) *a.shared.refused = refused;
-    }
     // rows that no unit writes: behind the last request's, and past maxRows
     if constexpr (!kPrefix) {
         const uint32_t covered = a.requests && !refused ? min(__ldg(a.rowStart + a.requests), a.tokens) : 0u;
@@ -379,7 +384,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
         if (blockIdx.x == 0) {
             if (tid == 0 && refused) *a.errorFlag = kFlagWork;
             __syncthreads();
-            if (kSuffix && shared_refused<false>(a, tid, kTilesThreads)) *a.errorFlag = kFlagRows;
+            if (kSuffix && shared_refused(a, tid, kTilesThreads)) *a.errorFlag = kFlagRows;
             if (tid == 0 && a.requests && __ldg(a.rowStart + a.requests) > a.tokens) *a.errorFlag = kFlagRows;
             for (uint32_t r = r0; r < r1; ++r) {
                 if (goes_back(r)) *a.errorFlag = kFlagRows;
@@ -527,13 +532,13 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                 if (!wait_warp<false>(barTile + 8 * slot, phase, &abortFlag)) return false;
                 tc_fence_after();
                 const uint64_t desc = desc_sw128(slots + slot * kSlot, 16);
-                const uint32_t d = tmem + kColS + (n & 1u) * kTileKeys;
+                const uint32_t d = tmem + kColS + n % kBuffers * kTileKeys;
                 if (elect_one()) {
 #pragma unroll
                     for (uint32_t k = 0; k < DIM / 16; ++k)
                         mma_a_tmem(d, tmem + kColQ + 8 * k, desc + (k / 4) * (kTileKeys * 128 >> 4) + 2 * (k % 4), idescS, k != 0);
                     commit(barTileFree + 8 * slot);
-                    commit(barS + 8 * (n & 1u));
+                    commit(barS + 8 * (n % kBuffers));
                 }
                 __syncwarp();
                 if (++slot == kSlots) slot = 0, phase ^= 1u;
@@ -542,20 +547,19 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
             for (bool more = firstMore; more && ok; more = ok && next_segment(w)) {
                 ok = wait_warp<false>(barQ, unitNo & 1u, &abortFlag);
                 tc_fence_after();
-                ok = ok && scores(tile);
+                for (uint32_t i = 0; i < min(kAhead, w.count) && ok; ++i) ok = scores(tile + i);
                 for (uint32_t i = 0; i < w.count && ok; ++i, ++tile) {
-                    if (i + 1 < w.count && !(ok = scores(tile + 1))) break;
                     if (!(ok = wait_warp<false>(barTile + 8 * slot, phase, &abortFlag))) break;
-                    if (!(ok = wait_warp<false>(barP + 16 * (tile & 1u), tile >> 1 & 1u, &abortFlag))) break;
+                    if (!(ok = wait_warp<false>(barP + 16 * (tile % kBuffers), tile / kBuffers & 1u, &abortFlag))) break;
                     tc_fence_after();
                     const uint64_t desc = desc_sw128(slots + slot * kSlot, kTileKeys * 128);
-                    const uint32_t p = tmem + kColS + (tile & 1u) * kTileKeys;
+                    const uint32_t p = tmem + kColS + tile % kBuffers * kTileKeys;
                     if (elect_one()) {
 #pragma unroll
                         for (uint32_t k = 0; k < kTileKeys / 32; ++k) mma_a_tmem(tmem + kColO, p + 8 * k, desc + k * (2048 >> 4), idescO, (i | k) != 0);
                     }
                     __syncwarp();
-                    if (!(ok = wait_warp<false>(barP + 16 * (tile & 1u) + 8, tile >> 1 & 1u, &abortFlag))) break;
+                    if (!(ok = wait_warp<false>(barP + 16 * (tile % kBuffers) + 8, tile / kBuffers & 1u, &abortFlag))) break;
                     tc_fence_after();
                     if (elect_one()) {
 #pragma unroll
@@ -566,6 +570,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                     }
                     __syncwarp();
                     if (++slot == kSlots) slot = 0, phase ^= 1u;
+                    if (i + kAhead < w.count) ok = scores(tile + kAhead);
                 }
                 ++unitNo;
             }
@@ -659,7 +664,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                 }
             }
         } else if (warp >= (uint32_t)kFirstDequant) {
-            // ---------------- expansion: the groups of warps take slots K0, K1, V0, K2, V1, ... in turn ----------------
+            // ---------------- expansion: the groups of warps take slots K0, K1, (K2,) V0, K2 (K3), V1, ... in turn ----------------
             const uint32_t dw = warp - kFirstDequant, grp = dw / kGroupWarps, inGroup = dw % kGroupWarps;
             uint32_t item = 0, tile = 0;  // slots filled by all groups; key tiles so far
             bool ok = true;
@@ -702,11 +707,12 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
             };
             Walk w = firstWalk;
             for (bool more = firstMore; more && ok; more = ok && next_segment(w)) {
-                // a segment of n tiles is 2 n slots: K0, then for every tile i the keys of i + 1 (all but the last) and the values of i
+                // a segment of n tiles is 2 n slots: the keys of the first kAhead, then for every tile i its values and the keys of i + kAhead
+                const uint32_t lead = min(kAhead, w.count), paired = lead + 2 * (w.count - lead);
                 for (uint32_t k = 0; k < 2 * w.count && ok; ++k, ++item) {
                     if (item % kGroups != grp) continue;
-                    const bool isKey = k == 0 || (k % 2 == 1 && k != 2 * w.count - 1);
-                    fill(tile + (isKey ? (k + 1) / 2 : (k == 2 * w.count - 1 ? w.count - 1 : k / 2 - 1)), isKey ? 0u : 1u);
+                    const bool isKey = k < lead || (k < paired && ((k - lead) & 1u));
+                    fill(tile + (k < lead ? k : k < paired ? (k - lead) / 2 + (isKey ? lead : 0u) : k - w.count), isKey ? 0u : 1u);
                 }
                 tile += w.count;
             }
@@ -719,6 +725,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
             const uint32_t lanes = (quarter * 32) << 16;
             uint32_t tile = 0, joins = 0;
             bool ok = true;
+            [[maybe_unused]] uint4 firstPart = make_uint4(0u, 0u, 0u, 0u);  // prefix: of the run's last unit, where others have the rest
             uint32_t mineRows[4];  // token << 16 | head of the rows lane / 4 + 8 k of the warp's 32
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -790,9 +797,9 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                 uint32_t i = (tile ^ wg) & 1u;  // the segment's first tile of this warpgroup
                 for (tile += i; i < w.count; i += 2, tile += 2) {
                     const uint32_t info = tile % kInfo;
-                    if (!(ok = wait_warp<false>(barS + 8 * wg, tile >> 1 & 1u, &abortFlag))) break;
+                    if (!(ok = wait_warp<false>(barS + 8 * (tile % kBuffers), tile / kBuffers & 1u, &abortFlag))) break;
                     tc_fence_after();
-                    const uint32_t s0 = tmem + lanes + kColS + wg * kTileKeys;
+                    const uint32_t s0 = tmem + lanes + kColS + tile % kBuffers * kTileKeys;
                     uint32_t lo[32], hi[32];
                     tc_load_32cols(s0, lo);
                     tc_load_32cols(s0 + 32, hi);
@@ -872,7 +879,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                     tc_wait_st();
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(barP + 16 * wg);  // (the products of the first 32 keys may begin)
+                    if (lane == 0) mbar_arrive(barP + 16 * (tile % kBuffers));  // (the products of the first 32 keys may begin)
                     weigh(u, s0 + 16);
                     part = add_f32x2(part, part2);
                     // (A weight is 2^(S f + eV - M) here.  M is at most 72 above the largest logit plus eV; where it is further above this warpgroup's,
@@ -881,7 +888,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                     tc_wait_st();
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(barP + 16 * wg + 8);
+                    if (lane == 0) mbar_arrive(barP + 16 * (tile % kBuffers) + 8);
                 }
                 if (!ok) break;
                 tile = tile - i + w.count;
@@ -891,6 +898,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                 refShared[wg][row] = ref;
                 if (!meet() || !(ok = wait_warp<false>(barO + 8 * ((tile - 1) & 1u), (tile - 1) >> 1 & 1u, &abortFlag))) break;
                 tc_fence_after();
+                if constexpr (kSuffix) pdl_wait();  // (for what the prefixes gave, and the parts' memory)
                 const float top = topShared[row];
                 const float largest = fmaxf(refShared[0][row], refShared[1][row]);
                 sum = sumShared[0][row] * exp2_fast(refShared[0][row] - largest) + sumShared[1][row] * exp2_fast(refShared[1][row] - largest);
@@ -982,6 +990,11 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                 if (!whole) {
                     if (there && wg == 0) args.stats[part * kRows + row] = make_float4(top, largest, sum, 0.0f);
                     const uint32_t c0 = cta_of(w.first + kUnitCost), c1 = cta_of(w.first + kUnitCost + w.q.tiles - 1), parts = c1 - c0 + 1;
+                    if constexpr (kPrefix) {  // (joined by a launch of their own: the last to arrive would take 13 us for ten)
+                        if (w.t0 == 0) firstPart = make_uint4(w.q.firstRow, w.q.tokens, w.head, parts);
+                        if (!meet()) break;
+                        continue;
+                    }
                     // whether this is the last of `expected` CTAs; then what they wrote is there
                     auto arrive = [&](uint32_t *counter, uint32_t expected) {
                         if (!meet()) return false;
@@ -1040,18 +1053,10 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                             }
                             if (last) {
                                 float f = weights == 0.0f ? 0.0f : exp2_fast(all - level) / weights;
-                                if constexpr (kPrefix || kSuffix) {
+                                if constexpr (kSuffix) {
                                     const size_t place = shared_place(mine / group, mine % group);
-                                    float *values = a.shared.values + place * DIM + d;
-                                    if constexpr (kPrefix) {
-                                        if (d == 0) a.shared.stats[place] = make_float2(level, weights * kUnweight);
-#pragma unroll
-                                        for (uint32_t k = 0; k < 4; ++k) {
-                                            *reinterpret_cast<float4 *>(values + 8 * k) = make_float4(v[2 * k] * f, v[8 + 2 * k] * f, v[16 + 2 * k] * f, v[24 + 2 * k] * f);
-                                            *reinterpret_cast<float4 *>(values + 8 * k + 4) = make_float4(v[2 * k + 1] * f, v[9 + 2 * k] * f, v[17 + 2 * k] * f, v[25 + 2 * k] * f);
-                                        }
-                                        continue;
-                                    } else if (w.q.joins) {
+                                    const float *values = a.shared.values + place * DIM + d;
+                                    if (w.q.joins) {
                                         float keep;
                                         const float g = join_prefix(place, level, weights, keep);
                                         f *= keep;
@@ -1099,8 +1104,14 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                 }
                 if (!meet()) break;  // (before the next unit's words in shared memory)
             }
+            if constexpr (kPrefix) {
+                if (warp == (uint32_t)kFirstRowWarp && lane == 0) a.shared.parts[cta] = firstPart;
+            }
+        } else if constexpr (kPrefix) {
+            if (warp == (uint32_t)kFirstRowWarp && lane == 0) a.shared.parts[cta] = make_uint4(0u, 0u, 0u, 0u);
         }
     }
+    if constexpr (kSuffix) pdl_wait();  // (this launch is not over before the one in front)
     // every role is done, or gave up after a bounded wait; copies and products have landed
     tc_fence_before();
     __syncthreads();
@@ -1109,12 +1120,67 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
     if (warp == (uint32_t)kMmaWarp) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
 }
 
+// The parts of a prefix's units joined, in the CTAs' order: a CTA takes sixteen values of one unit's rows, a thread a row.  Bound by latency:
+// four parts' loads in flight.
+template <int DIM>
+__global__ void __launch_bounds__(kTileRows) k_join_prefix(const __grid_constant__ TilesArgs args) {
+    constexpr float kUnweight = 1.0f / (1u << (int)kWeightScale);
+    constexpr uint32_t kAtOnce = 4;
+    const AttendArgs &a = args.a;
+    const uint32_t row = threadIdx.x, c0 = blockIdx.x, block = blockIdx.y / 2, half = blockIdx.y % 2, group = a.heads / a.kvHeads;
+    pdl_trigger();  // (the successor reads what is older than the launch in front before it waits, and that was complete when this one began)
+    pdl_wait();
+    const uint4 unit = a.shared.parts[c0];  // first row, rows, head, parts
+    if (row >= unit.y * group || unit.w == 0u) return;
+    auto slot_of = [&](uint32_t k) { return 2 * (c0 + k) + (k == 0 ? 1u : 0u); };
+    float all = kNone, level = kNone, weights = 0.0f, v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = 0.0f;
+    for (uint32_t k0 = 0; k0 < unit.w; k0 += kAtOnce) {
+        float4 st[kAtOnce], t[kAtOnce][4];
+#pragma unroll
+        for (uint32_t k = 0; k < kAtOnce; ++k) {
+            const uint32_t slot = slot_of(min(k0 + k, unit.w - 1u));
+            st[k] = __ldcg(args.stats + slot * kRows + row);
+            // columns of the block of 32: four at 4 half + 8 i, values i and i + 4 of runs 2 half and 2 half + 1 of eight
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) t[k][i] = __ldcg(reinterpret_cast<const float4 *>(args.partials) + ((size_t)slot * (DIM / 4) + block * 8 + half + 2 * i) * kRows + row);
+        }
+        float next = all, nextLevel = level;
+#pragma unroll
+        for (uint32_t k = 0; k < kAtOnce; ++k) next = fmaxf(next, st[k].x), nextLevel = fmaxf(nextLevel, st[k].y);
+        const float keep = exp2_fast(all - next);
+        weights *= exp2_fast(level - nextLevel);
+        all = next, level = nextLevel;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] *= keep;
+#pragma unroll
+        for (uint32_t k = 0; k < kAtOnce; ++k) {
+            if (k0 + k >= unit.w) break;
+            const float g = exp2_fast(st[k].x - all);
+            weights = fmaf(st[k].z, exp2_fast(st[k].y - level), weights);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[i] = fmaf(t[k][i].x, g, v[i]), v[i + 4] = fmaf(t[k][i].y, g, v[i + 4]);
+                v[8 + i] = fmaf(t[k][i].z, g, v[8 + i]), v[12 + i] = fmaf(t[k][i].w, g, v[12 + i]);
+            }
+        }
+    }
+    const float f = weights == 0.0f ? 0.0f : exp2_fast(all - level) / weights;
+    const size_t place = (size_t)(unit.x + row / group) * a.heads + unit.z * group + row % group;
+    if (blockIdx.y == 0) a.shared.stats[place] = make_float2(level, weights * kUnweight);
+    float4 *to = reinterpret_cast<float4 *>(a.shared.values + place * DIM + block * 32 + half * 16);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) to[i] = make_float4(v[4 * i] * f, v[4 * i + 1] * f, v[4 * i + 2] * f, v[4 * i + 3] * f);
+}
+
 KernelSmemMemo tilesMemo[3][3];
 
 template <TilesOf OF, int DIM>
 bool launch_tiles(FFAttention *att, KernelSmemMemo &memo, const CUtensorMap &codes, const CUtensorMap &words, const TilesArgs &args, cudaStream_t stream, const char **error) {
     if (!memo.prepare(k_attend_tiles<DIM, OF>, att->device, tiles_smem(DIM), kTilesThreads, nullptr, error)) return false;
-    return launched(att, launch_pdl(k_attend_tiles<DIM, OF>, dim3(att->smCount), dim3(kTilesThreads), tiles_smem(DIM), stream, codes, words, args), "k_attend_tiles", error);
+    return launched(att, launch_pdl(k_attend_tiles<DIM, OF>, dim3(att->smCount), dim3(kTilesThreads), tiles_smem(DIM), stream, codes, words, args), "k_attend_tiles", error) &&
+           (OF != TilesOf::kPrefix || launched(att, launch_pdl(k_join_prefix<DIM>, dim3(att->smCount, DIM / 16), dim3(kTileRows), 0, stream, args), "k_join_prefix", error));
 }
 
 }  // namespace

@@ -6,6 +6,9 @@
 
 namespace ff {
 
+constexpr uint32_t kBlockKeys = 64;
+constexpr uint32_t kSharedLaunch = 180000;  // what the launches over prefixes take besides their tiles, 0.1 ns
+
 bool launch_attend(FFAttention *att, const AttendArgs &a, cudaStream_t stream, const char **error) {
     // Columns of a key/value head: up to 16 as columns of mma.sync, which then take as long as the cache's bytes; more as rows of
     // tcgen05.mma.  us as columns / as rows: 16 columns of 128, 64 requests of up to 16384 keys 72 / 98; 32 of 128, 16 requests of
@@ -16,15 +19,30 @@ bool launch_attend(FFAttention *att, const AttendArgs &a, cudaStream_t stream, c
     return launch_attend_tiles(att, a, stream, error);
 }
 
-// Two launches: the groups' rows over their prefixes, then the requests' rows from behind them.  Each goes to the kernel that its columns
-// ask for, as above; those of a group are all its rows' (bounded by the rows of the call).
-bool launch_attend_shared(FFAttention *att, AttendArgs a, cudaStream_t stream, const char **error) {
-    const uint64_t group = a.heads / a.kvHeads;
-    const uint32_t maxRows = a.maxRows;
-    a.maxRows = a.tokens;
-    if (!(a.tokens * group <= 16 ? launch_attend_prefix_rows(att, a, stream, error) : launch_attend_prefix_tiles(att, a, stream, error))) return false;
-    a.maxRows = maxRows;
-    return maxRows * group <= 16 ? launch_attend_suffix_rows(att, a, stream, error) : launch_attend_suffix_tiles(att, a, stream, error);
+// The groups' rows over their prefixes, then the requests' rows from behind them.  Each goes to the kernel that its columns ask for, as above;
+// those of a group are all its rows' (bounded by the rows of the call; at 256 values a head eight, where more spill registers).
+bool launch_attend_shared(FFAttention *att, AttendArgs a, bool always, cudaStream_t stream, const char **error) {
+    const uint32_t group = a.heads / a.kvHeads, maxRows = a.maxRows, dim = att->cfg.headDim, size = dim == 256 ? 2 : dim == 128 ? 1 : 0;
+    const bool fewOfRequest = (uint64_t)maxRows * group <= 16, fewOfGroup = (uint64_t)a.tokens * group <= (dim == 256 ? 8 : 16);
+    // Time in units of 0.1 ns that the GPU takes for a tile of 64 keys: on the kernel for few rows (by columns 4, 8, 16), for many.
+    static const uint32_t rowsCost[3][3] = {{18, 22, 32}, {28, 34, 50}, {50, 60, 110}}, tilesCost[3] = {40, 52, 81};
+    const uint64_t columns = (uint64_t)std::min(maxRows, a.tokens) * group;
+    const uint32_t of = columns <= 4 ? 0 : columns <= 8 ? 1 : 2, tileColumns = fewOfRequest ? 4u << of : kTileRows;
+    SharedPrefix &p = a.shared;
+    p.requestCost = (fewOfRequest ? rowsCost[size][of] : tilesCost[size]) * a.kvHeads * ((group + tileColumns - 1) / tileColumns);
+    p.requestRows = std::max(1u, tileColumns / group);
+    p.groupCost = (fewOfGroup ? rowsCost[size][2] : tilesCost[size]) * a.kvHeads;
+    p.groupRows = std::max(1u, (fewOfGroup ? 16u : kTileRows) / group);
+    p.least = always ? 0 : kSharedLaunch;
+    // (no prefix that the table has room for would be worth it)
+    const uint64_t most = ((uint64_t)std::min(a.tokens, a.requests) * ((std::min(maxRows, a.tokens) + p.requestRows - 1) / p.requestRows)) * p.requestCost * (a.tableKeys / kBlockKeys) * p.groups;
+    p.launched = p.groups && (always || most > p.least);
+    if (p.launched) {
+        a.maxRows = a.tokens;
+        if (!(fewOfGroup ? launch_attend_prefix_rows(att, a, stream, error) : launch_attend_prefix_tiles(att, a, stream, error))) return false;
+        a.maxRows = maxRows;
+    }
+    return fewOfRequest ? launch_attend_suffix_rows(att, a, stream, error) : launch_attend_suffix_tiles(att, a, stream, error);
 }
 
 }  // namespace ff
@@ -89,16 +107,15 @@ bool check_table(const uint32_t *blockTable, uint32_t tableStride, const uint32_
     return true;
 }
 
-constexpr uint32_t kSelectBlock = 64;  // keys
 constexpr uint32_t kMostListed = 1u << 20;
 
-// The workspace of ff_attention_shared: a word, the rows' maxima and sums, their values.
+// The workspace of ff_attention_shared: units in parts, the rows' maxima and sums, their values.
 struct SharedLayout {
     uint64_t stats, values, bytes;
 };
 SharedLayout shared_layout(const FFAttentionConfig &c, uint32_t tokens) {
     const uint64_t rows = (uint64_t)tokens * c.heads;
-    SharedLayout l{16, 0, 0};
+    SharedLayout l{kSharedCtas * sizeof(uint4), 0, 0};
     l.values = (l.stats + rows * sizeof(float2) + 15) / 16 * 16;
     l.bytes = l.values + rows * c.headDim * sizeof(float);
     return l;
@@ -348,7 +365,7 @@ bool ff_select_blocks(FFAttention *att, const uint16_t *q, uint32_t qStride, uin
     if ((uint64_t)pageCount * c.pageTokens >= FF_NO_SLOT) return fail(error, "the cache has more slots than 32 bits name");
     const uint64_t keys = (uint64_t)tableStride * c.pageTokens;
     if (keys > 1u << 21) return fail(error, "block table rows of more than 2^21 keys: their scores do not fit a CTA");
-    return launch_select_blocks(att, q, qStride, tokens, means, pageCount, blockTable, tableStride, (uint32_t)((keys + kSelectBlock - 1) / kSelectBlock), rowStart,
+    return launch_select_blocks(att, q, qStride, tokens, means, pageCount, blockTable, tableStride, (uint32_t)((keys + kBlockKeys - 1) / kBlockKeys), rowStart,
                                 lengths, requests, blocks, first, last, ids, static_cast<cudaStream_t>(stream), error);
 }
 
@@ -376,7 +393,7 @@ uint64_t ff_attention_shared_bytes(const FFAttentionConfig *config, uint32_t tok
 
 bool ff_attention_shared(FFAttention *att, const uint16_t *q, uint32_t qStride, uint32_t tokens, const void *pages, uint32_t pageCount,
                          const uint32_t *blockTable, uint32_t tableStride, const uint32_t *rowStart, const uint32_t *lengths, uint32_t requests,
-                         uint32_t maxRows, const uint32_t *groupStart, const uint32_t *prefixLengths, uint32_t groups, float scale, void *workspace,
+                         uint32_t maxRows, const uint32_t *groupStart, const uint32_t *prefixLengths, uint32_t groups, bool always, float scale, void *workspace,
                          uint16_t *out, uint32_t outStride, void *stream, const char **error) {
     if (!begin(att, error)) return false;
     const FFAttentionConfig &c = att->cfg;
@@ -395,8 +412,9 @@ bool ff_attention_shared(FFAttention *att, const uint16_t *q, uint32_t qStride, 
     uint8_t *w = static_cast<uint8_t *>(workspace);
     AttendArgs a{q, out, qStride, outStride, tokens, static_cast<const uint8_t *>(pages), pageCount, tableStride, table_keys(c, tableStride), blockTable,
                  rowStart, lengths, requests, std::min(maxRows, tokens), scale, 0, 0, c.heads, c.kvHeads, page_layout(c), att->errorFlag, nullptr, 0,
-                 {groupStart, prefixLengths, groups, reinterpret_cast<uint32_t *>(w), reinterpret_cast<float2 *>(w + l.stats), reinterpret_cast<float *>(w + l.values)}};
-    return launch_attend_shared(att, a, static_cast<cudaStream_t>(stream), error);
+                 {groupStart, prefixLengths, groups, 0, 0, 1, 0, 1, 0, reinterpret_cast<uint4 *>(w), reinterpret_cast<float2 *>(w + l.stats), reinterpret_cast<float *>(w + l.values)}};
+    if (att->smCount > (int)kSharedCtas) return fail(error, "more SMs than the workspace has room for");
+    return launch_attend_shared(att, a, always, static_cast<cudaStream_t>(stream), error);
 }
 
 }  // extern "C"

@@ -90,42 +90,45 @@ __device__ __forceinline__ uint32_t add_work(uint32_t a, uint32_t b) { return a 
 __device__ __forceinline__ uint32_t work_of(uint32_t tiles, uint32_t units) { return __umulhi(tiles, units) ? kTooMuch : tiles * units; }
 
 // A group of requests that share a prefix: its rows, its first request, and the keys of the prefix in whole tiles (the others are
-// walked with the requests' own).
+// walked with the requests' own).  None where walking them for the group is not shorter, or more than 32 bits count.
 struct SharedGroup {
     uint32_t firstRow, rows, request, keys;
 };
-__device__ __forceinline__ uint32_t prefix_keys(const AttendArgs &a, uint32_t g, uint32_t first) {  // no longer than its first request
-    return min(min(__ldg(a.shared.prefixLengths + g), a.tableKeys), min(__ldg(a.lengths + first), 0x7FFFFFFFu)) / kTileKeys * kTileKeys;
-}
 __device__ __forceinline__ SharedGroup shared_group(const AttendArgs &a, uint32_t g) {
-    const uint32_t first = min(__ldg(a.shared.groupStart + g), a.requests), last = min(__ldg(a.shared.groupStart + g + 1), a.requests);
+    const SharedPrefix &p = a.shared;
+    const uint32_t first = min(__ldg(p.groupStart + g), a.requests), last = min(__ldg(p.groupStart + g + 1), a.requests);
     SharedGroup s{0u, 0u, first, 0u};
     if (first >= last) return s;
     const uint32_t begin = min(__ldg(a.rowStart + first), a.tokens), end = min(__ldg(a.rowStart + last), a.tokens);
+    if (begin >= end) return s;
     s.firstRow = begin;
-    s.rows = end > begin ? end - begin : 0u;
-    s.keys = prefix_keys(a, g, first);
+    s.rows = end - begin;
+    const uint32_t tiles = min(min(__ldg(p.prefixLengths + g), a.tableKeys), min(__ldg(a.lengths + first), 0x7FFFFFFFu)) / kTileKeys;  // (no longer than its first request)
+    // (in whole numbers: every launch of a call comes to the same)
+    const unsigned long long requests = last - first, each = (s.rows + requests - 1) / requests;
+    const unsigned long long apart = requests * ((each + p.requestRows - 1) / p.requestRows) * p.requestCost, together = (unsigned long long)((s.rows + p.groupRows - 1) / p.groupRows) * p.groupCost;
+    const bool shorter = p.least == 0u || (apart > together && (apart - together) * tiles * p.groups > p.least);
+    const bool counted = (unsigned long long)s.rows * a.heads * p.groups < 1ull << 32 && (unsigned long long)s.rows * a.heads * p.groups * (tiles + 64ull) < 1ull << 32;
+    s.keys = shorter && counted ? tiles * kTileKeys : 0u;
     return s;
 }
 // The keys of request r's prefix, as its rows from position p0 on take them from the group's launch: none where the first of them does not
 // see them all (the request then walks all of its keys by itself), or where r is in no group.
 __device__ __forceinline__ uint32_t shared_keys(const AttendArgs &a, uint32_t r, int p0) {
+    if (!a.shared.launched) return 0u;
     uint32_t low = 0, high = a.shared.groups;
     while (high - low > 1) {
         const uint32_t mid = (low + high) >> 1;
         if (__ldg(a.shared.groupStart + mid) <= r) low = mid;
         else high = mid;
     }
-    if (a.shared.groups == 0) return 0u;
-    const uint32_t first = __ldg(a.shared.groupStart + low);
-    if (r < first || r >= __ldg(a.shared.groupStart + low + 1)) return 0u;
-    const uint32_t keys = prefix_keys(a, low, first);
+    if (r < __ldg(a.shared.groupStart + low) || r >= __ldg(a.shared.groupStart + low + 1)) return 0u;
+    const uint32_t keys = shared_group(a, low).keys;
     return p0 >= 0 && (uint32_t)p0 + 1u >= keys ? keys : 0u;
 }
-// Whether the thread's share of the groups goes back, or of the row starts (groups' rows could overlap then); behind the prefix launch (kSaid): or that wrote nothing.
-template <bool kSaid>
+// Whether the thread's share of the groups goes back, or of the row starts (groups' rows could overlap then).
 __device__ __forceinline__ bool shared_refused(const AttendArgs &a, uint32_t thread, uint32_t threads) {
-    bool back = kSaid && __ldcg(a.shared.refused) != 0u;
+    bool back = false;
     for (uint32_t g = thread; g < a.shared.groups; g += threads) back |= __ldg(a.shared.groupStart + g + 1) < __ldg(a.shared.groupStart + g);
     for (uint32_t r = thread; r < a.requests; r += threads) back |= __ldg(a.rowStart + r + 1) < __ldg(a.rowStart + r);
     return back;

@@ -21,10 +21,10 @@ class Shared(Batch):
                 self.table[r, :have] = self.table[groups[g], :have]
         self.slots = [[int(self.table[r, p // page]) * page + p % page for p in range(n)] for r, n in enumerate(self.lengths)]
 
-    def shared(self, scale=None, maxRows=None, **more):
+    def shared(self, scale=None, maxRows=None, always=True, **more):
         start = np.concatenate([[0], np.cumsum(self.rows)])
         return self.ctx.attendShared(self.q, self.cache, ints(self.table), ints(start), ints(self.lengths), max(self.rows + [1]) if maxRows is None else maxRows,
-                                     ints(self.groups), ints(self.prefix), scale=scale, **more)
+                                     ints(self.groups), ints(self.prefix), scale=scale, always=always, **more)
 
 
 # few columns in both launches, many in the first alone, many in both
@@ -86,7 +86,7 @@ def test_rows_without_keys_and_of_no_request_are_zero(rows):
     out = b.shared(out=torch.full_like(b.q, 7.0))
     assert not out[sum(rows):].any() and not out[rows[0]].any() and out[:rows[0]].any()
     b.check(out)
-    out = b.ctx.attendShared(b.q, b.cache, ints(b.table), ints([2, 3, 4, 4]), ints([140, 140, 0]), 2, ints([0, 2]), ints([128]), out=torch.full_like(b.q, 7.0))
+    out = b.ctx.attendShared(b.q, b.cache, ints(b.table), ints([2, 3, 4, 4]), ints([140, 140, 0]), 2, ints([0, 2]), ints([128]), always=True, out=torch.full_like(b.q, 7.0))
     assert not out[:2].any() and out[2].any() and not out[4:].any()
     out = b.ctx.attendShared(b.q, b.cache, ints(np.zeros((0, 3))), ints([0]), ints([]), 1, ints([0]), ints([]), out=torch.full_like(b.q, 7.0))
     assert not out.any() and b.ctx.info().deviceErrorFlag == 0
@@ -176,7 +176,7 @@ def test_a_prefix_longer_than_what_the_requests_hold():
 def test_row_starts_and_groups_that_go_back_are_reported(rows):
     b = Shared(4, 2, 64, 16, [200, 190, 180], [rows] * 3, [0, 3], [128])
     for start, groups in (([0, 2 * rows, rows, 3 * rows], [0, 3]), ([0, rows, 2 * rows, 3 * rows], [2, 0, 3])):
-        out = b.ctx.attendShared(b.q, b.cache, ints(b.table), ints(start), ints(b.lengths), 2 * rows, ints(groups), ints([128] * (len(groups) - 1)), out=torch.full_like(b.q, 7.0))
+        out = b.ctx.attendShared(b.q, b.cache, ints(b.table), ints(start), ints(b.lengths), 2 * rows, ints(groups), ints([128] * (len(groups) - 1)), always=True, out=torch.full_like(b.q, 7.0))
         assert not out.any() and b.ctx.info().deviceErrorFlag == 15
         b.ctx.resetDeviceError()
     b.check(b.shared())
@@ -190,7 +190,7 @@ def test_more_work_than_a_call_counts_is_reported(rows):
     ctx = context(1024, 1024, 64, 16, requests=1, tokens=rows)
     q = rows_of(generator(), rows, 1024, 64)
     table = torch.full((1, 1 << 27), -1, dtype=torch.int32, device="cuda")
-    out = ctx.attendShared(q, ctx.newCache(1), table, ints([0, rows]), ints([2 ** 31 - 1]), rows, ints([0, 1]), ints([2 ** 31 - 1 - rows]), out=torch.full_like(q, 7.0))
+    out = ctx.attendShared(q, ctx.newCache(1), table, ints([0, rows]), ints([2 ** 31 - 1]), rows, ints([0, 1]), ints([2 ** 31 - 1 - rows]), always=True, out=torch.full_like(q, 7.0))
     assert not out.any()
     assert ctx.info().deviceErrorFlag == 19
 
@@ -208,13 +208,13 @@ def test_strides_streams_and_graphs(rows):
     args = ints(b.table), ints([0, rows, 2 * rows, tokens]), ints(b.lengths), rows, ints(b.groups), ints(b.prefix)
     stream = torch.cuda.Stream()
     stream.wait_stream(torch.cuda.current_stream())
-    b.ctx.attendShared(wide[:, heads:2 * heads], b.cache, *args, out=out[:, :heads], stream=stream)
+    b.ctx.attendShared(wide[:, heads:2 * heads], b.cache, *args, always=True, out=out[:, :heads], stream=stream)
     stream.synchronize()
     assert torch.equal(out[:, :heads], want) and (out[:, heads:] == 7.0).all()
     out = torch.empty_like(want)
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
-        b.ctx.attendShared(b.q, b.cache, *args, out=out)
+        b.ctx.attendShared(b.q, b.cache, *args, always=True, out=out)
     for lengths, prefix in (([700, 600 + rows, 650], [576]), ([650, 600, 640], [512]), ([576 + rows, 600, 10], [576])):
         b.lengths = lengths
         b.slots = [[int(b.table[r, p // page]) * page + p % page for p in range(n)] for r, n in enumerate(lengths)]
@@ -230,6 +230,12 @@ def test_many_requests():
     requests = 1000
     b = Shared(2, 1, 64, 64, [70 + r % 60 for r in range(requests)], [1 if r % 3 else 0 for r in range(requests)], list(range(0, requests + 1, 5)), [64] * 200)
     b.check(b.shared())
+
+
+@pytest.mark.parametrize("requests,rows,prefix", [(2, 1, 128), (40, 1, 6400), (12, 9, 6400), (3, 200, 640)])
+def test_where_sharing_is_chosen_by_its_cost(requests, rows, prefix):
+    b = Shared(8, 2, 128, 64, [prefix + rows + 11 * r % 90 for r in range(requests)], [rows] * requests, [0, requests], [prefix])
+    b.check(b.shared(always=False))
 
 
 def test_refusals():
