@@ -243,17 +243,20 @@ class AttentionContext:
         return out
 
     def attendShared(self, q: torch.Tensor, pages: torch.Tensor, blockTable: torch.Tensor, rowStart: torch.Tensor,
-                     lengths: torch.Tensor, maxRows: int, groupStart: torch.Tensor, prefixLengths: torch.Tensor, *, always: bool = False,
+                     lengths: torch.Tensor, maxRows: int, groupStart: torch.Tensor, prefixLengths: torch.Tensor, *,
+                     maxPrefix: Optional[int] = None, always: bool = False,
                      scale: Optional[float] = None, out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
         """`attend` without a window, where requests groupStart[g] .. groupStart[g + 1] - 1 hold the same first prefixLengths[g]
-        keys on the same pages: these are read once for all rows of the group, where that is shorter (always: in any case)."""
+        keys on the same pages: these are read once for all rows of the group, where that is shorter (always: in any case).  maxPrefix:
+        no prefix is longer (without it, than a row of the block table), which it goes by."""
         tokens, requests, groups, shape = q.shape[0], lengths.numel(), prefixLengths.numel(), blockTable.shape
         if rowStart.numel() != requests + 1 or len(shape) != 2 or shape[0] != requests:
             raise ValueError("lengths, blockTable and rowStart must agree on the number of requests")
         if groupStart.numel() != groups + 1:
             raise ValueError("groupStart must have one entry more than prefixLengths")
-        if maxRows < 0:
-            raise ValueError("maxRows must not be negative")
+        if maxRows < 0 or (maxPrefix is not None and maxPrefix < 0):
+            raise ValueError("maxRows and maxPrefix must not be negative")
+        longest = _WORD if always else _WORD - 1 if maxPrefix is None else min(maxPrefix, _WORD - 1)
         if out is None:
             out = self._new((tokens, self.heads, self.headDim), torch.bfloat16, stream)
         self._ints("blockTable rowStart lengths groupStart prefixLengths", blockTable, rowStart, lengths, groupStart, prefixLengths)
@@ -262,7 +265,7 @@ class AttentionContext:
             bytes_ = self._sharedBytes.setdefault(tokens, binding.load().ff_attention_shared_bytes(ctypes.byref(self.config), tokens))
         workspace = self._new((bytes_,), torch.uint8, stream)
         call("ff_attention_shared", self.handle, *self._heads(q, self.heads, tokens, "q"), tokens, *self._cache(pages), blockTable.data_ptr(), shape[1],
-             rowStart.data_ptr(), lengths.data_ptr(), requests, min(maxRows, _WORD), groupStart.data_ptr(), prefixLengths.data_ptr(), groups, always,
+             rowStart.data_ptr(), lengths.data_ptr(), requests, min(maxRows, _WORD), groupStart.data_ptr(), prefixLengths.data_ptr(), groups, longest,
              self.headDim ** -0.5 if scale is None else scale, workspace.data_ptr(), *self._heads(out, self.heads, tokens, "out"),
              _stream(stream))
         return out

@@ -156,7 +156,7 @@ SIGNATURES = {
                                        c_uint32, c_float, _P, c_uint32, _P, _ERR]),
     "ff_attention_shared_bytes": (c_uint64, [POINTER(FFAttentionConfig), c_uint32]),
     "ff_attention_shared": (c_bool, [c_void_p, _P, c_uint32, c_uint32, _P, c_uint32, _P, c_uint32, _P, _P, c_uint32, c_uint32, _P,
-                                     _P, c_uint32, c_bool, c_float, _P, _P, c_uint32, _P, _ERR]),
+                                     _P, c_uint32, c_uint32, c_float, _P, _P, c_uint32, _P, _ERR]),
     "ff_rope_table": (c_bool, [c_void_p, POINTER(FFRopeConfig), _P, c_uint32, _P, _ERR]),
     "ff_rope": (c_bool, [c_void_p, _P, c_uint32, POINTER(FFRope), _P, c_uint32, c_uint32, _P, c_uint32, _P, _ERR]),
     "ff_cache_append": (c_bool, [c_void_p, _P, c_uint32, _P, c_uint32, _P, c_uint32, POINTER(FFRope), _P, _P, c_uint32,

@@ -156,8 +156,8 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    // (Behind a launch over the prefixes this one begins while that ends: what it reads of the caller's is from before both.)
-    if (!kSuffix || !a.shared.launched) pdl_enter();
+    // (Behind the launch over the prefixes this one begins while that ends: what it reads of the caller's is from before both.)
+    if (!kSuffix) pdl_enter();
 
     // ---- the plan: how many tiles each request is, and this CTA's run of them ----
     const uint32_t requests = kListed ? a.tokens : kPrefix ? a.shared.groups : a.requests;
@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
     if constexpr (!kPrefix) {
         const uint32_t covered = a.requests && !refused ? min(__ldg(a.rowStart + a.requests), a.tokens) : 0u;
         const uint32_t perRow = a.heads * DIM / 8;
-        if (OF != RowsOf::kRequest && covered)
+        if (kListed && covered)
             for (uint32_t row = blockIdx.x; row < min(__ldg(a.rowStart), covered); row += gridDim.x)
                 for (uint32_t i = tid; i < perRow; i += kRowsThreads) *reinterpret_cast<uint4 *>(a.out + (size_t)row * a.outStride + i * 8) = make_uint4(0u, 0u, 0u, 0u);
         for (uint32_t row = covered + blockIdx.x; row < a.tokens; row += gridDim.x)

@@ -239,8 +239,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xFFFFFFFFu, tmemSlot, 0);
-    // (Behind a launch over the prefixes this one begins while that ends: what it reads of the caller's is from before both.)
-    if (!kSuffix || !a.shared.launched) pdl_enter();
+    // (Behind the launch over the prefixes this one begins while that ends: what it reads of the caller's is from before both.)
+    if (!kSuffix) pdl_enter();
 
     // ---- the plan: row tiles of the requests, key tiles of those, this CTA's run ----
     // A request: its first row, rows, length; looked up once where there is a thread for each.
@@ -376,9 +376,6 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
     if constexpr (!kPrefix) {
         const uint32_t covered = a.requests && !refused ? min(__ldg(a.rowStart + a.requests), a.tokens) : 0u;
         const uint32_t perRow = a.heads * DIM / 8;
-        if (kSuffix && covered)
-            for (uint32_t row = blockIdx.x; row < min(__ldg(a.rowStart), covered); row += gridDim.x)
-                for (uint32_t i = tid; i < perRow; i += kTilesThreads) *reinterpret_cast<uint4 *>(a.out + (size_t)row * a.outStride + i * 8) = make_uint4(0u, 0u, 0u, 0u);
         for (uint32_t row = covered + blockIdx.x; row < a.tokens; row += gridDim.x)
             for (uint32_t i = tid; i < perRow; i += kTilesThreads) *reinterpret_cast<uint4 *>(a.out + (size_t)row * a.outStride + i * 8) = make_uint4(0u, 0u, 0u, 0u);
         if (blockIdx.x == 0) {

@@ -7,7 +7,7 @@
 namespace ff {
 
 constexpr uint32_t kBlockKeys = 64;
-constexpr uint32_t kSharedLaunch = 180000;  // what the launches over prefixes take besides their tiles, 0.1 ns
+constexpr uint32_t kSharedLaunch = 200000;  // what the launches over prefixes take besides their tiles, 0.1 ns
 
 bool launch_attend(FFAttention *att, const AttendArgs &a, cudaStream_t stream, const char **error) {
     // Columns of a key/value head: up to 16 as columns of mma.sync, which then take as long as the cache's bytes; more as rows of
@@ -20,28 +20,28 @@ bool launch_attend(FFAttention *att, const AttendArgs &a, cudaStream_t stream, c
 }
 
 // The groups' rows over their prefixes, then the requests' rows from behind them.  Each goes to the kernel that its columns ask for, as above;
-// those of a group are all its rows' (bounded by the rows of the call; at 256 values a head eight, where more spill registers).
-bool launch_attend_shared(FFAttention *att, AttendArgs a, bool always, cudaStream_t stream, const char **error) {
-    const uint32_t group = a.heads / a.kvHeads, maxRows = a.maxRows, dim = att->cfg.headDim, size = dim == 256 ? 2 : dim == 128 ? 1 : 0;
-    const bool fewOfRequest = (uint64_t)maxRows * group <= 16, fewOfGroup = (uint64_t)a.tokens * group <= (dim == 256 ? 8 : 16);
-    // Time in units of 0.1 ns that the GPU takes for a tile of 64 keys: on the kernel for few rows (by columns 4, 8, 16), for many.
-    static const uint32_t rowsCost[3][3] = {{18, 22, 32}, {28, 34, 50}, {50, 60, 110}}, tilesCost[3] = {40, 52, 81};
-    const uint64_t columns = (uint64_t)std::min(maxRows, a.tokens) * group;
-    const uint32_t of = columns <= 4 ? 0 : columns <= 8 ? 1 : 2, tileColumns = fewOfRequest ? 4u << of : kTileRows;
-    SharedPrefix &p = a.shared;
-    p.requestCost = (fewOfRequest ? rowsCost[size][of] : tilesCost[size]) * a.kvHeads * ((group + tileColumns - 1) / tileColumns);
-    p.requestRows = std::max(1u, tileColumns / group);
-    p.groupCost = (fewOfGroup ? rowsCost[size][2] : tilesCost[size]) * a.kvHeads;
-    p.groupRows = std::max(1u, (fewOfGroup ? 16u : kTileRows) / group);
-    p.least = always ? 0 : kSharedLaunch;
-    // (no prefix that the table has room for would be worth it)
-    const uint64_t most = ((uint64_t)std::min(a.tokens, a.requests) * ((std::min(maxRows, a.tokens) + p.requestRows - 1) / p.requestRows)) * p.requestCost * (a.tableKeys / kBlockKeys) * p.groups;
-    p.launched = p.groups && (always || most > p.least);
-    if (p.launched) {
-        a.maxRows = a.tokens;
-        if (!(fewOfGroup ? launch_attend_prefix_rows(att, a, stream, error) : launch_attend_prefix_tiles(att, a, stream, error))) return false;
-        a.maxRows = maxRows;
-    }
+// those of a group are all its rows' (bounded by the rows of the call; at 256 values a head eight, where more spill registers).  Or the requests'
+// launch alone, over all of their keys, where the other would take longer than it saves.  us alone / with both: 8 requests of 4 columns of
+// 128 behind 4096 keys 17.7 / 30.4, 16384 42 / 41; 64 behind 1024 31 / 35, 4096 80 / 42, 16384 271 / 62; 16 of 8 rows of 2 of 256 behind
+// 1024 48 / 46, 4096 103 / 55, 16384 324 / 83; 16 of 8 rows of 7 of 64 behind 16384 48 / 56.
+bool launch_attend_shared(FFAttention *att, const AttendArgs &a, uint32_t maxPrefix, cudaStream_t stream, const char **error) {
+    const uint32_t group = a.heads / a.kvHeads, dim = att->cfg.headDim, size = dim == 256 ? 2 : dim == 128 ? 1 : 0;
+    const uint32_t active = std::min(a.requests, a.tokens), rows = active ? std::min(a.maxRows, (a.tokens + active - 1) / active) : 0;  // requests with rows, and theirs (as if all had as many)
+    const bool fewOfRequest = (uint64_t)a.maxRows * group <= 16, fewOfGroup = (uint64_t)a.tokens * group <= (dim == 256 ? 8 : 16);
+    // what 64 keys cost a tile of columns, 0.1 ns of the whole GPU: of up to 4, 8 and 16, of 128 (where requests fill a part of them)
+    static const uint32_t few[3][3] = {{14, 15, 20}, {20, 21, 35}, {37, 42, 90}}, many[3] = {40, 44, 63}, full[3] = {50, 62, 78};
+    const uint64_t columns = (uint64_t)a.maxRows * group;
+    const uint32_t of = columns <= 4 ? 0 : columns <= 8 ? 1 : 2, width = fewOfRequest ? 4u << of : kTileRows;
+    auto tiles = [&](uint64_t n, uint32_t wide) {  // of n rows
+        return group <= wide ? (n + wide / group - 1) / (wide / group) : n * ((group + wide - 1) / wide);
+    };
+    const uint64_t apart = active * tiles(rows, width) * (fewOfRequest ? few[size][of] : many[size]);
+    const uint64_t together = std::max<uint64_t>(a.shared.groups, fewOfGroup ? tiles(a.tokens, 16) : tiles(a.tokens, kTileRows)) * (fewOfGroup ? few[size][dim == 256 ? 1 : 2] : full[size]);
+    const uint64_t keys = std::min(maxPrefix, a.tableKeys) / kBlockKeys;
+    if (!a.shared.groups || (maxPrefix != FF_SHARE_ALWAYS && (apart <= together || (apart - together) * keys * a.kvHeads <= kSharedLaunch))) return launch_attend(att, a, stream, error);
+    AttendArgs b = a;
+    b.maxRows = b.tokens;
+    if (!(fewOfGroup ? launch_attend_prefix_rows(att, b, stream, error) : launch_attend_prefix_tiles(att, b, stream, error))) return false;
     return fewOfRequest ? launch_attend_suffix_rows(att, a, stream, error) : launch_attend_suffix_tiles(att, a, stream, error);
 }
 
@@ -393,7 +393,7 @@ uint64_t ff_attention_shared_bytes(const FFAttentionConfig *config, uint32_t tok
 
 bool ff_attention_shared(FFAttention *att, const uint16_t *q, uint32_t qStride, uint32_t tokens, const void *pages, uint32_t pageCount,
                          const uint32_t *blockTable, uint32_t tableStride, const uint32_t *rowStart, const uint32_t *lengths, uint32_t requests,
-                         uint32_t maxRows, const uint32_t *groupStart, const uint32_t *prefixLengths, uint32_t groups, bool always, float scale, void *workspace,
+                         uint32_t maxRows, const uint32_t *groupStart, const uint32_t *prefixLengths, uint32_t groups, uint32_t maxPrefix, float scale, void *workspace,
                          uint16_t *out, uint32_t outStride, void *stream, const char **error) {
     if (!begin(att, error)) return false;
     const FFAttentionConfig &c = att->cfg;
@@ -412,9 +412,9 @@ bool ff_attention_shared(FFAttention *att, const uint16_t *q, uint32_t qStride, 
     uint8_t *w = static_cast<uint8_t *>(workspace);
     AttendArgs a{q, out, qStride, outStride, tokens, static_cast<const uint8_t *>(pages), pageCount, tableStride, table_keys(c, tableStride), blockTable,
                  rowStart, lengths, requests, std::min(maxRows, tokens), scale, 0, 0, c.heads, c.kvHeads, page_layout(c), att->errorFlag, nullptr, 0,
-                 {groupStart, prefixLengths, groups, 0, 0, 1, 0, 1, 0, reinterpret_cast<uint4 *>(w), reinterpret_cast<float2 *>(w + l.stats), reinterpret_cast<float *>(w + l.values)}};
+                 {groupStart, prefixLengths, groups, reinterpret_cast<uint4 *>(w), reinterpret_cast<float2 *>(w + l.stats), reinterpret_cast<float *>(w + l.values)}};
     if (att->smCount > (int)kSharedCtas) return fail(error, "more SMs than the workspace has room for");
-    return launch_attend_shared(att, a, always, static_cast<cudaStream_t>(stream), error);
+    return launch_attend_shared(att, a, maxPrefix, static_cast<cudaStream_t>(stream), error);
 }
 
 }  // extern "C"

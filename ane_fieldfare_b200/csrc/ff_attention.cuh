@@ -66,10 +66,6 @@ inline bool launched(FFAttention *att, cudaError_t status, const char *what, con
 struct SharedPrefix {
     const uint32_t *groupStart, *prefixLengths;
     uint32_t groups;
-    uint32_t launched;  // whether a launch over the prefixes goes before the requests'
-    // When a prefix is walked for its group: what 64 keys cost a tile of a request's rows and one of a group's, the rows of such tiles, and
-    // what is to be saved (0: always).
-    uint32_t requestCost, requestRows, groupCost, groupRows, least;
     uint4 *parts;   // [CTAs] the unit that a CTA has the first part of: first row, rows, head, parts
     float2 *stats;  // [tokens][heads] largest logit (log2), the weights' sum at it
     float *values;  // [tokens][heads][headDim] their mean of the values
@@ -133,6 +129,6 @@ bool launch_attend_suffix_tiles(FFAttention *att, const AttendArgs &args, cudaSt
 
 // ff_attention.cu
 bool launch_attend(FFAttention *att, const AttendArgs &args, cudaStream_t stream, const char **error);
-bool launch_attend_shared(FFAttention *att, AttendArgs args, bool always, cudaStream_t stream, const char **error);
+bool launch_attend_shared(FFAttention *att, const AttendArgs &args, uint32_t maxPrefix, cudaStream_t stream, const char **error);
 
 }  // namespace ff

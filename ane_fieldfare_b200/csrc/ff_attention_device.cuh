@@ -90,7 +90,7 @@ __device__ __forceinline__ uint32_t add_work(uint32_t a, uint32_t b) { return a 
 __device__ __forceinline__ uint32_t work_of(uint32_t tiles, uint32_t units) { return __umulhi(tiles, units) ? kTooMuch : tiles * units; }
 
 // A group of requests that share a prefix: its rows, its first request, and the keys of the prefix in whole tiles (the others are
-// walked with the requests' own).  None where walking them for the group is not shorter, or more than 32 bits count.
+// walked with the requests' own).  None where there is more work than 32 bits count.
 struct SharedGroup {
     uint32_t firstRow, rows, request, keys;
 };
@@ -104,18 +104,13 @@ __device__ __forceinline__ SharedGroup shared_group(const AttendArgs &a, uint32_
     s.firstRow = begin;
     s.rows = end - begin;
     const uint32_t tiles = min(min(__ldg(p.prefixLengths + g), a.tableKeys), min(__ldg(a.lengths + first), 0x7FFFFFFFu)) / kTileKeys;  // (no longer than its first request)
-    // (in whole numbers: every launch of a call comes to the same)
-    const unsigned long long requests = last - first, each = (s.rows + requests - 1) / requests;
-    const unsigned long long apart = requests * ((each + p.requestRows - 1) / p.requestRows) * p.requestCost, together = (unsigned long long)((s.rows + p.groupRows - 1) / p.groupRows) * p.groupCost;
-    const bool shorter = p.least == 0u || (apart > together && (apart - together) * tiles * p.groups > p.least);
     const bool counted = (unsigned long long)s.rows * a.heads * p.groups < 1ull << 32 && (unsigned long long)s.rows * a.heads * p.groups * (tiles + 64ull) < 1ull << 32;
-    s.keys = shorter && counted ? tiles * kTileKeys : 0u;
+    s.keys = counted ? tiles * kTileKeys : 0u;
     return s;
 }
 // The keys of request r's prefix, as its rows from position p0 on take them from the group's launch: none where the first of them does not
 // see them all (the request then walks all of its keys by itself), or where r is in no group.
 __device__ __forceinline__ uint32_t shared_keys(const AttendArgs &a, uint32_t r, int p0) {
-    if (!a.shared.launched) return 0u;
     uint32_t low = 0, high = a.shared.groups;
     while (high - low > 1) {
         const uint32_t mid = (low + high) >> 1;

@@ -583,18 +583,21 @@ bool ff_attention(FFAttention *attention, const uint16_t *q, uint32_t qStride, u
                   const uint32_t *lengths, uint32_t requests, uint32_t maxRows, float scale, uint32_t window,
                   uint32_t sinks, uint16_t *out, uint32_t outStride, void *stream, const char **error);
 
-/* ff_attention (every key up to the row's own) of requests that share prefixes: the requests groupStart[g] .. groupStart[g + 1] - 1 hold the same
- * first prefixLengths[g] keys, on pages that the block table row of the group's first request names and theirs name likewise.  The attention of
- * all rows of a group over those keys is one, as of one request: it reads them once.  (Whole tiles of 64 keys, and no more than the first
- * request holds; what is left of a prefix, and a request whose rows do not come behind it, is read by request.)  groupStart [groups + 1], ascending, prefixLengths [groups]; requests in no
- * group share nothing.  A groupStart or rowStart that goes back leaves every row zero (flag 15).  A prefix that is too short, or has too few rows behind
- * it, to make up for the further launches is read by request; `always` reads every one for its group (the results differ by rounding).
- * workspace: ff_attention_shared_bytes() of device memory for the call alone, 16-byte aligned.  Rows of no request are zero. */
+/* ff_attention (every key up to the row's own) of requests that share prefixes: the requests groupStart[g] .. groupStart[g + 1] - 1
+ * hold the same first prefixLengths[g] keys, on pages that the block table row of the group's first request names and theirs name
+ * likewise.  The attention of all rows of a group over those keys is one, as of one request: it reads them once.  (Whole tiles of
+ * 64 keys, and no more than the first request holds; what is left of a prefix, and a request whose rows do not come behind it, is
+ * read by request.)  groupStart [groups + 1], ascending, prefixLengths [groups]; requests in no group share nothing.
+ * maxPrefix: no prefix is longer.  It chooses the kernels: where such prefixes are too short, or have too few rows behind them, to
+ * make up for further launches, all keys are read by request and groupStart and prefixLengths not at all; FF_SHARE_ALWAYS: they are
+ * not, whatever that takes.  The two ways' results differ by rounding.  A groupStart that goes back leaves every row zero (flag 15), like
+ * such a rowStart.  workspace: ff_attention_shared_bytes() of device memory for the call alone, 16-byte aligned. */
+#define FF_SHARE_ALWAYS 0xFFFFFFFFu
 uint64_t ff_attention_shared_bytes(const FFAttentionConfig *config, uint32_t tokens);
 bool ff_attention_shared(FFAttention *attention, const uint16_t *q, uint32_t qStride, uint32_t tokens, const void *pages,
                          uint32_t pageCount, const uint32_t *blockTable, uint32_t tableStride, const uint32_t *rowStart,
                          const uint32_t *lengths, uint32_t requests, uint32_t maxRows, const uint32_t *groupStart,
-                         const uint32_t *prefixLengths, uint32_t groups, bool always, float scale, void *workspace,
+                         const uint32_t *prefixLengths, uint32_t groups, uint32_t maxPrefix, float scale, void *workspace,
                          uint16_t *out, uint32_t outStride, void *stream, const char **error);
 
 /* Attention over a part of a long context: blocks of 64 keys (positions 64 b .. 64 b + 63) chosen for every row and key/value
