@@ -3,10 +3,12 @@
     norm -> QKV product -> [rotary positions, INT4 cache, attention] -> output product -> fused setup -> router,
     shared FFN, routed experts -> combine -> fused tail
 
-`CacheBook` keeps the requests' lengths, block tables and free pages on the GPU; `DecoderLayer` is one layer's forward over the
-rows of a step, be they single tokens, blocks that are verified, prompts, or a mixture.  The two matrix products in front of and
-behind attention are plain library products.  `python -m ane_fieldfare_b200.decoder` runs a small one: a prompt, a block
-of which some rows are taken back, and single tokens.
+`CacheBook` keeps the requests' lengths, block tables and free pages on the GPU, and which requests share the pages of a prefix, whose
+attention is then computed once for all of them; `DecoderLayer` is one layer's forward over the rows of a step, be they single tokens,
+blocks that are verified, prompts, or a mixture.  A layer may attend to a part of a long context: for steps of few rows a request, the blocks whose
+mean keys a row's queries score highest.  The two matrix products in front of and behind attention are plain library products.
+`python -m ane_fieldfare_b200.decoder` runs a small one: a prompt, a block of which some rows are taken back, single tokens, and requests
+that go on from a shared prompt.
 """
 from __future__ import annotations
 
@@ -18,7 +20,7 @@ import torch
 from .attention import AttentionContext
 from .hotpath import HotpathContext, MoE, PrefillGroupedRoutedMoE, PrefillLayerGlue, PrefillMoE, PrefillRouter, PrefillSharedExpert
 
-__all__ = ["CacheBook", "DecoderLayer", "LayerWeights", "Step"]
+__all__ = ["CacheBook", "DecoderLayer", "LayerWeights", "Selection", "Step"]
 
 
 @dataclass
@@ -30,6 +32,10 @@ class Step:
     lengths: torch.Tensor
     blockTable: torch.Tensor
     maxRows: int
+    before: Optional[torch.Tensor] = None  # lengths in front of the step
+    groupStart: Optional[torch.Tensor] = None  # requests that share prefixes, where some do
+    prefixLengths: Optional[torch.Tensor] = None
+    maxPrefix: int = 0
 
 
 class CacheBook:
@@ -43,20 +49,88 @@ class CacheBook:
         self.freePages = torch.arange(pages - 1, -1, -1, dtype=i32, device=device)
         self.freeCount = torch.tensor([pages], dtype=i32, device=device)
         self._now = torch.zeros(requests, dtype=i32, device=device)
+        self.heldPages = torch.zeros(requests, dtype=i32, device=device)  # of a table row, the first that are another request's
+        self._prefix = [None] * requests  # (owner, pages) of the prefix that a request shares; the owner's own among them
+
+    def share(self, owner: int, requests: Sequence[int], tokens: int) -> int:
+        """`requests`, which have no tokens yet, go on from the first `tokens` of the owner's: as many as fill whole pages, which they
+        read and do not own.  Returns how many.  Requests that stand one behind the other have their attention over them in one."""
+        size = self.attention.pageTokens
+        pages = tokens // size
+        if not 0 <= tokens <= self.lengths[owner]:
+            raise ValueError(f"the owner holds {self.lengths[owner]} tokens")
+        if any(r == owner or self.lengths[r] or self._prefix[r] for r in requests):
+            raise ValueError("requests that share a prefix must have no tokens of their own yet")
+        if self._prefix[owner] and self._prefix[owner][0] != owner:
+            raise ValueError("the owner of a prefix must hold its pages itself")
+        if pages == 0 or not requests:
+            return 0
+        rows = torch.tensor(list(requests)).to(self.blockTable.device)
+        self.blockTable[rows, :pages] = self.blockTable[owner, :pages]
+        self.heldPages[rows] = pages
+        self._now = self._now.clone()  # (an earlier step's lengths are this tensor)
+        self._now[rows] = pages * size
+        for r in requests:
+            self.lengths[r], self._prefix[r] = pages * size, (owner, pages)
+        self._prefix[owner] = (owner, pages)
+        return pages * size
+
+    def _groups(self) -> tuple:
+        """(first requests and the end, prefix lengths) of the runs of requests that share a prefix."""
+        start, lengths, at = [], [], 0
+        while at < len(self._prefix):
+            prefix, first = self._prefix[at], at
+            while at < len(self._prefix) and self._prefix[at] == prefix:
+                at += 1
+            if prefix and at - first > 1:
+                if start and start[-1] != first:  # requests between two groups: a group that shares nothing
+                    lengths.append(0)
+                    start.append(first)
+                elif not start:
+                    start.append(first)
+                lengths.append(prefix[1] * self.attention.pageTokens)
+                start.append(at)
+        return start, lengths
 
     def step(self, newLengths: Sequence[int], maxRows: Optional[int] = None) -> Step:
         """Requests go to `newLengths` tokens: pages given back and taken, a row for every new token.  maxRows: a bound on
-        the new tokens of one request, where it has to be the same for several steps."""
+        the new tokens of one request, where it has to be the same for several steps.  A prefix stays as long as others share it."""
         new = list(newLengths)
+        for r, prefix in enumerate(self._prefix):
+            if prefix and prefix[0] != r and 0 < new[r] < prefix[1] * self.attention.pageTokens:
+                raise ValueError(f"request {r} shares its first {prefix[1] * self.attention.pageTokens} tokens")
+            if prefix and prefix[0] != r and new[r] and new[prefix[0]] < prefix[1] * self.attention.pageTokens:
+                raise ValueError(f"request {r} shares the first {prefix[1] * self.attention.pageTokens} tokens of request {prefix[0]}")
         rows = [max(0, b - a) for a, b in zip(self.lengths, new)]
         device, i32, total = self.attention.device, torch.int32, sum(rows)
         after = torch.tensor(new, dtype=i32).to(device)
         step = Step(torch.empty(len(new) + 1, dtype=i32, device=device), torch.empty(total, dtype=i32, device=device),
-                    torch.empty(total, dtype=i32, device=device), after, self.blockTable, max(rows + [1]) if maxRows is None else maxRows)
+                    torch.empty(total, dtype=i32, device=device), after, self.blockTable, max(rows + [1]) if maxRows is None else maxRows, self._now)
         self.attention.plan(self._now, after, self.blockTable, self.freePages, self.freeCount, self.freeCount, step.rowStart,
-                            step.positions, step.slots)
+                            step.positions, step.slots, heldPages=self.heldPages if any(self._prefix) else None)
+        gone = [r for r, prefix in enumerate(self._prefix) if prefix and prefix[0] != r and new[r] == 0]
+        if gone:
+            self.heldPages[torch.tensor(gone).to(device)] = 0
+            for r in gone:
+                self._prefix[r] = None
+            owners = {prefix[0] for r, prefix in enumerate(self._prefix) if prefix and prefix[0] != r}
+            self._prefix = [None if prefix and prefix[0] == r and r not in owners else prefix for r, prefix in enumerate(self._prefix)]
+        start, prefixes = self._groups()
+        if prefixes:
+            step.groupStart, step.prefixLengths = torch.tensor(start, dtype=i32).to(device), torch.tensor(prefixes, dtype=i32).to(device)
+            step.maxPrefix = max(prefixes)
         self.lengths, self._now = new, after
         return step
+
+
+@dataclass
+class Selection:
+    """Attention to a part of the context: `blocks` blocks of 64 keys a row and key/value head, the first and the last among them in
+    any case, in steps of up to `maxRows` rows a request (more of them read a block together by reading all)."""
+    blocks: int
+    first: int = 1
+    last: int = 1
+    maxRows: int = 16
 
 
 @dataclass
@@ -76,10 +150,14 @@ class DecoderLayer:
     """One layer: `layer` of the MoE context's resident layers behind attention over `pages` of a cache of its own."""
 
     def __init__(self, moe: HotpathContext, attention: AttentionContext, layer: int, weights: LayerWeights, ropeTable: torch.Tensor,
-                 pages: int, *, window: int = 0, sinks: int = 0, interleaved: bool = False, eps: float = 1e-6, layerScalar: float = 1.0):
+                 pages: int, *, window: int = 0, sinks: int = 0, interleaved: bool = False, eps: float = 1e-6, layerScalar: float = 1.0,
+                 selected: Optional[Selection] = None):
+        if selected and window:
+            raise ValueError("a layer with a window does not select blocks")
         self.moe, self.attention, self.layer, self.weights, self.ropeTable = moe, attention, layer, weights, ropeTable
         self.window, self.sinks, self.interleaved, self.eps, self.layerScalar = window, sinks, interleaved, eps, layerScalar
-        self.cache = attention.newCache(pages)
+        self.cache, self.selected = attention.newCache(pages), selected
+        self.means = attention.newMeans(pages) if selected else None
         self._ops = (MoE(moe), PrefillRouter(moe), PrefillSharedExpert(moe), PrefillGroupedRoutedMoE(moe), PrefillMoE(moe), PrefillLayerGlue(moe))
 
     def attend(self, x: torch.Tensor, step: Step) -> torch.Tensor:
@@ -88,6 +166,15 @@ class DecoderLayer:
         qkv = (x @ w.qkv.T).unflatten(1, (-1, att.headDim))
         q, k, v = qkv.split([att.heads, att.kvHeads, att.kvHeads], dim=1)
         q = att.append(q, k, v, self.ropeTable, step.positions, step.slots, self.cache, interleaved=self.interleaved)
+        if self.selected:
+            att.blockMeans(self.cache, step.blockTable, step.before, step.lengths, self.means)
+            if step.maxRows <= self.selected.maxRows:
+                ids = att.selectBlocks(q, self.means, step.blockTable, step.rowStart, step.lengths, self.selected.blocks, first=self.selected.first,
+                                       last=self.selected.last)
+                return att.attendSelected(q, self.cache, step.blockTable, step.rowStart, step.lengths, ids)
+        if step.groupStart is not None and not self.window:
+            return att.attendShared(q, self.cache, step.blockTable, step.rowStart, step.lengths, step.maxRows, step.groupStart, step.prefixLengths,
+                                    maxPrefix=step.maxPrefix)
         return att.attend(q, self.cache, step.blockTable, step.rowStart, step.lengths, step.maxRows, window=self.window, sinks=self.sinks)
 
     def forward(self, hidden: torch.Tensor, step: Step) -> torch.Tensor:
@@ -118,7 +205,8 @@ class DecoderLayer:
         return hidden
 
 
-def small_decoder(layers: int = 2, d: int = 256, requests: int = 2, pages: int = 64, seed: int = 1, **attention) -> tuple:
+def small_decoder(layers: int = 2, d: int = 256, requests: int = 2, pages: int = 64, seed: int = 1, selected: Optional[Selection] = None,
+                  **attention) -> tuple:
     """(CacheBook, layers) with random weights, for a demonstration or a test."""
     from . import workload
 
@@ -135,24 +223,34 @@ def small_decoder(layers: int = 2, d: int = 256, requests: int = 2, pages: int =
         norms = [(1 + 0.1 * torch.randn(d, device=att.device, generator=gen)).bfloat16() for _ in range(6)]
         weights = LayerWeights(draw((att.heads + 2 * att.kvHeads) * att.headDim, d), draw(d, att.heads * att.headDim), *norms)
         # every second layer sees a window and the first tokens
-        stack.append(DecoderLayer(moe, att, i, weights, table, pages, window=32 if i % 2 else 0, sinks=4 if i % 2 else 0))
+        stack.append(DecoderLayer(moe, att, i, weights, table, pages, window=32 if i % 2 else 0, sinks=4 if i % 2 else 0,
+                                  selected=None if i % 2 else selected))
     return book, stack
 
 
-def main():
-    book, stack = small_decoder()
+def _run(book: CacheBook, stack: Sequence[DecoderLayer], steps: Sequence[tuple]):
     device = book.attention.device
-    have = [0, 0]
-    for what, want in [("prompts", [70, 33]), ("a block of eight rows", [78, 41]), ("five of them taken back", [73, 36]),
-                       ("a token each", [74, 37]), ("one request ends", [75, 0])]:
-        rows = sum(max(0, b - a) for a, b in zip(have, want))
+    for what, want in steps:
+        rows = sum(max(0, b - a) for a, b in zip(book.lengths, want))
         hidden = torch.randn((rows, stack[0].moe.d), device=device).bfloat16()
         step = book.step(want)
         for layer in stack:
             layer.forward(hidden, step)
         torch.cuda.synchronize()
         print(f"{what}: {rows} rows, lengths {want}, {int(book.freeCount)} pages free" + (f", |hidden| {hidden.float().norm(dim=1).mean():.1f}" if rows else ""))
-        have = want
+
+
+def main():
+    book, stack = small_decoder()
+    _run(book, stack, [("prompts", [70, 33]), ("a block of eight rows", [78, 41]), ("five of them taken back", [73, 36]), ("a token each", [74, 37]),
+                       ("one request ends", [75, 0])])
+    print("error flag:", book.attention.info().deviceErrorFlag)
+    book, stack = small_decoder(requests=4, selected=Selection(blocks=3))
+    _run(book, stack, [("one prompt", [300, 0, 0, 0])])
+    shared = book.share(0, [1, 2, 3], 300)
+    print(f"three requests go on from its first {shared} tokens")
+    _run(book, stack, [("their questions", [300, shared + 20, shared + 33, shared + 5]), ("a token each", [301, shared + 21, shared + 34, shared + 6]),
+                       ("they end", [301, 0, 0, 0]), ("and their prompt", [0, 0, 0, 0])])
     print("error flag:", book.attention.info().deviceErrorFlag)
 
 
