@@ -49,6 +49,7 @@ class AttentionContext:
         self.maxRequests, self.maxTokens = maxRequests, maxTokens
         self.pageBytes = lib.ff_cache_page_bytes(ctypes.byref(self.config))
         self._sharedBytes = {}  # of attendShared's workspace, by rows
+        self._meanValues = kvHeads * max(1, pageTokens // BLOCK_KEYS) * headDim  # of a page
 
     @property
     def handle(self):
@@ -279,7 +280,7 @@ class AttentionContext:
     def _means(self, means: torch.Tensor) -> tuple:
         count = means.shape[0] if means.dim() else 0
         if (means.dtype is not torch.bfloat16 or means.get_device() != self._ordinal or not means.is_contiguous()
-                or means.numel() != count * self.kvHeads * max(1, self.pageTokens // BLOCK_KEYS) * self.headDim):
+                or means.numel() != count * self._meanValues):
             raise ValueError(f"mean keys are contiguous bf16 [pages][{self.kvHeads}][{max(1, self.pageTokens // BLOCK_KEYS)}][{self.headDim}] on {self.device}")
         return means.data_ptr(), count
 
@@ -305,7 +306,7 @@ class AttentionContext:
         tokens, requests, shape = q.shape[0], lengths.numel(), blockTable.shape
         if rowStart.numel() != requests + 1 or len(shape) != 2 or shape[0] != requests:
             raise ValueError("lengths, blockTable and rowStart must agree on the number of requests")
-        if not 0 <= first <= _WORD or not 0 <= last <= _WORD or not 0 <= blocks <= _WORD:
+        if not (0 <= first <= _WORD and 0 <= last <= _WORD and 0 <= blocks <= _WORD):
             raise ValueError("blocks, first and last must not be negative, or 2^32 and more")
         if ids is None:
             ids = self._new((tokens, self.kvHeads, blocks), torch.int32, stream)

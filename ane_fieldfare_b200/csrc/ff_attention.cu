@@ -98,8 +98,9 @@ bool check_requests(const FFAttention *att, uint32_t requests, const char **erro
     return true;
 }
 
-bool check_table(const uint32_t *blockTable, uint32_t tableStride, const uint32_t *rowStart, const uint32_t *lengths, uint32_t requests, const char **error) {
-    if (!rowStart || !aligned(rowStart, 4)) return fail(error, "rows' starts (or old lengths) must be non-null and 4-byte aligned");
+// the block table, and `starts` (one per request, or one more) and lengths; without requests `starts` alone
+bool check_table(const uint32_t *blockTable, uint32_t tableStride, const uint32_t *starts, const char *startsName, const uint32_t *lengths, uint32_t requests, const char **error) {
+    if (!starts || !aligned(starts, 4)) return fail(error, std::string(startsName) + " must be non-null and 4-byte aligned");
     if (requests == 0) return true;
     if (!lengths || !aligned(lengths, 4)) return fail(error, "lengths must be non-null and 4-byte aligned");
     if (!blockTable || !aligned(blockTable, 4)) return fail(error, "blockTable must be non-null and 4-byte aligned");
@@ -342,7 +343,7 @@ bool ff_block_means(FFAttention *att, const void *pages, uint32_t pageCount, con
     const FFAttentionConfig &c = att->cfg;
     if (!check_requests(att, requests, error)) return false;
     if (requests == 0) return true;
-    if (!check_cache(att, pages, pageCount, error) || !check_table(blockTable, tableStride, oldLengths, newLengths, requests, error)) return false;
+    if (!check_cache(att, pages, pageCount, error) || !check_table(blockTable, tableStride, oldLengths, "oldLengths", newLengths, requests, error)) return false;
     if (!means || !aligned(means, 16)) return fail(error, "means must be non-null and 16-byte aligned");
     return launch_block_means(att, static_cast<const uint8_t *>(pages), pageCount, blockTable, tableStride, table_keys(c, tableStride), oldLengths, newLengths,
                               requests, means, static_cast<cudaStream_t>(stream), error);
@@ -358,7 +359,7 @@ bool ff_select_blocks(FFAttention *att, const uint16_t *q, uint32_t qStride, uin
     if (first > blocks || last > blocks - first) return fail(error, "the first and the last blocks are more than a list holds");
     if (tokens == 0) return true;
     if (!check_tokens(att, tokens, error) || !check_heads(att, q, qStride, c.heads, "query", error) || !check_requests(att, requests, error) ||
-        !check_table(blockTable, tableStride, rowStart, lengths, requests, error))
+        !check_table(blockTable, tableStride, rowStart, "rowStart", lengths, requests, error))
         return false;
     if (!means || !aligned(means, 16)) return fail(error, "means must be non-null and 16-byte aligned");
     if (!ids || !aligned(ids, 4)) return fail(error, "ids must be non-null and 4-byte aligned");
@@ -379,7 +380,7 @@ bool ff_attention_selected(FFAttention *att, const uint16_t *q, uint32_t qStride
     if (tokens == 0) return true;
     if (!check_tokens(att, tokens, error) || !check_heads(att, q, qStride, c.heads, "query", error) ||
         !check_heads(att, out, outStride, c.heads, "output", error) || !check_cache(att, pages, pageCount, error) ||
-        !check_requests(att, requests, error) || !check_table(blockTable, tableStride, rowStart, lengths, requests, error))
+        !check_requests(att, requests, error) || !check_table(blockTable, tableStride, rowStart, "rowStart", lengths, requests, error))
         return false;
     if (!ids || !aligned(ids, 4)) return fail(error, "ids must be non-null and 4-byte aligned");
     AttendArgs a{q, out, qStride, outStride, tokens, static_cast<const uint8_t *>(pages), pageCount, tableStride, table_keys(c, tableStride), blockTable,
@@ -402,7 +403,7 @@ bool ff_attention_shared(FFAttention *att, const uint16_t *q, uint32_t qStride, 
     if (tokens == 0) return true;
     if (!check_tokens(att, tokens, error) || !check_heads(att, q, qStride, c.heads, "query", error) ||
         !check_heads(att, out, outStride, c.heads, "output", error) || !check_cache(att, pages, pageCount, error) ||
-        !check_requests(att, requests, error) || !check_table(blockTable, tableStride, rowStart, lengths, requests, error))
+        !check_requests(att, requests, error) || !check_table(blockTable, tableStride, rowStart, "rowStart", lengths, requests, error))
         return false;
     if (groups > requests) return fail(error, "more groups than requests");
     if (groups && (!groupStart || !prefixLengths || !aligned(groupStart, 4) || !aligned(prefixLengths, 4)))

@@ -229,3 +229,36 @@ def test_refusals():
         with pytest.raises(FieldfareError, match=says):
             call(**kw)
     assert call(q=b.q[:0], ids=ids[:0], rowStart=ints([0, 0])).shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("rows", [1, 20])
+def test_pages_behind_four_gigabytes(rows):
+    """Means, selected blocks and a shared prefix of keys whose pages lie past what 32 bits reach."""
+    heads, kvHeads, dim, page = 2, 2, 256, 256
+    ctx = context(heads, kvHeads, dim, page, requests=2, tokens=1300)
+    pages = (1 << 32) // ctx.pageBytes + 8
+    cache = torch.empty((pages, kvHeads, ctx.pageBytes // kvHeads), dtype=torch.uint8, device="cuda")
+    table = np.array([[pages - 1, 0, pages - 2, pages - 3], [pages - 1, 0, pages - 4, pages - 5]])
+    lengths, prefix = [900, 700], 512
+    gen = generator()
+    slots = [[int(table[r, p // page]) * page + p % page for p in range(n)] for r, n in enumerate(lengths)]
+    flat = slots[0] + slots[1][prefix:]
+    k, v, q = rows_of(gen, len(flat), kvHeads, dim), rows_of(gen, len(flat), kvHeads, dim), rows_of(gen, 2 * rows, heads, dim)
+    ctx.append(None, k, v, None, ints([0] * len(flat)), ints(flat), cache)
+    means = ctx.newMeans(pages)
+    start, held = ints([0, rows, 2 * rows]), ints(lengths)
+    ctx.blockMeans(cache, ints(table), ints([0, 0]), held, means)
+    kHeld, vHeld = R.quantized(numbers(k))[3], R.quantized(numbers(v))[3]
+    place = {s: i for i, s in enumerate(flat)}
+    at = [[place[s] for s in mine] for mine in slots]
+    meansOf = [np.stack([[L.block_mean(kHeld[mine[b * 64:b * 64 + 64], h]) for h in range(kvHeads)] for b in range(len(mine) // 64)]) for mine in at]
+    ids = ctx.selectBlocks(q, means, ints(table), start, held, 5)
+    chosen = ids.cpu().numpy().astype(np.int64)
+    assert np.array_equal(chosen, L.select(numbers(q), meansOf, lengths, [rows, rows], kvHeads, 5, 1, 1))
+    got = numbers(ctx.attendSelected(q, cache, ints(table), start, held, ids))
+    want, bound = L.attention_listed(numbers(q), kHeld, vHeld, at, lengths, [rows, rows], chosen, dim ** -0.5)
+    assert np.all(np.abs(got - want) <= 2.0 ** -8 * np.abs(want) + bound)
+    got = numbers(ctx.attendShared(q, cache, ints(table), start, held, rows, ints([0, 2]), ints([prefix]), always=True))
+    want, bound = R.attention(numbers(q), kHeld, vHeld, at, lengths, [rows, rows], 0, 0, dim ** -0.5)
+    assert np.all(np.abs(got - want) <= 2.0 ** -8 * np.abs(want) + bound)
+    assert ctx.info().deviceErrorFlag == 0
