@@ -52,16 +52,18 @@ constexpr uint32_t kRows = kTileRows;
 // is 2^-30 of the largest is still something.
 constexpr float kWeightScale = 6.0f;
 constexpr uint32_t kUnitCost = 8;  // tiles' time that a unit takes besides its tiles
-constexpr uint32_t kSlots = 4, kPacked = 3;  // expanded tiles; packed ones, of keys and of values each
+constexpr uint32_t kSlots = 4;  // expanded tiles
+__host__ __device__ constexpr uint32_t packed_tiles(int dim) { return dim == 128 ? 4u : 3u; }  // packed ones, of keys and of values each
 // S has as many buffers as tensor memory has room for beside queries and outputs; its products run as far ahead of those of the weights as
-// the rings allow; scales and exponents are kept for that many tiles and as many more.
+// the rings allow; scales and exponents are kept for that many tiles and as many more.  us a tile and CTA (full row tiles, three and four tiles
+// ahead): 64 values a head 0.57 with three, 0.60 with four; 128 0.75 with three, 0.72 with four.
 __host__ __device__ constexpr uint32_t score_buffers(int dim) { return dim == 256 ? 2u : 4u; }
-__host__ __device__ constexpr uint32_t tiles_ahead(int dim) { return dim == 256 ? 2u : 3u; }
+__host__ __device__ constexpr uint32_t tiles_ahead(int dim) { return dim == 256 ? 2u : dim == 128 ? 4u : 3u; }
 __host__ __device__ constexpr uint32_t info_tiles(int dim) { return dim == 256 ? 4u : 8u; }
 // The expansion's items are the keys of as many tiles, then values and keys in turn, at the end of a unit the values that are left: no more
-// values than that one behind the other.  So the values kPacked tiles before a tile's are at least kPacked + 1 items before.
-static_assert(kPacked + 1 >= kSlots && tiles_ahead(64) <= kPacked && tiles_ahead(256) <= kPacked, "a free slot says that the ring's place was read");
-static_assert(tiles_ahead(64) <= score_buffers(64) && tiles_ahead(256) <= score_buffers(256), "a buffer each");
+// values than that one behind the other.  So the values packed_tiles before a tile's are at least one item more before.
+__host__ __device__ constexpr bool rings_hold(int dim) { return packed_tiles(dim) + 1 >= kSlots && tiles_ahead(dim) <= packed_tiles(dim) && tiles_ahead(dim) <= score_buffers(dim); }
+static_assert(rings_hold(64) && rings_hold(128) && rings_hold(256), "a free slot says that the ring's place was read; a buffer each");
 
 struct TilesArgs {
     AttendArgs a;
@@ -74,7 +76,7 @@ struct TilesArgs {
 __host__ __device__ constexpr uint32_t slot_bytes(int dim) { return kTileKeys * dim * 2; }
 __host__ __device__ constexpr uint32_t packed_bytes(int dim) { return (kTileKeys * dim / 2 + 1023u) & ~1023u; }
 __host__ __device__ constexpr uint32_t words_bytes(int dim) { return 2u * kTileKeys * (dim / 64) * 4u; }  // of a tile, keys' and values'
-__host__ __device__ constexpr uint32_t tiles_smem(int dim) { return 1024u + kSlots * slot_bytes(dim) + 2 * kPacked * packed_bytes(dim) + (info_tiles(dim) + kPacked) * words_bytes(dim); }
+__host__ __device__ constexpr uint32_t tiles_smem(int dim) { return 1024u + kSlots * slot_bytes(dim) + 2 * packed_tiles(dim) * packed_bytes(dim) + (info_tiles(dim) + packed_tiles(dim)) * words_bytes(dim); }
 
 // K-major or N-major tile of f16 with the 128-byte swizzle: rows of 128 bytes, groups of eight 1024 bytes apart; N-major:
 // the next 64 values `lead` bytes further.
@@ -185,7 +187,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
     constexpr uint32_t kWordSide = words_bytes(DIM) / 2, kUnits = kTileKeys * NG;  // of a slot: a key's group of 64 values
     // (no more groups than slots: one that waited for a slot two rounds ahead would take one round's parity for the other's)
     constexpr uint32_t kGroupWarps = DIM == 64 ? 2 : 4, kGroups = kDequantWarps / kGroupWarps < kSlots ? kDequantWarps / kGroupWarps : kSlots, kUnitsEach = kUnits / (32 * kGroupWarps);
-    constexpr uint32_t kInfo = info_tiles(DIM), kBuffers = score_buffers(DIM), kAhead = tiles_ahead(DIM);
+    constexpr uint32_t kPacked = packed_tiles(DIM), kInfo = info_tiles(DIM), kBuffers = score_buffers(DIM), kAhead = tiles_ahead(DIM);
     constexpr uint32_t kColQ = 0, kColO = DIM / 2, kColS = kColO + DIM;
     extern __shared__ uint8_t tilesSmem[];
     __shared__ __align__(8) uint64_t barriers[2 * kSlots + 4 * kPacked + 2 * kInfo + kBuffers + 2 * kBuffers + 2 + 1 + 1 + 8 + 1];
