@@ -62,6 +62,8 @@ __host__ __device__ constexpr uint32_t tiles_ahead(int dim) { return dim == 256 
 __host__ __device__ constexpr uint32_t info_tiles(int dim) { return dim == 256 ? 4u : 8u; }
 // The expansion's items are the keys of as many tiles, then values and keys in turn, at the end of a unit the values that are left: no more
 // values than that one behind the other.  So the values packed_tiles before a tile's are at least one item more before.
+// A wait for O of a tile is by parity: the tile score_buffers before, whose product counts on the same barrier, is done when the tile's S is (S runs
+// no further ahead).
 __host__ __device__ constexpr bool rings_hold(int dim) { return packed_tiles(dim) + 1 >= kSlots && tiles_ahead(dim) <= packed_tiles(dim) && tiles_ahead(dim) <= score_buffers(dim); }
 static_assert(rings_hold(64) && rings_hold(128) && rings_hold(256), "a free slot says that the ring's place was read; a buffer each");
 
@@ -190,7 +192,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
     constexpr uint32_t kPacked = packed_tiles(DIM), kInfo = info_tiles(DIM), kBuffers = score_buffers(DIM), kAhead = tiles_ahead(DIM);
     constexpr uint32_t kColQ = 0, kColO = DIM / 2, kColS = kColO + DIM;
     extern __shared__ uint8_t tilesSmem[];
-    __shared__ __align__(8) uint64_t barriers[2 * kSlots + 4 * kPacked + 2 * kInfo + kBuffers + 2 * kBuffers + 2 + 1 + 1 + 8 + 1];
+    __shared__ __align__(8) uint64_t barriers[2 * kSlots + 4 * kPacked + 2 * kInfo + 4 * kBuffers + 1 + 1 + 8 + 1];
     __shared__ uint32_t tmemSlot, lastPart;
     __shared__ volatile uint32_t abortFlag;
     __shared__ uint32_t firstTile[kTilesThreads + 1], firstWork[kTilesThreads + 1], warpSums[32];
@@ -206,7 +208,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
     const uint32_t bar0 = sm_addr(barriers);
     const uint32_t barTile = bar0, barTileFree = barTile + 8 * kSlots, barPack = barTileFree + 8 * kSlots, barPackFree = barPack + 16 * kPacked;  // keys', then values'
     const uint32_t barInfo = barPackFree + 16 * kPacked, barInfoFree = barInfo + 8 * kInfo;
-    const uint32_t barS = barInfoFree + 8 * kInfo, barP = barS + 8 * kBuffers, barO = barP + 16 * kBuffers, barQ = barO + 16, barJoin = barQ + 8, barTop = barJoin + 8, barDone = barTop + 64;
+    const uint32_t barS = barInfoFree + 8 * kInfo, barP = barS + 8 * kBuffers, barO = barP + 16 * kBuffers, barQ = barO + 8 * kBuffers, barJoin = barQ + 8, barTop = barJoin + 8, barDone = barTop + 64;
     if (tid == 0) {
         abortFlag = 0;
         for (uint32_t s = 0; s < kSlots; ++s) {
@@ -225,8 +227,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
             mbar_init(barS + 8 * s, 1);
             mbar_init(barP + 16 * s, 4);  // the first 32 keys' weights
             mbar_init(barP + 16 * s + 8, 4);
+            mbar_init(barO + 8 * s, 1);
         }
-        for (uint32_t s = 0; s < 2; ++s) mbar_init(barO + 8 * s, 1);
         mbar_init(barQ, kRowWarps);
         mbar_init(barJoin, kRowWarps);
         for (uint32_t s = 0; s < 8; ++s) mbar_init(barTop + 8 * s, 1);
@@ -564,7 +566,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
 #pragma unroll
                         for (uint32_t k = kTileKeys / 32; k < kTileKeys / 16; ++k) mma_a_tmem(tmem + kColO, p + 8 * k, desc + k * (2048 >> 4), idescO, 1u);
                         commit(barTileFree + 8 * slot);
-                        commit(barO + 8 * (tile & 1u));
+                        commit(barO + 8 * (tile % kBuffers));
                         commit(barInfoFree + 8 * (tile % kInfo));  // weights formed, values expanded: nobody looks at the tile's scales any more
                     }
                     __syncwarp();
@@ -839,7 +841,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                         const float next = fmaxf(top, peak), down = exp2_fast(top - next);
                         top = next;
                         if (i) {  // O so far, once the products in flight are done
-                            if (!(ok = wait_warp<false>(barO + 8 * (wg ^ 1u), (tile - 1) >> 1 & 1u, &abortFlag))) break;
+                            if (!(ok = wait_warp<false>(barO + 8 * ((tile - 1) % kBuffers), (tile - 1) / kBuffers & 1u, &abortFlag))) break;
                             tc_fence_after();
 #pragma unroll 1
                             for (uint32_t c = 0; c < DIM; c += 16) {
@@ -895,7 +897,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
                 // ---- the unit's rows, or this CTA's part of them: either warpgroup every second 32 values ----
                 sumShared[wg][row] = sum;
                 refShared[wg][row] = ref;
-                if (!meet() || !(ok = wait_warp<false>(barO + 8 * ((tile - 1) & 1u), (tile - 1) >> 1 & 1u, &abortFlag))) break;
+                if (!meet() || !(ok = wait_warp<false>(barO + 8 * ((tile - 1) % kBuffers), (tile - 1) / kBuffers & 1u, &abortFlag))) break;
                 tc_fence_after();
                 if constexpr (kSuffix) pdl_wait();  // (for what the prefixes gave, and the parts' memory)
                 const float top = topShared[row];

@@ -223,6 +223,17 @@ def test_strides_streams_and_graphs(rows):
         b.check(out)
 
 
+@pytest.mark.parametrize("dim,page", [(64, 64), (128, 16), (128, 64), (256, 64)])
+def test_many_rows_are_the_same_every_time(dim, page):
+    """Logits that pass the maximum again and again: outputs are rescaled between products that run ahead of the rows."""
+    b = Shared(16, 2, dim, page, [1500, 700], [260, 130], [0, 2], [512], loud=3.0)
+    want, alone = b.shared().clone(), b.attend().clone()
+    b.check(want)
+    b.check(alone)
+    for _ in range(150):
+        assert torch.equal(b.shared(), want) and torch.equal(b.attend(), alone)
+
+
 def test_many_requests():
     """More requests than a CTA has threads, in groups of five."""
     requests = 1000
