@@ -228,8 +228,8 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
     const uint32_t r0 = min(tid * run, requests), r1 = min(r0 + run, requests);
     // rowStart goes back, to rows that several requests would write: such a call is refused like one with too much work
     auto goes_back = [&](uint32_t r) {
-        if constexpr (kPrefix) return __ldg(a.shared.groupStart + r + 1) < __ldg(a.shared.groupStart + r);
-        return __ldg(a.rowStart + r + 1) < __ldg(a.rowStart + r);
+        if constexpr (kPrefix) return false;  // (the requests' launch looks, and then takes nothing from this one)
+        else return __ldg(a.rowStart + r + 1) < __ldg(a.rowStart + r);
     };
     uint32_t sum = 0;
     for (uint32_t r = r0; r < r1; ++r) {
@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
     if (kListed)
         for (uint32_t r = tid; r < a.requests; r += kRowsThreads)
             if (goes_back(r)) sum = kTooMuch;
-    if ((kPrefix || kSuffix) && shared_refused(a, tid, kRowsThreads)) sum = kTooMuch;
+    if (kSuffix && groups_go_back(a, tid, kRowsThreads)) sum = kTooMuch;
     uint32_t scan = sum;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
@@ -275,7 +275,7 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
             if (tid == 0 && refused) *a.errorFlag = kFlagWork;
             __syncthreads();
             if (tid == 0 && a.requests && __ldg(a.rowStart + a.requests) > a.tokens) *a.errorFlag = kFlagRows;
-            if (kSuffix && shared_refused(a, tid, kRowsThreads)) *a.errorFlag = kFlagRows;
+            if (kSuffix && groups_go_back(a, tid, kRowsThreads)) *a.errorFlag = kFlagRows;
             if (kListed)
                 for (uint32_t r = tid; r < a.requests; r += kRowsThreads)
                     if (goes_back(r)) *a.errorFlag = kFlagRows;
@@ -296,8 +296,8 @@ __global__ void __launch_bounds__(kRowsThreads, DIM * NT <= 256 ? 2 : 1) k_atten
     if (total == 0 || refused) return leave();
     const uint32_t ctas = min(gridDim.x, max(1u, total / 3u)), cta = blockIdx.x;
     if (cta >= ctas) return leave();
-    auto start_of = [&](uint32_t c) { return (uint32_t)((unsigned long long)c * total / ctas); };
-    auto cta_of = [&](uint32_t x) { return (uint32_t)((((unsigned long long)x + 1) * ctas - 1) / total); };
+    auto start_of = [&](uint32_t c) { return divided((unsigned long long)c * total, ctas); };
+    auto cta_of = [&](uint32_t x) { return divided(((unsigned long long)x + 1) * ctas - 1, total); };
     const uint32_t begin = start_of(cta), end = start_of(cta + 1);
 
     // Where the run stands: a request's unit, whose tile i stands at x = first + kUnitCost + i; and the tiles of it that are

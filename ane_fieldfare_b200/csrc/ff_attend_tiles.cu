@@ -313,19 +313,10 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
         __syncthreads();
         return total;
     };
-    auto search = [&](const uint32_t *first, uint32_t n) {
-        uint32_t low = 0, high = kTilesThreads;
-        while (high - low > 1) {
-            const uint32_t mid = (low + high) >> 1;
-            if (first[mid] <= n) low = mid;
-            else high = mid;
-        }
-        return low;
-    };
     const uint32_t r0 = min(tid * run, requests), r1 = min(r0 + run, requests);
     // rowStart goes back, to rows that several requests would write: such a call is refused like one with too much work
     auto goes_back = [&](uint32_t r) {
-        if constexpr (kPrefix) return false;  // (shared_refused looks)
+        if constexpr (kPrefix) return false;  // (the requests' launch looks, and then takes nothing from this one)
         else return __ldg(a.rowStart + r + 1) < __ldg(a.rowStart + r);
     };
     uint32_t mineTiles = 0;
@@ -335,7 +326,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
         mineTiles = goes_back(r) ? kTooMuch : add_work(mineTiles, (min(of.y, a.maxRows) + args.tileTokens - 1) / args.tileTokens);
         if (!kPrefix && of.y && (int)of.z - (int)of.y + (int)min(of.y, a.maxRows) > 0 && of.z - of.y + min(of.y, a.maxRows) > a.tableKeys) *a.errorFlag = kFlagTableRow;  // (what the row has no room for is not walked)
     }
-    if ((kPrefix || kSuffix) && shared_refused(a, tid, kTilesThreads)) mineTiles = kTooMuch;
+    if (kSuffix && groups_go_back(a, tid, kTilesThreads)) mineTiles = kTooMuch;
     const uint32_t allTiles = block_scan(mineTiles, firstTile);
     const uint32_t rowTiles = allTiles == kTooMuch ? 0u : allTiles;
     // the n-th row tile
@@ -343,7 +334,12 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
         uint32_t r, i, count;  // request, row tile of it, row tiles that it has
     };
     auto place_of = [&](uint32_t n) {
-        const uint32_t low = search(firstTile, n);
+        uint32_t low = 0, high = (requests + run - 1) / run;  // (threads that have requests)
+        while (high - low > 1) {
+            const uint32_t mid = (low + high) >> 1;
+            if (firstTile[mid] <= n) low = mid;
+            else high = mid;
+        }
         n -= firstTile[low];
         Place p{low * run, 0u, 0u};
         for (;; ++p.r) {
@@ -385,7 +381,7 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
         if (blockIdx.x == 0) {
             if (tid == 0 && refused) *a.errorFlag = kFlagWork;
             __syncthreads();
-            if (kSuffix && shared_refused(a, tid, kTilesThreads)) *a.errorFlag = kFlagRows;
+            if (kSuffix && groups_go_back(a, tid, kTilesThreads)) *a.errorFlag = kFlagRows;
             if (tid == 0 && a.requests && __ldg(a.rowStart + a.requests) > a.tokens) *a.errorFlag = kFlagRows;
             for (uint32_t r = r0; r < r1; ++r) {
                 if (goes_back(r)) *a.errorFlag = kFlagRows;
@@ -399,8 +395,8 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
         }
     }
     const uint32_t ctas = min(gridDim.x, max(1u, total / 2u)), cta = blockIdx.x;
-    auto start_of = [&](uint32_t c) { return (uint32_t)((unsigned long long)c * total / ctas); };
-    auto cta_of = [&](uint32_t x) { return (uint32_t)((((unsigned long long)x + 1) * ctas - 1) / total); };
+    auto start_of = [&](uint32_t c) { return divided((unsigned long long)c * total, ctas); };
+    auto cta_of = [&](uint32_t x) { return divided(((unsigned long long)x + 1) * ctas - 1, total); };
     const uint32_t begin = cta < ctas && total ? start_of(cta) : 0u, end = cta < ctas && total ? start_of(cta + 1) : 0u;
 
     // The run's segments: consecutive key tiles of one unit, whose tile i stands at x = first + kUnitCost + i.  A unit costs its
@@ -434,7 +430,12 @@ __global__ void __launch_bounds__(kTilesThreads, 1) k_attend_tiles(const __grid_
         return true;
     };
     auto first_segment = [&](Walk &w) {
-        const uint32_t low = search(firstWork, begin);
+        uint32_t low = 0, high = kTilesThreads;
+        while (high - low > 1) {
+            const uint32_t mid = (low + high) >> 1;
+            if (firstWork[mid] <= begin) low = mid;
+            else high = mid;
+        }
         w.place = place_of(low * perThread);
         uint32_t n = begin - firstWork[low];
         for (;; advance(w.place)) {

@@ -89,6 +89,9 @@ constexpr uint32_t kTooMuch = 0xFFFFFFFFu;
 __device__ __forceinline__ uint32_t add_work(uint32_t a, uint32_t b) { return a + b < a ? kTooMuch : a + b; }
 __device__ __forceinline__ uint32_t work_of(uint32_t tiles, uint32_t units) { return __umulhi(tiles, units) ? kTooMuch : tiles * units; }
 
+// a / b, which fits 32 bits (a division of 64 takes several hundred cycles)
+__device__ __forceinline__ uint32_t divided(unsigned long long a, uint32_t b) { return a >> 32 ? (uint32_t)(a / b) : (uint32_t)a / b; }
+
 // A group of requests that share a prefix: its rows, its first request, and the keys of the prefix in whole tiles (the others are
 // walked with the requests' own).  None where there is more work than 32 bits count.
 struct SharedGroup {
@@ -121,11 +124,10 @@ __device__ __forceinline__ uint32_t shared_keys(const AttendArgs &a, uint32_t r,
     const uint32_t keys = shared_group(a, low).keys;
     return p0 >= 0 && (uint32_t)p0 + 1u >= keys ? keys : 0u;
 }
-// Whether the thread's share of the groups goes back, or of the row starts (groups' rows could overlap then).
-__device__ __forceinline__ bool shared_refused(const AttendArgs &a, uint32_t thread, uint32_t threads) {
+// Whether the thread's share of the groups goes back (their rows could overlap then).
+__device__ __forceinline__ bool groups_go_back(const AttendArgs &a, uint32_t thread, uint32_t threads) {
     bool back = false;
     for (uint32_t g = thread; g < a.shared.groups; g += threads) back |= __ldg(a.shared.groupStart + g + 1) < __ldg(a.shared.groupStart + g);
-    for (uint32_t r = thread; r < a.requests; r += threads) back |= __ldg(a.rowStart + r + 1) < __ldg(a.rowStart + r);
     return back;
 }
 
