@@ -137,8 +137,8 @@ __global__ void __launch_bounds__(kMeansThreads) k_block_means(const __grid_cons
     auto locate = [&](unsigned long long item) {
         Block b{0u, 0u, 0u};
         if (item >= items) return b;
-        uint32_t n = (uint32_t)(item / a.kvHeads), low = 0, high = kMeansThreads;
-        b.head = (uint32_t)(item % a.kvHeads);
+        uint32_t n = divided(item, a.kvHeads), low = 0, high = kMeansThreads;
+        b.head = (uint32_t)item - n * a.kvHeads;
         while (high - low > 1) {
             const uint32_t mid = (low + high) >> 1;
             if (first[mid] <= n) low = mid;
@@ -187,13 +187,25 @@ __global__ void __launch_bounds__(kMeansThreads) k_block_means(const __grid_cons
         const uint32_t myCodes = held + keyLane * CB + inKey * 16, myWords = heldWords + (keyLane * NG + inKey / (kLanes / NG)) * 4;
         auto word_of = [&](int k) { return hole ? 0u : lds32(myWords + k * (kKeys * NG * 4)); };
         auto codes_of = [&](int k) { return hole ? make_uint4(0u, 0u, 0u, 0u) : lds128(myCodes + k * (kKeys * CB)); };
-        uint32_t most = 0, least = 0xFFu, biasMost = 0, biasLeast = 0xFFu, at;  // exponents of the scales, of the biases
+        // exponents of the scales, of the biases; exact down to numbers that are zero or below the normal ones, which are looked at one by one
+        uint32_t most = 0, least = 0xFFu, biasMost = 0, biasLeast = 0xFFu, at;
+        {
+            uint32_t greatest = 0u, smallest = 0xFFFFFFFFu;
 #pragma unroll
-        for (int k = 0; k < kSteps; ++k) {
-            const uint32_t w = word_of(k), e = w >> 7 & 0xFFu, f = w >> 23 & 0xFFu;
-            most = max(most, e), biasMost = max(biasMost, f);
-            if (w & 0x7FFFu) least = min(least, max(e, 1u));
-            if (w & 0x7FFF0000u) biasLeast = min(biasLeast, max(f, 1u));
+            for (int k = 0; k < kSteps; ++k) {
+                const uint32_t e = word_of(k) & 0x7F807F80u;
+                greatest = __vmaxu2(greatest, e), smallest = __vminu2(smallest, e);
+            }
+            most = (greatest & 0xFFFFu) >> 7, biasMost = greatest >> 23, least = (smallest & 0xFFFFu) >> 7, biasLeast = smallest >> 23;
+            if (__any_sync(0xFFFFFFFFu, least == 0u || biasLeast == 0u)) {
+                least = biasLeast = 0xFFu;
+#pragma unroll 1
+                for (int k = 0; k < kSteps; ++k) {
+                    const uint32_t w = word_of(k);
+                    if (w & 0x7FFFu) least = min(least, max(w >> 7 & 0xFFu, 1u));
+                    if (w & 0x7FFF0000u) biasLeast = min(biasLeast, max(w >> 23 & 0xFFu, 1u));
+                }
+            }
         }
         most = __reduce_max_sync(0xFFFFFFFFu, most), least = __reduce_min_sync(0xFFFFFFFFu, least);
         biasMost = __reduce_max_sync(0xFFFFFFFFu, biasMost), biasLeast = __reduce_min_sync(0xFFFFFFFFu, biasLeast);
@@ -268,7 +280,7 @@ __global__ void __launch_bounds__(kMeansThreads) k_block_means(const __grid_cons
         for (int i = 0; i < kMine; i += 2) {
             float v[2];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) v[k] = broken ? NAN : (float)fmin(fmax(rint(mean[i + k] * down), -127.0), 127.0) * up;
+            for (int k = 0; k < 2; ++k) v[k] = broken ? NAN : (float)max(min(__double2int_rn(mean[i + k] * down), 127), -127) * up;
             out[i / 2] = pack_bf16x2(v[0], v[1]);
         }
         const uint32_t perPage = max(1u, pageTokens >> kBlockShift), place = (key0 & (pageTokens - 1u)) >> kBlockShift;
