@@ -26,7 +26,7 @@
 // with fewer registers a thread: 131072 keys 48.4 us where two took 44.3, ragged 73.4 and 73.1.  2000 keys of 8 heads of 256 are 14.1 us of
 // waits one after another (in a timeline of 13.5: look-up of the requests 1.0, queries 1.7, tiles 3.4, joins in the CTA 1 and of the
 // parts 2; the checks of lengths and row starts came behind it).
-// The same kernel takes rows over listed blocks (64 of 2048 blocks of 8 heads of 128 13.5 us; 64 ragged requests of up to 32 blocks, 111 MB, 40.4 us, 2.8 TB/s;
+// The same kernel takes rows over listed blocks (64 of 2048 blocks of 8 heads of 128 13.5 us; 64 ragged requests of up to 32 blocks, 111 MB, 40.4 us, 2.7 TB/s;
 // 64 rows of 24 blocks of 8 heads of 256 59 us: 226 MB, each row's blocks by themselves, 3.8 TB/s) and the two halves of attention
 // behind a shared prefix, as far as they have so few columns.
 // Registers: none spill at 64 values a head; at 128, 240 bytes with more than 8 columns; at 256, 144 bytes with up to 4 columns, 128

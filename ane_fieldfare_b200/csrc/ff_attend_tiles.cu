@@ -24,7 +24,7 @@
 // part of the keys; it is in the sum of the weights all the same, which does not know E.  A code masked in place is the f16 code * 2^-24 or * 2^-20, and one FMA with scale times 2^24 or
 // 2^20 and the bias rounds once: nine instructions a word of eight codes.
 //
-// 4096 rows of 16 heads of 256 over 36864 keys take 2.2 to 2.26 ms, 1.05 PFLOP/s: 64 % of the burst bf16 rate, 77 % of the sustained one
+// 4096 rows of 16 heads of 256 over 36864 keys take 2.2 to 2.26 ms, 1.05 PFLOP/s: 63 % of the burst bf16 rate, 75 % of the sustained one
 // (at 36864 keys the power limit holds the clock below its maximum).  A tile takes 1.0 to 1.2 us.  Its MMAs alone are 1077 cycles: 16 of
 // 32.8 and 4 of 138, each form timed by itself.  The tensor pipe is active 45 % of the time at 8192 keys: S of a tile waits in one of
 // two buffers until its weights are formed, and tensor memory has no third at 256 values a head.  4096 rows in a window of 1024 take
@@ -33,8 +33,8 @@
 //
 // Attention behind a shared prefix is three launches: this kernel with the groups' rows over their prefixes, whose units' parts stay apart; a join;
 // then the requests' rows from behind the prefixes, here or in the kernel for few rows, what the join gave added to their own.  64 requests with
-// 256 columns a key/value head behind 32768 keys of 8 heads of 128 take 83 us: 55 tiles a CTA of 0.72 us, in front of them 15 us (plan, queries, first
-// logits), 4 of the join and 25 of the requests' launch, which begins while the join runs.  Read by request they take 565.  With fewer columns or keys the
+// 256 columns a key/value head behind 32768 keys of 8 heads of 128 take 83 us with up to 2048 keys of their own: 1.27 us for 1024 keys of the prefix (0.73 a tile of 128 columns
+// and CTA), 14 more than with 64 keys of their own, the rest whatever the lengths.  The requests' launch begins while the join runs.  Read by request they take 565.  With fewer columns or keys the
 // launches cost more than they save (ff_attention.cu).  In copies that skip a part (for the time alone) a tile takes at 64, 128 and 256 values a head 0.57,
 // 0.74 and 1.0 us, without the expansion 0.55, 0.66 and 0.77, without exponentials 0.58, 0.72 and 0.96, with a quarter of the products 0.59, 0.74 and
 // 0.92: up to 128 values a chain of hand-overs, not one unit, sets the pace.  A second warp for the scales (32 warps, 40 registers) was slower: 0.61, 0.78.

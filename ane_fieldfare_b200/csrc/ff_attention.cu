@@ -22,8 +22,8 @@ bool launch_attend(FFAttention *att, const AttendArgs &a, cudaStream_t stream, c
 // The groups' rows over their prefixes, then the requests' rows from behind them.  Each goes to the kernel that its columns ask for, as above;
 // those of a group are all its rows' (bounded by the rows of the call; at 256 values a head eight, where more spill registers).  Or the requests'
 // launch alone, over all of their keys, where the other would take longer than it saves.  us alone / with both: 8 requests of 4 columns of
-// 128 behind 4096 keys 17.7 / 30.4, 16384 42 / 41; 64 behind 1024 31 / 35, 4096 80 / 42, 16384 271 / 62; 16 of 8 rows of 2 of 256 behind
-// 1024 48 / 46, 4096 103 / 55, 16384 324 / 83; 16 of 8 rows of 7 of 64 behind 16384 48 / 56.
+// 128 behind 4096 keys 17.8 / 25.8, 16384 42 / 34; 64 behind 1024 31 / 30, 4096 80 / 35, 16384 271 / 51; 16 of 8 rows of 2 of 256 behind
+// 1024 48 / 43 (the rule takes the former), 4096 103 / 50, 16384 323 / 73; 16 of 8 rows of 7 of 64 behind 16384 49 / 47 (likewise).
 bool launch_attend_shared(FFAttention *att, const AttendArgs &a, uint32_t maxPrefix, cudaStream_t stream, const char **error) {
     const uint32_t group = a.heads / a.kvHeads, dim = att->cfg.headDim, size = dim == 256 ? 2 : dim == 128 ? 1 : 0;
     const uint32_t active = std::min(a.requests, a.tokens), rows = active ? std::min(a.maxRows, (a.tokens + active - 1) / active) : 0;  // requests with rows, and theirs (as if all had as many)
