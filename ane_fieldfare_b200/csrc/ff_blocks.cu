@@ -15,8 +15,8 @@ constexpr int kLeastExponent = -60, kMostExponent = 60;  // of a mean's largest 
 // ---- mean keys -----------------------------------------------------------------------------------
 
 // A warp takes a block of a key/value head, 64 keys of code * scale + bias, 32 codes a lane and load.  Where the scales are no more than 2^6
-// apart the products' sum is exact in 32 bits (a code times a scale has 12 bits, 64 of them 18); other blocks are summed in 64 bits, as the
-// biases are, exact unless the scales are 2^35 apart.  Then whole numbers of 2^(e - 6), e the exponent of the largest value: 7 bits and a sign,
+// and the biases no more than 2^9 apart their sums are exact in 32 bits (a code times a scale has 12 bits, 64 of them 18), and below 2^128 where no
+// exponent is above kMostSummed (64 * 15 * 2^118); other blocks are summed in 64 bits, exact unless the scales are 2^35 apart.  Then whole numbers of 2^(e - 6), e the exponent of the largest value: 7 bits and a sign,
 // which bf16 holds.  So nothing about a mean depends on the order of sums.
 // Bound by issue slots, the pipe of logical operations first: a code takes one to mask it, half a product and half a sum.  576 blocks of 8 heads of
 // 256 (45 MB) take 18.6 us, 2.4 TB/s, 37 % of a copy's rate; with 64-bit sums throughout and loads of 8 bytes 29, with 32-bit sums 23.4, with the
@@ -24,6 +24,7 @@ constexpr int kLeastExponent = -60, kMostExponent = 60;  // of a mean's largest 
 // block, 4.9 us: launch and look-up.
 constexpr int kMeansThreads = 512;
 constexpr uint32_t kMeansWaitLimit = 1u << 20;
+constexpr uint32_t kMostSummed = 127 + 117;  // exponent field of the scales and biases that are summed in 32 bits
 
 struct MeansArgs {
     const uint8_t *pages;
@@ -214,7 +215,7 @@ __global__ void __launch_bounds__(kMeansThreads) k_block_means(const __grid_cons
         most = __reduce_max_sync(0xFFFFFFFFu, most), least = __reduce_min_sync(0xFFFFFFFFu, least);
         biasMost = __reduce_max_sync(0xFFFFFFFFu, biasMost), biasLeast = __reduce_min_sync(0xFFFFFFFFu, biasLeast);
         double mean[kMine], bias = 0.0;
-        if (max(most, biasMost) < 0xFFu && most <= least + 6u && biasMost <= biasLeast + 9u) {
+        if (max(most, biasMost) <= kMostSummed && most <= least + 6u && biasMost <= biasLeast + 9u) {
             // Nibbles i and i + 4 of a word, masked in place: 2^23 + 16^i code, less 2^23, times the scale / 16^i; two codes an instruction.
             unsigned long long sums[16];
             float biases = 0.0f;

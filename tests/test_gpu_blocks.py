@@ -105,6 +105,27 @@ def test_means_at_the_ends_of_range_and_of_no_number():
     assert np.array_equal(got, want, equal_nan=True)
 
 
+@pytest.mark.parametrize("dim", [64, 256])
+def test_means_of_keys_whose_sum_passes_32_bits(dim):
+    """Finite keys near the end of bf16's range: equal ones, which lie in the biases, and others of either sign, which lie in the scales too."""
+    ctx = context(heads=1, kvHeads=1, dim=dim, page=64, requests=1, tokens=1024)
+    gen = generator(8)
+    parts = [torch.full((64, 1, dim), sign * 2.0 ** e, device="cuda") for e, sign in ((115, 1), (117, -1), (118, 1), (121, -1), (122, 1), (127, -1))]
+    parts += [2.0 ** e * (2 * torch.rand((64, 1, dim), generator=gen, device="cuda") - 1) for e in (112, 119, 120, 121, 122, 124, 126)]  # (a group's width stays below 2^128)
+    parts += [2.0 ** e * torch.rand((64, 1, dim), generator=gen, device="cuda") for e in (120, 122, 127)]
+    x = torch.cat(parts).bfloat16()
+    blocks = len(parts)
+    pages, slots = ctx.newCache(blocks), ints(range(blocks * 64))
+    for a in range(0, blocks * 64, 1024):
+        ctx.append(None, x[a:a + 1024], x[a:a + 1024], None, slots[a:a + 1024], slots[a:a + 1024], pages)
+    means = ctx.newMeans(blocks)
+    ctx.blockMeans(pages, ints([list(range(blocks))]), ints([0]), ints([blocks * 64]), means)
+    keys, _ = R.unpack(pages.cpu().numpy(), 1, dim, 64)
+    assert np.isfinite(keys).all()
+    want = np.stack([L.block_mean(keys[b * 64:b * 64 + 64, 0]) for b in range(blocks)])
+    assert np.array_equal(numbers(means)[:, 0, 0], want) and ctx.info().deviceErrorFlag == 0
+
+
 def test_means_past_the_table_and_the_cache():
     ctx = context(heads=1, kvHeads=1, page=16, requests=1, tokens=256)
     pages, _ = cache_of(ctx, [256])
