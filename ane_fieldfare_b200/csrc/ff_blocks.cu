@@ -182,11 +182,17 @@ __global__ void __launch_bounds__(kMeansThreads) k_block_means(const __grid_cons
             bool there = mbar_try_wait(bar, parity);
 #pragma unroll 1
             for (uint32_t i = 0; i < kMeansWaitLimit && !there; ++i) there = mbar_try_wait(bar, parity);
-            parity ^= 1u;
             if (!__all_sync(0xFFFFFFFFu, there)) {
                 if (lane == 0) *a.errorFlag = kFlagWait;
-                break;  // (a later copy would take this one's bytes for its own)
+                // given up: no copy is in flight when the CTA ends, and no later one takes this one's bytes for its own
+#pragma unroll 1
+                for (uint32_t i = 0; i < kMeansWaitLimit && !there; ++i) {
+                    __nanosleep(40);
+                    there = mbar_try_wait(bar, parity);
+                }
+                break;
             }
+            parity ^= 1u;
         }
         // key k * kKeys + keyLane of the block: its word, its codes
         const uint32_t myCodes = held + keyLane * CB + inKey * 16, myWords = heldWords + (keyLane * NG + inKey / (kLanes / NG)) * 4;
