@@ -5,14 +5,16 @@
 
 `CacheBook` keeps the requests' lengths, block tables and free pages on the GPU, and which requests share the pages of a prefix, whose
 attention is then computed once for all of them; `DecoderLayer` is one layer's forward over the rows of a step, be they single tokens,
-blocks that are verified, prompts, or a mixture.  A layer may attend to a part of a long context: for steps of few rows a request, the blocks whose
+blocks that are verified, prompts, or a mixture.  A layer may attend to a part of a long context: for requests with few rows in a step, the blocks whose
 mean keys a row's queries score highest.  The two matrix products in front of and behind attention are plain library products.
 `python -m ane_fieldfare_b200.decoder` runs a small one: a prompt, a block of which some rows are taken back, single tokens, and requests
 that go on from a shared prompt.
 """
 from __future__ import annotations
 
-from dataclasses import dataclass
+from bisect import bisect_left
+from dataclasses import dataclass, field, replace
+from itertools import accumulate
 from typing import List, Optional, Sequence
 
 import torch
@@ -36,6 +38,40 @@ class Step:
     groupStart: Optional[torch.Tensor] = None  # requests that share prefixes, where some do
     prefixLengths: Optional[torch.Tensor] = None
     maxPrefix: int = 0
+    rows: Optional[Sequence[int]] = None  # new tokens of each request; None: maxRows, a bound, stands for all of them
+    sharing: tuple = ((), ())  # groupStart and prefixLengths on the host
+    _parts: dict = field(default_factory=dict, repr=False)
+
+    def parts(self, most: int) -> tuple:
+        """(requests with up to `most` new tokens, the others), each (rows of the step, a step for the attention of them alone); None for rows
+        is all of them, None for a part that there is none."""
+        if self.rows is None:
+            return ((None, self), None) if self.maxRows <= most else (None, (None, self))
+        few = [r for r, n in enumerate(self.rows) if 0 < n <= most]
+        many = [r for r, n in enumerate(self.rows) if n > most]
+        if not many:
+            return (None, self), None
+        if not few:
+            return None, (None, self)
+        if most not in self._parts:
+            self._parts[most] = self._part(few), self._part(many)
+        # (what the host knows is laid out once for all layers; lengths and tables are the device's, taken at every call)
+        return tuple((index, replace(part, lengths=self.lengths[chosen], blockTable=self.blockTable[chosen])) for index, chosen, part in self._parts[most])
+
+    def _part(self, requests: Sequence[int]) -> tuple:
+        to = lambda values: torch.tensor(values, dtype=torch.int32).to(self.lengths.device)  # noqa: E731
+        first, rows = [0, *accumulate(self.rows)], [self.rows[r] for r in requests]
+        index = torch.cat([torch.arange(first[r], first[r + 1], dtype=torch.int32) for r in requests]).to(self.lengths.device)
+        part = Step(to([0, *accumulate(rows)]), self.positions, self.slots, self.lengths, self.blockTable, max(rows), rows=rows)
+        # groups of which two or more are here; they stand one behind the other as before
+        start, prefixes = [bisect_left(requests, r) for r in self.sharing[0]], []
+        for g, prefix in enumerate(self.sharing[1]):
+            prefixes.append(prefix if start[g + 1] - start[g] > 1 else 0)
+        there = [g for g in range(len(prefixes)) if start[g + 1] > start[g]]
+        if any(prefixes):
+            part.sharing = [*(start[g] for g in there), start[-1]], [prefixes[g] for g in there]
+            part.groupStart, part.prefixLengths, part.maxPrefix = to(part.sharing[0]), to(part.sharing[1]), max(prefixes)
+        return index, to(requests), part
 
 
 class CacheBook:
@@ -105,7 +141,8 @@ class CacheBook:
         device, i32, total = self.attention.device, torch.int32, sum(rows)
         after = torch.tensor(new, dtype=i32).to(device)
         step = Step(torch.empty(len(new) + 1, dtype=i32, device=device), torch.empty(total, dtype=i32, device=device),
-                    torch.empty(total, dtype=i32, device=device), after, self.blockTable, max(rows + [1]) if maxRows is None else maxRows, self._now)
+                    torch.empty(total, dtype=i32, device=device), after, self.blockTable, max(rows + [1]) if maxRows is None else maxRows, self._now,
+                    rows=rows if maxRows is None else None)
         self.attention.plan(self._now, after, self.blockTable, self.freePages, self.freeCount, self.freeCount, step.rowStart,
                             step.positions, step.slots, heldPages=self.heldPages if any(self._prefix) else None)
         gone = [r for r, prefix in enumerate(self._prefix) if prefix and prefix[0] != r and new[r] == 0]
@@ -118,7 +155,7 @@ class CacheBook:
         start, prefixes = self._groups()
         if prefixes:
             step.groupStart, step.prefixLengths = torch.tensor(start, dtype=i32).to(device), torch.tensor(prefixes, dtype=i32).to(device)
-            step.maxPrefix = max(prefixes)
+            step.maxPrefix, step.sharing = max(prefixes), (start, prefixes)
         self.lengths, self._now = new, after
         return step
 
@@ -126,7 +163,8 @@ class CacheBook:
 @dataclass
 class Selection:
     """Attention to a part of the context: `blocks` blocks of 64 keys a row and key/value head, the first and the last among them in
-    any case, in steps of up to `maxRows` rows a request (more of them read a block together by reading all)."""
+    any case, for requests that bring up to `maxRows` rows to a step (more of them read a block together by reading all).  A request's rows
+    attend alike whatever others the step has, but where `CacheBook.step` is given a bound, which then decides for all."""
     blocks: int
     first: int = 1
     last: int = 1
@@ -166,12 +204,26 @@ class DecoderLayer:
         qkv = (x @ w.qkv.T).unflatten(1, (-1, att.headDim))
         q, k, v = qkv.split([att.heads, att.kvHeads, att.kvHeads], dim=1)
         q = att.append(q, k, v, self.ropeTable, step.positions, step.slots, self.cache, interleaved=self.interleaved)
-        if self.selected:
-            att.blockMeans(self.cache, step.blockTable, step.before, step.lengths, self.means)
-            if step.maxRows <= self.selected.maxRows:
-                ids = att.selectBlocks(q, self.means, step.blockTable, step.rowStart, step.lengths, self.selected.blocks, first=self.selected.first,
-                                       last=self.selected.last)
-                return att.attendSelected(q, self.cache, step.blockTable, step.rowStart, step.lengths, ids)
+        if not self.selected:
+            return self._all_keys(q, step)
+        att.blockMeans(self.cache, step.blockTable, step.before, step.lengths, self.means)
+        few, many = step.parts(self.selected.maxRows)
+        if many is None:
+            return self._blocks(q, step)
+        if few is None:
+            return self._all_keys(q, step)
+        out = torch.empty_like(q)
+        for (index, part), attention in ((few, self._blocks), (many, self._all_keys)):
+            out[index] = attention(q[index], part)
+        return out
+
+    def _blocks(self, q: torch.Tensor, step: Step) -> torch.Tensor:
+        att, choice = self.attention, self.selected
+        ids = att.selectBlocks(q, self.means, step.blockTable, step.rowStart, step.lengths, choice.blocks, first=choice.first, last=choice.last)
+        return att.attendSelected(q, self.cache, step.blockTable, step.rowStart, step.lengths, ids)
+
+    def _all_keys(self, q: torch.Tensor, step: Step) -> torch.Tensor:
+        att = self.attention
         if step.groupStart is not None and not self.window:
             return att.attendShared(q, self.cache, step.blockTable, step.rowStart, step.lengths, step.maxRows, step.groupStart, step.prefixLengths,
                                     maxPrefix=step.maxPrefix)

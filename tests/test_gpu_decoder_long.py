@@ -169,3 +169,87 @@ def test_whole_layers_with_both_and_the_demonstration(capsys):
     decoder.main()
     said = capsys.readouterr().out
     assert said.count("error flag: 0") == 2 and "288 tokens" in said
+
+
+def spied(monkeypatch, unit):
+    """(rows, lengths, queries, ids) of every call that selects blocks, each checked against the definition."""
+    from ane_fieldfare_b200 import attention
+
+    calls, plain = [], attention.AttentionContext.selectBlocks
+
+    def select(self, q, means, table, start, lengths, blocks, **kw):
+        ids = plain(self, q, means, table, start, lengths, blocks, **kw)
+        rows, n, held, pages = torch.diff(start).tolist(), lengths.tolist(), numbers(means), table.tolist()
+        size = self.pageTokens
+        of = [np.stack([held[pages[r][(b * 64 + 63) // size], :, (b * 64 + 63) % size // 64] for b in range(m // 64)]) if m >= 64
+              else np.zeros((0, self.kvHeads, self.headDim)) for r, m in enumerate(n)]
+        assert np.array_equal(ids.cpu().numpy(), L.select(numbers(q), of, n, rows, self.kvHeads, blocks, kw["first"], kw["last"]))
+        calls.append((rows, n, ids.cpu().numpy()))
+        return ids
+
+    monkeypatch.setattr(attention.AttentionContext, "selectBlocks", select)
+    return calls
+
+
+def test_a_prompt_in_the_step_leaves_the_other_requests_their_blocks(monkeypatch):
+    """Requests with few rows attend to their blocks, requests with many to all keys, in whatever order and whatever else the step has."""
+    from ane_fieldfare_b200 import decoder
+
+    book, stack = decoder.small_decoder(requests=5, pages=160, selected=decoder.Selection(blocks=3, maxRows=4))
+    unit, x = stack[0], inputs(5, 600, 0)
+    calls = spied(monkeypatch, unit)
+    steps = [[400, 0, 0, 430, 0], [401, 40, 0, 433, 70], [402, 41, 30, 434, 71], [408, 42, 31, 438, 75], [412, 43, 31, 470, 80]]
+    few = [[], [0, 3], [0, 1, 3, 4], [1, 2, 3, 4], [0, 1]]
+    run(book, unit, x, [[400, 0, 0, 0, 0], steps[0]])
+    assert not calls
+    for before, want, chosen in zip(steps, steps[1:], few[1:]):
+        calls.clear()
+        got = run(book, unit, x, [want])
+        rows = [b - a for a, b in zip(before, want)]
+        (ran, lengths, ids), = calls
+        assert ran == [rows[r] for r in chosen] and lengths == [want[r] for r in chosen]
+        at = 0
+        for r, n in enumerate(want):
+            if not rows[r]:
+                continue
+            listed = None
+            if r in chosen:
+                listed = np.full((n, *ids.shape[1:]), -1)
+                listed[n - rows[r]:] = ids[at:at + rows[r]]
+                at += rows[r]
+            near(np.stack([numbers(got[r, p]) for p in range(n - rows[r], n)]), exact(book, unit, x, want, r, listed)[n - rows[r]:])
+    assert book.attention.info().deviceErrorFlag == 0
+    # a bound that has to be the same for several steps decides for all requests
+    calls.clear()
+    step = book.step([413, 44, 31, 471, 80], maxRows=16)
+    unit.attend(torch.stack([x[0][412], x[1][43], x[3][470]]), step)
+    assert not calls
+    unit.attend(torch.stack([x[0][413], x[1][44], x[3][471]]), book.step([414, 45, 31, 472, 80], maxRows=4))
+    assert len(calls) == 1
+
+
+@pytest.mark.parametrize("always", [False, True])
+def test_prompts_behind_a_shared_prefix_beside_single_tokens(always, monkeypatch):
+    from ane_fieldfare_b200 import attention, decoder
+
+    plain, shared = attention.AttentionContext.attendShared, []
+
+    def attend(self, q, pages, table, start, lengths, most, groups, prefixes, **kw):
+        shared.append((groups.tolist(), prefixes.tolist(), lengths.tolist()))
+        return plain(self, q, pages, table, start, lengths, most, groups, prefixes, **(kw | {"always": always}))
+
+    monkeypatch.setattr(attention.AttentionContext, "attendShared", attend)
+    book, stack = decoder.small_decoder(requests=8, pages=200, selected=decoder.Selection(blocks=2, maxRows=4))
+    unit, x = stack[0], inputs(8, 400, 140)
+    x[5:] = inputs(3, 400, 80, seed=9)
+    calls = spied(monkeypatch, unit)
+    run(book, unit, x, [[140, 0, 0, 0, 30, 90, 0, 0]])
+    assert book.share(0, [1, 2, 3], 140) == 128 and book.share(5, [6, 7], 80) == 80
+    #                 single, few, many, many, single, many, few, many
+    steps = [[141, 130, 160, 150, 31, 120, 82, 110], [142, 150, 161, 170, 40, 121, 83, 111], [143, 151, 181, 171, 41, 122, 84, 112]]
+    got = run(book, unit, x, steps)
+    assert shared == [([0, 2, 4], [128, 80], [160, 150, 120, 110]), ([0, 2, 3], [128, 0], [150, 170, 40])]
+    assert [c[0] for c in calls] == [[1, 2, 1, 2], [1, 1, 1, 1, 1], [1, 1, 1, 1, 1, 1, 1]]
+    for r, p0, p1 in [(2, 128, 160), (3, 128, 150), (5, 90, 120), (7, 80, 110), (1, 130, 150), (3, 150, 170), (4, 31, 40), (2, 161, 181)]:
+        near(np.stack([numbers(got[r, p]) for p in range(p0, p1)]), exact(book, unit, x, steps[-1], r)[p0:p1])
+    assert book.attention.info().deviceErrorFlag == 0
