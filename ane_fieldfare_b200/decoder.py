@@ -93,6 +93,8 @@ class CacheBook:
         read and do not own.  Returns how many.  Requests that stand one behind the other have their attention over them in one."""
         size = self.attention.pageTokens
         pages = tokens // size
+        if any(not 0 <= r < len(self.lengths) for r in (owner, *requests)):
+            raise ValueError(f"requests are 0 .. {len(self.lengths) - 1}")
         if not 0 <= tokens <= self.lengths[owner]:
             raise ValueError(f"the owner holds {self.lengths[owner]} tokens")
         if any(r == owner or self.lengths[r] or self._prefix[r] for r in requests):

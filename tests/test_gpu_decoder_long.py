@@ -122,6 +122,22 @@ def test_a_prefix_is_not_taken_from_those_who_share_it():
     assert int(book.freeCount) == 39
 
 
+def test_requests_that_share_are_named_by_their_numbers():
+    """-1 for the last one would be another owner than itself: kept from giving its own pages back once those who shared them had ended."""
+    from ane_fieldfare_b200 import decoder
+
+    book, _ = decoder.small_decoder(requests=3, pages=40)
+    book.step([0, 0, 40])
+    for owner, requests in [(-1, [0]), (2, [-3]), (2, [0, 3]), (3, [0])]:
+        with pytest.raises(ValueError, match="0 .. 2"):
+            book.share(owner, requests, 40)
+    assert book.share(2, [0, 1], 40) == 32
+    book.step([33, 34, 41])
+    book.step([0, 0, 41])
+    book.step([0, 0, 10])
+    assert int(book.freeCount) == 39 and book.attention.info().deviceErrorFlag == 0
+
+
 def test_selected_blocks_of_a_layer():
     """Of a prompt all keys; of the decode steps behind it the blocks that the definition chooses."""
     from ane_fieldfare_b200 import decoder
