@@ -399,8 +399,8 @@ bool ff_attention_shared(FFAttention *att, const uint16_t *q, uint32_t qStride, 
     if (!begin(att, error)) return false;
     const FFAttentionConfig &c = att->cfg;
     if (!(scale > 0.0f && scale < INFINITY)) return fail(error, "scale must be positive and finite");
-    if (maxRows == 0) return fail(error, "maxRows must be positive");
     if (tokens == 0) return true;
+    if (maxRows == 0) return fail(error, "maxRows must be positive");
     if (!check_tokens(att, tokens, error) || !check_heads(att, q, qStride, c.heads, "query", error) ||
         !check_heads(att, out, outStride, c.heads, "output", error) || !check_cache(att, pages, pageCount, error) ||
         !check_requests(att, requests, error) || !check_table(blockTable, tableStride, rowStart, "rowStart", lengths, requests, error))

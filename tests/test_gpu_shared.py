@@ -272,3 +272,12 @@ def test_refusals():
             call(**kw)
     assert call(q=b.q[:0], rowStart=ints([0, 0, 0])).shape == (0, 4, 64)
     assert numbers(call()).shape == (2, 4, 64)
+
+
+def test_a_step_without_rows_may_say_so_in_its_bound():
+    """As `attend` has it: nothing to do, whatever maxRows is."""
+    b = Shared(4, 2, 64, 16, [100, 100], [1, 1], [0, 2], [64])
+    none = ints([0, 0, 0])
+    for always in (False, True):
+        assert b.ctx.attendShared(b.q[:0], b.cache, ints(b.table), none, ints(b.lengths), 0, ints(b.groups), ints(b.prefix), always=always).shape == (0, 4, 64)
+    assert b.ctx.attend(b.q[:0], b.cache, ints(b.table), none, ints(b.lengths), 0).shape == (0, 4, 64)
