@@ -40,15 +40,15 @@ class AttentionContext:
                  maxTokens: int = 4096, device: int = 0):
         lib = binding.load()
         self.config = FFAttentionConfig(heads, kvHeads, headDim, pageTokens, maxRequests, maxTokens)
+        self._config = ctypes.byref(self.config)
         err = ctypes.c_char_p()
-        self._handle = lib.ff_attention_create(device, ctypes.byref(self.config), ctypes.byref(err))
+        self._handle = lib.ff_attention_create(device, self._config, ctypes.byref(err))
         if not self._handle:
             raise FieldfareError(err.value.decode() if err.value else "ff_attention_create failed")
         self.device, self._ordinal = torch.device("cuda", device), device
         self.heads, self.kvHeads, self.headDim, self.pageTokens = heads, kvHeads, headDim, pageTokens
         self.maxRequests, self.maxTokens = maxRequests, maxTokens
-        self.pageBytes = lib.ff_cache_page_bytes(ctypes.byref(self.config))
-        self._sharedBytes = {}  # of attendShared's workspace, by rows
+        self.pageBytes = lib.ff_cache_page_bytes(self._config)
         self._meanValues = kvHeads * max(1, pageTokens // BLOCK_KEYS) * headDim  # of a page
 
     @property
@@ -261,13 +261,12 @@ class AttentionContext:
         if out is None:
             out = self._new((tokens, self.heads, self.headDim), torch.bfloat16, stream)
         self._ints("blockTable rowStart lengths groupStart prefixLengths", blockTable, rowStart, lengths, groupStart, prefixLengths)
-        bytes_ = self._sharedBytes.get(tokens)
-        if bytes_ is None:
-            bytes_ = self._sharedBytes.setdefault(tokens, binding.load().ff_attention_shared_bytes(ctypes.byref(self.config), tokens))
-        workspace = self._new((bytes_,), torch.uint8, stream)
+        most, workspace, lib = min(maxRows, _WORD), None, binding.load()
+        if lib.ff_attention_shares(self._config, tokens, shape[1], requests, most, groups, longest):
+            workspace = self._new((lib.ff_attention_shared_bytes(self._config, tokens),), torch.uint8, stream)
         call("ff_attention_shared", self.handle, *self._heads(q, self.heads, tokens, "q"), tokens, *self._cache(pages), blockTable.data_ptr(), shape[1],
-             rowStart.data_ptr(), lengths.data_ptr(), requests, min(maxRows, _WORD), groupStart.data_ptr(), prefixLengths.data_ptr(), groups, longest,
-             self.headDim ** -0.5 if scale is None else scale, workspace.data_ptr(), *self._heads(out, self.heads, tokens, "out"),
+             rowStart.data_ptr(), lengths.data_ptr(), requests, most, groupStart.data_ptr(), prefixLengths.data_ptr(), groups, longest,
+             self.headDim ** -0.5 if scale is None else scale, None if workspace is None else workspace.data_ptr(), *self._heads(out, self.heads, tokens, "out"),
              _stream(stream))
         return out
 

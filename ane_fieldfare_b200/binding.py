@@ -155,6 +155,7 @@ SIGNATURES = {
     "ff_attention_selected": (c_bool, [c_void_p, _P, c_uint32, c_uint32, _P, c_uint32, _P, c_uint32, _P, _P, c_uint32, _P,
                                        c_uint32, c_float, _P, c_uint32, _P, _ERR]),
     "ff_attention_shared_bytes": (c_uint64, [POINTER(FFAttentionConfig), c_uint32]),
+    "ff_attention_shares": (c_bool, [POINTER(FFAttentionConfig), c_uint32, c_uint32, c_uint32, c_uint32, c_uint32, c_uint32]),
     "ff_attention_shared": (c_bool, [c_void_p, _P, c_uint32, c_uint32, _P, c_uint32, _P, c_uint32, _P, _P, c_uint32, c_uint32, _P,
                                      _P, c_uint32, c_uint32, c_float, _P, _P, c_uint32, _P, _ERR]),
     "ff_rope_table": (c_bool, [c_void_p, POINTER(FFRopeConfig), _P, c_uint32, _P, _ERR]),

@@ -19,30 +19,38 @@ bool launch_attend(FFAttention *att, const AttendArgs &a, cudaStream_t stream, c
     return launch_attend_tiles(att, a, stream, error);
 }
 
-// The groups' rows over their prefixes, then the requests' rows from behind them.  Each goes to the kernel that its columns ask for, as above;
-// those of a group are all its rows' (bounded by the rows of the call; at 256 values a head eight, where more spill registers).  Or the requests'
-// launch alone, over all of their keys, where the other would take longer than it saves.  us alone / with both: 8 requests of 4 columns of
+// Whether groups share: their rows over their prefixes in one launch and the requests' rows from behind them in another, or the requests' launch
+// alone, over all of their keys, where the other would take longer than it saves.  us alone / with both: 8 requests of 4 columns of
 // 128 behind 4096 keys 17.8 / 25.8, 16384 42 / 34; 64 behind 1024 31 / 30, 4096 80 / 35, 16384 271 / 51; 16 of 8 rows of 2 of 256 behind
-// 1024 48 / 43 (the rule takes the former), 4096 103 / 50, 16384 323 / 73; 16 of 8 rows of 7 of 64 behind 16384 49 / 47 (likewise).
-bool launch_attend_shared(FFAttention *att, const AttendArgs &a, uint32_t maxPrefix, cudaStream_t stream, const char **error) {
-    const uint32_t group = a.heads / a.kvHeads, dim = att->cfg.headDim, size = dim == 256 ? 2 : dim == 128 ? 1 : 0;
-    const uint32_t active = std::min(a.requests, a.tokens), rows = active ? std::min(a.maxRows, (a.tokens + active - 1) / active) : 0;  // requests with rows, and theirs (as if all had as many)
-    const bool fewOfRequest = (uint64_t)a.maxRows * group <= 16, fewOfGroup = (uint64_t)a.tokens * group <= (dim == 256 ? 8 : 16);
+// 1024 48 / 43 (the rule takes the former), 4096 103 / 50, 16384 323 / 73; 16 of 8 rows of 7 of 64 behind 16384 49 / 47 (likewise).  It goes by
+// what the host knows: all rows as if behind the longest prefix, every request as if it had as many of them.
+static bool few_of_group(const FFAttentionConfig &c, uint32_t tokens) { return (uint64_t)tokens * (c.heads / c.kvHeads) <= (c.headDim == 256 ? 8 : 16); }
+static bool few_of_request(const FFAttentionConfig &c, uint32_t maxRows) { return (uint64_t)maxRows * (c.heads / c.kvHeads) <= 16; }
+bool attend_shares(const FFAttentionConfig &c, uint32_t tokens, uint32_t tableKeys, uint32_t requests, uint32_t maxRows, uint32_t groups, uint32_t maxPrefix) {
+    if (!groups || maxPrefix == FF_SHARE_ALWAYS) return groups != 0;
+    const uint32_t group = c.heads / c.kvHeads, dim = c.headDim, size = dim == 256 ? 2 : dim == 128 ? 1 : 0;
+    const uint32_t active = std::min(requests, tokens), rows = active ? std::min(maxRows, (tokens + active - 1) / active) : 0;  // requests with rows, and theirs (as if all had as many)
+    const bool fewOfRequest = few_of_request(c, maxRows), fewOfGroup = few_of_group(c, tokens);
     // what 64 keys cost a tile of columns, 0.1 ns of the whole GPU: of up to 4, 8 and 16, of 128 (where requests fill a part of them)
     static const uint32_t few[3][3] = {{14, 15, 20}, {20, 21, 35}, {37, 42, 90}}, many[3] = {40, 44, 63}, full[3] = {50, 62, 78};
-    const uint64_t columns = (uint64_t)a.maxRows * group;
+    const uint64_t columns = (uint64_t)maxRows * group;
     const uint32_t of = columns <= 4 ? 0 : columns <= 8 ? 1 : 2, width = fewOfRequest ? 4u << of : kTileRows;
     auto tiles = [&](uint64_t n, uint32_t wide) {  // of n rows
         return group <= wide ? (n + wide / group - 1) / (wide / group) : n * ((group + wide - 1) / wide);
     };
     const uint64_t apart = active * tiles(rows, width) * (fewOfRequest ? few[size][of] : many[size]);
-    const uint64_t together = std::max<uint64_t>(a.shared.groups, fewOfGroup ? tiles(a.tokens, 16) : tiles(a.tokens, kTileRows)) * (fewOfGroup ? few[size][dim == 256 ? 1 : 2] : full[size]);
-    const uint64_t keys = std::min(maxPrefix, a.tableKeys) / kBlockKeys;
-    if (!a.shared.groups || (maxPrefix != FF_SHARE_ALWAYS && (apart <= together || (apart - together) * keys * a.kvHeads <= kSharedLaunch))) return launch_attend(att, a, stream, error);
+    const uint64_t together = std::max<uint64_t>(groups, fewOfGroup ? tiles(tokens, 16) : tiles(tokens, kTileRows)) * (fewOfGroup ? few[size][dim == 256 ? 1 : 2] : full[size]);
+    const uint64_t keys = std::min(maxPrefix, tableKeys) / kBlockKeys;
+    return apart > together && (apart - together) * keys * c.kvHeads > kSharedLaunch;
+}
+
+// Each launch goes to the kernel that its columns ask for, as in launch_attend; those of a group are all its rows' (bounded by the rows of the
+// call; at 256 values a head eight, where more spill registers).
+bool launch_attend_shared(FFAttention *att, const AttendArgs &a, cudaStream_t stream, const char **error) {
     AttendArgs b = a;
     b.maxRows = b.tokens;
-    if (!(fewOfGroup ? launch_attend_prefix_rows(att, b, stream, error) : launch_attend_prefix_tiles(att, b, stream, error))) return false;
-    return fewOfRequest ? launch_attend_suffix_rows(att, a, stream, error) : launch_attend_suffix_tiles(att, a, stream, error);
+    if (!(few_of_group(att->cfg, a.tokens) ? launch_attend_prefix_rows(att, b, stream, error) : launch_attend_prefix_tiles(att, b, stream, error))) return false;
+    return few_of_request(att->cfg, a.maxRows) ? launch_attend_suffix_rows(att, a, stream, error) : launch_attend_suffix_tiles(att, a, stream, error);
 }
 
 }  // namespace ff
@@ -392,6 +400,10 @@ uint64_t ff_attention_shared_bytes(const FFAttentionConfig *config, uint32_t tok
     return config && supported(*config, nullptr) ? shared_layout(*config, tokens).bytes : 0;
 }
 
+bool ff_attention_shares(const FFAttentionConfig *config, uint32_t tokens, uint32_t tableStride, uint32_t requests, uint32_t maxRows, uint32_t groups, uint32_t maxPrefix) {
+    return config && supported(*config, nullptr) && attend_shares(*config, tokens, table_keys(*config, tableStride), requests, std::min(maxRows, tokens), groups, maxPrefix);
+}
+
 bool ff_attention_shared(FFAttention *att, const uint16_t *q, uint32_t qStride, uint32_t tokens, const void *pages, uint32_t pageCount,
                          const uint32_t *blockTable, uint32_t tableStride, const uint32_t *rowStart, const uint32_t *lengths, uint32_t requests,
                          uint32_t maxRows, const uint32_t *groupStart, const uint32_t *prefixLengths, uint32_t groups, uint32_t maxPrefix, float scale, void *workspace,
@@ -408,14 +420,16 @@ bool ff_attention_shared(FFAttention *att, const uint16_t *q, uint32_t qStride, 
     if (groups > requests) return fail(error, "more groups than requests");
     if (groups && (!groupStart || !prefixLengths || !aligned(groupStart, 4) || !aligned(prefixLengths, 4)))
         return fail(error, "groupStart and prefixLengths must be non-null and 4-byte aligned");
-    if (!workspace || !aligned(workspace, 16)) return fail(error, "workspace must be non-null and 16-byte aligned");
+    const bool shares = attend_shares(c, tokens, table_keys(c, tableStride), requests, std::min(maxRows, tokens), groups, maxPrefix);
+    if (shares && (!workspace || !aligned(workspace, 16))) return fail(error, "workspace must be non-null and 16-byte aligned");
     const SharedLayout l = shared_layout(c, tokens);
     uint8_t *w = static_cast<uint8_t *>(workspace);
     AttendArgs a{q, out, qStride, outStride, tokens, static_cast<const uint8_t *>(pages), pageCount, tableStride, table_keys(c, tableStride), blockTable,
                  rowStart, lengths, requests, std::min(maxRows, tokens), scale, 0, 0, c.heads, c.kvHeads, page_layout(c), att->errorFlag, nullptr, 0,
                  {groupStart, prefixLengths, groups, reinterpret_cast<uint4 *>(w), reinterpret_cast<float2 *>(w + l.stats), reinterpret_cast<float *>(w + l.values)}};
+    if (!shares) return launch_attend(att, a, static_cast<cudaStream_t>(stream), error);
     if (att->smCount > (int)kSharedCtas) return fail(error, "more SMs than the workspace has room for");
-    return launch_attend_shared(att, a, maxPrefix, static_cast<cudaStream_t>(stream), error);
+    return launch_attend_shared(att, a, static_cast<cudaStream_t>(stream), error);
 }
 
 }  // extern "C"

@@ -129,6 +129,7 @@ bool launch_attend_suffix_tiles(FFAttention *att, const AttendArgs &args, cudaSt
 
 // ff_attention.cu
 bool launch_attend(FFAttention *att, const AttendArgs &args, cudaStream_t stream, const char **error);
-bool launch_attend_shared(FFAttention *att, const AttendArgs &args, uint32_t maxPrefix, cudaStream_t stream, const char **error);
+bool attend_shares(const FFAttentionConfig &c, uint32_t tokens, uint32_t tableKeys, uint32_t requests, uint32_t maxRows, uint32_t groups, uint32_t maxPrefix);
+bool launch_attend_shared(FFAttention *att, const AttendArgs &args, cudaStream_t stream, const char **error);
 
 }  // namespace ff

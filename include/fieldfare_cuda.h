@@ -591,9 +591,12 @@ bool ff_attention(FFAttention *attention, const uint16_t *q, uint32_t qStride, u
  * maxPrefix: no prefix is longer.  It chooses the kernels: where such prefixes are too short, or have too few rows behind them, to
  * make up for further launches, all keys are read by request and groupStart and prefixLengths not at all; FF_SHARE_ALWAYS: they are
  * not, whatever that takes.  The two ways' results differ by rounding.  A groupStart that goes back leaves every row zero (flag 15), like
- * such a rowStart.  workspace: ff_attention_shared_bytes() of device memory for the call alone, 16-byte aligned. */
+ * such a rowStart.  workspace: ff_attention_shared_bytes() of device memory for the call alone (4 headDim + 8 a row and head), 16-byte
+ * aligned; it may be null where ff_attention_shares() says that such a call reads all keys by request. */
 #define FF_SHARE_ALWAYS 0xFFFFFFFFu
 uint64_t ff_attention_shared_bytes(const FFAttentionConfig *config, uint32_t tokens);
+bool ff_attention_shares(const FFAttentionConfig *config, uint32_t tokens, uint32_t tableStride, uint32_t requests,
+                         uint32_t maxRows, uint32_t groups, uint32_t maxPrefix);
 bool ff_attention_shared(FFAttention *attention, const uint16_t *q, uint32_t qStride, uint32_t tokens, const void *pages,
                          uint32_t pageCount, const uint32_t *blockTable, uint32_t tableStride, const uint32_t *rowStart,
                          const uint32_t *lengths, uint32_t requests, uint32_t maxRows, const uint32_t *groupStart,

@@ -56,3 +56,22 @@ def test_the_reference_reads_what_it_quantizes():
 def test_to_bf16_rounds_once():
     assert R.to_bf16(1 + 2.0 ** -8) == 1.0 and R.to_bf16(1 + 2.0 ** -8 + 2.0 ** -40) == 1 + 2.0 ** -7
     assert R.to_bf16(1 + 3 * 2.0 ** -8) == 1 + 2.0 ** -6 and np.isnan(R.to_bf16(np.nan)) and R.to_bf16(-np.inf) == -np.inf
+
+
+def test_whether_prefixes_are_shared_is_known_on_the_host():
+    lib = binding.load()
+    always = 0xFFFFFFFF
+    c = FFAttentionConfig(32, 8, 128, 64, 64, 4096)
+
+    def shares(tokens, stride, requests, maxRows, groups, maxPrefix, config=c):
+        return lib.ff_attention_shares(ctypes.byref(config), tokens, stride, requests, maxRows, groups, maxPrefix)
+
+    assert shares(64, 600, 64, 1, 1, 32768) and not shares(64, 600, 64, 1, 1, 64) and not shares(64, 600, 64, 1, 1, 0)
+    assert shares(64, 600, 64, 1, 1, always - 1) and not shares(64, 4, 64, 1, 1, always - 1)  # (no longer than the table's row)
+    assert shares(2, 4, 2, 1, 1, always) and not shares(2, 4, 2, 1, 0, always)
+    assert not shares(0, 600, 64, 1, 1, 32768) and not shares(64, 600, 0, 1, 1, 32768) and not shares(64, 600, 64, 0, 1, 32768)
+    assert not lib.ff_attention_shares(None, 64, 600, 64, 1, 1, always) and not shares(64, 600, 64, 1, 1, always, FFAttentionConfig(32, 8, 96, 64, 64, 4096))
+    for group, dim in [(1, 64), (7, 256), (64, 128), (64, 64), (17, 256)]:
+        for tokens in (1, 16, 1 << 24):
+            for maxRows in (0, 1, 3, 1 << 24):
+                shares(tokens, 1 << 20, 64, maxRows, 3, always - 1, FFAttentionConfig(group, 1, dim, 16, 64, 1 << 24))  # (nothing is divided by zero)

@@ -281,3 +281,22 @@ def test_a_step_without_rows_may_say_so_in_its_bound():
     for always in (False, True):
         assert b.ctx.attendShared(b.q[:0], b.cache, ints(b.table), none, ints(b.lengths), 0, ints(b.groups), ints(b.prefix), always=always).shape == (0, 4, 64)
     assert b.ctx.attend(b.q[:0], b.cache, ints(b.table), none, ints(b.lengths), 0).shape == (0, 4, 64)
+
+
+def test_memory_is_taken_where_prefixes_are_shared_alone():
+    """Room for the rows' results over the prefixes, 32 bits each, is needed only by calls that share."""
+    b = Shared(8, 2, 128, 64, [900] * 2, [400, 400], [0, 2], [64])
+    want = b.shared(always=False, maxPrefix=64).clone()
+    out = torch.empty_like(want)
+
+    def peak(**kw):
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        b.shared(out=out, **kw)
+        return torch.cuda.max_memory_allocated() - before
+
+    small = 1 << 16  # (the step's lists)
+    assert peak(always=False, maxPrefix=64) < small and torch.equal(out, want)
+    assert peak(always=True) >= 800 * 8 * (128 * 4 + 8)
+    b.check(out)
