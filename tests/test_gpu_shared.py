@@ -300,3 +300,13 @@ def test_memory_is_taken_where_prefixes_are_shared_alone():
     assert peak(always=False, maxPrefix=64) < small and torch.equal(out, want)
     assert peak(always=True) >= 800 * 8 * (128 * 4 + 8)
     b.check(out)
+
+
+def test_more_groups_than_threads():
+    """In either kernel over the prefixes; in the one of few rows most requests have none."""
+    b = Shared(2, 1, 64, 64, [66 + r % 60 for r in range(2200)], [1] * 2200, list(range(0, 2201, 2)), [64] * 1100)
+    b.check(b.shared())
+    rows = [1 if r % 90 == 7 else 0 for r in range(700)]
+    b = Shared(2, 1, 64, 64, [130 + r % 60 for r in range(700)], rows, [*range(0, 698, 2), 700], [128] * 349)
+    assert sum(rows) * 2 <= 16
+    b.check(b.shared())
