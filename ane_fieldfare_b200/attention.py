@@ -249,7 +249,7 @@ class AttentionContext:
                      scale: Optional[float] = None, out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
         """`attend` without a window, where requests groupStart[g] .. groupStart[g + 1] - 1 hold the same first prefixLengths[g]
         keys on the same pages: these are read once for all rows of the group, where that is shorter (always: in any case).  maxPrefix:
-        no prefix is longer (without it, than a row of the block table), which it goes by."""
+        no prefix is longer, which it goes by; without it no longer than a row of the block table, which may be far more than they are."""
         tokens, requests, groups, shape = q.shape[0], lengths.numel(), prefixLengths.numel(), blockTable.shape
         if rowStart.numel() != requests + 1 or len(shape) != 2 or shape[0] != requests:
             raise ValueError("lengths, blockTable and rowStart must agree on the number of requests")
@@ -301,7 +301,8 @@ class AttentionContext:
                      lengths: torch.Tensor, blocks: int, *, first: int = 1, last: int = 1, ids: Optional[torch.Tensor] = None,
                      stream=None) -> torch.Tensor:
         """The blocks that every row attends to, int32 [tokens][kvHeads][blocks] in ascending order, -1 behind: the first
-        `first`, the last `last`, and of those between them the ones whose mean keys the row's queries score highest."""
+        `first`, the last `last`, and of those between them the ones whose mean keys the row's queries score highest.  Scores are exact in
+        means and queries of 7 bits a vector, which channels far louder than the others leave few of (include/fieldfare_cuda.h says what that costs)."""
         tokens, requests, shape = q.shape[0], lengths.numel(), blockTable.shape
         if rowStart.numel() != requests + 1 or len(shape) != 2 or shape[0] != requests:
             raise ValueError("lengths, blockTable and rowStart must agree on the number of requests")

@@ -15,7 +15,7 @@
 // A tile's warpgroup waits for the maximum M that the one before it settled on, not for its weights; M moves, and O with it, only
 // where a row passes it by 2^8.  (Both warpgroups on each tile, half a row a thread, were slower: what a tile costs besides its
 // arithmetic was paid twice.)
-// Tensor memory: Q dim/2, O dim, S two tiles of 64 columns: all 512 at dim 256.
+// Tensor memory: Q dim/2, O dim, S tiles of 64 columns, two at dim 256 (512 in all, which is all there is), four below.
 //
 // f16 holds 11 bits of keys, values and weights where bf16 would hold 8; its range is kept by powers of two: a row's
 // own for the queries, a tile's own for keys (taken back with the logits) and for values (E, part of the exponent of P and
@@ -24,7 +24,7 @@
 // part of the keys; it is in the sum of the weights all the same, which does not know E.  A code masked in place is the f16 code * 2^-24 or * 2^-20, and one FMA with scale times 2^24 or
 // 2^20 and the bias rounds once: nine instructions a word of eight codes.
 //
-// 4096 rows of 16 heads of 256 over 36864 keys take 2.2 to 2.26 ms, 1.05 PFLOP/s: 63 % of the burst bf16 rate, 75 % of the sustained one
+// 4096 rows of 16 heads of 256 over 36864 keys take 2.2 ms, 1.06 PFLOP/s: 63 % of the burst bf16 rate, 75 % of the sustained one
 // (at 36864 keys the power limit holds the clock below its maximum).  A tile takes 1.0 to 1.2 us.  Its MMAs alone are 1077 cycles: 16 of
 // 32.8 and 4 of 138, each form timed by itself.  The tensor pipe is active 45 % of the time at 8192 keys: S of a tile waits in one of
 // two buffers until its weights are formed, and tensor memory has no third at 256 values a head.  4096 rows in a window of 1024 take

@@ -18,10 +18,11 @@ constexpr int kLeastExponent = -60, kMostExponent = 60;  // of a mean's largest 
 // and the biases no more than 2^9 apart their sums are exact in 32 bits (a code times a scale has 12 bits, 64 of them 18), and below 2^128 where no
 // exponent is above kMostSummed (64 * 15 * 2^118); other blocks are summed in 64 bits, exact unless the scales are 2^35 apart.  Then whole numbers of 2^(e - 6), e the exponent of the largest value: 7 bits and a sign,
 // which bf16 holds.  So nothing about a mean depends on the order of sums.
-// Bound by issue slots, the pipe of logical operations first: a code takes one to mask it, half a product and half a sum.  576 blocks of 8 heads of
-// 256 (45 MB) take 18.6 us, 2.4 TB/s, 37 % of a copy's rate; with 64-bit sums throughout and loads of 8 bytes 29, with 32-bit sums 23.4, with the
-// block by bulk copies into shared memory 20.6, the next one looked up meanwhile 19.4.  A decode step of 64 requests, one of which completes a
-// block, 4.9 us: launch and look-up.
+// Bound by issue slots (56 % of them while active) and by the block's own copies: a code takes a logical operation to mask it, half a product and
+// half a sum, and a warp waits for its one block in flight.  576 blocks of 8 heads of 256 (45 MB) take 21.5 us from memory, 2.1 TB/s or 32 % of a copy's
+// rate, and 17.9 from L2, as right behind a step's appends.  Steps towards it, from L2: 64-bit sums throughout and loads of 8 bytes 29, 32-bit sums
+// 23.4, the block by bulk copies into shared memory 20.6, the next one looked up meanwhile 19.4.  A decode step of 64 requests, one of which completes
+// a block, 4.8 us: launch and look-up.
 constexpr int kMeansThreads = 512;
 constexpr uint32_t kMeansWaitLimit = 1u << 20;
 constexpr uint32_t kMostSummed = 127 + 117;  // exponent field of the scales and biases that are summed in 32 bits
@@ -314,9 +315,10 @@ __global__ void __launch_bounds__(kMeansThreads) k_block_means(const __grid_cons
 // Two forms.  k_select_split: a cluster of CTAs for each row and head, which share the blocks; the first of them gets the others' scores and
 // makes the list.  k_select_rows: some neighbouring rows a CTA, which read the means of their request once; a warp makes a list.
 // Bound by latency: look-up, queries, table and means, exchange, ranges, list, one after the other.  2048 blocks of 8 heads of 128 for one row 8.1 us
-// (with one CTA of 512 threads a head and a search by halves 22.4, in an instrumented copy 21 thousand cycles for the scores in four rounds and
-// 13 thousand for the search; a cluster and two bits at a time 11.9); 64 ragged requests of up to 256 blocks 8.5; prompts of up to 613 rows, 2110 rows of
-// 7 heads a group over up to 312 blocks, 18.7 (47.9 % of the issue slots while active).
+// (with one CTA of 512 threads a head and a search by halves 22.4; a cluster and two bits at a time 11.9).  In an instrumented copy 14.3 thousand cycles of
+// the list's CTA: 1430 look-up and queries, 2970 scores, 680 exchange, 1260 for the least and the greatest score, 3750 one level of ranges, 1390 the few
+// left, 2280 the list.  64 ragged requests of up to 256 blocks 8.4 us (8.0 thousand cycles); prompts of up to 613 rows, 2110 rows of 7 heads a group
+// over up to 312 blocks, 18.7 (47 % of the issue slots while active).
 constexpr uint32_t kRowsWarps = 8;        // of k_select_rows
 constexpr uint32_t kSelectColumns = 64;   // of a CTA's product, at most
 constexpr uint32_t kMostSplit = 8;        // CTAs of a cluster, at most

@@ -480,7 +480,7 @@ FFAttentionInfo ff_attention_get_info(const FFAttention *attention);
 /* Waits for the device and clears the flag that FFAttentionInfo reports, and what a call that gave up a wait leaves in
  * the handle: after flag 17 results are undefined until this is called.  It is sticky; a kernel sets it to
  * 13: no free page was left, 14: a request is longer than its block table row, 15: more rows than the
- * arrays hold, or a rowStart that goes back (every row is zero then), 16: a page or slot outside the cache, 17: a wait was
+ * arrays hold, or a rowStart that goes back (every row is zero then; lists of blocks are those of one of the requests that have the row), 16: a page or slot outside the cache, 17: a wait was
  * given up, 18: a position outside the rotary table (its row is turned as position 0), 19: more work in a call of ff_attention than 2^32 tiles of 64 keys,
  * counted for every head and tile of rows (every row is zero then), 20: a new token on a page that its request only
  * shares.  What else such an entry names is left out; nothing
@@ -621,7 +621,9 @@ bool ff_block_means(FFAttention *attention, const void *pages, uint32_t pageCoun
  * sees no key, and rows of no request, FF_NO_SLOT alone.  Score of a block: the largest q'.m over the head's query heads, m its mean as held,
  * q' the query in whole numbers of 2^(e-6), to the nearest, at most 127 (e the exponent of its largest value, at least -100 and
  * 60 below the largest e of the group; a query with a value that is not finite counts as zeros).  Such sums are exact: the lists do not
- * depend on how they are formed.  NaN scores come first; blocks whose mean lies on a page outside the cache (flag 16) last.  q, rowStart
+ * depend on how they are formed.  But 7 bits for a whole vector are fewer than bf16 has for each value: beside a channel far louder than the others these
+ * lose theirs.  Where some do not matter (random vectors) the lists name 98 % of the blocks that 64-bit scores of the exact means would; with an offset
+ * common to all keys in 5 % of the channels, 10, 30 and 100 times as loud as the rest, 95, 86 and 57 % (2048 blocks of 128 values, 4 heads, the best 62).  NaN scores come first; blocks whose mean lies on a page outside the cache (flag 16) last.  q, rowStart
  * and lengths as for ff_attention.  A row of the block table has room for at most 2^21 keys. */
 bool ff_select_blocks(FFAttention *attention, const uint16_t *q, uint32_t qStride, uint32_t tokens, const uint16_t *means,
                       uint32_t pageCount, const uint32_t *blockTable, uint32_t tableStride, const uint32_t *rowStart,
