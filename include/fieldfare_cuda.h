@@ -587,7 +587,7 @@ bool ff_attention(FFAttention *attention, const uint16_t *q, uint32_t qStride, u
  * hold the same first prefixLengths[g] keys, on pages that the block table row of the group's first request names and theirs name
  * likewise.  The attention of all rows of a group over those keys is one, as of one request: it reads them once.  (Whole tiles of
  * 64 keys, and no more than the first request holds; what is left of a prefix, and a request whose rows do not come behind it, is
- * read by request.)  groupStart [groups + 1], ascending, prefixLengths [groups]; requests in no group share nothing.
+ * read by request.)  groupStart [groups + 1], ascending, prefixLengths [groups], no more groups than requests; requests in no group share nothing.
  * maxPrefix: no prefix is longer.  It chooses the kernels: where such prefixes are too short, or have too few rows behind them, to
  * make up for further launches, all keys are read by request and groupStart and prefixLengths not at all; FF_SHARE_ALWAYS: they are
  * not, whatever that takes.  The two ways' results differ by rounding.  A groupStart that goes back leaves every row zero (flag 15), like
