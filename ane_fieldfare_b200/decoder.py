@@ -12,7 +12,6 @@ that go on from a shared prompt.
 """
 from __future__ import annotations
 
-from bisect import bisect_left
 from dataclasses import dataclass, field, replace
 from itertools import accumulate
 from typing import List, Optional, Sequence
@@ -47,31 +46,44 @@ class Step:
         is all of them, None for a part that there is none."""
         if self.rows is None:
             return ((None, self), None) if self.maxRows <= most else (None, (None, self))
-        few = [r for r, n in enumerate(self.rows) if 0 < n <= most]
-        many = [r for r, n in enumerate(self.rows) if n > most]
-        if not many:
+        few = [0 < n <= most for n in self.rows]
+        many = [n > most for n in self.rows]
+        if not any(many):
             return (None, self), None
-        if not few:
+        if not any(few):
             return None, (None, self)
-        if most not in self._parts:
-            self._parts[most] = self._part(few), self._part(many)
-        # (what the host knows is laid out once for all layers; lengths and tables are the device's, taken at every call)
-        return tuple((index, replace(part, lengths=self.lengths[chosen], blockTable=self.blockTable[chosen])) for index, chosen, part in self._parts[most])
+        laid = self._parts.get(most)
+        if laid is None:
+            new = torch.diff(self.rowStart)
+            laid = self._part(few, new, (new > 0) & (new <= most)), self._part(many, new, new > most)
+            if not (self.rowStart.is_cuda and torch.cuda.is_current_stream_capturing()):  # (what is captured has no values yet)
+                self._parts[most] = laid
+        # (the rows' places are laid out once for all layers; lengths and tables are taken at every call)
+        return tuple((index, replace(part, lengths=self.lengths[chosen], blockTable=self.blockTable[chosen])) for index, chosen, part in laid)
 
-    def _part(self, requests: Sequence[int]) -> tuple:
-        to = lambda values: torch.tensor(values, dtype=torch.int32).to(self.lengths.device)  # noqa: E731
-        first, rows = [0, *accumulate(self.rows)], [self.rows[r] for r in requests]
-        index = torch.cat([torch.arange(first[r], first[r + 1], dtype=torch.int32) for r in requests]).to(self.lengths.device)
-        part = Step(to([0, *accumulate(rows)]), self.positions, self.slots, self.lengths, self.blockTable, max(rows), rows=rows)
+    def _part(self, here: Sequence[bool], new: torch.Tensor, mine: torch.Tensor) -> tuple:
+        """Of the requests that are `here`, on the device `mine`, of `new` rows each: their rows, their numbers, a step.  Nothing is copied
+        from the host, so that a first call may be captured too."""
+        i32, rows = torch.int32, [n for n, is_here in zip(self.rows, here) if is_here]
+        first = lambda flags, n: torch.sort(flags.to(i32), descending=True, stable=True).indices[:n]  # noqa: E731  (places of n flags)
+        index = first(torch.repeat_interleave(mine, new, output_size=sum(self.rows)), sum(rows))
+        chosen = first(mine, len(rows))
+        start = torch.zeros(len(rows) + 1, dtype=i32, device=new.device)
+        torch.cumsum(new[chosen], 0, dtype=i32, out=start[1:])
+        part = Step(start, self.positions, self.slots, self.lengths, self.blockTable, max(rows), rows=rows)
         # groups of which two or more are here; they stand one behind the other as before
-        start, prefixes = [bisect_left(requests, r) for r in self.sharing[0]], []
-        for g, prefix in enumerate(self.sharing[1]):
-            prefixes.append(prefix if start[g + 1] - start[g] > 1 else 0)
-        there = [g for g in range(len(prefixes)) if start[g + 1] > start[g]]
+        before = [0, *accumulate(here)]
+        starts = [before[r] for r in self.sharing[0]]
+        there = [g for g in range(len(self.sharing[1])) if starts[g + 1] > starts[g]]
+        prefixes = [self.sharing[1][g] if starts[g + 1] - starts[g] > 1 else 0 for g in there]
         if any(prefixes):
-            part.sharing = [*(start[g] for g in there), start[-1]], [prefixes[g] for g in there]
-            part.groupStart, part.prefixLengths, part.maxPrefix = to(part.sharing[0]), to(part.sharing[1]), max(prefixes)
-        return index, to(requests), part
+            counts = torch.zeros(len(here) + 1, dtype=i32, device=new.device)
+            torch.cumsum(mine, 0, dtype=i32, out=counts[1:])
+            none = torch.zeros(1, dtype=i32, device=new.device)
+            part.sharing, part.maxPrefix = ([*(starts[g] for g in there), starts[-1]], prefixes), max(prefixes)
+            part.groupStart = counts[torch.cat([self.groupStart[g:g + 1] for g in there] + [self.groupStart[-1:]])]
+            part.prefixLengths = torch.cat([self.prefixLengths[g:g + 1] if prefix else none for g, prefix in zip(there, prefixes)])
+        return index, chosen, part
 
 
 class CacheBook:

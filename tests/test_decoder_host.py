@@ -6,9 +6,10 @@ from ane_fieldfare_b200.decoder import Step
 
 def step(rows, sharing=((), ()), maxRows=99):
     total, requests = sum(rows or []), len(rows or [0])
-    start = torch.tensor([0, *torch.tensor(rows or [0]).cumsum(0).tolist()])
+    start = torch.tensor([0, *torch.tensor(rows or [0]).cumsum(0).tolist()], dtype=torch.int32)
     s = Step(start, torch.zeros(total), torch.zeros(total), torch.arange(requests) + 100, torch.arange(requests)[:, None] * 10 + torch.arange(3), maxRows, rows=rows)
     s.sharing = sharing
+    s.groupStart, s.prefixLengths = (torch.tensor(x, dtype=torch.int32) for x in sharing)
     return s
 
 

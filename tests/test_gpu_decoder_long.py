@@ -269,3 +269,33 @@ def test_prompts_behind_a_shared_prefix_beside_single_tokens(always, monkeypatch
     for r, p0, p1 in [(2, 128, 160), (3, 128, 150), (5, 90, 120), (7, 80, 110), (1, 130, 150), (3, 150, 170), (4, 31, 40), (2, 161, 181)]:
         near(np.stack([numbers(got[r, p]) for p in range(p0, p1)]), exact(book, unit, x, steps[-1], r)[p0:p1])
     assert book.attention.info().deviceErrorFlag == 0
+
+
+def test_a_mixed_step_is_captured_at_first_sight():
+    from ane_fieldfare_b200 import decoder
+
+    book, stack = decoder.small_decoder(requests=6, pages=160, selected=decoder.Selection(blocks=20, maxRows=4))
+    unit, x = stack[0], inputs(6, 300, 64)
+    run(book, unit, x, [[200, 0, 0, 100, 0, 0]])
+    assert book.share(0, [1, 2], 64) == 64
+    have, want = list(book.lengths), [201, 104, 100, 140, 3, 0]  # blocks enough for all keys: whatever the split, every row sees all
+    step = book.step(want)
+    rows = torch.stack([x[r][p] for r in range(6) for p in range(have[r], want[r])])
+    torch.cuda.synchronize()
+    graph, out = torch.cuda.CUDAGraph(), None
+    with torch.cuda.graph(graph):
+        out = unit.attend(rows, step)
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    captured = out.clone()
+    assert torch.equal(unit.attend(rows, step), captured) and torch.equal(unit.attend(rows, step), captured)
+    graph.replay()
+    assert torch.equal(out, captured)
+    at = 0
+    for r in range(6):
+        n = want[r] - have[r]
+        if n:
+            near(numbers(captured[at:at + n]), exact(book, unit, x, want, r)[have[r]:])
+        at += n
+    assert book.attention.info().deviceErrorFlag == 0
